@@ -298,7 +298,8 @@ bool k3_moe_latent_layer_forward(const k3_moe_latent_desc *desc, void *out,
  * bit 0 (1) = a bounded barrier wait of a tensor-core kernel gave up (that
  * launch's output is undefined); bit 1 (2) = a dispatch (either entry point)
  * met an expert id >= experts: such routes are skipped, so the offsets
- * undercount and the sorted arrays keep stale entries for them.
+ * undercount and the sorted arrays keep stale entries for them (or an entry
+ * point of k3_moe_balance.h met one).
  * Synchronises with the device. */
 uint32_t k3_moe_device_status(void);
 

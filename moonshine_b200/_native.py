@@ -40,6 +40,18 @@ class LatentDesc(C.Structure):
 _LP = C.POINTER(LatentDesc)
 
 
+class Fp8ExpertsDesc(C.Structure):
+    """Mirror of ``k3_moe_fp8_experts_desc`` (include/k3_moe_fp8.h)."""
+    _fields_ = [
+        ("hidden", u32), ("expert_hidden", u32), ("experts", u32), ("top_k", u32),
+        ("activation", C.c_int32), ("beta", f32), ("linear_beta", f32),
+        ("w1", vp), ("w1_scales", vp), ("w3", vp), ("w3_scales", vp), ("w2", vp), ("w2_scales", vp),
+    ]
+
+
+_FP = C.POINTER(Fp8ExpertsDesc)
+
+
 class PhaseStats(C.Structure):
     """Mirror of ``k3_moe_phase_stats`` (include/k3_moe_layer.h)."""
     _fields_ = [("router_seconds", C.c_double), ("routed_index_seconds", C.c_double),
@@ -167,6 +179,22 @@ SIGNATURES = {
     "k3_moe_ep_decode_workspace_bytes": (sz, [vp, _DP]),
     "k3_moe_ep_decode": (C.c_bool, [vp, _DP, vp, vp, vp, vp, sz, vp]),
     "k3_moe_ep_decode_stack": (C.c_bool, [vp, C.POINTER(_DP), u32, vp, vp, vp, f32, vp, sz, vp]),
+    # E4M3 tables with a scale per block of 128
+    "k3_moe_fp8_quantize_rows": (C.c_bool, [vp, vp, vp, u32, u32, i32, vp]),
+    "k3_moe_fp8_quantize_columns": (C.c_bool, [vp, vp, vp, u32, u32, i32, vp]),
+    "k3_moe_fp8_quantize_blocks": (C.c_bool, [vp, vp, vp, u32, u32, i32, vp]),
+    "k3_moe_fp8_transpose_blocks": (C.c_bool, [vp, vp, vp, vp, u32, u32, vp]),
+    "k3_moe_fp8_product": (C.c_bool, [vp, vp, vp, vp, vp, u32, u32, u32, i32, i32, i32, vp]),
+    "k3_moe_fp8_linear_workspace_bytes": (sz, [u32, u32]),
+    "k3_moe_fp8_linear": (C.c_bool, [vp, vp, vp, vp, u32, u32, u32, vp, sz, vp]),
+    "k3_moe_fp8_weight_gradient_workspace_bytes": (sz, [u32, u32, u32]),
+    "k3_moe_fp8_weight_gradient": (C.c_bool, [vp, vp, vp, u32, u32, u32, i32, vp, sz, vp]),
+    "k3_moe_fp8_experts_workspace_bytes": (sz, [_FP, u32]),
+    "k3_moe_fp8_experts_forward": (C.c_bool, [_FP, vp, vp, vp, vp, vp, u32, vp, sz, vp]),
+    # expert load, balance loss and the router's gradient
+    "k3_moe_balance_workspace_bytes": (sz, [u32, u32, u32]),
+    "k3_moe_balance": (C.c_bool, [vp, vp, vp, vp, vp, vp, u32, u32, u32, u32, i32, f32, vp, sz, vp]),
+    "k3_moe_router_backward": (C.c_bool, [vp, vp, vp, vp, vp, vp, vp, u32, u32, u32, u32, i32, f32, f32, vp]),
     "k3_synth_fill_bytes": (C.c_bool, [vp, u64, u64, u64, u32, u32, vp]),
     "k3_synth_fill_int8": (C.c_bool, [vp, u64, u64, u64, vp]),
     "k3_synth_fill_uniform": (C.c_bool, [vp, u64, u64, u64, f32, f32, i32, vp]),

@@ -1,0 +1,420 @@
+// Expert load, balance loss and the router's gradient (include/k3_moe_balance.h has the formulas).
+//
+// All three are one pass over logits f32 [tokens, experts], so HBM bounds them.  A warp takes a token's
+// row: lane l holds experts 4 l .. 4 l + 3 of every 128 (or l of every 32 where rows are not whole 16-byte
+// units), so the row's sums are shuffles, and in the forward pass the sums over tokens stay in the same
+// registers from token to token.
+//
+// Sums over tokens have a fixed order.  Block b takes tokens [b C, (b + 1) C); at the end of its range
+// and at each end of a sequence inside it the block writes what it has as a partial row.  Block b and
+// sequence s share the partial row b + s: along the tokens each step raises one of the two, so no two
+// pairs meet in a row and there are at most blocks + sequences of them.  A second kernel adds a
+// sequence's partial rows, in ascending order, and forms the loss.
+#include "k3_common.cuh"
+#include "k3_grouped.h"
+#include "k3_moe_balance.h"
+
+#include <algorithm>
+
+using namespace k3;
+
+namespace {
+
+constexpr uint32_t kThreads = 256, kWarps = kThreads / kWarp;
+constexpr uint32_t kMaxExperts = 1024;
+constexpr float kTiny = 1e-20f;
+
+__device__ uint32_t g_balance_status = 0;          // 2: an expert id >= experts
+
+struct Shape {
+    uint32_t tokens, sequences, experts, top_k;
+    uint32_t chunk;                                // tokens per block
+    int softmax;
+};
+
+// A warp's row: kV groups of four experts per lane, neighbours (kVector) or 32 apart.
+template <uint32_t kV, bool kVector>
+struct Row {
+    float v[kV * 4u];
+    static K3_DEVINL uint32_t expert(uint32_t i, uint32_t lane) {
+        return kVector ? (i / 4u) * 128u + lane * 4u + i % 4u : i * 32u + lane;
+    }
+    template <typename T>
+    K3_DEVINL void load(const T *row, uint32_t experts, uint32_t lane, float fill) {
+#pragma unroll
+        for (uint32_t i = 0; i < kV * 4u; i += kVector ? 4u : 1u) {
+            const uint32_t e = expert(i, lane);
+            if (kVector) {
+                if (e < experts) {
+                    const uint4 q = *reinterpret_cast<const uint4 *>(row + e);
+                    v[i] = value(q.x, row); v[i + 1u] = value(q.y, row); v[i + 2u] = value(q.z, row); v[i + 3u] = value(q.w, row);
+                } else {
+                    v[i] = v[i + 1u] = v[i + 2u] = v[i + 3u] = fill;
+                }
+            } else {
+                v[i] = e < experts ? (float)row[e] : fill;
+            }
+        }
+    }
+    K3_DEVINL void store(float *row, uint32_t experts, uint32_t lane) const {
+#pragma unroll
+        for (uint32_t i = 0; i < kV * 4u; i += kVector ? 4u : 1u) {
+            const uint32_t e = expert(i, lane);
+            if (e >= experts) continue;
+            if (kVector) *reinterpret_cast<float4 *>(row + e) = make_float4(v[i], v[i + 1u], v[i + 2u], v[i + 3u]);
+            else row[e] = v[i];
+        }
+    }
+    static K3_DEVINL float value(uint32_t bits, const float *) { return __uint_as_float(bits); }
+    static K3_DEVINL float value(uint32_t bits, const uint32_t *) { return (float)bits; }
+    K3_DEVINL float sum() const {
+        float s = 0.f;
+#pragma unroll
+        for (uint32_t i = 0; i < kV * 4u; i++) s += v[i];
+        return warp_sum(s);
+    }
+    // logits -> scores; experts past the end have the logit -inf and get the score 0
+    K3_DEVINL void scores(int softmax) {
+        if (!softmax) {
+#pragma unroll
+            for (uint32_t i = 0; i < kV * 4u; i++) v[i] = 1.0f / (1.0f + expf(-v[i]));
+            return;
+        }
+        float m = -INFINITY;
+        bool nan = false;                          // fmaxf drops a NaN
+#pragma unroll
+        for (uint32_t i = 0; i < kV * 4u; i++) {
+            m = fmaxf(m, v[i]);
+            nan |= v[i] != v[i];
+        }
+        m = warp_max(m);
+        if (__any_sync(0xffffffffu, nan)) m = __uint_as_float(0x7fffffffu);
+        if (m == -INFINITY) {
+#pragma unroll
+            for (uint32_t i = 0; i < kV * 4u; i++) v[i] = 0.f;
+            return;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kV * 4u; i++) v[i] = expf(v[i] - m);
+        const float r = 1.0f / sum();
+#pragma unroll
+        for (uint32_t i = 0; i < kV * 4u; i++) v[i] *= r;
+    }
+};
+
+// the sequence that holds `token`: the last one that starts at or before it (sequences - 1 at most)
+K3_DEVINL uint32_t sequence_of(const uint32_t *offsets, uint32_t sequences, uint32_t token) {
+    if (offsets == nullptr) return 0u;
+    uint32_t lo = 0u, hi = sequences;              // offsets[lo] <= token < offsets[hi]
+    while (hi - lo > 1u) {
+        const uint32_t mid = (lo + hi) / 2u;
+        if (offsets[mid] <= token) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+K3_DEVINL uint32_t begin_of(const uint32_t *offsets, uint32_t s) { return offsets ? offsets[s] : 0u; }
+K3_DEVINL uint32_t end_of(const uint32_t *offsets, uint32_t s, uint32_t tokens) {
+    return offsets ? min(offsets[s + 1u], tokens) : tokens;
+}
+
+// ---------------------------------------------------------------------------------------- forward
+template <uint32_t kV, bool kVector>
+__global__ void __launch_bounds__(kThreads)
+balance_tokens_kernel(float *part_sums, uint32_t *part_counts, const float *logits, const uint32_t *ids, const uint32_t *offsets,
+                      Shape a) {
+    extern __shared__ float sums_s[];              // [kWarps][experts], then counts u32 [experts]
+    uint32_t *counts_s = reinterpret_cast<uint32_t *>(sums_s + (logits ? kWarps * a.experts : 0u));
+    const uint32_t warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+    pdl_wait();
+    uint32_t t = blockIdx.x * a.chunk;
+    const uint32_t last = min(a.tokens, t + a.chunk);
+    uint32_t s = sequence_of(offsets, a.sequences, t);
+    for (; t < last && s < a.sequences; s++) {
+        const uint32_t end = min(last, end_of(offsets, s, a.tokens));
+        if (end <= t) continue;                    // an empty sequence, or tokens past the last one
+        Row<kV, kVector> acc;
+#pragma unroll
+        for (uint32_t i = 0; i < kV * 4u; i++) acc.v[i] = 0.f;
+        for (uint32_t e = threadIdx.x; e < a.experts; e += kThreads) counts_s[e] = 0u;
+        __syncthreads();
+        for (uint32_t r = t * a.top_k + threadIdx.x; r < end * a.top_k; r += kThreads) {
+            const uint32_t id = ids[r];
+            if (id < a.experts) atomicAdd(&counts_s[id], 1u);
+            else g_balance_status = 2u;
+        }
+        if (logits) {
+            for (uint32_t u = t + warp; u < end; u += kWarps) {
+                Row<kV, kVector> p;
+                p.load(logits + (uint64_t)u * a.experts, a.experts, lane, -INFINITY);
+                p.scores(a.softmax);
+                const float r = a.softmax ? 1.0f : 1.0f / (kTiny + p.sum());
+#pragma unroll
+                for (uint32_t i = 0; i < kV * 4u; i++) acc.v[i] = fmaf(p.v[i], r, acc.v[i]);
+            }
+            acc.store(sums_s + warp * a.experts, a.experts, lane);
+        }
+        __syncthreads();
+        const uint64_t to = (uint64_t)(blockIdx.x + s) * a.experts;
+        for (uint32_t e = threadIdx.x; e < a.experts; e += kThreads) {
+            part_counts[to + e] = counts_s[e];
+            if (logits) {
+                float sum = 0.f;
+#pragma unroll
+                for (uint32_t w = 0; w < kWarps; w++) sum += sums_s[w * a.experts + e];
+                part_sums[to + e] = sum;
+            }
+        }
+        __syncthreads();
+        t = end;
+    }
+}
+
+// one block per sequence
+__global__ void __launch_bounds__(1024)
+balance_sequences_kernel(uint32_t *counts, float *loss, float *means, const float *part_sums, const uint32_t *part_counts,
+                         const uint32_t *offsets, Shape a, float coefficient) {
+    __shared__ float total[32];
+    pdl_wait();
+    const uint32_t s = blockIdx.x, begin = begin_of(offsets, s), end = end_of(offsets, s, a.tokens);
+    const uint32_t length = end > begin ? end - begin : 0u;
+    float product = 0.f;
+    for (uint32_t e = threadIdx.x; e < a.experts; e += blockDim.x) {
+        uint32_t n = 0u;
+        float sum = 0.f;
+        if (length) {
+            for (uint32_t b = begin / a.chunk; b <= (end - 1u) / a.chunk; b++) {
+                n += part_counts[(uint64_t)(b + s) * a.experts + e];
+                if (means) sum += part_sums[(uint64_t)(b + s) * a.experts + e];
+            }
+        }
+        counts[(uint64_t)s * a.experts + e] = n;
+        if (means) {
+            const float mean = length ? sum / (float)length : 0.f;
+            means[(uint64_t)s * a.experts + e] = mean;
+            product = fmaf((float)n, mean, product);
+        }
+    }
+    if (!means) return;
+    product = warp_sum(product);
+    if (threadIdx.x % kWarp == 0u) total[threadIdx.x / kWarp] = product;
+    __syncthreads();
+    if (threadIdx.x < kWarp) {
+        const float sum = warp_sum(threadIdx.x < blockDim.x / kWarp ? total[threadIdx.x] : 0.f);
+        if (threadIdx.x == 0u) {
+            loss[s] = length ? coefficient * sum * ((float)a.experts / ((float)a.top_k * (float)length)) : 0.f;
+        }
+    }
+}
+
+// --------------------------------------------------------------------------------------- backward
+// A warp's tokens follow one another, so a sequence's shares f stay in registers while it lasts.
+template <uint32_t kV, bool kVector>
+__global__ void __launch_bounds__(kThreads)
+router_backward_kernel(float *d_logits, const float *logits, const uint32_t *ids, const uint32_t *counts, const uint32_t *offsets,
+                       const float *d_loss, const float *d_weights, Shape a, float coefficient, float route_scale) {
+    extern __shared__ float rows_s[];              // [kWarps][experts]
+    const uint32_t warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+    float *row_s = rows_s + warp * a.experts;
+    pdl_wait();
+    const uint32_t first = (blockIdx.x * kWarps + warp) * a.chunk;
+    if (first >= a.tokens) return;
+    const uint32_t last = min(a.tokens, first + a.chunk);
+    uint32_t s = 0u, end = first;
+    Row<kV, kVector> f;
+    float c = 0.f;
+    for (uint32_t t = first; t < last; t++) {
+        if (d_loss && t >= end) {
+            s = sequence_of(offsets, a.sequences, t);
+            const uint32_t begin = begin_of(offsets, s);
+            end = end_of(offsets, s, a.tokens);
+            if (t >= end) {                        // past the last sequence: no loss
+                end = a.tokens;
+                c = 0.f;
+#pragma unroll
+                for (uint32_t i = 0; i < kV * 4u; i++) f.v[i] = 0.f;
+            } else {
+                const float length = (float)(end - begin), scale = (float)a.experts / ((float)a.top_k * length);
+                c = coefficient * d_loss[s] / length;
+                f.load(counts + (uint64_t)s * a.experts, a.experts, lane, 0.f);
+#pragma unroll
+                for (uint32_t i = 0; i < kV * 4u; i++) f.v[i] *= scale;
+            }
+        }
+        Row<kV, kVector> p, d;
+        p.load(logits + (uint64_t)t * a.experts, a.experts, lane, -INFINITY);
+        p.scores(a.softmax);
+        if (d_loss && a.softmax) {
+#pragma unroll
+            for (uint32_t i = 0; i < kV * 4u; i++) d.v[i] = c * f.v[i];
+        } else if (d_loss) {
+            float z = 0.f, fp = 0.f;
+#pragma unroll
+            for (uint32_t i = 0; i < kV * 4u; i++) {
+                z += p.v[i];
+                fp = fmaf(f.v[i], p.v[i], fp);
+            }
+            const float r = 1.0f / (kTiny + warp_sum(z));
+            const float mean = warp_sum(fp) * r, cr = c * r;
+#pragma unroll
+            for (uint32_t i = 0; i < kV * 4u; i++) d.v[i] = cr * (f.v[i] - mean);
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < kV * 4u; i++) d.v[i] = 0.f;
+        }
+        if (d_weights) {
+            // the chosen scores from the row in shared memory, then their share added to it there
+            p.store(row_s, a.experts, lane);
+            __syncwarp();
+            const bool has = lane < a.top_k;
+            const uint32_t id = has ? ids[(uint64_t)t * a.top_k + lane] : 0xffffffffu;
+            const bool chosen = has && id < a.experts;
+            if (has && !chosen) g_balance_status = 2u;
+            const float w = chosen ? d_weights[(uint64_t)t * a.top_k + lane] : 0.f, si = chosen ? row_s[id] : 0.f;
+            const float under = 1.0f / (kTiny + warp_sum(si));
+            const float share = route_scale * (w - warp_sum(w * si) * under) * under;
+            __syncwarp();
+            d.store(row_s, a.experts, lane);
+            __syncwarp();
+            const uint32_t same = __match_any_sync(0xffffffffu, chosen ? id : 0x80000000u + lane);
+            if (!__any_sync(0xffffffffu, chosen && (same & (same - 1u)) != 0u)) {
+                if (chosen) row_s[id] += share;
+            } else {                               // an expert named twice: one after the other
+                for (uint32_t r = 0; r < a.top_k; r++) {
+                    if (lane == r && chosen) row_s[id] += share;
+                    __syncwarp();
+                }
+            }
+            __syncwarp();
+            d.load(row_s, a.experts, lane, 0.f);
+            __syncwarp();
+        }
+        if (a.softmax) {
+            float dp = 0.f;
+#pragma unroll
+            for (uint32_t i = 0; i < kV * 4u; i++) dp = fmaf(d.v[i], p.v[i], dp);
+            dp = warp_sum(dp);
+#pragma unroll
+            for (uint32_t i = 0; i < kV * 4u; i++) d.v[i] = p.v[i] * (d.v[i] - dp);
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < kV * 4u; i++) d.v[i] *= p.v[i] * (1.0f - p.v[i]);
+        }
+        d.store(d_logits + (uint64_t)t * a.experts, a.experts, lane);
+    }
+}
+
+bool shape_ok(uint32_t tokens, uint32_t sequences, uint32_t experts, uint32_t top_k, int score, const void *offsets) {
+    return tokens != 0u && tokens <= (1u << 26) && sequences != 0u && sequences <= (1u << 26) && (offsets || sequences == 1u) &&
+           experts != 0u && experts <= kMaxExperts && top_k != 0u && top_k <= 32u && top_k <= experts &&
+           (score == K3_MOE_SCORE_SIGMOID || score == K3_MOE_SCORE_SOFTMAX);
+}
+
+// Tokens per block of the forward pass: two blocks per SM have work, and a warp has at least one token.
+uint32_t forward_chunk(uint32_t tokens) {
+    const uint32_t blocks = 148u * 2u;             // the same partial sums on any device
+    return std::max((tokens + blocks - 1u) / blocks, kWarps);
+}
+
+struct BalanceWorkspace {
+    uint64_t rows;
+    size_t sums, total;
+    BalanceWorkspace(uint32_t tokens, uint32_t sequences, uint32_t experts) {
+        const uint32_t chunk = forward_chunk(tokens);
+        rows = (uint64_t)(tokens + chunk - 1u) / chunk + sequences;
+        sums = (size_t)(rows * experts * sizeof(float) + 255u) / 256u * 256u;
+        total = sums + (size_t)(rows * experts * sizeof(uint32_t));
+    }
+};
+
+// The instance for a number of experts: one to eight groups of 128.
+template <template <uint32_t, bool> class Pick, typename... A>
+bool pick(uint32_t experts, bool vector, A... args) {
+    if (experts <= 128u) return vector ? Pick<1, true>::go(args...) : Pick<1, false>::go(args...);
+    if (experts <= 256u) return vector ? Pick<2, true>::go(args...) : Pick<2, false>::go(args...);
+    if (experts <= 512u) return vector ? Pick<4, true>::go(args...) : Pick<4, false>::go(args...);
+    return vector ? Pick<8, true>::go(args...) : Pick<8, false>::go(args...);
+}
+
+template <uint32_t kV, bool kVector>
+struct Forward {
+    static bool go(float *sums, uint32_t *counts, const float *logits, const uint32_t *ids, const uint32_t *offsets, Shape a,
+                   cudaStream_t stream) {
+        const size_t smem = ((logits ? kWarps : 0u) + 1u) * a.experts * sizeof(float);
+        return set_max_dynamic_smem((const void *)balance_tokens_kernel<kV, kVector>, smem) &&
+               launch_chained(balance_tokens_kernel<kV, kVector>, (a.tokens + a.chunk - 1u) / a.chunk, kThreads, smem, stream,
+                              sums, counts, logits, ids, offsets, a);
+    }
+};
+
+template <uint32_t kV, bool kVector>
+struct Backward {
+    static bool go(float *d_logits, const float *logits, const uint32_t *ids, const uint32_t *counts, const uint32_t *offsets,
+                   const float *d_loss, const float *d_weights, Shape a, float coefficient, float route_scale,
+                   cudaStream_t stream) {
+        const size_t smem = kWarps * a.experts * sizeof(float);
+        const uint32_t warps = (a.tokens + a.chunk - 1u) / a.chunk;
+        return set_max_dynamic_smem((const void *)router_backward_kernel<kV, kVector>, smem) &&
+               launch_chained(router_backward_kernel<kV, kVector>, (warps + kWarps - 1u) / kWarps, kThreads, smem, stream,
+                              d_logits, logits, ids, counts, offsets, d_loss, d_weights, a, coefficient, route_scale);
+    }
+};
+
+bool words_ok(const void *p) { return ((uintptr_t)p & 3u) == 0u; }
+
+}  // namespace
+
+uint32_t k3_balance_status() {
+    uint32_t v = 0xffffffffu;
+    if (cudaMemcpyFromSymbol(&v, g_balance_status, sizeof(v)) != cudaSuccess) (void)cudaGetLastError();
+    return v;
+}
+
+bool k3_balance_status_clear() {
+    const uint32_t zero = 0u;
+    const bool ok = cudaMemcpyToSymbol(g_balance_status, &zero, sizeof(zero)) == cudaSuccess;
+    if (!ok) (void)cudaGetLastError();
+    return ok;
+}
+
+extern "C" size_t k3_moe_balance_workspace_bytes(uint32_t tokens, uint32_t sequences, uint32_t experts) {
+    if (!shape_ok(tokens, sequences, experts, 1u, K3_MOE_SCORE_SIGMOID, &tokens)) return 0;
+    return BalanceWorkspace(tokens, sequences, experts).total;
+}
+
+extern "C" bool k3_moe_balance(void *counts, void *loss, void *means, const void *logits, const void *ids, const void *offsets,
+                               uint32_t tokens, uint32_t sequences, uint32_t experts, uint32_t top_k, int score,
+                               float coefficient, void *workspace, size_t workspace_bytes, void *stream_pointer) {
+    if (!shape_ok(tokens, sequences, experts, top_k, score, offsets) || !counts || !ids || !workspace ||
+        (logits != nullptr) != (loss != nullptr) || (logits != nullptr) != (means != nullptr) || ((uintptr_t)workspace & 15u) != 0u ||
+        !words_ok(counts) || !words_ok(loss) || !words_ok(means) || !words_ok(logits) || !words_ok(ids) || !words_ok(offsets)) {
+        return false;
+    }
+    const BalanceWorkspace w(tokens, sequences, experts);
+    if (workspace_bytes < w.total) return false;
+    cudaStream_t stream = (cudaStream_t)stream_pointer;
+    const Shape a{tokens, sequences, experts, top_k, forward_chunk(tokens), score};
+    float *sums = (float *)workspace;
+    uint32_t *part_counts = (uint32_t *)((char *)workspace + w.sums);
+    const bool vector = experts % 4u == 0u && ((uintptr_t)logits & 15u) == 0u;
+    return pick<Forward>(experts, vector, sums, part_counts, (const float *)logits, (const uint32_t *)ids, (const uint32_t *)offsets,
+                         a, stream) &&
+           launch_chained(balance_sequences_kernel, sequences, 1024, 0, stream, (uint32_t *)counts, (float *)loss, (float *)means,
+                          (const float *)sums, (const uint32_t *)part_counts, (const uint32_t *)offsets, a, coefficient);
+}
+
+extern "C" bool k3_moe_router_backward(void *d_logits, const void *logits, const void *ids, const void *counts,
+                                       const void *offsets, const void *d_loss, const void *d_weights, uint32_t tokens,
+                                       uint32_t sequences, uint32_t experts, uint32_t top_k, int score, float coefficient,
+                                       float route_scale, void *stream) {
+    if (!shape_ok(tokens, sequences, experts, top_k, score, offsets) || !d_logits || !logits || (!d_loss && !d_weights) ||
+        (d_loss && !counts) || (d_weights && (!ids || !(route_scale > 0.0f))) || !words_ok(d_logits) || !words_ok(logits) ||
+        !words_ok(ids) || !words_ok(counts) || !words_ok(offsets) || !words_ok(d_loss) || !words_ok(d_weights)) {
+        return false;
+    }
+    const uint32_t warps = (uint32_t)sm_count() * 2u * kWarps;
+    const Shape a{tokens, sequences, experts, top_k, std::max((tokens + warps - 1u) / warps, 1u), score};
+    const bool vector = experts % 4u == 0u && (((uintptr_t)logits | (uintptr_t)d_logits | (uintptr_t)counts) & 15u) == 0u;
+    return pick<Backward>(experts, vector, (float *)d_logits, (const float *)logits, (const uint32_t *)ids, (const uint32_t *)counts,
+                          (const uint32_t *)offsets, (const float *)d_loss, (const float *)d_weights, a, coefficient, route_scale,
+                          (cudaStream_t)stream);
+}

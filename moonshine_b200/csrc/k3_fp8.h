@@ -1,0 +1,54 @@
+// Internal interface of the E4M3 block-scaled operators: quantisers (k3_fp8_quantize.cu),
+// products (k3_fp8_product.cu), experts (k3_fp8_experts.cu).
+#pragma once
+
+#include "k3_moe_fp8.h"
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace k3::fp8 {
+
+constexpr uint32_t kBlock = 128;
+
+constexpr uint32_t pitch_of(uint32_t columns) { return (columns + 15u) & ~15u; }
+constexpr uint32_t blocks_of(uint32_t n) { return (n + kBlock - 1u) / kBlock; }
+constexpr uint32_t scale_pitch_of(uint32_t columns) { return (blocks_of(columns) + 3u) & ~3u; }
+
+// every extent of an entry point: coordinates and row numbers stay well inside 32 bits
+inline bool extent_ok(uint32_t n) { return n != 0u && n <= (1u << 30); }
+inline bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0u; }
+
+// Rows of x quantised and put where a dispatch wants them: row t goes to rows place[t * top_k + r] of
+// codes and scales.  A route whose id is no expert (ids[...] >= experts) goes nowhere, and its place is
+// set to `spare`; zero_row (zero_bytes, whole 16-byte units) is cleared on the way.
+struct Placement {
+    uint32_t *place;
+    const uint32_t *ids;
+    uint32_t top_k, experts, spare;
+};
+bool quantize_placed(void *codes, void *scales, const void *x_bf16, uint32_t rows, uint32_t columns,
+                     const Placement &placement, void *zero_row, uint32_t zero_bytes, cudaStream_t stream);
+
+}  // namespace k3::fp8
+
+namespace k3::fp8 {
+
+enum Epilogue : int { kOutBf16 = 0, kOutF32 = 1, kOutActivated = 2 };
+
+// out [rows, n] = a [rows, k] b^T.  With offsets (u32 [groups + 1] on the device) a's rows are grouped:
+// rows [offsets[g], offsets[g + 1]) are multiplied by matrix g of b [groups, n, k].  kOutActivated: b is
+// the gate, b2 the up matrix, and what is written is the activation, quantised by rows (out, out_scales).
+struct Product {
+    void *out, *out_scales;
+    const void *a, *a_scales;
+    const void *b, *b_scales, *b2, *b2_scales;
+    const uint32_t *offsets;
+    uint32_t groups, rows, n, k;
+    int b_scale_layout, epilogue, accumulate;
+    int activation;
+    float beta, linear_beta;
+};
+bool product(const Product &p, cudaStream_t stream);
+
+}  // namespace k3::fp8

@@ -1,0 +1,166 @@
+// What is composed of the E4M3 quantisers and products: a linear layer, its weight's gradient, and the
+// routed experts (dispatch, rows quantised into place, gate/up with the activation, down, combine).
+#include "k3_common.cuh"
+#include "k3_fp8.h"
+#include "k3_moe_layer.h"
+#include "k3_moe_ops.h"
+
+using namespace k3;
+using namespace k3::fp8;
+
+namespace {
+
+// Pieces of a caller's workspace, each on 256 bytes; with base null only the total is counted.
+struct Carve {
+    char *base;
+    size_t total = 0;
+    void *take(uint64_t bytes) {
+        void *p = base ? base + total : nullptr;
+        total += (size_t)((bytes + 255u) / 256u * 256u);
+        return p;
+    }
+};
+
+struct Rows {                        // codes with scales per row
+    void *codes, *scales;
+    Rows(Carve &c, uint64_t rows, uint32_t columns)
+        : codes(c.take(rows * pitch_of(columns))), scales(c.take(rows * scale_pitch_of(columns) * sizeof(float))) {}
+};
+
+struct ExpertsWorkspace {
+    Carve carve;
+    uint32_t *offsets, *sorted_route, *sorted_token, *inv_perm;
+    size_t dispatch_bytes;
+    void *dispatch;
+    Rows x, act;
+    uint16_t *rows_out;              // one row more than there are routes: the spare one
+    ExpertsWorkspace(const k3_moe_fp8_experts_desc *d, uint32_t tokens, void *base)
+        : carve{(char *)base},
+          offsets((uint32_t *)carve.take((d->experts + 1u) * sizeof(uint32_t))),
+          sorted_route((uint32_t *)carve.take((uint64_t)tokens * d->top_k * sizeof(uint32_t))),
+          sorted_token((uint32_t *)carve.take((uint64_t)tokens * d->top_k * sizeof(uint32_t))),
+          inv_perm((uint32_t *)carve.take((uint64_t)tokens * d->top_k * sizeof(uint32_t))),
+          dispatch_bytes(k3_moe_dispatch_workspace_bytes(tokens, d->top_k, d->experts)),
+          dispatch(carve.take(dispatch_bytes)),
+          x(carve, (uint64_t)tokens * d->top_k, d->hidden),
+          act(carve, (uint64_t)tokens * d->top_k, d->expert_hidden),
+          rows_out((uint16_t *)carve.take(((uint64_t)tokens * d->top_k + 1u) * d->hidden * 2u)) {}
+};
+
+bool experts_ok(const k3_moe_fp8_experts_desc *d, uint32_t tokens) {
+    return d && extent_ok(d->hidden) && d->hidden % 16u == 0 && extent_ok(d->expert_hidden) && d->expert_hidden % 16u == 0 &&
+           d->experts != 0u && d->experts <= 1024u && d->top_k != 0u && d->top_k <= 32u && d->top_k <= d->experts &&
+           (d->activation == K3_MOE_ACT_SITU || d->activation == K3_MOE_ACT_SWIGLU) &&
+           (d->activation != K3_MOE_ACT_SITU || (d->beta > 0.0f && d->linear_beta > 0.0f)) &&
+           (uint64_t)d->experts * d->hidden <= (1u << 30) && (uint64_t)d->experts * d->expert_hidden <= (1u << 30) &&
+           tokens != 0u && (uint64_t)tokens * d->top_k <= (1u << 30);
+}
+
+bool table_ok(const void *codes, const void *scales) { return codes && scales && aligned16(codes) && ((uintptr_t)scales & 3u) == 0u; }
+
+}  // namespace
+
+extern "C" size_t k3_moe_fp8_linear_workspace_bytes(uint32_t tokens, uint32_t columns) {
+    if (!extent_ok(tokens) || !extent_ok(columns)) return 0;
+    Carve c{nullptr};
+    Rows x(c, tokens, columns);
+    return c.total;
+}
+
+extern "C" bool k3_moe_fp8_linear(void *out, const void *x, const void *w, const void *w_scales, uint32_t tokens, uint32_t rows,
+                                  uint32_t columns, void *workspace, size_t workspace_bytes, void *stream) {
+    if (!out || !x || !table_ok(w, w_scales) || !extent_ok(tokens) || !extent_ok(rows) || !extent_ok(columns) || !workspace ||
+        !aligned16(workspace) || (((uintptr_t)out | (uintptr_t)x) & 1u) != 0u) {
+        return false;
+    }
+    Carve c{(char *)workspace};
+    const Rows q(c, tokens, columns);
+    if (workspace_bytes < c.total) return false;
+    return k3_moe_fp8_quantize_rows(q.codes, q.scales, x, tokens, columns, K3_MOE_FP8_BF16, stream) &&
+           k3_moe_fp8_product(out, q.codes, q.scales, w, w_scales, tokens, rows, columns, K3_MOE_FP8_BLOCKS, K3_MOE_FP8_BF16, 0,
+                              stream);
+}
+
+extern "C" size_t k3_moe_fp8_weight_gradient_workspace_bytes(uint32_t tokens, uint32_t rows, uint32_t columns) {
+    if (!extent_ok(tokens) || !extent_ok(rows) || !extent_ok(columns)) return 0;
+    Carve c{nullptr};
+    Rows dy(c, rows, tokens), x(c, columns, tokens);
+    return c.total;
+}
+
+extern "C" bool k3_moe_fp8_weight_gradient(void *dw, const void *dy, const void *x, uint32_t tokens, uint32_t rows,
+                                           uint32_t columns, int accumulate, void *workspace, size_t workspace_bytes,
+                                           void *stream) {
+    if (!dw || !dy || !x || !extent_ok(tokens) || !extent_ok(rows) || !extent_ok(columns) || !workspace ||
+        !aligned16(workspace) || ((uintptr_t)dw & 3u) != 0u || (((uintptr_t)dy | (uintptr_t)x) & 1u) != 0u) {
+        return false;
+    }
+    Carve c{(char *)workspace};
+    const Rows dyq(c, rows, tokens), xq(c, columns, tokens);
+    if (workspace_bytes < c.total) return false;
+    return k3_moe_fp8_quantize_columns(dyq.codes, dyq.scales, dy, tokens, rows, K3_MOE_FP8_BF16, stream) &&
+           k3_moe_fp8_quantize_columns(xq.codes, xq.scales, x, tokens, columns, K3_MOE_FP8_BF16, stream) &&
+           k3_moe_fp8_product(dw, dyq.codes, dyq.scales, xq.codes, xq.scales, rows, columns, tokens, K3_MOE_FP8_ROWS,
+                              K3_MOE_FP8_F32, accumulate, stream);
+}
+
+extern "C" size_t k3_moe_fp8_experts_workspace_bytes(const k3_moe_fp8_experts_desc *d, uint32_t tokens) {
+    if (!experts_ok(d, tokens)) return 0;
+    return ExpertsWorkspace(d, tokens, nullptr).carve.total;
+}
+
+extern "C" bool k3_moe_fp8_experts_forward(const k3_moe_fp8_experts_desc *d, void *out, const void *x, const void *ids,
+                                           const void *weights, const void *shared, uint32_t tokens, void *workspace,
+                                           size_t workspace_bytes, void *stream_pointer) {
+    if (!experts_ok(d, tokens) || !out || !x || !ids || !weights || !workspace || !aligned16(workspace) ||
+        !table_ok(d->w1, d->w1_scales) || !table_ok(d->w3, d->w3_scales) || !table_ok(d->w2, d->w2_scales) ||
+        (((uintptr_t)out | (uintptr_t)shared) & 15u) != 0u || ((uintptr_t)x & 1u) != 0u ||
+        (((uintptr_t)ids | (uintptr_t)weights) & 3u) != 0u) {
+        return false;
+    }
+    const ExpertsWorkspace w(d, tokens, workspace);
+    if (workspace_bytes < w.carve.total) return false;
+    cudaStream_t stream = (cudaStream_t)stream_pointer;
+    const uint32_t routes = tokens * d->top_k;
+    if (!k3_moe_dispatch_build(w.offsets, w.sorted_route, w.sorted_token, w.inv_perm, ids, tokens, d->top_k, d->experts,
+                               w.dispatch, w.dispatch_bytes, stream)) {
+        return false;
+    }
+    const Placement at{w.inv_perm, (const uint32_t *)ids, d->top_k, d->experts, routes};
+    if (!quantize_placed(w.x.codes, w.x.scales, x, tokens, d->hidden, at, w.rows_out + (uint64_t)routes * d->hidden,
+                         d->hidden * 2u, stream)) {
+        return false;
+    }
+    Product p{};
+    p.out = w.act.codes;
+    p.out_scales = w.act.scales;
+    p.a = w.x.codes;
+    p.a_scales = w.x.scales;
+    p.b = d->w1;
+    p.b_scales = d->w1_scales;
+    p.b2 = d->w3;
+    p.b2_scales = d->w3_scales;
+    p.offsets = w.offsets;
+    p.groups = d->experts;
+    p.rows = routes;
+    p.n = d->expert_hidden;
+    p.k = d->hidden;
+    p.b_scale_layout = K3_MOE_FP8_BLOCKS;
+    p.epilogue = kOutActivated;
+    p.activation = d->activation;
+    p.beta = d->beta;
+    p.linear_beta = d->linear_beta;
+    if (!product(p, stream)) return false;
+    p.out = w.rows_out;
+    p.out_scales = nullptr;
+    p.a = w.act.codes;
+    p.a_scales = w.act.scales;
+    p.b = d->w2;
+    p.b_scales = d->w2_scales;
+    p.b2 = p.b2_scales = nullptr;
+    p.n = d->hidden;
+    p.k = d->expert_hidden;
+    p.epilogue = kOutBf16;
+    if (!product(p, stream)) return false;
+    return k3_moe_combine(out, w.rows_out, w.inv_perm, weights, shared, tokens, d->top_k, d->hidden, stream);
+}

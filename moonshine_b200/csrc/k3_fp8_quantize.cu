@@ -1,0 +1,362 @@
+// Matrices to E4M3 codes with one f32 scale per block of 128: of a row, of a column (transposed), of a
+// 128 x 128 tile; and a weight table's transposed layout.
+//
+//   scale = max(largest |x| of the block / 448, 2^-126),  code = e4m3(x / scale)
+//
+// Both quotients are those of f32 division.  One division per block gives the scale, one its
+// reciprocal; an element's quotient is then the product with the reciprocal, corrected once by its
+// remainder (Markstein 1990: with a correctly rounded reciprocal this is the rounded quotient), three
+// operations in place of a division.  The distance matters: where the largest magnitude of bf16 data
+// is a multiple of 7, one element in some hundred lies exactly between two codes.
+//
+// The largest magnitude is taken of the bit patterns without their signs, which order like the
+// values and put infinities and NaN above all of them; a block with one gets the scale NaN.
+#include "k3_common.cuh"
+#include "k3_fp8.h"
+
+#include <cuda_fp8.h>
+
+using namespace k3;
+using namespace k3::fp8;
+
+namespace {
+
+constexpr uint32_t kThreads = 256;
+
+K3_DEVINL float scale_of(uint32_t largest_bits) {
+    if (largest_bits >= 0x7f800000u) return __uint_as_float(0x7fffffffu);
+    return fmaxf(__fdiv_rn(__uint_as_float(largest_bits), 448.0f), 0x1p-126f);
+}
+
+K3_DEVINL float quotient(float x, float scale, float inverse) {
+    const float r = x * inverse;
+    return copysignf(fmaf(fmaf(-r, scale, x), inverse, r), x);       // the correction would turn -0 into 0
+}
+
+// two codes, `lo` in the low byte
+K3_DEVINL uint32_t codes2(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+K3_DEVINL uint2 codes8(const uint32_t (&bits)[8], float scale, float inverse) {
+    uint32_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        h[i] = codes2(quotient(__uint_as_float(bits[2 * i]), scale, inverse),
+                      quotient(__uint_as_float(bits[2 * i + 1]), scale, inverse));
+    }
+    return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+}
+
+K3_DEVINL uint32_t largest8(const uint32_t (&bits)[8]) {
+    uint32_t m = 0u;
+#pragma unroll
+    for (int i = 0; i < 8; i++) m = max(m, bits[i] & 0x7fffffffu);
+    return m;
+}
+
+// Eight elements of a row from column c as f32 bit patterns, zeros past the end.  kVector: the row
+// starts on 16 bytes and its length is a multiple of 8 elements.
+template <bool kF32, bool kVector>
+K3_DEVINL void load8(uint32_t (&bits)[8], const void *row, uint32_t c, uint32_t columns) {
+    if (kVector) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) bits[i] = 0u;
+        if (c >= columns) return;
+        if (kF32) {
+            const uint4 a = *reinterpret_cast<const uint4 *>((const uint32_t *)row + c);
+            const uint4 b = *reinterpret_cast<const uint4 *>((const uint32_t *)row + c + 4u);
+            bits[0] = a.x; bits[1] = a.y; bits[2] = a.z; bits[3] = a.w;
+            bits[4] = b.x; bits[5] = b.y; bits[6] = b.z; bits[7] = b.w;
+        } else {
+            const uint4 a = *reinterpret_cast<const uint4 *>((const uint16_t *)row + c);
+            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                bits[2 * i] = w[i] << 16;
+                bits[2 * i + 1] = w[i] & 0xffff0000u;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            bits[i] = 0u;
+            if (c + i < columns) {
+                bits[i] = kF32 ? ((const uint32_t *)row)[c + i] : (uint32_t)((const uint16_t *)row)[c + i] << 16;
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------- rows
+// Half a warp takes four neighbouring blocks of a row: lane l holds elements 8 l .. 8 l + 7 of each.
+struct RowsArgs {
+    uint8_t *codes;
+    float *scales;
+    const void *x;
+    uint32_t rows, columns, tasks_per_row;
+    Placement at;
+    uint4 *zero_row;                 // cleared on the way (zero_units 16-byte units), or null
+    uint32_t zero_units;
+};
+
+template <bool kF32, bool kVector, bool kPlaced>
+__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(RowsArgs a) {
+    pdl_wait();
+    if (kPlaced && blockIdx.x == 0u) {
+        for (uint32_t i = threadIdx.x; i < a.zero_units; i += kThreads) a.zero_row[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    const uint32_t half = threadIdx.x / 16u, l = threadIdx.x % 16u;
+    const uint64_t task = (uint64_t)blockIdx.x * (kThreads / 16u) + half;
+    const uint32_t row = (uint32_t)task / a.tasks_per_row;
+    const uint32_t group = (uint32_t)task - row * a.tasks_per_row;
+    const bool live = task < (uint64_t)a.rows * a.tasks_per_row;     // the shuffles below want every lane
+    const char *x = (const char *)a.x + (uint64_t)(live ? row : 0u) * a.columns * (kF32 ? 4u : 2u);
+    uint32_t bits[4][8];
+#pragma unroll
+    for (int b = 0; b < 4; b++) {
+        load8<kF32, kVector>(bits[b], x, (group * 4u + b) * kBlock + l * 8u, live ? a.columns : 0u);
+    }
+    float scale[4];
+    uint2 out[4];
+#pragma unroll
+    for (int b = 0; b < 4; b++) {
+        uint32_t m = largest8(bits[b]);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        scale[b] = scale_of(m);
+        out[b] = codes8(bits[b], scale[b], __frcp_rn(scale[b]));
+        if ((group * 4u + b) * kBlock >= a.columns) scale[b] = 0.0f;  // padding of the scales' row
+    }
+    if (!live) return;
+    const uint32_t pitch = pitch_of(a.columns), scale_pitch = a.tasks_per_row * 4u;
+    auto store = [&](uint32_t to) {
+        if (l == 0u) {
+            *reinterpret_cast<float4 *>(a.scales + (uint64_t)to * scale_pitch + group * 4u) =
+                make_float4(scale[0], scale[1], scale[2], scale[3]);
+        }
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+            const uint32_t c = (group * 4u + b) * kBlock + l * 8u;
+            if (c < pitch) *reinterpret_cast<uint2 *>(a.codes + (uint64_t)to * pitch + c) = out[b];
+        }
+    };
+    if (!kPlaced) {
+        store(row);
+    } else {
+        for (uint32_t r = 0; r < a.at.top_k; r++) {
+            const uint32_t route = row * a.at.top_k + r;
+            if (a.at.ids[route] < a.at.experts) {
+                store(a.at.place[route]);
+            } else if (group == 0u && l == 0u) {
+                a.at.place[route] = a.at.spare;
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------- columns
+// One block of threads takes 128 rows x 64 columns: thread (rt, ct) the rows 4 rt .. 4 rt + 3 of
+// columns 8 ct .. 8 ct + 7.  Four codes of a column make one word of the transposed tile, which
+// goes through shared memory and leaves as 128 contiguous bytes per column.
+constexpr uint32_t kTileColumns = 64, kTileWords = 33;                // words per column, one to spare
+
+template <bool kF32, bool kVector>
+__global__ void __launch_bounds__(kThreads)
+quantize_columns_kernel(uint8_t *codes, float *scales, const void *x, uint32_t rows, uint32_t columns) {
+    __shared__ uint32_t largest[8][kTileColumns];
+    __shared__ uint32_t tile[kTileColumns * kTileWords];
+    pdl_wait();
+    const uint32_t r0 = blockIdx.y * kBlock, c0 = blockIdx.x * kTileColumns;
+    const uint32_t ct = threadIdx.x % 8u, rt = threadIdx.x / 8u, warp = threadIdx.x / kWarp;
+    uint32_t bits[4][8];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t r = r0 + rt * 4u + i;
+        const char *row = (const char *)x + (uint64_t)(r < rows ? r : 0u) * columns * (kF32 ? 4u : 2u);
+        load8<kF32, kVector>(bits[i], row, c0 + ct * 8u, r < rows ? columns : 0u);
+    }
+    uint32_t m[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        m[j] = 0u;
+#pragma unroll
+        for (int i = 0; i < 4; i++) m[j] = max(m[j], bits[i][j] & 0x7fffffffu);
+        m[j] = max(m[j], __shfl_xor_sync(0xffffffffu, m[j], 8));
+        m[j] = max(m[j], __shfl_xor_sync(0xffffffffu, m[j], 16));
+    }
+    if (threadIdx.x % kWarp < 8u) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) largest[warp][ct * 8u + j] = m[j];
+    }
+    __syncthreads();
+    const uint32_t scale_pitch = scale_pitch_of(rows);
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        uint32_t all = 0u;
+#pragma unroll
+        for (int w = 0; w < 8; w++) all = max(all, largest[w][ct * 8u + j]);
+        const float scale = scale_of(all), inverse = __frcp_rn(scale);
+        float q[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) q[i] = quotient(__uint_as_float(bits[i][j]), scale, inverse);
+        tile[(ct * 8u + j) * kTileWords + rt] = codes2(q[0], q[1]) | (codes2(q[2], q[3]) << 16);
+        const uint32_t c = c0 + ct * 8u + j;
+        if (rt == 0u && c < columns) {
+            float *to = scales + (uint64_t)c * scale_pitch + blockIdx.y;
+            *to = scale;
+            if (blockIdx.y + 1u == gridDim.y) {
+                for (uint32_t p = 1u; blockIdx.y + p < scale_pitch; p++) to[p] = 0.0f;
+            }
+        }
+    }
+    __syncthreads();
+    const uint32_t pitch = pitch_of(rows);
+#pragma unroll
+    for (uint32_t i = 0; i < 2u; i++) {
+        const uint32_t unit = i * kThreads + threadIdx.x, c = unit / 8u, u = unit % 8u;
+        const uint32_t r = r0 + u * 16u;
+        if (c0 + c < columns && r < pitch) {
+            const uint32_t *w = tile + c * kTileWords + u * 4u;
+            *reinterpret_cast<uint4 *>(codes + (uint64_t)(c0 + c) * pitch + r) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+}
+
+// ----------------------------------------------------------------------------------------- blocks
+template <bool kF32, bool kVector>
+__global__ void __launch_bounds__(kThreads)
+quantize_blocks_kernel(uint8_t *codes, float *scales, const void *x, uint32_t rows, uint32_t columns) {
+    __shared__ uint32_t largest[8];
+    pdl_wait();
+    const uint32_t r0 = blockIdx.y * kBlock, c = blockIdx.x * kBlock + (threadIdx.x % 16u) * 8u, rt = threadIdx.x / 16u;
+    uint32_t bits[8][8], m = 0u;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const uint32_t r = r0 + i * 16u + rt;
+        const char *row = (const char *)x + (uint64_t)(r < rows ? r : 0u) * columns * (kF32 ? 4u : 2u);
+        load8<kF32, kVector>(bits[i], row, c, r < rows ? columns : 0u);
+        m = max(m, largest8(bits[i]));
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (threadIdx.x % kWarp == 0u) largest[threadIdx.x / kWarp] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; w++) m = max(m, largest[w]);
+    const float scale = scale_of(m), inverse = __frcp_rn(scale);
+    if (threadIdx.x == 0u) scales[(uint64_t)blockIdx.y * gridDim.x + blockIdx.x] = scale;
+    const uint32_t pitch = pitch_of(columns);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const uint32_t r = r0 + i * 16u + rt;
+        if (r < rows && c < pitch) {
+            *reinterpret_cast<uint2 *>(codes + (uint64_t)r * pitch + c) = codes8(bits[i], scale, inverse);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------- transposing
+// 128 x 128 codes through shared memory; a table is laid out once, so this is plain.
+__global__ void __launch_bounds__(kThreads)
+transpose_blocks_kernel(uint8_t *to, float *to_scales, const uint8_t *from, const float *from_scales, uint32_t rows,
+                        uint32_t columns) {
+    __shared__ uint8_t tile[kBlock][kBlock + 4u];
+    pdl_wait();
+    const uint32_t r0 = blockIdx.y * kBlock, c0 = blockIdx.x * kBlock;
+    const uint32_t from_pitch = pitch_of(columns), to_pitch = pitch_of(rows);
+    for (uint32_t i = threadIdx.x; i < kBlock * kBlock; i += kThreads) {
+        const uint32_t r = i / kBlock, c = i % kBlock;
+        tile[r][c] = r0 + r < rows && c0 + c < columns ? from[(uint64_t)(r0 + r) * from_pitch + c0 + c] : 0u;
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < kBlock * kBlock; i += kThreads) {
+        const uint32_t c = i / kBlock, r = i % kBlock;
+        if (c0 + c < columns && r0 + r < to_pitch) to[(uint64_t)(c0 + c) * to_pitch + r0 + r] = tile[r][c];
+    }
+    if (threadIdx.x == 0u) to_scales[(uint64_t)blockIdx.x * gridDim.y + blockIdx.y] = from_scales[(uint64_t)blockIdx.y * gridDim.x + blockIdx.x];
+}
+
+// Rows whose length and start allow 16-byte loads.
+bool vector_rows(const void *x, uint32_t columns) { return aligned16(x) && columns % 8u == 0u; }
+
+bool arguments_ok(const void *codes, const void *scales, const void *x, uint32_t rows, uint32_t columns, int type) {
+    return codes && scales && x && aligned16(codes) && aligned16(scales) && extent_ok(rows) && extent_ok(columns) &&
+           (type == K3_MOE_FP8_BF16 || type == K3_MOE_FP8_F32) &&
+           ((uintptr_t)x & (type == K3_MOE_FP8_F32 ? 3u : 1u)) == 0u;
+}
+
+bool launch_rows(RowsArgs a, bool f32, bool placed, cudaStream_t stream) {
+    a.tasks_per_row = scale_pitch_of(a.columns) / 4u;
+    const uint64_t tasks = (uint64_t)a.rows * a.tasks_per_row;
+    if (tasks > 0xffffffffull) return false;
+    const dim3 grid((uint32_t)((tasks + kThreads / 16u - 1u) / (kThreads / 16u)));
+    const bool v = vector_rows(a.x, a.columns);
+    if (placed) {
+        return launch_chained(v ? quantize_rows_kernel<false, true, true> : quantize_rows_kernel<false, false, true>, grid,
+                              kThreads, 0, stream, a);
+    }
+    return launch_chained(f32 ? (v ? quantize_rows_kernel<true, true, false> : quantize_rows_kernel<true, false, false>)
+                              : (v ? quantize_rows_kernel<false, true, false> : quantize_rows_kernel<false, false, false>),
+                          grid, kThreads, 0, stream, a);
+}
+
+}  // namespace
+
+bool k3::fp8::quantize_placed(void *codes, void *scales, const void *x, uint32_t rows, uint32_t columns,
+                              const Placement &placement, void *zero_row, uint32_t zero_bytes, cudaStream_t stream) {
+    RowsArgs a{};
+    a.codes = (uint8_t *)codes;
+    a.scales = (float *)scales;
+    a.x = x;
+    a.rows = rows;
+    a.columns = columns;
+    a.at = placement;
+    a.zero_row = (uint4 *)zero_row;
+    a.zero_units = zero_bytes / 16u;
+    return launch_rows(a, false, true, stream);
+}
+
+extern "C" bool k3_moe_fp8_quantize_rows(void *codes, void *scales, const void *x, uint32_t rows, uint32_t columns,
+                                         int x_type, void *stream) {
+    if (!arguments_ok(codes, scales, x, rows, columns, x_type)) return false;
+    RowsArgs a{};
+    a.codes = (uint8_t *)codes;
+    a.scales = (float *)scales;
+    a.x = x;
+    a.rows = rows;
+    a.columns = columns;
+    return launch_rows(a, x_type == K3_MOE_FP8_F32, false, (cudaStream_t)stream);
+}
+
+extern "C" bool k3_moe_fp8_quantize_columns(void *codes, void *scales, const void *x, uint32_t rows, uint32_t columns,
+                                            int x_type, void *stream) {
+    if (!arguments_ok(codes, scales, x, rows, columns, x_type) || blocks_of(rows) > 65535u) return false;
+    const dim3 grid((columns + kTileColumns - 1u) / kTileColumns, blocks_of(rows));
+    const bool f32 = x_type == K3_MOE_FP8_F32, v = vector_rows(x, columns);
+    return launch_chained(f32 ? (v ? quantize_columns_kernel<true, true> : quantize_columns_kernel<true, false>)
+                              : (v ? quantize_columns_kernel<false, true> : quantize_columns_kernel<false, false>),
+                          grid, kThreads, 0, (cudaStream_t)stream, (uint8_t *)codes, (float *)scales, x, rows, columns);
+}
+
+extern "C" bool k3_moe_fp8_quantize_blocks(void *codes, void *scales, const void *x, uint32_t rows, uint32_t columns,
+                                           int x_type, void *stream) {
+    if (!arguments_ok(codes, scales, x, rows, columns, x_type) || blocks_of(rows) > 65535u) return false;
+    const dim3 grid(blocks_of(columns), blocks_of(rows));
+    const bool f32 = x_type == K3_MOE_FP8_F32, v = vector_rows(x, columns);
+    return launch_chained(f32 ? (v ? quantize_blocks_kernel<true, true> : quantize_blocks_kernel<true, false>)
+                              : (v ? quantize_blocks_kernel<false, true> : quantize_blocks_kernel<false, false>),
+                          grid, kThreads, 0, (cudaStream_t)stream, (uint8_t *)codes, (float *)scales, x, rows, columns);
+}
+
+extern "C" bool k3_moe_fp8_transpose_blocks(void *codes_out, void *scales_out, const void *codes, const void *scales,
+                                            uint32_t rows, uint32_t columns, void *stream) {
+    if (!codes_out || !scales_out || !codes || !scales || codes_out == codes || !aligned16(codes_out) || !aligned16(codes) ||
+        !extent_ok(rows) || !extent_ok(columns) || blocks_of(rows) > 65535u) {
+        return false;
+    }
+    return launch_chained(transpose_blocks_kernel, dim3(blocks_of(columns), blocks_of(rows)), kThreads, 0, (cudaStream_t)stream,
+                          (uint8_t *)codes_out, (float *)scales_out, (const uint8_t *)codes, (const float *)scales, rows,
+                          columns);
+}

@@ -9,6 +9,8 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include "k3_moe_balance.h"
+#include "k3_moe_fp8.h"
 #include "k3_moe_layer.h"
 #include "k3_moe_ops.h"
 
@@ -18,7 +20,7 @@
 
 namespace {
 
-PyObject *g_tensor_type, *g_layer_desc_type, *g_latent_desc_type, *g_get_stream, *g_get_device, *g_is_contiguous, *g_data_ptr, *g_stream_kw;
+PyObject *g_tensor_type, *g_layer_desc_type, *g_latent_desc_type, *g_fp8_desc_type, *g_get_stream, *g_get_device, *g_is_contiguous, *g_data_ptr, *g_stream_kw;
 
 enum class Got { kYes, kFallback, kError };
 
@@ -96,6 +98,7 @@ struct Structure {                                         // the ctypes structu
 };
 template <> struct Arg<const k3_moe_layer_desc *> : Structure<k3_moe_layer_desc, &g_layer_desc_type> {};
 template <> struct Arg<const k3_moe_latent_desc *> : Structure<k3_moe_latent_desc, &g_latent_desc_type> {};
+template <> struct Arg<const k3_moe_fp8_experts_desc *> : Structure<k3_moe_fp8_experts_desc, &g_fp8_desc_type> {};
 
 Got current_stream(void **out) {
     PyObject *device = PyObject_CallNoArgs(g_get_device);
@@ -206,22 +209,33 @@ PyMethodDef kBound[] = {
     K3_BIND(k3_moe_layer_forward),
     K3_BIND(k3_moe_block_forward),
     K3_BIND(k3_moe_latent_layer_forward),
+    K3_BIND(k3_moe_fp8_quantize_rows),
+    K3_BIND(k3_moe_fp8_quantize_columns),
+    K3_BIND(k3_moe_fp8_quantize_blocks),
+    K3_BIND(k3_moe_fp8_product),
+    K3_BIND(k3_moe_fp8_linear),
+    K3_BIND(k3_moe_fp8_weight_gradient),
+    K3_BIND(k3_moe_fp8_experts_forward),
+    K3_BIND(k3_moe_balance),
+    K3_BIND(k3_moe_router_backward),
     {nullptr, nullptr, 0, nullptr},
 };
 
-// bind(fallbacks, tensor type, layer and latent description types, raw stream getter, device
+// bind(fallbacks, tensor type, layer, latent and fp8 experts description types, raw stream getter, device
 // getter) -> {name: function}
 PyObject *bind(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
-    if (nargs != 6 || !PyDict_Check(args[0]) || !PyType_Check(args[1]) || !PyType_Check(args[2]) ||
-        !PyType_Check(args[3])) {
-        PyErr_SetString(PyExc_TypeError, "bind(dict, tensor type, layer type, latent type, stream getter, device getter)");
+    if (nargs != 7 || !PyDict_Check(args[0]) || !PyType_Check(args[1]) || !PyType_Check(args[2]) ||
+        !PyType_Check(args[3]) || !PyType_Check(args[4])) {
+        PyErr_SetString(PyExc_TypeError,
+                        "bind(dict, tensor type, layer type, latent type, fp8 experts type, stream getter, device getter)");
         return nullptr;
     }
     g_tensor_type = Py_NewRef(args[1]);
     g_layer_desc_type = Py_NewRef(args[2]);
     g_latent_desc_type = Py_NewRef(args[3]);
-    g_get_stream = Py_NewRef(args[4]);
-    g_get_device = Py_NewRef(args[5]);
+    g_fp8_desc_type = Py_NewRef(args[4]);
+    g_get_stream = Py_NewRef(args[5]);
+    g_get_device = Py_NewRef(args[6]);
     PyObject *out = PyDict_New();
     for (PyMethodDef *d = kBound; out && d->ml_name; d++) {
         PyObject *fallback = PyDict_GetItemString(args[0], d->ml_name);

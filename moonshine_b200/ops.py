@@ -73,8 +73,11 @@ if (os.path.exists(os.path.join(os.path.dirname(__file__), "_k3ops.so"))
         and hasattr(torch._C, "_cuda_getCurrentRawStream") and hasattr(torch._C, "_cuda_getDevice")):
     from . import _k3ops
     _CALLS.update(_k3ops.bind(_CALLS, torch.Tensor, _native.LayerDesc, _native.LatentDesc,
-                              torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice))
+                              _native.Fp8ExpertsDesc, torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice))
 globals().update(_CALLS)
 
 ACT_SITU, ACT_SWIGLU = 0, 1
 Q8_F32, Q8_F16 = 0, 1
+FP8_BF16, FP8_F32 = 0, 1
+FP8_BLOCKS, FP8_ROWS = 0, 1
+SCORE_SIGMOID, SCORE_SOFTMAX = 0, 1
