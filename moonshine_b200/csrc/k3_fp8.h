@@ -50,5 +50,7 @@ struct Product {
     float beta, linear_beta;
 };
 bool product(const Product &p, cudaStream_t stream);
+// the kernels behind it: tiles of 128 rows (k3_fp8_wide.cu)
+bool wide_product(const Product &p, cudaStream_t stream);
 
 }  // namespace k3::fp8

@@ -1,0 +1,120 @@
+// What the E4M3 product kernels add to k3_tc_ptx.cuh: the kind::f8f6f4 MMA, packed f32 arithmetic, register
+// shares of warpgroups, tensor maps of code matrices.
+#pragma once
+
+#include "k3_fp8.h"
+#include "k3_tc_ptx.cuh"
+
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
+namespace k3::fp8 {
+
+using namespace k3::tc;
+
+// Instruction descriptor, kind::f8f6f4: D f32 (bits 4..5 = 1), A and B E4M3 (0), both K-major, N >> 3 at bit 17, M >> 4 at 24.
+K3_DEVINL constexpr uint32_t make_idesc_e4m3(uint32_t m, uint32_t n) { return (1u << 4) | ((n >> 3) << 17) | ((m >> 4) << 24); }
+
+// D[tmem] (+)= A[smem] B[smem]^T over 32 E4M3 columns
+K3_DEVINL void mma_e4m3_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// Two f32 in a 64-bit register pair: one instruction for both.
+K3_DEVINL uint64_t pack2(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+K3_DEVINL uint64_t pack2(uint32_t lo, uint32_t hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+    return r;
+}
+K3_DEVINL float lo2(uint64_t v) { return __uint_as_float((uint32_t)v); }
+K3_DEVINL float hi2(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+K3_DEVINL uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+K3_DEVINL uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+K3_DEVINL uint32_t bf16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+template <uint32_t kRegisters>
+K3_DEVINL void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegisters)); }
+template <uint32_t kRegisters>
+K3_DEVINL void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegisters)); }
+
+// A wait that does not stop for the abort flag: for copies in flight, on the way out.
+K3_DEVINL void mbar_drain(uint64_t *bar, uint32_t parity) {
+    const unsigned long long t0 = global_timer_ns();
+    while (!mbar_try_wait(bar, parity) && global_timer_ns() - t0 < 100000000ull) {}
+}
+
+// ------------------------------------------------------------------------------------------- codes
+// scale and codes of a block whose largest magnitude has these bits (without the sign)
+K3_DEVINL float scale_of(uint32_t largest_bits) {
+    if (largest_bits >= 0x7f800000u) return __uint_as_float(0x7fffffffu);
+    return fmaxf(__fdiv_rn(__uint_as_float(largest_bits), 448.0f), 0x1p-126f);
+}
+// x / scale as an f32 division gives it: the product with the rounded reciprocal, corrected once by its
+// remainder (Markstein 1990)
+K3_DEVINL float quotient(float x, float scale, float inverse) {
+    const float r = x * inverse;
+    return copysignf(fmaf(fmaf(-r, scale, x), inverse, r), x);       // the correction would turn -0 into 0
+}
+// two codes, `lo` in the low byte
+K3_DEVINL uint32_t codes2(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// ------------------------------------------------------------------------------------- tensor maps
+inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess) {
+            fn = (PFN_cuTensorMapEncodeTiled_v12000)p;
+        } else {
+            (void)cudaGetLastError();
+        }
+    });
+    return fn;
+}
+
+// Codes [rows, columns] with rows on 16 bytes; boxes of 128 columns x box_rows, 128-byte swizzle.  What lies past the
+// columns reads as zero, whatever the padding holds.
+inline bool map_codes(CUtensorMap *map, const void *codes, uint64_t rows, uint32_t columns, uint32_t box_rows) {
+    auto fn = tensor_map_encoder();
+    if (!fn) return false;
+    const cuuint64_t dims[2] = {columns, rows};
+    const cuuint64_t strides[1] = {pitch_of(columns)};
+    const cuuint32_t box[2] = {kBlock, box_rows};
+    const cuuint32_t steps[2] = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(codes), dims, strides, box, steps,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace k3::fp8

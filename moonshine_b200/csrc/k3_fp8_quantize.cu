@@ -12,9 +12,7 @@
 // The largest magnitude is taken of the bit patterns without their signs, which order like the
 // values and put infinities and NaN above all of them; a block with one gets the scale NaN.
 #include "k3_common.cuh"
-#include "k3_fp8.h"
-
-#include <cuda_fp8.h>
+#include "k3_fp8_ptx.cuh"
 
 using namespace k3;
 using namespace k3::fp8;
@@ -22,23 +20,6 @@ using namespace k3::fp8;
 namespace {
 
 constexpr uint32_t kThreads = 256;
-
-K3_DEVINL float scale_of(uint32_t largest_bits) {
-    if (largest_bits >= 0x7f800000u) return __uint_as_float(0x7fffffffu);
-    return fmaxf(__fdiv_rn(__uint_as_float(largest_bits), 448.0f), 0x1p-126f);
-}
-
-K3_DEVINL float quotient(float x, float scale, float inverse) {
-    const float r = x * inverse;
-    return copysignf(fmaf(fmaf(-r, scale, x), inverse, r), x);       // the correction would turn -0 into 0
-}
-
-// two codes, `lo` in the low byte
-K3_DEVINL uint32_t codes2(float lo, float hi) {
-    uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
-    return r;
-}
 
 K3_DEVINL uint2 codes8(const uint32_t (&bits)[8], float scale, float inverse) {
     uint32_t h[4];

@@ -1,0 +1,519 @@
+// Products of E4M3 matrices with many rows on tcgen05 (kind::f8f6f4).
+//
+//   out[m, n] = sum_kb sa[m, kb] sb[n, kb] sum_{k in kb} a[m, k] b[n, k]
+//
+// The scales are f32, so no MMA kind applies them: the tensor cores sum one block of 128 columns into
+// tensor memory, and warps with the running f32 sums in registers read it, scale it and add it while the
+// tensor cores sum the next block into the other half of tensor memory.  a's rows are the lanes, so a
+// thread's row scale is one register, and 128 of b's rows share a block scale: one packed FMA per two
+// elements and block is all the arithmetic there is.
+//
+// One work item = 128 rows x 256 columns over the whole depth (kOutActivated: 128 columns of gate and
+// the same 128 of up).  384 threads, one block per SM, items in a static order:
+//   warp 0        loads by TMA: a stage is 128 columns of 128 rows of a and 256 rows of b, 48 KB
+//   warp 1        MMA issuer, owns the tensor memory
+//   warp 2        scales of b per row (kColumnScales), put where the adding warps read them
+//   warps 4-11    running sums: lane quadrant warp % 4, columns in two halves
+// The two warpgroups of running sums (128 of them per thread) take registers over from the first one:
+// 2 x 128 x 232 + 128 x 40 are the 384 x 168 of the launch.
+//
+// Every wait is bounded; on give-up the block raises the status word, waits for its copies and frees its
+// tensor memory.
+#include "k3_fp8_ptx.cuh"
+#include "k3_grouped.h"
+#include "k3_moe_layer.h"
+
+#include <algorithm>
+
+using namespace k3;
+using namespace k3::fp8;
+
+namespace {
+
+constexpr uint32_t kThreads = 384;
+constexpr uint32_t BM = 128, BN = 256;
+constexpr uint32_t kATile = BM * kBlock, kBTile = BN * kBlock;       // 16 KB, 32 KB
+constexpr uint32_t kStageBytes = kATile + kBTile;
+constexpr uint32_t kSumWarps = 8;
+constexpr uint32_t kStoreBytes = 32u * 64u;                          // per warp: 32 rows of 64 bytes on their way out
+constexpr uint32_t kMaxGroups = 1024;
+constexpr uint32_t kScaleSlots = 2;                                  // of b's row scales: four blocks each
+
+template <bool kColumnScales>
+struct Layout {
+    static constexpr uint32_t kStages = kColumnScales ? 3u : 4u;     // 8 KB of scales take the fourth stage's place
+    static constexpr uint32_t kScaleBytes = kColumnScales ? kScaleSlots * 4u * BN * 4u : 0u;
+    static constexpr uint32_t kStore = kStages * kStageBytes;
+    static constexpr uint32_t kScales = kStore + kSumWarps * kStoreBytes;
+    static constexpr uint32_t kLargest = kScales + kScaleBytes;      // f32 bits [2][128]: halves' largest activations
+    static constexpr uint32_t kPrefix = kLargest + 2u * BM * 4u;
+    static constexpr uint32_t kBars = (kPrefix + (kMaxGroups + 1u) * 4u + 15u) / 16u * 16u;
+    static constexpr uint32_t kBytes = kBars + 256u + 1024u;         // the last: alignment
+};
+
+__device__ uint32_t g_fp8_wide_status = 0;
+
+struct WideArgs {
+    void *out;
+    float *out_scales;
+    const float *a_scales, *b_scales, *b2_scales;
+    const uint32_t *offsets;
+    uint32_t groups, rows, n, k;
+    uint32_t column_items;
+    int accumulate;
+    int activation;
+    float beta, linear_beta;
+};
+
+struct Item {
+    uint32_t group, row, rows, column;
+};
+
+K3_DEVINL Item item_of(uint32_t w, const uint32_t *prefix, const WideArgs &a, uint32_t columns) {
+    Item it;
+    const uint32_t tile = w / a.column_items;
+    it.column = (w - tile * a.column_items) * columns;
+    if (a.offsets == nullptr) {
+        it.group = 0u;
+        it.row = tile * BM;
+        it.rows = min(BM, a.rows - it.row);
+        return it;
+    }
+    uint32_t lo = 0u, hi = a.groups;                                 // the last group whose first tile is at most `tile`
+    while (hi - lo > 1u) {
+        const uint32_t mid = (lo + hi) / 2u;
+        if (prefix[mid] <= tile) lo = mid; else hi = mid;
+    }
+    it.group = lo;
+    it.row = a.offsets[lo] + (tile - prefix[lo]) * BM;
+    it.rows = min(BM, a.offsets[lo + 1u] - it.row);
+    return it;
+}
+
+template <int kEpilogue, bool kColumnScales>
+__global__ void __launch_bounds__(kThreads, 1)
+fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                const __grid_constant__ CUtensorMap map_b2, WideArgs a) {
+    using L = Layout<kColumnScales>;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char *base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint64_t *full = reinterpret_cast<uint64_t *>(base + L::kBars);  // [kStages]
+    uint64_t *empty = full + L::kStages;                             // [kStages]
+    uint64_t *sum_full = empty + L::kStages;                         // [2] a block's products are in tensor memory
+    uint64_t *sum_empty = sum_full + 2;                              // [2] and have been read
+    uint64_t *scale_full = sum_empty + 2;                            // [kScaleSlots]
+    uint64_t *scale_empty = scale_full + kScaleSlots;                // [kScaleSlots]
+    uint64_t *largest_full = scale_empty + kScaleSlots;              // [1]
+    uint64_t *done = largest_full + 1;                               // [1] every MMA issued has run
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 1);
+    volatile uint32_t *abort_flag = tmem_slot + 1;
+    uint32_t *total_s = tmem_slot + 2;
+    uint32_t *prefix = reinterpret_cast<uint32_t *>(base + L::kPrefix);
+    const uint32_t warp = warp_index(), lane = threadIdx.x % kWarp;
+    const uint32_t blocks = blocks_of(a.k);
+    constexpr uint32_t kColumns = kEpilogue == kOutActivated ? kBlock : BN;
+
+    if (threadIdx.x == 0) {
+        *abort_flag = 0u;
+        for (uint32_t s = 0; s < L::kStages; s++) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (uint32_t s = 0; s < 2u; s++) {
+            mbar_init(&sum_full[s], 1);
+            mbar_init(&sum_empty[s], kSumWarps);
+        }
+        for (uint32_t s = 0; s < kScaleSlots; s++) {
+            mbar_init(&scale_full[s], kWarp);
+            mbar_init(&scale_empty[s], kSumWarps);
+        }
+        mbar_init(largest_full, kSumWarps);
+        mbar_init(done, 1);
+        fence_barrier_init();
+    }
+    if (warp == 1u) {
+        tmem_alloc(tmem_slot, 512u);
+        tmem_relinquish();
+    }
+    pdl_wait();
+    if (a.offsets != nullptr) {
+        // exclusive prefix of the groups' row tiles, one warp, 32 groups at a time
+        if (warp == 2u) {
+            uint32_t before = 0u;
+            for (uint32_t g0 = 0; g0 < a.groups; g0 += kWarp) {
+                const uint32_t g = g0 + lane;
+                const uint32_t n = g < a.groups ? (a.offsets[g + 1u] - a.offsets[g] + BM - 1u) / BM : 0u;
+                uint32_t scan = n;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t up = __shfl_up_sync(0xffffffffu, scan, o);
+                    if (lane >= (uint32_t)o) scan += up;
+                }
+                if (g < a.groups) prefix[g] = before + scan - n;
+                before += __shfl_sync(0xffffffffu, scan, 31);
+            }
+            if (lane == 0u) *total_s = before * a.column_items;
+        }
+    } else if (threadIdx.x == 0) {
+        *total_s = (a.rows + BM - 1u) / BM * a.column_items;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot, total = *total_s;
+
+    if (warp < 4u) {
+        fewer_registers<40>();
+        if (warp == 0u) {
+            // ------------------------------------------------------------------------- loads
+            if (elect_one()) {
+                prefetch_tensormap(&map_a);
+                prefetch_tensormap(&map_b);
+                prefetch_tensormap(&map_b2);
+                uint32_t s = 0u, ph = 0u, issued = 0u;
+                bool ok = true;
+                for (uint32_t w = blockIdx.x; ok && w < total; w += gridDim.x) {
+                    const Item it = item_of(w, prefix, a, kColumns);
+                    const int32_t y = (int32_t)(it.group * a.n + it.column);
+                    for (uint32_t kb = 0; kb < blocks; kb++) {
+                        if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag)) { ok = false; break; }
+                        unsigned char *st = base + s * kStageBytes;
+                        const int32_t x = (int32_t)(kb * kBlock);
+                        mbar_arrive_expect_tx(&full[s], kStageBytes);
+                        tma_load_2d(st, &map_a, &full[s], x, (int32_t)it.row);
+                        tma_load_2d(st + kATile, &map_b, &full[s], x, y);
+                        if (kEpilogue == kOutActivated) tma_load_2d(st + kATile + kBTile / 2u, &map_b2, &full[s], x, y);
+                        else tma_load_2d(st + kATile + kBTile / 2u, &map_b, &full[s], x, y + (int32_t)kBlock);
+                        issued++;
+                        if (++s == L::kStages) { s = 0u; ph ^= 1u; }
+                    }
+                }
+                if (*abort_flag != 0u) {                             // nothing may land in a block that has left
+                    for (uint32_t i = issued > L::kStages ? issued - L::kStages : 0u; i < issued; i++) {
+                        mbar_drain(&full[i % L::kStages], (i / L::kStages) & 1u);
+                    }
+                }
+            }
+        } else if (warp == 1u) {
+            // --------------------------------------------------------------------------- MMA
+            if (elect_one()) {
+                constexpr uint32_t idesc = make_idesc_e4m3(BM, BN);
+                uint32_t s = 0u, ph = 0u, at = 0u, aph = 0u;
+                bool ok = true;
+                for (uint32_t w = blockIdx.x; ok && w < total; w += gridDim.x) {
+                    for (uint32_t kb = 0; kb < blocks; kb++) {
+                        if (!mbar_wait(&sum_empty[at], aph ^ 1u, abort_flag) || !mbar_wait(&full[s], ph, abort_flag)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t addr = smem_u32(base + s * kStageBytes), d = tmem + at * BN;
+                        const uint64_t da = make_desc_sw128(addr), db = make_desc_sw128(addr + kATile);
+#pragma unroll
+                        for (uint32_t j = 0; j < 4u; j++) mma_e4m3_ss(d, da + 2u * j, db + 2u * j, idesc, j != 0u);
+                        mma_commit(&empty[s]);
+                        mma_commit(&sum_full[at]);
+                        if (++s == L::kStages) { s = 0u; ph ^= 1u; }
+                        if (++at == 2u) { at = 0u; aph ^= 1u; }
+                    }
+                }
+                if (*abort_flag != 0u) {
+                    mma_commit(done);
+                    mbar_drain(done, 0u);
+                }
+            }
+        } else if (warp == 2u && kColumnScales) {
+            // ------------------------------------------------------- b's scales, four blocks at a time
+            uint32_t slot = 0u, ph = 0u;
+            bool ok = true;
+            const uint32_t pitch = (blocks + 3u) & ~3u;
+            for (uint32_t w = blockIdx.x; ok && w < total; w += gridDim.x) {
+                const Item it = item_of(w, prefix, a, kColumns);
+                for (uint32_t kb = 0; kb < blocks; kb += 4u) {
+                    float4 v[8];
+#pragma unroll
+                    for (uint32_t j = 0; j < 8u; j++) {
+                        const uint32_t c = min(it.column + j * kWarp + lane, a.n - 1u);
+                        v[j] = *reinterpret_cast<const float4 *>(a.b_scales + (uint64_t)c * pitch + kb);
+                    }
+                    if (!mbar_wait(&scale_empty[slot], ph ^ 1u, abort_flag)) { ok = false; break; }
+                    float *to = reinterpret_cast<float *>(base + L::kScales) + slot * 4u * BN;
+#pragma unroll
+                    for (uint32_t j = 0; j < 8u; j++) {
+                        const uint32_t c = j * kWarp + lane;
+                        to[c] = v[j].x;
+                        to[BN + c] = v[j].y;
+                        to[2u * BN + c] = v[j].z;
+                        to[3u * BN + c] = v[j].w;
+                    }
+                    mbar_arrive(&scale_full[slot]);
+                    if (++slot == kScaleSlots) { slot = 0u; ph ^= 1u; }
+                }
+            }
+        }
+    } else {
+        // ---------------------------------------------------------------------- running sums
+        more_registers<232>();
+        const uint32_t q = warp % 4u, half = (warp - 4u) / 4u;
+        // a thread's 128 sums are columns first, first + 1, .. of the tile, and 64 more from second
+        const uint32_t first = kEpilogue == kOutActivated ? half * 64u : half * 128u;
+        const uint32_t second = kEpilogue == kOutActivated ? first + kBlock : first + 64u;
+        const uint32_t lanes = tmem + ((32u * q) << 16);
+        const uint32_t a_pitch = (blocks + 3u) & ~3u, b_blocks = blocks_of(a.n);
+        uint32_t at = 0u, aph = 0u, slot = 0u, sph = 0u, lph = 0u;
+        bool ok = true;
+        for (uint32_t w = blockIdx.x; ok && w < total; w += gridDim.x) {
+            const Item it = item_of(w, prefix, a, kColumns);
+            const uint32_t row_in = 32u * q + lane;
+            const float *sa_row = a.a_scales + (uint64_t)min(it.row + row_in, a.rows - 1u) * a_pitch;
+            // b's block scales: one row of blocks, or gate's and up's
+            const uint32_t nb = min(it.column / kBlock + (kEpilogue == kOutActivated ? 0u : half), b_blocks - 1u);
+            const uint64_t sb_at = ((uint64_t)it.group * b_blocks + nb) * blocks;
+            const float *sb_row = kColumnScales ? nullptr : a.b_scales + sb_at;
+            const float *sb2_row = kEpilogue == kOutActivated ? a.b2_scales + sb_at : sb_row;
+            uint64_t sum[64];
+#pragma unroll
+            for (int i = 0; i < 64; i++) sum[i] = 0ull;
+            float4 next_a = *reinterpret_cast<const float4 *>(sa_row);
+            float next_b[4], next_b2[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; i++) {
+                next_b[i] = kColumnScales ? 1.f : sb_row[min(i, blocks - 1u)];
+                next_b2[i] = kEpilogue == kOutActivated ? sb2_row[min(i, blocks - 1u)] : next_b[i];
+            }
+            for (uint32_t kb = 0; ok && kb < blocks; kb += 4u) {
+                const float sa[4] = {next_a.x, next_a.y, next_a.z, next_a.w};
+                float s0[4], s1[4];
+#pragma unroll
+                for (uint32_t i = 0; i < 4u; i++) {
+                    s0[i] = sa[i] * next_b[i];
+                    s1[i] = kEpilogue == kOutActivated ? sa[i] * next_b2[i] : s0[i];
+                }
+                if (kb + 4u < blocks) {
+                    next_a = *reinterpret_cast<const float4 *>(sa_row + kb + 4u);
+                    if (!kColumnScales) {
+#pragma unroll
+                        for (uint32_t i = 0; i < 4u; i++) {
+                            next_b[i] = sb_row[min(kb + 4u + i, blocks - 1u)];
+                            if (kEpilogue == kOutActivated) next_b2[i] = sb2_row[min(kb + 4u + i, blocks - 1u)];
+                        }
+                    }
+                }
+                if (kColumnScales && !mbar_wait(&scale_full[slot], sph, abort_flag)) { ok = false; break; }
+                const float *columns = reinterpret_cast<const float *>(base + L::kScales) + slot * 4u * BN;
+#pragma unroll
+                for (uint32_t i = 0; i < 4u; i++) {
+                    if (kb + i >= blocks) break;
+                    if (!mbar_wait(&sum_full[at], aph, abort_flag)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t t = lanes + at * BN;
+#pragma unroll
+                    for (uint32_t c = 0; c < 4u; c++) {
+                        uint32_t r[32];
+                        const uint32_t column = (c < 2u ? first : second) + (c & 1u) * 32u;
+                        tmem_ld_32x32(t + column, r);
+                        tmem_ld_wait();
+                        if (c == 3u) {
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0u) mbar_arrive(&sum_empty[at]);
+                        }
+                        const float sc = c < 2u ? s0[i] : s1[i];
+                        const uint64_t s2 = pack2(sc, sc);
+                        if (kColumnScales) {
+                            const ulonglong2 *by = reinterpret_cast<const ulonglong2 *>(columns + i * BN + column);
+#pragma unroll
+                            for (uint32_t j = 0; j < 8u; j++) {
+                                const ulonglong2 b = by[j];
+                                const uint32_t p = c * 16u + j * 2u;
+                                sum[p] = fma2(mul2(pack2(r[4u * j], r[4u * j + 1u]), s2), b.x, sum[p]);
+                                sum[p + 1u] = fma2(mul2(pack2(r[4u * j + 2u], r[4u * j + 3u]), s2), b.y, sum[p + 1u]);
+                            }
+                        } else {
+#pragma unroll
+                            for (uint32_t j = 0; j < 16u; j++) {
+                                sum[c * 16u + j] = fma2(pack2(r[2u * j], r[2u * j + 1u]), s2, sum[c * 16u + j]);
+                            }
+                        }
+                    }
+                    if (++at == 2u) { at = 0u; aph ^= 1u; }
+                }
+                if (kColumnScales && ok) {
+                    __syncwarp();
+                    if (lane == 0u) mbar_arrive(&scale_empty[slot]);
+                    if (++slot == kScaleSlots) { slot = 0u; sph ^= 1u; }
+                }
+            }
+            if (!ok) break;
+            if (kEpilogue == kOutActivated) {
+                // ------------------------------------------ activation, largest of the row's 128, codes
+                uint32_t most = 0u;
+#pragma unroll
+                for (uint32_t j = 0; j < 32u; j++) {
+                    float v[2];
+#pragma unroll
+                    for (uint32_t p = 0; p < 2u; p++) {
+                        const float g = p ? hi2(sum[j]) : lo2(sum[j]), u = p ? hi2(sum[32u + j]) : lo2(sum[32u + j]);
+                        const bool inside = it.column + first + 2u * j + p < a.n;
+                        v[p] = inside ? activation(g, u, a.activation, a.beta, a.linear_beta) : 0.f;
+                        most = max(most, __float_as_uint(v[p]) & 0x7fffffffu);
+                    }
+                    sum[j] = pack2(v[0], v[1]);
+                }
+                uint32_t *largest = reinterpret_cast<uint32_t *>(base + L::kLargest);
+                largest[half * BM + row_in] = most;
+                __syncwarp();
+                if (lane == 0u) mbar_arrive(largest_full);
+                if (!mbar_wait(largest_full, lph, abort_flag)) { ok = false; break; }
+                lph ^= 1u;
+                most = max(most, largest[(half ^ 1u) * BM + row_in]);
+                __syncwarp();
+                if (lane == 0u) mbar_arrive(largest_full);            // read: the next item may overwrite it
+                if (!mbar_wait(largest_full, lph, abort_flag)) { ok = false; break; }
+                lph ^= 1u;
+                const float scale = scale_of(most), inverse = __frcp_rn(scale);
+                if (row_in < it.rows) {
+                    const uint64_t row = it.row + row_in;
+                    const uint32_t out_pitch = pitch_of(a.n), scale_pitch = scale_pitch_of(a.n);
+                    if (half == 0u) a.out_scales[row * scale_pitch + it.column / kBlock] = scale;
+                    uint8_t *to = (uint8_t *)a.out + row * out_pitch + it.column + first;
+#pragma unroll
+                    for (uint32_t c = 0; c < 4u; c++) {
+                        uint32_t word[4];
+#pragma unroll
+                        for (uint32_t j = 0; j < 4u; j++) {
+                            const uint64_t x = sum[c * 8u + 2u * j], y = sum[c * 8u + 2u * j + 1u];
+                            word[j] = codes2(quotient(lo2(x), scale, inverse), quotient(hi2(x), scale, inverse)) |
+                                      (codes2(quotient(lo2(y), scale, inverse), quotient(hi2(y), scale, inverse)) << 16);
+                        }
+                        if (it.column + first + c * 16u < out_pitch) {
+                            *reinterpret_cast<uint4 *>(to + c * 16u) = make_uint4(word[0], word[1], word[2], word[3]);
+                        }
+                    }
+                }
+            } else {
+                // ---------------------- rows of 64 bytes through shared memory: a warp then stores 8 rows at once
+                constexpr uint32_t kBytesEach = kEpilogue == kOutF32 ? 4u : 2u;
+                constexpr uint32_t kPer = 64u / kBytesEach;            // elements per pass
+                unsigned char *mine = base + L::kStore + (warp - 4u) * kStoreBytes;
+                const bool vector = (a.n * kBytesEach) % 16u == 0u && ((uintptr_t)a.out & 15u) == 0u;
+#pragma unroll
+                for (uint32_t pass = 0; pass < 128u / kPer; pass++) {
+#pragma unroll
+                    for (uint32_t c = 0; c < 4u; c++) {
+                        uint4 v;
+                        if (kEpilogue == kOutF32) {
+                            const uint64_t x = sum[pass * 8u + c * 2u], y = sum[pass * 8u + c * 2u + 1u];
+                            v = make_uint4((uint32_t)x, (uint32_t)(x >> 32), (uint32_t)y, (uint32_t)(y >> 32));
+                        } else {
+                            const uint64_t *p = sum + pass * 16u + c * 4u;
+                            v = make_uint4(bf16x2(lo2(p[0]), hi2(p[0])), bf16x2(lo2(p[1]), hi2(p[1])),
+                                           bf16x2(lo2(p[2]), hi2(p[2])), bf16x2(lo2(p[3]), hi2(p[3])));
+                        }
+                        *reinterpret_cast<uint4 *>(mine + lane * 64u + ((c ^ ((lane >> 1) & 3u)) * 16u)) = v;
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (uint32_t i = 0; i < 4u; i++) {
+                        const uint32_t r = i * 8u + lane / 4u, c = lane % 4u;
+                        const uint4 v = *reinterpret_cast<const uint4 *>(mine + r * 64u + ((c ^ ((r >> 1) & 3u)) * 16u));
+                        const uint32_t column = it.column + first + pass * kPer + c * (16u / kBytesEach);
+                        if (32u * q + r >= it.rows || column >= a.n) continue;
+                        const uint64_t to = (uint64_t)(it.row + 32u * q + r) * a.n + column;
+                        if (kEpilogue == kOutF32) {
+                            float *out = (float *)a.out + to;
+                            const float f[4] = {__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w)};
+                            if (vector) {
+                                float4 o = a.accumulate ? *reinterpret_cast<const float4 *>(out) : make_float4(0.f, 0.f, 0.f, 0.f);
+                                if (a.accumulate) o = make_float4(o.x + f[0], o.y + f[1], o.z + f[2], o.w + f[3]);
+                                else o = make_float4(f[0], f[1], f[2], f[3]);
+                                *reinterpret_cast<float4 *>(out) = o;
+                            } else {
+#pragma unroll
+                                for (uint32_t j = 0; j < 4u; j++) {
+                                    if (column + j < a.n) out[j] = a.accumulate ? out[j] + f[j] : f[j];
+                                }
+                            }
+                        } else {
+                            uint16_t *out = (uint16_t *)a.out + to;
+                            if (vector) {
+                                *reinterpret_cast<uint4 *>(out) = v;
+                            } else {
+                                const uint32_t word[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                                for (uint32_t j = 0; j < 8u; j++) {
+                                    if (column + j < a.n) out[j] = (uint16_t)(word[j / 2u] >> (16u * (j & 1u)));
+                                }
+                            }
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0 && *abort_flag != 0u) atomicExch(&g_fp8_wide_status, 1u);
+    if (warp == 1u) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512u);
+    }
+}
+
+template <int kEpilogue, bool kColumnScales>
+bool launch_wide(const Product &p, cudaStream_t stream) {
+    constexpr uint32_t kColumns = kEpilogue == kOutActivated ? kBlock : BN;
+    CUtensorMap a_map, b_map, b2_map;
+    const uint64_t b_rows = (uint64_t)p.groups * p.n;
+    if (!map_codes(&a_map, p.a, p.rows, p.k, BM) || !map_codes(&b_map, p.b, b_rows, p.k, kBlock) ||
+        !map_codes(&b2_map, kEpilogue == kOutActivated ? p.b2 : p.b, b_rows, p.k, kBlock)) {
+        return false;
+    }
+    WideArgs a{};
+    a.out = p.out;
+    a.out_scales = (float *)p.out_scales;
+    a.a_scales = (const float *)p.a_scales;
+    a.b_scales = (const float *)p.b_scales;
+    a.b2_scales = (const float *)p.b2_scales;
+    a.offsets = p.offsets;
+    a.groups = p.groups;
+    a.rows = p.rows;
+    a.n = p.n;
+    a.k = p.k;
+    a.column_items = (p.n + kColumns - 1u) / kColumns;
+    a.accumulate = p.accumulate;
+    a.activation = p.activation;
+    a.beta = p.beta;
+    a.linear_beta = p.linear_beta;
+    const uint64_t items = ((uint64_t)(p.rows + BM - 1u) / BM + (p.offsets ? p.groups : 0u)) * a.column_items;
+    if (items > 0x7fffffffull) return false;
+    auto kernel = fp8_wide_kernel<kEpilogue, kColumnScales>;
+    constexpr uint32_t kBytes = Layout<kColumnScales>::kBytes;
+    return set_max_dynamic_smem((const void *)kernel, kBytes) &&
+           launch_chained(kernel, (uint32_t)std::min<uint64_t>(items, sm_count()), kThreads, kBytes, stream, a_map, b_map, b2_map, a);
+}
+
+}  // namespace
+
+bool k3::fp8::wide_product(const Product &p, cudaStream_t stream) {
+    if (p.epilogue == kOutActivated) return launch_wide<kOutActivated, false>(p, stream);
+    if (p.b_scale_layout == K3_MOE_FP8_ROWS) {
+        return p.epilogue == kOutF32 ? launch_wide<kOutF32, true>(p, stream) : launch_wide<kOutBf16, true>(p, stream);
+    }
+    return p.epilogue == kOutF32 ? launch_wide<kOutF32, false>(p, stream) : launch_wide<kOutBf16, false>(p, stream);
+}
+
+uint32_t k3_fp8_wide_status() {
+    uint32_t v = 0xffffffffu;
+    if (cudaMemcpyFromSymbol(&v, g_fp8_wide_status, sizeof(v)) != cudaSuccess) (void)cudaGetLastError();
+    return v;
+}
+
+bool k3_fp8_wide_status_clear() {
+    const uint32_t zero = 0u;
+    const bool ok = cudaMemcpyToSymbol(g_fp8_wide_status, &zero, sizeof(zero)) == cudaSuccess;
+    if (!ok) (void)cudaGetLastError();
+    return ok;
+}
