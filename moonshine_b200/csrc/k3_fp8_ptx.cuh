@@ -61,6 +61,15 @@ K3_DEVINL void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 
 template <uint32_t kRegisters>
 K3_DEVINL void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegisters)); }
 
+// tcgen05.wait::ld that the loaded registers depend on: no use of them moves in front of it
+K3_DEVINL void tmem_ld_wait_for(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+                   "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                   "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
+
 // A wait that does not stop for the abort flag: for copies in flight, on the way out.
 K3_DEVINL void mbar_drain(uint64_t *bar, uint32_t parity) {
     const unsigned long long t0 = global_timer_ns();

@@ -12,7 +12,7 @@
 // the same 128 of up).  384 threads, one block per SM, items in a static order:
 //   warp 0        loads by TMA: a stage is 128 columns of 128 rows of a and 256 rows of b, 48 KB
 //   warp 1        MMA issuer, owns the tensor memory
-//   warp 2        scales of b per row (kColumnScales), put where the adding warps read them
+//   warp 2        scales, four blocks ahead: a row's times the block's, where the adding warps read them
 //   warps 4-11    running sums: lane quadrant warp % 4, columns in two halves
 // The two warpgroups of running sums (128 of them per thread) take registers over from the first one:
 // 2 x 128 x 232 + 128 x 40 are the 384 x 168 of the launch.
@@ -37,18 +37,21 @@ constexpr uint32_t kStageBytes = kATile + kBTile;
 constexpr uint32_t kSumWarps = 8;
 constexpr uint32_t kStoreBytes = 32u * 64u;                          // per warp: 32 rows of 64 bytes on their way out
 constexpr uint32_t kMaxGroups = 1024;
-constexpr uint32_t kScaleSlots = 2;                                  // of b's row scales: four blocks each
+constexpr uint32_t kScaleSlots = 2, kSlotBlocks = 4;                 // scales travel four blocks at a time
 
 template <bool kColumnScales>
 struct Layout {
-    static constexpr uint32_t kStages = kColumnScales ? 3u : 4u;     // 8 KB of scales take the fourth stage's place
-    static constexpr uint32_t kScaleBytes = kColumnScales ? kScaleSlots * 4u * BN * 4u : 0u;
+    // a block's scales: of the 128 rows for each half of the columns, or of the rows and of the 256 columns
+    static constexpr uint32_t kBlockScales = kColumnScales ? BM + BN : 2u * BM;
+    static constexpr uint32_t kSlotFloats = kSlotBlocks * kBlockScales;
+    static constexpr uint32_t kStages = kColumnScales ? 3u : 4u;     // the columns' scales take the fourth stage's place
     static constexpr uint32_t kStore = kStages * kStageBytes;
     static constexpr uint32_t kScales = kStore + kSumWarps * kStoreBytes;
-    static constexpr uint32_t kLargest = kScales + kScaleBytes;      // f32 bits [2][128]: halves' largest activations
+    static constexpr uint32_t kLargest = kScales + kScaleSlots * kSlotFloats * 4u;   // f32 bits [2][128]: halves' largest activations
     static constexpr uint32_t kPrefix = kLargest + 2u * BM * 4u;
     static constexpr uint32_t kBars = (kPrefix + (kMaxGroups + 1u) * 4u + 15u) / 16u * 16u;
     static constexpr uint32_t kBytes = kBars + 256u + 1024u;         // the last: alignment
+    static_assert(kBytes <= 232448u, "shared memory of a block");
 };
 
 __device__ uint32_t g_fp8_wide_status = 0;
@@ -222,29 +225,51 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                     mbar_drain(done, 0u);
                 }
             }
-        } else if (warp == 2u && kColumnScales) {
-            // ------------------------------------------------------- b's scales, four blocks at a time
+        } else if (warp == 2u) {
+            // ------------------------------------------------------------- scales, a slot at a time
             uint32_t slot = 0u, ph = 0u;
             bool ok = true;
-            const uint32_t pitch = (blocks + 3u) & ~3u;
+            const uint32_t pitch = (blocks + 3u) & ~3u, b_blocks = blocks_of(a.n);
             for (uint32_t w = blockIdx.x; ok && w < total; w += gridDim.x) {
                 const Item it = item_of(w, prefix, a, kColumns);
-                for (uint32_t kb = 0; kb < blocks; kb += 4u) {
-                    float4 v[8];
-#pragma unroll
-                    for (uint32_t j = 0; j < 8u; j++) {
-                        const uint32_t c = min(it.column + j * kWarp + lane, a.n - 1u);
-                        v[j] = *reinterpret_cast<const float4 *>(a.b_scales + (uint64_t)c * pitch + kb);
-                    }
+                // b's rows of block scales: of the two halves of the columns, or gate's and up's
+                const uint64_t sb = ((uint64_t)it.group * b_blocks + it.column / kBlock) * blocks;
+                const float *b0 = a.b_scales + sb;
+                const float *b1 = kEpilogue == kOutActivated ? a.b2_scales + sb
+                                  : it.column / kBlock + 1u < b_blocks ? b0 + blocks : b0;
+                for (uint32_t kb = 0; kb < blocks; kb += kSlotBlocks) {
                     if (!mbar_wait(&scale_empty[slot], ph ^ 1u, abort_flag)) { ok = false; break; }
-                    float *to = reinterpret_cast<float *>(base + L::kScales) + slot * 4u * BN;
+                    float *to = reinterpret_cast<float *>(base + L::kScales) + slot * L::kSlotFloats;
+                    float f0[4], f1[4];
+                    if (!kColumnScales) {
 #pragma unroll
-                    for (uint32_t j = 0; j < 8u; j++) {
-                        const uint32_t c = j * kWarp + lane;
-                        to[c] = v[j].x;
-                        to[BN + c] = v[j].y;
-                        to[2u * BN + c] = v[j].z;
-                        to[3u * BN + c] = v[j].w;
+                        for (uint32_t i = 0; i < 4u; i++) {
+                            f0[i] = b0[min(kb + i, blocks - 1u)];
+                            f1[i] = b1[min(kb + i, blocks - 1u)];
+                        }
+                    }
+#pragma unroll
+                    for (uint32_t j = 0; j < 4u; j++) {
+                        const uint32_t r = j * kWarp + lane;
+                        const float4 v = *reinterpret_cast<const float4 *>(
+                            a.a_scales + (uint64_t)min(it.row + r, a.rows - 1u) * pitch + kb);
+                        const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (uint32_t i = 0; i < 4u; i++) {
+                            to[i * L::kBlockScales + r] = kColumnScales ? x[i] : x[i] * f0[i];
+                            if (!kColumnScales) to[i * L::kBlockScales + BM + r] = x[i] * f1[i];
+                        }
+                    }
+                    if (kColumnScales) {
+#pragma unroll
+                        for (uint32_t j = 0; j < 8u; j++) {
+                            const uint32_t c = j * kWarp + lane;
+                            const float4 v = *reinterpret_cast<const float4 *>(
+                                a.b_scales + (uint64_t)min(it.column + c, a.n - 1u) * pitch + kb);
+                            const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                            for (uint32_t i = 0; i < 4u; i++) to[i * L::kBlockScales + BM + c] = x[i];
+                        }
                     }
                     mbar_arrive(&scale_full[slot]);
                     if (++slot == kScaleSlots) { slot = 0u; ph ^= 1u; }
@@ -259,86 +284,62 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         const uint32_t first = kEpilogue == kOutActivated ? half * 64u : half * 128u;
         const uint32_t second = kEpilogue == kOutActivated ? first + kBlock : first + 64u;
         const uint32_t lanes = tmem + ((32u * q) << 16);
-        const uint32_t a_pitch = (blocks + 3u) & ~3u, b_blocks = blocks_of(a.n);
+        const uint32_t row_in = 32u * q + lane;
         uint32_t at = 0u, aph = 0u, slot = 0u, sph = 0u, lph = 0u;
         bool ok = true;
         for (uint32_t w = blockIdx.x; ok && w < total; w += gridDim.x) {
             const Item it = item_of(w, prefix, a, kColumns);
-            const uint32_t row_in = 32u * q + lane;
-            const float *sa_row = a.a_scales + (uint64_t)min(it.row + row_in, a.rows - 1u) * a_pitch;
-            // b's block scales: one row of blocks, or gate's and up's
-            const uint32_t nb = min(it.column / kBlock + (kEpilogue == kOutActivated ? 0u : half), b_blocks - 1u);
-            const uint64_t sb_at = ((uint64_t)it.group * b_blocks + nb) * blocks;
-            const float *sb_row = kColumnScales ? nullptr : a.b_scales + sb_at;
-            const float *sb2_row = kEpilogue == kOutActivated ? a.b2_scales + sb_at : sb_row;
             uint64_t sum[64];
 #pragma unroll
             for (int i = 0; i < 64; i++) sum[i] = 0ull;
-            float4 next_a = *reinterpret_cast<const float4 *>(sa_row);
-            float next_b[4], next_b2[4];
-#pragma unroll
-            for (uint32_t i = 0; i < 4u; i++) {
-                next_b[i] = kColumnScales ? 1.f : sb_row[min(i, blocks - 1u)];
-                next_b2[i] = kEpilogue == kOutActivated ? sb2_row[min(i, blocks - 1u)] : next_b[i];
-            }
-            for (uint32_t kb = 0; ok && kb < blocks; kb += 4u) {
-                const float sa[4] = {next_a.x, next_a.y, next_a.z, next_a.w};
-                float s0[4], s1[4];
-#pragma unroll
-                for (uint32_t i = 0; i < 4u; i++) {
-                    s0[i] = sa[i] * next_b[i];
-                    s1[i] = kEpilogue == kOutActivated ? sa[i] * next_b2[i] : s0[i];
+            for (uint32_t kb = 0; kb < blocks; kb++) {
+                if (kb % kSlotBlocks == 0u && !mbar_wait(&scale_full[slot], sph, abort_flag)) { ok = false; break; }
+                const float *scales = reinterpret_cast<const float *>(base + L::kScales) + slot * L::kSlotFloats +
+                                      kb % kSlotBlocks * L::kBlockScales;
+                float s0, s1;
+                if (kColumnScales) {
+                    s0 = s1 = scales[row_in];
+                } else if (kEpilogue == kOutActivated) {
+                    s0 = scales[row_in];
+                    s1 = scales[BM + row_in];
+                } else {
+                    s0 = s1 = scales[half * BM + row_in];
                 }
-                if (kb + 4u < blocks) {
-                    next_a = *reinterpret_cast<const float4 *>(sa_row + kb + 4u);
-                    if (!kColumnScales) {
+                if (!mbar_wait(&sum_full[at], aph, abort_flag)) { ok = false; break; }
+                tc_fence_after();
+                // the next 32 columns are on their way while these are added
+                uint32_t r[2][32];
+                tmem_ld_32x32(lanes + at * BN + first, r[0]);
 #pragma unroll
-                        for (uint32_t i = 0; i < 4u; i++) {
-                            next_b[i] = sb_row[min(kb + 4u + i, blocks - 1u)];
-                            if (kEpilogue == kOutActivated) next_b2[i] = sb2_row[min(kb + 4u + i, blocks - 1u)];
+                for (uint32_t c = 0; c < 4u; c++) {
+                    tmem_ld_wait_for(r[c & 1u]);
+                    if (c < 3u) {
+                        tmem_ld_32x32(lanes + at * BN + (c < 1u ? first : second) + (c == 1u ? 0u : 32u), r[(c + 1u) & 1u]);
+                    } else {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0u) mbar_arrive(&sum_empty[at]);
+                    }
+                    const uint64_t s2 = c < 2u ? pack2(s0, s0) : pack2(s1, s1);
+                    const uint32_t (&v)[32] = r[c & 1u];
+                    if (kColumnScales) {
+                        const ulonglong2 *by = reinterpret_cast<const ulonglong2 *>(scales + BM + (c < 2u ? first : second) + (c & 1u) * 32u);
+#pragma unroll
+                        for (uint32_t j = 0; j < 8u; j++) {
+                            const ulonglong2 b = by[j];
+                            const uint32_t p = c * 16u + j * 2u;
+                            sum[p] = fma2(mul2(pack2(v[4u * j], v[4u * j + 1u]), s2), b.x, sum[p]);
+                            sum[p + 1u] = fma2(mul2(pack2(v[4u * j + 2u], v[4u * j + 3u]), s2), b.y, sum[p + 1u]);
+                        }
+                    } else {
+#pragma unroll
+                        for (uint32_t j = 0; j < 16u; j++) {
+                            sum[c * 16u + j] = fma2(pack2(v[2u * j], v[2u * j + 1u]), s2, sum[c * 16u + j]);
                         }
                     }
                 }
-                if (kColumnScales && !mbar_wait(&scale_full[slot], sph, abort_flag)) { ok = false; break; }
-                const float *columns = reinterpret_cast<const float *>(base + L::kScales) + slot * 4u * BN;
-#pragma unroll
-                for (uint32_t i = 0; i < 4u; i++) {
-                    if (kb + i >= blocks) break;
-                    if (!mbar_wait(&sum_full[at], aph, abort_flag)) { ok = false; break; }
-                    tc_fence_after();
-                    const uint32_t t = lanes + at * BN;
-#pragma unroll
-                    for (uint32_t c = 0; c < 4u; c++) {
-                        uint32_t r[32];
-                        const uint32_t column = (c < 2u ? first : second) + (c & 1u) * 32u;
-                        tmem_ld_32x32(t + column, r);
-                        tmem_ld_wait();
-                        if (c == 3u) {
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0u) mbar_arrive(&sum_empty[at]);
-                        }
-                        const float sc = c < 2u ? s0[i] : s1[i];
-                        const uint64_t s2 = pack2(sc, sc);
-                        if (kColumnScales) {
-                            const ulonglong2 *by = reinterpret_cast<const ulonglong2 *>(columns + i * BN + column);
-#pragma unroll
-                            for (uint32_t j = 0; j < 8u; j++) {
-                                const ulonglong2 b = by[j];
-                                const uint32_t p = c * 16u + j * 2u;
-                                sum[p] = fma2(mul2(pack2(r[4u * j], r[4u * j + 1u]), s2), b.x, sum[p]);
-                                sum[p + 1u] = fma2(mul2(pack2(r[4u * j + 2u], r[4u * j + 3u]), s2), b.y, sum[p + 1u]);
-                            }
-                        } else {
-#pragma unroll
-                            for (uint32_t j = 0; j < 16u; j++) {
-                                sum[c * 16u + j] = fma2(pack2(r[2u * j], r[2u * j + 1u]), s2, sum[c * 16u + j]);
-                            }
-                        }
-                    }
-                    if (++at == 2u) { at = 0u; aph ^= 1u; }
-                }
-                if (kColumnScales && ok) {
+                if (++at == 2u) { at = 0u; aph ^= 1u; }
+                if (kb % kSlotBlocks == kSlotBlocks - 1u || kb + 1u == blocks) {
                     __syncwarp();
                     if (lane == 0u) mbar_arrive(&scale_empty[slot]);
                     if (++slot == kScaleSlots) { slot = 0u; sph ^= 1u; }
