@@ -52,5 +52,8 @@ struct Product {
 bool product(const Product &p, cudaStream_t stream);
 // the kernels behind it: tiles of 128 rows (k3_fp8_wide.cu)
 bool wide_product(const Product &p, cudaStream_t stream);
+// tiles of 16 or 64 rows, b in 128 x 128 blocks only (k3_fp8_few.cu)
+constexpr uint32_t few_rows = 64;
+bool few_product(const Product &p, cudaStream_t stream);
 
 }  // namespace k3::fp8

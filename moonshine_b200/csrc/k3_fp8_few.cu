@@ -1,0 +1,585 @@
+// Products of E4M3 matrices with few rows on tcgen05 (kind::f8f6f4): what has to be read is b, a weight
+// table, and HBM bounds it.
+//
+//   out[m, n] = sum_kb sa[m, kb] sb[n / 128, kb] sum_{k in kb} a[m, k] b[n, k]
+//
+// Here b's rows are the lanes (the MMA's 128) and a's rows its N extent, 16 to 64 columns, so a few rows
+// of a cost no more than their own loads.  128 lanes share a block scale; a row's scale goes with the
+// column, so the factors sa sb of a block lie in shared memory and every lane reads the same one.
+//
+// kSplit (one matrix): a work item is 128 rows of b and a part of the depth; the parts of an item are a
+// cluster, which adds its sums through distributed shared memory in ascending order of the depth.  Two
+// blocks fit an SM, so any number of them up to 296 streams at once.
+// Otherwise (grouped): one block per SM goes over items of 256 rows of b (kOutActivated: 128 of gate and
+// the same 128 of up) over the whole depth.
+//
+// Warps: 0 loads by TMA, 1 MMA issuer and owner of the tensor memory, 2 factors, then four per 32 rows
+// of a with the running sums.  Every wait is bounded; on give-up the block raises the status word,
+// waits for its copies and frees its tensor memory.
+#include "k3_fp8_ptx.cuh"
+#include "k3_grouped.h"
+#include "k3_moe_layer.h"
+
+#include <algorithm>
+
+using namespace k3;
+using namespace k3::fp8;
+
+namespace {
+
+constexpr uint32_t kMaxGroups = 1024;
+constexpr uint32_t kMaxSplits = 8;                                   // of the depth: the portable cluster
+constexpr uint32_t kScaleSlots = 2, kSlotBlocks = 4;
+constexpr uint32_t kBoxRows = 16;                                    // a's rows per box: what an MMA column step is
+
+__device__ uint32_t g_fp8_few_status = 0;
+
+template <uint32_t kTiles, uint32_t kRows, bool kSplit>
+struct Layout {
+    static constexpr uint32_t kHalves = (kRows + 31u) / 32u;
+    static constexpr uint32_t kThreads = (4u + 4u * kHalves) * kWarp;
+    static constexpr uint32_t kBTile = kBlock * kBlock;              // 128 rows of b, 128 columns
+    static constexpr uint32_t kStageBytes = kTiles * kBTile + kRows * kBlock;
+    static constexpr uint32_t kStages = kSplit ? (kRows <= 16u ? 6u : 4u) : 5u;
+    static constexpr uint32_t kFactors = kStages * kStageBytes;      // f32 [slots][4 blocks][tiles][rows]
+    static constexpr uint32_t kSlotFloats = kSlotBlocks * kTiles * kRows;
+    static constexpr uint32_t kLargest = kFactors + kScaleSlots * kSlotFloats * 4u;   // f32 bits [4][kRows]
+    static constexpr uint32_t kPrefix = kLargest + 4u * kRows * 4u;
+    static constexpr uint32_t kBars = (kPrefix + (kSplit ? 0u : (kMaxGroups + 1u) * 4u) + 15u) / 16u * 16u;
+    static constexpr uint32_t kBytes = kBars + 256u + 1024u;         // the last: alignment
+    static constexpr uint32_t kTmem = kTiles * kRows * 2u < 32u ? 32u : kTiles * kRows * 2u;
+    static_assert(kBytes <= (kSplit ? 115000u : 232448u), "two blocks of a split product share an SM");
+    static_assert(!kSplit || kRows * kBlock * 4u <= kFactors, "partial sums take the ring's place");
+};
+
+struct FewArgs {
+    void *out;
+    float *out_scales;
+    const float *a_scales, *b_scales, *b2_scales;
+    const uint32_t *offsets;
+    uint32_t groups, rows, n, k;
+    uint32_t column_items;                         // grouped: items along b's rows
+    uint32_t split_blocks;                         // kSplit: blocks of 128 per part of the depth
+    int accumulate;
+    int activation;
+    float beta, linear_beta;
+};
+
+struct Item {
+    uint32_t group, row, rows, column, kb_begin, kb_end;
+};
+
+K3_DEVINL uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+K3_DEVINL uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+K3_DEVINL void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// f32 at the same place of another block's shared memory
+K3_DEVINL float cluster_load(const float *mine, uint32_t rank) {
+    uint32_t addr;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(mine)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+K3_DEVINL void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+K3_DEVINL void tmem_ld_wait_for(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+}
+
+template <int kEpilogue, uint32_t kTiles, uint32_t kRows, bool kSplit>
+__global__ void __launch_bounds__(Layout<kTiles, kRows, kSplit>::kThreads, kSplit ? 2 : 1)
+fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+               const __grid_constant__ CUtensorMap map_b2, FewArgs a) {
+    using L = Layout<kTiles, kRows, kSplit>;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char *base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint64_t *full = reinterpret_cast<uint64_t *>(base + L::kBars);  // [kStages]
+    uint64_t *empty = full + L::kStages;                             // [kStages]
+    uint64_t *sum_full = empty + L::kStages;                         // [2] a block's products are in tensor memory
+    uint64_t *sum_empty = sum_full + 2;                              // [2] and have been read
+    uint64_t *factor_full = sum_empty + 2;                           // [kScaleSlots]
+    uint64_t *factor_empty = factor_full + kScaleSlots;              // [kScaleSlots]
+    uint64_t *largest_full = factor_empty + kScaleSlots;             // [2] one per half
+    uint64_t *done = largest_full + 2;                               // [1] every MMA issued has run
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 1);
+    volatile uint32_t *abort_flag = tmem_slot + 1;
+    uint32_t *total_s = tmem_slot + 2;
+    uint32_t *prefix = reinterpret_cast<uint32_t *>(base + L::kPrefix);
+    const uint32_t warp = warp_index(), lane = threadIdx.x % kWarp;
+    const uint32_t blocks = blocks_of(a.k);
+    constexpr uint32_t kColumns = kEpilogue == kOutActivated ? kBlock : kTiles * kBlock;
+
+    if (threadIdx.x == 0) {
+        *abort_flag = 0u;
+        for (uint32_t s = 0; s < L::kStages; s++) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (uint32_t s = 0; s < 2u; s++) {
+            mbar_init(&sum_full[s], 1);
+            mbar_init(&sum_empty[s], 4u * L::kHalves);
+            mbar_init(&largest_full[s], 4);
+        }
+        for (uint32_t s = 0; s < kScaleSlots; s++) {
+            mbar_init(&factor_full[s], kWarp);
+            mbar_init(&factor_empty[s], 4u * L::kHalves);
+        }
+        mbar_init(done, 1);
+        fence_barrier_init();
+    }
+    if (warp == 1u) {
+        tmem_alloc(tmem_slot, L::kTmem);
+        tmem_relinquish();
+    }
+    pdl_wait();
+    if (!kSplit && warp == 2u) {
+        // exclusive prefix of the groups' row tiles, 32 groups at a time
+        uint32_t before = 0u;
+        for (uint32_t g0 = 0; g0 < a.groups; g0 += kWarp) {
+            const uint32_t g = g0 + lane;
+            const uint32_t n = g < a.groups ? (a.offsets[g + 1u] - a.offsets[g] + kRows - 1u) / kRows : 0u;
+            uint32_t scan = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t up = __shfl_up_sync(0xffffffffu, scan, o);
+                if (lane >= (uint32_t)o) scan += up;
+            }
+            if (g < a.groups) prefix[g] = before + scan - n;
+            before += __shfl_sync(0xffffffffu, scan, 31);
+        }
+        if (lane == 0u) *total_s = before * a.column_items;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t first_item = kSplit ? 0u : blockIdx.x, step = kSplit ? 1u : gridDim.x, total = kSplit ? 1u : *total_s;
+
+    auto item_of = [&](uint32_t w) {
+        Item it;
+        it.kb_begin = 0u;
+        it.kb_end = blocks;
+        if (kSplit) {
+            it.group = 0u;
+            it.row = blockIdx.z * kRows;
+            it.rows = min(kRows, a.rows - it.row);
+            it.column = blockIdx.y * kBlock;
+            it.kb_begin = blockIdx.x * a.split_blocks;
+            it.kb_end = min(blocks, it.kb_begin + a.split_blocks);
+            return it;
+        }
+        const uint32_t tile = w / a.column_items;
+        it.column = (w - tile * a.column_items) * kColumns;
+        uint32_t lo = 0u, hi = a.groups;                             // the last group whose first tile is at most `tile`
+        while (hi - lo > 1u) {
+            const uint32_t mid = (lo + hi) / 2u;
+            if (prefix[mid] <= tile) lo = mid; else hi = mid;
+        }
+        it.group = lo;
+        it.row = a.offsets[lo] + (tile - prefix[lo]) * kRows;
+        it.rows = min(kRows, a.offsets[lo + 1u] - it.row);
+        return it;
+    };
+
+    if (warp == 0u) {
+        // ----------------------------------------------------------------------------- loads
+        if (elect_one()) {
+            prefetch_tensormap(&map_a);
+            prefetch_tensormap(&map_b);
+            if (kEpilogue == kOutActivated) prefetch_tensormap(&map_b2);
+            const uint64_t stream_once = l2_policy_evict_first();
+            uint32_t s = 0u, ph = 0u, issued = 0u;
+            bool ok = true;
+            for (uint32_t w = first_item; ok && w < total; w += step) {
+                const Item it = item_of(w);
+                const int32_t y = (int32_t)(it.group * a.n + it.column);
+                const uint32_t boxes = (it.rows + kBoxRows - 1u) / kBoxRows;
+                for (uint32_t kb = it.kb_begin; kb < it.kb_end; kb++) {
+                    if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag)) { ok = false; break; }
+                    unsigned char *st = base + s * L::kStageBytes;
+                    const int32_t x = (int32_t)(kb * kBlock);
+                    mbar_arrive_expect_tx(&full[s], kTiles * L::kBTile + boxes * kBoxRows * kBlock);
+                    tma_load_2d_hint(st, &map_b, &full[s], x, y, stream_once);
+                    if (kTiles == 2u) {
+                        if (kEpilogue == kOutActivated) tma_load_2d_hint(st + L::kBTile, &map_b2, &full[s], x, y, stream_once);
+                        else tma_load_2d_hint(st + L::kBTile, &map_b, &full[s], x, y + (int32_t)kBlock, stream_once);
+                    }
+                    for (uint32_t i = 0; i < boxes; i++) {
+                        tma_load_2d(st + kTiles * L::kBTile + i * kBoxRows * kBlock, &map_a, &full[s], x,
+                                    (int32_t)(it.row + i * kBoxRows));
+                    }
+                    issued++;
+                    if (++s == L::kStages) { s = 0u; ph ^= 1u; }
+                }
+            }
+            if (*abort_flag != 0u) {                                 // nothing may land in a block that has left
+                for (uint32_t i = issued > L::kStages ? issued - L::kStages : 0u; i < issued; i++) {
+                    mbar_drain(&full[i % L::kStages], (i / L::kStages) & 1u);
+                }
+            }
+        }
+    } else if (warp == 1u) {
+        // ------------------------------------------------------------------------------- MMA
+        if (elect_one()) {
+            uint32_t s = 0u, ph = 0u, at = 0u, aph = 0u;
+            bool ok = true;
+            for (uint32_t w = first_item; ok && w < total; w += step) {
+                const Item it = item_of(w);
+                const uint32_t idesc = make_idesc_e4m3(kBlock, (it.rows + 15u) & ~15u);
+                for (uint32_t kb = it.kb_begin; kb < it.kb_end; kb++) {
+                    if (!mbar_wait(&sum_empty[at], aph ^ 1u, abort_flag) || !mbar_wait(&full[s], ph, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t addr = smem_u32(base + s * L::kStageBytes), d = tmem + at * (kTiles * kRows);
+                    const uint64_t rows = make_desc_sw128(addr + kTiles * L::kBTile);
+#pragma unroll
+                    for (uint32_t t = 0; t < kTiles; t++) {
+                        const uint64_t lanes = make_desc_sw128(addr + t * L::kBTile);
+#pragma unroll
+                        for (uint32_t j = 0; j < 4u; j++) {
+                            mma_e4m3_ss(d + t * kRows, lanes + 2u * j, rows + 2u * j, idesc, j != 0u);
+                        }
+                    }
+                    mma_commit(&empty[s]);
+                    mma_commit(&sum_full[at]);
+                    if (++s == L::kStages) { s = 0u; ph ^= 1u; }
+                    if (++at == 2u) { at = 0u; aph ^= 1u; }
+                }
+            }
+            if (*abort_flag != 0u) {
+                mma_commit(done);
+                mbar_drain(done, 0u);
+            }
+        }
+    } else if (warp == 2u) {
+        // --------------------------------------------------------------- factors, a slot at a time
+        uint32_t slot = 0u, ph = 0u;
+        bool ok = true;
+        const uint32_t pitch = (blocks + 3u) & ~3u, b_blocks = blocks_of(a.n);
+        for (uint32_t w = first_item; ok && w < total; w += step) {
+            const Item it = item_of(w);
+            const uint64_t sb = ((uint64_t)it.group * b_blocks + it.column / kBlock) * blocks;
+            const float *b_row[2] = {a.b_scales + sb, nullptr};
+            if (kTiles == 2u) {
+                b_row[1] = kEpilogue == kOutActivated ? a.b2_scales + sb
+                           : it.column / kBlock + 1u < b_blocks ? b_row[0] + blocks : b_row[0];
+            }
+            for (uint32_t kb = it.kb_begin; kb < it.kb_end; kb += kSlotBlocks) {
+                float f[kTiles][4];
+#pragma unroll
+                for (uint32_t t = 0; t < kTiles; t++) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 4u; i++) f[t][i] = b_row[t][min(kb + i, blocks - 1u)];
+                }
+                float x[(kRows + 31u) / 32u][4];
+#pragma unroll
+                for (uint32_t j = 0; j < (kRows + 31u) / 32u; j++) {
+                    // rows past the tile's take the last row's scales: their columns are not kept
+                    const float *row = a.a_scales + (uint64_t)(it.row + min(j * kWarp + lane, it.rows - 1u)) * pitch;
+#pragma unroll
+                    for (uint32_t i = 0; i < 4u; i++) x[j][i] = row[min(kb + i, blocks - 1u)];
+                }
+                if (!mbar_wait(&factor_empty[slot], ph ^ 1u, abort_flag)) { ok = false; break; }
+                float *to = reinterpret_cast<float *>(base + L::kFactors) + slot * L::kSlotFloats;
+#pragma unroll
+                for (uint32_t j = 0; j < (kRows + 31u) / 32u; j++) {
+                    if (j * kWarp + lane >= kRows) continue;
+#pragma unroll
+                    for (uint32_t i = 0; i < 4u; i++) {
+#pragma unroll
+                        for (uint32_t t = 0; t < kTiles; t++) to[(i * kTiles + t) * kRows + j * kWarp + lane] = x[j][i] * f[t][i];
+                    }
+                }
+                mbar_arrive(&factor_full[slot]);
+                if (++slot == kScaleSlots) { slot = 0u; ph ^= 1u; }
+            }
+        }
+    } else if (warp >= 4u) {
+        // --------------------------------------------------------------------------- running sums
+        constexpr uint32_t kMine = kRows < 32u ? kRows : 32u;         // rows of a per warp
+        const uint32_t q = warp % 4u, half = (warp - 4u) / 4u;
+        const uint32_t lanes = tmem + ((32u * q) << 16) + half * kMine;
+        uint32_t at = 0u, aph = 0u, slot = 0u, sph = 0u, lph = 0u;
+        bool ok = true;
+        for (uint32_t w = first_item; ok && w < total; w += step) {
+            const Item it = item_of(w);
+            const uint32_t n = it.rows > half * kMine ? min(kMine, it.rows - half * kMine) : 0u;
+            uint64_t sum[kTiles][kMine / 2u];
+#pragma unroll
+            for (uint32_t t = 0; t < kTiles; t++) {
+#pragma unroll
+                for (uint32_t j = 0; j < kMine / 2u; j++) sum[t][j] = 0ull;
+            }
+            for (uint32_t kb = it.kb_begin; kb < it.kb_end; kb++) {
+                const uint32_t in_slot = (kb - it.kb_begin) % kSlotBlocks;
+                if ((in_slot == 0u && !mbar_wait(&factor_full[slot], sph, abort_flag)) || !mbar_wait(&sum_full[at], aph, abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const float *factors = reinterpret_cast<const float *>(base + L::kFactors) + slot * L::kSlotFloats +
+                                       in_slot * kTiles * kRows + half * kMine;
+                constexpr uint32_t kChunks = kMine / 16u;
+                uint32_t r[kTiles][kChunks][16];
+#pragma unroll
+                for (uint32_t c = 0; c < kChunks; c++) {
+                    if (c * 16u < n) {
+#pragma unroll
+                        for (uint32_t t = 0; t < kTiles; t++) tmem_ld_32x16(lanes + at * (kTiles * kRows) + t * kRows + c * 16u, r[t][c]);
+                    }
+                }
+#pragma unroll
+                for (uint32_t c = 0; c < kChunks; c++) {
+#pragma unroll
+                    for (uint32_t t = 0; t < kTiles; t++) tmem_ld_wait_for(r[t][c]);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0u) mbar_arrive(&sum_empty[at]);
+#pragma unroll
+                for (uint32_t c = 0; c < kChunks; c++) {
+                    if (c * 16u < n) {
+#pragma unroll
+                        for (uint32_t t = 0; t < kTiles; t++) {
+                            const ulonglong2 *f = reinterpret_cast<const ulonglong2 *>(factors + t * kRows + c * 16u);
+#pragma unroll
+                            for (uint32_t j = 0; j < 4u; j++) {
+                                const ulonglong2 v = f[j];
+                                uint64_t *to = &sum[t][c * 8u + j * 2u];
+                                to[0] = fma2(pack2(r[t][c][4u * j], r[t][c][4u * j + 1u]), v.x, to[0]);
+                                to[1] = fma2(pack2(r[t][c][4u * j + 2u], r[t][c][4u * j + 3u]), v.y, to[1]);
+                            }
+                        }
+                    }
+                }
+                if (++at == 2u) { at = 0u; aph ^= 1u; }
+                if (in_slot == kSlotBlocks - 1u || kb + 1u == it.kb_end) {
+                    __syncwarp();
+                    if (lane == 0u) mbar_arrive(&factor_empty[slot]);
+                    if (++slot == kScaleSlots) { slot = 0u; sph ^= 1u; }
+                }
+            }
+            if (!ok) break;
+            const uint32_t column = 32u * q + lane;                  // of the tile
+            auto value = [&](uint32_t t, uint32_t j) { return j & 1u ? hi2(sum[t][j / 2u]) : lo2(sum[t][j / 2u]); };
+            if (kSplit) {
+                float *part = reinterpret_cast<float *>(base);       // [kRows][128]; every stage has been read
+#pragma unroll
+                for (uint32_t j = 0; j < kMine; j++) {
+                    if (j < n) part[(half * kMine + j) * kBlock + column] = value(0u, j);
+                }
+            } else if (kEpilogue == kOutActivated) {
+                // ---------------------------------- activation, largest of a row's 128 columns, codes
+                const bool inside = it.column + column < a.n;
+                uint32_t *largest = reinterpret_cast<uint32_t *>(base + L::kLargest) + half * kMine;   // [4][kRows]
+                float act[kMine];
+#pragma unroll
+                for (uint32_t j = 0; j < kMine; j++) {
+                    act[j] = 0.f;
+                    if (j < n) {
+                        if (inside) act[j] = activation(value(0u, j), value(kTiles - 1u, j), a.activation, a.beta, a.linear_beta);
+                        const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(act[j]) & 0x7fffffffu);
+                        if (lane == 0u) largest[q * kRows + j] = most;
+                    }
+                }
+                __syncwarp();
+                if (lane == 0u) mbar_arrive(&largest_full[half]);
+                if (!mbar_wait(&largest_full[half], lph, abort_flag)) { ok = false; break; }
+                lph ^= 1u;
+                const uint32_t out_pitch = pitch_of(a.n), scale_pitch = scale_pitch_of(a.n);
+#pragma unroll
+                for (uint32_t j = 0; j < kMine; j++) {
+                    if (j < n) {
+                        const uint32_t most = max(max(largest[j], largest[kRows + j]), max(largest[2u * kRows + j], largest[3u * kRows + j]));
+                        const float scale = scale_of(most);
+                        const uint64_t row = it.row + half * kMine + j;
+                        if (q == 0u && lane == 0u) a.out_scales[row * scale_pitch + it.column / kBlock] = scale;
+                        if (it.column + column < out_pitch) {
+                            ((uint8_t *)a.out)[row * out_pitch + it.column + column] =
+                                (uint8_t)codes2(quotient(act[j], scale, __frcp_rn(scale)), 0.f);
+                        }
+                    }
+                }
+                __syncwarp();
+                if (lane == 0u) mbar_arrive(&largest_full[half]);     // read: the next item may overwrite it
+                if (!mbar_wait(&largest_full[half], lph, abort_flag)) { ok = false; break; }
+                lph ^= 1u;
+            } else {
+#pragma unroll
+                for (uint32_t t = 0; t < kTiles; t++) {
+                    const uint32_t c = it.column + t * kBlock + column;
+                    if (c < a.n) {
+#pragma unroll
+                        for (uint32_t j = 0; j < kMine; j++) {
+                            if (j < n) {
+                                const uint64_t to = (uint64_t)(it.row + half * kMine + j) * a.n + c;
+                                if (kEpilogue == kOutF32) ((float *)a.out)[to] = value(t, j);
+                                else ((uint16_t *)a.out)[to] = float_to_bf16_bits(value(t, j));
+                            }
+                        }
+                    }
+                }
+            }
+        }
+    }
+
+    if (kSplit) {
+        // the parts' sums, in ascending order of the depth; each block adds its share of the item
+        __syncthreads();
+        cluster_barrier();
+        const Item it = item_of(0u);
+        const uint32_t size = cluster_size(), all = it.rows * kBlock;
+        const uint32_t share = (all + size - 1u) / size, begin = cluster_rank() * share, end = min(all, begin + share);
+        const float *part = reinterpret_cast<const float *>(base);
+        for (uint32_t e = begin + threadIdx.x; e < end; e += L::kThreads) {
+            float v[kMaxSplits];
+#pragma unroll
+            for (uint32_t r = 0; r < kMaxSplits; r++) v[r] = r < size ? cluster_load(part + e, r) : 0.f;
+            float sum = v[0];
+#pragma unroll
+            for (uint32_t r = 1; r < kMaxSplits; r++) {
+                if (r < size) sum += v[r];
+            }
+            const uint32_t c = it.column + e % kBlock;
+            if (c < a.n) {
+                const uint64_t to = (uint64_t)(it.row + e / kBlock) * a.n + c;
+                if (kEpilogue == kOutF32) {
+                    float *out = (float *)a.out + to;
+                    *out = a.accumulate ? *out + sum : sum;
+                } else {
+                    ((uint16_t *)a.out)[to] = float_to_bf16_bits(sum);
+                }
+            }
+        }
+        cluster_barrier();                                           // nobody leaves while its sums are read
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0 && *abort_flag != 0u) atomicExch(&g_fp8_few_status, 1u);
+    if (warp == 1u) {
+        tc_fence_after();
+        tmem_dealloc(tmem, L::kTmem);
+    }
+}
+
+FewArgs args_of(const Product &p) {
+    FewArgs a{};
+    a.out = p.out;
+    a.out_scales = (float *)p.out_scales;
+    a.a_scales = (const float *)p.a_scales;
+    a.b_scales = (const float *)p.b_scales;
+    a.b2_scales = (const float *)p.b2_scales;
+    a.offsets = p.offsets;
+    a.groups = p.groups;
+    a.rows = p.rows;
+    a.n = p.n;
+    a.k = p.k;
+    a.accumulate = p.accumulate;
+    a.activation = p.activation;
+    a.beta = p.beta;
+    a.linear_beta = p.linear_beta;
+    return a;
+}
+
+template <int kEpilogue, uint32_t kRows>
+bool launch_split(const Product &p, cudaStream_t stream) {
+    using L = Layout<1, kRows, true>;
+    CUtensorMap a_map, b_map;
+    if (!map_codes(&a_map, p.a, p.rows, p.k, kBoxRows) || !map_codes(&b_map, p.b, p.n, p.k, kBlock)) return false;
+    FewArgs a = args_of(p);
+    const uint32_t tiles = blocks_of(p.n), row_tiles = (p.rows + kRows - 1u) / kRows, blocks = blocks_of(p.k);
+    if (tiles > 65535u || row_tiles > 65535u) return false;
+    // as many parts as the SMs hold at two blocks each, with two blocks of 128 in a part at least
+    const uint32_t room = (uint32_t)sm_count() * 2u / std::max(1u, tiles * row_tiles);
+    const uint32_t splits = std::max(1u, std::min({kMaxSplits, room, blocks / 2u}));
+    a.split_blocks = (blocks + splits - 1u) / splits;
+    const uint32_t parts = (blocks + a.split_blocks - 1u) / a.split_blocks;
+    auto kernel = fp8_few_kernel<kEpilogue, 1, kRows, true>;
+    if (!set_max_dynamic_smem((const void *)kernel, L::kBytes)) return false;
+    cudaLaunchAttribute attributes[2]{};
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = parts;
+    attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(parts, tiles, row_tiles);
+    config.blockDim = L::kThreads;
+    config.dynamicSmemBytes = L::kBytes;
+    config.stream = stream;
+    config.attrs = attributes;
+    config.numAttrs = 2;
+    if (cudaLaunchKernelEx(&config, kernel, a_map, b_map, b_map, a) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return false;
+    }
+    return true;
+}
+
+template <int kEpilogue>
+bool launch_grouped(const Product &p, cudaStream_t stream) {
+    constexpr uint32_t kRows = few_rows, kColumns = kEpilogue == kOutActivated ? kBlock : 2u * kBlock;
+    using L = Layout<2, kRows, false>;
+    CUtensorMap a_map, b_map, b2_map;
+    const uint64_t b_rows = (uint64_t)p.groups * p.n;
+    if (!map_codes(&a_map, p.a, p.rows, p.k, kBoxRows) || !map_codes(&b_map, p.b, b_rows, p.k, kBlock) ||
+        !map_codes(&b2_map, kEpilogue == kOutActivated ? p.b2 : p.b, b_rows, p.k, kBlock)) {
+        return false;
+    }
+    FewArgs a = args_of(p);
+    a.column_items = (p.n + kColumns - 1u) / kColumns;
+    const uint64_t items = ((uint64_t)(p.rows + kRows - 1u) / kRows + p.groups) * a.column_items;
+    if (items > 0x7fffffffull) return false;
+    auto kernel = fp8_few_kernel<kEpilogue, 2, kRows, false>;
+    return set_max_dynamic_smem((const void *)kernel, L::kBytes) &&
+           launch_chained(kernel, (uint32_t)std::min<uint64_t>(items, sm_count()), L::kThreads, L::kBytes, stream, a_map, b_map,
+                          b2_map, a);
+}
+
+}  // namespace
+
+bool k3::fp8::few_product(const Product &p, cudaStream_t stream) {
+    if (p.offsets) {
+        return p.epilogue == kOutActivated ? launch_grouped<kOutActivated>(p, stream)
+               : p.epilogue == kOutF32     ? launch_grouped<kOutF32>(p, stream)
+                                           : launch_grouped<kOutBf16>(p, stream);
+    }
+    if (p.rows <= 16u) return p.epilogue == kOutF32 ? launch_split<kOutF32, 16>(p, stream) : launch_split<kOutBf16, 16>(p, stream);
+    return p.epilogue == kOutF32 ? launch_split<kOutF32, few_rows>(p, stream) : launch_split<kOutBf16, few_rows>(p, stream);
+}
+
+uint32_t k3_fp8_few_status() {
+    uint32_t v = 0xffffffffu;
+    if (cudaMemcpyFromSymbol(&v, g_fp8_few_status, sizeof(v)) != cudaSuccess) (void)cudaGetLastError();
+    return v;
+}
+
+bool k3_fp8_few_status_clear() {
+    const uint32_t zero = 0u;
+    const bool ok = cudaMemcpyToSymbol(g_fp8_few_status, &zero, sizeof(zero)) == cudaSuccess;
+    if (!ok) (void)cudaGetLastError();
+    return ok;
+}

@@ -3,7 +3,11 @@
 
 using namespace k3::fp8;
 
-bool k3::fp8::product(const Product &p, cudaStream_t stream) { return wide_product(p, stream); }
+bool k3::fp8::product(const Product &p, cudaStream_t stream) {
+    const bool few = p.offsets ? p.rows <= few_rows * p.groups : p.rows <= few_rows;
+    if (few && p.b_scale_layout == K3_MOE_FP8_BLOCKS) return few_product(p, stream);
+    return wide_product(p, stream);
+}
 
 extern "C" bool k3_moe_fp8_product(void *out, const void *a, const void *a_scales, const void *b, const void *b_scales,
                                    uint32_t m, uint32_t n, uint32_t k, int b_scale_layout, int out_type, int accumulate,

@@ -135,6 +135,8 @@ uint32_t k3_balance_status();      // 2: a balance or router gradient call saw a
 bool k3_balance_status_clear();
 uint32_t k3_fp8_wide_status();
 bool k3_fp8_wide_status_clear();
+uint32_t k3_fp8_few_status();
+bool k3_fp8_few_status_clear();
 bool k3_grouped_mx_status_clear();
 bool k3_status_words_clear();   // all of the above and the dense kernels' word   // 2: a dispatch saw an expert id >= experts
 
