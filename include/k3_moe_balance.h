@@ -32,7 +32,8 @@ extern "C" {
  * the last offset belong to none) -> counts u32 [sequences, experts], loss f32
  * [sequences], means f32 [sequences, experts] (P).  logits, loss and means may
  * be NULL together: counts alone.  An id >= experts is not counted and raises
- * bit 1 of k3_moe_device_status().  experts <= 1024, top_k <= 32.  Sums run in
+ * bit 1 of k3_moe_device_status().  experts <= 1024, top_k <= 32,
+ * sequences <= 65535.  The workspace of more tokens serves fewer.  Sums run in
  * an order that only tokens and experts decide: the same call gives the same
  * bits. */
 size_t k3_moe_balance_workspace_bytes(uint32_t tokens, uint32_t sequences, uint32_t experts);

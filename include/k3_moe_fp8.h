@@ -68,7 +68,8 @@ bool k3_moe_fp8_product(void *out, const void *a, const void *a_scales, const vo
 
 /* out bf16 [tokens, rows] = x bf16 [tokens, columns] W^T with W [rows, columns]
  * in blocks: quantises x by rows into the workspace and multiplies.  The
- * gradient by the input is this call on dY and the transposed table. */
+ * gradient by the input is this call on dY and the transposed table.  (Here and
+ * below the workspace of more tokens serves fewer.) */
 size_t k3_moe_fp8_linear_workspace_bytes(uint32_t tokens, uint32_t columns);
 bool k3_moe_fp8_linear(void *out, const void *x, const void *w, const void *w_scales,
                        uint32_t tokens, uint32_t rows, uint32_t columns, void *workspace,

@@ -29,7 +29,7 @@ class RouterBalance:
             raise ValueError("score: 'sigmoid' or 'softmax'")
         self.experts, self.top_k, self.score = experts, top_k, _SCORES[score]
         self.coefficient, self.route_scale = float(coefficient), float(route_scale)
-        self._workspace = _Workspace()
+        self._workspace = _Workspace(lambda tokens, sequences: ops.k3_moe_balance_workspace_bytes(tokens, sequences, experts))
 
     def _sequences(self, ids, offsets):
         tokens = ids.shape[0]
@@ -53,9 +53,9 @@ class RouterBalance:
             loss = make(sequences, dtype=torch.float32, device=ids.device)
             means = make((sequences, self.experts), dtype=torch.float32, device=ids.device)
         if tokens:
-            ws = self._workspace.of(ops.k3_moe_balance_workspace_bytes(tokens, sequences, self.experts), ids.device)
+            ws = self._workspace.of(tokens, sequences, ids.device)
             _done(ops.k3_moe_balance(counts, loss, means, logits, ids, offsets, tokens, sequences, self.experts, self.top_k,
-                                     self.score, self.coefficient, ws, ws.numel()), "k3_moe_balance")
+                                     self.score, self.coefficient, ws, self._workspace.bytes), "k3_moe_balance")
         return counts if logits is None else (counts, loss, means)
 
     def backward(self, logits: torch.Tensor, ids: torch.Tensor, counts: torch.Tensor | None = None,

@@ -32,6 +32,15 @@ struct Shape {
     int softmax;
 };
 
+// The fast exponential and quotient (2 units in the last place each, of an argument's size the exponent's): 4e-7 of
+// a score.  With expf and the rounded quotient the pass over the logits was bound by its instructions,
+// 32768 x 896 forward and backward 198 us.
+K3_DEVINL float sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
+
+struct Softmax {
+    float top, over;                               // a score is exp(logit - top) * over
+};
+
 // A warp's row: kV groups of four experts per lane, neighbours (kVector) or 32 apart.
 template <uint32_t kV, bool kVector>
 struct Row {
@@ -39,30 +48,48 @@ struct Row {
     static K3_DEVINL uint32_t expert(uint32_t i, uint32_t lane) {
         return kVector ? (i / 4u) * 128u + lane * 4u + i % 4u : i * 32u + lane;
     }
+    // elements i .. i + 3 (i a multiple of 4) of a row in memory, and back
+    template <typename T>
+    static K3_DEVINL void get4(float (&to)[4], const T *row, uint32_t experts, uint32_t lane, uint32_t i, float fill) {
+        if (kVector) {
+            const uint32_t e = expert(i, lane);
+            uint4 q = make_uint4(0u, 0u, 0u, 0u);
+            if (e < experts) q = *reinterpret_cast<const uint4 *>(row + e);
+            to[0] = e < experts ? value(q.x, row) : fill;
+            to[1] = e < experts ? value(q.y, row) : fill;
+            to[2] = e < experts ? value(q.z, row) : fill;
+            to[3] = e < experts ? value(q.w, row) : fill;
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < 4u; j++) to[j] = expert(i + j, lane) < experts ? (float)row[expert(i + j, lane)] : fill;
+        }
+    }
+    static K3_DEVINL void put4(float *row, const float (&from)[4], uint32_t experts, uint32_t lane, uint32_t i) {
+        if (kVector) {
+            const uint32_t e = expert(i, lane);
+            if (e < experts) *reinterpret_cast<float4 *>(row + e) = make_float4(from[0], from[1], from[2], from[3]);
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < 4u; j++) {
+                if (expert(i + j, lane) < experts) row[expert(i + j, lane)] = from[j];
+            }
+        }
+    }
     template <typename T>
     K3_DEVINL void load(const T *row, uint32_t experts, uint32_t lane, float fill) {
 #pragma unroll
-        for (uint32_t i = 0; i < kV * 4u; i += kVector ? 4u : 1u) {
-            const uint32_t e = expert(i, lane);
-            if (kVector) {
-                if (e < experts) {
-                    const uint4 q = *reinterpret_cast<const uint4 *>(row + e);
-                    v[i] = value(q.x, row); v[i + 1u] = value(q.y, row); v[i + 2u] = value(q.z, row); v[i + 3u] = value(q.w, row);
-                } else {
-                    v[i] = v[i + 1u] = v[i + 2u] = v[i + 3u] = fill;
-                }
-            } else {
-                v[i] = e < experts ? (float)row[e] : fill;
-            }
+        for (uint32_t i = 0; i < kV * 4u; i += 4u) {
+            float q[4];
+            get4(q, row, experts, lane, i, fill);
+#pragma unroll
+            for (uint32_t j = 0; j < 4u; j++) v[i + j] = q[j];
         }
     }
     K3_DEVINL void store(float *row, uint32_t experts, uint32_t lane) const {
 #pragma unroll
-        for (uint32_t i = 0; i < kV * 4u; i += kVector ? 4u : 1u) {
-            const uint32_t e = expert(i, lane);
-            if (e >= experts) continue;
-            if (kVector) *reinterpret_cast<float4 *>(row + e) = make_float4(v[i], v[i + 1u], v[i + 2u], v[i + 3u]);
-            else row[e] = v[i];
+        for (uint32_t i = 0; i < kV * 4u; i += 4u) {
+            const float q[4] = {v[i], v[i + 1u], v[i + 2u], v[i + 3u]};
+            put4(row, q, experts, lane, i);
         }
     }
     static K3_DEVINL float value(uint32_t bits, const float *) { return __uint_as_float(bits); }
@@ -74,31 +101,37 @@ struct Row {
         return warp_sum(s);
     }
     // logits -> scores; experts past the end have the logit -inf and get the score 0
-    K3_DEVINL void scores(int softmax) {
+    K3_DEVINL Softmax scores(int softmax) {
+        Softmax f{0.f, 0.f};
         if (!softmax) {
 #pragma unroll
-            for (uint32_t i = 0; i < kV * 4u; i++) v[i] = 1.0f / (1.0f + expf(-v[i]));
-            return;
+            for (uint32_t i = 0; i < kV * 4u; i++) v[i] = sigmoid(v[i]);
+            return f;
         }
-        float m = -INFINITY;
-        bool nan = false;                          // fmaxf drops a NaN
+        f.top = -INFINITY;
 #pragma unroll
-        for (uint32_t i = 0; i < kV * 4u; i++) {
-            m = fmaxf(m, v[i]);
-            nan |= v[i] != v[i];
-        }
-        m = warp_max(m);
-        if (__any_sync(0xffffffffu, nan)) m = __uint_as_float(0x7fffffffu);
-        if (m == -INFINITY) {
+        for (uint32_t i = 0; i < kV * 4u; i++) f.top = fmaxf(f.top, v[i]);
+        f.top = warp_max(f.top);
+        if (f.top == -INFINITY) {                  // every logit is -inf, or NaN, which fmaxf drops
+            float s = 0.f;
+#pragma unroll
+            for (uint32_t i = 0; i < kV * 4u; i++) s += v[i] != v[i] ? v[i] : 0.f;
+            f.top = 0.f;
+            f.over = warp_sum(s);                  // 0, or NaN
 #pragma unroll
             for (uint32_t i = 0; i < kV * 4u; i++) v[i] = 0.f;
-            return;
+        } else {
+            float s = 0.f;
+#pragma unroll
+            for (uint32_t i = 0; i < kV * 4u; i++) {
+                v[i] = __expf(v[i] - f.top);
+                s += v[i];
+            }
+            f.over = 1.0f / warp_sum(s);
         }
 #pragma unroll
-        for (uint32_t i = 0; i < kV * 4u; i++) v[i] = expf(v[i] - m);
-        const float r = 1.0f / sum();
-#pragma unroll
-        for (uint32_t i = 0; i < kV * 4u; i++) v[i] *= r;
+        for (uint32_t i = 0; i < kV * 4u; i++) v[i] *= f.over;
+        return f;
     }
 };
 
@@ -119,7 +152,7 @@ K3_DEVINL uint32_t end_of(const uint32_t *offsets, uint32_t s, uint32_t tokens) 
 
 // ---------------------------------------------------------------------------------------- forward
 template <uint32_t kV, bool kVector>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 2)
 balance_tokens_kernel(float *part_sums, uint32_t *part_counts, const float *logits, const uint32_t *ids, const uint32_t *offsets,
                       Shape a) {
     extern __shared__ float sums_s[];              // [kWarps][experts], then counts u32 [experts]
@@ -143,9 +176,11 @@ balance_tokens_kernel(float *part_sums, uint32_t *part_counts, const float *logi
             else g_balance_status = 2u;
         }
         if (logits) {
+            Row<kV, kVector> next;                 // on its way while the row in front of it is added
+            if (t + warp < end) next.load(logits + (uint64_t)(t + warp) * a.experts, a.experts, lane, -INFINITY);
             for (uint32_t u = t + warp; u < end; u += kWarps) {
-                Row<kV, kVector> p;
-                p.load(logits + (uint64_t)u * a.experts, a.experts, lane, -INFINITY);
+                Row<kV, kVector> p = next;
+                if (u + kWarps < end) next.load(logits + (uint64_t)(u + kWarps) * a.experts, a.experts, lane, -INFINITY);
                 p.scores(a.softmax);
                 const float r = a.softmax ? 1.0f : 1.0f / (kTiny + p.sum());
 #pragma unroll
@@ -169,60 +204,94 @@ balance_tokens_kernel(float *part_sums, uint32_t *part_counts, const float *logi
     }
 }
 
-// one block per sequence
+// A cluster of blocks per sequence, 128 experts each; eight groups of threads take every eighth partial row.
 __global__ void __launch_bounds__(1024)
 balance_sequences_kernel(uint32_t *counts, float *loss, float *means, const float *part_sums, const uint32_t *part_counts,
                          const uint32_t *offsets, Shape a, float coefficient) {
-    __shared__ float total[32];
+    __shared__ float sums_s[8][128];
+    __shared__ uint32_t counts_s[8][128];
+    __shared__ float total[4], mine;
     pdl_wait();
-    const uint32_t s = blockIdx.x, begin = begin_of(offsets, s), end = end_of(offsets, s, a.tokens);
+    const uint32_t s = blockIdx.y, begin = begin_of(offsets, s), end = end_of(offsets, s, a.tokens);
     const uint32_t length = end > begin ? end - begin : 0u;
-    float product = 0.f;
-    for (uint32_t e = threadIdx.x; e < a.experts; e += blockDim.x) {
-        uint32_t n = 0u;
-        float sum = 0.f;
-        if (length) {
-            for (uint32_t b = begin / a.chunk; b <= (end - 1u) / a.chunk; b++) {
-                n += part_counts[(uint64_t)(b + s) * a.experts + e];
-                if (means) sum += part_sums[(uint64_t)(b + s) * a.experts + e];
-            }
+    const uint32_t column = threadIdx.x % 128u, group = threadIdx.x / 128u, e = blockIdx.x * 128u + column;
+    uint32_t n = 0u;
+    float sum = 0.f;
+    if (length && e < a.experts) {
+        const uint32_t last = (end - 1u) / a.chunk;
+#pragma unroll 4
+        for (uint32_t b = begin / a.chunk + group; b <= last; b += 8u) {
+            const uint64_t at = (uint64_t)(b + s) * a.experts + e;
+            n += part_counts[at];
+            if (means) sum += part_sums[at];
         }
-        counts[(uint64_t)s * a.experts + e] = n;
-        if (means) {
-            const float mean = length ? sum / (float)length : 0.f;
-            means[(uint64_t)s * a.experts + e] = mean;
-            product = fmaf((float)n, mean, product);
+    }
+    sums_s[group][column] = sum;
+    counts_s[group][column] = n;
+    __syncthreads();
+    if (threadIdx.x < 128u) {
+#pragma unroll
+        for (uint32_t g = 1; g < 8u; g++) {
+            n += counts_s[g][column];
+            sum += sums_s[g][column];
         }
+        const float mean = length ? sum / (float)length : 0.f;
+        if (e < a.experts) {
+            counts[(uint64_t)s * a.experts + e] = n;
+            if (means) means[(uint64_t)s * a.experts + e] = mean;
+        }
+        const float part = warp_sum((float)n * mean);              // an expert past the end has none
+        if (threadIdx.x % kWarp == 0u) total[threadIdx.x / kWarp] = part;
     }
     if (!means) return;
-    product = warp_sum(product);
-    if (threadIdx.x % kWarp == 0u) total[threadIdx.x / kWarp] = product;
     __syncthreads();
-    if (threadIdx.x < kWarp) {
-        const float sum = warp_sum(threadIdx.x < blockDim.x / kWarp ? total[threadIdx.x] : 0.f);
-        if (threadIdx.x == 0u) {
-            loss[s] = length ? coefficient * sum * ((float)a.experts / ((float)a.top_k * (float)length)) : 0.f;
-        }
+    if (threadIdx.x == 0u) mine = total[0] + total[1] + total[2] + total[3];
+    __syncthreads();
+    cluster_barrier();
+    if (cluster_rank() == 0u && threadIdx.x == 0u) {
+        float all = 0.f;
+        for (uint32_t r = 0; r < cluster_size(); r++) all += cluster_load(&mine, r);
+        loss[s] = length ? coefficient * all * ((float)a.experts / ((float)a.top_k * (float)length)) : 0.f;
     }
+    cluster_barrier();                             // nobody leaves while its sum is read
 }
 
 // --------------------------------------------------------------------------------------- backward
 // A warp's tokens follow one another, so a sequence's shares f stay in registers while it lasts.
 template <uint32_t kV, bool kVector>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 2)
 router_backward_kernel(float *d_logits, const float *logits, const uint32_t *ids, const uint32_t *counts, const uint32_t *offsets,
                        const float *d_loss, const float *d_weights, Shape a, float coefficient, float route_scale) {
-    extern __shared__ float rows_s[];              // [kWarps][experts]
+    extern __shared__ float rows_s[];              // [kWarps][experts], zeros but for the chosen of the token at hand
     const uint32_t warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
     float *row_s = rows_s + warp * a.experts;
+    for (uint32_t e = lane; d_weights && e < a.experts; e += kWarp) row_s[e] = 0.f;
     pdl_wait();
     const uint32_t first = (blockIdx.x * kWarps + warp) * a.chunk;
     if (first >= a.tokens) return;
     const uint32_t last = min(a.tokens, first + a.chunk);
     uint32_t s = 0u, end = first;
-    Row<kV, kVector> f;
+    Row<kV, kVector> f, next;
     float c = 0.f;
+    uint32_t next_id = 0xffffffffu;
+    float next_w = 0.f, next_l = 0.f;
+    // a token's row and what lane r needs of its r-th choice
+    auto fetch = [&](uint32_t t) {
+        next.load(logits + (uint64_t)t * a.experts, a.experts, lane, -INFINITY);
+        if (d_weights) {
+            next_id = lane < a.top_k ? ids[(uint64_t)t * a.top_k + lane] : 0xffffffffu;
+            const bool chosen = next_id < a.experts;
+            if (lane < a.top_k && !chosen) g_balance_status = 2u;
+            next_w = chosen ? d_weights[(uint64_t)t * a.top_k + lane] : 0.f;
+            next_l = chosen ? logits[(uint64_t)t * a.experts + next_id] : -INFINITY;
+        }
+    };
+    fetch(first);
     for (uint32_t t = first; t < last; t++) {
+        Row<kV, kVector> p = next;
+        const uint32_t id = next_id;
+        const float w = next_w, l = next_l;
+        if (t + 1u < last) fetch(t + 1u);
         if (d_loss && t >= end) {
             s = sequence_of(offsets, a.sequences, t);
             const uint32_t begin = begin_of(offsets, s);
@@ -240,13 +309,10 @@ router_backward_kernel(float *d_logits, const float *logits, const uint32_t *ids
                 for (uint32_t i = 0; i < kV * 4u; i++) f.v[i] *= scale;
             }
         }
-        Row<kV, kVector> p, d;
-        p.load(logits + (uint64_t)t * a.experts, a.experts, lane, -INFINITY);
-        p.scores(a.softmax);
-        if (d_loss && a.softmax) {
-#pragma unroll
-            for (uint32_t i = 0; i < kV * 4u; i++) d.v[i] = c * f.v[i];
-        } else if (d_loss) {
+        const Softmax soft = p.scores(a.softmax);
+        // the loss by a score is by (f - mean)
+        float by = c, mean = 0.f;
+        if (d_loss && !a.softmax) {
             float z = 0.f, fp = 0.f;
 #pragma unroll
             for (uint32_t i = 0; i < kV * 4u; i++) {
@@ -254,30 +320,18 @@ router_backward_kernel(float *d_logits, const float *logits, const uint32_t *ids
                 fp = fmaf(f.v[i], p.v[i], fp);
             }
             const float r = 1.0f / (kTiny + warp_sum(z));
-            const float mean = warp_sum(fp) * r, cr = c * r;
-#pragma unroll
-            for (uint32_t i = 0; i < kV * 4u; i++) d.v[i] = cr * (f.v[i] - mean);
-        } else {
-#pragma unroll
-            for (uint32_t i = 0; i < kV * 4u; i++) d.v[i] = 0.f;
+            mean = warp_sum(fp) * r;
+            by = c * r;
         }
+        const bool chosen = id < a.experts;
         if (d_weights) {
-            // the chosen scores from the row in shared memory, then their share added to it there
-            p.store(row_s, a.experts, lane);
-            __syncwarp();
-            const bool has = lane < a.top_k;
-            const uint32_t id = has ? ids[(uint64_t)t * a.top_k + lane] : 0xffffffffu;
-            const bool chosen = has && id < a.experts;
-            if (has && !chosen) g_balance_status = 2u;
-            const float w = chosen ? d_weights[(uint64_t)t * a.top_k + lane] : 0.f, si = chosen ? row_s[id] : 0.f;
+            // the weights' share at the chosen, through shared memory to the lanes that hold them
+            const float si = !chosen ? 0.f : a.softmax ? __expf(l - soft.top) * soft.over : sigmoid(l);
             const float under = 1.0f / (kTiny + warp_sum(si));
             const float share = route_scale * (w - warp_sum(w * si) * under) * under;
-            __syncwarp();
-            d.store(row_s, a.experts, lane);
-            __syncwarp();
             const uint32_t same = __match_any_sync(0xffffffffu, chosen ? id : 0x80000000u + lane);
             if (!__any_sync(0xffffffffu, chosen && (same & (same - 1u)) != 0u)) {
-                if (chosen) row_s[id] += share;
+                if (chosen) row_s[id] = share;
             } else {                               // an expert named twice: one after the other
                 for (uint32_t r = 0; r < a.top_k; r++) {
                     if (lane == r && chosen) row_s[id] += share;
@@ -285,54 +339,76 @@ router_backward_kernel(float *d_logits, const float *logits, const uint32_t *ids
                 }
             }
             __syncwarp();
-            d.load(row_s, a.experts, lane, 0.f);
-            __syncwarp();
         }
+        // by the scores i .. i + 3
+        auto by_scores = [&](float (&d)[4], uint32_t i) {
+            if (d_weights) {
+                Row<kV, kVector>::get4(d, row_s, a.experts, lane, i, 0.f);
+            } else {
+                d[0] = d[1] = d[2] = d[3] = 0.f;
+            }
+            if (d_loss) {
+#pragma unroll
+                for (uint32_t j = 0; j < 4u; j++) d[j] = fmaf(by, f.v[i + j] - mean, d[j]);
+            }
+        };
+        float dp = 0.f;
         if (a.softmax) {
-            float dp = 0.f;
 #pragma unroll
-            for (uint32_t i = 0; i < kV * 4u; i++) dp = fmaf(d.v[i], p.v[i], dp);
+            for (uint32_t i = 0; i < kV * 4u; i += 4u) {
+                float d[4];
+                by_scores(d, i);
+#pragma unroll
+                for (uint32_t j = 0; j < 4u; j++) dp = fmaf(d[j], p.v[i + j], dp);
+            }
             dp = warp_sum(dp);
-#pragma unroll
-            for (uint32_t i = 0; i < kV * 4u; i++) d.v[i] = p.v[i] * (d.v[i] - dp);
-        } else {
-#pragma unroll
-            for (uint32_t i = 0; i < kV * 4u; i++) d.v[i] *= p.v[i] * (1.0f - p.v[i]);
         }
-        d.store(d_logits + (uint64_t)t * a.experts, a.experts, lane);
+        float *out = d_logits + (uint64_t)t * a.experts;
+#pragma unroll
+        for (uint32_t i = 0; i < kV * 4u; i += 4u) {
+            float d[4];
+            by_scores(d, i);
+#pragma unroll
+            for (uint32_t j = 0; j < 4u; j++) {
+                const float q = p.v[i + j];
+                d[j] = a.softmax ? q * (d[j] - dp) : d[j] * (q * (1.0f - q));
+            }
+            Row<kV, kVector>::put4(out, d, a.experts, lane, i);
+        }
+        __syncwarp();
+        if (d_weights && chosen) row_s[id] = 0.f;
+        __syncwarp();                              // the zeros are back before the next token's shares
     }
 }
 
 bool shape_ok(uint32_t tokens, uint32_t sequences, uint32_t experts, uint32_t top_k, int score, const void *offsets) {
-    return tokens != 0u && tokens <= (1u << 26) && sequences != 0u && sequences <= (1u << 26) && (offsets || sequences == 1u) &&
+    return tokens != 0u && tokens <= (1u << 26) && sequences != 0u && sequences <= 65535u && (offsets || sequences == 1u) &&
            experts != 0u && experts <= kMaxExperts && top_k != 0u && top_k <= 32u && top_k <= experts &&
            (score == K3_MOE_SCORE_SIGMOID || score == K3_MOE_SCORE_SOFTMAX);
 }
 
-// Tokens per block of the forward pass: two blocks per SM have work, and a warp has at least one token.
-uint32_t forward_chunk(uint32_t tokens) {
-    const uint32_t blocks = 148u * 2u;             // the same partial sums on any device
-    return std::max((tokens + blocks - 1u) / blocks, kWarps);
-}
+// Tokens per block of the forward pass: two blocks per SM, the same partial sums on any device, and a token per warp
+// at least.
+constexpr uint32_t kForwardBlocks = 148u * 2u;
+uint32_t forward_chunk(uint32_t tokens) { return std::max((tokens + kForwardBlocks - 1u) / kForwardBlocks, kWarps); }
 
 struct BalanceWorkspace {
     uint64_t rows;
     size_t sums, total;
     BalanceWorkspace(uint32_t tokens, uint32_t sequences, uint32_t experts) {
-        const uint32_t chunk = forward_chunk(tokens);
-        rows = (uint64_t)(tokens + chunk - 1u) / chunk + sequences;
+        rows = std::min((tokens + kWarps - 1u) / kWarps, kForwardBlocks) + (uint64_t)sequences;   // never less for more tokens
         sums = (size_t)(rows * experts * sizeof(float) + 255u) / 256u * 256u;
         total = sums + (size_t)(rows * experts * sizeof(uint32_t));
     }
 };
 
 // The instance for a number of experts: one to eight groups of 128.
-template <template <uint32_t, bool> class Pick, typename... A>
+template <template <uint32_t, bool> class Pick, uint32_t kV = 1, typename... A>
 bool pick(uint32_t experts, bool vector, A... args) {
-    if (experts <= 128u) return vector ? Pick<1, true>::go(args...) : Pick<1, false>::go(args...);
-    if (experts <= 256u) return vector ? Pick<2, true>::go(args...) : Pick<2, false>::go(args...);
-    if (experts <= 512u) return vector ? Pick<4, true>::go(args...) : Pick<4, false>::go(args...);
-    return vector ? Pick<8, true>::go(args...) : Pick<8, false>::go(args...);
+    if constexpr (kV < 8u) {
+        if (experts > kV * 128u) return pick<Pick, kV + 1u>(experts, vector, args...);
+    }
+    return vector ? Pick<kV, true>::go(args...) : Pick<kV, false>::go(args...);
 }
 
 template <uint32_t kV, bool kVector>
@@ -396,9 +472,10 @@ extern "C" bool k3_moe_balance(void *counts, void *loss, void *means, const void
     float *sums = (float *)workspace;
     uint32_t *part_counts = (uint32_t *)((char *)workspace + w.sums);
     const bool vector = experts % 4u == 0u && ((uintptr_t)logits & 15u) == 0u;
+    const uint32_t slices = (experts + 127u) / 128u;
     return pick<Forward>(experts, vector, sums, part_counts, (const float *)logits, (const uint32_t *)ids, (const uint32_t *)offsets,
                          a, stream) &&
-           launch_chained(balance_sequences_kernel, sequences, 1024, 0, stream, (uint32_t *)counts, (float *)loss, (float *)means,
+           launch_chained_cluster(balance_sequences_kernel, dim3(slices, sequences), 1024, dim3(slices, 1, 1), 0, stream, (uint32_t *)counts, (float *)loss, (float *)means,
                           (const float *)sums, (const uint32_t *)part_counts, (const uint32_t *)offsets, a, coefficient);
 }
 

@@ -100,6 +100,29 @@ K3_DEVINL uint2 ld_stream_8(const void *p) {
 K3_DEVINL void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 K3_DEVINL void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// Thread block clusters: this block's place, the barrier of all its threads (release / acquire), and an f32 at
+// the same place of another block's shared memory.
+K3_DEVINL uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+K3_DEVINL uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+K3_DEVINL void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+K3_DEVINL float cluster_load(const float *mine, uint32_t rank) {
+    uint32_t addr;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"((uint32_t)__cvta_generic_to_shared(mine)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
 // One thread: bring [p, p + bytes) into L2 (whole 16-byte units inside the range).
 K3_DEVINL void prefetch_l2(const void *p, uint64_t bytes) {
     const uint64_t begin = ((uint64_t)p + 15u) & ~15ull, end = ((uint64_t)p + bytes) & ~15ull;
@@ -108,23 +131,34 @@ K3_DEVINL void prefetch_l2(const void *p, uint64_t bytes) {
     }
 }
 
+// A programmatic launch in clusters of `cluster` blocks (at most 8 in all, dividing the grid; 1 x 1 x 1: none).
 template <typename... P, typename... A>
-inline bool launch_chained(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A... args) {
-    cudaLaunchAttribute attribute{};
-    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attribute.val.programmaticStreamSerializationAllowed = 1;
+inline bool launch_chained_cluster(void (*kernel)(P...), dim3 grid, dim3 block, dim3 cluster, size_t smem, cudaStream_t stream,
+                                   A... args) {
+    cudaLaunchAttribute attributes[2]{};
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = cluster.x;
+    attributes[1].val.clusterDim.y = cluster.y;
+    attributes[1].val.clusterDim.z = cluster.z;
     cudaLaunchConfig_t config{};
     config.gridDim = grid;
     config.blockDim = block;
     config.dynamicSmemBytes = smem;
     config.stream = stream;
-    config.attrs = &attribute;
-    config.numAttrs = 1;
+    config.attrs = attributes;
+    config.numAttrs = cluster.x * cluster.y * cluster.z > 1u ? 2 : 1;
     if (cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...) != cudaSuccess) {
         (void)cudaGetLastError();
         return false;
     }
     return true;
+}
+
+template <typename... P, typename... A>
+inline bool launch_chained(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A... args) {
+    return launch_chained_cluster(kernel, grid, block, dim3(1, 1, 1), smem, stream, args...);
 }
 
 inline bool launch_ok() { return cudaGetLastError() == cudaSuccess; }

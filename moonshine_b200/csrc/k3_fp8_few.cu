@@ -69,28 +69,6 @@ struct Item {
     uint32_t group, row, rows, column, kb_begin, kb_end;
 };
 
-K3_DEVINL uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-K3_DEVINL uint32_t cluster_size() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-    return r;
-}
-K3_DEVINL void cluster_barrier() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// f32 at the same place of another block's shared memory
-K3_DEVINL float cluster_load(const float *mine, uint32_t rank) {
-    uint32_t addr;
-    float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(mine)), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-    return v;
-}
-
 K3_DEVINL void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -519,24 +497,8 @@ bool launch_split(const Product &p, cudaStream_t stream) {
     const uint32_t parts = (blocks + a.split_blocks - 1u) / a.split_blocks;
     auto kernel = fp8_few_kernel<kEpilogue, 1, kRows, true>;
     if (!set_max_dynamic_smem((const void *)kernel, L::kBytes)) return false;
-    cudaLaunchAttribute attributes[2]{};
-    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attributes[0].val.programmaticStreamSerializationAllowed = 1;
-    attributes[1].id = cudaLaunchAttributeClusterDimension;
-    attributes[1].val.clusterDim.x = parts;
-    attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
-    cudaLaunchConfig_t config{};
-    config.gridDim = dim3(parts, tiles, row_tiles);
-    config.blockDim = L::kThreads;
-    config.dynamicSmemBytes = L::kBytes;
-    config.stream = stream;
-    config.attrs = attributes;
-    config.numAttrs = 2;
-    if (cudaLaunchKernelEx(&config, kernel, a_map, b_map, b_map, a) != cudaSuccess) {
-        (void)cudaGetLastError();
-        return false;
-    }
-    return true;
+    return launch_chained_cluster(kernel, dim3(parts, tiles, row_tiles), L::kThreads, dim3(parts, 1, 1), L::kBytes, stream, a_map,
+                                  b_map, b_map, a);
 }
 
 template <int kEpilogue>

@@ -93,18 +93,24 @@ def transpose_blocks(codes: torch.Tensor, scales: torch.Tensor, rows: int, colum
 
 
 class _Workspace:
-    """Device scratch of an object, as large as its largest call so far."""
+    """Device scratch of an object for the largest sizes (tokens, or tokens and sequences) it has seen;
+    ``need(*sizes)`` gives the bytes."""
 
-    def __init__(self):
-        self._held = None
+    def __init__(self, need):
+        self._need, self._held, self._sizes, self.bytes = need, None, (), 0
 
-    def of(self, need: int, device) -> torch.Tensor:
+    def of(self, *sizes_device) -> torch.Tensor:
+        *sizes, device = sizes_device
+        if self._held is not None and self._held.device == device and all(map(int.__le__, sizes, self._sizes)):
+            return self._held
+        sizes = [max(pair) for pair in zip(sizes, self._sizes)] if self._sizes else sizes
+        need = self._need(*sizes)
         if need == 0:
             raise RuntimeError("the sizes of this call are not supported")
-        if self._held is None or self._held.numel() < need or self._held.device != device:
-            if self._held is not None:          # the last call may still be running on this stream
-                self._held.record_stream(torch.cuda.current_stream(self._held.device))
-            self._held = torch.empty(need, dtype=torch.uint8, device=device)
+        if self._held is not None:              # the last call may still be running on this stream
+            self._held.record_stream(torch.cuda.current_stream(self._held.device))
+        self._held = torch.empty(need, dtype=torch.uint8, device=device)
+        self._sizes, self.bytes = sizes, need
         return self._held
 
 
@@ -114,16 +120,15 @@ class Fp8Linear:
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, columns: int):
         _table(codes, scales, (), rows, columns, "table")
         self.codes, self.scales, self.rows, self.columns = codes, scales, rows, columns
-        self._workspace = _Workspace()
+        self._workspace = _Workspace(lambda tokens: ops.k3_moe_fp8_linear_workspace_bytes(tokens, columns))
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         """x bf16 [tokens, columns] -> bf16 [tokens, rows]."""
         tokens, _ = _matrix(x, "x", self.columns)
         out = torch.empty((tokens, self.rows), dtype=torch.bfloat16, device=x.device)
         if tokens:
-            need = ops.k3_moe_fp8_linear_workspace_bytes(tokens, self.columns)
-            ws = self._workspace.of(need, x.device)
-            _done(ops.k3_moe_fp8_linear(out, x, self.codes, self.scales, tokens, self.rows, self.columns, ws, ws.numel()),
+            ws = self._workspace.of(tokens, x.device)
+            _done(ops.k3_moe_fp8_linear(out, x, self.codes, self.scales, tokens, self.rows, self.columns, ws, self._workspace.bytes),
                   "k3_moe_fp8_linear")
         return out
 
@@ -134,7 +139,7 @@ class Fp8LinearGradient:
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, columns: int):
         self.rows, self.columns = rows, columns
         self._by_input = Fp8Linear(codes, scales, columns, rows)
-        self._workspace = _Workspace()
+        self._workspace = _Workspace(lambda tokens: ops.k3_moe_fp8_weight_gradient_workspace_bytes(tokens, rows, columns))
 
     def by_input(self, dy: torch.Tensor) -> torch.Tensor:
         """dy bf16 [tokens, rows] -> dx bf16 [tokens, columns]."""
@@ -152,9 +157,9 @@ class Fp8LinearGradient:
         if tokens == 0:
             return into if into is not None else torch.zeros((self.rows, self.columns), dtype=torch.float32, device=dy.device)
         dw = into if into is not None else torch.empty((self.rows, self.columns), dtype=torch.float32, device=dy.device)
-        ws = self._workspace.of(ops.k3_moe_fp8_weight_gradient_workspace_bytes(tokens, self.rows, self.columns), dy.device)
-        _done(ops.k3_moe_fp8_weight_gradient(dw, dy, x, tokens, self.rows, self.columns, int(into is not None), ws, ws.numel()),
-              "k3_moe_fp8_weight_gradient")
+        ws = self._workspace.of(tokens, dy.device)
+        _done(ops.k3_moe_fp8_weight_gradient(dw, dy, x, tokens, self.rows, self.columns, int(into is not None), ws,
+                                             self._workspace.bytes), "k3_moe_fp8_weight_gradient")
         return dw
 
 
@@ -179,7 +184,7 @@ class Fp8Experts:
             hidden=hidden, expert_hidden=expert_hidden, experts=experts, top_k=top_k, activation=_ACTIVATIONS[activation],
             beta=beta, linear_beta=linear_beta, w1=w1.data_ptr(), w1_scales=w1_scales.data_ptr(), w3=w3.data_ptr(),
             w3_scales=w3_scales.data_ptr(), w2=w2.data_ptr(), w2_scales=w2_scales.data_ptr())
-        self._workspace = _Workspace()
+        self._workspace = _Workspace(lambda tokens: ops.k3_moe_fp8_experts_workspace_bytes(self.desc, tokens))
 
     def forward(self, x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
                 shared: torch.Tensor | None = None) -> torch.Tensor:
@@ -193,7 +198,7 @@ class Fp8Experts:
             raise ValueError("shared: another number of tokens than x")
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
         if tokens:
-            ws = self._workspace.of(ops.k3_moe_fp8_experts_workspace_bytes(self.desc, tokens), x.device)
-            _done(ops.k3_moe_fp8_experts_forward(self.desc, out, x, ids, weights, shared, tokens, ws, ws.numel()),
+            ws = self._workspace.of(tokens, x.device)
+            _done(ops.k3_moe_fp8_experts_forward(self.desc, out, x, ids, weights, shared, tokens, ws, self._workspace.bytes),
                   "k3_moe_fp8_experts_forward")
         return out
