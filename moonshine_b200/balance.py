@@ -15,7 +15,7 @@ _SCORES = {"sigmoid": ops.SCORE_SIGMOID, "softmax": ops.SCORE_SOFTMAX}
 
 
 def _check(t, name, dtype, shape):
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape):
+    if t.dtype is not dtype or t.shape != shape:
         raise ValueError(f"{name}: expected {dtype} {list(shape)}, got {t.dtype} {list(t.shape)}")
 
 
@@ -36,7 +36,7 @@ class RouterBalance:
         _check(ids, "ids", torch.int32, (tokens, self.top_k))
         if offsets is None:
             return tokens, 1
-        if offsets.dim() != 1 or offsets.dtype != torch.int32 or offsets.shape[0] < 2:
+        if offsets.dtype is not torch.int32 or offsets.dim() != 1 or offsets.shape[0] < 2:
             raise ValueError(f"offsets: expected int32 [sequences + 1], got {offsets.dtype} {list(offsets.shape)}")
         return tokens, offsets.shape[0] - 1
 
@@ -46,12 +46,12 @@ class RouterBalance:
         tokens, sequences = self._sequences(ids, offsets)
         if logits is not None:
             _check(logits, "logits", torch.float32, (tokens, self.experts))
-        make = torch.empty if tokens else torch.zeros
-        counts = make((sequences, self.experts), dtype=torch.int32, device=ids.device)
+        make = ids.new_empty if tokens else ids.new_zeros
+        counts = make((sequences, self.experts))
         loss = means = None
         if logits is not None:
-            loss = make(sequences, dtype=torch.float32, device=ids.device)
-            means = make((sequences, self.experts), dtype=torch.float32, device=ids.device)
+            loss = make(sequences, dtype=torch.float32)
+            means = make((sequences, self.experts), dtype=torch.float32)
         if tokens:
             ws = self._workspace.of(tokens, sequences, ids.device)
             _done(ops.k3_moe_balance(counts, loss, means, logits, ids, offsets, tokens, sequences, self.experts, self.top_k,
@@ -72,7 +72,7 @@ class RouterBalance:
             _check(counts, "counts", torch.int32, (sequences, self.experts))
         if d_weights is not None:
             _check(d_weights, "d_weights", torch.float32, (tokens, self.top_k))
-        d_logits = torch.empty_like(logits, memory_format=torch.contiguous_format)
+        d_logits = logits.new_empty((tokens, self.experts))
         if tokens:
             _done(ops.k3_moe_router_backward(d_logits, logits, ids, counts, offsets, d_loss, d_weights, tokens, sequences,
                                              self.experts, self.top_k, self.score, self.coefficient, self.route_scale),

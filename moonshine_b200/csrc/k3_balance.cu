@@ -23,6 +23,7 @@ namespace {
 constexpr uint32_t kThreads = 256, kWarps = kThreads / kWarp;
 constexpr uint32_t kMaxExperts = 1024;
 constexpr float kTiny = 1e-20f;
+constexpr uint32_t kForwardStages = 3, kBackwardStages = 2;   // rows of a warp in shared memory
 
 __device__ uint32_t g_balance_status = 0;          // 2: an expert id >= experts
 
@@ -36,6 +37,16 @@ struct Shape {
 // a score.  With expf and the rounded quotient the pass over the logits was bound by its instructions,
 // 32768 x 896 forward and backward 198 us.
 K3_DEVINL float sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
+
+template <int kBytes>
+K3_DEVINL void copy_async(float *to, const float *from) {
+    const uint32_t addr = (uint32_t)__cvta_generic_to_shared(to);
+    if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(addr), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(addr), "l"(from) : "memory");
+}
+K3_DEVINL void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+K3_DEVINL void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
 
 struct Softmax {
     float top, over;                               // a score is exp(logit - top) * over
@@ -73,6 +84,15 @@ struct Row {
             for (uint32_t j = 0; j < 4u; j++) {
                 if (expert(i + j, lane) < experts) row[expert(i + j, lane)] = from[j];
             }
+        }
+    }
+    // The same row by asynchronous copies into shared memory (kV * 128 floats; what lies past the experts stays).
+    // A lane copies what it reads itself.
+    static K3_DEVINL void fetch(float *to, const float *row, uint32_t experts, uint32_t lane) {
+#pragma unroll
+        for (uint32_t i = 0; i < kV * 4u; i += kVector ? 4u : 1u) {
+            const uint32_t e = expert(i, lane);
+            if (e < experts) copy_async<kVector ? 16 : 4>(to + e, row + e);
         }
     }
     template <typename T>
@@ -155,9 +175,11 @@ template <uint32_t kV, bool kVector>
 __global__ void __launch_bounds__(kThreads, 2)
 balance_tokens_kernel(float *part_sums, uint32_t *part_counts, const float *logits, const uint32_t *ids, const uint32_t *offsets,
                       Shape a) {
-    extern __shared__ float sums_s[];              // [kWarps][experts], then counts u32 [experts]
-    uint32_t *counts_s = reinterpret_cast<uint32_t *>(sums_s + (logits ? kWarps * a.experts : 0u));
+    constexpr uint32_t kPitch = kV * 128u;
+    extern __shared__ __align__(16) float rows_s[];   // counts u32 [kPitch], then [kWarps][kForwardStages][kPitch], at the end sums [kWarps][kPitch]
+    uint32_t *counts_s = reinterpret_cast<uint32_t *>(rows_s);
     const uint32_t warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+    float *mine = rows_s + kPitch + warp * (kForwardStages * kPitch), *sums_s = rows_s + kPitch;
     pdl_wait();
     uint32_t t = blockIdx.x * a.chunk;
     const uint32_t last = min(a.tokens, t + a.chunk);
@@ -168,6 +190,17 @@ balance_tokens_kernel(float *part_sums, uint32_t *part_counts, const float *logi
         Row<kV, kVector> acc;
 #pragma unroll
         for (uint32_t i = 0; i < kV * 4u; i++) acc.v[i] = 0.f;
+        auto fetch = [&](uint32_t u, uint32_t stage) {
+            if (u < end) Row<kV, kVector>::fetch(mine + stage * kPitch, logits + (uint64_t)u * a.experts, a.experts, lane);
+            copies_commit();
+        };
+        if (logits) {                              // on their way while the routes are counted
+#pragma unroll
+            for (uint32_t g = 0; g + 1u < kForwardStages; g++) fetch(t + warp + g * kWarps, g);
+            for (uint32_t e = a.experts + lane; e < kPitch; e += kWarp) {
+                for (uint32_t g = 0; g < kForwardStages; g++) mine[g * kPitch + e] = -INFINITY;
+            }
+        }
         for (uint32_t e = threadIdx.x; e < a.experts; e += kThreads) counts_s[e] = 0u;
         __syncthreads();
         for (uint32_t r = t * a.top_k + threadIdx.x; r < end * a.top_k; r += kThreads) {
@@ -176,17 +209,21 @@ balance_tokens_kernel(float *part_sums, uint32_t *part_counts, const float *logi
             else g_balance_status = 2u;
         }
         if (logits) {
-            Row<kV, kVector> next;                 // on its way while the row in front of it is added
-            if (t + warp < end) next.load(logits + (uint64_t)(t + warp) * a.experts, a.experts, lane, -INFINITY);
+            uint32_t stage = 0u;
             for (uint32_t u = t + warp; u < end; u += kWarps) {
-                Row<kV, kVector> p = next;
-                if (u + kWarps < end) next.load(logits + (uint64_t)(u + kWarps) * a.experts, a.experts, lane, -INFINITY);
+                fetch(u + (kForwardStages - 1u) * kWarps, stage == 0u ? kForwardStages - 1u : stage - 1u);
+                copies_wait<kForwardStages - 1>();
+                Row<kV, kVector> p;
+                p.load(mine + stage * kPitch, kPitch, lane, 0.f);
                 p.scores(a.softmax);
-                const float r = a.softmax ? 1.0f : 1.0f / (kTiny + p.sum());
+                const float r = a.softmax ? 1.0f : __fdividef(1.0f, kTiny + p.sum());
 #pragma unroll
                 for (uint32_t i = 0; i < kV * 4u; i++) acc.v[i] = fmaf(p.v[i], r, acc.v[i]);
+                if (++stage == kForwardStages) stage = 0u;
             }
-            acc.store(sums_s + warp * a.experts, a.experts, lane);
+            copies_wait<0>();
+            __syncthreads();                       // everyone's rows have been read: the sums take their place
+            acc.store(sums_s + warp * kPitch, kPitch, lane);
         }
         __syncthreads();
         const uint64_t to = (uint64_t)(blockIdx.x + s) * a.experts;
@@ -195,7 +232,7 @@ balance_tokens_kernel(float *part_sums, uint32_t *part_counts, const float *logi
             if (logits) {
                 float sum = 0.f;
 #pragma unroll
-                for (uint32_t w = 0; w < kWarps; w++) sum += sums_s[w * a.experts + e];
+                for (uint32_t w = 0; w < kWarps; w++) sum += sums_s[w * kPitch + e];
                 part_sums[to + e] = sum;
             }
         }
@@ -262,36 +299,52 @@ template <uint32_t kV, bool kVector>
 __global__ void __launch_bounds__(kThreads, 2)
 router_backward_kernel(float *d_logits, const float *logits, const uint32_t *ids, const uint32_t *counts, const uint32_t *offsets,
                        const float *d_loss, const float *d_weights, Shape a, float coefficient, float route_scale) {
-    extern __shared__ float rows_s[];              // [kWarps][experts], zeros but for the chosen of the token at hand
+    constexpr uint32_t kPitch = kV * 128u;
+    // per warp: kBackwardStages rows of logits, and a row of zeros but for the chosen of the token at hand
+    extern __shared__ __align__(16) float rows_s[];
     const uint32_t warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
-    float *row_s = rows_s + warp * a.experts;
-    for (uint32_t e = lane; d_weights && e < a.experts; e += kWarp) row_s[e] = 0.f;
+    float *mine = rows_s + warp * ((kBackwardStages + 1u) * kPitch), *row_s = mine + kBackwardStages * kPitch;
+    for (uint32_t e = lane; e < kPitch; e += kWarp) {
+        row_s[e] = 0.f;
+        for (uint32_t g = 0; e >= a.experts && g < kBackwardStages; g++) mine[g * kPitch + e] = -INFINITY;
+    }
+    __syncwarp();
     pdl_wait();
     const uint32_t first = (blockIdx.x * kWarps + warp) * a.chunk;
     if (first >= a.tokens) return;
     const uint32_t last = min(a.tokens, first + a.chunk);
     uint32_t s = 0u, end = first;
-    Row<kV, kVector> f, next;
+    Row<kV, kVector> f;
     float c = 0.f;
     uint32_t next_id = 0xffffffffu;
-    float next_w = 0.f, next_l = 0.f;
-    // a token's row and what lane r needs of its r-th choice
-    auto fetch = [&](uint32_t t) {
-        next.load(logits + (uint64_t)t * a.experts, a.experts, lane, -INFINITY);
-        if (d_weights) {
+    float next_w = 0.f;
+    // a token's row, and what lane r needs of its r-th choice
+    auto fetch = [&](uint32_t t, uint32_t stage) {
+        if (t < last) Row<kV, kVector>::fetch(mine + stage * kPitch, logits + (uint64_t)t * a.experts, a.experts, lane);
+        copies_commit();
+    };
+    auto fetch_choice = [&](uint32_t t) {
+        if (d_weights && t < last) {
             next_id = lane < a.top_k ? ids[(uint64_t)t * a.top_k + lane] : 0xffffffffu;
-            const bool chosen = next_id < a.experts;
-            if (lane < a.top_k && !chosen) g_balance_status = 2u;
-            next_w = chosen ? d_weights[(uint64_t)t * a.top_k + lane] : 0.f;
-            next_l = chosen ? logits[(uint64_t)t * a.experts + next_id] : -INFINITY;
+            if (lane < a.top_k && next_id >= a.experts) g_balance_status = 2u;
+            next_w = next_id < a.experts ? d_weights[(uint64_t)t * a.top_k + lane] : 0.f;
         }
     };
-    fetch(first);
+#pragma unroll
+    for (uint32_t g = 0; g + 1u < kBackwardStages; g++) fetch(first + g, g);
+    fetch_choice(first);
+    uint32_t stage = 0u;
     for (uint32_t t = first; t < last; t++) {
-        Row<kV, kVector> p = next;
+        fetch(t + kBackwardStages - 1u, stage == 0u ? kBackwardStages - 1u : stage - 1u);
         const uint32_t id = next_id;
-        const float w = next_w, l = next_l;
-        if (t + 1u < last) fetch(t + 1u);
+        const float w = next_w;
+        fetch_choice(t + 1u);
+        copies_wait<kBackwardStages - 1>();
+        __syncwarp();                              // the lanes' chosen lie in one another's copies
+        const float l = id < a.experts ? mine[stage * kPitch + id] : 0.f;
+        Row<kV, kVector> p;
+        p.load(mine + stage * kPitch, kPitch, lane, 0.f);
+        if (++stage == kBackwardStages) stage = 0u;
         if (d_loss && t >= end) {
             s = sequence_of(offsets, a.sequences, t);
             const uint32_t begin = begin_of(offsets, s);
@@ -319,7 +372,7 @@ router_backward_kernel(float *d_logits, const float *logits, const uint32_t *ids
                 z += p.v[i];
                 fp = fmaf(f.v[i], p.v[i], fp);
             }
-            const float r = 1.0f / (kTiny + warp_sum(z));
+            const float r = __fdividef(1.0f, kTiny + warp_sum(z));
             mean = warp_sum(fp) * r;
             by = c * r;
         }
@@ -327,7 +380,7 @@ router_backward_kernel(float *d_logits, const float *logits, const uint32_t *ids
         if (d_weights) {
             // the weights' share at the chosen, through shared memory to the lanes that hold them
             const float si = !chosen ? 0.f : a.softmax ? __expf(l - soft.top) * soft.over : sigmoid(l);
-            const float under = 1.0f / (kTiny + warp_sum(si));
+            const float under = __fdividef(1.0f, kTiny + warp_sum(si));
             const float share = route_scale * (w - warp_sum(w * si) * under) * under;
             const uint32_t same = __match_any_sync(0xffffffffu, chosen ? id : 0x80000000u + lane);
             if (!__any_sync(0xffffffffu, chosen && (same & (same - 1u)) != 0u)) {
@@ -343,7 +396,7 @@ router_backward_kernel(float *d_logits, const float *logits, const uint32_t *ids
         // by the scores i .. i + 3
         auto by_scores = [&](float (&d)[4], uint32_t i) {
             if (d_weights) {
-                Row<kV, kVector>::get4(d, row_s, a.experts, lane, i, 0.f);
+                Row<kV, kVector>::get4(d, row_s, kPitch, lane, i, 0.f);
             } else {
                 d[0] = d[1] = d[2] = d[3] = 0.f;
             }
@@ -415,7 +468,7 @@ template <uint32_t kV, bool kVector>
 struct Forward {
     static bool go(float *sums, uint32_t *counts, const float *logits, const uint32_t *ids, const uint32_t *offsets, Shape a,
                    cudaStream_t stream) {
-        const size_t smem = ((logits ? kWarps : 0u) + 1u) * a.experts * sizeof(float);
+        const size_t smem = (1u + (logits ? kWarps * kForwardStages : 0u)) * kV * 128u * sizeof(float);
         return set_max_dynamic_smem((const void *)balance_tokens_kernel<kV, kVector>, smem) &&
                launch_chained(balance_tokens_kernel<kV, kVector>, (a.tokens + a.chunk - 1u) / a.chunk, kThreads, smem, stream,
                               sums, counts, logits, ids, offsets, a);
@@ -427,7 +480,7 @@ struct Backward {
     static bool go(float *d_logits, const float *logits, const uint32_t *ids, const uint32_t *counts, const uint32_t *offsets,
                    const float *d_loss, const float *d_weights, Shape a, float coefficient, float route_scale,
                    cudaStream_t stream) {
-        const size_t smem = kWarps * a.experts * sizeof(float);
+        const size_t smem = kWarps * (kBackwardStages + 1u) * kV * 128u * sizeof(float);
         const uint32_t warps = (a.tokens + a.chunk - 1u) / a.chunk;
         return set_max_dynamic_smem((const void *)router_backward_kernel<kV, kVector>, smem) &&
                launch_chained(router_backward_kernel<kV, kVector>, (warps + kWarps - 1u) / kWarps, kThreads, smem, stream,

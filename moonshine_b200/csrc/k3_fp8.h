@@ -48,6 +48,7 @@ struct Product {
     int b_scale_layout, epilogue, accumulate;
     int activation;
     float beta, linear_beta;
+    bool b_ready;                    // the launch in front is quantize_rows(), which lets this one start behind its own wait
 };
 bool product(const Product &p, cudaStream_t stream);
 // the kernels behind it: tiles of 128 rows (k3_fp8_wide.cu)
@@ -55,5 +56,8 @@ bool wide_product(const Product &p, cudaStream_t stream);
 // tiles of 16 or 64 rows, b in 128 x 128 blocks only (k3_fp8_few.cu)
 constexpr uint32_t few_rows = 64;
 bool few_product(const Product &p, cudaStream_t stream);
+// the same of up to 16 rows of a as bf16 (p.a and p.a_scales unused), quantised by rows on the way; out bf16
+constexpr uint32_t few_linear_rows = 16;
+bool few_linear(const Product &p, const void *x_bf16, cudaStream_t stream);
 
 }  // namespace k3::fp8

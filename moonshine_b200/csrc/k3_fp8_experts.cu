@@ -76,9 +76,22 @@ extern "C" bool k3_moe_fp8_linear(void *out, const void *x, const void *w, const
     Carve c{(char *)workspace};
     const Rows q(c, tokens, columns);
     if (workspace_bytes < c.total) return false;
+    Product p{};
+    p.out = out;
+    p.a = q.codes;
+    p.a_scales = q.scales;
+    p.b = w;
+    p.b_scales = w_scales;
+    p.groups = 1u;
+    p.rows = tokens;
+    p.n = rows;
+    p.k = columns;
+    p.b_scale_layout = K3_MOE_FP8_BLOCKS;
+    p.epilogue = kOutBf16;
+    p.b_ready = true;
+    if (tokens <= few_linear_rows) return few_linear(p, x, (cudaStream_t)stream);
     return k3_moe_fp8_quantize_rows(q.codes, q.scales, x, tokens, columns, K3_MOE_FP8_BF16, stream) &&
-           k3_moe_fp8_product(out, q.codes, q.scales, w, w_scales, tokens, rows, columns, K3_MOE_FP8_BLOCKS, K3_MOE_FP8_BF16, 0,
-                              stream);
+           product(p, (cudaStream_t)stream);
 }
 
 extern "C" size_t k3_moe_fp8_weight_gradient_workspace_bytes(uint32_t tokens, uint32_t rows, uint32_t columns) {

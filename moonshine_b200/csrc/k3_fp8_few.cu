@@ -13,8 +13,15 @@
 // Otherwise (grouped): one block per SM goes over items of 256 rows of b (kOutActivated: 128 of gate and
 // the same 128 of up) over the whole depth.
 //
+// kQuantize (a linear layer's call with up to 16 rows, split): a is bf16, and four more warps quantise the
+// part of its rows that a block needs, a block of 128 columns each, straight into the operand's place. Every
+// tile of b does so again, which is little beside the launch it saves.  For more rows that takes longer
+// than b: 47 rows of 7168 x 2048 18.2 us, against 12.3 with a launch of its own.
+// b_ready (split): the kernel in front, a quantiser, has waited for everything in front of it before it let
+// this one start, so b's first stages may be fetched while it runs.
+//
 // Warps: 0 loads by TMA, 1 MMA issuer and owner of the tensor memory, 2 factors, then four per 32 rows
-// of a with the running sums.  Every wait is bounded; on give-up the block raises the status word,
+// of a with the running sums, then the quantising ones.  Every wait is bounded; on give-up the block raises the status word,
 // waits for its copies and frees its tensor memory.
 #include "k3_fp8_ptx.cuh"
 #include "k3_grouped.h"
@@ -29,26 +36,30 @@ namespace {
 
 constexpr uint32_t kMaxGroups = 1024;
 constexpr uint32_t kMaxSplits = 8;                                   // of the depth: the portable cluster
-constexpr uint32_t kScaleSlots = 2, kSlotBlocks = 4;
 constexpr uint32_t kBoxRows = 16;                                    // a's rows per box: what an MMA column step is
 
 __device__ uint32_t g_fp8_few_status = 0;
 
-template <uint32_t kTiles, uint32_t kRows, bool kSplit>
+template <uint32_t kTiles, uint32_t kRows, bool kSplit, bool kQuantize>
 struct Layout {
+    static_assert(!kQuantize || (kSplit && kRows == 16u), "only a linear layer of few rows quantises here");
     static constexpr uint32_t kHalves = (kRows + 31u) / 32u;
-    static constexpr uint32_t kThreads = (4u + 4u * kHalves) * kWarp;
+    static constexpr uint32_t kSumWarps = 4u * kHalves, kQuantizeWarps = kQuantize ? 4u : 0u;
+    static constexpr uint32_t kThreads = (4u + kSumWarps + kQuantizeWarps) * kWarp;
+    static constexpr uint32_t kPerSm = kSplit ? 2u : 1u;
     static constexpr uint32_t kBTile = kBlock * kBlock;              // 128 rows of b, 128 columns
     static constexpr uint32_t kStageBytes = kTiles * kBTile + kRows * kBlock;
-    static constexpr uint32_t kStages = kSplit ? (kRows <= 16u ? 6u : 4u) : 5u;
-    static constexpr uint32_t kFactors = kStages * kStageBytes;      // f32 [slots][4 blocks][tiles][rows]
+    static constexpr uint32_t kStages = !kSplit ? 5u : kRows <= 16u ? 6u : 4u;
+    // factors travel four blocks at a time, or with the codes
+    static constexpr uint32_t kSlots = kQuantize ? 8u : 2u, kSlotBlocks = kQuantize ? 1u : 4u;
+    static constexpr uint32_t kFactors = kStages * kStageBytes;      // f32 [kSlots][kSlotBlocks][kTiles][kRows]
     static constexpr uint32_t kSlotFloats = kSlotBlocks * kTiles * kRows;
-    static constexpr uint32_t kLargest = kFactors + kScaleSlots * kSlotFloats * 4u;   // f32 bits [4][kRows]
+    static constexpr uint32_t kLargest = kFactors + kSlots * kSlotFloats * 4u;   // f32 bits [4][kRows]
     static constexpr uint32_t kPrefix = kLargest + 4u * kRows * 4u;
     static constexpr uint32_t kBars = (kPrefix + (kSplit ? 0u : (kMaxGroups + 1u) * 4u) + 15u) / 16u * 16u;
-    static constexpr uint32_t kBytes = kBars + 256u + 1024u;         // the last: alignment
+    static constexpr uint32_t kBytes = kBars + 512u + 1024u;         // the last: alignment
     static constexpr uint32_t kTmem = kTiles * kRows * 2u < 32u ? 32u : kTiles * kRows * 2u;
-    static_assert(kBytes <= (kSplit ? 115000u : 232448u), "two blocks of a split product share an SM");
+    static_assert(kBytes <= (kPerSm == 2u ? 115000u : 232448u), "two blocks of a split product share an SM");
     static_assert(!kSplit || kRows * kBlock * 4u <= kFactors, "partial sums take the ring's place");
 };
 
@@ -56,6 +67,9 @@ struct FewArgs {
     void *out;
     float *out_scales;
     const float *a_scales, *b_scales, *b2_scales;
+    const uint16_t *x;                             // kQuantize: a as bf16
+    bool x_vector;                                 // its rows are whole 16-byte units
+    bool b_ready;
     const uint32_t *offsets;
     uint32_t groups, rows, n, k;
     uint32_t column_items;                         // grouped: items along b's rows
@@ -84,20 +98,20 @@ K3_DEVINL void tmem_ld_wait_for(uint32_t (&r)[16]) {
                    "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 }
 
-template <int kEpilogue, uint32_t kTiles, uint32_t kRows, bool kSplit>
-__global__ void __launch_bounds__(Layout<kTiles, kRows, kSplit>::kThreads, kSplit ? 2 : 1)
+template <int kEpilogue, uint32_t kTiles, uint32_t kRows, bool kSplit, bool kQuantize>
+__global__ void __launch_bounds__(Layout<kTiles, kRows, kSplit, kQuantize>::kThreads, Layout<kTiles, kRows, kSplit, kQuantize>::kPerSm)
 fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                const __grid_constant__ CUtensorMap map_b2, FewArgs a) {
-    using L = Layout<kTiles, kRows, kSplit>;
+    using L = Layout<kTiles, kRows, kSplit, kQuantize>;
     extern __shared__ unsigned char smem_raw[];
     unsigned char *base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint64_t *full = reinterpret_cast<uint64_t *>(base + L::kBars);  // [kStages]
     uint64_t *empty = full + L::kStages;                             // [kStages]
     uint64_t *sum_full = empty + L::kStages;                         // [2] a block's products are in tensor memory
     uint64_t *sum_empty = sum_full + 2;                              // [2] and have been read
-    uint64_t *factor_full = sum_empty + 2;                           // [kScaleSlots]
-    uint64_t *factor_empty = factor_full + kScaleSlots;              // [kScaleSlots]
-    uint64_t *largest_full = factor_empty + kScaleSlots;             // [2] one per half
+    uint64_t *factor_full = sum_empty + 2;                           // [kSlots]
+    uint64_t *factor_empty = factor_full + L::kSlots;                // [kSlots]
+    uint64_t *largest_full = factor_empty + L::kSlots;               // [2] one per half
     uint64_t *done = largest_full + 2;                               // [1] every MMA issued has run
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 1);
     volatile uint32_t *abort_flag = tmem_slot + 1;
@@ -110,17 +124,17 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     if (threadIdx.x == 0) {
         *abort_flag = 0u;
         for (uint32_t s = 0; s < L::kStages; s++) {
-            mbar_init(&full[s], 1);
+            mbar_init(&full[s], kQuantize ? 2u : 1u);
             mbar_init(&empty[s], 1);
         }
         for (uint32_t s = 0; s < 2u; s++) {
             mbar_init(&sum_full[s], 1);
-            mbar_init(&sum_empty[s], 4u * L::kHalves);
+            mbar_init(&sum_empty[s], L::kSumWarps);
             mbar_init(&largest_full[s], 4);
         }
-        for (uint32_t s = 0; s < kScaleSlots; s++) {
-            mbar_init(&factor_full[s], kWarp);
-            mbar_init(&factor_empty[s], 4u * L::kHalves);
+        for (uint32_t s = 0; s < L::kSlots; s++) {
+            mbar_init(&factor_full[s], kQuantize ? 1u : kWarp);
+            mbar_init(&factor_empty[s], L::kSumWarps);
         }
         mbar_init(done, 1);
         fence_barrier_init();
@@ -129,7 +143,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         tmem_alloc(tmem_slot, L::kTmem);
         tmem_relinquish();
     }
-    pdl_wait();
+    if (!kSplit || warp != 0u) pdl_wait();         // split: the loading warp waits further down
     if (!kSplit && warp == 2u) {
         // exclusive prefix of the groups' row tiles, 32 groups at a time
         uint32_t before = 0u;
@@ -182,28 +196,40 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     if (warp == 0u) {
         // ----------------------------------------------------------------------------- loads
         if (elect_one()) {
-            prefetch_tensormap(&map_a);
+            if (!kQuantize) prefetch_tensormap(&map_a);
             prefetch_tensormap(&map_b);
             if (kEpilogue == kOutActivated) prefetch_tensormap(&map_b2);
             const uint64_t stream_once = l2_policy_evict_first();
-            uint32_t s = 0u, ph = 0u, issued = 0u;
+            uint32_t s = 0u, ph = 0u, issued = 0u, early = 0u;
+            auto load_b = [&](const Item &it, uint32_t stage, uint32_t kb) {
+                unsigned char *st = base + stage * L::kStageBytes;
+                const int32_t x = (int32_t)(kb * kBlock), y = (int32_t)(it.group * a.n + it.column);
+                const uint32_t boxes = kQuantize ? 0u : (it.rows + kBoxRows - 1u) / kBoxRows;
+                mbar_arrive_expect_tx(&full[stage], kTiles * L::kBTile + boxes * kBoxRows * kBlock);
+                tma_load_2d_hint(st, &map_b, &full[stage], x, y, stream_once);
+                if (kTiles == 2u) {
+                    if (kEpilogue == kOutActivated) tma_load_2d_hint(st + L::kBTile, &map_b2, &full[stage], x, y, stream_once);
+                    else tma_load_2d_hint(st + L::kBTile, &map_b, &full[stage], x, y + (int32_t)kBlock, stream_once);
+                }
+            };
+            if (kSplit) {
+                if (a.b_ready) {
+                    const Item it = item_of(0u);
+                    early = min(L::kStages, it.kb_end - it.kb_begin);
+                    for (uint32_t i = 0; i < early; i++) load_b(it, i, it.kb_begin + i);
+                }
+                pdl_wait();
+            }
             bool ok = true;
             for (uint32_t w = first_item; ok && w < total; w += step) {
                 const Item it = item_of(w);
-                const int32_t y = (int32_t)(it.group * a.n + it.column);
                 const uint32_t boxes = (it.rows + kBoxRows - 1u) / kBoxRows;
                 for (uint32_t kb = it.kb_begin; kb < it.kb_end; kb++) {
                     if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag)) { ok = false; break; }
-                    unsigned char *st = base + s * L::kStageBytes;
-                    const int32_t x = (int32_t)(kb * kBlock);
-                    mbar_arrive_expect_tx(&full[s], kTiles * L::kBTile + boxes * kBoxRows * kBlock);
-                    tma_load_2d_hint(st, &map_b, &full[s], x, y, stream_once);
-                    if (kTiles == 2u) {
-                        if (kEpilogue == kOutActivated) tma_load_2d_hint(st + L::kBTile, &map_b2, &full[s], x, y, stream_once);
-                        else tma_load_2d_hint(st + L::kBTile, &map_b, &full[s], x, y + (int32_t)kBlock, stream_once);
-                    }
-                    for (uint32_t i = 0; i < boxes; i++) {
-                        tma_load_2d(st + kTiles * L::kBTile + i * kBoxRows * kBlock, &map_a, &full[s], x,
+                    if (issued >= early) load_b(it, s, kb);
+                    unsigned char *rows = base + s * L::kStageBytes + kTiles * L::kBTile;
+                    for (uint32_t i = 0; !kQuantize && i < boxes; i++) {
+                        tma_load_2d(rows + i * kBoxRows * kBlock, &map_a, &full[s], (int32_t)(kb * kBlock),
                                     (int32_t)(it.row + i * kBoxRows));
                     }
                     issued++;
@@ -251,7 +277,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 mbar_drain(done, 0u);
             }
         }
-    } else if (warp == 2u) {
+    } else if (warp == 2u && !kQuantize) {
         // --------------------------------------------------------------- factors, a slot at a time
         uint32_t slot = 0u, ph = 0u;
         bool ok = true;
@@ -264,7 +290,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 b_row[1] = kEpilogue == kOutActivated ? a.b2_scales + sb
                            : it.column / kBlock + 1u < b_blocks ? b_row[0] + blocks : b_row[0];
             }
-            for (uint32_t kb = it.kb_begin; kb < it.kb_end; kb += kSlotBlocks) {
+            for (uint32_t kb = it.kb_begin; kb < it.kb_end; kb += L::kSlotBlocks) {
                 float f[kTiles][4];
 #pragma unroll
                 for (uint32_t t = 0; t < kTiles; t++) {
@@ -291,7 +317,67 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     }
                 }
                 mbar_arrive(&factor_full[slot]);
-                if (++slot == kScaleSlots) { slot = 0u; ph ^= 1u; }
+                if (++slot == L::kSlots) { slot = 0u; ph ^= 1u; }
+            }
+        }
+    } else if (kQuantize && warp >= 4u + L::kSumWarps) {
+        // ------------------ a's rows: a warp takes every fourth block of 128 columns, eight lanes a row's
+        const Item it = item_of(0u);
+        const uint32_t mine = warp - 4u - L::kSumWarps, in_pass = lane / 8u, first = lane % 8u * 16u;
+        const float *sb = a.b_scales + (uint64_t)(it.column / kBlock) * blocks;
+        for (uint32_t kb = it.kb_begin + mine; kb < it.kb_end; kb += L::kQuantizeWarps) {
+            const uint32_t at = kb - it.kb_begin, s = at % L::kStages, slot = at % L::kSlots;
+            uint32_t v[4][8];                                        // 16 bf16 of each of four rows
+#pragma unroll
+            for (uint32_t p = 0; p < 4u; p++) {
+                const uint32_t row = p * 4u + in_pass, c = kb * kBlock + first;
+                const uint16_t *from = a.x + (uint64_t)(it.row + row) * a.k + c;
+#pragma unroll
+                for (uint32_t h = 0; h < 2u; h++) {
+                    uint4 q = make_uint4(0u, 0u, 0u, 0u);
+                    if (a.x_vector) {
+                        if (row < it.rows && c + h * 8u < a.k) q = *reinterpret_cast<const uint4 *>(from + h * 8u);
+                    } else if (row < it.rows) {
+                        uint32_t e[8];
+#pragma unroll
+                        for (uint32_t i = 0; i < 8u; i++) e[i] = c + h * 8u + i < a.k ? from[h * 8u + i] : 0u;
+                        q = make_uint4(e[0] | (e[1] << 16), e[2] | (e[3] << 16), e[4] | (e[5] << 16), e[6] | (e[7] << 16));
+                    }
+                    v[p][h * 4u] = q.x; v[p][h * 4u + 1u] = q.y; v[p][h * 4u + 2u] = q.z; v[p][h * 4u + 3u] = q.w;
+                }
+            }
+            const float by = sb[kb];
+            if (!mbar_wait(&empty[s], (at / L::kStages & 1u) ^ 1u, abort_flag) ||
+                !mbar_wait(&factor_empty[slot], (at / L::kSlots & 1u) ^ 1u, abort_flag)) {
+                break;
+            }
+            unsigned char *to = base + s * L::kStageBytes + kTiles * L::kBTile;
+            float *factors = reinterpret_cast<float *>(base + L::kFactors) + slot * L::kSlotFloats;
+#pragma unroll
+            for (uint32_t p = 0; p < 4u; p++) {
+                if (p * 4u >= it.rows) break;                         // what rows past the end hold is not kept
+                uint32_t most = 0u;
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; i++) most = max(most, max((v[p][i] << 16) & 0x7fffffffu, v[p][i] & 0x7fff0000u));
+#pragma unroll
+                for (int o = 4; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+                const float scale = scale_of(most), inverse = __frcp_rn(scale);
+                uint32_t w[4];
+#pragma unroll
+                for (uint32_t i = 0; i < 4u; i++) {
+                    const uint32_t x = v[p][2u * i], y = v[p][2u * i + 1u];
+                    w[i] = codes2(quotient(bf16_lo(x), scale, inverse), quotient(bf16_hi(x), scale, inverse)) |
+                           (codes2(quotient(bf16_lo(y), scale, inverse), quotient(bf16_hi(y), scale, inverse)) << 16);
+                }
+                const uint32_t row = p * 4u + in_pass;                // 128-byte rows, 16-byte units swizzled as TMA does
+                *reinterpret_cast<uint4 *>(to + row * kBlock + ((lane % 8u) ^ (row % 8u)) * 16u) = make_uint4(w[0], w[1], w[2], w[3]);
+                if (lane % 8u == 0u) factors[row] = scale * by;
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0u) {
+                mbar_arrive(&full[s]);
+                mbar_arrive(&factor_full[slot]);
             }
         }
     } else if (warp >= 4u) {
@@ -311,7 +397,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 for (uint32_t j = 0; j < kMine / 2u; j++) sum[t][j] = 0ull;
             }
             for (uint32_t kb = it.kb_begin; kb < it.kb_end; kb++) {
-                const uint32_t in_slot = (kb - it.kb_begin) % kSlotBlocks;
+                const uint32_t in_slot = (kb - it.kb_begin) % L::kSlotBlocks;
                 if ((in_slot == 0u && !mbar_wait(&factor_full[slot], sph, abort_flag)) || !mbar_wait(&sum_full[at], aph, abort_flag)) {
                     ok = false;
                     break;
@@ -353,10 +439,10 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     }
                 }
                 if (++at == 2u) { at = 0u; aph ^= 1u; }
-                if (in_slot == kSlotBlocks - 1u || kb + 1u == it.kb_end) {
+                if (in_slot == L::kSlotBlocks - 1u || kb + 1u == it.kb_end) {
                     __syncwarp();
                     if (lane == 0u) mbar_arrive(&factor_empty[slot]);
-                    if (++slot == kScaleSlots) { slot = 0u; sph ^= 1u; }
+                    if (++slot == L::kSlots) { slot = 0u; sph ^= 1u; }
                 }
             }
             if (!ok) break;
@@ -482,20 +568,23 @@ FewArgs args_of(const Product &p) {
     return a;
 }
 
-template <int kEpilogue, uint32_t kRows>
-bool launch_split(const Product &p, cudaStream_t stream) {
-    using L = Layout<1, kRows, true>;
-    CUtensorMap a_map, b_map;
-    if (!map_codes(&a_map, p.a, p.rows, p.k, kBoxRows) || !map_codes(&b_map, p.b, p.n, p.k, kBlock)) return false;
+template <int kEpilogue, uint32_t kRows, bool kQuantize>
+bool launch_split(const Product &p, const void *x, bool b_ready, cudaStream_t stream) {
+    using L = Layout<1, kRows, true, kQuantize>;
+    CUtensorMap a_map{}, b_map;
+    if ((!kQuantize && !map_codes(&a_map, p.a, p.rows, p.k, kBoxRows)) || !map_codes(&b_map, p.b, p.n, p.k, kBlock)) return false;
     FewArgs a = args_of(p);
+    a.x = (const uint16_t *)x;
+    a.x_vector = aligned16(x) && p.k % 8u == 0u;
+    a.b_ready = b_ready;
     const uint32_t tiles = blocks_of(p.n), row_tiles = (p.rows + kRows - 1u) / kRows, blocks = blocks_of(p.k);
     if (tiles > 65535u || row_tiles > 65535u) return false;
-    // as many parts as the SMs hold at two blocks each, with two blocks of 128 in a part at least
-    const uint32_t room = (uint32_t)sm_count() * 2u / std::max(1u, tiles * row_tiles);
+    // as many parts as the SMs hold, with two blocks of 128 in a part at least
+    const uint32_t room = (uint32_t)sm_count() * L::kPerSm / std::max(1u, tiles * row_tiles);
     const uint32_t splits = std::max(1u, std::min({kMaxSplits, room, blocks / 2u}));
     a.split_blocks = (blocks + splits - 1u) / splits;
     const uint32_t parts = (blocks + a.split_blocks - 1u) / a.split_blocks;
-    auto kernel = fp8_few_kernel<kEpilogue, 1, kRows, true>;
+    auto kernel = fp8_few_kernel<kEpilogue, 1, kRows, true, kQuantize>;
     if (!set_max_dynamic_smem((const void *)kernel, L::kBytes)) return false;
     return launch_chained_cluster(kernel, dim3(parts, tiles, row_tiles), L::kThreads, dim3(parts, 1, 1), L::kBytes, stream, a_map,
                                   b_map, b_map, a);
@@ -504,7 +593,7 @@ bool launch_split(const Product &p, cudaStream_t stream) {
 template <int kEpilogue>
 bool launch_grouped(const Product &p, cudaStream_t stream) {
     constexpr uint32_t kRows = few_rows, kColumns = kEpilogue == kOutActivated ? kBlock : 2u * kBlock;
-    using L = Layout<2, kRows, false>;
+    using L = Layout<2, kRows, false, false>;
     CUtensorMap a_map, b_map, b2_map;
     const uint64_t b_rows = (uint64_t)p.groups * p.n;
     if (!map_codes(&a_map, p.a, p.rows, p.k, kBoxRows) || !map_codes(&b_map, p.b, b_rows, p.k, kBlock) ||
@@ -515,7 +604,7 @@ bool launch_grouped(const Product &p, cudaStream_t stream) {
     a.column_items = (p.n + kColumns - 1u) / kColumns;
     const uint64_t items = ((uint64_t)(p.rows + kRows - 1u) / kRows + p.groups) * a.column_items;
     if (items > 0x7fffffffull) return false;
-    auto kernel = fp8_few_kernel<kEpilogue, 2, kRows, false>;
+    auto kernel = fp8_few_kernel<kEpilogue, 2, kRows, false, false>;
     return set_max_dynamic_smem((const void *)kernel, L::kBytes) &&
            launch_chained(kernel, (uint32_t)std::min<uint64_t>(items, sm_count()), L::kThreads, L::kBytes, stream, a_map, b_map,
                           b2_map, a);
@@ -529,8 +618,16 @@ bool k3::fp8::few_product(const Product &p, cudaStream_t stream) {
                : p.epilogue == kOutF32     ? launch_grouped<kOutF32>(p, stream)
                                            : launch_grouped<kOutBf16>(p, stream);
     }
-    if (p.rows <= 16u) return p.epilogue == kOutF32 ? launch_split<kOutF32, 16>(p, stream) : launch_split<kOutBf16, 16>(p, stream);
-    return p.epilogue == kOutF32 ? launch_split<kOutF32, few_rows>(p, stream) : launch_split<kOutBf16, few_rows>(p, stream);
+    if (p.rows <= 16u) {
+        return p.epilogue == kOutF32 ? launch_split<kOutF32, 16, false>(p, nullptr, p.b_ready, stream)
+                                     : launch_split<kOutBf16, 16, false>(p, nullptr, p.b_ready, stream);
+    }
+    return p.epilogue == kOutF32 ? launch_split<kOutF32, few_rows, false>(p, nullptr, p.b_ready, stream)
+                                 : launch_split<kOutBf16, few_rows, false>(p, nullptr, p.b_ready, stream);
+}
+
+bool k3::fp8::few_linear(const Product &p, const void *x_bf16, cudaStream_t stream) {
+    return launch_split<kOutBf16, 16, true>(p, x_bf16, false, stream);
 }
 
 uint32_t k3_fp8_few_status() {

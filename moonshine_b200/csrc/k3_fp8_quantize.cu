@@ -100,6 +100,7 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(RowsArgs a) {
     for (int b = 0; b < 4; b++) {
         load8<kF32, kVector>(bits[b], x, (group * 4u + b) * kBlock + l * 8u, live ? a.columns : 0u);
     }
+    pdl_trigger();                   // a product behind may fetch its table now (Product::b_ready)
     float scale[4];
     uint2 out[4];
 #pragma unroll

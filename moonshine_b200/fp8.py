@@ -43,10 +43,11 @@ def _done(ok: bool, name: str) -> None:
 
 
 def _matrix(x: torch.Tensor, name: str, columns: int | None = None, dtypes=(torch.bfloat16,)) -> tuple[int, int]:
-    if x.dim() != 2 or x.dtype not in dtypes or (columns is not None and x.shape[1] != columns):
+    shape = x.shape
+    if len(shape) != 2 or x.dtype not in dtypes or (columns is not None and shape[1] != columns):
         raise ValueError(f"{name}: expected [rows, {columns if columns is not None else 'columns'}] of "
-                         f"{' or '.join(str(d) for d in dtypes)}, got {list(x.shape)} {x.dtype}")
-    return x.shape[0], x.shape[1]
+                         f"{' or '.join(str(d) for d in dtypes)}, got {list(shape)} {x.dtype}")
+    return shape
 
 
 def _table(codes: torch.Tensor, scales: torch.Tensor, lead: tuple, rows: int, columns: int, name: str) -> None:
@@ -58,28 +59,29 @@ def _table(codes: torch.Tensor, scales: torch.Tensor, lead: tuple, rows: int, co
 
 
 def _quantized(name: str, x: torch.Tensor, codes_shape: tuple, scales_shape: tuple):
-    codes = torch.empty(codes_shape, dtype=torch.float8_e4m3fn, device=x.device)
-    scales = torch.empty(scales_shape, dtype=torch.float32, device=x.device)
-    if x.numel():
-        _done(getattr(ops, name)(codes, scales, x, x.shape[0], x.shape[1], _TYPES[x.dtype]), name)
+    codes = x.new_empty(codes_shape, dtype=torch.float8_e4m3fn)
+    scales = x.new_empty(scales_shape, dtype=torch.float32)
+    rows, columns = x.shape
+    if rows and columns:
+        _done(getattr(ops, name)(codes, scales, x, rows, columns, _TYPES[x.dtype]), name)
     return codes, scales
 
 
 def quantize_rows(x: torch.Tensor):
     """bf16 or f32 [rows, columns] -> codes [rows, pitch(columns)], scales [rows, scale_pitch(columns)]."""
-    rows, columns = _matrix(x, "x", dtypes=tuple(_TYPES))
+    rows, columns = _matrix(x, "x", dtypes=_TYPES)
     return _quantized("k3_moe_fp8_quantize_rows", x, (rows, pitch(columns)), (rows, scale_pitch(columns)))
 
 
 def quantize_columns(x: torch.Tensor):
     """The same of x transposed: codes [columns, pitch(rows)], scales [columns, scale_pitch(rows)]."""
-    rows, columns = _matrix(x, "x", dtypes=tuple(_TYPES))
+    rows, columns = _matrix(x, "x", dtypes=_TYPES)
     return _quantized("k3_moe_fp8_quantize_columns", x, (columns, pitch(rows)), (columns, scale_pitch(rows)))
 
 
 def quantize_blocks(x: torch.Tensor):
     """A weight table: codes [rows, pitch(columns)], scales [blocks(rows), blocks(columns)]."""
-    rows, columns = _matrix(x, "x", dtypes=tuple(_TYPES))
+    rows, columns = _matrix(x, "x", dtypes=_TYPES)
     return _quantized("k3_moe_fp8_quantize_blocks", x, (rows, pitch(columns)), (blocks(rows), blocks(columns)))
 
 
@@ -125,7 +127,7 @@ class Fp8Linear:
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         """x bf16 [tokens, columns] -> bf16 [tokens, rows]."""
         tokens, _ = _matrix(x, "x", self.columns)
-        out = torch.empty((tokens, self.rows), dtype=torch.bfloat16, device=x.device)
+        out = x.new_empty((tokens, self.rows))
         if tokens:
             ws = self._workspace.of(tokens, x.device)
             _done(ops.k3_moe_fp8_linear(out, x, self.codes, self.scales, tokens, self.rows, self.columns, ws, self._workspace.bytes),
@@ -192,11 +194,11 @@ class Fp8Experts:
         ``shared`` (bf16, the shared expert's output) if given."""
         tokens, _ = _matrix(x, "x", self.hidden)
         for name, t, dtype in (("ids", ids, torch.int32), ("weights", weights, torch.float32)):
-            if t.dtype != dtype or tuple(t.shape) != (tokens, self.top_k):
+            if t.dtype is not dtype or t.shape != (tokens, self.top_k):
                 raise ValueError(f"{name}: expected {dtype} {[tokens, self.top_k]}, got {t.dtype} {list(t.shape)}")
         if shared is not None and _matrix(shared, "shared", self.hidden)[0] != tokens:
             raise ValueError("shared: another number of tokens than x")
-        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        out = x.new_empty((tokens, self.hidden))
         if tokens:
             ws = self._workspace.of(tokens, x.device)
             _done(ops.k3_moe_fp8_experts_forward(self.desc, out, x, ids, weights, shared, tokens, ws, self._workspace.bytes),

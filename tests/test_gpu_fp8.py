@@ -210,6 +210,23 @@ def test_linear_and_its_gradients(tokens, rows, columns):
     assert abs(float((dw.cpu().double() * dw_dir).sum()) - by_w) <= noise(dy.cpu().double().t(), x64, dw_dir)
 
 
+@pytest.mark.parametrize("start", [0, 1])
+@pytest.mark.parametrize("tokens,rows,columns", [(1, 1, 1), (1, 3584, 7168), (2, 130, 1001), (15, 300, 640), (16, 2048, 136), (17, 129, 1000),
+                                                 (33, 512, 2048), (63, 260, 131), (64, 7168, 2048)])
+def test_linear_of_few_tokens(tokens, rows, columns, start):
+    """Tokens quantised inside the product; `start`: from a place between 16-byte boundaries."""
+    x = normal(tokens, tokens * columns + 1).cuda()[start:][:tokens * columns].view(tokens, columns)
+    x[:, ::7] *= 50
+    table, scales = fp8.quantize_blocks(normal(3, rows, columns, scale=0.02).cuda())
+    dirty(table, columns)
+    w = R.values(table.view(torch.uint8)[:, :columns].cpu().view(E4M3), scales.cpu(), R.BLOCK)
+    xv = R.values(*R.quantize(x.cpu(), 1), 1)
+    lin = fp8.Fp8Linear(table, scales, rows, columns)
+    y = lin.forward(x)
+    assert bool(((y.cpu().double() - xv @ w.t()).abs() <= bound(xv, w, columns, xv @ w.t())).all())
+    assert torch.equal(y, lin.forward(x))
+
+
 def expert_tables(seed, experts, hidden, expert_hidden):
     made = []
     for i, (r, c) in enumerate(((expert_hidden, hidden), (expert_hidden, hidden), (hidden, expert_hidden))):
