@@ -100,7 +100,7 @@ K3_DEVINL uint2 ld_stream_8(const void *p) {
 K3_DEVINL void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 K3_DEVINL void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// Thread block clusters: this block's place, the barrier of all its threads (release / acquire), and an f32 at
+// Thread block clusters: this block's place, the barrier of all its threads (release / acquire), and f32 at
 // the same place of another block's shared memory.
 K3_DEVINL uint32_t cluster_rank() {
     uint32_t r;
@@ -120,6 +120,14 @@ K3_DEVINL float cluster_load(const float *mine, uint32_t rank) {
     float v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"((uint32_t)__cvta_generic_to_shared(mine)), "r"(rank));
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+K3_DEVINL float4 cluster_load4(const float *mine, uint32_t rank) {
+    uint32_t addr;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"((uint32_t)__cvta_generic_to_shared(mine)), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
     return v;
 }
 

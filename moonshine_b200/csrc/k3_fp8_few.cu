@@ -121,52 +121,6 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     const uint32_t blocks = blocks_of(a.k);
     constexpr uint32_t kColumns = kEpilogue == kOutActivated ? kBlock : kTiles * kBlock;
 
-    if (threadIdx.x == 0) {
-        *abort_flag = 0u;
-        for (uint32_t s = 0; s < L::kStages; s++) {
-            mbar_init(&full[s], kQuantize ? 2u : 1u);
-            mbar_init(&empty[s], 1);
-        }
-        for (uint32_t s = 0; s < 2u; s++) {
-            mbar_init(&sum_full[s], 1);
-            mbar_init(&sum_empty[s], L::kSumWarps);
-            mbar_init(&largest_full[s], 4);
-        }
-        for (uint32_t s = 0; s < L::kSlots; s++) {
-            mbar_init(&factor_full[s], kQuantize ? 1u : kWarp);
-            mbar_init(&factor_empty[s], L::kSumWarps);
-        }
-        mbar_init(done, 1);
-        fence_barrier_init();
-    }
-    if (warp == 1u) {
-        tmem_alloc(tmem_slot, L::kTmem);
-        tmem_relinquish();
-    }
-    if (!kSplit || warp != 0u) pdl_wait();         // split: the loading warp waits further down
-    if (!kSplit && warp == 2u) {
-        // exclusive prefix of the groups' row tiles, 32 groups at a time
-        uint32_t before = 0u;
-        for (uint32_t g0 = 0; g0 < a.groups; g0 += kWarp) {
-            const uint32_t g = g0 + lane;
-            const uint32_t n = g < a.groups ? (a.offsets[g + 1u] - a.offsets[g] + kRows - 1u) / kRows : 0u;
-            uint32_t scan = n;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t up = __shfl_up_sync(0xffffffffu, scan, o);
-                if (lane >= (uint32_t)o) scan += up;
-            }
-            if (g < a.groups) prefix[g] = before + scan - n;
-            before += __shfl_sync(0xffffffffu, scan, 31);
-        }
-        if (lane == 0u) *total_s = before * a.column_items;
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
-    const uint32_t first_item = kSplit ? 0u : blockIdx.x, step = kSplit ? 1u : gridDim.x, total = kSplit ? 1u : *total_s;
-
     auto item_of = [&](uint32_t w) {
         Item it;
         it.kb_begin = 0u;
@@ -193,40 +147,85 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         return it;
     };
 
+    const uint64_t stream_once = l2_policy_evict_first();
+    auto load_b = [&](const Item &it, uint32_t stage, uint32_t kb) {
+        unsigned char *st = base + stage * L::kStageBytes;
+        const int32_t x = (int32_t)(kb * kBlock), y = (int32_t)(it.group * a.n + it.column);
+        const uint32_t boxes = kQuantize ? 0u : (it.rows + kBoxRows - 1u) / kBoxRows;
+        mbar_arrive_expect_tx(&full[stage], kTiles * L::kBTile + boxes * kBoxRows * kBlock);
+        tma_load_2d_hint(st, &map_b, &full[stage], x, y, stream_once);
+        if (kTiles == 2u) {
+            if (kEpilogue == kOutActivated) tma_load_2d_hint(st + L::kBTile, &map_b2, &full[stage], x, y, stream_once);
+            else tma_load_2d_hint(st + L::kBTile, &map_b, &full[stage], x, y + (int32_t)kBlock, stream_once);
+        }
+    };
+
+    if (warp == 0u && elect_one()) {
+        *abort_flag = 0u;
+        for (uint32_t s = 0; s < L::kStages; s++) {
+            mbar_init(&full[s], kQuantize ? 2u : 1u);
+            mbar_init(&empty[s], 1);
+        }
+        for (uint32_t s = 0; s < 2u; s++) {
+            mbar_init(&sum_full[s], 1);
+            mbar_init(&sum_empty[s], L::kSumWarps);
+            mbar_init(&largest_full[s], 4);
+        }
+        for (uint32_t s = 0; s < L::kSlots; s++) {
+            mbar_init(&factor_full[s], kQuantize ? 1u : kWarp);
+            mbar_init(&factor_empty[s], L::kSumWarps);
+        }
+        mbar_init(done, 1);
+        fence_barrier_init();
+        prefetch_tensormap(&map_b);
+        if (kEpilogue == kOutActivated) prefetch_tensormap(&map_b2);
+        if (!kQuantize) prefetch_tensormap(&map_a);
+        if (kSplit) {                                                // b's first stages, before anyone waits for anyone
+            if (!a.b_ready) pdl_wait();
+            const Item it = item_of(0u);
+            for (uint32_t i = 0; i < min(L::kStages, it.kb_end - it.kb_begin); i++) load_b(it, i, it.kb_begin + i);
+            pdl_wait();
+        }
+    }
+    if (warp == 1u) {
+        tmem_alloc(tmem_slot, L::kTmem);
+        tmem_relinquish();
+    }
+    if (!kSplit || warp != 0u) pdl_wait();
+    if (!kSplit && warp == 2u) {
+        // exclusive prefix of the groups' row tiles, 32 groups at a time
+        uint32_t before = 0u;
+        for (uint32_t g0 = 0; g0 < a.groups; g0 += kWarp) {
+            const uint32_t g = g0 + lane;
+            const uint32_t n = g < a.groups ? (a.offsets[g + 1u] - a.offsets[g] + kRows - 1u) / kRows : 0u;
+            uint32_t scan = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t up = __shfl_up_sync(0xffffffffu, scan, o);
+                if (lane >= (uint32_t)o) scan += up;
+            }
+            if (g < a.groups) prefix[g] = before + scan - n;
+            before += __shfl_sync(0xffffffffu, scan, 31);
+        }
+        if (lane == 0u) *total_s = before * a.column_items;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t first_item = kSplit ? 0u : blockIdx.x, step = kSplit ? 1u : gridDim.x, total = kSplit ? 1u : *total_s;
+
     if (warp == 0u) {
         // ----------------------------------------------------------------------------- loads
         if (elect_one()) {
-            if (!kQuantize) prefetch_tensormap(&map_a);
-            prefetch_tensormap(&map_b);
-            if (kEpilogue == kOutActivated) prefetch_tensormap(&map_b2);
-            const uint64_t stream_once = l2_policy_evict_first();
-            uint32_t s = 0u, ph = 0u, issued = 0u, early = 0u;
-            auto load_b = [&](const Item &it, uint32_t stage, uint32_t kb) {
-                unsigned char *st = base + stage * L::kStageBytes;
-                const int32_t x = (int32_t)(kb * kBlock), y = (int32_t)(it.group * a.n + it.column);
-                const uint32_t boxes = kQuantize ? 0u : (it.rows + kBoxRows - 1u) / kBoxRows;
-                mbar_arrive_expect_tx(&full[stage], kTiles * L::kBTile + boxes * kBoxRows * kBlock);
-                tma_load_2d_hint(st, &map_b, &full[stage], x, y, stream_once);
-                if (kTiles == 2u) {
-                    if (kEpilogue == kOutActivated) tma_load_2d_hint(st + L::kBTile, &map_b2, &full[stage], x, y, stream_once);
-                    else tma_load_2d_hint(st + L::kBTile, &map_b, &full[stage], x, y + (int32_t)kBlock, stream_once);
-                }
-            };
-            if (kSplit) {
-                if (a.b_ready) {
-                    const Item it = item_of(0u);
-                    early = min(L::kStages, it.kb_end - it.kb_begin);
-                    for (uint32_t i = 0; i < early; i++) load_b(it, i, it.kb_begin + i);
-                }
-                pdl_wait();
-            }
+            uint32_t s = 0u, ph = 0u, issued = 0u;
             bool ok = true;
             for (uint32_t w = first_item; ok && w < total; w += step) {
                 const Item it = item_of(w);
                 const uint32_t boxes = (it.rows + kBoxRows - 1u) / kBoxRows;
                 for (uint32_t kb = it.kb_begin; kb < it.kb_end; kb++) {
                     if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag)) { ok = false; break; }
-                    if (issued >= early) load_b(it, s, kb);
+                    if (!kSplit || issued >= L::kStages) load_b(it, s, kb);
                     unsigned char *rows = base + s * L::kStageBytes + kTiles * L::kBTile;
                     for (uint32_t i = 0; !kQuantize && i < boxes; i++) {
                         tma_load_2d(rows + i * kBoxRows * kBlock, &map_a, &full[s], (int32_t)(kb * kBlock),
@@ -236,7 +235,9 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     if (++s == L::kStages) { s = 0u; ph ^= 1u; }
                 }
             }
+            if (kSplit) pdl_trigger();                               // the blocks of the next kernel may take places as these leave
             if (*abort_flag != 0u) {                                 // nothing may land in a block that has left
+                if (kSplit) issued = max(issued, min(L::kStages, blocks));
                 for (uint32_t i = issued > L::kStages ? issued - L::kStages : 0u; i < issued; i++) {
                     mbar_drain(&full[i % L::kStages], (i / L::kStages) & 1u);
                 }
@@ -514,26 +515,50 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         __syncthreads();
         cluster_barrier();
         const Item it = item_of(0u);
-        const uint32_t size = cluster_size(), all = it.rows * kBlock;
+        const uint32_t size = cluster_size(), all = it.rows * (kBlock / 4u);        // four columns at a time
         const uint32_t share = (all + size - 1u) / size, begin = cluster_rank() * share, end = min(all, begin + share);
         const float *part = reinterpret_cast<const float *>(base);
+        const bool vector = a.n % 4u == 0u && ((uintptr_t)a.out & (kEpilogue == kOutF32 ? 15u : 7u)) == 0u;
         for (uint32_t e = begin + threadIdx.x; e < end; e += L::kThreads) {
-            float v[kMaxSplits];
+            float4 v[kMaxSplits];
 #pragma unroll
-            for (uint32_t r = 0; r < kMaxSplits; r++) v[r] = r < size ? cluster_load(part + e, r) : 0.f;
-            float sum = v[0];
+            for (uint32_t r = 0; r < kMaxSplits; r++) v[r] = r < size ? cluster_load4(part + e * 4u, r) : make_float4(0.f, 0.f, 0.f, 0.f);
+            float sum[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
 #pragma unroll
             for (uint32_t r = 1; r < kMaxSplits; r++) {
-                if (r < size) sum += v[r];
+                if (r < size) {
+                    sum[0] += v[r].x;
+                    sum[1] += v[r].y;
+                    sum[2] += v[r].z;
+                    sum[3] += v[r].w;
+                }
             }
-            const uint32_t c = it.column + e % kBlock;
-            if (c < a.n) {
-                const uint64_t to = (uint64_t)(it.row + e / kBlock) * a.n + c;
-                if (kEpilogue == kOutF32) {
-                    float *out = (float *)a.out + to;
-                    *out = a.accumulate ? *out + sum : sum;
+            const uint32_t c = it.column + e % (kBlock / 4u) * 4u;
+            if (c >= a.n) continue;
+            const uint64_t to = (uint64_t)(it.row + e / (kBlock / 4u)) * a.n + c;
+            if (kEpilogue == kOutF32) {
+                float *out = (float *)a.out + to;
+#pragma unroll
+                for (uint32_t j = 0; j < 4u; j++) {
+                    if (a.accumulate && c + j < a.n) sum[j] += out[j];
+                }
+                if (vector) {
+                    *reinterpret_cast<float4 *>(out) = make_float4(sum[0], sum[1], sum[2], sum[3]);
                 } else {
-                    ((uint16_t *)a.out)[to] = float_to_bf16_bits(sum);
+#pragma unroll
+                    for (uint32_t j = 0; j < 4u; j++) {
+                        if (c + j < a.n) out[j] = sum[j];
+                    }
+                }
+            } else {
+                uint16_t *out = (uint16_t *)a.out + to;
+                if (vector) {
+                    *reinterpret_cast<uint2 *>(out) = make_uint2(bf16x2(sum[0], sum[1]), bf16x2(sum[2], sum[3]));
+                } else {
+#pragma unroll
+                    for (uint32_t j = 0; j < 4u; j++) {
+                        if (c + j < a.n) out[j] = float_to_bf16_bits(sum[j]);
+                    }
                 }
             }
         }
