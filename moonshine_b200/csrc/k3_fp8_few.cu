@@ -464,7 +464,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 for (uint32_t j = 0; j < kMine; j++) {
                     act[j] = 0.f;
                     if (j < n) {
-                        if (inside) act[j] = activation(value(0u, j), value(kTiles - 1u, j), a.activation, a.beta, a.linear_beta);
+                        if (inside) act[j] = activated(value(0u, j), value(kTiles - 1u, j), a.activation, a.beta, a.linear_beta);
                         const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(act[j]) & 0x7fffffffu);
                         if (lane == 0u) largest[q * kRows + j] = most;
                     }

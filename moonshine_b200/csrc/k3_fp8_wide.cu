@@ -205,7 +205,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 bool ok = true;
                 for (uint32_t w = blockIdx.x; ok && w < total; w += gridDim.x) {
                     for (uint32_t kb = 0; kb < blocks; kb++) {
-                        if (!mbar_wait(&sum_empty[at], aph ^ 1u, abort_flag) || !mbar_wait(&full[s], ph, abort_flag)) {
+                        if (!mbar_wait(&full[s], ph, abort_flag) || !mbar_wait(&sum_empty[at], aph ^ 1u, abort_flag)) {
                             ok = false;
                             break;
                         }
@@ -356,7 +356,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                     for (uint32_t p = 0; p < 2u; p++) {
                         const float g = p ? hi2(sum[j]) : lo2(sum[j]), u = p ? hi2(sum[32u + j]) : lo2(sum[32u + j]);
                         const bool inside = it.column + first + 2u * j + p < a.n;
-                        v[p] = inside ? activation(g, u, a.activation, a.beta, a.linear_beta) : 0.f;
+                        v[p] = inside ? activated(g, u, a.activation, a.beta, a.linear_beta) : 0.f;
                         most = max(most, __float_as_uint(v[p]) & 0x7fffffffu);
                     }
                     sum[j] = pack2(v[0], v[1]);
