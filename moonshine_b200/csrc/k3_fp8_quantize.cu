@@ -21,55 +21,64 @@ namespace {
 
 constexpr uint32_t kThreads = 256;
 
-K3_DEVINL uint2 codes8(const uint32_t (&bits)[8], float scale, float inverse) {
-    uint32_t h[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        h[i] = codes2(quotient(__uint_as_float(bits[2 * i]), scale, inverse),
-                      quotient(__uint_as_float(bits[2 * i + 1]), scale, inverse));
-    }
-    return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
-}
+// Eight neighbouring elements as they lie in memory: bf16 stay packed until they are used, which leaves
+// registers for more blocks of threads on an SM, and these for more bytes in flight.
+template <bool kF32>
+struct Eight {
+    static constexpr uint32_t kWords = kF32 ? 8u : 4u;
+    uint32_t w[kWords];
 
-K3_DEVINL uint32_t largest8(const uint32_t (&bits)[8]) {
-    uint32_t m = 0u;
+    // elements c .. c + 7 of a row, zeros past its end.  kVector: the row starts on 16 bytes and is a
+    // multiple of 8 elements long.
+    template <bool kVector>
+    K3_DEVINL void load(const void *row, uint32_t c, uint32_t columns) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) m = max(m, bits[i] & 0x7fffffffu);
-    return m;
-}
-
-// Eight elements of a row from column c as f32 bit patterns, zeros past the end.  kVector: the row
-// starts on 16 bytes and its length is a multiple of 8 elements.
-template <bool kF32, bool kVector>
-K3_DEVINL void load8(uint32_t (&bits)[8], const void *row, uint32_t c, uint32_t columns) {
-    if (kVector) {
+        for (uint32_t i = 0; i < kWords; i++) w[i] = 0u;
+        if (kVector) {
+            if (c >= columns) return;
 #pragma unroll
-        for (int i = 0; i < 8; i++) bits[i] = 0u;
-        if (c >= columns) return;
-        if (kF32) {
-            const uint4 a = *reinterpret_cast<const uint4 *>((const uint32_t *)row + c);
-            const uint4 b = *reinterpret_cast<const uint4 *>((const uint32_t *)row + c + 4u);
-            bits[0] = a.x; bits[1] = a.y; bits[2] = a.z; bits[3] = a.w;
-            bits[4] = b.x; bits[5] = b.y; bits[6] = b.z; bits[7] = b.w;
+            for (uint32_t h = 0; h < kWords / 4u; h++) {
+                const uint4 q = *reinterpret_cast<const uint4 *>((const char *)row + (uint64_t)c * (kF32 ? 4u : 2u) + h * 16u);
+                w[4u * h] = q.x; w[4u * h + 1u] = q.y; w[4u * h + 2u] = q.z; w[4u * h + 3u] = q.w;
+            }
         } else {
-            const uint4 a = *reinterpret_cast<const uint4 *>((const uint16_t *)row + c);
-            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                bits[2 * i] = w[i] << 16;
-                bits[2 * i + 1] = w[i] & 0xffff0000u;
-            }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            bits[i] = 0u;
-            if (c + i < columns) {
-                bits[i] = kF32 ? ((const uint32_t *)row)[c + i] : (uint32_t)((const uint16_t *)row)[c + i] << 16;
+            for (uint32_t i = 0; i < 8u; i++) {
+                if (c + i >= columns) continue;
+                if (kF32) w[i % kWords] = ((const uint32_t *)row)[c + i];
+                else w[i / 2u] |= (uint32_t)((const uint16_t *)row)[c + i] << (16u * (i & 1u));
             }
         }
     }
-}
+    K3_DEVINL float value(uint32_t i) const {
+        if (kF32) return __uint_as_float(w[i % kWords]);
+        return i & 1u ? bf16_hi(w[i / 2u]) : bf16_lo(w[i / 2u]);
+    }
+    // largest magnitudes: one word for f32, both halves of a word for bf16
+    K3_DEVINL uint32_t largest() const {
+        uint32_t m = magnitude(w[0]);
+#pragma unroll
+        for (uint32_t i = 1; i < kWords; i++) m = larger(m, magnitude(w[i]));
+        return m;
+    }
+    static K3_DEVINL uint32_t magnitude(uint32_t x) { return x & (kF32 ? 0x7fffffffu : 0x7fff7fffu); }
+    static K3_DEVINL uint32_t larger(uint32_t a, uint32_t b) {
+        if (kF32) return max(a, b);
+        uint32_t r;
+        asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    // of a word of larger(): the f32 bits
+    static K3_DEVINL uint32_t bits(uint32_t m) { return kF32 ? m : max(m & 0xffff0000u, m << 16); }
+    K3_DEVINL uint2 codes(float scale, float inverse) const {
+        uint32_t h[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; i++) {
+            h[i] = codes2(quotient(value(2u * i), scale, inverse), quotient(value(2u * i + 1u), scale, inverse));
+        }
+        return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+    }
+};
 
 // ------------------------------------------------------------------------------------------- rows
 // Half a warp takes four neighbouring blocks of a row: lane l holds elements 8 l .. 8 l + 7 of each.
@@ -95,21 +104,28 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(RowsArgs a) {
     const uint32_t group = (uint32_t)task - row * a.tasks_per_row;
     const bool live = task < (uint64_t)a.rows * a.tasks_per_row;     // the shuffles below want every lane
     const char *x = (const char *)a.x + (uint64_t)(live ? row : 0u) * a.columns * (kF32 ? 4u : 2u);
-    uint32_t bits[4][8];
+    Eight<kF32> x8[4];
 #pragma unroll
     for (int b = 0; b < 4; b++) {
-        load8<kF32, kVector>(bits[b], x, (group * 4u + b) * kBlock + l * 8u, live ? a.columns : 0u);
+        x8[b].template load<kVector>(x, (group * 4u + b) * kBlock + l * 8u, live ? a.columns : 0u);
     }
     pdl_trigger();                   // a product behind may fetch its table now (Product::b_ready)
+    // lane l divides for block l % 4
+    uint32_t most = 0u;
+#pragma unroll
+    for (int b = 0; b < 4; b++) {
+        uint32_t m = x8[b].largest();
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) m = Eight<kF32>::larger(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (l % 4u == (uint32_t)b) most = m;
+    }
+    const float my_scale = scale_of(Eight<kF32>::bits(most)), my_inverse = __frcp_rn(my_scale);
     float scale[4];
     uint2 out[4];
 #pragma unroll
     for (int b = 0; b < 4; b++) {
-        uint32_t m = largest8(bits[b]);
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-        scale[b] = scale_of(m);
-        out[b] = codes8(bits[b], scale[b], __frcp_rn(scale[b]));
+        scale[b] = __shfl_sync(0xffffffffu, my_scale, b, 16);
+        out[b] = x8[b].codes(scale[b], __shfl_sync(0xffffffffu, my_inverse, b, 16));
         if ((group * 4u + b) * kBlock >= a.columns) scale[b] = 0.0f;  // padding of the scales' row
     }
     if (!live) return;
@@ -150,49 +166,59 @@ __global__ void __launch_bounds__(kThreads)
 quantize_columns_kernel(uint8_t *codes, float *scales, const void *x, uint32_t rows, uint32_t columns) {
     __shared__ uint32_t largest[8][kTileColumns];
     __shared__ uint32_t tile[kTileColumns * kTileWords];
+    __shared__ float2 column_scale[kTileColumns];
     pdl_wait();
     const uint32_t r0 = blockIdx.y * kBlock, c0 = blockIdx.x * kTileColumns;
     const uint32_t ct = threadIdx.x % 8u, rt = threadIdx.x / 8u, warp = threadIdx.x / kWarp;
-    uint32_t bits[4][8];
+    Eight<kF32> x8[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const uint32_t r = r0 + rt * 4u + i;
         const char *row = (const char *)x + (uint64_t)(r < rows ? r : 0u) * columns * (kF32 ? 4u : 2u);
-        load8<kF32, kVector>(bits[i], row, c0 + ct * 8u, r < rows ? columns : 0u);
+        x8[i].template load<kVector>(row, c0 + ct * 8u, r < rows ? columns : 0u);
     }
-    uint32_t m[8];
+    // of each column: this thread's four rows, the warp's four threads with the column, the eight warps
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        m[j] = 0u;
+    for (uint32_t k = 0; k < Eight<kF32>::kWords; k++) {
+        uint32_t m = 0u;
 #pragma unroll
-        for (int i = 0; i < 4; i++) m[j] = max(m[j], bits[i][j] & 0x7fffffffu);
-        m[j] = max(m[j], __shfl_xor_sync(0xffffffffu, m[j], 8));
-        m[j] = max(m[j], __shfl_xor_sync(0xffffffffu, m[j], 16));
-    }
-    if (threadIdx.x % kWarp < 8u) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) largest[warp][ct * 8u + j] = m[j];
+        for (int i = 0; i < 4; i++) m = Eight<kF32>::larger(m, Eight<kF32>::magnitude(x8[i].w[k]));
+        m = Eight<kF32>::larger(m, __shfl_xor_sync(0xffffffffu, m, 8));
+        m = Eight<kF32>::larger(m, __shfl_xor_sync(0xffffffffu, m, 16));
+        if (threadIdx.x % kWarp < 8u) {
+            if (kF32) {
+                largest[warp][ct * 8u + k] = m;
+            } else {
+                largest[warp][ct * 8u + 2u * k] = m << 16;
+                largest[warp][ct * 8u + 2u * k + 1u] = m & 0xffff0000u;
+            }
+        }
     }
     __syncthreads();
+    // a column's scale and reciprocal once, by one thread
     const uint32_t scale_pitch = scale_pitch_of(rows);
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
+    if (threadIdx.x < kTileColumns) {
         uint32_t all = 0u;
 #pragma unroll
-        for (int w = 0; w < 8; w++) all = max(all, largest[w][ct * 8u + j]);
-        const float scale = scale_of(all), inverse = __frcp_rn(scale);
-        float q[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) q[i] = quotient(__uint_as_float(bits[i][j]), scale, inverse);
-        tile[(ct * 8u + j) * kTileWords + rt] = codes2(q[0], q[1]) | (codes2(q[2], q[3]) << 16);
-        const uint32_t c = c0 + ct * 8u + j;
-        if (rt == 0u && c < columns) {
-            float *to = scales + (uint64_t)c * scale_pitch + blockIdx.y;
+        for (int w = 0; w < 8; w++) all = max(all, largest[w][threadIdx.x]);
+        const float scale = scale_of(all);
+        column_scale[threadIdx.x] = make_float2(scale, __frcp_rn(scale));
+        if (c0 + threadIdx.x < columns) {
+            float *to = scales + (uint64_t)(c0 + threadIdx.x) * scale_pitch + blockIdx.y;
             *to = scale;
             if (blockIdx.y + 1u == gridDim.y) {
                 for (uint32_t p = 1u; blockIdx.y + p < scale_pitch; p++) to[p] = 0.0f;
             }
         }
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t j = 0; j < 8u; j++) {
+        const float2 s = column_scale[ct * 8u + j];
+        float q[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) q[i] = quotient(x8[i].value(j), s.x, s.y);
+        tile[(ct * 8u + j) * kTileWords + rt] = codes2(q[0], q[1]) | (codes2(q[2], q[3]) << 16);
     }
     __syncthreads();
     const uint32_t pitch = pitch_of(rows);
@@ -214,14 +240,16 @@ quantize_blocks_kernel(uint8_t *codes, float *scales, const void *x, uint32_t ro
     __shared__ uint32_t largest[8];
     pdl_wait();
     const uint32_t r0 = blockIdx.y * kBlock, c = blockIdx.x * kBlock + (threadIdx.x % 16u) * 8u, rt = threadIdx.x / 16u;
-    uint32_t bits[8][8], m = 0u;
+    Eight<kF32> x8[8];
+    uint32_t m = 0u;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         const uint32_t r = r0 + i * 16u + rt;
         const char *row = (const char *)x + (uint64_t)(r < rows ? r : 0u) * columns * (kF32 ? 4u : 2u);
-        load8<kF32, kVector>(bits[i], row, c, r < rows ? columns : 0u);
-        m = max(m, largest8(bits[i]));
+        x8[i].template load<kVector>(row, c, r < rows ? columns : 0u);
     }
+#pragma unroll
+    for (int i = 0; i < 8; i++) m = max(m, Eight<kF32>::bits(x8[i].largest()));
     m = __reduce_max_sync(0xffffffffu, m);
     if (threadIdx.x % kWarp == 0u) largest[threadIdx.x / kWarp] = m;
     __syncthreads();
@@ -234,7 +262,7 @@ quantize_blocks_kernel(uint8_t *codes, float *scales, const void *x, uint32_t ro
     for (int i = 0; i < 8; i++) {
         const uint32_t r = r0 + i * 16u + rt;
         if (r < rows && c < pitch) {
-            *reinterpret_cast<uint2 *>(codes + (uint64_t)r * pitch + c) = codes8(bits[i], scale, inverse);
+            *reinterpret_cast<uint2 *>(codes + (uint64_t)r * pitch + c) = x8[i].codes(scale, inverse);
         }
     }
 }
