@@ -48,7 +48,9 @@ struct Product {
     int b_scale_layout, epilogue, accumulate;
     int activation;
     float beta, linear_beta;
-    bool b_ready;                    // the launch in front is quantize_rows(), which lets this one start behind its own wait
+    // The launch in front writes neither b nor the offsets, and lets this one start only behind its own wait for what
+    // is in front of it (a quantiser of rows, a product): b may be read before this one's wait.
+    bool b_ready;
 };
 bool product(const Product &p, cudaStream_t stream);
 // the kernels behind it: tiles of 128 rows (k3_fp8_wide.cu)

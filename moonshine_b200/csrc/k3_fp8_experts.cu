@@ -160,6 +160,7 @@ extern "C" bool k3_moe_fp8_experts_forward(const k3_moe_fp8_experts_desc *d, voi
     p.k = d->hidden;
     p.b_scale_layout = K3_MOE_FP8_BLOCKS;
     p.epilogue = kOutActivated;
+    p.b_ready = true;                // the launch in front is the quantiser, then the gate/up product
     p.activation = d->activation;
     p.beta = d->beta;
     p.linear_beta = d->linear_beta;

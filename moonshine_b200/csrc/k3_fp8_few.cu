@@ -17,8 +17,8 @@
 // part of its rows that a block needs, a block of 128 columns each, straight into the operand's place. Every
 // tile of b does so again, which is little beside the launch it saves.  For more rows that takes longer
 // than b: 47 rows of 7168 x 2048 18.2 us, against 12.3 with a launch of its own.
-// b_ready (split): the kernel in front, a quantiser, has waited for everything in front of it before it let
-// this one start, so b's first stages may be fetched while it runs.
+// b_ready: the kernel in front writes neither b nor the offsets, and has waited for everything in front of it
+// before it let this one start, so b's first stages are fetched while it runs.
 //
 // Warps: 0 loads by TMA, 1 MMA issuer and owner of the tensor memory, 2 factors, then four per 32 rows
 // of a with the running sums, then the quantising ones.  Every wait is bounded; on give-up the block raises the status word,
@@ -191,7 +191,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         tmem_alloc(tmem_slot, L::kTmem);
         tmem_relinquish();
     }
-    if (!kSplit || warp != 0u) pdl_wait();
+    if (kSplit ? warp != 0u : !a.b_ready) pdl_wait();
     if (!kSplit && warp == 2u) {
         // exclusive prefix of the groups' row tiles, 32 groups at a time
         uint32_t before = 0u;
@@ -218,14 +218,22 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     if (warp == 0u) {
         // ----------------------------------------------------------------------------- loads
         if (elect_one()) {
-            uint32_t s = 0u, ph = 0u, issued = 0u;
+            uint32_t s = 0u, ph = 0u, issued = 0u, early = kSplit ? L::kStages : 0u;
             bool ok = true;
+            if (!kSplit && a.b_ready) {
+                if (first_item < total) {
+                    const Item it = item_of(first_item);
+                    early = min(L::kStages, it.kb_end);
+                    for (uint32_t i = 0; i < early; i++) load_b(it, i, i);
+                }
+                pdl_wait();
+            }
             for (uint32_t w = first_item; ok && w < total; w += step) {
                 const Item it = item_of(w);
                 const uint32_t boxes = (it.rows + kBoxRows - 1u) / kBoxRows;
                 for (uint32_t kb = it.kb_begin; kb < it.kb_end; kb++) {
                     if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag)) { ok = false; break; }
-                    if (!kSplit || issued >= L::kStages) load_b(it, s, kb);
+                    if (issued >= early) load_b(it, s, kb);
                     unsigned char *rows = base + s * L::kStageBytes + kTiles * L::kBTile;
                     for (uint32_t i = 0; !kQuantize && i < boxes; i++) {
                         tma_load_2d(rows + i * kBoxRows * kBlock, &map_a, &full[s], (int32_t)(kb * kBlock),
@@ -235,9 +243,9 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     if (++s == L::kStages) { s = 0u; ph ^= 1u; }
                 }
             }
-            if (kSplit) pdl_trigger();                               // the blocks of the next kernel may take places as these leave
+            pdl_trigger();                                           // the blocks of the next kernel may take places as these leave
             if (*abort_flag != 0u) {                                 // nothing may land in a block that has left
-                if (kSplit) issued = max(issued, min(L::kStages, blocks));
+                issued = max(issued, min(early, blocks));
                 for (uint32_t i = issued > L::kStages ? issued - L::kStages : 0u; i < issued; i++) {
                     mbar_drain(&full[i % L::kStages], (i / L::kStages) & 1u);
                 }
@@ -280,6 +288,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         }
     } else if (warp == 2u && !kQuantize) {
         // --------------------------------------------------------------- factors, a slot at a time
+        if (!kSplit && a.b_ready) pdl_wait();
         uint32_t slot = 0u, ph = 0u;
         bool ok = true;
         const uint32_t pitch = (blocks + 3u) & ~3u, b_blocks = blocks_of(a.n);
@@ -383,6 +392,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         }
     } else if (warp >= 4u) {
         // --------------------------------------------------------------------------- running sums
+        if (!kSplit && a.b_ready) pdl_wait();                        // before the first store
         constexpr uint32_t kMine = kRows < 32u ? kRows : 32u;         // rows of a per warp
         const uint32_t q = warp % 4u, half = (warp - 4u) / 4u;
         const uint32_t lanes = tmem + ((32u * q) << 16) + half * kMine;
@@ -626,6 +636,7 @@ bool launch_grouped(const Product &p, cudaStream_t stream) {
         return false;
     }
     FewArgs a = args_of(p);
+    a.b_ready = p.b_ready;
     a.column_items = (p.n + kColumns - 1u) / kColumns;
     const uint64_t items = ((uint64_t)(p.rows + kRows - 1u) / kRows + p.groups) * a.column_items;
     if (items > 0x7fffffffull) return false;

@@ -104,6 +104,17 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(RowsArgs a) {
     const uint32_t group = (uint32_t)task - row * a.tasks_per_row;
     const bool live = task < (uint64_t)a.rows * a.tasks_per_row;     // the shuffles below want every lane
     const char *x = (const char *)a.x + (uint64_t)(live ? row : 0u) * a.columns * (kF32 ? 4u : 2u);
+    // kPlaced: lane l has the places of the row's routes l and 16 + l
+    constexpr uint32_t kNowhere = 0xffffffffu;
+    uint32_t place[2] = {kNowhere, kNowhere};
+#pragma unroll
+    for (uint32_t h = 0; kPlaced && h < 2u; h++) {
+        const uint32_t r = h * 16u + l, route = row * a.at.top_k + r;
+        if (live && r < a.at.top_k) {
+            if (a.at.ids[route] < a.at.experts) place[h] = a.at.place[route];
+            else if (group == 0u) a.at.place[route] = a.at.spare;
+        }
+    }
     Eight<kF32> x8[4];
 #pragma unroll
     for (int b = 0; b < 4; b++) {
@@ -128,7 +139,6 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(RowsArgs a) {
         out[b] = x8[b].codes(scale[b], __shfl_sync(0xffffffffu, my_inverse, b, 16));
         if ((group * 4u + b) * kBlock >= a.columns) scale[b] = 0.0f;  // padding of the scales' row
     }
-    if (!live) return;
     const uint32_t pitch = pitch_of(a.columns), scale_pitch = a.tasks_per_row * 4u;
     auto store = [&](uint32_t to) {
         if (l == 0u) {
@@ -142,15 +152,16 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(RowsArgs a) {
         }
     };
     if (!kPlaced) {
-        store(row);
+        if (live) store(row);
     } else {
-        for (uint32_t r = 0; r < a.at.top_k; r++) {
-            const uint32_t route = row * a.at.top_k + r;
-            if (a.at.ids[route] < a.at.experts) {
-                store(a.at.place[route]);
-            } else if (group == 0u && l == 0u) {
-                a.at.place[route] = a.at.spare;
+#pragma unroll
+        for (uint32_t h = 0; h < 2u; h++) {
+            for (uint32_t r = 0; r < 16u; r++) {
+                const uint32_t to = __shfl_sync(0xffffffffu, place[h], r, 16);
+                if (to != kNowhere) store(to);
+                if (h * 16u + r + 1u >= a.at.top_k) break;
             }
+            if (a.at.top_k <= 16u) break;
         }
     }
 }

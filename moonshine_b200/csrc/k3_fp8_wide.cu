@@ -191,6 +191,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                         if (++s == L::kStages) { s = 0u; ph ^= 1u; }
                     }
                 }
+                pdl_trigger();                                       // the blocks of the next kernel may take places as these leave
                 if (*abort_flag != 0u) {                             // nothing may land in a block that has left
                     for (uint32_t i = issued > L::kStages ? issued - L::kStages : 0u; i < issued; i++) {
                         mbar_drain(&full[i % L::kStages], (i / L::kStages) & 1u);
