@@ -194,7 +194,7 @@ balance_tokens_kernel(float *part_sums, uint32_t *part_counts, const float *logi
             if (u < end) Row<kV, kVector>::fetch(mine + stage * kPitch, logits + (uint64_t)u * a.experts, a.experts, lane);
             copies_commit();
         };
-        if (logits) {                              // on their way while the routes are counted
+        if (logits) {
 #pragma unroll
             for (uint32_t g = 0; g + 1u < kForwardStages; g++) fetch(t + warp + g * kWarps, g);
             for (uint32_t e = a.experts + lane; e < kPitch; e += kWarp) {
@@ -203,15 +203,18 @@ balance_tokens_kernel(float *part_sums, uint32_t *part_counts, const float *logi
         }
         for (uint32_t e = threadIdx.x; e < a.experts; e += kThreads) counts_s[e] = 0u;
         __syncthreads();
-        for (uint32_t r = t * a.top_k + threadIdx.x; r < end * a.top_k; r += kThreads) {
-            const uint32_t id = ids[r];
+        auto count = [&](uint32_t id) {
             if (id < a.experts) atomicAdd(&counts_s[id], 1u);
             else g_balance_status = 2u;
-        }
-        if (logits) {
-            uint32_t stage = 0u;
+        };
+        if (!logits) {
+            for (uint32_t r = t * a.top_k + threadIdx.x; r < end * a.top_k; r += kThreads) count(ids[r]);
+        } else {
+            uint32_t stage = 0u, next_id = t + warp < end && lane < a.top_k ? ids[(uint64_t)(t + warp) * a.top_k + lane] : 0u;
             for (uint32_t u = t + warp; u < end; u += kWarps) {
                 fetch(u + (kForwardStages - 1u) * kWarps, stage == 0u ? kForwardStages - 1u : stage - 1u);
+                const uint32_t id = next_id;
+                if (u + kWarps < end && lane < a.top_k) next_id = ids[(uint64_t)(u + kWarps) * a.top_k + lane];
                 copies_wait<kForwardStages - 1>();
                 Row<kV, kVector> p;
                 p.load(mine + stage * kPitch, kPitch, lane, 0.f);
@@ -219,6 +222,7 @@ balance_tokens_kernel(float *part_sums, uint32_t *part_counts, const float *logi
                 const float r = a.softmax ? 1.0f : __fdividef(1.0f, kTiny + p.sum());
 #pragma unroll
                 for (uint32_t i = 0; i < kV * 4u; i++) acc.v[i] = fmaf(p.v[i], r, acc.v[i]);
+                if (lane < a.top_k) count(id);
                 if (++stage == kForwardStages) stage = 0u;
             }
             copies_wait<0>();
@@ -226,6 +230,7 @@ balance_tokens_kernel(float *part_sums, uint32_t *part_counts, const float *logi
             acc.store(sums_s + warp * kPitch, kPitch, lane);
         }
         __syncthreads();
+        pdl_trigger();                             // the second stage's blocks may take places as these leave
         const uint64_t to = (uint64_t)(blockIdx.x + s) * a.experts;
         for (uint32_t e = threadIdx.x; e < a.experts; e += kThreads) {
             part_counts[to + e] = counts_s[e];
@@ -249,6 +254,7 @@ balance_sequences_kernel(uint32_t *counts, float *loss, float *means, const floa
     __shared__ uint32_t counts_s[8][128];
     __shared__ float total[4], mine;
     pdl_wait();
+    pdl_trigger();
     const uint32_t s = blockIdx.y, begin = begin_of(offsets, s), end = end_of(offsets, s, a.tokens);
     const uint32_t length = end > begin ? end - begin : 0u;
     const uint32_t column = threadIdx.x % 128u, group = threadIdx.x / 128u, e = blockIdx.x * 128u + column;
