@@ -44,6 +44,10 @@ struct Product {
     const void *a, *a_scales;
     const void *b, *b_scales, *b2, *b2_scales;
     const uint32_t *offsets;
+    const uint32_t *ids;             // token_gateup, token_down: the routes' matrices, u32 [top_k]
+    const float *weights;            // token_down: f32 [top_k]
+    const void *shared;              // token_down: bf16 [n] or null
+    uint32_t top_k;
     uint32_t groups, rows, n, k;
     int b_scale_layout, epilogue, accumulate;
     int activation;
@@ -61,5 +65,9 @@ bool few_product(const Product &p, cudaStream_t stream);
 // the same of up to 16 rows of a as bf16 (p.a and p.a_scales unused), quantised by rows on the way; out bf16
 constexpr uint32_t few_linear_rows = 16;
 bool few_linear(const Product &p, const void *x_bf16, cudaStream_t stream);
+// one token's experts: a [1, k] times the gate and up matrices of each route -> activated rows [top_k, n]; and
+// out bf16 [n] = sum over routes of weight * (a [top_k, k] row) times its down matrix, plus shared
+bool token_gateup(const Product &p, cudaStream_t stream);
+bool token_down(const Product &p, cudaStream_t stream);
 
 }  // namespace k3::fp8

@@ -135,14 +135,21 @@ extern "C" bool k3_moe_fp8_experts_forward(const k3_moe_fp8_experts_desc *d, voi
     if (workspace_bytes < w.carve.total) return false;
     cudaStream_t stream = (cudaStream_t)stream_pointer;
     const uint32_t routes = tokens * d->top_k;
-    if (!k3_moe_dispatch_build(w.offsets, w.sorted_route, w.sorted_token, w.inv_perm, ids, tokens, d->top_k, d->experts,
-                               w.dispatch, w.dispatch_bytes, stream)) {
-        return false;
-    }
-    const Placement at{w.inv_perm, (const uint32_t *)ids, d->top_k, d->experts, routes};
-    if (!quantize_placed(w.x.codes, w.x.scales, x, tokens, d->hidden, at, w.rows_out + (uint64_t)routes * d->hidden,
-                         d->hidden * 2u, stream)) {
-        return false;
+    // One token: its routes are the groups as they come, and the down product forms their weighted sum.  Three
+    // launches; with dispatch, placed rows and combine 16 of 64 experts of 7168 x 2048 took 141 us.
+    const bool token = tokens == 1u;
+    if (token) {
+        if (!k3_moe_fp8_quantize_rows(w.x.codes, w.x.scales, x, 1u, d->hidden, K3_MOE_FP8_BF16, stream)) return false;
+    } else {
+        if (!k3_moe_dispatch_build(w.offsets, w.sorted_route, w.sorted_token, w.inv_perm, ids, tokens, d->top_k, d->experts,
+                                   w.dispatch, w.dispatch_bytes, stream)) {
+            return false;
+        }
+        const Placement at{w.inv_perm, (const uint32_t *)ids, d->top_k, d->experts, routes};
+        if (!quantize_placed(w.x.codes, w.x.scales, x, tokens, d->hidden, at, w.rows_out + (uint64_t)routes * d->hidden,
+                             d->hidden * 2u, stream)) {
+            return false;
+        }
     }
     Product p{};
     p.out = w.act.codes;
@@ -153,9 +160,11 @@ extern "C" bool k3_moe_fp8_experts_forward(const k3_moe_fp8_experts_desc *d, voi
     p.b_scales = d->w1_scales;
     p.b2 = d->w3;
     p.b2_scales = d->w3_scales;
-    p.offsets = w.offsets;
+    p.offsets = token ? nullptr : w.offsets;
+    p.ids = (const uint32_t *)ids;
+    p.top_k = d->top_k;
     p.groups = d->experts;
-    p.rows = routes;
+    p.rows = token ? 1u : routes;
     p.n = d->expert_hidden;
     p.k = d->hidden;
     p.b_scale_layout = K3_MOE_FP8_BLOCKS;
@@ -164,7 +173,7 @@ extern "C" bool k3_moe_fp8_experts_forward(const k3_moe_fp8_experts_desc *d, voi
     p.activation = d->activation;
     p.beta = d->beta;
     p.linear_beta = d->linear_beta;
-    if (!product(p, stream)) return false;
+    if (token ? !token_gateup(p, stream) : !product(p, stream)) return false;
     p.out = w.rows_out;
     p.out_scales = nullptr;
     p.a = w.act.codes;
@@ -175,6 +184,13 @@ extern "C" bool k3_moe_fp8_experts_forward(const k3_moe_fp8_experts_desc *d, voi
     p.n = d->hidden;
     p.k = d->expert_hidden;
     p.epilogue = kOutBf16;
+    if (token) {
+        p.out = out;
+        p.rows = 1u;
+        p.weights = (const float *)weights;
+        p.shared = shared;
+        return token_down(p, stream);
+    }
     if (!product(p, stream)) return false;
     return k3_moe_combine(out, w.rows_out, w.inv_perm, weights, shared, tokens, d->top_k, d->hidden, stream);
 }

@@ -17,6 +17,11 @@
 // part of its rows that a block needs, a block of 128 columns each, straight into the operand's place. Every
 // tile of b does so again, which is little beside the launch it saves.  For more rows that takes longer
 // than b: 47 rows of 7168 x 2048 18.2 us, against 12.3 with a launch of its own.
+// kToken (the routed experts of one token): the groups are the token's routes, one row each, without a
+// dispatch.  Gate/up (grouped): item (route, 128 columns), all routes read the same row of a.  Down (split):
+// the depth runs over the routes one after the other and a route's weight is part of its factors, so the
+// sum over the experts is formed like any other and nothing is written in between.  A route whose id is no
+// expert reads zeros.
 // b_ready: the kernel in front writes neither b nor the offsets, and has waited for everything in front of it
 // before it let this one start, so b's first stages are fetched while it runs.
 //
@@ -49,14 +54,15 @@ struct Layout {
     static constexpr uint32_t kPerSm = kSplit ? 2u : 1u;
     static constexpr uint32_t kBTile = kBlock * kBlock;              // 128 rows of b, 128 columns
     static constexpr uint32_t kStageBytes = kTiles * kBTile + kRows * kBlock;
-    static constexpr uint32_t kStages = !kSplit ? 5u : kRows <= 16u ? 6u : 4u;
+    static constexpr uint32_t kStages = !kSplit ? (kRows <= 16u ? 6u : 5u) : kRows <= 16u ? 6u : 4u;
     // factors travel four blocks at a time, or with the codes
     static constexpr uint32_t kSlots = kQuantize ? 8u : 2u, kSlotBlocks = kQuantize ? 1u : 4u;
     static constexpr uint32_t kFactors = kStages * kStageBytes;      // f32 [kSlots][kSlotBlocks][kTiles][kRows]
     static constexpr uint32_t kSlotFloats = kSlotBlocks * kTiles * kRows;
     static constexpr uint32_t kLargest = kFactors + kSlots * kSlotFloats * 4u;   // f32 bits [4][kRows]
     static constexpr uint32_t kPrefix = kLargest + 4u * kRows * 4u;
-    static constexpr uint32_t kBars = (kPrefix + (kSplit ? 0u : (kMaxGroups + 1u) * 4u) + 15u) / 16u * 16u;
+    static constexpr uint32_t kRoutes = kPrefix;                     // kToken: ids [32], weights [32] in the prefix's place
+    static constexpr uint32_t kBars = (kPrefix + (kSplit ? 256u : (kMaxGroups + 1u) * 4u) + 15u) / 16u * 16u;
     static constexpr uint32_t kBytes = kBars + 512u + 1024u;         // the last: alignment
     static constexpr uint32_t kTmem = kTiles * kRows * 2u < 32u ? 32u : kTiles * kRows * 2u;
     static_assert(kBytes <= (kPerSm == 2u ? 115000u : 232448u), "two blocks of a split product share an SM");
@@ -71,6 +77,10 @@ struct FewArgs {
     bool x_vector;                                 // its rows are whole 16-byte units
     bool b_ready;
     const uint32_t *offsets;
+    const uint32_t *ids;                           // kToken
+    const float *weights;
+    const uint16_t *shared;                        // kToken, split: bf16 [n] or null
+    uint32_t top_k;
     uint32_t groups, rows, n, k;
     uint32_t column_items;                         // grouped: items along b's rows
     uint32_t split_blocks;                         // kSplit: blocks of 128 per part of the depth
@@ -98,7 +108,7 @@ K3_DEVINL void tmem_ld_wait_for(uint32_t (&r)[16]) {
                    "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 }
 
-template <int kEpilogue, uint32_t kTiles, uint32_t kRows, bool kSplit, bool kQuantize>
+template <int kEpilogue, uint32_t kTiles, uint32_t kRows, bool kSplit, bool kQuantize, bool kToken>
 __global__ void __launch_bounds__(Layout<kTiles, kRows, kSplit, kQuantize>::kThreads, Layout<kTiles, kRows, kSplit, kQuantize>::kPerSm)
 fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                const __grid_constant__ CUtensorMap map_b2, FewArgs a) {
@@ -117,6 +127,8 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     volatile uint32_t *abort_flag = tmem_slot + 1;
     uint32_t *total_s = tmem_slot + 2;
     uint32_t *prefix = reinterpret_cast<uint32_t *>(base + L::kPrefix);
+    uint32_t *ids_s = reinterpret_cast<uint32_t *>(base + L::kRoutes);
+    float *weights_s = reinterpret_cast<float *>(ids_s + 32);
     const uint32_t warp = warp_index(), lane = threadIdx.x % kWarp;
     const uint32_t blocks = blocks_of(a.k);
     constexpr uint32_t kColumns = kEpilogue == kOutActivated ? kBlock : kTiles * kBlock;
@@ -131,11 +143,17 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             it.rows = min(kRows, a.rows - it.row);
             it.column = blockIdx.y * kBlock;
             it.kb_begin = blockIdx.x * a.split_blocks;
-            it.kb_end = min(blocks, it.kb_begin + a.split_blocks);
+            it.kb_end = min(kToken ? a.top_k * blocks : blocks, it.kb_begin + a.split_blocks);
             return it;
         }
         const uint32_t tile = w / a.column_items;
         it.column = (w - tile * a.column_items) * kColumns;
+        if (kToken) {
+            it.group = ids_s[tile];
+            it.row = tile;
+            it.rows = 1u;
+            return it;
+        }
         uint32_t lo = 0u, hi = a.groups;                             // the last group whose first tile is at most `tile`
         while (hi - lo > 1u) {
             const uint32_t mid = (lo + hi) / 2u;
@@ -148,9 +166,13 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     };
 
     const uint64_t stream_once = l2_policy_evict_first();
-    auto load_b = [&](const Item &it, uint32_t stage, uint32_t kb) {
+    // kToken, split: step kb of the depth is block kb % blocks of this route
+    auto route_of = [&](uint32_t kb) { return kSplit && kToken ? kb / blocks : 0u; };
+    auto load_b = [&](const Item &it, uint32_t stage, uint32_t kb, uint32_t group) {
         unsigned char *st = base + stage * L::kStageBytes;
-        const int32_t x = (int32_t)(kb * kBlock), y = (int32_t)(it.group * a.n + it.column);
+        const int32_t x = (int32_t)((kb - route_of(kb) * blocks) * kBlock);
+        // past the table's end: zeros
+        const int32_t y = (int32_t)(kToken && group >= a.groups ? a.groups * a.n : group * a.n + it.column);
         const uint32_t boxes = kQuantize ? 0u : (it.rows + kBoxRows - 1u) / kBoxRows;
         mbar_arrive_expect_tx(&full[stage], kTiles * L::kBTile + boxes * kBoxRows * kBlock);
         tma_load_2d_hint(st, &map_b, &full[stage], x, y, stream_once);
@@ -183,7 +205,15 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         if (kSplit) {                                                // b's first stages, before anyone waits for anyone
             if (!a.b_ready) pdl_wait();
             const Item it = item_of(0u);
-            for (uint32_t i = 0; i < min(L::kStages, it.kb_end - it.kb_begin); i++) load_b(it, i, it.kb_begin + i);
+            uint32_t route = 0xffffffffu, group = 0u;
+            for (uint32_t i = 0; i < min(L::kStages, it.kb_end - it.kb_begin); i++) {
+                const uint32_t kb = it.kb_begin + i;
+                if (kToken && route_of(kb) != route) {
+                    route = route_of(kb);
+                    group = a.ids[route];
+                }
+                load_b(it, i, kb, group);
+            }
             pdl_wait();
         }
     }
@@ -192,7 +222,13 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         tmem_relinquish();
     }
     if (kSplit ? warp != 0u : !a.b_ready) pdl_wait();
-    if (!kSplit && warp == 2u) {
+    if (kToken && warp == 3u && lane < a.top_k) {
+        ids_s[lane] = a.ids[lane];
+        weights_s[lane] = kSplit ? a.weights[lane] : 0.f;
+        if (!kSplit && blockIdx.x == 0u && ids_s[lane] >= a.groups) atomicOr(&g_fp8_few_status, 2u);
+    }
+    if (kToken && !kSplit && threadIdx.x == 0u) *total_s = a.top_k * a.column_items;
+    if (!kSplit && !kToken && warp == 2u) {
         // exclusive prefix of the groups' row tiles, 32 groups at a time
         uint32_t before = 0u;
         for (uint32_t g0 = 0; g0 < a.groups; g0 += kWarp) {
@@ -218,13 +254,17 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     if (warp == 0u) {
         // ----------------------------------------------------------------------------- loads
         if (elect_one()) {
-            uint32_t s = 0u, ph = 0u, issued = 0u, early = kSplit ? L::kStages : 0u;
+            uint32_t s = 0u, ph = 0u, issued = 0u, early = 0u;
             bool ok = true;
+            if (kSplit) {
+                const Item it = item_of(0u);
+                early = min(L::kStages, it.kb_end - it.kb_begin);
+            }
             if (!kSplit && a.b_ready) {
                 if (first_item < total) {
                     const Item it = item_of(first_item);
                     early = min(L::kStages, it.kb_end);
-                    for (uint32_t i = 0; i < early; i++) load_b(it, i, i);
+                    for (uint32_t i = 0; i < early; i++) load_b(it, i, i, it.group);
                 }
                 pdl_wait();
             }
@@ -233,11 +273,14 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 const uint32_t boxes = (it.rows + kBoxRows - 1u) / kBoxRows;
                 for (uint32_t kb = it.kb_begin; kb < it.kb_end; kb++) {
                     if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag)) { ok = false; break; }
-                    if (issued >= early) load_b(it, s, kb);
+                    const uint32_t route = route_of(kb), group = kSplit && kToken ? ids_s[route] : it.group;
+                    if (issued >= early) load_b(it, s, kb, group);
                     unsigned char *rows = base + s * L::kStageBytes + kTiles * L::kBTile;
+                    // one token: its only row, or the route's
+                    const uint32_t row = !kToken ? it.row : kSplit ? (group < a.groups ? route : a.top_k) : 0u;
                     for (uint32_t i = 0; !kQuantize && i < boxes; i++) {
-                        tma_load_2d(rows + i * kBoxRows * kBlock, &map_a, &full[s], (int32_t)(kb * kBlock),
-                                    (int32_t)(it.row + i * kBoxRows));
+                        tma_load_2d(rows + i * kBoxRows * kBlock, &map_a, &full[s], (int32_t)((kb - route * blocks) * kBlock),
+                                    (int32_t)(row + i * kBoxRows));
                     }
                     issued++;
                     if (++s == L::kStages) { s = 0u; ph ^= 1u; }
@@ -245,7 +288,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             }
             pdl_trigger();                                           // the blocks of the next kernel may take places as these leave
             if (*abort_flag != 0u) {                                 // nothing may land in a block that has left
-                issued = max(issued, min(early, blocks));
+                issued = max(issued, early);
                 for (uint32_t i = issued > L::kStages ? issued - L::kStages : 0u; i < issued; i++) {
                     mbar_drain(&full[i % L::kStages], (i / L::kStages) & 1u);
                 }
@@ -294,7 +337,32 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         const uint32_t pitch = (blocks + 3u) & ~3u, b_blocks = blocks_of(a.n);
         for (uint32_t w = first_item; ok && w < total; w += step) {
             const Item it = item_of(w);
-            const uint64_t sb = ((uint64_t)it.group * b_blocks + it.column / kBlock) * blocks;
+            if constexpr (kToken && kSplit) {
+                for (uint32_t kb = it.kb_begin; kb < it.kb_end; kb += L::kSlotBlocks) {
+                    float f[4];
+#pragma unroll
+                    for (uint32_t i = 0; i < 4u; i++) {
+                        const uint32_t at = min(kb + i, it.kb_end - 1u), route = at / blocks, in = at - route * blocks;
+                        const uint32_t group = ids_s[route];
+                        f[i] = 0.f;
+                        if (group < a.groups) {
+                            f[i] = a.a_scales[(uint64_t)route * pitch + in] *
+                                   a.b_scales[((uint64_t)group * b_blocks + it.column / kBlock) * blocks + in] * weights_s[route];
+                        }
+                    }
+                    if (!mbar_wait(&factor_empty[slot], ph ^ 1u, abort_flag)) { ok = false; break; }
+                    float *to = reinterpret_cast<float *>(base + L::kFactors) + slot * L::kSlotFloats;
+                    if (lane < kRows) {
+#pragma unroll
+                        for (uint32_t i = 0; i < 4u; i++) to[i * kRows + lane] = f[i];
+                    }
+                    mbar_arrive(&factor_full[slot]);
+                    if (++slot == L::kSlots) { slot = 0u; ph ^= 1u; }
+                }
+                continue;
+            }
+            const bool valid = !kToken || it.group < a.groups;
+            const uint64_t sb = ((uint64_t)(valid ? it.group : 0u) * b_blocks + it.column / kBlock) * blocks;
             const float *b_row[2] = {a.b_scales + sb, nullptr};
             if (kTiles == 2u) {
                 b_row[1] = kEpilogue == kOutActivated ? a.b2_scales + sb
@@ -305,13 +373,13 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 #pragma unroll
                 for (uint32_t t = 0; t < kTiles; t++) {
 #pragma unroll
-                    for (uint32_t i = 0; i < 4u; i++) f[t][i] = b_row[t][min(kb + i, blocks - 1u)];
+                    for (uint32_t i = 0; i < 4u; i++) f[t][i] = valid ? b_row[t][min(kb + i, blocks - 1u)] : 0.f;
                 }
                 float x[(kRows + 31u) / 32u][4];
 #pragma unroll
                 for (uint32_t j = 0; j < (kRows + 31u) / 32u; j++) {
                     // rows past the tile's take the last row's scales: their columns are not kept
-                    const float *row = a.a_scales + (uint64_t)(it.row + min(j * kWarp + lane, it.rows - 1u)) * pitch;
+                    const float *row = a.a_scales + (uint64_t)(kToken ? 0u : it.row + min(j * kWarp + lane, it.rows - 1u)) * pitch;
 #pragma unroll
                     for (uint32_t i = 0; i < 4u; i++) x[j][i] = row[min(kb + i, blocks - 1u)];
                 }
@@ -562,6 +630,14 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 }
             } else {
                 uint16_t *out = (uint16_t *)a.out + to;
+                if (kToken && a.shared) {                             // added as k3_moe_combine does
+#pragma unroll
+                    for (uint32_t j = 0; j < 4u; j++) {
+                        if (c + j < a.n) {
+                            sum[j] = bf16_bits_to_float(float_to_bf16_bits(sum[j])) + bf16_bits_to_float(a.shared[c + j]);
+                        }
+                    }
+                }
                 if (vector) {
                     *reinterpret_cast<uint2 *>(out) = make_uint2(bf16x2(sum[0], sum[1]), bf16x2(sum[2], sum[3]));
                 } else {
@@ -592,6 +668,10 @@ FewArgs args_of(const Product &p) {
     a.b_scales = (const float *)p.b_scales;
     a.b2_scales = (const float *)p.b2_scales;
     a.offsets = p.offsets;
+    a.ids = p.ids;
+    a.weights = p.weights;
+    a.shared = (const uint16_t *)p.shared;
+    a.top_k = p.top_k;
     a.groups = p.groups;
     a.rows = p.rows;
     a.n = p.n;
@@ -603,31 +683,35 @@ FewArgs args_of(const Product &p) {
     return a;
 }
 
-template <int kEpilogue, uint32_t kRows, bool kQuantize>
+template <int kEpilogue, uint32_t kRows, bool kQuantize, bool kToken = false>
 bool launch_split(const Product &p, const void *x, bool b_ready, cudaStream_t stream) {
     using L = Layout<1, kRows, true, kQuantize>;
     CUtensorMap a_map{}, b_map;
-    if ((!kQuantize && !map_codes(&a_map, p.a, p.rows, p.k, kBoxRows)) || !map_codes(&b_map, p.b, p.n, p.k, kBlock)) return false;
+    if ((!kQuantize && !map_codes(&a_map, p.a, kToken ? p.top_k : p.rows, p.k, kBoxRows)) ||
+        !map_codes(&b_map, p.b, (uint64_t)p.groups * p.n, p.k, kBlock)) {
+        return false;
+    }
     FewArgs a = args_of(p);
     a.x = (const uint16_t *)x;
     a.x_vector = aligned16(x) && p.k % 8u == 0u;
     a.b_ready = b_ready;
-    const uint32_t tiles = blocks_of(p.n), row_tiles = (p.rows + kRows - 1u) / kRows, blocks = blocks_of(p.k);
+    const uint32_t tiles = blocks_of(p.n), row_tiles = (p.rows + kRows - 1u) / kRows;
+    const uint32_t blocks = blocks_of(p.k) * (kToken ? p.top_k : 1u);
     if (tiles > 65535u || row_tiles > 65535u) return false;
     // as many parts as the SMs hold, with two blocks of 128 in a part at least
     const uint32_t room = (uint32_t)sm_count() * L::kPerSm / std::max(1u, tiles * row_tiles);
     const uint32_t splits = std::max(1u, std::min({kMaxSplits, room, blocks / 2u}));
     a.split_blocks = (blocks + splits - 1u) / splits;
     const uint32_t parts = (blocks + a.split_blocks - 1u) / a.split_blocks;
-    auto kernel = fp8_few_kernel<kEpilogue, 1, kRows, true, kQuantize>;
+    auto kernel = fp8_few_kernel<kEpilogue, 1, kRows, true, kQuantize, kToken>;
     if (!set_max_dynamic_smem((const void *)kernel, L::kBytes)) return false;
     return launch_chained_cluster(kernel, dim3(parts, tiles, row_tiles), L::kThreads, dim3(parts, 1, 1), L::kBytes, stream, a_map,
                                   b_map, b_map, a);
 }
 
-template <int kEpilogue>
+template <int kEpilogue, bool kToken = false>
 bool launch_grouped(const Product &p, cudaStream_t stream) {
-    constexpr uint32_t kRows = few_rows, kColumns = kEpilogue == kOutActivated ? kBlock : 2u * kBlock;
+    constexpr uint32_t kRows = kToken ? 16u : few_rows, kColumns = kEpilogue == kOutActivated ? kBlock : 2u * kBlock;
     using L = Layout<2, kRows, false, false>;
     CUtensorMap a_map, b_map, b2_map;
     const uint64_t b_rows = (uint64_t)p.groups * p.n;
@@ -638,9 +722,9 @@ bool launch_grouped(const Product &p, cudaStream_t stream) {
     FewArgs a = args_of(p);
     a.b_ready = p.b_ready;
     a.column_items = (p.n + kColumns - 1u) / kColumns;
-    const uint64_t items = ((uint64_t)(p.rows + kRows - 1u) / kRows + p.groups) * a.column_items;
+    const uint64_t items = (kToken ? p.top_k : (uint64_t)(p.rows + kRows - 1u) / kRows + p.groups) * a.column_items;
     if (items > 0x7fffffffull) return false;
-    auto kernel = fp8_few_kernel<kEpilogue, 2, kRows, false, false>;
+    auto kernel = fp8_few_kernel<kEpilogue, 2, kRows, false, false, kToken>;
     return set_max_dynamic_smem((const void *)kernel, L::kBytes) &&
            launch_chained(kernel, (uint32_t)std::min<uint64_t>(items, sm_count()), L::kThreads, L::kBytes, stream, a_map, b_map,
                           b2_map, a);
@@ -660,6 +744,12 @@ bool k3::fp8::few_product(const Product &p, cudaStream_t stream) {
     }
     return p.epilogue == kOutF32 ? launch_split<kOutF32, few_rows, false>(p, nullptr, p.b_ready, stream)
                                  : launch_split<kOutBf16, few_rows, false>(p, nullptr, p.b_ready, stream);
+}
+
+bool k3::fp8::token_gateup(const Product &p, cudaStream_t stream) { return launch_grouped<kOutActivated, true>(p, stream); }
+
+bool k3::fp8::token_down(const Product &p, cudaStream_t stream) {
+    return launch_split<kOutBf16, 16, false, true>(p, nullptr, p.b_ready, stream);
 }
 
 bool k3::fp8::few_linear(const Product &p, const void *x_bf16, cudaStream_t stream) {

@@ -256,7 +256,7 @@ EXPERTS_REL = 3.5e-3
 
 @pytest.mark.parametrize("kind", ["swiglu", "situ"])
 @pytest.mark.parametrize("tokens,hidden,expert_hidden,experts,top_k", [
-    (1, 512, 256, 8, 2), (1, 1024, 1040, 4, 4), (2, 144, 80, 3, 1), (7, 256, 128, 16, 5), (33, 640, 384, 6, 3), (64, 528, 272, 5, 2),
+    (1, 512, 256, 8, 2), (1, 1024, 1040, 4, 4), (1, 128, 16, 33, 32), (1, 7168, 2048, 3, 3), (1, 16, 400, 1, 1), (1, 2064, 144, 20, 11), (2, 144, 80, 3, 1), (7, 256, 128, 16, 5), (33, 640, 384, 6, 3), (64, 528, 272, 5, 2),
     (150, 512, 256, 4, 4), (300, 400, 144, 33, 8), (700, 256, 384, 2, 2), (1200, 272, 160, 3, 1)])
 def test_experts(tokens, hidden, expert_hidden, experts, top_k, kind):
     tables = expert_tables(tokens, experts, hidden, expert_hidden)
