@@ -57,10 +57,31 @@ struct Product {
     bool b_ready;
 };
 bool product(const Product &p, cudaStream_t stream);
+
+// Parts that the depth of an item is cut into, a cluster of one block per part: the number with the shortest time for
+// `items` items of `blocks` steps each, where a wave of as many clusters as fit takes the steps of a part (a multiple of
+// `multiple`) and `fixed` steps more.  active(size): clusters that fit at once.
+template <typename F>
+uint32_t best_parts(uint64_t items, uint32_t blocks, uint32_t multiple, uint32_t fixed, F active) {
+    uint32_t best = 1u;
+    uint64_t shortest = ~0ull;
+    for (uint32_t s = 1u; s <= 8u; s++) {
+        const uint32_t steps = ((blocks + s - 1u) / s + multiple - 1u) / multiple * multiple, parts = (blocks + steps - 1u) / steps;
+        const uint32_t fit = parts == s ? active(s) : 0u;               // a number of parts that rounding does not give
+        if (fit == 0u) continue;
+        const uint64_t time = (items + fit - 1u) / fit * (steps + fixed);
+        if (time < shortest) {
+            shortest = time;
+            best = s;
+        }
+    }
+    return best;
+}
 // the kernels behind it: tiles of 128 rows (k3_fp8_wide.cu)
 bool wide_product(const Product &p, cudaStream_t stream);
-// tiles of 16 or 64 rows, b in 128 x 128 blocks only (k3_fp8_few.cu)
-constexpr uint32_t few_rows = 64;
+// tiles of 16 rows of one matrix or 64 of a group, b in 128 x 128 blocks only (k3_fp8_few.cu)
+constexpr uint32_t grouped_few_rows = 40;    // per group on average
+constexpr bool grouped_few(uint32_t rows, uint32_t groups) { return rows <= grouped_few_rows * groups; }
 bool few_product(const Product &p, cudaStream_t stream);
 // the same of up to 16 rows of a as bf16 (p.a and p.a_scales unused), quantised by rows on the way; out bf16
 constexpr uint32_t few_linear_rows = 16;

@@ -85,10 +85,10 @@ struct ExpertsWorkspace {
           x(carve, (uint64_t)tokens * d->top_k, d->hidden),
           act(carve, (uint64_t)tokens * d->top_k, d->expert_hidden),
           rows_out(carve.take(std::max(((uint64_t)tokens * d->top_k + 1u) * 2u,       // never less for more tokens
-                                       (std::min((uint64_t)tokens * d->top_k, (uint64_t)few_rows * d->experts) + 1u) * 4u) *
+                                       (std::min((uint64_t)tokens * d->top_k, (uint64_t)grouped_few_rows * d->experts) + 1u) * 4u) *
                               d->hidden)) {}
     // expert rows in f32: where the kernels for few rows compute them
-    static bool rows_f32(const k3_moe_fp8_experts_desc *d, uint32_t routes) { return routes <= few_rows * d->experts; }
+    static bool rows_f32(const k3_moe_fp8_experts_desc *d, uint32_t routes) { return grouped_few(routes, d->experts); }
 };
 
 bool experts_ok(const k3_moe_fp8_experts_desc *d, uint32_t tokens) {

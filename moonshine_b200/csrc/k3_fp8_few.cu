@@ -7,16 +7,16 @@
 // of a cost no more than their own loads.  128 lanes share a block scale; a row's scale goes with the
 // column, so the factors sa sb of a block lie in shared memory and every lane reads the same one.
 //
-// kSplit (one matrix): a work item is 128 rows of b and a part of the depth; the parts of an item are a
-// cluster, which adds its sums through distributed shared memory in ascending order of the depth.  Two
-// blocks fit an SM, so any number of them up to 296 streams at once.
-// Otherwise (grouped): one block per SM goes over items of 256 rows of b (kOutActivated: 128 of gate and
-// the same 128 of up) over the whole depth.
+// kSplit (one matrix, up to 16 rows): a work item is 128 rows of b and a part of the depth; the parts of an
+// item are a cluster, which adds its sums through distributed shared memory in ascending order of the
+// depth.  Two blocks fit an SM.
+// Otherwise (groups of a few dozen rows): one block per SM goes over items of 256 rows of b (kOutActivated:
+// 128 of gate and the same 128 of up) and up to 64 of a over the whole depth.
 //
 // kQuantize (a linear layer's call with up to 16 rows, split): a is bf16, and four more warps quantise the
 // part of its rows that a block needs, a block of 128 columns each, straight into the operand's place. Every
-// tile of b does so again, which is little beside the launch it saves.  For more rows that takes longer
-// than b: 47 rows of 7168 x 2048 18.2 us, against 12.3 with a launch of its own.
+// tile of b does so again, which is little beside the launch it saves: one token of 3584 x 7168 takes 7.6 us,
+// with a launch of its own 10.0.
 // kToken (the routed experts of one token): the groups are the token's routes, one row each, without a
 // dispatch.  Gate/up (grouped): item (route, 128 columns), all routes read the same row of a.  Down (split):
 // the depth runs over the routes one after the other and a route's weight is part of its factors, so the
@@ -41,20 +41,22 @@ namespace {
 
 constexpr uint32_t kMaxGroups = 1024;
 constexpr uint32_t kMaxSplits = 8;                                   // of the depth: the portable cluster
+constexpr uint32_t kGroupRows = 64;                                  // of a group per item
 constexpr uint32_t kBoxRows = 16;                                    // a's rows per box: what an MMA column step is
 
 __device__ uint32_t g_fp8_few_status = 0;
 
 template <uint32_t kTiles, uint32_t kRows, bool kSplit, bool kQuantize>
 struct Layout {
-    static_assert(!kQuantize || (kSplit && kRows == 16u), "only a linear layer of few rows quantises here");
+    static_assert(!kSplit || kRows == 16u, "more rows of one matrix: k3_fp8_wide.cu");
+    static_assert(kSplit || !kQuantize, "only a linear layer quantises here");
     static constexpr uint32_t kHalves = (kRows + 31u) / 32u;
     static constexpr uint32_t kSumWarps = 4u * kHalves, kQuantizeWarps = kQuantize ? 4u : 0u;
     static constexpr uint32_t kThreads = (4u + kSumWarps + kQuantizeWarps) * kWarp;
     static constexpr uint32_t kPerSm = kSplit ? 2u : 1u;
     static constexpr uint32_t kBTile = kBlock * kBlock;              // 128 rows of b, 128 columns
     static constexpr uint32_t kStageBytes = kTiles * kBTile + kRows * kBlock;
-    static constexpr uint32_t kStages = !kSplit ? (kRows <= 16u ? 6u : 5u) : kRows <= 16u ? 6u : 4u;
+    static constexpr uint32_t kStages = kRows <= 16u ? 6u : 5u;
     // factors travel four blocks at a time, or with the codes
     static constexpr uint32_t kSlots = kQuantize ? 8u : 2u, kSlotBlocks = kQuantize ? 1u : 4u;
     static constexpr uint32_t kFactors = kStages * kStageBytes;      // f32 [kSlots][kSlotBlocks][kTiles][kRows]
@@ -683,8 +685,9 @@ FewArgs args_of(const Product &p) {
     return a;
 }
 
-template <int kEpilogue, uint32_t kRows, bool kQuantize, bool kToken = false>
-bool launch_split(const Product &p, const void *x, bool b_ready, cudaStream_t stream) {
+template <int kEpilogue, bool kQuantize, bool kToken = false>
+bool launch_split(const Product &p, const void *x, cudaStream_t stream) {
+    constexpr uint32_t kRows = few_linear_rows;
     using L = Layout<1, kRows, true, kQuantize>;
     CUtensorMap a_map{}, b_map;
     if ((!kQuantize && !map_codes(&a_map, p.a, kToken ? p.top_k : p.rows, p.k, kBoxRows)) ||
@@ -694,24 +697,24 @@ bool launch_split(const Product &p, const void *x, bool b_ready, cudaStream_t st
     FewArgs a = args_of(p);
     a.x = (const uint16_t *)x;
     a.x_vector = aligned16(x) && p.k % 8u == 0u;
-    a.b_ready = b_ready;
+    a.b_ready = p.b_ready && !kQuantize;
     const uint32_t tiles = blocks_of(p.n), row_tiles = (p.rows + kRows - 1u) / kRows;
     const uint32_t blocks = blocks_of(p.k) * (kToken ? p.top_k : 1u);
     if (tiles > 65535u || row_tiles > 65535u) return false;
-    // as many parts as the SMs hold, with two blocks of 128 in a part at least
-    const uint32_t room = (uint32_t)sm_count() * L::kPerSm / std::max(1u, tiles * row_tiles);
-    const uint32_t splits = std::max(1u, std::min({kMaxSplits, room, blocks / 2u}));
-    a.split_blocks = (blocks + splits - 1u) / splits;
-    const uint32_t parts = (blocks + a.split_blocks - 1u) / a.split_blocks;
     auto kernel = fp8_few_kernel<kEpilogue, 1, kRows, true, kQuantize, kToken>;
     if (!set_max_dynamic_smem((const void *)kernel, L::kBytes)) return false;
+    // a launch, the first loads and the sums' way through the cluster take as long as 8 steps
+    const uint32_t parts = best_parts((uint64_t)tiles * row_tiles, blocks, 1u, 8u, [&](uint32_t size) {
+        return active_clusters((const void *)kernel, size, L::kThreads, L::kBytes);
+    });
+    a.split_blocks = (blocks + parts - 1u) / parts;
     return launch_chained_cluster(kernel, dim3(parts, tiles, row_tiles), L::kThreads, dim3(parts, 1, 1), L::kBytes, stream, a_map,
                                   b_map, b_map, a);
 }
 
 template <int kEpilogue, bool kToken = false>
 bool launch_grouped(const Product &p, cudaStream_t stream) {
-    constexpr uint32_t kRows = kToken ? 16u : few_rows, kColumns = kEpilogue == kOutActivated ? kBlock : 2u * kBlock;
+    constexpr uint32_t kRows = kToken ? 16u : kGroupRows, kColumns = kEpilogue == kOutActivated ? kBlock : 2u * kBlock;
     using L = Layout<2, kRows, false, false>;
     CUtensorMap a_map, b_map, b2_map;
     const uint64_t b_rows = (uint64_t)p.groups * p.n;
@@ -738,22 +741,17 @@ bool k3::fp8::few_product(const Product &p, cudaStream_t stream) {
                : p.epilogue == kOutF32     ? launch_grouped<kOutF32>(p, stream)
                                            : launch_grouped<kOutBf16>(p, stream);
     }
-    if (p.rows <= 16u) {
-        return p.epilogue == kOutF32 ? launch_split<kOutF32, 16, false>(p, nullptr, p.b_ready, stream)
-                                     : launch_split<kOutBf16, 16, false>(p, nullptr, p.b_ready, stream);
-    }
-    return p.epilogue == kOutF32 ? launch_split<kOutF32, few_rows, false>(p, nullptr, p.b_ready, stream)
-                                 : launch_split<kOutBf16, few_rows, false>(p, nullptr, p.b_ready, stream);
+    return p.epilogue == kOutF32 ? launch_split<kOutF32, false>(p, nullptr, stream) : launch_split<kOutBf16, false>(p, nullptr, stream);
 }
 
 bool k3::fp8::token_gateup(const Product &p, cudaStream_t stream) { return launch_grouped<kOutActivated, true>(p, stream); }
 
 bool k3::fp8::token_down(const Product &p, cudaStream_t stream) {
-    return launch_split<kOutBf16, 16, false, true>(p, nullptr, p.b_ready, stream);
+    return launch_split<kOutBf16, false, true>(p, nullptr, stream);
 }
 
 bool k3::fp8::few_linear(const Product &p, const void *x_bf16, cudaStream_t stream) {
-    return launch_split<kOutBf16, 16, true>(p, x_bf16, false, stream);
+    return launch_split<kOutBf16, true>(p, x_bf16, stream);
 }
 
 uint32_t k3_fp8_few_status() {

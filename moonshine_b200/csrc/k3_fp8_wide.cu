@@ -14,6 +14,8 @@
 //   warp 1        MMA issuer, owns the tensor memory
 //   warp 2        scales, four blocks ahead: a row's times the block's, where the adding warps read them
 //   warps 4-11    running sums: lane quadrant warp % 4, columns in two halves
+// kSplit (one matrix, fewer items than SMs): an item is a cluster of up to 8 blocks with a part of the
+// depth each, which add their sums through distributed shared memory in ascending order of the depth.
 // The two warpgroups of running sums (128 of them per thread) take registers over from the first one:
 // 2 x 128 x 232 + 128 x 40 are the 384 x 168 of the launch.
 //
@@ -37,6 +39,7 @@ constexpr uint32_t kStageBytes = kATile + kBTile;
 constexpr uint32_t kSumWarps = 8;
 constexpr uint32_t kStoreBytes = 32u * 64u;                          // per warp: 32 rows of 64 bytes on their way out
 constexpr uint32_t kMaxGroups = 1024;
+constexpr uint32_t kMaxSplits = 8;                                   // of the depth: the portable cluster
 constexpr uint32_t kScaleSlots = 2, kSlotBlocks = 4;                 // scales travel four blocks at a time
 
 template <bool kColumnScales>
@@ -63,37 +66,43 @@ struct WideArgs {
     const uint32_t *offsets;
     uint32_t groups, rows, n, k;
     uint32_t column_items;
+    uint32_t split_blocks;                                           // kSplit: blocks of 128 per part, a multiple of 4
+    bool b_ready;                                                    // kSplit: Product::b_ready
     int accumulate;
     int activation;
     float beta, linear_beta;
 };
 
 struct Item {
-    uint32_t group, row, rows, column;
+    uint32_t group, row, rows, column, kb_begin, kb_end;
 };
 
-K3_DEVINL Item item_of(uint32_t w, const uint32_t *prefix, const WideArgs &a, uint32_t columns) {
-    Item it;
-    const uint32_t tile = w / a.column_items;
-    it.column = (w - tile * a.column_items) * columns;
-    if (a.offsets == nullptr) {
-        it.group = 0u;
-        it.row = tile * BM;
-        it.rows = min(BM, a.rows - it.row);
-        return it;
+// four neighbouring results at `out`, of which `left` columns exist
+K3_DEVINL void store4(float *out, const float (&sum)[4], uint32_t left, bool vector, int accumulate) {
+    float v[4];
+#pragma unroll
+    for (uint32_t j = 0; j < 4u; j++) v[j] = accumulate && j < left ? out[j] + sum[j] : sum[j];
+    if (vector) {
+        *reinterpret_cast<float4 *>(out) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+        for (uint32_t j = 0; j < 4u; j++) {
+            if (j < left) out[j] = v[j];
+        }
     }
-    uint32_t lo = 0u, hi = a.groups;                                 // the last group whose first tile is at most `tile`
-    while (hi - lo > 1u) {
-        const uint32_t mid = (lo + hi) / 2u;
-        if (prefix[mid] <= tile) lo = mid; else hi = mid;
+}
+K3_DEVINL void store4(uint16_t *out, const float (&sum)[4], uint32_t left, bool vector, int) {
+    if (vector) {
+        *reinterpret_cast<uint2 *>(out) = make_uint2(bf16x2(sum[0], sum[1]), bf16x2(sum[2], sum[3]));
+    } else {
+#pragma unroll
+        for (uint32_t j = 0; j < 4u; j++) {
+            if (j < left) out[j] = float_to_bf16_bits(sum[j]);
+        }
     }
-    it.group = lo;
-    it.row = a.offsets[lo] + (tile - prefix[lo]) * BM;
-    it.rows = min(BM, a.offsets[lo + 1u] - it.row);
-    return it;
 }
 
-template <int kEpilogue, bool kColumnScales>
+template <int kEpilogue, bool kColumnScales, bool kSplit>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                 const __grid_constant__ CUtensorMap map_b2, WideArgs a) {
@@ -116,7 +125,48 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     const uint32_t blocks = blocks_of(a.k);
     constexpr uint32_t kColumns = kEpilogue == kOutActivated ? kBlock : BN;
 
-    if (threadIdx.x == 0) {
+    auto item_of = [&](uint32_t w) {
+        Item it;
+        it.kb_begin = 0u;
+        it.kb_end = blocks;
+        if (kSplit) {
+            it.group = 0u;
+            it.column = blockIdx.y * kColumns;
+            it.row = blockIdx.z * BM;
+            it.rows = min(BM, a.rows - it.row);
+            it.kb_begin = blockIdx.x * a.split_blocks;
+            it.kb_end = min(blocks, it.kb_begin + a.split_blocks);
+            return it;
+        }
+        const uint32_t tile = w / a.column_items;
+        it.column = (w - tile * a.column_items) * kColumns;
+        if (a.offsets == nullptr) {
+            it.group = 0u;
+            it.row = tile * BM;
+            it.rows = min(BM, a.rows - it.row);
+            return it;
+        }
+        uint32_t lo = 0u, hi = a.groups;                             // the last group whose first tile is at most `tile`
+        while (hi - lo > 1u) {
+            const uint32_t mid = (lo + hi) / 2u;
+            if (prefix[mid] <= tile) lo = mid; else hi = mid;
+        }
+        it.group = lo;
+        it.row = a.offsets[lo] + (tile - prefix[lo]) * BM;
+        it.rows = min(BM, a.offsets[lo + 1u] - it.row);
+        return it;
+    };
+    // b's 256 rows of a stage; the barrier waits for a's 128 as well
+    auto load_b = [&](const Item &it, uint32_t stage, uint32_t kb) {
+        unsigned char *st = base + stage * kStageBytes + kATile;
+        const int32_t x = (int32_t)(kb * kBlock), y = (int32_t)(it.group * a.n + it.column);
+        mbar_arrive_expect_tx(&full[stage], kStageBytes);
+        tma_load_2d(st, &map_b, &full[stage], x, y);
+        if (kEpilogue == kOutActivated) tma_load_2d(st + kBTile / 2u, &map_b2, &full[stage], x, y);
+        else tma_load_2d(st + kBTile / 2u, &map_b, &full[stage], x, y + (int32_t)kBlock);
+    };
+
+    if (warp == 0u && elect_one()) {
         *abort_flag = 0u;
         for (uint32_t s = 0; s < L::kStages; s++) {
             mbar_init(&full[s], 1);
@@ -133,6 +183,14 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         mbar_init(largest_full, kSumWarps);
         mbar_init(done, 1);
         fence_barrier_init();
+        prefetch_tensormap(&map_a);
+        prefetch_tensormap(&map_b);
+        if (kEpilogue == kOutActivated) prefetch_tensormap(&map_b2);
+        if (kSplit) {                                                // b's first stages, before anyone waits for anyone
+            if (!a.b_ready) pdl_wait();
+            const Item it = item_of(0u);
+            for (uint32_t i = 0; i < min(L::kStages, it.kb_end - it.kb_begin); i++) load_b(it, i, it.kb_begin + i);
+        }
     }
     if (warp == 1u) {
         tmem_alloc(tmem_slot, 512u);
@@ -158,41 +216,38 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             if (lane == 0u) *total_s = before * a.column_items;
         }
     } else if (threadIdx.x == 0) {
-        *total_s = (a.rows + BM - 1u) / BM * a.column_items;
+        *total_s = kSplit ? 1u : (a.rows + BM - 1u) / BM * a.column_items;
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot, total = *total_s;
+    const uint32_t first_item = kSplit ? 0u : blockIdx.x, step = kSplit ? 1u : gridDim.x;
 
     if (warp < 4u) {
         fewer_registers<40>();
         if (warp == 0u) {
             // ------------------------------------------------------------------------- loads
             if (elect_one()) {
-                prefetch_tensormap(&map_a);
-                prefetch_tensormap(&map_b);
-                prefetch_tensormap(&map_b2);
-                uint32_t s = 0u, ph = 0u, issued = 0u;
+                uint32_t s = 0u, ph = 0u, issued = 0u, early = 0u;
                 bool ok = true;
-                for (uint32_t w = blockIdx.x; ok && w < total; w += gridDim.x) {
-                    const Item it = item_of(w, prefix, a, kColumns);
-                    const int32_t y = (int32_t)(it.group * a.n + it.column);
-                    for (uint32_t kb = 0; kb < blocks; kb++) {
+                if (kSplit) {
+                    const Item it = item_of(0u);
+                    early = min(L::kStages, it.kb_end - it.kb_begin);
+                }
+                for (uint32_t w = first_item; ok && w < total; w += step) {
+                    const Item it = item_of(w);
+                    for (uint32_t kb = it.kb_begin; kb < it.kb_end; kb++) {
                         if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag)) { ok = false; break; }
-                        unsigned char *st = base + s * kStageBytes;
-                        const int32_t x = (int32_t)(kb * kBlock);
-                        mbar_arrive_expect_tx(&full[s], kStageBytes);
-                        tma_load_2d(st, &map_a, &full[s], x, (int32_t)it.row);
-                        tma_load_2d(st + kATile, &map_b, &full[s], x, y);
-                        if (kEpilogue == kOutActivated) tma_load_2d(st + kATile + kBTile / 2u, &map_b2, &full[s], x, y);
-                        else tma_load_2d(st + kATile + kBTile / 2u, &map_b, &full[s], x, y + (int32_t)kBlock);
+                        if (issued >= early) load_b(it, s, kb);
+                        tma_load_2d(base + s * kStageBytes, &map_a, &full[s], (int32_t)(kb * kBlock), (int32_t)it.row);
                         issued++;
                         if (++s == L::kStages) { s = 0u; ph ^= 1u; }
                     }
                 }
                 pdl_trigger();                                       // the blocks of the next kernel may take places as these leave
                 if (*abort_flag != 0u) {                             // nothing may land in a block that has left
+                    issued = max(issued, early);
                     for (uint32_t i = issued > L::kStages ? issued - L::kStages : 0u; i < issued; i++) {
                         mbar_drain(&full[i % L::kStages], (i / L::kStages) & 1u);
                     }
@@ -204,8 +259,9 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 constexpr uint32_t idesc = make_idesc_e4m3(BM, BN);
                 uint32_t s = 0u, ph = 0u, at = 0u, aph = 0u;
                 bool ok = true;
-                for (uint32_t w = blockIdx.x; ok && w < total; w += gridDim.x) {
-                    for (uint32_t kb = 0; kb < blocks; kb++) {
+                for (uint32_t w = first_item; ok && w < total; w += step) {
+                    const uint32_t n = kSplit ? item_of(w).kb_end - item_of(w).kb_begin : blocks;
+                    for (uint32_t kb = 0; kb < n; kb++) {
                         if (!mbar_wait(&full[s], ph, abort_flag) || !mbar_wait(&sum_empty[at], aph ^ 1u, abort_flag)) {
                             ok = false;
                             break;
@@ -231,14 +287,14 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             uint32_t slot = 0u, ph = 0u;
             bool ok = true;
             const uint32_t pitch = (blocks + 3u) & ~3u, b_blocks = blocks_of(a.n);
-            for (uint32_t w = blockIdx.x; ok && w < total; w += gridDim.x) {
-                const Item it = item_of(w, prefix, a, kColumns);
+            for (uint32_t w = first_item; ok && w < total; w += step) {
+                const Item it = item_of(w);
                 // b's rows of block scales: of the two halves of the columns, or gate's and up's
                 const uint64_t sb = ((uint64_t)it.group * b_blocks + it.column / kBlock) * blocks;
                 const float *b0 = a.b_scales + sb;
                 const float *b1 = kEpilogue == kOutActivated ? a.b2_scales + sb
                                   : it.column / kBlock + 1u < b_blocks ? b0 + blocks : b0;
-                for (uint32_t kb = 0; kb < blocks; kb += kSlotBlocks) {
+                for (uint32_t kb = it.kb_begin; kb < it.kb_end; kb += kSlotBlocks) {
                     if (!mbar_wait(&scale_empty[slot], ph ^ 1u, abort_flag)) { ok = false; break; }
                     float *to = reinterpret_cast<float *>(base + L::kScales) + slot * L::kSlotFloats;
                     float f0[4], f1[4];
@@ -277,6 +333,11 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 }
             }
         }
+        if (kSplit) {                                                // the other warps' two barriers, see below
+            __syncwarp();
+            cluster_barrier();
+            cluster_barrier();
+        }
     } else {
         // ---------------------------------------------------------------------- running sums
         more_registers<232>();
@@ -288,12 +349,12 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         const uint32_t row_in = 32u * q + lane;
         uint32_t at = 0u, aph = 0u, slot = 0u, sph = 0u, lph = 0u;
         bool ok = true;
-        for (uint32_t w = blockIdx.x; ok && w < total; w += gridDim.x) {
-            const Item it = item_of(w, prefix, a, kColumns);
+        for (uint32_t w = first_item; ok && w < total; w += step) {
+            const Item it = item_of(w);
             uint64_t sum[64];
 #pragma unroll
             for (int i = 0; i < 64; i++) sum[i] = 0ull;
-            for (uint32_t kb = 0; kb < blocks; kb++) {
+            for (uint32_t kb = it.kb_begin; kb < it.kb_end; kb++) {
                 if (kb % kSlotBlocks == 0u && !mbar_wait(&scale_full[slot], sph, abort_flag)) { ok = false; break; }
                 const float *scales = reinterpret_cast<const float *>(base + L::kScales) + slot * L::kSlotFloats +
                                       kb % kSlotBlocks * L::kBlockScales;
@@ -340,14 +401,22 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                     }
                 }
                 if (++at == 2u) { at = 0u; aph ^= 1u; }
-                if (kb % kSlotBlocks == kSlotBlocks - 1u || kb + 1u == blocks) {
+                if (kb % kSlotBlocks == kSlotBlocks - 1u || kb + 1u == it.kb_end) {
                     __syncwarp();
                     if (lane == 0u) mbar_arrive(&scale_empty[slot]);
                     if (++slot == kScaleSlots) { slot = 0u; sph ^= 1u; }
                 }
             }
             if (!ok) break;
-            if (kEpilogue == kOutActivated) {
+            if (kSplit) {
+                // [128][64] units of 16 bytes in the ring's place (every stage has been read), swizzled by the row
+                float4 *part = reinterpret_cast<float4 *>(base) + row_in * (BN / 4u);
+#pragma unroll
+                for (uint32_t j = 0; j < 32u; j++) {
+                    const uint32_t unit = (j < 16u ? first : second) / 4u + j % 16u;
+                    part[unit ^ (row_in & 7u)] = make_float4(lo2(sum[2u * j]), hi2(sum[2u * j]), lo2(sum[2u * j + 1u]), hi2(sum[2u * j + 1u]));
+                }
+            } else if (kEpilogue == kOutActivated) {
                 // ------------------------------------------ activation, largest of the row's 128, codes
                 uint32_t most = 0u;
 #pragma unroll
@@ -453,6 +522,38 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 }
             }
         }
+        if (kSplit) {
+            // the parts' sums, in ascending order of the depth; each block adds its share of the item
+            __syncwarp();
+            cluster_barrier();
+            const Item it = item_of(0u);
+            constexpr uint32_t kUnits = BN / 4u;
+            const uint32_t size = cluster_size(), all = it.rows * kUnits;
+            const uint32_t share = (all + size - 1u) / size, begin = cluster_rank() * share, end = min(all, begin + share);
+            const bool vector = a.n % 4u == 0u && ((uintptr_t)a.out & (kEpilogue == kOutF32 ? 15u : 7u)) == 0u;
+            for (uint32_t e = begin + threadIdx.x - 4u * kWarp; e < end; e += kSumWarps * kWarp) {
+                const uint32_t row = e / kUnits, unit = e % kUnits, c = it.column + unit * 4u;
+                if (c >= a.n) continue;
+                const float *part = reinterpret_cast<const float *>(base) + (row * kUnits + (unit ^ (row & 7u))) * 4u;
+                float4 v[kMaxSplits];
+#pragma unroll
+                for (uint32_t r = 0; r < kMaxSplits; r++) v[r] = r < size ? cluster_load4(part, r) : make_float4(0.f, 0.f, 0.f, 0.f);
+                float sum[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+#pragma unroll
+                for (uint32_t r = 1; r < kMaxSplits; r++) {
+                    if (r < size) {
+                        sum[0] += v[r].x;
+                        sum[1] += v[r].y;
+                        sum[2] += v[r].z;
+                        sum[3] += v[r].w;
+                    }
+                }
+                const uint64_t to = (uint64_t)(it.row + row) * a.n + c;
+                if (kEpilogue == kOutF32) store4((float *)a.out + to, sum, a.n - c, vector, a.accumulate);
+                else store4((uint16_t *)a.out + to, sum, a.n - c, vector, 0);
+            }
+            cluster_barrier();                                           // nobody leaves while its sums are read
+        }
     }
 
     tc_fence_before();
@@ -464,8 +565,21 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     }
 }
 
+// Parts of the depth.  A step takes 0.44 us where few blocks run, and the sums' way through the cluster 3 us (7 steps).
+// Measured, one part / the choice: 128 rows of 7168 x 7168 26.1 / 17.1 us, 512 of 2048 x 7168 26.4 / 15.6.
 template <int kEpilogue, bool kColumnScales>
-bool launch_wide(const Product &p, cudaStream_t stream) {
+uint32_t wide_parts(const Product &p) {
+    const void *kernel = (const void *)fp8_wide_kernel<kEpilogue, kColumnScales, true>;
+    constexpr uint32_t kBytes = Layout<kColumnScales>::kBytes;
+    const uint64_t items = (uint64_t)((p.rows + BM - 1u) / BM) * ((p.n + BN - 1u) / BN);
+    if (items * 2u > (uint32_t)sm_count() || !set_max_dynamic_smem(kernel, kBytes)) return 1u;
+    return best_parts(items, blocks_of(p.k), kSlotBlocks, 7u, [&](uint32_t size) {
+        return size == 1u ? (uint32_t)sm_count() : active_clusters(kernel, size, kThreads, kBytes);
+    });
+}
+
+template <int kEpilogue, bool kColumnScales, bool kSplit>
+bool launch_wide(const Product &p, uint32_t parts, cudaStream_t stream) {
     constexpr uint32_t kColumns = kEpilogue == kOutActivated ? kBlock : BN;
     CUtensorMap a_map, b_map, b2_map;
     const uint64_t b_rows = (uint64_t)p.groups * p.n;
@@ -485,26 +599,44 @@ bool launch_wide(const Product &p, cudaStream_t stream) {
     a.n = p.n;
     a.k = p.k;
     a.column_items = (p.n + kColumns - 1u) / kColumns;
+    a.b_ready = p.b_ready;
     a.accumulate = p.accumulate;
     a.activation = p.activation;
     a.beta = p.beta;
     a.linear_beta = p.linear_beta;
-    const uint64_t items = ((uint64_t)(p.rows + BM - 1u) / BM + (p.offsets ? p.groups : 0u)) * a.column_items;
-    if (items > 0x7fffffffull) return false;
-    auto kernel = fp8_wide_kernel<kEpilogue, kColumnScales>;
+    auto kernel = fp8_wide_kernel<kEpilogue, kColumnScales, kSplit>;
     constexpr uint32_t kBytes = Layout<kColumnScales>::kBytes;
-    return set_max_dynamic_smem((const void *)kernel, kBytes) &&
-           launch_chained(kernel, (uint32_t)std::min<uint64_t>(items, sm_count()), kThreads, kBytes, stream, a_map, b_map, b2_map, a);
+    if (!set_max_dynamic_smem((const void *)kernel, kBytes)) return false;
+    const uint32_t row_tiles = (p.rows + BM - 1u) / BM;
+    if (kSplit) {
+        a.split_blocks = ((blocks_of(p.k) + parts - 1u) / parts + kSlotBlocks - 1u) / kSlotBlocks * kSlotBlocks;
+        return launch_chained_cluster(kernel, dim3(parts, a.column_items, row_tiles), kThreads, dim3(parts, 1, 1), kBytes, stream,
+                                      a_map, b_map, b2_map, a);
+    }
+    const uint64_t items = ((uint64_t)row_tiles + (p.offsets ? p.groups : 0u)) * a.column_items;
+    return items <= 0x7fffffffull && launch_chained(kernel, (uint32_t)std::min<uint64_t>(items, sm_count()), kThreads, kBytes, stream,
+                                                    a_map, b_map, b2_map, a);
+}
+
+template <int kEpilogue, bool kColumnScales>
+bool launch_whole(const Product &p, cudaStream_t stream) {
+    const uint32_t parts = wide_parts<kEpilogue, kColumnScales>(p);
+    return parts > 1u ? launch_wide<kEpilogue, kColumnScales, true>(p, parts, stream)
+                      : launch_wide<kEpilogue, kColumnScales, false>(p, 1u, stream);
 }
 
 }  // namespace
 
 bool k3::fp8::wide_product(const Product &p, cudaStream_t stream) {
-    if (p.epilogue == kOutActivated) return launch_wide<kOutActivated, false>(p, stream);
-    if (p.b_scale_layout == K3_MOE_FP8_ROWS) {
-        return p.epilogue == kOutF32 ? launch_wide<kOutF32, true>(p, stream) : launch_wide<kOutBf16, true>(p, stream);
+    if (p.epilogue == kOutActivated) return launch_wide<kOutActivated, false, false>(p, 1u, stream);
+    if (p.offsets) {
+        return p.epilogue == kOutF32 ? launch_wide<kOutF32, false, false>(p, 1u, stream)
+                                       : launch_wide<kOutBf16, false, false>(p, 1u, stream);
     }
-    return p.epilogue == kOutF32 ? launch_wide<kOutF32, false>(p, stream) : launch_wide<kOutBf16, false>(p, stream);
+    if (p.b_scale_layout == K3_MOE_FP8_ROWS) {
+        return p.epilogue == kOutF32 ? launch_whole<kOutF32, true>(p, stream) : launch_whole<kOutBf16, true>(p, stream);
+    }
+    return p.epilogue == kOutF32 ? launch_whole<kOutF32, false>(p, stream) : launch_whole<kOutBf16, false>(p, stream);
 }
 
 uint32_t k3_fp8_wide_status() {
