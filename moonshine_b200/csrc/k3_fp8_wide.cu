@@ -14,8 +14,9 @@
 //   warp 1        MMA issuer, owns the tensor memory
 //   warp 2        scales, four blocks ahead: a row's times the block's, where the adding warps read them
 //   warps 4-11    running sums: lane quadrant warp % 4, columns in two halves
-// kSplit (one matrix, fewer items than SMs): an item is a cluster of up to 8 blocks with a part of the
-// depth each, which add their sums through distributed shared memory in ascending order of the depth.
+// kSplit (one matrix, fewer items than SMs, or the items that are left over when every SM has had as many as
+// the others): an item is a cluster of up to 8 blocks with a part of the depth each, which add their sums
+// through distributed shared memory in ascending order of the depth.
 // The two warpgroups of running sums (128 of them per thread) take registers over from the first one:
 // 2 x 128 x 232 + 128 x 40 are the 384 x 168 of the launch.
 //
@@ -66,6 +67,8 @@ struct WideArgs {
     const uint32_t *offsets;
     uint32_t groups, rows, n, k;
     uint32_t column_items;
+    uint32_t items;                                                  // one matrix: items of this launch
+    uint32_t first_item;                                             // kSplit: and the first of them
     uint32_t split_blocks;                                           // kSplit: blocks of 128 per part, a multiple of 4
     bool b_ready;                                                    // kSplit: Product::b_ready
     int accumulate;
@@ -130,13 +133,9 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         it.kb_begin = 0u;
         it.kb_end = blocks;
         if (kSplit) {
-            it.group = 0u;
-            it.column = blockIdx.y * kColumns;
-            it.row = blockIdx.z * BM;
-            it.rows = min(BM, a.rows - it.row);
+            w = a.first_item + blockIdx.y;
             it.kb_begin = blockIdx.x * a.split_blocks;
             it.kb_end = min(blocks, it.kb_begin + a.split_blocks);
-            return it;
         }
         const uint32_t tile = w / a.column_items;
         it.column = (w - tile * a.column_items) * kColumns;
@@ -216,7 +215,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             if (lane == 0u) *total_s = before * a.column_items;
         }
     } else if (threadIdx.x == 0) {
-        *total_s = kSplit ? 1u : (a.rows + BM - 1u) / BM * a.column_items;
+        *total_s = kSplit ? 1u : a.items;
     }
     tc_fence_before();
     __syncthreads();
@@ -565,28 +564,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     }
 }
 
-// Parts of the depth.  A step takes 0.44 us where few blocks run, and the sums' way through the cluster 3 us (7 steps).
-// Measured, one part / the choice: 128 rows of 7168 x 7168 26.1 / 17.1 us, 512 of 2048 x 7168 26.4 / 15.6.
-template <int kEpilogue, bool kColumnScales>
-uint32_t wide_parts(const Product &p) {
-    const void *kernel = (const void *)fp8_wide_kernel<kEpilogue, kColumnScales, true>;
-    constexpr uint32_t kBytes = Layout<kColumnScales>::kBytes;
-    const uint64_t items = (uint64_t)((p.rows + BM - 1u) / BM) * ((p.n + BN - 1u) / BN);
-    if (items * 2u > (uint32_t)sm_count() || !set_max_dynamic_smem(kernel, kBytes)) return 1u;
-    return best_parts(items, blocks_of(p.k), kSlotBlocks, 7u, [&](uint32_t size) {
-        return size == 1u ? (uint32_t)sm_count() : active_clusters(kernel, size, kThreads, kBytes);
-    });
-}
-
-template <int kEpilogue, bool kColumnScales, bool kSplit>
-bool launch_wide(const Product &p, uint32_t parts, cudaStream_t stream) {
-    constexpr uint32_t kColumns = kEpilogue == kOutActivated ? kBlock : BN;
-    CUtensorMap a_map, b_map, b2_map;
-    const uint64_t b_rows = (uint64_t)p.groups * p.n;
-    if (!map_codes(&a_map, p.a, p.rows, p.k, BM) || !map_codes(&b_map, p.b, b_rows, p.k, kBlock) ||
-        !map_codes(&b2_map, kEpilogue == kOutActivated ? p.b2 : p.b, b_rows, p.k, kBlock)) {
-        return false;
-    }
+WideArgs args_of(const Product &p, uint32_t columns) {
     WideArgs a{};
     a.out = p.out;
     a.out_scales = (float *)p.out_scales;
@@ -598,41 +576,74 @@ bool launch_wide(const Product &p, uint32_t parts, cudaStream_t stream) {
     a.rows = p.rows;
     a.n = p.n;
     a.k = p.k;
-    a.column_items = (p.n + kColumns - 1u) / kColumns;
-    a.b_ready = p.b_ready;
+    a.column_items = (p.n + columns - 1u) / columns;
     a.accumulate = p.accumulate;
     a.activation = p.activation;
     a.beta = p.beta;
     a.linear_beta = p.linear_beta;
-    auto kernel = fp8_wide_kernel<kEpilogue, kColumnScales, kSplit>;
-    constexpr uint32_t kBytes = Layout<kColumnScales>::kBytes;
-    if (!set_max_dynamic_smem((const void *)kernel, kBytes)) return false;
-    const uint32_t row_tiles = (p.rows + BM - 1u) / BM;
-    if (kSplit) {
-        a.split_blocks = ((blocks_of(p.k) + parts - 1u) / parts + kSlotBlocks - 1u) / kSlotBlocks * kSlotBlocks;
-        return launch_chained_cluster(kernel, dim3(parts, a.column_items, row_tiles), kThreads, dim3(parts, 1, 1), kBytes, stream,
-                                      a_map, b_map, b2_map, a);
-    }
-    const uint64_t items = ((uint64_t)row_tiles + (p.offsets ? p.groups : 0u)) * a.column_items;
-    return items <= 0x7fffffffull && launch_chained(kernel, (uint32_t)std::min<uint64_t>(items, sm_count()), kThreads, kBytes, stream,
-                                                    a_map, b_map, b2_map, a);
+    return a;
 }
 
+struct Maps {
+    CUtensorMap a, b, b2;
+    bool make(const Product &p) {
+        const uint64_t b_rows = (uint64_t)p.groups * p.n;
+        return map_codes(&a, p.a, p.rows, p.k, BM) && map_codes(&b, p.b, b_rows, p.k, kBlock) &&
+               map_codes(&b2, p.b2 ? p.b2 : p.b, b_rows, p.k, kBlock);
+    }
+};
+
+template <int kEpilogue>
+bool launch_grouped(const Product &p, cudaStream_t stream) {
+    Maps m;
+    if (!m.make(p)) return false;
+    const WideArgs a = args_of(p, kEpilogue == kOutActivated ? kBlock : BN);
+    const uint64_t items = ((uint64_t)(p.rows + BM - 1u) / BM + p.groups) * a.column_items;
+    auto kernel = fp8_wide_kernel<kEpilogue, false, false>;
+    constexpr uint32_t kBytes = Layout<false>::kBytes;
+    return items <= 0x7fffffffull && set_max_dynamic_smem((const void *)kernel, kBytes) &&
+           launch_chained(kernel, (uint32_t)std::min<uint64_t>(items, sm_count()), kThreads, kBytes, stream, m.a, m.b, m.b2, a);
+}
+
+// One matrix.  Every SM takes the same number of whole items; what is left, or all where there are fewer items than SMs,
+// is split along the depth if that is sooner done than one more round of whole items.  A step takes 0.44 us where few
+// blocks run, and the sums' way through the cluster 3 us (7 steps).  Measured, without / with: 128 rows of 7168 x 7168
+// 26.1 / 17.1 us, 512 of 2048 x 7168 26.4 / 15.6.
 template <int kEpilogue, bool kColumnScales>
 bool launch_whole(const Product &p, cudaStream_t stream) {
-    const uint32_t parts = wide_parts<kEpilogue, kColumnScales>(p);
-    return parts > 1u ? launch_wide<kEpilogue, kColumnScales, true>(p, parts, stream)
-                      : launch_wide<kEpilogue, kColumnScales, false>(p, 1u, stream);
+    Maps m;
+    if (!m.make(p)) return false;
+    auto whole = fp8_wide_kernel<kEpilogue, kColumnScales, false>, split = fp8_wide_kernel<kEpilogue, kColumnScales, true>;
+    constexpr uint32_t kBytes = Layout<kColumnScales>::kBytes, kFixed = 7u;
+    if (!set_max_dynamic_smem((const void *)whole, kBytes) || !set_max_dynamic_smem((const void *)split, kBytes)) return false;
+    WideArgs a = args_of(p, BN);
+    const uint32_t sms = (uint32_t)sm_count(), blocks = blocks_of(p.k);
+    const uint64_t items = (uint64_t)((p.rows + BM - 1u) / BM) * a.column_items;
+    if (items > 0x7fffffffull) return false;
+    const uint32_t left = (uint32_t)(items % sms);
+    uint32_t parts = 1u;
+    if (left != 0u) {
+        parts = best_parts(left, blocks, kSlotBlocks, kFixed, [&](uint32_t size) {
+            return size == 1u ? sms : active_clusters((const void *)split, size, kThreads, kBytes);
+        });
+    }
+    a.split_blocks = ((blocks + parts - 1u) / parts + kSlotBlocks - 1u) / kSlotBlocks * kSlotBlocks;
+    const bool cut = parts > 1u && a.split_blocks + kFixed < blocks;
+    a.items = (uint32_t)items - (cut ? left : 0u);
+    a.b_ready = p.b_ready;
+    if (a.items != 0u) {
+        if (!launch_chained(whole, std::min(a.items, sms), kThreads, kBytes, stream, m.a, m.b, m.b2, a)) return false;
+        a.b_ready = true;                          // the launch in front is then the one above
+    }
+    a.first_item = a.items;
+    return !cut || launch_chained_cluster(split, dim3(parts, left), kThreads, dim3(parts, 1, 1), kBytes, stream, m.a, m.b, m.b2, a);
 }
 
 }  // namespace
 
 bool k3::fp8::wide_product(const Product &p, cudaStream_t stream) {
-    if (p.epilogue == kOutActivated) return launch_wide<kOutActivated, false, false>(p, 1u, stream);
-    if (p.offsets) {
-        return p.epilogue == kOutF32 ? launch_wide<kOutF32, false, false>(p, 1u, stream)
-                                       : launch_wide<kOutBf16, false, false>(p, 1u, stream);
-    }
+    if (p.epilogue == kOutActivated) return launch_grouped<kOutActivated>(p, stream);
+    if (p.offsets) return p.epilogue == kOutF32 ? launch_grouped<kOutF32>(p, stream) : launch_grouped<kOutBf16>(p, stream);
     if (p.b_scale_layout == K3_MOE_FP8_ROWS) {
         return p.epilogue == kOutF32 ? launch_whole<kOutF32, true>(p, stream) : launch_whole<kOutBf16, true>(p, stream);
     }
