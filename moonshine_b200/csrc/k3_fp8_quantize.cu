@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(RowsArgs a) {
 constexpr uint32_t kTileColumns = 64, kTileWords = 33;                // words per column, one to spare
 
 template <bool kF32, bool kVector>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kF32 ? 4 : 6)
 quantize_columns_kernel(uint8_t *codes, float *scales, const void *x, uint32_t rows, uint32_t columns) {
     __shared__ uint32_t largest[8][kTileColumns];
     __shared__ uint32_t tile[kTileColumns * kTileWords];

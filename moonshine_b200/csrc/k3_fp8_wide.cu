@@ -70,7 +70,7 @@ struct WideArgs {
     uint32_t items;                                                  // one matrix: items of this launch
     uint32_t first_item;                                             // kSplit: and the first of them
     uint32_t split_blocks;                                           // kSplit: blocks of 128 per part, a multiple of 4
-    bool b_ready;                                                    // kSplit: Product::b_ready
+    bool b_ready;                                                    // Product::b_ready
     int accumulate;
     int activation;
     float beta, linear_beta;
@@ -195,7 +195,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         tmem_alloc(tmem_slot, 512u);
         tmem_relinquish();
     }
-    pdl_wait();
+    if (!a.b_ready) pdl_wait();                                      // otherwise every role waits for itself
     if (a.offsets != nullptr) {
         // exclusive prefix of the groups' row tiles, one warp, 32 groups at a time
         if (warp == 2u) {
@@ -233,7 +233,12 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 if (kSplit) {
                     const Item it = item_of(0u);
                     early = min(L::kStages, it.kb_end - it.kb_begin);
+                } else if (a.b_ready && first_item < total) {
+                    const Item it = item_of(first_item);
+                    early = min(L::kStages, blocks);
+                    for (uint32_t i = 0; i < early; i++) load_b(it, i, i);
                 }
+                if (a.b_ready) pdl_wait();
                 for (uint32_t w = first_item; ok && w < total; w += step) {
                     const Item it = item_of(w);
                     for (uint32_t kb = it.kb_begin; kb < it.kb_end; kb++) {
@@ -283,6 +288,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             }
         } else if (warp == 2u) {
             // ------------------------------------------------------------- scales, a slot at a time
+            if (a.b_ready) pdl_wait();
             uint32_t slot = 0u, ph = 0u;
             bool ok = true;
             const uint32_t pitch = (blocks + 3u) & ~3u, b_blocks = blocks_of(a.n);
@@ -340,6 +346,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     } else {
         // ---------------------------------------------------------------------- running sums
         more_registers<232>();
+        if (a.b_ready) pdl_wait();                                   // before the first store
         const uint32_t q = warp % 4u, half = (warp - 4u) / 4u;
         // a thread's 128 sums are columns first, first + 1, .. of the tile, and 64 more from second
         const uint32_t first = kEpilogue == kOutActivated ? half * 64u : half * 128u;
@@ -577,6 +584,7 @@ WideArgs args_of(const Product &p, uint32_t columns) {
     a.n = p.n;
     a.k = p.k;
     a.column_items = (p.n + columns - 1u) / columns;
+    a.b_ready = p.b_ready;
     a.accumulate = p.accumulate;
     a.activation = p.activation;
     a.beta = p.beta;
@@ -630,7 +638,6 @@ bool launch_whole(const Product &p, cudaStream_t stream) {
     a.split_blocks = ((blocks + parts - 1u) / parts + kSlotBlocks - 1u) / kSlotBlocks * kSlotBlocks;
     const bool cut = parts > 1u && a.split_blocks + kFixed < blocks;
     a.items = (uint32_t)items - (cut ? left : 0u);
-    a.b_ready = p.b_ready;
     if (a.items != 0u) {
         if (!launch_chained(whole, std::min(a.items, sms), kThreads, kBytes, stream, m.a, m.b, m.b2, a)) return false;
         a.b_ready = true;                          // the launch in front is then the one above
