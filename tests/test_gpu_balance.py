@@ -215,3 +215,27 @@ def test_unaligned_rows():
     d = router.backward(view, ids.cuda(), counts, device(cuts), d_loss.cuda(), d_weights.cuda())
     e = router.backward(logits.cuda(), ids.cuda(), counts, device(cuts), d_loss.cuda(), d_weights.cuda())
     assert bool(((d - e).abs() <= 1e-5 * e.abs() + 1e-8).all())
+
+
+def test_logits_of_more_than_four_billion_values():
+    """The last tokens of a long batch give what they give alone."""
+    tokens, experts, tail = 4_300_001, 1000, 9
+    logits, ids, _, d_loss, d_weights = case(12, tail, experts, 2, 1)
+    long_logits = torch.zeros(tokens, experts, device="cuda")
+    long_ids = torch.zeros(tokens, 2, dtype=torch.int32, device="cuda")
+    long_ids[:, 1] = 1
+    long_logits[-tail:], long_ids[-tail:] = logits.cuda(), ids.cuda()
+    assert long_logits.numel() > 1 << 32
+    router = balance.RouterBalance(experts, 2, "sigmoid", ALPHA, SCALE)
+    cuts = device([0, tokens - tail, tokens])
+    counts, loss, means = router.forward(long_logits, long_ids, cuts)
+    alone = router.forward(logits.cuda(), ids.cuda())
+    assert torch.equal(counts[1:], alone[0])
+    assert bool(((means[1:] - alone[2]).abs() <= REL * alone[2]).all())
+    assert counts[0].tolist()[:3] == [tokens - tail, tokens - tail, 0]
+    both = torch.cat([torch.ones(1), d_loss]).cuda()
+    long_weights = torch.zeros(tokens, 2, device="cuda")
+    long_weights[-tail:] = d_weights.cuda()
+    d = router.backward(long_logits, long_ids, counts, cuts, both, long_weights)
+    e = router.backward(logits.cuda(), ids.cuda(), alone[0], None, d_loss.cuda(), d_weights.cuda())
+    assert torch.equal(d[-tail:], e)

@@ -147,6 +147,21 @@ def test_product(m, n, k, layout):
     assert bool(((plain.cpu().double() - want).abs() <= bound(av, bv, k, torch.zeros_like(want)) + want.abs() * 2.0 ** -23).all())
 
 
+@pytest.mark.parametrize("layout", [ops.FP8_BLOCKS, ops.FP8_ROWS])
+@pytest.mark.parametrize("m,n,k", [(2500, 2100, 2050), (700, 4000, 3000)])
+def test_product_of_more_items_than_sms(m, n, k, layout):
+    """Whole items for every SM, and the ones that are left split along the depth."""
+    a, b = normal(m + 1, m, k).cuda(), normal(n + 2, n, k, scale=0.02).cuda()
+    qa, sa = fp8.quantize_rows(a)
+    qb, sb = (fp8.quantize_rows if layout == ops.FP8_ROWS else fp8.quantize_blocks)(b)
+    av = R.values(qa[:, :k].cpu(), sa.cpu()[:, :-(-k // 128)], 1)
+    bv = R.values(qb[:, :k].cpu(), sb.cpu()[:, :-(-k // 128)], 1 if layout == ops.FP8_ROWS else R.BLOCK)
+    want = av @ bv.t()
+    out = torch.empty(m, n, device="cuda")
+    assert ops.k3_moe_fp8_product(out, dirty(qa, k), sa, dirty(qb, k), sb, m, n, k, layout, ops.FP8_F32, 0)
+    assert bool(((out.cpu().double() - want).abs() <= bound(av, bv, k, torch.zeros_like(want)) + want.abs() * 2.0 ** -23).all())
+
+
 @pytest.mark.parametrize("m", [1, 40, 300])
 def test_product_of_large_and_small_scales(m):
     """Blocks 2^60 apart: each is scaled on its own."""
@@ -312,6 +327,28 @@ def test_a_token_that_is_not_finite_stays_alone():
     assert bool(torch.isnan(got[13]).all())
     keep = [i for i in range(50) if i != 13]
     assert torch.equal(got[keep], clean[keep])
+
+
+@pytest.mark.parametrize("tokens", [1, 40, 600])
+def test_tables_of_more_than_four_gigabytes(tokens):
+    """The last expert of a large table gives the bits that it gives alone."""
+    experts, hidden, expert_hidden = 300, 7168, 2048
+    g = torch.Generator(device="cuda").manual_seed(3)
+    tables = []
+    for r, c in ((expert_hidden, hidden), (expert_hidden, hidden), (hidden, expert_hidden)):
+        codes = torch.empty(experts, r, c, dtype=torch.uint8, device="cuda").random_(0, 256, generator=g)
+        codes[-1] &= 0xf7                                                   # no NaN codes (0x7f, 0xff)
+        scales = torch.rand(experts, -(-r // 128), -(-c // 128), generator=g, device="cuda") * 1e-4
+        tables.append((codes.view(E4M3), scales))
+    assert tables[0][0].numel() > 1 << 32
+    x = normal(6, tokens, hidden).cuda()
+    weights = torch.rand(tokens, 1, generator=g, device="cuda")
+    last = torch.full((tokens, 1), experts - 1, dtype=torch.int32, device="cuda")
+    got = expert_layer(tables, 1, "situ").forward(x, last, weights)
+    # alone, among as many experts that nobody selects as the choice of kernel (by rows per expert) wants
+    alone = [(torch.cat([c[-1:]] * 16), torch.cat([s[-1:]] * 16)) for c, s in tables]
+    want = expert_layer(alone, 1, "situ").forward(x, torch.full_like(last, 15), weights)
+    assert bool(torch.isfinite(want).all()) and torch.equal(got, want)
 
 
 def test_another_stream_and_a_captured_call():
