@@ -47,6 +47,8 @@ def _matrix(x: torch.Tensor, name: str, columns: int | None = None, dtypes=(torc
     if len(shape) != 2 or x.dtype not in dtypes or (columns is not None and shape[1] != columns):
         raise ValueError(f"{name}: expected [rows, {columns if columns is not None else 'columns'}] of "
                          f"{' or '.join(str(d) for d in dtypes)}, got {list(shape)} {x.dtype}")
+    if not x.is_cuda:
+        raise ValueError(f"{name}: expected a CUDA tensor")
     return shape
 
 
@@ -194,8 +196,8 @@ class Fp8Experts:
         ``shared`` (bf16, the shared expert's output) if given."""
         tokens, _ = _matrix(x, "x", self.hidden)
         for name, t, dtype in (("ids", ids, torch.int32), ("weights", weights, torch.float32)):
-            if t.dtype is not dtype or t.shape != (tokens, self.top_k):
-                raise ValueError(f"{name}: expected {dtype} {[tokens, self.top_k]}, got {t.dtype} {list(t.shape)}")
+            if t.dtype is not dtype or t.shape != (tokens, self.top_k) or not t.is_cuda:
+                raise ValueError(f"{name}: expected {dtype} {[tokens, self.top_k]} on the GPU, got {t.dtype} {list(t.shape)}")
         if shared is not None and _matrix(shared, "shared", self.hidden)[0] != tokens:
             raise ValueError("shared: another number of tokens than x")
         out = x.new_empty((tokens, self.hidden))
