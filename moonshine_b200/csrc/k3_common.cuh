@@ -228,32 +228,39 @@ inline bool set_max_dynamic_smem(const void *kernel, size_t bytes) {
     return true;
 }
 
-// Clusters of `size` blocks of `kernel` that the current device holds at once, remembered per (device, kernel, size).
+// How many clusters of 1 to 8 blocks of `kernel` the current device holds at once, remembered per (device, kernel).
 // A cluster lies within a group of 16 to 20 SMs, so sizes that do not divide such a group well leave SMs
 // without work: five blocks of a whole SM each fit about 24 times instead of 29.
-inline uint32_t active_clusters(const void *kernel, uint32_t size, uint32_t threads, size_t smem) {
+struct ActiveClusters {
+    uint32_t of_size[9];             // [1 .. 8]; 0: not at all
+};
+inline ActiveClusters active_clusters(const void *kernel, uint32_t threads, size_t smem) {
     static std::mutex lock;
-    static std::map<std::pair<std::pair<int, uint32_t>, const void *>, uint32_t> known;
-    const auto key = std::make_pair(std::make_pair(current_device(), size), kernel);
+    static std::map<std::pair<int, const void *>, ActiveClusters> known;
+    const auto key = std::make_pair(current_device(), kernel);
     std::lock_guard<std::mutex> guard(lock);
     auto it = known.find(key);
     if (it == known.end()) {
-        cudaLaunchAttribute attribute{};
-        attribute.id = cudaLaunchAttributeClusterDimension;
-        attribute.val.clusterDim.x = size;
-        attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-        cudaLaunchConfig_t config{};
-        config.gridDim = dim3(size, 1, 1);
-        config.blockDim = dim3(threads, 1, 1);
-        config.dynamicSmemBytes = smem;
-        config.attrs = &attribute;
-        config.numAttrs = 1;
-        int n = 0;
-        if (cudaOccupancyMaxActiveClusters(&n, kernel, &config) != cudaSuccess || n <= 0) {
-            (void)cudaGetLastError();
-            n = 0;
+        ActiveClusters c{};
+        for (uint32_t size = 1; size <= 8u; size++) {
+            cudaLaunchAttribute attribute{};
+            attribute.id = cudaLaunchAttributeClusterDimension;
+            attribute.val.clusterDim.x = size;
+            attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+            cudaLaunchConfig_t config{};
+            config.gridDim = dim3(size, 1, 1);
+            config.blockDim = dim3(threads, 1, 1);
+            config.dynamicSmemBytes = smem;
+            config.attrs = &attribute;
+            config.numAttrs = 1;
+            int n = 0;
+            if (cudaOccupancyMaxActiveClusters(&n, kernel, &config) != cudaSuccess || n < 0) {
+                (void)cudaGetLastError();
+                n = 0;
+            }
+            c.of_size[size] = (uint32_t)n;
         }
-        it = known.emplace(key, (uint32_t)n).first;
+        it = known.emplace(key, c).first;
     }
     return it->second;
 }

@@ -2,10 +2,8 @@
 // products (k3_fp8_product.cu), experts (k3_fp8_experts.cu).
 #pragma once
 
+#include "k3_common.cuh"
 #include "k3_moe_fp8.h"
-
-#include <cuda_runtime.h>
-#include <stdint.h>
 
 namespace k3::fp8 {
 
@@ -60,14 +58,13 @@ bool product(const Product &p, cudaStream_t stream);
 
 // Parts that the depth of an item is cut into, a cluster of one block per part: the number with the shortest time for
 // `items` items of `blocks` steps each, where a wave of as many clusters as fit takes the steps of a part (a multiple of
-// `multiple`) and `fixed` steps more.  active(size): clusters that fit at once.
-template <typename F>
-uint32_t best_parts(uint64_t items, uint32_t blocks, uint32_t multiple, uint32_t fixed, F active) {
+// `multiple`) and `fixed` steps more.
+inline uint32_t best_parts(uint64_t items, uint32_t blocks, uint32_t multiple, uint32_t fixed, const ActiveClusters &active) {
     uint32_t best = 1u;
     uint64_t shortest = ~0ull;
     for (uint32_t s = 1u; s <= 8u; s++) {
         const uint32_t steps = ((blocks + s - 1u) / s + multiple - 1u) / multiple * multiple, parts = (blocks + steps - 1u) / steps;
-        const uint32_t fit = parts == s ? active(s) : 0u;               // a number of parts that rounding does not give
+        const uint32_t fit = parts == s ? active.of_size[s] : 0u;               // a number of parts that rounding does not give
         if (fit == 0u) continue;
         const uint64_t time = (items + fit - 1u) / fit * (steps + fixed);
         if (time < shortest) {

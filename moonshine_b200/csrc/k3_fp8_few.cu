@@ -704,9 +704,8 @@ bool launch_split(const Product &p, const void *x, cudaStream_t stream) {
     auto kernel = fp8_few_kernel<kEpilogue, 1, kRows, true, kQuantize, kToken>;
     if (!set_max_dynamic_smem((const void *)kernel, L::kBytes)) return false;
     // a launch, the first loads and the sums' way through the cluster take as long as 8 steps
-    const uint32_t parts = best_parts((uint64_t)tiles * row_tiles, blocks, 1u, 8u, [&](uint32_t size) {
-        return active_clusters((const void *)kernel, size, L::kThreads, L::kBytes);
-    });
+    const uint32_t parts = best_parts((uint64_t)tiles * row_tiles, blocks, 1u, 8u,
+                                      active_clusters((const void *)kernel, L::kThreads, L::kBytes));
     a.split_blocks = (blocks + parts - 1u) / parts;
     return launch_chained_cluster(kernel, dim3(parts, tiles, row_tiles), L::kThreads, dim3(parts, 1, 1), L::kBytes, stream, a_map,
                                   b_map, b_map, a);
