@@ -374,7 +374,7 @@ extern "C" bool k3_moe_fp8_quantize_blocks(void *codes, void *scales, const void
 extern "C" bool k3_moe_fp8_transpose_blocks(void *codes_out, void *scales_out, const void *codes, const void *scales,
                                             uint32_t rows, uint32_t columns, void *stream) {
     if (!codes_out || !scales_out || !codes || !scales || codes_out == codes || !aligned16(codes_out) || !aligned16(codes) ||
-        !extent_ok(rows) || !extent_ok(columns) || blocks_of(rows) > 65535u) {
+        (((uintptr_t)scales_out | (uintptr_t)scales) & 3u) != 0u || !extent_ok(rows) || !extent_ok(columns) || blocks_of(rows) > 65535u) {
         return false;
     }
     return launch_chained(transpose_blocks_kernel, dim3(blocks_of(columns), blocks_of(rows)), kThreads, 0, (cudaStream_t)stream,

@@ -22,6 +22,13 @@
 //
 // Every wait is bounded; on give-up the block raises the status word, waits for its copies and frees its
 // tensor memory.
+//
+// Measured, 8192 x 7168 x 7168: 374 us = 2.25 PFLOP/s in a burst at 1965 MHz, 436 us = 1.93 back to back,
+// where the power limit holds the clock at 1410 MHz.  With half of the reads and adds left out (a wrong
+// result) it takes 331 and 388 us: power bounds what is left.  Pairs of blocks (cta_group::2), which halve
+// b's way from L2, take the same time with arrivals across the pair that carry no release, and twice as
+// long with release.  Loads of 64 columns at once, or the next block's before the last adds, change
+// nothing or cost 5 %.
 #include "k3_fp8_ptx.cuh"
 #include "k3_grouped.h"
 #include "k3_moe_layer.h"
@@ -648,7 +655,7 @@ bool launch_whole(const Product &p, cudaStream_t stream) {
 
 bool k3::fp8::wide_product(const Product &p, cudaStream_t stream) {
     if (p.epilogue == kOutActivated) return launch_grouped<kOutActivated>(p, stream);
-    if (p.offsets) return p.epilogue == kOutF32 ? launch_grouped<kOutF32>(p, stream) : launch_grouped<kOutBf16>(p, stream);
+    if (p.offsets) return launch_grouped<kOutBf16>(p, stream);
     if (p.b_scale_layout == K3_MOE_FP8_ROWS) {
         return p.epilogue == kOutF32 ? launch_whole<kOutF32, true>(p, stream) : launch_whole<kOutBf16, true>(p, stream);
     }
