@@ -27,16 +27,32 @@ constexpr uint32_t kForwardStages = 3, kBackwardStages = 2;   // rows of a warp 
 
 __device__ uint32_t g_balance_status = 0;          // 2: an expert id >= experts
 
+// Blocks of the backward pass on an SM, two in the forward pass.  30000 x 160, us with two / three / four: backward 19.7 / 17.1 /
+// 17.0, forward 11.5 / 10.4 / 10.2, and the second stage, which has a partial row for each block, 8.3 / 9.5 / 10.8.
+constexpr uint32_t kForwardPerSm = 2;
+constexpr uint32_t backward_per_sm(uint32_t groups) { return groups <= 4u ? 3u : 2u; }
+
 struct Shape {
     uint32_t tokens, sequences, experts, top_k;
     uint32_t chunk;                                // tokens per block
     int softmax;
 };
 
-// The fast exponential and quotient (2 units in the last place each, of an argument's size the exponent's): 4e-7 of
-// a score.  With expf and the rounded quotient the pass over the logits was bound by its instructions,
-// 32768 x 896 forward and backward 198 us.
-K3_DEVINL float sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
+// The fast base-2 exponential and reciprocal (2 units in the last place each, of an argument's size the
+// exponential's): 4e-7 of a score.  With expf, a rounded quotient and single operations the pass over the
+// logits was bound by its instructions, 32768 x 896 forward and backward 198 us.
+K3_DEVINL float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+K3_DEVINL float reciprocal_fast(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+constexpr float kLog2E = 1.44269504f;
+K3_DEVINL float sigmoid(float x) { return reciprocal_fast(1.0f + exp2_fast(x * -kLog2E)); }
 
 template <int kBytes>
 K3_DEVINL void copy_async(float *to, const float *from) {
@@ -52,37 +68,42 @@ struct Softmax {
     float top, over;                               // a score is exp(logit - top) * over
 };
 
-// A warp's row: kV groups of four experts per lane, neighbours (kVector) or 32 apart.
+// A warp's row: kV groups of four experts per lane, neighbours (kVector) or 32 apart, two to a register pair.
 template <uint32_t kV, bool kVector>
 struct Row {
-    float v[kV * 4u];
+    uint64_t v[kV * 2u];
+    // expert of element i of this lane
     static K3_DEVINL uint32_t expert(uint32_t i, uint32_t lane) {
         return kVector ? (i / 4u) * 128u + lane * 4u + i % 4u : i * 32u + lane;
     }
-    // elements i .. i + 3 (i a multiple of 4) of a row in memory, and back
+    // group g (elements 4 g .. 4 g + 3) of a row in memory, and back
     template <typename T>
-    static K3_DEVINL void get4(float (&to)[4], const T *row, uint32_t experts, uint32_t lane, uint32_t i, float fill) {
+    static K3_DEVINL void get(uint64_t (&to)[2], const T *row, uint32_t experts, uint32_t lane, uint32_t g, float fill) {
+        float q[4];
         if (kVector) {
-            const uint32_t e = expert(i, lane);
-            uint4 q = make_uint4(0u, 0u, 0u, 0u);
-            if (e < experts) q = *reinterpret_cast<const uint4 *>(row + e);
-            to[0] = e < experts ? value(q.x, row) : fill;
-            to[1] = e < experts ? value(q.y, row) : fill;
-            to[2] = e < experts ? value(q.z, row) : fill;
-            to[3] = e < experts ? value(q.w, row) : fill;
+            const uint32_t e = expert(4u * g, lane);
+            uint4 bits = make_uint4(0u, 0u, 0u, 0u);
+            if (e < experts) bits = *reinterpret_cast<const uint4 *>(row + e);
+            q[0] = e < experts ? value(bits.x, row) : fill;
+            q[1] = e < experts ? value(bits.y, row) : fill;
+            q[2] = e < experts ? value(bits.z, row) : fill;
+            q[3] = e < experts ? value(bits.w, row) : fill;
         } else {
 #pragma unroll
-            for (uint32_t j = 0; j < 4u; j++) to[j] = expert(i + j, lane) < experts ? (float)row[expert(i + j, lane)] : fill;
+            for (uint32_t j = 0; j < 4u; j++) q[j] = expert(4u * g + j, lane) < experts ? (float)row[expert(4u * g + j, lane)] : fill;
         }
+        to[0] = pack2(q[0], q[1]);
+        to[1] = pack2(q[2], q[3]);
     }
-    static K3_DEVINL void put4(float *row, const float (&from)[4], uint32_t experts, uint32_t lane, uint32_t i) {
+    static K3_DEVINL void put(float *row, const uint64_t (&from)[2], uint32_t experts, uint32_t lane, uint32_t g) {
+        const float q[4] = {lo2(from[0]), hi2(from[0]), lo2(from[1]), hi2(from[1])};
         if (kVector) {
-            const uint32_t e = expert(i, lane);
-            if (e < experts) *reinterpret_cast<float4 *>(row + e) = make_float4(from[0], from[1], from[2], from[3]);
+            const uint32_t e = expert(4u * g, lane);
+            if (e < experts) *reinterpret_cast<float4 *>(row + e) = make_float4(q[0], q[1], q[2], q[3]);
         } else {
 #pragma unroll
             for (uint32_t j = 0; j < 4u; j++) {
-                if (expert(i + j, lane) < experts) row[expert(i + j, lane)] = from[j];
+                if (expert(4u * g + j, lane) < experts) row[expert(4u * g + j, lane)] = q[j];
             }
         }
     }
@@ -98,59 +119,74 @@ struct Row {
     template <typename T>
     K3_DEVINL void load(const T *row, uint32_t experts, uint32_t lane, float fill) {
 #pragma unroll
-        for (uint32_t i = 0; i < kV * 4u; i += 4u) {
-            float q[4];
-            get4(q, row, experts, lane, i, fill);
-#pragma unroll
-            for (uint32_t j = 0; j < 4u; j++) v[i + j] = q[j];
+        for (uint32_t g = 0; g < kV; g++) {
+            uint64_t q[2];
+            get(q, row, experts, lane, g, fill);
+            v[2u * g] = q[0];
+            v[2u * g + 1u] = q[1];
         }
     }
     K3_DEVINL void store(float *row, uint32_t experts, uint32_t lane) const {
 #pragma unroll
-        for (uint32_t i = 0; i < kV * 4u; i += 4u) {
-            const float q[4] = {v[i], v[i + 1u], v[i + 2u], v[i + 3u]};
-            put4(row, q, experts, lane, i);
+        for (uint32_t g = 0; g < kV; g++) {
+            const uint64_t q[2] = {v[2u * g], v[2u * g + 1u]};
+            put(row, q, experts, lane, g);
         }
     }
     static K3_DEVINL float value(uint32_t bits, const float *) { return __uint_as_float(bits); }
     static K3_DEVINL float value(uint32_t bits, const uint32_t *) { return (float)bits; }
-    K3_DEVINL float sum() const {
-        float s = 0.f;
+    K3_DEVINL void fill(float x) {
 #pragma unroll
-        for (uint32_t i = 0; i < kV * 4u; i++) s += v[i];
-        return warp_sum(s);
+        for (uint32_t i = 0; i < kV * 2u; i++) v[i] = pack2(x, x);
+    }
+    K3_DEVINL void scale(float x) {
+        const uint64_t by = pack2(x, x);
+#pragma unroll
+        for (uint32_t i = 0; i < kV * 2u; i++) v[i] = mul2(v[i], by);
+    }
+    K3_DEVINL float sum() const {
+        uint64_t s = v[0];
+#pragma unroll
+        for (uint32_t i = 1; i < kV * 2u; i++) s = add2(s, v[i]);
+        return warp_sum(lo2(s) + hi2(s));
     }
     // logits -> scores; experts past the end have the logit -inf and get the score 0
     K3_DEVINL Softmax scores(int softmax) {
         Softmax f{0.f, 0.f};
         if (!softmax) {
+            const uint64_t by = pack2(-kLog2E, -kLog2E), one = pack2(1.0f, 1.0f);
 #pragma unroll
-            for (uint32_t i = 0; i < kV * 4u; i++) v[i] = sigmoid(v[i]);
+            for (uint32_t i = 0; i < kV * 2u; i++) {
+                const uint64_t t = mul2(v[i], by), y = add2(pack2(exp2_fast(lo2(t)), exp2_fast(hi2(t))), one);
+                v[i] = pack2(reciprocal_fast(lo2(y)), reciprocal_fast(hi2(y)));
+            }
             return f;
         }
         f.top = -INFINITY;
 #pragma unroll
-        for (uint32_t i = 0; i < kV * 4u; i++) f.top = fmaxf(f.top, v[i]);
+        for (uint32_t i = 0; i < kV * 2u; i++) f.top = fmaxf(f.top, fmaxf(lo2(v[i]), hi2(v[i])));
         f.top = warp_max(f.top);
         if (f.top == -INFINITY) {                  // every logit is -inf, or NaN, which fmaxf drops
             float s = 0.f;
 #pragma unroll
-            for (uint32_t i = 0; i < kV * 4u; i++) s += v[i] != v[i] ? v[i] : 0.f;
+            for (uint32_t i = 0; i < kV * 2u; i++) {
+                const float a = lo2(v[i]), b = hi2(v[i]);
+                s += (a != a ? a : 0.f) + (b != b ? b : 0.f);
+            }
             f.top = 0.f;
             f.over = warp_sum(s);                  // 0, or NaN
-#pragma unroll
-            for (uint32_t i = 0; i < kV * 4u; i++) v[i] = 0.f;
-        } else {
-            float s = 0.f;
-#pragma unroll
-            for (uint32_t i = 0; i < kV * 4u; i++) {
-                v[i] = __expf(v[i] - f.top);
-                s += v[i];
-            }
-            f.over = 1.0f / warp_sum(s);
+            fill(f.over);
+            return f;
         }
+        // the difference first: a product with the logarithm of the lowest values would not be finite
+        const uint64_t less = pack2(-f.top, -f.top), by = pack2(kLog2E, kLog2E);
 #pragma unroll
-        for (uint32_t i = 0; i < kV * 4u; i++) v[i] *= f.over;
+        for (uint32_t i = 0; i < kV * 2u; i++) {
+            const uint64_t t = mul2(add2(v[i], less), by);
+            v[i] = pack2(exp2_fast(lo2(t)), exp2_fast(hi2(t)));
+        }
+        f.over = 1.0f / sum();
+        scale(f.over);
         return f;
     }
 };
@@ -188,8 +224,7 @@ K3_DEVINL void sum_tokens(float *rows_s, const float *logits, const uint32_t *id
         copies_commit();
     };
     Row<kV, kVector> acc;
-#pragma unroll
-    for (uint32_t i = 0; i < kV * 4u; i++) acc.v[i] = 0.f;
+    acc.fill(0.f);
     const uint32_t t = first + warp;
     if (logits) {
 #pragma unroll
@@ -210,9 +245,10 @@ K3_DEVINL void sum_tokens(float *rows_s, const float *logits, const uint32_t *id
             Row<kV, kVector> p;
             p.load(mine + stage * kPitch, kPitch, lane, 0.f);
             p.scores(a.softmax);
-            const float r = a.softmax ? 1.0f : __fdividef(1.0f, kTiny + p.sum());
+            const float r = a.softmax ? 1.0f : reciprocal_fast(kTiny + p.sum());
+            const uint64_t r2 = pack2(r, r);
 #pragma unroll
-            for (uint32_t i = 0; i < kV * 4u; i++) acc.v[i] = fmaf(p.v[i], r, acc.v[i]);
+            for (uint32_t i = 0; i < kV * 2u; i++) acc.v[i] = fma2(p.v[i], r2, acc.v[i]);
             if (++stage == kForwardStages) stage = 0u;
         }
         if (lane < a.top_k) {
@@ -229,7 +265,7 @@ K3_DEVINL void sum_tokens(float *rows_s, const float *logits, const uint32_t *id
 }
 
 template <uint32_t kV, bool kVector>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, kForwardPerSm)
 balance_tokens_kernel(float *part_sums, uint32_t *part_counts, const float *logits, const uint32_t *ids, const uint32_t *offsets,
                       Shape a) {
     constexpr uint32_t kPitch = kV * 128u;
@@ -372,7 +408,7 @@ balance_sequences_kernel(uint32_t *counts, float *loss, float *means, const floa
 // --------------------------------------------------------------------------------------- backward
 // A warp's tokens follow one another, so a sequence's shares f stay in registers while it lasts.
 template <uint32_t kV, bool kVector>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, backward_per_sm(kV))
 router_backward_kernel(float *d_logits, const float *logits, const uint32_t *ids, const uint32_t *counts, const uint32_t *offsets,
                        const float *d_loss, const float *d_weights, Shape a, float coefficient, float route_scale) {
     constexpr uint32_t kPitch = kV * 128u;
@@ -399,11 +435,10 @@ router_backward_kernel(float *d_logits, const float *logits, const uint32_t *ids
         if (t < last) Row<kV, kVector>::fetch(mine + stage * kPitch, logits + (uint64_t)t * a.experts, a.experts, lane);
         copies_commit();
     };
-    auto fetch_choice = [&](uint32_t t) {
-        if (d_weights && t < last) {
-            next_id = lane < a.top_k ? ids[(uint64_t)t * a.top_k + lane] : 0xffffffffu;
-            if (lane < a.top_k && next_id >= a.experts) g_balance_status = 2u;
-            next_w = next_id < a.experts ? d_weights[(uint64_t)t * a.top_k + lane] : 0.f;
+    auto fetch_choice = [&](uint32_t t) {          // neither load waits for the other; the id is looked at when its token comes
+        if (d_weights && t < last && lane < a.top_k) {
+            next_id = ids[(uint64_t)t * a.top_k + lane];
+            next_w = d_weights[(uint64_t)t * a.top_k + lane];
         }
     };
 #pragma unroll
@@ -413,7 +448,7 @@ router_backward_kernel(float *d_logits, const float *logits, const uint32_t *ids
     for (uint32_t t = first; t < last; t++) {
         fetch(t + kBackwardStages - 1u, stage == 0u ? kBackwardStages - 1u : stage - 1u);
         const uint32_t id = next_id;
-        const float w = next_w;
+        const float w = id < a.experts ? next_w : 0.f;
         fetch_choice(t + 1u);
         copies_wait<kBackwardStages - 1>();
         __syncwarp();                              // the lanes' chosen lie in one another's copies
@@ -428,40 +463,46 @@ router_backward_kernel(float *d_logits, const float *logits, const uint32_t *ids
             if (t >= end) {                        // past the last sequence: no loss
                 end = a.tokens;
                 c = 0.f;
-#pragma unroll
-                for (uint32_t i = 0; i < kV * 4u; i++) f.v[i] = 0.f;
+                f.fill(0.f);
             } else {
                 const float length = (float)(end - begin), scale = (float)a.experts / ((float)a.top_k * length);
                 c = coefficient * d_loss[s] / length;
                 f.load(counts + (uint64_t)s * a.experts, a.experts, lane, 0.f);
-#pragma unroll
-                for (uint32_t i = 0; i < kV * 4u; i++) f.v[i] *= scale;
+                f.scale(scale);
             }
         }
         const Softmax soft = p.scores(a.softmax);
         // the loss by a score is by (f - mean)
         float by = c, mean = 0.f;
         if (d_loss && !a.softmax) {
-            float z = 0.f, fp = 0.f;
+            uint64_t z = pack2(0.f, 0.f), fp = z;
 #pragma unroll
-            for (uint32_t i = 0; i < kV * 4u; i++) {
-                z += p.v[i];
-                fp = fmaf(f.v[i], p.v[i], fp);
+            for (uint32_t i = 0; i < kV * 2u; i++) {
+                z = add2(z, p.v[i]);
+                fp = fma2(f.v[i], p.v[i], fp);
             }
-            const float r = __fdividef(1.0f, kTiny + warp_sum(z));
-            mean = warp_sum(fp) * r;
+            const float r = reciprocal_fast(kTiny + warp_sum(lo2(z) + hi2(z)));
+            mean = warp_sum(lo2(fp) + hi2(fp)) * r;
             by = c * r;
         }
         const bool chosen = id < a.experts;
         if (d_weights) {
+            if (lane < a.top_k && !chosen) g_balance_status = 2u;
             // the weights' share at the chosen, through shared memory to the lanes that hold them
-            const float si = !chosen ? 0.f : a.softmax ? __expf(l - soft.top) * soft.over : sigmoid(l);
-            const float under = __fdividef(1.0f, kTiny + warp_sum(si));
-            const float share = route_scale * (w - warp_sum(w * si) * under) * under;
-            const uint32_t same = __match_any_sync(0xffffffffu, chosen ? id : 0x80000000u + lane);
-            if (!__any_sync(0xffffffffu, chosen && (same & (same - 1u)) != 0u)) {
+            const float si = !chosen ? 0.f : a.softmax ? exp2_fast((l - soft.top) * kLog2E) * soft.over : sigmoid(l);
+            const float all = warp_sum(si), weighted = warp_sum(w * si);
+            const float under = reciprocal_fast(kTiny + all);
+            const float share = route_scale * (w - weighted * under) * under;
+            // an expert named twice keeps one of the lanes' numbers (with __match_any_sync for this 30000 x 160 took 32 us
+            // instead of 20)
+            if (chosen) row_s[id] = __uint_as_float(lane);
+            __syncwarp();
+            const bool other = chosen && __float_as_uint(row_s[id]) != lane;
+            if (!__any_sync(0xffffffffu, other)) {
                 if (chosen) row_s[id] = share;
-            } else {                               // an expert named twice: one after the other
+            } else {                               // one after the other
+                if (chosen) row_s[id] = 0.f;
+                __syncwarp();
                 for (uint32_t r = 0; r < a.top_k; r++) {
                     if (lane == r && chosen) row_s[id] += share;
                     __syncwarp();
@@ -469,40 +510,42 @@ router_backward_kernel(float *d_logits, const float *logits, const uint32_t *ids
             }
             __syncwarp();
         }
-        // by the scores i .. i + 3
-        auto by_scores = [&](float (&d)[4], uint32_t i) {
+        // by the scores of group g
+        const uint64_t by2 = pack2(by, by), less = pack2(-mean, -mean);
+        auto by_scores = [&](uint64_t (&d)[2], uint32_t g) {
             if (d_weights) {
-                Row<kV, kVector>::get4(d, row_s, kPitch, lane, i, 0.f);
+                Row<kV, kVector>::get(d, row_s, kPitch, lane, g, 0.f);
             } else {
-                d[0] = d[1] = d[2] = d[3] = 0.f;
+                d[0] = d[1] = pack2(0.f, 0.f);
             }
             if (d_loss) {
-#pragma unroll
-                for (uint32_t j = 0; j < 4u; j++) d[j] = fmaf(by, f.v[i + j] - mean, d[j]);
+                d[0] = fma2(by2, add2(f.v[2u * g], less), d[0]);
+                d[1] = fma2(by2, add2(f.v[2u * g + 1u], less), d[1]);
             }
         };
-        float dp = 0.f;
+        uint64_t dp = pack2(0.f, 0.f);
         if (a.softmax) {
 #pragma unroll
-            for (uint32_t i = 0; i < kV * 4u; i += 4u) {
-                float d[4];
-                by_scores(d, i);
-#pragma unroll
-                for (uint32_t j = 0; j < 4u; j++) dp = fmaf(d[j], p.v[i + j], dp);
+            for (uint32_t g = 0; g < kV; g++) {
+                uint64_t d[2];
+                by_scores(d, g);
+                dp = fma2(d[0], p.v[2u * g], fma2(d[1], p.v[2u * g + 1u], dp));
             }
-            dp = warp_sum(dp);
+            const float all = warp_sum(lo2(dp) + hi2(dp));
+            dp = pack2(-all, -all);
         }
         float *out = d_logits + (uint64_t)t * a.experts;
+        const uint64_t one = pack2(1.0f, 1.0f), minus = pack2(-1.0f, -1.0f);
 #pragma unroll
-        for (uint32_t i = 0; i < kV * 4u; i += 4u) {
-            float d[4];
-            by_scores(d, i);
+        for (uint32_t g = 0; g < kV; g++) {
+            uint64_t d[2];
+            by_scores(d, g);
 #pragma unroll
-            for (uint32_t j = 0; j < 4u; j++) {
-                const float q = p.v[i + j];
-                d[j] = a.softmax ? q * (d[j] - dp) : d[j] * (q * (1.0f - q));
+            for (uint32_t j = 0; j < 2u; j++) {
+                const uint64_t q = p.v[2u * g + j];
+                d[j] = a.softmax ? mul2(q, add2(d[j], dp)) : mul2(d[j], mul2(q, fma2(q, minus, one)));
             }
-            Row<kV, kVector>::put4(out, d, a.experts, lane, i);
+            Row<kV, kVector>::put(out, d, a.experts, lane, g);
         }
         __syncwarp();
         if (d_weights && chosen) row_s[id] = 0.f;
@@ -516,9 +559,11 @@ bool shape_ok(uint32_t tokens, uint32_t sequences, uint32_t experts, uint32_t to
            (score == K3_MOE_SCORE_SIGMOID || score == K3_MOE_SCORE_SOFTMAX);
 }
 
-// Tokens per block of the forward pass: two blocks per SM, the same partial sums on any device, and a token per warp
-// at least.
-constexpr uint32_t kForwardBlocks = 148u * 2u;
+constexpr uint32_t groups_of(uint32_t experts) { return (experts + 127u) / 128u; }
+
+// Blocks of the forward pass's first stage (148 SMs whatever the device: the same partial sums on any), and tokens per
+// block: one per warp at least.
+constexpr uint32_t kForwardBlocks = 148u * kForwardPerSm;
 uint32_t forward_chunk(uint32_t tokens) { return std::max((tokens + kForwardBlocks - 1u) / kForwardBlocks, kWarps); }
 
 struct BalanceWorkspace {
@@ -616,7 +661,7 @@ extern "C" bool k3_moe_balance(void *counts, void *loss, void *means, const void
         return pick<Few>(experts, vector, (uint32_t *)counts, (float *)loss, (float *)means, (const float *)logits, (const uint32_t *)ids,
                          (const uint32_t *)offsets, a, coefficient, stream);
     }
-    const uint32_t slices = (experts + 127u) / 128u;
+    const uint32_t slices = groups_of(experts);
     return pick<Forward>(experts, vector, sums, part_counts, (const float *)logits, (const uint32_t *)ids, (const uint32_t *)offsets,
                          a, stream) &&
            launch_chained_cluster(balance_sequences_kernel, dim3(slices, sequences), 1024, dim3(slices, 1, 1), 0, stream, (uint32_t *)counts, (float *)loss, (float *)means,
@@ -632,7 +677,7 @@ extern "C" bool k3_moe_router_backward(void *d_logits, const void *logits, const
         !words_ok(ids) || !words_ok(counts) || !words_ok(offsets) || !words_ok(d_loss) || !words_ok(d_weights)) {
         return false;
     }
-    const uint32_t warps = (uint32_t)sm_count() * 2u * kWarps;
+    const uint32_t warps = (uint32_t)sm_count() * backward_per_sm(groups_of(experts)) * kWarps;
     const Shape a{tokens, sequences, experts, top_k, std::max((tokens + warps - 1u) / warps, 1u), score};
     const bool vector = experts % 4u == 0u && (((uintptr_t)logits | (uintptr_t)d_logits | (uintptr_t)counts) & 15u) == 0u;
     return pick<Backward>(experts, vector, (float *)d_logits, (const float *)logits, (const uint32_t *)ids, (const uint32_t *)counts,

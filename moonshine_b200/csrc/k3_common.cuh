@@ -69,6 +69,35 @@ K3_DEVINL float warp_max(float v) {
     return v;
 }
 
+// Two f32 in a 64-bit register pair: one instruction for both.
+K3_DEVINL uint64_t pack2(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+K3_DEVINL uint64_t pack2(uint32_t lo, uint32_t hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+    return r;
+}
+K3_DEVINL float lo2(uint64_t v) { return __uint_as_float((uint32_t)v); }
+K3_DEVINL float hi2(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+K3_DEVINL uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+K3_DEVINL uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+K3_DEVINL uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 // 16-byte global load that does not allocate in L1 (weights are streamed once).
 K3_DEVINL uint4 ld_stream_16(const void *p) {
     uint4 v;

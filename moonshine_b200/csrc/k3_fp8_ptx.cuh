@@ -1,5 +1,5 @@
-// What the E4M3 product kernels add to k3_tc_ptx.cuh: the kind::f8f6f4 MMA, packed f32 arithmetic, register
-// shares of warpgroups, tensor maps of code matrices.
+// What the E4M3 product kernels add to k3_tc_ptx.cuh: the kind::f8f6f4 MMA, register shares of
+// warpgroups, scales and codes, tensor maps of code matrices.
 #pragma once
 
 #include "k3_fp8.h"
@@ -27,29 +27,6 @@ K3_DEVINL void mma_e4m3_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, ui
         : "memory");
 }
 
-// Two f32 in a 64-bit register pair: one instruction for both.
-K3_DEVINL uint64_t pack2(float lo, float hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-K3_DEVINL uint64_t pack2(uint32_t lo, uint32_t hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-    return r;
-}
-K3_DEVINL float lo2(uint64_t v) { return __uint_as_float((uint32_t)v); }
-K3_DEVINL float hi2(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
-K3_DEVINL uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-K3_DEVINL uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 K3_DEVINL uint32_t bf16x2(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
