@@ -544,11 +544,15 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 const bool inside = it.column + column < a.n;
                 uint32_t *largest = reinterpret_cast<uint32_t *>(base + L::kLargest) + half * kMine;   // [4][kRows]
                 float act[kMine];
+                auto activate = [&](auto f) {
+#pragma unroll
+                    for (uint32_t j = 0; j < kMine; j++) act[j] = j < n && inside ? f(value(0u, j), value(kTiles - 1u, j)) : 0.f;
+                };
+                if (a.activation == kActSitu) activate(ExpertActivation<true>(a.beta, a.linear_beta));
+                else activate(ExpertActivation<false>(a.beta, a.linear_beta));
 #pragma unroll
                 for (uint32_t j = 0; j < kMine; j++) {
-                    act[j] = 0.f;
                     if (j < n) {
-                        if (inside) act[j] = activated(value(0u, j), value(kTiles - 1u, j), a.activation, a.beta, a.linear_beta);
                         const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(act[j]) & 0x7fffffffu);
                         if (lane == 0u) largest[q * kRows + j] = most;
                     }

@@ -87,6 +87,23 @@ struct Item {
     uint32_t group, row, rows, column, kb_begin, kb_end;
 };
 
+// The first 32 pairs of sums (gate) and the other 32 (up) to 64 activations in the first 32, zero past `left`; the largest
+// magnitude's bits.
+template <bool kSitu>
+K3_DEVINL uint32_t activate(uint64_t (&sum)[64], uint32_t left, float beta, float linear_beta) {
+    const ExpertActivation<kSitu> act(beta, linear_beta);
+    uint32_t most = 0u;
+#pragma unroll
+    for (uint32_t j = 0; j < 32u; j++) {
+        float x = act(lo2(sum[j]), lo2(sum[32u + j])), y = act(hi2(sum[j]), hi2(sum[32u + j]));
+        if (2u * j >= left) x = 0.f;
+        if (2u * j + 1u >= left) y = 0.f;
+        most = max(most, max(__float_as_uint(x) & 0x7fffffffu, __float_as_uint(y) & 0x7fffffffu));
+        sum[j] = pack2(x, y);
+    }
+    return most;
+}
+
 // four neighbouring results at `out`, of which `left` columns exist
 K3_DEVINL void store4(float *out, const float (&sum)[4], uint32_t left, bool vector, int accumulate) {
     float v[4];
@@ -431,26 +448,16 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 }
             } else if (kEpilogue == kOutActivated) {
                 // ------------------------------------------ activation, largest of the row's 128, codes
-                uint32_t most = 0u;
-#pragma unroll
-                for (uint32_t j = 0; j < 32u; j++) {
-                    float v[2];
-#pragma unroll
-                    for (uint32_t p = 0; p < 2u; p++) {
-                        const float g = p ? hi2(sum[j]) : lo2(sum[j]), u = p ? hi2(sum[32u + j]) : lo2(sum[32u + j]);
-                        const bool inside = it.column + first + 2u * j + p < a.n;
-                        v[p] = inside ? activated(g, u, a.activation, a.beta, a.linear_beta) : 0.f;
-                        most = max(most, __float_as_uint(v[p]) & 0x7fffffffu);
-                    }
-                    sum[j] = pack2(v[0], v[1]);
-                }
+                const uint32_t left = it.column + first < a.n ? a.n - it.column - first : 0u;       // columns of the 64 that exist
+                const uint32_t most_here = a.activation == kActSitu ? activate<true>(sum, left, a.beta, a.linear_beta)
+                                                                    : activate<false>(sum, left, a.beta, a.linear_beta);
                 uint32_t *largest = reinterpret_cast<uint32_t *>(base + L::kLargest);
-                largest[half * BM + row_in] = most;
+                largest[half * BM + row_in] = most_here;
                 __syncwarp();
                 if (lane == 0u) mbar_arrive(largest_full);
                 if (!mbar_wait(largest_full, lph, abort_flag)) { ok = false; break; }
                 lph ^= 1u;
-                most = max(most, largest[(half ^ 1u) * BM + row_in]);
+                const uint32_t most = max(most_here, largest[(half ^ 1u) * BM + row_in]);
                 __syncwarp();
                 if (lane == 0u) mbar_arrive(largest_full);            // read: the next item may overwrite it
                 if (!mbar_wait(largest_full, lph, abort_flag)) { ok = false; break; }
