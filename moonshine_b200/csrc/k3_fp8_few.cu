@@ -92,7 +92,7 @@ struct FewArgs {
     uint32_t split_blocks;                         // kSplit: blocks of 128 per part of the depth
     int accumulate;
     int activation;
-    float beta, linear_beta;
+    float beta, by_beta, linear_beta, by_linear_beta;                // by_: the reciprocals
 };
 
 struct Item {
@@ -445,7 +445,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 for (uint32_t i = 0; i < 8u; i++) most = max(most, max((v[p][i] << 16) & 0x7fffffffu, v[p][i] & 0x7fff0000u));
 #pragma unroll
                 for (int o = 4; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-                const float scale = scale_of(most), inverse = __frcp_rn(scale);
+                const float scale = scale_of(most), inverse = inverse_of(scale);
                 uint32_t w[4];
 #pragma unroll
                 for (uint32_t i = 0; i < 4u; i++) {
@@ -548,8 +548,8 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 #pragma unroll
                     for (uint32_t j = 0; j < kMine; j++) act[j] = j < n && inside ? f(value(0u, j), value(kTiles - 1u, j)) : 0.f;
                 };
-                if (a.activation == kActSitu) activate(ExpertActivation<true>(a.beta, a.linear_beta));
-                else activate(ExpertActivation<false>(a.beta, a.linear_beta));
+                if (a.activation == kActSitu) activate(ExpertActivation<true>{a.beta, a.by_beta, a.linear_beta, a.by_linear_beta});
+                else activate(ExpertActivation<false>{});
 #pragma unroll
                 for (uint32_t j = 0; j < kMine; j++) {
                     if (j < n) {
@@ -571,7 +571,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                         if (q == 0u && lane == 0u) a.out_scales[row * scale_pitch + it.column / kBlock] = scale;
                         if (it.column + column < out_pitch) {
                             ((uint8_t *)a.out)[row * out_pitch + it.column + column] =
-                                (uint8_t)codes2(quotient(act[j], scale, __frcp_rn(scale)), 0.f);
+                                (uint8_t)codes2(quotient(act[j], scale, inverse_of(scale)), 0.f);
                         }
                     }
                 }
@@ -688,6 +688,8 @@ FewArgs args_of(const Product &p) {
     a.activation = p.activation;
     a.beta = p.beta;
     a.linear_beta = p.linear_beta;
+    a.by_beta = 1.0f / p.beta;
+    a.by_linear_beta = 1.0f / p.linear_beta;
     return a;
 }
 

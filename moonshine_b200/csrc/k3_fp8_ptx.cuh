@@ -55,7 +55,7 @@ K3_DEVINL void mbar_drain(uint64_t *bar, uint32_t parity) {
 
 // The expert activation with the fast exponential and reciprocal, 4e-7 of the result: it is quantised to 4 bits next.
 // The kind is a template argument, so that many elements go side by side: with a branch in each of a thread's 64
-// the warps waited for one element's chain after the other, 4.5 us a gate/up tile instead of PENDING.
+// the warps waited for one element's chain after the other.
 //
 // tanh x: its Taylor series up to x^11 below 0.4, where the next term is 6e-8 of the value, and 1 - 2 / (1 + e^2x)
 // above, which is off by 1e-7.
@@ -71,8 +71,6 @@ K3_DEVINL float tanh_fast(float x) {
 template <bool kSitu>
 struct ExpertActivation {
     float beta, by_beta, linear, by_linear;        // by_: the reciprocals
-    K3_DEVINL ExpertActivation(float beta_, float linear_)
-        : beta(beta_), by_beta(1.0f / beta_), linear(linear_), by_linear(1.0f / linear_) {}
     K3_DEVINL float operator()(float g, float u) const {
         const float sig = __fdividef(1.0f, 1.0f + __expf(-g));
         if (kSitu) return beta * tanh_fast(g * by_beta) * sig * (linear * tanh_fast(u * by_linear));
@@ -80,17 +78,68 @@ struct ExpertActivation {
     }
 };
 
-// ------------------------------------------------------------------------------------------- codes
-// scale and codes of a block whose largest magnitude has these bits (without the sign)
-K3_DEVINL float scale_of(uint32_t largest_bits) {
-    if (largest_bits >= 0x7f800000u) return __uint_as_float(0x7fffffffu);
-    return fmaxf(__fdiv_rn(__uint_as_float(largest_bits), 448.0f), 0x1p-126f);
+// The same for two elements at a time, with the sign turned around.
+K3_DEVINL uint64_t both2(float x) { return pack2(x, x); }
+K3_DEVINL float exponential_of_2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
 }
+K3_DEVINL float reciprocal(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+constexpr float kLog2E = 1.44269504f;
+// 1 / (c + c e^(x s)), with s times log2 e
+K3_DEVINL uint64_t logistic2(uint64_t x, float s, float c) {
+    const uint64_t t = mul2(x, both2(s));
+    const uint64_t d = fma2(pack2(exponential_of_2(lo2(t)), exponential_of_2(hi2(t))), both2(c), both2(c));
+    return pack2(reciprocal(lo2(d)), reciprocal(hi2(d)));
+}
+K3_DEVINL uint64_t tanh2(uint64_t x) {
+    const uint64_t y = mul2(x, x);
+    uint64_t p = fma2(y, both2(-1382.0f / 155925.0f), both2(62.0f / 2835.0f));
+    p = fma2(y, p, both2(-17.0f / 315.0f));
+    p = fma2(y, p, both2(2.0f / 15.0f));
+    p = fma2(y, p, both2(-1.0f / 3.0f));
+    const uint64_t small = fma2(mul2(x, y), p, x), large = fma2(both2(-2.0f), logistic2(x, 2.0f * kLog2E, 1.0f), both2(1.0f));
+    return pack2(fabsf(lo2(x)) < 0.4f ? lo2(small) : lo2(large), fabsf(hi2(x)) < 0.4f ? hi2(small) : hi2(large));
+}
+template <bool kSitu>
+K3_DEVINL uint64_t negative_activation2(const ExpertActivation<kSitu> &a, uint64_t g, uint64_t u) {
+    const uint64_t sig = logistic2(g, -kLog2E, -1.0f);
+    if (kSitu) return mul2(mul2(mul2(tanh2(mul2(g, both2(a.by_beta))), both2(a.beta * a.linear)), sig), tanh2(mul2(u, both2(a.by_linear))));
+    return mul2(mul2(g, sig), u);
+}
+
+// ------------------------------------------------------------------------------------------- codes
 // x / scale as an f32 division gives it: the product with the rounded reciprocal, corrected once by its
-// remainder (Markstein 1990)
+// remainder (Markstein 1990).  The remainder is taken from the product, and its negative added: the other way
+// round -0 would become 0.
 K3_DEVINL float quotient(float x, float scale, float inverse) {
     const float r = x * inverse;
-    return copysignf(fmaf(fmaf(-r, scale, x), inverse, r), x);       // the correction would turn -0 into 0
+    return fmaf(fmaf(r, scale, -x), -inverse, r);
+}
+// of two elements, given as -x; s, n: the scale and -1 / scale, twice each
+K3_DEVINL uint64_t quotient2(uint64_t negative_x, uint64_t s, uint64_t n) {
+    const uint64_t r = mul2(negative_x, n);
+    return fma2(fma2(r, s, negative_x), n, r);
+}
+// scale of a block whose largest magnitude has these bits (without the sign): that over 448
+K3_DEVINL float scale_of(uint32_t largest_bits) {
+    if (largest_bits >= 0x7f800000u) return __uint_as_float(0x7fffffffu);
+    return fmaxf(quotient(__uint_as_float(largest_bits), 448.0f, 1.0f / 448.0f), 0x1p-126f);
+}
+// 1 / scale, rounded once: Newton's iteration from an estimate within two units of the last place, which ends beside
+// the rounded value only where the mantissa is all ones (Markstein 1990).  No subroutine, as f32 division and the
+// rounded reciprocal have for their rare cases: where the kernel of the wide products called one, its main loop moved
+// the running sums between registers.
+K3_DEVINL float inverse_of(float scale) {
+    float y = reciprocal(scale);
+    y = fmaf(y, fmaf(-scale, y, 1.0f), y);
+    y = fmaf(y, fmaf(-scale, y, 1.0f), y);
+    return (__float_as_uint(scale) & 0x7fffffu) == 0x7fffffu ? __uint_as_float(__float_as_uint(y) | 1u) : y;
 }
 // two codes, `lo` in the low byte
 K3_DEVINL uint32_t codes2(float lo, float hi) {

@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(RowsArgs a) {
         for (int o = 8; o > 0; o >>= 1) m = Eight<kF32>::larger(m, __shfl_xor_sync(0xffffffffu, m, o));
         if (l % 4u == (uint32_t)b) most = m;
     }
-    const float my_scale = scale_of(Eight<kF32>::bits(most)), my_inverse = __frcp_rn(my_scale);
+    const float my_scale = scale_of(Eight<kF32>::bits(most)), my_inverse = inverse_of(my_scale);
     float scale[4];
     uint2 out[4];
 #pragma unroll
@@ -213,7 +213,7 @@ quantize_columns_kernel(uint8_t *codes, float *scales, const void *x, uint32_t r
 #pragma unroll
         for (int w = 0; w < 8; w++) all = max(all, largest[w][threadIdx.x]);
         const float scale = scale_of(all);
-        column_scale[threadIdx.x] = make_float2(scale, __frcp_rn(scale));
+        column_scale[threadIdx.x] = make_float2(scale, inverse_of(scale));
         if (c0 + threadIdx.x < columns) {
             float *to = scales + (uint64_t)(c0 + threadIdx.x) * scale_pitch + blockIdx.y;
             *to = scale;
@@ -266,7 +266,7 @@ quantize_blocks_kernel(uint8_t *codes, float *scales, const void *x, uint32_t ro
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < 8; w++) m = max(m, largest[w]);
-    const float scale = scale_of(m), inverse = __frcp_rn(scale);
+    const float scale = scale_of(m), inverse = inverse_of(scale);
     if (threadIdx.x == 0u) scales[(uint64_t)blockIdx.y * gridDim.x + blockIdx.x] = scale;
     const uint32_t pitch = pitch_of(columns);
 #pragma unroll

@@ -58,8 +58,8 @@ struct Layout {
     static constexpr uint32_t kStages = kColumnScales ? 3u : 4u;     // the columns' scales take the fourth stage's place
     static constexpr uint32_t kStore = kStages * kStageBytes;
     static constexpr uint32_t kScales = kStore + kSumWarps * kStoreBytes;
-    static constexpr uint32_t kLargest = kScales + kScaleSlots * kSlotFloats * 4u;   // f32 bits [2][128]: halves' largest activations
-    static constexpr uint32_t kPrefix = kLargest + 2u * BM * 4u;
+    static constexpr uint32_t kLargest = kScales + kScaleSlots * kSlotFloats * 4u;   // f32 bits [2][2][128]: halves' largest activations
+    static constexpr uint32_t kPrefix = kLargest + 4u * BM * 4u;
     static constexpr uint32_t kBars = (kPrefix + (kMaxGroups + 1u) * 4u + 15u) / 16u * 16u;
     static constexpr uint32_t kBytes = kBars + 256u + 1024u;         // the last: alignment
     static_assert(kBytes <= 232448u, "shared memory of a block");
@@ -80,28 +80,31 @@ struct WideArgs {
     bool b_ready;                                                    // Product::b_ready
     int accumulate;
     int activation;
-    float beta, linear_beta;
+    float beta, by_beta, linear_beta, by_linear_beta;                // by_: the reciprocals
 };
 
 struct Item {
     uint32_t group, row, rows, column, kb_begin, kb_end;
 };
 
-// The first 32 pairs of sums (gate) and the other 32 (up) to 64 activations in the first 32, zero past `left`; the largest
-// magnitude's bits.
+// the largest of a and the magnitudes of b and c; NaN if one of them is
+K3_DEVINL float largest_of(float a, float b, float c) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// The first 32 pairs of sums (gate) and the other 32 (up) to the negatives of 64 activations in the first 32, zero past
+// `left`; the largest magnitude's bits, or a NaN's.
 template <bool kSitu>
-K3_DEVINL uint32_t activate(uint64_t (&sum)[64], uint32_t left, float beta, float linear_beta) {
-    const ExpertActivation<kSitu> act(beta, linear_beta);
-    uint32_t most = 0u;
+K3_DEVINL uint32_t activate(uint64_t (&sum)[64], uint32_t left, const ExpertActivation<kSitu> &act) {
+    float most = 0.f;
 #pragma unroll
     for (uint32_t j = 0; j < 32u; j++) {
-        float x = act(lo2(sum[j]), lo2(sum[32u + j])), y = act(hi2(sum[j]), hi2(sum[32u + j]));
-        if (2u * j >= left) x = 0.f;
-        if (2u * j + 1u >= left) y = 0.f;
-        most = max(most, max(__float_as_uint(x) & 0x7fffffffu, __float_as_uint(y) & 0x7fffffffu));
-        sum[j] = pack2(x, y);
+        sum[j] = negative_activation2(act, sum[j], sum[32u + j]);
+        if (left < kBlock / 2u) sum[j] = pack2(2u * j < left ? lo2(sum[j]) : 0.f, 2u * j + 1u < left ? hi2(sum[j]) : 0.f);
+        most = largest_of(most, lo2(sum[j]), hi2(sum[j]));
     }
-    return most;
+    return __float_as_uint(most);
 }
 
 // four neighbouring results at `out`, of which `left` columns exist
@@ -380,11 +383,12 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         uint32_t at = 0u, aph = 0u, slot = 0u, sph = 0u, lph = 0u;
         bool ok = true;
         for (uint32_t w = first_item; ok && w < total; w += step) {
-            const Item it = item_of(w);
+            const uint32_t kb_begin = kSplit ? blockIdx.x * a.split_blocks : 0u;
+            const uint32_t kb_end = kSplit ? min(blocks, kb_begin + a.split_blocks) : blocks;
             uint64_t sum[64];
 #pragma unroll
             for (int i = 0; i < 64; i++) sum[i] = 0ull;
-            for (uint32_t kb = it.kb_begin; kb < it.kb_end; kb++) {
+            for (uint32_t kb = kb_begin; kb < kb_end; kb++) {
                 if (kb % kSlotBlocks == 0u && !mbar_wait(&scale_full[slot], sph, abort_flag)) { ok = false; break; }
                 const float *scales = reinterpret_cast<const float *>(base + L::kScales) + slot * L::kSlotFloats +
                                       kb % kSlotBlocks * L::kBlockScales;
@@ -431,13 +435,14 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                     }
                 }
                 if (++at == 2u) { at = 0u; aph ^= 1u; }
-                if (kb % kSlotBlocks == kSlotBlocks - 1u || kb + 1u == it.kb_end) {
+                if (kb % kSlotBlocks == kSlotBlocks - 1u || kb + 1u == kb_end) {
                     __syncwarp();
                     if (lane == 0u) mbar_arrive(&scale_empty[slot]);
                     if (++slot == kScaleSlots) { slot = 0u; sph ^= 1u; }
                 }
             }
             if (!ok) break;
+            const Item it = item_of(w);                              // looked up here: the loop above has no registers to spare
             if (kSplit) {
                 // [128][64] units of 16 bytes in the ring's place (every stage has been read), swizzled by the row
                 float4 *part = reinterpret_cast<float4 *>(base) + row_in * (BN / 4u);
@@ -449,20 +454,19 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             } else if (kEpilogue == kOutActivated) {
                 // ------------------------------------------ activation, largest of the row's 128, codes
                 const uint32_t left = it.column + first < a.n ? a.n - it.column - first : 0u;       // columns of the 64 that exist
-                const uint32_t most_here = a.activation == kActSitu ? activate<true>(sum, left, a.beta, a.linear_beta)
-                                                                    : activate<false>(sum, left, a.beta, a.linear_beta);
-                uint32_t *largest = reinterpret_cast<uint32_t *>(base + L::kLargest);
+                const uint32_t most_here = a.activation == kActSitu
+                    ? activate<true>(sum, left, {a.beta, a.by_beta, a.linear_beta, a.by_linear_beta})
+                    : activate<false>(sum, left, {});
+                // one of two buffers in turn: a warp is here again only when all have read what it wrote two items ago
+                uint32_t *largest = reinterpret_cast<uint32_t *>(base + L::kLargest) + lph * 2u * BM;
                 largest[half * BM + row_in] = most_here;
                 __syncwarp();
                 if (lane == 0u) mbar_arrive(largest_full);
                 if (!mbar_wait(largest_full, lph, abort_flag)) { ok = false; break; }
                 lph ^= 1u;
                 const uint32_t most = max(most_here, largest[(half ^ 1u) * BM + row_in]);
-                __syncwarp();
-                if (lane == 0u) mbar_arrive(largest_full);            // read: the next item may overwrite it
-                if (!mbar_wait(largest_full, lph, abort_flag)) { ok = false; break; }
-                lph ^= 1u;
-                const float scale = scale_of(most), inverse = __frcp_rn(scale);
+                const float scale = scale_of(most);
+                const uint64_t scales2 = both2(scale), inverses2 = both2(-inverse_of(scale));
                 if (row_in < it.rows) {
                     const uint64_t row = it.row + row_in;
                     const uint32_t out_pitch = pitch_of(a.n), scale_pitch = scale_pitch_of(a.n);
@@ -473,9 +477,9 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                         uint32_t word[4];
 #pragma unroll
                         for (uint32_t j = 0; j < 4u; j++) {
-                            const uint64_t x = sum[c * 8u + 2u * j], y = sum[c * 8u + 2u * j + 1u];
-                            word[j] = codes2(quotient(lo2(x), scale, inverse), quotient(hi2(x), scale, inverse)) |
-                                      (codes2(quotient(lo2(y), scale, inverse), quotient(hi2(y), scale, inverse)) << 16);
+                            const uint64_t x = quotient2(sum[c * 8u + 2u * j], scales2, inverses2);
+                            const uint64_t y = quotient2(sum[c * 8u + 2u * j + 1u], scales2, inverses2);
+                            word[j] = codes2(lo2(x), hi2(x)) | (codes2(lo2(y), hi2(y)) << 16);
                         }
                         if (it.column + first + c * 16u < out_pitch) {
                             *reinterpret_cast<uint4 *>(to + c * 16u) = make_uint4(word[0], word[1], word[2], word[3]);
@@ -603,6 +607,8 @@ WideArgs args_of(const Product &p, uint32_t columns) {
     a.activation = p.activation;
     a.beta = p.beta;
     a.linear_beta = p.linear_beta;
+    a.by_beta = 1.0f / p.beta;
+    a.by_linear_beta = 1.0f / p.linear_beta;
     return a;
 }
 
