@@ -9,16 +9,19 @@
 // elements and block is all the arithmetic there is.
 //
 // One work item = 128 rows x 256 columns over the whole depth (kOutActivated: 128 columns of gate and
-// the same 128 of up).  384 threads, one block per SM, items in a static order:
+// the same 128 of up).  One block per SM, items in a static order:
 //   warp 0        loads by TMA: a stage is 128 columns of 128 rows of a and 256 rows of b, 48 KB
 //   warp 1        MMA issuer, owns the tensor memory
 //   warp 2        scales, four blocks ahead: a row's times the block's, where the adding warps read them
-//   warps 4-11    running sums: lane quadrant warp % 4, columns in two halves
+//   warps 4-11    running sums: lane quadrant warp % 4, columns in two halves (kOutActivated: warps 4-19, quarters)
 // kSplit (one matrix, fewer items than SMs, or the items that are left over when every SM has had as many as
 // the others): an item is a cluster of up to 8 blocks with a part of the depth each, which add their sums
 // through distributed shared memory in ascending order of the depth.
-// The two warpgroups of running sums (128 of them per thread) take registers over from the first one:
-// 2 x 128 x 232 + 128 x 40 are the 384 x 168 of the launch.
+// The warpgroups of running sums take registers over from the first one: with 128 sums per thread
+// 2 x 128 x 232 + 128 x 40 are the 384 x 168 of the launch, with 64 (kOutActivated) 4 x 128 x 112 + 128 x 32 the
+// 640 x 96.  Four warps per scheduler instead of two hide more of the activations' chains, but the stores of the
+// other epilogues take longer: gate/up of 4096 tokens (16 of 64 experts, 7168 x 2048) 2.09 ms back to back against
+// 2.40, 8192 x 7168 x 7168 386 us against 364.
 //
 // Every wait is bounded; on give-up the block raises the status word, waits for its copies and frees its
 // tensor memory.
@@ -40,12 +43,16 @@ using namespace k3::fp8;
 
 namespace {
 
-constexpr uint32_t kThreads = 384;
 constexpr uint32_t BM = 128, BN = 256;
 constexpr uint32_t kATile = BM * kBlock, kBTile = BN * kBlock;       // 16 KB, 32 KB
 constexpr uint32_t kStageBytes = kATile + kBTile;
-constexpr uint32_t kSumWarps = 8;
-constexpr uint32_t kStoreBytes = 32u * 64u;                          // per warp: 32 rows of 64 bytes on their way out
+// Column parts of an item, and threads: a warp of running sums has a quarter of the rows and one part of the columns.
+// Four parts where the epilogue is the activation, two elsewhere.
+template <int kEpilogue>
+constexpr uint32_t kParts = kEpilogue == kOutActivated ? 4u : 2u;
+template <int kEpilogue>
+constexpr uint32_t kThreads = 128u + 128u * kParts<kEpilogue>;
+constexpr uint32_t kStoreBytes = 8u * 32u * 64u;                     // 8 warps: 32 rows of 64 bytes on their way out
 constexpr uint32_t kMaxGroups = 1024;
 constexpr uint32_t kMaxSplits = 8;                                   // of the depth: the portable cluster
 constexpr uint32_t kScaleSlots = 2, kSlotBlocks = 4;                 // scales travel four blocks at a time
@@ -57,9 +64,9 @@ struct Layout {
     static constexpr uint32_t kSlotFloats = kSlotBlocks * kBlockScales;
     static constexpr uint32_t kStages = kColumnScales ? 3u : 4u;     // the columns' scales take the fourth stage's place
     static constexpr uint32_t kStore = kStages * kStageBytes;
-    static constexpr uint32_t kScales = kStore + kSumWarps * kStoreBytes;
-    static constexpr uint32_t kLargest = kScales + kScaleSlots * kSlotFloats * 4u;   // f32 bits [2][2][128]: halves' largest activations
-    static constexpr uint32_t kPrefix = kLargest + 4u * BM * 4u;
+    static constexpr uint32_t kScales = kStore + kStoreBytes;
+    static constexpr uint32_t kLargest = kScales + kScaleSlots * kSlotFloats * 4u;   // f32 bits [2][4][128]: the parts' largest activations
+    static constexpr uint32_t kPrefix = kLargest + 8u * BM * 4u;
     static constexpr uint32_t kBars = (kPrefix + (kMaxGroups + 1u) * 4u + 15u) / 16u * 16u;
     static constexpr uint32_t kBytes = kBars + 256u + 1024u;         // the last: alignment
     static_assert(kBytes <= 232448u, "shared memory of a block");
@@ -93,15 +100,15 @@ K3_DEVINL float largest_of(float a, float b, float c) {
     asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// The first 32 pairs of sums (gate) and the other 32 (up) to the negatives of 64 activations in the first 32, zero past
-// `left`; the largest magnitude's bits, or a NaN's.
-template <bool kSitu>
-K3_DEVINL uint32_t activate(uint64_t (&sum)[64], uint32_t left, const ExpertActivation<kSitu> &act) {
+// The first half of the pairs of sums (gate) and the other half (up) to the negatives of the activations in the first,
+// zero past `left`; the largest magnitude's bits, or a NaN's.
+template <bool kSitu, uint32_t kPairs>
+K3_DEVINL uint32_t activate(uint64_t (&sum)[kPairs], uint32_t left, const ExpertActivation<kSitu> &act) {
     float most = 0.f;
 #pragma unroll
-    for (uint32_t j = 0; j < 32u; j++) {
-        sum[j] = negative_activation2(act, sum[j], sum[32u + j]);
-        if (left < kBlock / 2u) sum[j] = pack2(2u * j < left ? lo2(sum[j]) : 0.f, 2u * j + 1u < left ? hi2(sum[j]) : 0.f);
+    for (uint32_t j = 0; j < kPairs / 2u; j++) {
+        sum[j] = negative_activation2(act, sum[j], sum[kPairs / 2u + j]);
+        if (left < kPairs) sum[j] = pack2(2u * j < left ? lo2(sum[j]) : 0.f, 2u * j + 1u < left ? hi2(sum[j]) : 0.f);
         most = largest_of(most, lo2(sum[j]), hi2(sum[j]));
     }
     return __float_as_uint(most);
@@ -133,10 +140,11 @@ K3_DEVINL void store4(uint16_t *out, const float (&sum)[4], uint32_t left, bool 
 }
 
 template <int kEpilogue, bool kColumnScales, bool kSplit>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads<kEpilogue>, 1)
 fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                 const __grid_constant__ CUtensorMap map_b2, WideArgs a) {
     using L = Layout<kColumnScales>;
+    constexpr uint32_t kSumWarps = 4u * kParts<kEpilogue>, kPairs = BN / kParts<kEpilogue> / 2u;
     extern __shared__ unsigned char smem_raw[];
     unsigned char *base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint64_t *full = reinterpret_cast<uint64_t *>(base + L::kBars);  // [kStages]
@@ -251,7 +259,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     const uint32_t first_item = kSplit ? 0u : blockIdx.x, step = kSplit ? 1u : gridDim.x;
 
     if (warp < 4u) {
-        fewer_registers<40>();
+        fewer_registers<kPairs == 64u ? 40u : 32u>();
         if (warp == 0u) {
             // ------------------------------------------------------------------------- loads
             if (elect_one()) {
@@ -372,12 +380,12 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         }
     } else {
         // ---------------------------------------------------------------------- running sums
-        more_registers<232>();
+        more_registers<kPairs == 64u ? 232u : 112u>();
         if (a.b_ready) pdl_wait();                                   // before the first store
-        const uint32_t q = warp % 4u, half = (warp - 4u) / 4u;
-        // a thread's 128 sums are columns first, first + 1, .. of the tile, and 64 more from second
-        const uint32_t first = kEpilogue == kOutActivated ? half * 64u : half * 128u;
-        const uint32_t second = kEpilogue == kOutActivated ? first + kBlock : first + 64u;
+        const uint32_t q = warp % 4u, part = (warp - 4u) / 4u;
+        // half of a thread's sums are columns first, first + 1, .. of the tile, the other half those from second
+        const uint32_t first = part * (kEpilogue == kOutActivated ? kPairs : 2u * kPairs);
+        const uint32_t second = first + (kEpilogue == kOutActivated ? kBlock : kPairs);
         const uint32_t lanes = tmem + ((32u * q) << 16);
         const uint32_t row_in = 32u * q + lane;
         uint32_t at = 0u, aph = 0u, slot = 0u, sph = 0u, lph = 0u;
@@ -385,9 +393,9 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         for (uint32_t w = first_item; ok && w < total; w += step) {
             const uint32_t kb_begin = kSplit ? blockIdx.x * a.split_blocks : 0u;
             const uint32_t kb_end = kSplit ? min(blocks, kb_begin + a.split_blocks) : blocks;
-            uint64_t sum[64];
+            uint64_t sum[kPairs];
 #pragma unroll
-            for (int i = 0; i < 64; i++) sum[i] = 0ull;
+            for (uint32_t i = 0; i < kPairs; i++) sum[i] = 0ull;
             for (uint32_t kb = kb_begin; kb < kb_end; kb++) {
                 if (kb % kSlotBlocks == 0u && !mbar_wait(&scale_full[slot], sph, abort_flag)) { ok = false; break; }
                 const float *scales = reinterpret_cast<const float *>(base + L::kScales) + slot * L::kSlotFloats +
@@ -399,27 +407,31 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                     s0 = scales[row_in];
                     s1 = scales[BM + row_in];
                 } else {
-                    s0 = s1 = scales[half * BM + row_in];
+                    s0 = s1 = scales[first / kBlock * BM + row_in];
                 }
                 if (!mbar_wait(&sum_full[at], aph, abort_flag)) { ok = false; break; }
                 tc_fence_after();
-                // the next 32 columns are on their way while these are added
-                uint32_t r[2][32];
-                tmem_ld_32x32(lanes + at * BN + first, r[0]);
+                // with registers for it the next 32 columns are on their way while these are added
+                constexpr uint32_t kChunks = kPairs / 16u, kAhead = kPairs == 64u ? 1u : 0u;
+                auto column_of = [&](uint32_t c) { return (c < kChunks / 2u ? first : second) + c % (kChunks / 2u) * 32u; };
+                uint32_t r[kAhead + 1u][32];
+                if (kAhead) tmem_ld_32x32(lanes + at * BN + first, r[0]);
 #pragma unroll
-                for (uint32_t c = 0; c < 4u; c++) {
-                    tmem_ld_wait_for(r[c & 1u]);
-                    if (c < 3u) {
-                        tmem_ld_32x32(lanes + at * BN + (c < 1u ? first : second) + (c == 1u ? 0u : 32u), r[(c + 1u) & 1u]);
+                for (uint32_t c = 0; c < kChunks; c++) {
+                    const uint32_t column = column_of(c);
+                    uint32_t (&v)[32] = r[c & kAhead];
+                    if (!kAhead) tmem_ld_32x32(lanes + at * BN + column, v);
+                    tmem_ld_wait_for(v);
+                    if (c < kChunks - 1u) {
+                        if (kAhead) tmem_ld_32x32(lanes + at * BN + column_of(c + 1u), r[(c + 1u) & kAhead]);
                     } else {
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0u) mbar_arrive(&sum_empty[at]);
                     }
-                    const uint64_t s2 = c < 2u ? pack2(s0, s0) : pack2(s1, s1);
-                    const uint32_t (&v)[32] = r[c & 1u];
+                    const uint64_t s2 = both2(c < kChunks / 2u ? s0 : s1);
                     if (kColumnScales) {
-                        const ulonglong2 *by = reinterpret_cast<const ulonglong2 *>(scales + BM + (c < 2u ? first : second) + (c & 1u) * 32u);
+                        const ulonglong2 *by = reinterpret_cast<const ulonglong2 *>(scales + BM + column);
 #pragma unroll
                         for (uint32_t j = 0; j < 8u; j++) {
                             const ulonglong2 b = by[j];
@@ -447,33 +459,35 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 // [128][64] units of 16 bytes in the ring's place (every stage has been read), swizzled by the row
                 float4 *part = reinterpret_cast<float4 *>(base) + row_in * (BN / 4u);
 #pragma unroll
-                for (uint32_t j = 0; j < 32u; j++) {
-                    const uint32_t unit = (j < 16u ? first : second) / 4u + j % 16u;
+                for (uint32_t j = 0; j < kPairs / 2u; j++) {
+                    const uint32_t unit = (j < kPairs / 4u ? first : second) / 4u + j % (kPairs / 4u);
                     part[unit ^ (row_in & 7u)] = make_float4(lo2(sum[2u * j]), hi2(sum[2u * j]), lo2(sum[2u * j + 1u]), hi2(sum[2u * j + 1u]));
                 }
             } else if (kEpilogue == kOutActivated) {
                 // ------------------------------------------ activation, largest of the row's 128, codes
-                const uint32_t left = it.column + first < a.n ? a.n - it.column - first : 0u;       // columns of the 64 that exist
+                const uint32_t left = it.column + first < a.n ? a.n - it.column - first : 0u;       // of the thread's columns, those that exist
                 const uint32_t most_here = a.activation == kActSitu
                     ? activate<true>(sum, left, {a.beta, a.by_beta, a.linear_beta, a.by_linear_beta})
                     : activate<false>(sum, left, {});
                 // one of two buffers in turn: a warp is here again only when all have read what it wrote two items ago
-                uint32_t *largest = reinterpret_cast<uint32_t *>(base + L::kLargest) + lph * 2u * BM;
-                largest[half * BM + row_in] = most_here;
+                uint32_t *largest = reinterpret_cast<uint32_t *>(base + L::kLargest) + lph * 4u * BM;
+                largest[part * BM + row_in] = most_here;
                 __syncwarp();
                 if (lane == 0u) mbar_arrive(largest_full);
                 if (!mbar_wait(largest_full, lph, abort_flag)) { ok = false; break; }
                 lph ^= 1u;
-                const uint32_t most = max(most_here, largest[(half ^ 1u) * BM + row_in]);
+                uint32_t most = most_here;
+#pragma unroll
+                for (uint32_t i = 1; i < kParts<kEpilogue>; i++) most = max(most, largest[(part ^ i) * BM + row_in]);
                 const float scale = scale_of(most);
                 const uint64_t scales2 = both2(scale), inverses2 = both2(-inverse_of(scale));
                 if (row_in < it.rows) {
                     const uint64_t row = it.row + row_in;
                     const uint32_t out_pitch = pitch_of(a.n), scale_pitch = scale_pitch_of(a.n);
-                    if (half == 0u) a.out_scales[row * scale_pitch + it.column / kBlock] = scale;
+                    if (part == 0u) a.out_scales[row * scale_pitch + it.column / kBlock] = scale;
                     uint8_t *to = (uint8_t *)a.out + row * out_pitch + it.column + first;
 #pragma unroll
-                    for (uint32_t c = 0; c < 4u; c++) {
+                    for (uint32_t c = 0; c < kPairs / 16u; c++) {
                         uint32_t word[4];
 #pragma unroll
                         for (uint32_t j = 0; j < 4u; j++) {
@@ -490,7 +504,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 // ---------------------- rows of 64 bytes through shared memory: a warp then stores 8 rows at once
                 constexpr uint32_t kBytesEach = kEpilogue == kOutF32 ? 4u : 2u;
                 constexpr uint32_t kPer = 64u / kBytesEach;            // elements per pass
-                unsigned char *mine = base + L::kStore + (warp - 4u) * kStoreBytes;
+                unsigned char *mine = base + L::kStore + (warp - 4u) * (kStoreBytes / kSumWarps);
                 const bool vector = (a.n * kBytesEach) % 16u == 0u && ((uintptr_t)a.out & 15u) == 0u;
 #pragma unroll
                 for (uint32_t pass = 0; pass < 128u / kPer; pass++) {
@@ -630,7 +644,7 @@ bool launch_grouped(const Product &p, cudaStream_t stream) {
     auto kernel = fp8_wide_kernel<kEpilogue, false, false>;
     constexpr uint32_t kBytes = Layout<false>::kBytes;
     return items <= 0x7fffffffull && set_max_dynamic_smem((const void *)kernel, kBytes) &&
-           launch_chained(kernel, (uint32_t)std::min<uint64_t>(items, sm_count()), kThreads, kBytes, stream, m.a, m.b, m.b2, a);
+           launch_chained(kernel, (uint32_t)std::min<uint64_t>(items, sm_count()), kThreads<kEpilogue>, kBytes, stream, m.a, m.b, m.b2, a);
 }
 
 // One matrix.  Every SM takes the same number of whole items; what is left, or all where there are fewer items than SMs,
@@ -651,17 +665,17 @@ bool launch_whole(const Product &p, cudaStream_t stream) {
     const uint32_t left = (uint32_t)(items % sms);
     uint32_t parts = 1u;
     if (left != 0u && left * 2u <= sms) {          // two rounds of clusters take longer than they should: 384 rows of 7168 x 7168 34.3 us, whole 28.2
-        parts = best_parts(left, blocks, kSlotBlocks, kFixed, active_clusters((const void *)split, kThreads, kBytes));
+        parts = best_parts(left, blocks, kSlotBlocks, kFixed, active_clusters((const void *)split, kThreads<kEpilogue>, kBytes));
     }
     a.split_blocks = ((blocks + parts - 1u) / parts + kSlotBlocks - 1u) / kSlotBlocks * kSlotBlocks;
     const bool cut = parts > 1u && a.split_blocks + kFixed < blocks;
     a.items = (uint32_t)items - (cut ? left : 0u);
     if (a.items != 0u) {
-        if (!launch_chained(whole, std::min(a.items, sms), kThreads, kBytes, stream, m.a, m.b, m.b2, a)) return false;
+        if (!launch_chained(whole, std::min(a.items, sms), kThreads<kEpilogue>, kBytes, stream, m.a, m.b, m.b2, a)) return false;
         a.b_ready = true;                          // the launch in front is then the one above
     }
     a.first_item = a.items;
-    return !cut || launch_chained_cluster(split, dim3(parts, left), kThreads, dim3(parts, 1, 1), kBytes, stream, m.a, m.b, m.b2, a);
+    return !cut || launch_chained_cluster(split, dim3(parts, left), kThreads<kEpilogue>, dim3(parts, 1, 1), kBytes, stream, m.a, m.b, m.b2, a);
 }
 
 }  // namespace
