@@ -54,7 +54,7 @@ K3_DEVINL void mbar_drain(uint64_t *bar, uint32_t parity) {
 }
 
 // The expert activation with the fast exponential and reciprocal, 4e-7 of the result: it is quantised to 4 bits next.
-// The kind is a template argument, so that many elements go side by side: with a branch in each of a thread's 64
+// The kind is a template argument, so that many elements go side by side: with a branch in each of a thread's elements
 // the warps waited for one element's chain after the other.
 //
 // tanh x: its Taylor series up to x^11 below 0.4, where the next term is 6e-8 of the value, and 1 - 2 / (1 + e^2x)
@@ -114,32 +114,40 @@ K3_DEVINL uint64_t negative_activation2(const ExpertActivation<kSitu> &a, uint64
 }
 
 // ------------------------------------------------------------------------------------------- codes
-// x / scale as an f32 division gives it: the product with the rounded reciprocal, corrected once by its
+// x / by as an f32 division gives it: the product with the rounded reciprocal, corrected once by its
 // remainder (Markstein 1990).  The remainder is taken from the product, and its negative added: the other way
 // round -0 would become 0.
-K3_DEVINL float quotient(float x, float scale, float inverse) {
+K3_DEVINL float divided(float x, float by, float inverse) {
     const float r = x * inverse;
-    return fmaf(fmaf(r, scale, -x), -inverse, r);
-}
-// of two elements, given as -x; s, n: the scale and -1 / scale, twice each
-K3_DEVINL uint64_t quotient2(uint64_t negative_x, uint64_t s, uint64_t n) {
-    const uint64_t r = mul2(negative_x, n);
-    return fma2(fma2(r, s, negative_x), n, r);
+    return fmaf(fmaf(r, by, -x), -inverse, r);
 }
 // scale of a block whose largest magnitude has these bits (without the sign): that over 448
 K3_DEVINL float scale_of(uint32_t largest_bits) {
     if (largest_bits >= 0x7f800000u) return __uint_as_float(0x7fffffffu);
-    return fmaxf(quotient(__uint_as_float(largest_bits), 448.0f, 1.0f / 448.0f), 0x1p-126f);
+    return fmaxf(divided(__uint_as_float(largest_bits), 448.0f, 1.0f / 448.0f), 0x1p-126f);
 }
-// 1 / scale, rounded once: Newton's iteration from an estimate within two units of the last place, which ends beside
-// the rounded value only where the mantissa is all ones (Markstein 1990).  No subroutine, as f32 division and the
-// rounded reciprocal have for their rare cases: where the kernel of the wide products called one, its main loop moved
-// the running sums between registers.
+// Below 2^-90 the remainders are subnormal and lose bits, so there x and the scale are both multiplied by 2^64.
+K3_DEVINL float lift_of(float scale) { return scale < 0x1p-90f ? 0x1p64f : 1.0f; }
+// 1 / (scale lift), rounded once: Newton's iteration from an estimate within two units of the last place, which ends
+// beside the rounded value only where the mantissa is all ones (Markstein 1990).  No subroutine, as f32 division and
+// the rounded reciprocal have for their rare cases: where the kernel of the wide products called one, its main loop
+// moved the running sums between registers.
 K3_DEVINL float inverse_of(float scale) {
-    float y = reciprocal(scale);
-    y = fmaf(y, fmaf(-scale, y, 1.0f), y);
-    y = fmaf(y, fmaf(-scale, y, 1.0f), y);
-    return (__float_as_uint(scale) & 0x7fffffu) == 0x7fffffu ? __uint_as_float(__float_as_uint(y) | 1u) : y;
+    const float by = scale * lift_of(scale);
+    float y = reciprocal(by);
+    y = fmaf(y, fmaf(-by, y, 1.0f), y);
+    y = fmaf(y, fmaf(-by, y, 1.0f), y);
+    return (__float_as_uint(by) & 0x7fffffu) == 0x7fffffu ? __uint_as_float(__float_as_uint(y) | 1u) : y;
+}
+// x / scale; inverse: inverse_of(scale)
+K3_DEVINL float quotient(float x, float scale, float inverse) {
+    const float lift = lift_of(scale);
+    return divided(x * lift, scale * lift, inverse);
+}
+// divided() for two elements, given as -x; the divisor and the negative of its reciprocal, twice each
+K3_DEVINL uint64_t divided2(uint64_t negative_x, uint64_t by, uint64_t negative_inverse) {
+    const uint64_t r = mul2(negative_x, negative_inverse);
+    return fma2(fma2(r, by, negative_x), negative_inverse, r);
 }
 // two codes, `lo` in the low byte
 K3_DEVINL uint32_t codes2(float lo, float hi) {

@@ -70,11 +70,19 @@ struct Eight {
     }
     // of a word of larger(): the f32 bits
     static K3_DEVINL uint32_t bits(uint32_t m) { return kF32 ? m : max(m & 0xffff0000u, m << 16); }
-    K3_DEVINL uint2 codes(float scale, float inverse) const {
+    // quotient() with the rare lift in a branch: 8192 x 7168 in 30.0 us, 29.1 without any lift, 31.1 with a product each
+    K3_DEVINL uint2 codes(float scale, float inverse) {
+        const float lift = lift_of(scale), by = scale * lift;
+        if (lift != 1.0f) {
+#pragma unroll
+            for (uint32_t i = 0; i < kWords; i++) {                  // exact in bf16 as well
+                w[i] = kF32 ? __float_as_uint(value(i) * lift) : bf16x2(value(2u * i) * lift, value(2u * i + 1u) * lift);
+            }
+        }
         uint32_t h[4];
 #pragma unroll
         for (uint32_t i = 0; i < 4u; i++) {
-            h[i] = codes2(quotient(value(2u * i), scale, inverse), quotient(value(2u * i + 1u), scale, inverse));
+            h[i] = codes2(divided(value(2u * i), by, inverse), divided(value(2u * i + 1u), by, inverse));
         }
         return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
     }

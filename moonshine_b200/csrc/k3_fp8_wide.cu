@@ -480,7 +480,11 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 #pragma unroll
                 for (uint32_t i = 1; i < kParts<kEpilogue>; i++) most = max(most, largest[(part ^ i) * BM + row_in]);
                 const float scale = scale_of(most);
-                const uint64_t scales2 = both2(scale), inverses2 = both2(-inverse_of(scale));
+                const uint64_t by = both2(scale * lift_of(scale)), inverse = both2(-inverse_of(scale));
+                if (lift_of(scale) != 1.0f) {
+#pragma unroll
+                    for (uint32_t j = 0; j < kPairs / 2u; j++) sum[j] = mul2(sum[j], both2(lift_of(scale)));
+                }
                 if (row_in < it.rows) {
                     const uint64_t row = it.row + row_in;
                     const uint32_t out_pitch = pitch_of(a.n), scale_pitch = scale_pitch_of(a.n);
@@ -491,8 +495,8 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                         uint32_t word[4];
 #pragma unroll
                         for (uint32_t j = 0; j < 4u; j++) {
-                            const uint64_t x = quotient2(sum[c * 8u + 2u * j], scales2, inverses2);
-                            const uint64_t y = quotient2(sum[c * 8u + 2u * j + 1u], scales2, inverses2);
+                            const uint64_t x = divided2(sum[c * 8u + 2u * j], by, inverse);
+                            const uint64_t y = divided2(sum[c * 8u + 2u * j + 1u], by, inverse);
                             word[j] = codes2(lo2(x), hi2(x)) | (codes2(lo2(y), hi2(y)) << 16);
                         }
                         if (it.column + first + c * 16u < out_pitch) {

@@ -83,6 +83,24 @@ def test_quantisers_where_quotients_fall_between_two_codes(form):
     check_quantized(form, x, *getattr(fp8, "quantize_" + form)(x))
 
 
+def test_quotients_by_every_kind_of_scale():
+    """Scales of all exponents with mantissas at both ends (all ones: the reciprocal that Newton's iteration misses) and
+    in between, and quotients at and beside the middle of two codes."""
+    bits = torch.arange(2, 245, dtype=torch.int32).repeat_interleave(16) << 23
+    g = torch.Generator().manual_seed(4)
+    ends = torch.tensor([0x7fffff, 0x7ffffe, 0x7ffffd, 0, 1, 2], dtype=torch.int32)
+    mantissas = torch.cat([ends, torch.randint(0, 1 << 23, (10,), generator=g, dtype=torch.int32)]).repeat(bits.numel() // 16)
+    scales = (bits | mantissas).view(F32)
+    middles = torch.tensor([(8 + m + 0.5) * 2.0 ** (e - 10) for e in range(16) for m in range(8)])[:126]
+    x = scales[:, None] * torch.cat([torch.tensor([448.0]), middles, torch.tensor([0.0])])[None]
+    x[:, 1:127:3] = torch.nextafter(x[:, 1:127:3], torch.tensor(0.0))
+    x[:, 2:127:3] = torch.nextafter(x[:, 2:127:3], torch.tensor(float("inf")))
+    x[:, 1:127:2] *= -1
+    assert ((x[:, 0] / 448).view(torch.int32) & 0x7fffff == 0x7fffff).sum() > 200
+    x = x.cuda()
+    check_quantized("rows", x, *fp8.quantize_rows(x))
+
+
 @pytest.mark.parametrize("form", ["rows", "columns", "blocks"])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_quantisers_take_any_start(form, dtype):
