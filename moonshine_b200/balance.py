@@ -9,14 +9,15 @@ from __future__ import annotations
 import torch
 
 from . import ops
-from .fp8 import _done, _Workspace
+from .fp8 import _done, _placed, _Workspace
 
 _SCORES = {"sigmoid": ops.SCORE_SIGMOID, "softmax": ops.SCORE_SOFTMAX}
 
 
 def _check(t, name, dtype, shape):
-    if t.dtype is not dtype or t.shape != shape or not t.is_cuda:
-        raise ValueError(f"{name}: expected {dtype} {list(shape)} on the GPU, got {t.dtype} {list(t.shape)}")
+    if t.dtype is not dtype or t.shape != shape:
+        raise ValueError(f"{name}: expected {dtype} {list(shape)}, got {t.dtype} {list(t.shape)}")
+    _placed(t, name)
 
 
 class RouterBalance:
@@ -36,8 +37,9 @@ class RouterBalance:
         _check(ids, "ids", torch.int32, (tokens, self.top_k))
         if offsets is None:
             return tokens, 1
-        if offsets.dtype is not torch.int32 or offsets.dim() != 1 or offsets.shape[0] < 2 or not offsets.is_cuda:
-            raise ValueError(f"offsets: expected int32 [sequences + 1] on the GPU, got {offsets.dtype} {list(offsets.shape)}")
+        if offsets.dtype is not torch.int32 or offsets.dim() != 1 or offsets.shape[0] < 2:
+            raise ValueError(f"offsets: expected int32 [sequences + 1], got {offsets.dtype} {list(offsets.shape)}")
+        _placed(offsets, "offsets")
         return tokens, offsets.shape[0] - 1
 
     def forward(self, logits: torch.Tensor | None, ids: torch.Tensor, offsets: torch.Tensor | None = None):

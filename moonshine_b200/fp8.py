@@ -4,7 +4,8 @@
 Codes are ``torch.float8_e4m3fn`` with rows padded to 16 bytes (``pitch``); activations get one
 scale per row and 128 columns, weights one per 128 x 128.  An object keeps its tables and a
 workspace that grows with the largest call, so its calls have to be ordered (one stream, or
-streams that wait for one another), as those of ``MoELayer``.
+streams that wait for one another), as those of ``MoELayer``.  All tensors of a call lie on the
+current CUDA device.
 
     table, scales = fp8.quantize_blocks(weight)             # bf16 or f32 [rows, columns]
     y = fp8.Fp8Linear(table, scales, rows, columns).forward(x)
@@ -42,22 +43,34 @@ def _done(ok: bool, name: str) -> None:
         raise RuntimeError(name + " failed")
 
 
-def _matrix(x: torch.Tensor, name: str, columns: int | None = None, dtypes=(torch.bfloat16,)) -> tuple[int, int]:
+def _placed(t: torch.Tensor, name: str, device: torch.device | None = None) -> None:
+    """Refuses a tensor that the kernels cannot read: they run on the current device, and take addresses."""
+    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name}: expected a tensor on the current CUDA device, got one on {t.device}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name}: on {t.device}, the tables are on {device}")
+
+
+def _matrix(x: torch.Tensor, name: str, columns: int | None = None, dtypes=(torch.bfloat16,),
+            device: torch.device | None = None) -> tuple[int, int]:
     shape = x.shape
     if len(shape) != 2 or x.dtype not in dtypes or (columns is not None and shape[1] != columns):
         raise ValueError(f"{name}: expected [rows, {columns if columns is not None else 'columns'}] of "
                          f"{' or '.join(str(d) for d in dtypes)}, got {list(shape)} {x.dtype}")
-    if not x.is_cuda:
-        raise ValueError(f"{name}: expected a CUDA tensor")
+    _placed(x, name, device)
     return shape
 
 
-def _table(codes: torch.Tensor, scales: torch.Tensor, lead: tuple, rows: int, columns: int, name: str) -> None:
+def _table(codes: torch.Tensor, scales: torch.Tensor, lead: tuple, rows: int, columns: int, name: str) -> torch.device:
+    """Checks a table; its device."""
     if codes.dtype != torch.float8_e4m3fn or tuple(codes.shape) != (*lead, rows, pitch(columns)):
         raise ValueError(f"{name}: expected float8_e4m3fn {[*lead, rows, pitch(columns)]}, got {codes.dtype} {list(codes.shape)}")
     if scales.dtype != torch.float32 or tuple(scales.shape) != (*lead, blocks(rows), blocks(columns)):
         raise ValueError(f"{name}: expected float32 scales {[*lead, blocks(rows), blocks(columns)]}, got {scales.dtype} "
                          f"{list(scales.shape)}")
+    if codes.device != scales.device:
+        raise ValueError(f"{name}: codes on {codes.device}, scales on {scales.device}")
+    return codes.device
 
 
 def _quantized(name: str, x: torch.Tensor, codes_shape: tuple, scales_shape: tuple):
@@ -90,6 +103,7 @@ def quantize_blocks(x: torch.Tensor):
 def transpose_blocks(codes: torch.Tensor, scales: torch.Tensor, rows: int, columns: int):
     """The table of the transposed matrix, for the gradient by the input."""
     _table(codes, scales, (), rows, columns, "table")
+    _placed(codes, "table")
     to = torch.empty((columns, pitch(rows)), dtype=torch.float8_e4m3fn, device=codes.device)
     to_scales = torch.empty((blocks(columns), blocks(rows)), dtype=torch.float32, device=codes.device)
     _done(ops.k3_moe_fp8_transpose_blocks(to, to_scales, codes, scales, rows, columns), "k3_moe_fp8_transpose_blocks")
@@ -122,13 +136,13 @@ class Fp8Linear:
     """y = x W^T for a table of W [rows, columns]."""
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, columns: int):
-        _table(codes, scales, (), rows, columns, "table")
+        self._device = _table(codes, scales, (), rows, columns, "table")
         self.codes, self.scales, self.rows, self.columns = codes, scales, rows, columns
         self._workspace = _Workspace(lambda tokens: ops.k3_moe_fp8_linear_workspace_bytes(tokens, columns))
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         """x bf16 [tokens, columns] -> bf16 [tokens, rows]."""
-        tokens, _ = _matrix(x, "x", self.columns)
+        tokens, _ = _matrix(x, "x", self.columns, device=self._device)
         out = x.new_empty((tokens, self.rows))
         if tokens:
             ws = self._workspace.of(tokens, x.device)
@@ -176,10 +190,12 @@ class Fp8Experts:
         if w1.dim() != 3 or activation not in _ACTIVATIONS:
             raise ValueError("w1: expected [experts, expert_hidden, hidden], activation 'swiglu' or 'situ'")
         experts, expert_hidden, hidden = w1.shape
+        self._device = w1.device
         for name, codes, scales, rows, columns in (("w1", w1, w1_scales, expert_hidden, hidden),
                                                    ("w3", w3, w3_scales, expert_hidden, hidden),
                                                    ("w2", w2, w2_scales, hidden, expert_hidden)):
-            _table(codes, scales, (experts,), rows, columns, name)
+            if _table(codes, scales, (experts,), rows, columns, name) != self._device:
+                raise ValueError(f"{name}: on {codes.device}, w1 on {self._device}")
             if not (codes.is_contiguous() and scales.is_contiguous()):
                 raise ValueError("operator arguments must be contiguous")
         self.hidden, self.top_k = hidden, top_k
@@ -194,10 +210,11 @@ class Fp8Experts:
                 shared: torch.Tensor | None = None) -> torch.Tensor:
         """x bf16 [tokens, hidden], ids int32 and weights f32 [tokens, top_k] -> bf16 [tokens, hidden], plus
         ``shared`` (bf16, the shared expert's output) if given."""
-        tokens, _ = _matrix(x, "x", self.hidden)
+        tokens, _ = _matrix(x, "x", self.hidden, device=self._device)
         for name, t, dtype in (("ids", ids, torch.int32), ("weights", weights, torch.float32)):
-            if t.dtype is not dtype or t.shape != (tokens, self.top_k) or not t.is_cuda:
-                raise ValueError(f"{name}: expected {dtype} {[tokens, self.top_k]} on the GPU, got {t.dtype} {list(t.shape)}")
+            if t.dtype is not dtype or t.shape != (tokens, self.top_k):
+                raise ValueError(f"{name}: expected {dtype} {[tokens, self.top_k]}, got {t.dtype} {list(t.shape)}")
+            _placed(t, name)
         if shared is not None and _matrix(shared, "shared", self.hidden)[0] != tokens:
             raise ValueError("shared: another number of tokens than x")
         out = x.new_empty((tokens, self.hidden))
