@@ -4,8 +4,9 @@
 Codes are ``torch.float8_e4m3fn`` with rows padded to 16 bytes (``pitch``); activations get one
 scale per row and 128 columns, weights one per 128 x 128.  An object keeps its tables and a
 workspace that grows with the largest call, so its calls have to be ordered (one stream, or
-streams that wait for one another), as those of ``MoELayer``.  All tensors of a call lie on the
-current CUDA device.
+streams that wait for one another), as those of ``MoELayer``.  A workspace that a captured call
+used stays with the object: a graph may be replayed after larger calls, while the object lives.
+All tensors of a call lie on the current CUDA device.
 
     table, scales = fp8.quantize_blocks(weight)             # bf16 or f32 [rows, columns]
     y = fp8.Fp8Linear(table, scales, rows, columns).forward(x)
@@ -112,15 +113,22 @@ def transpose_blocks(codes: torch.Tensor, scales: torch.Tensor, rows: int, colum
 
 class _Workspace:
     """Device scratch of an object for the largest sizes (tokens, or tokens and sequences) it has seen;
-    ``need(*sizes)`` gives the bytes."""
+    ``need(*sizes)`` gives the bytes.  A graph keeps the addresses of the calls that it captured, so what was
+    handed out during a capture is never given back, while other scratch is when a larger call replaces it."""
 
     def __init__(self, need):
         self._need, self._held, self._sizes, self.bytes = need, None, (), 0
+        self._captured: list[torch.Tensor] = []
+
+    def _keep(self) -> torch.Tensor:
+        if torch.cuda.is_current_stream_capturing() and not any(t is self._held for t in self._captured):
+            self._captured.append(self._held)
+        return self._held
 
     def of(self, *sizes_device) -> torch.Tensor:
         *sizes, device = sizes_device
         if self._held is not None and self._held.device == device and all(map(int.__le__, sizes, self._sizes)):
-            return self._held
+            return self._keep()
         sizes = [max(pair) for pair in zip(sizes, self._sizes)] if self._sizes else sizes
         need = self._need(*sizes)
         if need == 0:
@@ -129,7 +137,7 @@ class _Workspace:
             self._held.record_stream(torch.cuda.current_stream(self._held.device))
         self._held = torch.empty(need, dtype=torch.uint8, device=device)
         self._sizes, self.bytes = sizes, need
-        return self._held
+        return self._keep()
 
 
 class Fp8Linear:
