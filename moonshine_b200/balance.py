@@ -17,7 +17,10 @@ _SCORES = {"sigmoid": ops.SCORE_SIGMOID, "softmax": ops.SCORE_SOFTMAX}
 def _check(t, name, dtype, shape):
     if t.dtype is not dtype or t.shape != shape:
         raise ValueError(f"{name}: expected {dtype} {list(shape)}, got {t.dtype} {list(t.shape)}")
-    _placed(t, name)
+
+
+def _given(**tensors):
+    return [pair for pair in tensors.items() if pair[1] is not None]
 
 
 class RouterBalance:
@@ -39,7 +42,6 @@ class RouterBalance:
             return tokens, 1
         if offsets.dtype is not torch.int32 or offsets.dim() != 1 or offsets.shape[0] < 2:
             raise ValueError(f"offsets: expected int32 [sequences + 1], got {offsets.dtype} {list(offsets.shape)}")
-        _placed(offsets, "offsets")
         return tokens, offsets.shape[0] - 1
 
     def forward(self, logits: torch.Tensor | None, ids: torch.Tensor, offsets: torch.Tensor | None = None):
@@ -48,6 +50,7 @@ class RouterBalance:
         tokens, sequences = self._sequences(ids, offsets)
         if logits is not None:
             _check(logits, "logits", torch.float32, (tokens, self.experts))
+        _placed(*_given(ids=ids, logits=logits, offsets=offsets))
         make = ids.new_empty if tokens else ids.new_zeros
         counts = make((sequences, self.experts))
         loss = means = None
@@ -74,6 +77,7 @@ class RouterBalance:
             _check(counts, "counts", torch.int32, (sequences, self.experts))
         if d_weights is not None:
             _check(d_weights, "d_weights", torch.float32, (tokens, self.top_k))
+        _placed(*_given(ids=ids, logits=logits, counts=counts, offsets=offsets, d_loss=d_loss, d_weights=d_weights))
         d_logits = logits.new_empty((tokens, self.experts))
         if tokens:
             _done(ops.k3_moe_router_backward(d_logits, logits, ids, counts, offsets, d_loss, d_weights, tokens, sequences,
