@@ -34,7 +34,7 @@ enum Epilogue : int { kOutBf16 = 0, kOutF32 = 1, kOutActivated = 2 };
 // out [rows, n] = a [rows, k] b^T.  With offsets (u32 [groups + 1] on the device) a's rows are grouped:
 // rows [offsets[g], offsets[g + 1]) are multiplied by matrix g of b [groups, n, k].  kOutActivated: b is
 // the gate, b2 the up matrix, and what is written is the activation, quantised by rows (out,
-// out_scales).  Other grouped products write f32 where grouped_few() holds and bf16 elsewhere.
+// out_scales).  Other grouped products write f32.
 struct Product {
     void *out, *out_scales;
     const void *a, *a_scales;

@@ -5,18 +5,16 @@
 #include "k3_moe_layer.h"
 #include "k3_moe_ops.h"
 
-#include <algorithm>
-
 using namespace k3;
 using namespace k3::fp8;
 
 namespace {
 
 // out[t] = bf16(sum_r weights[t, r] * rows[index[t, r]]), and bf16(that + shared[t]) with shared, of f32 rows: what
-// k3_moe_combine does of bf16 ones.  Rounding the rows to bf16 adds an error as large as that of the output's own
-// rounding (2.4e-3 of the norm instead of 1.7e-3); for few rows f32 costs nothing, while for thousands of rows per
-// expert it would double the largest traffic of the call (4096 tokens, 16 of 64 experts: 0.94 GB more each way, 0.3 of
-// 3.7 ms), so there the rows are bf16.
+// k3_moe_combine does of bf16 ones.  Rows rounded to bf16 would add an error as large as that of the output's own
+// rounding (2.4e-3 of the norm instead of 1.7e-3), so they are f32 for any number of tokens, and a token's precision
+// does not depend on how many share its call.  4096 tokens, 16 of 64 experts of 7168 x 2048: 4.18 ms, with bf16 rows,
+// 0.94 GB less each way, 3.85.
 __global__ void __launch_bounds__(128)
 combine_f32_kernel(uint16_t *out, const float *rows, const uint32_t *index, const float *weights, const uint16_t *shared,
                    uint32_t top_k, uint32_t hidden) {
@@ -73,7 +71,7 @@ struct ExpertsWorkspace {
     size_t dispatch_bytes;
     void *dispatch;
     Rows x, act;
-    void *rows_out;                  // f32 or bf16 (rows_f32()), one row more than there are routes: the spare one
+    float *rows_out;                 // one row more than there are routes: the spare one
     ExpertsWorkspace(const k3_moe_fp8_experts_desc *d, uint32_t tokens, void *base)
         : carve{(char *)base},
           offsets((uint32_t *)carve.take((d->experts + 1u) * sizeof(uint32_t))),
@@ -84,11 +82,7 @@ struct ExpertsWorkspace {
           dispatch(carve.take(dispatch_bytes)),
           x(carve, (uint64_t)tokens * d->top_k, d->hidden),
           act(carve, (uint64_t)tokens * d->top_k, d->expert_hidden),
-          rows_out(carve.take(std::max(((uint64_t)tokens * d->top_k + 1u) * 2u,       // never less for more tokens
-                                       (std::min((uint64_t)tokens * d->top_k, (uint64_t)grouped_few_rows * d->experts) + 1u) * 4u) *
-                              d->hidden)) {}
-    // expert rows in f32: where the kernels for few rows compute them
-    static bool rows_f32(const k3_moe_fp8_experts_desc *d, uint32_t routes) { return grouped_few(routes, d->experts); }
+          rows_out((float *)carve.take(((uint64_t)tokens * d->top_k + 1u) * d->hidden * sizeof(float))) {}
 };
 
 bool experts_ok(const k3_moe_fp8_experts_desc *d, uint32_t tokens) {
@@ -181,7 +175,7 @@ extern "C" bool k3_moe_fp8_experts_forward(const k3_moe_fp8_experts_desc *d, voi
     const uint32_t routes = tokens * d->top_k;
     // One token: its routes are the groups as they come, and the down product forms their weighted sum.  Three
     // launches; with dispatch, placed rows and combine 16 of 64 experts of 7168 x 2048 took 141 us.
-    const bool token = tokens == 1u, f32 = ExpertsWorkspace::rows_f32(d, routes);
+    const bool token = tokens == 1u;
     if (token) {
         if (!k3_moe_fp8_quantize_rows(w.x.codes, w.x.scales, x, 1u, d->hidden, K3_MOE_FP8_BF16, stream)) return false;
     } else {
@@ -190,9 +184,8 @@ extern "C" bool k3_moe_fp8_experts_forward(const k3_moe_fp8_experts_desc *d, voi
             return false;
         }
         const Placement at{w.inv_perm, (const uint32_t *)ids, d->top_k, d->experts, routes};
-        const uint32_t row_bytes = d->hidden * (f32 ? 4u : 2u);
-        if (!quantize_placed(w.x.codes, w.x.scales, x, tokens, d->hidden, at, (char *)w.rows_out + (uint64_t)routes * row_bytes,
-                             row_bytes, stream)) {
+        if (!quantize_placed(w.x.codes, w.x.scales, x, tokens, d->hidden, at, w.rows_out + (uint64_t)routes * d->hidden,
+                             d->hidden * (uint32_t)sizeof(float), stream)) {
             return false;
         }
     }
@@ -228,7 +221,7 @@ extern "C" bool k3_moe_fp8_experts_forward(const k3_moe_fp8_experts_desc *d, voi
     p.b2 = p.b2_scales = nullptr;
     p.n = d->hidden;
     p.k = d->expert_hidden;
-    p.epilogue = token || !f32 ? kOutBf16 : kOutF32;
+    p.epilogue = token ? kOutBf16 : kOutF32;
     if (token) {
         p.out = out;
         p.rows = 1u;
@@ -237,10 +230,7 @@ extern "C" bool k3_moe_fp8_experts_forward(const k3_moe_fp8_experts_desc *d, voi
         return token_down(p, stream);
     }
     if (!product(p, stream)) return false;
-    if (f32) {
-        return launch_chained(combine_f32_kernel, dim3(tokens, (d->hidden / 4u + 127u) / 128u), 128, 0, stream, (uint16_t *)out,
-                              (const float *)w.rows_out, (const uint32_t *)w.inv_perm, (const float *)weights,
-                              (const uint16_t *)shared, d->top_k, d->hidden);
-    }
-    return k3_moe_combine(out, w.rows_out, w.inv_perm, weights, shared, tokens, d->top_k, d->hidden, stream);
+    return launch_chained(combine_f32_kernel, dim3(tokens, (d->hidden / 4u + 127u) / 128u), 128, 0, stream, (uint16_t *)out,
+                          (const float *)w.rows_out, (const uint32_t *)w.inv_perm, (const float *)weights,
+                          (const uint16_t *)shared, d->top_k, d->hidden);
 }

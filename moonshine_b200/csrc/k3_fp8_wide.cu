@@ -686,7 +686,7 @@ bool launch_whole(const Product &p, cudaStream_t stream) {
 
 bool k3::fp8::wide_product(const Product &p, cudaStream_t stream) {
     if (p.epilogue == kOutActivated) return launch_grouped<kOutActivated>(p, stream);
-    if (p.offsets) return launch_grouped<kOutBf16>(p, stream);
+    if (p.offsets) return launch_grouped<kOutF32>(p, stream);
     if (p.b_scale_layout == K3_MOE_FP8_ROWS) {
         return p.epilogue == kOutF32 ? launch_whole<kOutF32, true>(p, stream) : launch_whole<kOutBf16, true>(p, stream);
     }
