@@ -38,9 +38,10 @@ struct Shape {
     int softmax;
 };
 
-// The fast base-2 exponential and reciprocal (2 units in the last place each, of an argument's size the
-// exponential's): 4e-7 of a score.  With expf, a rounded quotient and single operations the pass over the
-// logits was bound by its instructions, 32768 x 896 forward and backward 198 us.
+// Scores with the fast base-2 exponential and reciprocal (2^-22 and 2^-23 of their results): 6e-7 of a score down to
+// 2^-126, below which it is 0.  The exponent's product with log2 e would be off by 2^-24 of itself, 5e-6 of a score at a
+// logit of -80, so what it rounds away goes into the result as a factor.  With expf, a rounded quotient and single
+// operations the pass over the logits was bound by its instructions, 32768 x 896 forward and backward 198 us.
 K3_DEVINL float exp2_fast(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -51,8 +52,28 @@ K3_DEVINL float reciprocal_fast(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-constexpr float kLog2E = 1.44269504f;
-K3_DEVINL float sigmoid(float x) { return reciprocal_fast(1.0f + exp2_fast(x * -kLog2E)); }
+constexpr float kLog2E = 1.44269502162933349609f, kLog2ELow = 1.92596299e-8f, kLn2 = 0.693147181f;    // log2 e in two parts
+K3_DEVINL uint64_t both(float x) { return pack2(x, x); }
+// a, but 200 where it is larger (e^-200 is 0, and an infinity would leave no remainder); NaN stays
+K3_DEVINL float bounded(float a) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(200.0f));
+    return r;
+}
+// e^-a of 0 <= a <= 200
+K3_DEVINL float exp_negative(float a) {
+    const float t = __fmul_rn(a, kLog2E), rest = fmaf(a, -kLog2ELow, fmaf(a, -kLog2E, t)), e = exp2_fast(-t);
+    return fmaf(e * kLn2, rest, e);
+}
+K3_DEVINL uint64_t exp_negative2(uint64_t a) {
+    const uint64_t t = mul2(a, both(kLog2E)), rest = fma2(a, both(-kLog2ELow), fma2(a, both(-kLog2E), t));
+    const uint64_t e = pack2(exp2_fast(-lo2(t)), exp2_fast(-hi2(t)));
+    return fma2(mul2(e, both(kLn2)), rest, e);
+}
+K3_DEVINL float sigmoid(float x) {
+    const float e = exp_negative(bounded(fabsf(x))), r = reciprocal_fast(1.0f + e);
+    return x > 0.0f ? r : e * r;
+}
 
 template <int kBytes>
 K3_DEVINL void copy_async(float *to, const float *from) {
@@ -154,11 +175,12 @@ struct Row {
     K3_DEVINL Softmax scores(int softmax) {
         Softmax f{0.f, 0.f};
         if (!softmax) {
-            const uint64_t by = pack2(-kLog2E, -kLog2E), one = pack2(1.0f, 1.0f);
 #pragma unroll
             for (uint32_t i = 0; i < kV * 2u; i++) {
-                const uint64_t t = mul2(v[i], by), y = add2(pack2(exp2_fast(lo2(t)), exp2_fast(hi2(t))), one);
-                v[i] = pack2(reciprocal_fast(lo2(y)), reciprocal_fast(hi2(y)));
+                const float x = lo2(v[i]), y = hi2(v[i]);
+                const uint64_t e = exp_negative2(pack2(bounded(fabsf(x)), bounded(fabsf(y)))), d = add2(e, both(1.0f));
+                const uint64_t r = pack2(reciprocal_fast(lo2(d)), reciprocal_fast(hi2(d))), small = mul2(e, r);
+                v[i] = pack2(x > 0.0f ? lo2(r) : lo2(small), y > 0.0f ? hi2(r) : hi2(small));
             }
             return f;
         }
@@ -178,12 +200,10 @@ struct Row {
             fill(f.over);
             return f;
         }
-        // the difference first: a product with the logarithm of the lowest values would not be finite
-        const uint64_t less = pack2(-f.top, -f.top), by = pack2(kLog2E, kLog2E);
 #pragma unroll
         for (uint32_t i = 0; i < kV * 2u; i++) {
-            const uint64_t t = mul2(add2(v[i], less), by);
-            v[i] = pack2(exp2_fast(lo2(t)), exp2_fast(hi2(t)));
+            const uint64_t less = fma2(v[i], both(-1.0f), both(f.top));
+            v[i] = exp_negative2(pack2(bounded(lo2(less)), bounded(hi2(less))));
         }
         f.over = 1.0f / sum();
         scale(f.over);
@@ -489,7 +509,7 @@ router_backward_kernel(float *d_logits, const float *logits, const uint32_t *ids
         if (d_weights) {
             if (lane < a.top_k && !chosen) g_balance_status = 2u;
             // the weights' share at the chosen, through shared memory to the lanes that hold them
-            const float si = !chosen ? 0.f : a.softmax ? exp2_fast((l - soft.top) * kLog2E) * soft.over : sigmoid(l);
+            const float si = !chosen ? 0.f : a.softmax ? exp_negative(bounded(soft.top - l)) * soft.over : sigmoid(l);
             const float all = warp_sum(si), weighted = warp_sum(w * si);
             const float under = reciprocal_fast(kTiny + all);
             const float share = route_scale * (w - weighted * under) * under;
