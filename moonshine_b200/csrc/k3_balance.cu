@@ -171,7 +171,10 @@ struct Row {
         for (uint32_t i = 1; i < kV * 2u; i++) s = add2(s, v[i]);
         return warp_sum(lo2(s) + hi2(s));
     }
-    // logits -> scores; experts past the end have the logit -inf and get the score 0
+    // logits -> scores; experts past the end have the logit -inf and get the score 0.  kSmaller: of a sigmoid s the
+    // smaller of s and 1 - s, negative (-0 too) where that is 1 - s: the derivative s (1 - s) of a score near 1 has no
+    // bits left in s.
+    template <bool kSmaller>
     K3_DEVINL Softmax scores(int softmax) {
         Softmax f{0.f, 0.f};
         if (!softmax) {
@@ -180,7 +183,8 @@ struct Row {
                 const float x = lo2(v[i]), y = hi2(v[i]);
                 const uint64_t e = exp_negative2(pack2(bounded(fabsf(x)), bounded(fabsf(y)))), d = add2(e, both(1.0f));
                 const uint64_t r = pack2(reciprocal_fast(lo2(d)), reciprocal_fast(hi2(d))), small = mul2(e, r);
-                v[i] = pack2(x > 0.0f ? lo2(r) : lo2(small), y > 0.0f ? hi2(r) : hi2(small));
+                v[i] = kSmaller ? pack2(x > 0.0f ? -lo2(small) : lo2(small), y > 0.0f ? -hi2(small) : hi2(small))
+                                : pack2(x > 0.0f ? lo2(r) : lo2(small), y > 0.0f ? hi2(r) : hi2(small));
             }
             return f;
         }
@@ -210,6 +214,14 @@ struct Row {
         return f;
     }
 };
+
+// Sigmoids of what scores<true>() gives for them, and their derivatives
+K3_DEVINL float sigmoid_of(float smaller) { return (int32_t)__float_as_uint(smaller) < 0 ? 1.0f + smaller : smaller; }
+K3_DEVINL uint64_t sigmoid_of2(uint64_t smaller) { return pack2(sigmoid_of(lo2(smaller)), sigmoid_of(hi2(smaller))); }
+K3_DEVINL uint64_t derivative_of2(uint64_t smaller) {
+    const uint64_t y = smaller & 0x7fffffff7fffffffull;
+    return mul2(y, fma2(y, both(-1.0f), both(1.0f)));
+}
 
 // the sequence that holds `token`: the last one that starts at or before it (sequences - 1 at most)
 K3_DEVINL uint32_t sequence_of(const uint32_t *offsets, uint32_t sequences, uint32_t token) {
@@ -264,7 +276,7 @@ K3_DEVINL void sum_tokens(float *rows_s, const float *logits, const uint32_t *id
             copies_wait<kForwardStages - 1>();
             Row<kV, kVector> p;
             p.load(mine + stage * kPitch, kPitch, lane, 0.f);
-            p.scores(a.softmax);
+            p.template scores<false>(a.softmax);
             const float r = a.softmax ? 1.0f : reciprocal_fast(kTiny + p.sum());
             const uint64_t r2 = pack2(r, r);
 #pragma unroll
@@ -491,15 +503,16 @@ router_backward_kernel(float *d_logits, const float *logits, const uint32_t *ids
                 f.scale(scale);
             }
         }
-        const Softmax soft = p.scores(a.softmax);
+        const Softmax soft = p.template scores<true>(a.softmax);
         // the loss by a score is by (f - mean)
         float by = c, mean = 0.f;
         if (d_loss && !a.softmax) {
             uint64_t z = pack2(0.f, 0.f), fp = z;
 #pragma unroll
             for (uint32_t i = 0; i < kV * 2u; i++) {
-                z = add2(z, p.v[i]);
-                fp = fma2(f.v[i], p.v[i], fp);
+                const uint64_t score = sigmoid_of2(p.v[i]);
+                z = add2(z, score);
+                fp = fma2(f.v[i], score, fp);
             }
             const float r = reciprocal_fast(kTiny + warp_sum(lo2(z) + hi2(z)));
             mean = warp_sum(lo2(fp) + hi2(fp)) * r;
@@ -510,9 +523,14 @@ router_backward_kernel(float *d_logits, const float *logits, const uint32_t *ids
             if (lane < a.top_k && !chosen) g_balance_status = 2u;
             // the weights' share at the chosen, through shared memory to the lanes that hold them
             const float si = !chosen ? 0.f : a.softmax ? exp_negative(bounded(soft.top - l)) * soft.over : sigmoid(l);
-            const float all = warp_sum(si), weighted = warp_sum(w * si);
+            // (w - sum w s / D) / D with D = tiny + sum s, of the weights' gradients less that of the largest score: where
+            // they are equal, as a single choice is with itself, the difference is 0 and w tiny / D is left
+            const uint32_t bits = __float_as_uint(si), most = __reduce_max_sync(0xffffffffu, bits);
+            const uint32_t holders = __ballot_sync(0xffffffffu, chosen && bits == most);
+            const float w0 = holders ? __shfl_sync(0xffffffffu, w, __ffs(holders) - 1) : 0.f, more = chosen ? w - w0 : 0.f;
+            const float all = warp_sum(si), weighted = warp_sum(more * si);
             const float under = reciprocal_fast(kTiny + all);
-            const float share = route_scale * (w - weighted * under) * under;
+            const float share = route_scale * (more - weighted * under + w0 * (kTiny * under)) * under;
             // an expert named twice keeps one of the lanes' numbers (with __match_any_sync for this 30000 x 160 took 32 us
             // instead of 20)
             if (chosen) row_s[id] = __uint_as_float(lane);
@@ -555,7 +573,6 @@ router_backward_kernel(float *d_logits, const float *logits, const uint32_t *ids
             dp = pack2(-all, -all);
         }
         float *out = d_logits + (uint64_t)t * a.experts;
-        const uint64_t one = pack2(1.0f, 1.0f), minus = pack2(-1.0f, -1.0f);
 #pragma unroll
         for (uint32_t g = 0; g < kV; g++) {
             uint64_t d[2];
@@ -563,7 +580,7 @@ router_backward_kernel(float *d_logits, const float *logits, const uint32_t *ids
 #pragma unroll
             for (uint32_t j = 0; j < 2u; j++) {
                 const uint64_t q = p.v[2u * g + j];
-                d[j] = a.softmax ? mul2(q, add2(d[j], dp)) : mul2(d[j], mul2(q, fma2(q, minus, one)));
+                d[j] = a.softmax ? mul2(q, add2(d[j], dp)) : mul2(d[j], derivative_of2(q));
             }
             Row<kV, kVector>::put(out, d, a.experts, lane, g);
         }
