@@ -561,16 +561,29 @@ router_backward_kernel(float *d_logits, const float *logits, const uint32_t *ids
                 d[1] = fma2(by2, add2(f.v[2u * g + 1u], less), d[1]);
             }
         };
-        uint64_t dp = pack2(0.f, 0.f);
+        // softmax: p (d - sum d p) of the d less that of the largest score, so that a score near 1 keeps the small sum of
+        // the others'.  The largest have the exponential 1, and so the score `over`.
+        uint64_t shift = pack2(0.f, 0.f), dp = shift;
         if (a.softmax) {
+            float top = -INFINITY;
 #pragma unroll
             for (uint32_t g = 0; g < kV; g++) {
                 uint64_t d[2];
                 by_scores(d, g);
-                dp = fma2(d[0], p.v[2u * g], fma2(d[1], p.v[2u * g + 1u], dp));
+#pragma unroll
+                for (uint32_t j = 0; j < 2u; j++) {
+                    if (lo2(p.v[2u * g + j]) == soft.over) top = fmaxf(top, lo2(d[j]));
+                    if (hi2(p.v[2u * g + j]) == soft.over) top = fmaxf(top, hi2(d[j]));
+                }
             }
-            const float all = warp_sum(lo2(dp) + hi2(dp));
-            dp = pack2(-all, -all);
+            shift = both(-warp_max(top));
+#pragma unroll
+            for (uint32_t g = 0; g < kV; g++) {
+                uint64_t d[2];
+                by_scores(d, g);
+                dp = fma2(add2(d[0], shift), p.v[2u * g], fma2(add2(d[1], shift), p.v[2u * g + 1u], dp));
+            }
+            dp = both(-warp_sum(lo2(dp) + hi2(dp)));
         }
         float *out = d_logits + (uint64_t)t * a.experts;
 #pragma unroll
@@ -580,7 +593,7 @@ router_backward_kernel(float *d_logits, const float *logits, const uint32_t *ids
 #pragma unroll
             for (uint32_t j = 0; j < 2u; j++) {
                 const uint64_t q = p.v[2u * g + j];
-                d[j] = a.softmax ? mul2(q, add2(d[j], dp)) : mul2(d[j], derivative_of2(q));
+                d[j] = a.softmax ? mul2(q, add2(add2(d[j], shift), dp)) : mul2(d[j], derivative_of2(q));
             }
             Row<kV, kVector>::put(out, d, a.experts, lane, g);
         }

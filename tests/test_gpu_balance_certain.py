@@ -93,3 +93,24 @@ def test_loss_gradient_of_large_logits():
     mean = (f * s).sum(1, keepdim=True) / z
     off = (got - by * (f - mean)).abs()
     assert bool((off <= LIMIT * by * (f + mean)).all())
+
+
+@pytest.mark.parametrize("experts", [48, 200, 1000])
+def test_softmax_gradient_of_a_nearly_certain_expert(experts):
+    """One logit 12 to 25 above the others: its gradient is the small sum of theirs.  The gradient by a score is a
+    share f of counts up to n, with three roundings; two that differ do so by 1 / n of themselves at least."""
+    tokens, top_k, g = 300, 4, torch.Generator().manual_seed(experts)
+    logits = torch.randn(tokens, experts, generator=g) * 0.5
+    logits.scatter_(1, torch.randint(0, experts, (tokens, 1), generator=g), torch.rand(tokens, 1, generator=g) * 13 + 14)
+    ids = (logits + 2 * torch.randn(tokens, experts, generator=g)).topk(top_k, 1).indices.to(torch.int32)
+    router = balance.RouterBalance(experts, top_k, "softmax", ALPHA, SCALE)
+    counts = router.forward(*cuda(logits, ids))[0]
+    got = router.backward(*cuda(logits, ids), counts, d_loss=torch.ones(1, device="cuda")).cpu().double()
+    n, f = shares(ids, tokens, experts, top_k)
+    p = torch.softmax(logits.double(), 1)
+    d = ALPHA / tokens * f.expand_as(p)
+    top = d.gather(1, p.argmax(1, keepdim=True))
+    others = ((d - top).abs() * p).sum(1, keepdim=True)
+    off = (got - p * ((d - top) - ((d - top) * p).sum(1, keepdim=True))).abs()
+    limit = LIMIT + 2 * 3 * 2.0 ** -24 * int(n.max())
+    assert bool((off <= limit * p * ((d - top).abs() + others)).all())
