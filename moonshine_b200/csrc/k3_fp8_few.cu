@@ -661,7 +661,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 
     tc_fence_before();
     __syncthreads();
-    if (threadIdx.x == 0 && *abort_flag != 0u) atomicExch(&g_fp8_few_status, 1u);
+    if (threadIdx.x == 0 && *abort_flag != 0u) atomicOr(&g_fp8_few_status, 1u);
     if (warp == 1u) {
         tc_fence_after();
         tmem_dealloc(tmem, L::kTmem);
