@@ -38,22 +38,11 @@ struct Shape {
     int softmax;
 };
 
-// Scores with the fast base-2 exponential and reciprocal (2^-22 and 2^-23 of their results): 6e-7 of a score down to
+// Scores with the fast base-2 exponential and reciprocal: 6e-7 of a score down to
 // 2^-126, below which it is 0.  The exponent's product with log2 e would be off by 2^-24 of itself, 5e-6 of a score at a
 // logit of -80, so what it rounds away goes into the result as a factor.  With expf, a rounded quotient and single
 // operations the pass over the logits was bound by its instructions, 32768 x 896 forward and backward 198 us.
-K3_DEVINL float exp2_fast(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-K3_DEVINL float reciprocal_fast(float x) {
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-constexpr float kLog2E = 1.44269502162933349609f, kLog2ELow = 1.92596299e-8f, kLn2 = 0.693147181f;    // log2 e in two parts
-K3_DEVINL uint64_t both(float x) { return pack2(x, x); }
+constexpr float kLn2 = 0.693147181f;
 // a, but 200 where it is larger (e^-200 is 0, and an infinity would leave no remainder); NaN stays
 K3_DEVINL float bounded(float a) {
     float r;
@@ -66,9 +55,9 @@ K3_DEVINL float exp_negative(float a) {
     return fmaf(e * kLn2, rest, e);
 }
 K3_DEVINL uint64_t exp_negative2(uint64_t a) {
-    const uint64_t t = mul2(a, both(kLog2E)), rest = fma2(a, both(-kLog2ELow), fma2(a, both(-kLog2E), t));
+    const uint64_t t = mul2(a, both2(kLog2E)), rest = fma2(a, both2(-kLog2ELow), fma2(a, both2(-kLog2E), t));
     const uint64_t e = pack2(exp2_fast(-lo2(t)), exp2_fast(-hi2(t)));
-    return fma2(mul2(e, both(kLn2)), rest, e);
+    return fma2(mul2(e, both2(kLn2)), rest, e);
 }
 K3_DEVINL float sigmoid(float x) {
     const float e = exp_negative(bounded(fabsf(x))), r = reciprocal_fast(1.0f + e);
@@ -181,7 +170,7 @@ struct Row {
 #pragma unroll
             for (uint32_t i = 0; i < kV * 2u; i++) {
                 const float x = lo2(v[i]), y = hi2(v[i]);
-                const uint64_t e = exp_negative2(pack2(bounded(fabsf(x)), bounded(fabsf(y)))), d = add2(e, both(1.0f));
+                const uint64_t e = exp_negative2(pack2(bounded(fabsf(x)), bounded(fabsf(y)))), d = add2(e, both2(1.0f));
                 const uint64_t r = pack2(reciprocal_fast(lo2(d)), reciprocal_fast(hi2(d))), small = mul2(e, r);
                 v[i] = kSmaller ? pack2(x > 0.0f ? -lo2(small) : lo2(small), y > 0.0f ? -hi2(small) : hi2(small))
                                 : pack2(x > 0.0f ? lo2(r) : lo2(small), y > 0.0f ? hi2(r) : hi2(small));
@@ -206,7 +195,7 @@ struct Row {
         }
 #pragma unroll
         for (uint32_t i = 0; i < kV * 2u; i++) {
-            const uint64_t less = fma2(v[i], both(-1.0f), both(f.top));
+            const uint64_t less = fma2(v[i], both2(-1.0f), both2(f.top));
             v[i] = exp_negative2(pack2(bounded(lo2(less)), bounded(hi2(less))));
         }
         f.over = 1.0f / sum();
@@ -220,7 +209,7 @@ K3_DEVINL float sigmoid_of(float smaller) { return (int32_t)__float_as_uint(smal
 K3_DEVINL uint64_t sigmoid_of2(uint64_t smaller) { return pack2(sigmoid_of(lo2(smaller)), sigmoid_of(hi2(smaller))); }
 K3_DEVINL uint64_t derivative_of2(uint64_t smaller) {
     const uint64_t y = smaller & 0x7fffffff7fffffffull;
-    return mul2(y, fma2(y, both(-1.0f), both(1.0f)));
+    return mul2(y, fma2(y, both2(-1.0f), both2(1.0f)));
 }
 
 // the sequence that holds `token`: the last one that starts at or before it (sequences - 1 at most)
@@ -576,14 +565,14 @@ router_backward_kernel(float *d_logits, const float *logits, const uint32_t *ids
                     if (hi2(p.v[2u * g + j]) == soft.over) top = fmaxf(top, hi2(d[j]));
                 }
             }
-            shift = both(-warp_max(top));
+            shift = both2(-warp_max(top));
 #pragma unroll
             for (uint32_t g = 0; g < kV; g++) {
                 uint64_t d[2];
                 by_scores(d, g);
                 dp = fma2(add2(d[0], shift), p.v[2u * g], fma2(add2(d[1], shift), p.v[2u * g + 1u], dp));
             }
-            dp = both(-warp_sum(lo2(dp) + hi2(dp)));
+            dp = both2(-warp_sum(lo2(dp) + hi2(dp)));
         }
         float *out = d_logits + (uint64_t)t * a.experts;
 #pragma unroll

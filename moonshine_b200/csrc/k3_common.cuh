@@ -98,6 +98,21 @@ K3_DEVINL uint64_t add2(uint64_t a, uint64_t b) {
     return r;
 }
 
+K3_DEVINL uint64_t both2(float x) { return pack2(x, x); }
+
+// The fast base-2 exponential and reciprocal, within 2^-22 and 2^-23 of their results.
+K3_DEVINL float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+K3_DEVINL float reciprocal_fast(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+constexpr float kLog2E = 1.44269502162933349609f, kLog2ELow = 1.92596299e-8f;      // log2 e in two parts
+
 // 16-byte global load that does not allocate in L1 (weights are streamed once).
 K3_DEVINL uint4 ld_stream_16(const void *p) {
     uint4 v;

@@ -53,7 +53,8 @@ K3_DEVINL void mbar_drain(uint64_t *bar, uint32_t parity) {
     while (!mbar_try_wait(bar, parity) && global_timer_ns() - t0 < 100000000ull) {}
 }
 
-// The expert activation with the fast exponential and reciprocal, 4e-7 of the result: it is quantised to 4 bits next.
+// The expert activation with the fast exponential and reciprocal, 4e-7 of the result and, of a negative gate, 1.4e-7 times
+// its size (the exponent's rounding), where the result is small: it is quantised to 4 bits next.
 // The kind is a template argument, so that many elements go side by side: with a branch in each of a thread's elements
 // the warps waited for one element's chain after the other.
 //
@@ -79,23 +80,11 @@ struct ExpertActivation {
 };
 
 // The same for two elements at a time, with the sign turned around.
-K3_DEVINL uint64_t both2(float x) { return pack2(x, x); }
-K3_DEVINL float exponential_of_2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-K3_DEVINL float reciprocal(float x) {
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-constexpr float kLog2E = 1.44269504f;
 // 1 / (c + c e^(x s)), with s times log2 e
 K3_DEVINL uint64_t logistic2(uint64_t x, float s, float c) {
     const uint64_t t = mul2(x, both2(s));
-    const uint64_t d = fma2(pack2(exponential_of_2(lo2(t)), exponential_of_2(hi2(t))), both2(c), both2(c));
-    return pack2(reciprocal(lo2(d)), reciprocal(hi2(d)));
+    const uint64_t d = fma2(pack2(exp2_fast(lo2(t)), exp2_fast(hi2(t))), both2(c), both2(c));
+    return pack2(reciprocal_fast(lo2(d)), reciprocal_fast(hi2(d)));
 }
 K3_DEVINL uint64_t tanh2(uint64_t x) {
     const uint64_t y = mul2(x, x);
@@ -134,7 +123,7 @@ K3_DEVINL float lift_of(float scale) { return scale < 0x1p-90f ? 0x1p64f : 1.0f;
 // moved the running sums between registers.
 K3_DEVINL float inverse_of(float scale) {
     const float by = scale * lift_of(scale);
-    float y = reciprocal(by);
+    float y = reciprocal_fast(by);
     y = fmaf(y, fmaf(-by, y, 1.0f), y);
     y = fmaf(y, fmaf(-by, y, 1.0f), y);
     return (__float_as_uint(by) & 0x7fffffu) == 0x7fffffu ? __uint_as_float(__float_as_uint(y) | 1u) : y;
