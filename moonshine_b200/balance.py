@@ -19,10 +19,6 @@ def _check(t, name, dtype, shape):
         raise ValueError(f"{name}: expected {dtype} {list(shape)}, got {t.dtype} {list(t.shape)}")
 
 
-def _given(**tensors):
-    return [pair for pair in tensors.items() if pair[1] is not None]
-
-
 class RouterBalance:
     """``score``: "sigmoid" (the layer's router) or "softmax".  ``offsets`` int32 [sequences + 1] cut the
     tokens into sequences, each with a loss of its own; None: one sequence."""
@@ -50,7 +46,7 @@ class RouterBalance:
         tokens, sequences = self._sequences(ids, offsets)
         if logits is not None:
             _check(logits, "logits", torch.float32, (tokens, self.experts))
-        _placed(*_given(ids=ids, logits=logits, offsets=offsets))
+        _placed(("ids", ids), ("logits", logits), ("offsets", offsets))
         make = ids.new_empty if tokens else ids.new_zeros
         counts = make((sequences, self.experts))
         loss = means = None
@@ -77,7 +73,8 @@ class RouterBalance:
             _check(counts, "counts", torch.int32, (sequences, self.experts))
         if d_weights is not None:
             _check(d_weights, "d_weights", torch.float32, (tokens, self.top_k))
-        _placed(*_given(ids=ids, logits=logits, counts=counts, offsets=offsets, d_loss=d_loss, d_weights=d_weights))
+        _placed(("ids", ids), ("logits", logits), ("counts", counts), ("offsets", offsets), ("d_loss", d_loss),
+                ("d_weights", d_weights))
         d_logits = logits.new_empty((tokens, self.experts))
         if tokens:
             _done(ops.k3_moe_router_backward(d_logits, logits, ids, counts, offsets, d_loss, d_weights, tokens, sequences,

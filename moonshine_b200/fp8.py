@@ -44,20 +44,26 @@ def _done(ok: bool, name: str) -> None:
         raise RuntimeError(name + " failed")
 
 
-def _placed(*named, tables: torch.device | None = None) -> None:
-    """Refuses (name, tensor) that the kernels cannot read: they run on the current device, and take addresses.
-    One lookup of that device for all of them: with one for each the two balance calls took 4 us longer."""
-    at = None
-    for name, t in named:
-        if at is None:
-            at = t.device
-            wrong = at.type != "cuda" or at.index != torch.cuda.current_device()
-        else:
-            wrong = t.device != at
-        if wrong:
-            raise ValueError(f"{name}: expected a tensor on the current CUDA device, got one on {t.device}")
-    if tables is not None and tables != at:
-        raise ValueError(f"{named[0][0]}: on {at}, the tables are on {tables}")
+# the calls behind torch.cuda.current_device and is_current_stream_capturing, a fraction of their time
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
+
+
+def _placed(first, *others, tables: torch.device | None = None) -> None:
+    """Refuses a (name, tensor) that the kernels cannot read: they run on the current device, and take addresses.
+    None among the others is passed over.  ``tables``: the device that an object's tables are on."""
+    name, t = first
+    here = t.get_device()
+    wrong = here < 0 or here != _current_device()
+    if not wrong:
+        for name, t in others:
+            if t is not None and t.get_device() != here:
+                wrong = True
+                break
+    if wrong:
+        raise ValueError(f"{name}: expected a tensor on the current CUDA device, got one on {t.device}")
+    if tables is not None and tables.index != here:
+        raise ValueError(f"{first[0]}: on {first[1].device}, the tables are on {tables}")
 
 
 def _matrix(x: torch.Tensor, name: str, columns: int | None = None, dtypes=(torch.bfloat16,)) -> tuple[int, int]:
@@ -127,16 +133,19 @@ class _Workspace:
 
     def __init__(self, need):
         self._need, self._held, self._sizes, self.bytes = need, None, (), 0
-        self._captured: list[torch.Tensor] = []
+        self._last, self._captured = None, []
 
     def _keep(self) -> torch.Tensor:
-        if torch.cuda.is_current_stream_capturing() and not any(t is self._held for t in self._captured):
+        if _capturing() and not any(t is self._held for t in self._captured):
             self._captured.append(self._held)
         return self._held
 
     def of(self, *sizes_device) -> torch.Tensor:
+        if sizes_device == self._last:
+            return self._keep()
         *sizes, device = sizes_device
         if self._held is not None and self._held.device == device and all(map(int.__le__, sizes, self._sizes)):
+            self._last = sizes_device
             return self._keep()
         sizes = [max(pair) for pair in zip(sizes, self._sizes)] if self._sizes else sizes
         need = self._need(*sizes)
@@ -145,7 +154,7 @@ class _Workspace:
         if self._held is not None:              # the last call may still be running on this stream
             self._held.record_stream(torch.cuda.current_stream(self._held.device))
         self._held = torch.empty(need, dtype=torch.uint8, device=device)
-        self._sizes, self.bytes = sizes, need
+        self._sizes, self._last, self.bytes = sizes, sizes_device, need
         return self._keep()
 
 
@@ -190,7 +199,7 @@ class Fp8LinearGradient:
             _matrix(into, "into", self.columns, (torch.float32,))
             if into.shape[0] != self.rows:
                 raise ValueError(f"into: expected {[self.rows, self.columns]}, got {list(into.shape)}")
-        _placed(("dy", dy), ("x", x), *([("into", into)] if into is not None else ()))
+        _placed(("dy", dy), ("x", x), ("into", into))
         if tokens == 0:
             return into if into is not None else torch.zeros((self.rows, self.columns), dtype=torch.float32, device=dy.device)
         dw = into if into is not None else torch.empty((self.rows, self.columns), dtype=torch.float32, device=dy.device)
@@ -235,8 +244,7 @@ class Fp8Experts:
                 raise ValueError(f"{name}: expected {dtype} {[tokens, self.top_k]}, got {t.dtype} {list(t.shape)}")
         if shared is not None and _matrix(shared, "shared", self.hidden)[0] != tokens:
             raise ValueError("shared: another number of tokens than x")
-        _placed(("x", x), ("ids", ids), ("weights", weights), *([("shared", shared)] if shared is not None else ()),
-                tables=self._device)
+        _placed(("x", x), ("ids", ids), ("weights", weights), ("shared", shared), tables=self._device)
         out = x.new_empty((tokens, self.hidden))
         if tokens:
             ws = self._workspace.of(tokens, x.device)

@@ -23,7 +23,7 @@ def capturing(monkeypatch):
     state = [False]
     monkeypatch.setattr(torch, "empty", lambda need, dtype, device: Buffer(need, device))
     monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: None)
-    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state[-1])
+    monkeypatch.setattr(fp8, "_capturing", lambda: state[-1])
     return state
 
 
