@@ -34,8 +34,10 @@ extern "C" {
  * be NULL together: counts alone.  An id >= experts is not counted and raises
  * bit 1 of k3_moe_device_status().  experts <= 1024, top_k <= 32,
  * sequences <= 65535.  The workspace of more tokens serves fewer.  Sums run in
- * an order that only tokens and experts decide: the same call gives the same
- * bits. */
+ * an order that the numbers of tokens, sequences and experts, the cuts and the
+ * logits' alignment decide: the same call gives the same bits.  A score lies
+ * within 6e-7 of itself (softmax: besides the f32 rounding of the logit's
+ * distance from the row's largest) down to 2^-126, and is 0 below. */
 size_t k3_moe_balance_workspace_bytes(uint32_t tokens, uint32_t sequences, uint32_t experts);
 bool k3_moe_balance(void *counts, void *loss, void *means, const void *logits, const void *ids,
                     const void *offsets, uint32_t tokens, uint32_t sequences, uint32_t experts,
@@ -45,7 +47,8 @@ bool k3_moe_balance(void *counts, void *loss, void *means, const void *logits, c
 /* d_logits f32 [tokens, experts] from d_loss f32 [sequences] (NULL: none) and
  * d_weights f32 [tokens, top_k] (NULL: none; not both).  counts as
  * k3_moe_balance wrote them: the loss's f does not depend on the logits, so
- * nothing else of the forward pass is kept. */
+ * nothing else of the forward pass is kept.  An id >= experts has no weight, and
+ * raises bit 1 of k3_moe_device_status() where d_weights is given. */
 bool k3_moe_router_backward(void *d_logits, const void *logits, const void *ids,
                             const void *counts, const void *offsets, const void *d_loss,
                             const void *d_weights, uint32_t tokens, uint32_t sequences,

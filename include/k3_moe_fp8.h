@@ -18,6 +18,14 @@
  * value / scale rounded to nearest even, both as f32 divisions.  A block that
  * holds an infinity or a NaN gets the scale NaN and codes NaN, so every
  * result that it enters is NaN.
+ *
+ * Limits
+ *   A product multiplies a block's two scales in f32 before its sum, so that
+ *   product keeps its bits between 2^-126 and 2^128 (scales per row on both
+ *   sides: the sum times the left one).
+ *   Matrices of more than 65535 x 128 rows are refused by the quantisers by
+ *   columns and by blocks and by the transposed layout, and as a table by a
+ *   product with up to 16 rows.
  */
 #ifndef K3_MOE_FP8_H
 #define K3_MOE_FP8_H
@@ -104,7 +112,8 @@ typedef struct k3_moe_fp8_experts_desc {
  * [tokens, d]), plus shared bf16 [tokens, d] unless NULL, added as
  * k3_moe_combine does.  ids u32, weights f32 [tokens, top_k] on the device, as
  * k3_moe_route writes them.  Rows are quantised once per token and again after
- * the activation, which is not rounded in between.  An id >= experts
+ * the activation, which is not rounded in between; an expert's output rows are
+ * f32 up to their weighted sum, whatever the number of tokens.  An id >= experts
  * contributes nothing and raises bit 1 of k3_moe_device_status(). */
 size_t k3_moe_fp8_experts_workspace_bytes(const k3_moe_fp8_experts_desc *desc, uint32_t tokens);
 bool k3_moe_fp8_experts_forward(const k3_moe_fp8_experts_desc *desc, void *out, const void *x,

@@ -1,6 +1,7 @@
 // Expert load, balance loss and the router's gradient (include/k3_moe_balance.h has the formulas).
 //
-// All three are one pass over logits f32 [tokens, experts], so HBM bounds them.  A warp takes a token's
+// All three are one pass over logits f32 [tokens, experts], so HBM bounds them; 32768 x 896 takes 31 us forward (3.8 TB/s), where
+// the exponentials' chains stand beside the loads, and 50 us backward (4.7 TB/s).  A warp takes a token's
 // row: lane l holds experts 4 l .. 4 l + 3 of every 128 (or l of every 32 where rows are not whole 16-byte
 // units), so the row's sums are shuffles, and in the forward pass the sums over tokens stay in the same
 // registers from token to token.
@@ -27,8 +28,9 @@ constexpr uint32_t kForwardStages = 3, kBackwardStages = 2;   // rows of a warp 
 
 __device__ uint32_t g_balance_status = 0;          // 2: an expert id >= experts
 
-// Blocks of the backward pass on an SM, two in the forward pass.  30000 x 160, us with two / three / four: backward 19.7 / 17.1 /
-// 17.0, forward 11.5 / 10.4 / 10.2, and the second stage, which has a partial row for each block, 8.3 / 9.5 / 10.8.
+// Blocks of the backward pass on an SM, two in the forward pass.  30000 x 160 in one sequence, us with two / three / four:
+// backward 19.6 / 18.0 / 18.1, forward 10.0 / 10.1 / 25.7, and its second stage, which has a partial row for each
+// block, 13.3 / 18.8 / 23.8.  32768 x 896 in 16: forward 31 / 38 / 41, second stage 7.2 / 6.5 / 7.1.
 constexpr uint32_t kForwardPerSm = 2;
 constexpr uint32_t backward_per_sm(uint32_t groups) { return groups <= 4u ? 3u : 2u; }
 
@@ -38,9 +40,9 @@ struct Shape {
     int softmax;
 };
 
-// Scores with the fast base-2 exponential and reciprocal: 6e-7 of a score down to
-// 2^-126, below which it is 0.  The exponent's product with log2 e would be off by 2^-24 of itself, 5e-6 of a score at a
-// logit of -80, so what it rounds away goes into the result as a factor.  With expf, a rounded quotient and single
+// Scores with the fast base-2 exponential and reciprocal: 6e-7 of a score down to 2^-126, below which it is 0.  The
+// exponent's product with log2 e would be off by 2^-24 of itself, 5e-6 of a score at a logit of -80, so what it rounds
+// away goes into the result as a factor (5 us of 78 at 32768 x 896).  With expf, a rounded quotient and single
 // operations the pass over the logits was bound by its instructions, 32768 x 896 forward and backward 198 us.
 constexpr float kLn2 = 0.693147181f;
 // a, but 200 where it is larger (e^-200 is 0, and an infinity would leave no remainder); NaN stays
@@ -316,8 +318,8 @@ balance_tokens_kernel(float *part_sums, uint32_t *part_counts, const float *logi
 }
 
 // Few tokens: one cluster of eight blocks per sequence does both stages, with the blocks' partial rows in shared memory.
-// The second launch takes longer than that while few tokens are each warp's: 257 tokens x 160 experts 5.3 us instead of
-// 8.0, but 1000 tokens x 896 experts in one sequence 17.7 instead of 12.4.
+// The second launch takes longer than that while few tokens are each warp's: 257 tokens x 160 experts 4.6 us instead of
+// 3.7 + 3.8, but 1000 tokens x 896 experts in one sequence 19.2 instead of 3.5 + 8.5.
 constexpr uint32_t kFewTokens = 512, kFewSequences = 64, kCluster = 8;
 
 template <uint32_t kV, bool kVector>
