@@ -166,6 +166,27 @@ bool k3_moe_activation_bf16(void *output, const void *gate, const void *up,
                             uint64_t element_count, int activation, float beta,
                             float linear_beta, void *stream);
 
+/* Its gradient for rows of routed experts, grouped: row r of gate, up and d_out
+ * (bf16 [rows, columns]) belongs to route routes[r] (u32, as
+ * k3_moe_dispatch_build's sorted routes; NULL: route r), whose routing weight is
+ * w = weights[route] (f32 [route_count]; NULL: 1).  With d_out the gradient that
+ * the down matrix sends back for an unweighted row, and act = activation(gate) up:
+ *   d_gate = w d_out d act / d gate       d_up = w d_out d act / d up     (bf16)
+ *   scaled = w act                        (bf16; NULL: not wanted)
+ *   d_weights[route] = sum over columns of d_out act     (f32; NULL: not wanted)
+ * scaled is the row that the down matrix's gradient reads.  Arithmetic is f32.
+ * d_gate may be gate, d_up may be up and scaled may be d_out.  A route >=
+ * route_count has weight 0 and no d_weights; two rows of one route leave either's
+ * d_weights.  With offsets (u32 [groups + 1] on the device, as
+ * k3_moe_dispatch_build leaves them; NULL: all rows) rows in front of offsets[0]
+ * and from offsets[groups] on are neither read nor written. */
+bool k3_moe_activation_backward(void *d_gate, void *d_up, void *scaled, void *d_weights,
+                                const void *d_out, const void *gate, const void *up,
+                                const void *weights, const void *routes, const void *offsets,
+                                uint32_t groups, uint32_t rows, uint32_t columns,
+                                uint32_t route_count, int activation, float beta,
+                                float linear_beta, void *stream);
+
 /* Q8 with a selectable block (multiple of 8 dividing columns) and scale type. */
 bool k3_moe_q8_quantize(void *quantized, void *scales, const void *weights,
                         uint32_t rows, uint32_t columns, uint32_t block,

@@ -195,6 +195,15 @@ SIGNATURES = {
     "k3_moe_balance_workspace_bytes": (sz, [u32, u32, u32]),
     "k3_moe_balance": (C.c_bool, [vp, vp, vp, vp, vp, vp, u32, u32, u32, u32, i32, f32, vp, sz, vp]),
     "k3_moe_router_backward": (C.c_bool, [vp, vp, vp, vp, vp, vp, vp, u32, u32, u32, u32, i32, f32, f32, vp]),
+    # bf16 products grouped by expert and their gradients, the activation's gradient, norm
+    "k3_moe_grouped_workspace_bytes": (sz, [u32, u32]),
+    "k3_moe_grouped_product": (C.c_bool, [vp, vp, vp, vp, u32, u32, u32, u32, i32, i32, vp, sz, vp]),
+    "k3_moe_grouped_by_input": (C.c_bool, [vp, vp, vp, vp, u32, u32, u32, u32, i32, i32, vp, sz, vp]),
+    "k3_moe_grouped_by_weight": (C.c_bool, [vp, vp, vp, vp, u32, u32, u32, u32, i32, i32, vp, sz, vp]),
+    "k3_moe_activation_backward": (C.c_bool, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, u32, u32, u32, u32, i32, f32, f32, vp]),
+    "k3_moe_norm": (C.c_bool, [vp, vp, vp, vp, vp, vp, vp, vp, u32, u32, i32, f32, vp]),
+    "k3_moe_norm_workspace_bytes": (sz, [u32, u32]),
+    "k3_moe_norm_backward": (C.c_bool, [vp, vp, vp, vp, vp, vp, vp, u32, u32, i32, i32, vp, sz, vp]),
     "k3_synth_fill_bytes": (C.c_bool, [vp, u64, u64, u64, u32, u32, vp]),
     "k3_synth_fill_int8": (C.c_bool, [vp, u64, u64, u64, vp]),
     "k3_synth_fill_uniform": (C.c_bool, [vp, u64, u64, u64, f32, f32, i32, vp]),

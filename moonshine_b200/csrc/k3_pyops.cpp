@@ -11,7 +11,9 @@
 
 #include "k3_moe_balance.h"
 #include "k3_moe_fp8.h"
+#include "k3_moe_grouped.h"
 #include "k3_moe_layer.h"
+#include "k3_moe_norm.h"
 #include "k3_moe_ops.h"
 
 #include <tuple>
@@ -218,6 +220,12 @@ PyMethodDef kBound[] = {
     K3_BIND(k3_moe_fp8_experts_forward),
     K3_BIND(k3_moe_balance),
     K3_BIND(k3_moe_router_backward),
+    K3_BIND(k3_moe_grouped_product),
+    K3_BIND(k3_moe_grouped_by_input),
+    K3_BIND(k3_moe_grouped_by_weight),
+    K3_BIND(k3_moe_activation_backward),
+    K3_BIND(k3_moe_norm),
+    K3_BIND(k3_moe_norm_backward),
     {nullptr, nullptr, 0, nullptr},
 };
 

@@ -178,6 +178,20 @@ class Fp8Linear:
         return out
 
 
+    def forward_codes(self, codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+        """The same of rows that are quantised already (``quantize_rows``, ``norm.RmsNorm``): codes [tokens,
+        pitch(columns)], scales [tokens, scale_pitch(columns)]."""
+        tokens, _ = _matrix(codes, "codes", pitch(self.columns), (torch.float8_e4m3fn,))
+        if _matrix(scales, "scales", scale_pitch(self.columns), (torch.float32,))[0] != tokens:
+            raise ValueError("codes and scales: different numbers of tokens")
+        _placed(("codes", codes), ("scales", scales), tables=self._device)
+        out = codes.new_empty((tokens, self.rows), dtype=torch.bfloat16)
+        if tokens:
+            _done(ops.k3_moe_fp8_product(out, codes, scales, self.codes, self.scales, tokens, self.rows, self.columns, ops.FP8_BLOCKS,
+                                         ops.FP8_BF16, 0), "k3_moe_fp8_product")
+        return out
+
+
 class Fp8LinearGradient:
     """The gradients of y = x W^T, W [rows, columns], from the table of W transposed (``transpose_blocks``)."""
 

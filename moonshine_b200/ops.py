@@ -81,3 +81,5 @@ Q8_F32, Q8_F16 = 0, 1
 FP8_BF16, FP8_F32 = 0, 1
 FP8_BLOCKS, FP8_ROWS = 0, 1
 SCORE_SIGMOID, SCORE_SOFTMAX = 0, 1
+GROUPED_BF16, GROUPED_F32 = 0, 1
+NORM_BF16, NORM_F32 = 0, 1
