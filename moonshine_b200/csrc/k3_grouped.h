@@ -133,6 +133,8 @@ bool k3_decode_mx_status_clear();
 bool k3_dispatch_status_clear();
 uint32_t k3_balance_status();      // 2: a balance or router gradient call saw an expert id >= experts
 bool k3_balance_status_clear();
+uint32_t k3_grouped_bf16_status();
+bool k3_grouped_bf16_status_clear();
 uint32_t k3_fp8_wide_status();
 bool k3_fp8_wide_status_clear();
 uint32_t k3_fp8_few_status();

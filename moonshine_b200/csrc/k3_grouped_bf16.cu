@@ -18,14 +18,16 @@ bool run(const Product &p, int out_type, size_t workspace_bytes, void *stream) {
         !aligned(p.workspace, 16u) || workspace_bytes < k3_moe_grouped_workspace_bytes(p.rows, p.groups)) {
         return false;
     }
-    return product_any(p, (cudaStream_t)stream);
+    // what the TMA unit reads: rows of whole 16-byte units
+    const bool tc = p.n % 8u == 0u && p.k % 8u == 0u && aligned(p.out, 16u) && aligned(p.a, 16u) && aligned(p.b, 16u);
+    return tc ? product_tc(p, (cudaStream_t)stream) : product_any(p, (cudaStream_t)stream);
 }
 
 }  // namespace
 
 extern "C" size_t k3_moe_grouped_workspace_bytes(uint32_t rows, uint32_t groups) {
     if (!extent_ok(rows) || groups == 0u || groups > kMaxGroups) return 0;
-    return 16;
+    return tc_workspace_bytes(rows, groups);
 }
 
 extern "C" bool k3_moe_grouped_product(void *out, const void *x, const void *w, const void *offsets, uint32_t rows,

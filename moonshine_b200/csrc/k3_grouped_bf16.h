@@ -1,5 +1,5 @@
-// Internal interface of the bf16 products grouped by expert: entry points and choice (k3_grouped_bf16.cu),
-// the kernel for any sizes (k3_grouped_bf16_any.cu).
+// Internal interface of the bf16 products grouped by expert: entry points and choice (k3_grouped_bf16.cu), the
+// tensor-core kernels (k3_grouped_bf16_tc.cu), the kernel for any sizes (k3_grouped_bf16_any.cu).
 #pragma once
 
 #include "k3_common.cuh"
@@ -29,5 +29,8 @@ K3_DEVINL void group_rows(const uint32_t *offsets, uint32_t g, uint32_t rows, ui
 }
 
 bool product_any(const Product &p, cudaStream_t stream);
+// n and k multiples of 8, all pointers but the offsets on 16 bytes
+bool product_tc(const Product &p, cudaStream_t stream);
+uint64_t tc_workspace_bytes(uint32_t rows, uint32_t groups);
 
 }  // namespace k3::gb

@@ -1,0 +1,556 @@
+// bf16 products grouped by expert, and their gradients, on tcgen05 (kind::f16).
+//
+// D[m, c] = sum_r A(m, r) B(c, r), the tensor cores' 128 lanes along m:
+//   forward    A = w_g   [n, k], m a feature of the output, c a row of the group, r < k
+//   by input   A = w_g^T [k, n], m a feature of the input,  c a row of the group, r < n
+//   by weight  A = dy^T  [n, rows], B = x^T [k, rows],      r a row of the group
+// A group's rows are the N extent of the first two, which takes any multiple of 16: a group of 130 rows costs a tile
+// of 160, where rows as lanes would cost 256.  What lies in memory with its depth in neighbouring rows (w by input,
+// both operands by weight) goes to shared memory as it is and is read "MN-major".
+//
+// An item is kHalves x 128 lanes by up to kMaxN columns over the whole depth, 64 of it per stage.  One block per SM:
+//   warp 0       loads by TMA
+//   warp 1       MMA issuer, owns the tensor memory: an accumulator of kMaxN columns for each of two halves
+//   warp 2       draws items from a counter and tells the others, one ahead
+//   warp 3       by weight: clears what a group's last stage holds of the rows behind the group
+//   warps 4-11   results: lane quadrant warp % 4, every second chunk of 32 columns; the accumulator is free again once
+//                it is in registers, before anything is stored
+// Items that share a matrix are neighbours in the order, so it is in L2 for all but one of them.  Their results do not
+// depend on who draws what.
+//
+// Every wait is bounded; on give-up the block raises the status word, waits for its copies and frees its tensor memory.
+#include "k3_fp8_ptx.cuh"
+#include "k3_grouped.h"
+#include "k3_grouped_bf16.h"
+
+#include <algorithm>
+
+using namespace k3;
+using namespace k3::tc;
+using namespace k3::gb;
+using k3::fp8::bf16x2;
+using k3::fp8::fewer_registers;
+using k3::fp8::more_registers;
+using k3::fp8::mbar_drain;
+using k3::fp8::tensor_map_encoder;
+
+namespace {
+
+constexpr uint32_t kThreads = 384, kResultWarps = 8, kDepth = 64;      // depth of a stage: 128 bytes of bf16
+constexpr uint32_t kBox = 64 * kDepth * 2;                             // 8 KB: 64 x 64 elements
+constexpr uint32_t kSlots = 2;                                         // items that are known ahead
+constexpr uint32_t kNoItem = 0xffffffffu;
+
+__device__ uint32_t g_grouped_bf16_status = 0;
+
+// What the kernel in front leaves in the workspace: the counter, the number of row tiles, and of each row tile its
+// group, rows, and its group's tiles.
+struct Plan {
+    uint32_t counter, tiles, pad[2];
+};
+struct Tile {
+    uint32_t group, row, rows, first, count, pad[3];                   // first .. first + count - 1: the group's tiles
+};
+
+template <uint32_t kHalves_, uint32_t kMaxN_, uint32_t kStages_>
+struct Shape {
+    static constexpr uint32_t kHalves = kHalves_, kMaxN = kMaxN_, kStages = kStages_;
+    static constexpr uint32_t kA = kHalves * 2u * kBox, kStage = kA + kMaxN * kDepth * 2u;
+    static constexpr uint32_t kStore = kStages * kStage;               // 4 KB per result warp
+    static constexpr uint32_t kBars = kStore + kResultWarps * 4096u;
+    static constexpr uint32_t kBytes = kBars + 512u + 1024u;           // the last: alignment
+    static constexpr uint32_t kTmem = 2u * kMaxN;
+    static_assert(kBytes <= 232448u && kTmem <= 512u && (kTmem & (kTmem - 1u)) == 0u, "");
+};
+
+struct TcArgs {
+    void *out;
+    const uint32_t *offsets;
+    Plan *plan;
+    const Tile *tiles;
+    uint32_t rows, groups, n, k;
+    uint32_t lane_tiles;                                               // items side by side along the lanes
+    uint32_t column_tiles;                                             // by weight: and along the columns
+    int accumulate;
+};
+
+struct Item {
+    uint32_t group, row, rows;                                         // by weight: the group's rows, all of them
+    uint32_t lane0, column0;                                           // by weight: column0 of k
+};
+
+// Instruction descriptor, kind::f16, as make_idesc_bf16, with bits 15 and 16 for operands whose depth is not what lies
+// side by side.
+K3_DEVINL constexpr uint32_t idesc_of(uint32_t n, bool a_by_depth, bool b_by_depth) {
+    return make_idesc_bf16(128u, n) | (a_by_depth ? 1u << 15 : 0u) | (b_by_depth ? 1u << 16 : 0u);
+}
+// Shared-memory descriptor of a tile whose rows are its depth: boxes of 64 elements x 64 rows of 128 bytes with the
+// 128-byte swizzle, 8 KB apart (the leading offset); groups of 8 rows are 1024 bytes apart (the stride offset).
+K3_DEVINL uint64_t make_desc_by_depth(uint32_t smem_addr) {
+    return (make_desc_sw128(smem_addr) & ~((uint64_t)0x3fffu << 16)) | ((uint64_t)(kBox >> 4) << 16);
+}
+
+K3_DEVINL void tma_load_3d(void *dst, const void *map, uint64_t *bar, int32_t x, int32_t y, int32_t z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
+// ------------------------------------------------------------------------------------------- the plan
+// One thread per group.  A group's rows in as few tiles of up to max_n as there can be, equally large.
+__global__ void __launch_bounds__(kMaxGroups) grouped_plan_kernel(Plan *plan, Tile *tiles, const uint32_t *offsets, uint32_t rows,
+                                                                  uint32_t groups, uint32_t max_n, uint32_t capacity) {
+    pdl_trigger();
+    pdl_wait();
+    __shared__ uint32_t sums[kMaxGroups / kWarp];
+    const uint32_t g = threadIdx.x, lane = g % kWarp, warp = g / kWarp;
+    uint32_t begin = 0u, end = 0u;
+    if (g < groups) group_rows(offsets, g, rows, begin, end);
+    const uint32_t count = (end - begin + max_n - 1u) / max_n;
+    uint32_t scan = count;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, scan, o);
+        if (lane >= (uint32_t)o) scan += up;
+    }
+    if (lane == 31u) sums[warp] = scan;
+    __syncthreads();
+    uint32_t first = scan - count;
+    for (uint32_t w = 0; w < warp; w++) first += sums[w];
+    if (count != 0u) {
+        const uint32_t size = ((end - begin + count - 1u) / count + 31u) & ~31u;
+        for (uint32_t i = 0; i < count && first + i < capacity; i++) {
+            Tile t{g, begin + i * size, min(size, end - begin - i * size), first, min(count, capacity - first), {}};
+            tiles[first + i] = t;
+        }
+    }
+    if (g == kMaxGroups - 1u) {
+        plan->counter = 0u;
+        plan->tiles = min(first + count, capacity);
+    }
+}
+
+// by weight: no row tiles
+__global__ void grouped_counter_kernel(Plan *plan) {
+    pdl_trigger();
+    pdl_wait();
+    plan->counter = 0u;
+}
+
+// ---------------------------------------------------------------------------------------- the product
+template <int kForm, bool kF32, typename S>
+__global__ void __launch_bounds__(kThreads, 1)
+grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, TcArgs a) {
+    constexpr bool kRows = kForm != kByWeight;                         // the columns are rows of the group
+    constexpr bool kADepth = kForm != kForward, kBDepth = kForm == kByWeight;
+    constexpr uint32_t kLanes = 128u * S::kHalves;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char *base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint64_t *full = reinterpret_cast<uint64_t *>(base + S::kBars);    // [kStages]
+    uint64_t *empty = full + S::kStages;                               // [kStages]
+    uint64_t *acc_full = empty + S::kStages;                           // [2]
+    uint64_t *acc_empty = acc_full + 2;                                // [2]
+    uint64_t *item_full = acc_empty + 2;                               // [kSlots]
+    uint64_t *item_empty = item_full + kSlots;                         // [kSlots]
+    uint64_t *loaded = item_empty + kSlots;                            // [1] a last stage to be cleared is there
+    uint64_t *cleared = loaded + 1;                                    // [1] and its rows behind the group are zeros
+    uint64_t *done = cleared + 1;                                      // [1] every MMA issued has run
+    Item *items = reinterpret_cast<Item *>(done + 1);                  // [kSlots]
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(items + kSlots);
+    volatile uint32_t *abort_flag = tmem_slot + 1;
+    const uint32_t warp = warp_index(), lane = threadIdx.x % kWarp;
+    // the extent along the lanes, the depth, and the output's row length
+    const uint32_t lanes = kForm == kByInput ? a.k : a.n;
+
+    if (warp == 0u && elect_one()) {
+        *abort_flag = 0u;
+        for (uint32_t s = 0; s < S::kStages; s++) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (uint32_t s = 0; s < 2u; s++) {
+            mbar_init(&acc_full[s], 1);
+            mbar_init(&acc_empty[s], kResultWarps);
+        }
+        for (uint32_t s = 0; s < kSlots; s++) {
+            mbar_init(&item_full[s], 1);
+            mbar_init(&item_empty[s], 2u + kResultWarps + (kRows ? 0u : 1u));
+        }
+        mbar_init(loaded, 1);
+        mbar_init(cleared, 1);
+        mbar_init(done, 1);
+        fence_barrier_init();
+        prefetch_tensormap(&map_a);
+        prefetch_tensormap(&map_b);
+    }
+    if (warp == 1u) {
+        tmem_alloc(tmem_slot, S::kTmem);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_wait();
+
+    // Items one after the other, as every role reads them.
+    uint32_t slot = 0u, slot_phase = 0u;
+    auto next_item = [&](Item &it) {
+        if (!mbar_wait(&item_full[slot], slot_phase, abort_flag)) return false;
+        it = items[slot];
+        return it.group != kNoItem;
+    };
+    auto item_read = [&]() {                                           // by one thread
+        mbar_arrive(&item_empty[slot]);
+    };
+    auto item_done = [&]() {
+        if (++slot == kSlots) { slot = 0u; slot_phase ^= 1u; }
+    };
+    auto depth_of = [&](const Item &it) { return kForm == kForward ? a.k : kForm == kByInput ? a.n : it.rows; };
+    auto halves_of = [&](const Item &it) { return min(S::kHalves, (lanes - it.lane0 + 127u) / 128u); };
+    auto columns_of = [&](const Item &it) { return kRows ? it.rows : min(S::kMaxN, a.k - it.column0); };
+
+    // an accumulator half in registers is 128 of them: 2 x 128 x 232 + 128 x 40 are the 384 x 168 of the launch
+    constexpr bool kShares = S::kMaxN == 256u;
+    if (kShares && warp < 4u) fewer_registers<40>();
+    if (warp == 0u) {
+        // ----------------------------------------------------------------------------- loads
+        if (elect_one()) {
+            uint32_t s = 0u, ph = 0u, issued = 0u;
+            bool ok = true;
+            Item it;
+            while (ok && next_item(it)) {
+                item_read();
+                item_done();
+                const uint32_t blocks = (depth_of(it) + kDepth - 1u) / kDepth, halves = halves_of(it), columns = columns_of(it);
+                const uint32_t b_boxes = kRows ? (columns + 31u) / 32u : (columns + 63u) / 64u;
+                const uint32_t bytes = halves * 2u * kBox + b_boxes * (kRows ? kBox / 2u : kBox);
+                for (uint32_t kb = 0; kb < blocks; kb++) {
+                    if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag)) { ok = false; break; }
+                    unsigned char *at = base + s * S::kStage, *bt = at + S::kA;
+                    const int32_t d = (int32_t)(kb * kDepth), r = (int32_t)it.row;
+                    mbar_arrive_expect_tx(&full[s], bytes);
+                    for (uint32_t h = 0; h < halves; h++) {
+                        const int32_t l = (int32_t)(it.lane0 + 128u * h);
+                        unsigned char *to = at + h * 2u * kBox;
+                        if (kForm == kForward) {
+                            tma_load_3d(to, &map_a, &full[s], d, l, (int32_t)it.group);
+                        } else if (kForm == kByInput) {
+                            tma_load_3d(to, &map_a, &full[s], l, d, (int32_t)it.group);
+                            tma_load_3d(to + kBox, &map_a, &full[s], l + 64, d, (int32_t)it.group);
+                        } else {
+                            tma_load_2d(to, &map_a, &full[s], l, r + d);
+                            tma_load_2d(to + kBox, &map_a, &full[s], l + 64, r + d);
+                        }
+                    }
+                    for (uint32_t b = 0; b < b_boxes; b++) {
+                        if (kRows) tma_load_2d(bt + b * (kBox / 2u), &map_b, &full[s], d, r + (int32_t)(32u * b));
+                        else tma_load_2d(bt + b * kBox, &map_b, &full[s], (int32_t)(it.column0 + 64u * b), r + d);
+                    }
+                    issued++;
+                    if (++s == S::kStages) { s = 0u; ph ^= 1u; }
+                }
+            }
+            pdl_trigger();                                             // the blocks of the next kernel may take places as these leave
+            if (*abort_flag != 0u) {                                   // nothing may land in a block that has left
+                for (uint32_t i = issued > S::kStages ? issued - S::kStages : 0u; i < issued; i++) {
+                    mbar_drain(&full[i % S::kStages], (i / S::kStages) & 1u);
+                }
+            }
+        }
+    } else if (warp == 1u) {
+        // ------------------------------------------------------------------------------- MMA
+        if (elect_one()) {
+            uint32_t s = 0u, ph = 0u, clear_phase = 0u, turn = 0u, acc_phase[2] = {1u, 1u};
+            bool ok = true;
+            Item it;
+            while (ok && next_item(it)) {
+                item_read();
+                item_done();
+                const uint32_t depth = depth_of(it), blocks = (depth + kDepth - 1u) / kDepth, halves = halves_of(it);
+                const uint32_t columns = columns_of(it);
+                const uint32_t idesc = idesc_of(kRows ? (columns + 31u) & ~31u : (columns + 15u) & ~15u, kADepth, kBDepth);
+                for (uint32_t kb = 0; ok && kb < blocks; kb++) {
+                    const bool last = kb + 1u == blocks;
+                    if (!mbar_wait(&full[s], ph, abort_flag)) { ok = false; break; }
+                    // by weight: only the steps of 16 that have rows, the last of them with zeros behind the group
+                    const uint32_t steps = kRows || !last ? 4u : (depth - kb * kDepth + 15u) / 16u;
+                    const bool clear = !kRows && last && depth % 16u != 0u;
+                    if (clear) mbar_arrive(loaded);
+                    const uint32_t at = smem_u32(base + s * S::kStage);
+                    const uint64_t db = kBDepth ? make_desc_by_depth(at + S::kA) : make_desc_sw128(at + S::kA);
+                    for (uint32_t h = 0; h < halves; h++) {
+                        const uint32_t acc = S::kHalves == 2u ? h : turn;
+                        if (kb == 0u) {
+                            if (!mbar_wait(&acc_empty[acc], acc_phase[acc], abort_flag)) { ok = false; break; }
+                            acc_phase[acc] ^= 1u;
+                        }
+                        if (clear && h == 0u) {
+                            if (!mbar_wait(cleared, clear_phase, abort_flag)) { ok = false; break; }
+                            clear_phase ^= 1u;
+                        }
+                        tc_fence_after();
+                        const uint32_t ah = at + h * 2u * kBox, d = tmem + acc * S::kMaxN;
+                        const uint64_t da = kADepth ? make_desc_by_depth(ah) : make_desc_sw128(ah);
+#pragma unroll
+                        for (uint32_t j = 0; j < 4u; j++) {            // 16 of the depth: 32 bytes on, or 16 rows of 128
+                            if (j < steps) {
+                                mma_f16_ss(d, da + (kADepth ? 128u : 2u) * j, db + (kBDepth ? 128u : 2u) * j, idesc, kb != 0u || j != 0u);
+                            }
+                        }
+                        if (last) mma_commit(&acc_full[acc]);
+                    }
+                    if (!ok) break;
+                    mma_commit(&empty[s]);
+                    if (++s == S::kStages) { s = 0u; ph ^= 1u; }
+                }
+                if (S::kHalves == 1u && blocks != 0u) turn ^= 1u;
+            }
+            if (*abort_flag != 0u) {
+                mma_commit(done);
+                mbar_drain(done, 0u);
+            }
+        }
+    } else if (warp == 2u) {
+        // ---------------------------------------------------------------------- items, one ahead
+        if (elect_one()) {
+            const uint32_t total = kRows ? a.plan->tiles * a.lane_tiles : a.groups * a.lane_tiles * a.column_tiles;
+            uint32_t w = blockIdx.x;
+            for (;;) {
+                Item it{kNoItem, 0u, 0u, 0u, 0u};
+                if (w < total) {
+                    if (kRows) {
+                        const Tile of = a.tiles[w / a.lane_tiles];
+                        const uint32_t local = w - of.first * a.lane_tiles, t = local % of.count;
+                        const Tile tile = t + of.first == w / a.lane_tiles ? of : a.tiles[of.first + t];
+                        it = {tile.group, tile.row, tile.rows, local / of.count * kLanes, 0u};
+                    } else {
+                        const uint32_t per = a.lane_tiles * a.column_tiles, g = w / per, at = w - g * per;
+                        uint32_t begin, end;
+                        group_rows(a.offsets, g, a.rows, begin, end);
+                        it = {g, begin, end - begin, at / a.column_tiles * kLanes, at % a.column_tiles * S::kMaxN};
+                    }
+                }
+                if (!mbar_wait(&item_empty[slot], slot_phase ^ 1u, abort_flag)) break;
+                items[slot] = it;
+                mbar_arrive(&item_full[slot]);
+                item_done();
+                if (it.group == kNoItem) break;
+                w = gridDim.x + atomicAdd(&a.plan->counter, 1u);
+            }
+        }
+    } else if (warp == 3u) {
+        if (!kRows) {
+            // ---------------------------------------------------- rows behind the group in its last stage
+            uint32_t used = 0u, load_phase = 0u;                       // stages so far
+            Item it;
+            while (next_item(it)) {
+                __syncwarp();
+                if (lane == 0u) item_read();
+                item_done();
+                const uint32_t blocks = (it.rows + kDepth - 1u) / kDepth;
+                used += blocks;
+                if (it.rows % 16u == 0u) continue;
+                if (!mbar_wait(loaded, load_phase, abort_flag)) break;
+                load_phase ^= 1u;
+                unsigned char *at = base + (used - 1u) % S::kStages * S::kStage;
+                const uint32_t a_boxes = halves_of(it) * 2u, boxes = a_boxes + (columns_of(it) + 63u) / 64u;
+                const uint32_t from = it.rows % kDepth, rows = (16u - from % 16u) % 16u;
+                for (uint32_t e = lane; e < boxes * rows * 8u; e += kWarp) {
+                    const uint32_t box = e / (rows * 8u), in = e - box * rows * 8u;
+                    unsigned char *to = box < a_boxes ? at + box * kBox : at + S::kA + (box - a_boxes) * kBox;
+                    *reinterpret_cast<uint4 *>(to + from * 128u + in * 16u) = make_uint4(0u, 0u, 0u, 0u);
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0u) mbar_arrive(cleared);
+            }
+        }
+    } else {
+        // --------------------------------------------------------------------------- results
+        if (kShares) more_registers<232>();
+        const uint32_t q = warp % 4u, part = (warp - 4u) / 4u;
+        unsigned char *mine = base + S::kStore + (warp - 4u) * 4096u;
+        const uint32_t row_length = kRows ? lanes : a.k;
+        uint32_t acc_phase[2] = {0u, 0u}, turn = 0u;
+        bool ok = true;
+        Item it;
+        while (ok && next_item(it)) {
+            __syncwarp();
+            if (lane == 0u) item_read();
+            item_done();
+            const uint32_t halves = halves_of(it), columns = columns_of(it);
+            const bool nothing = depth_of(it) == 0u;                   // by weight: a group without rows
+            if (nothing && a.accumulate) continue;
+            for (uint32_t h = 0; h < halves; h++) {
+                const uint32_t acc = S::kHalves == 2u ? h : turn;
+                constexpr uint32_t kChunks = S::kMaxN / 64u;           // of 32 columns, for this warp
+                uint32_t v[kChunks][32];
+                if (!nothing) {
+                    if (!mbar_wait(&acc_full[acc], acc_phase[acc], abort_flag)) { ok = false; break; }
+                    acc_phase[acc] ^= 1u;
+                    tc_fence_after();
+#pragma unroll
+                    for (uint32_t c = 0; c < kChunks; c++) {           // those past the columns too: they are in the accumulator
+                        tmem_ld_32x32(tmem + acc * S::kMaxN + (2u * c + part) * 32u + ((32u * q) << 16), v[c]);
+                    }
+#pragma unroll
+                    for (uint32_t c = 0; c < kChunks; c++) k3::fp8::tmem_ld_wait_for(v[c]);
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0u) mbar_arrive(&acc_empty[acc]);
+                } else {
+#pragma unroll
+                    for (uint32_t c = 0; c < kChunks; c++) {
+#pragma unroll
+                        for (uint32_t i = 0; i < 32u; i++) v[c][i] = 0u;
+                    }
+                }
+                const uint32_t lane0 = it.lane0 + 128u * h + 32u * q;  // this warp's first lane
+#pragma unroll
+                for (uint32_t c = 0; c < kChunks; c++) {
+                    const uint32_t column = (2u * c + part) * 32u;
+                    if (column >= columns) break;
+                    // 32 x 32 through shared memory: rows of the output, units of 16 bytes, permuted by the row
+                    constexpr uint32_t kUnits = kF32 ? 8u : 4u;
+                    auto unit = [&](uint32_t row, uint32_t u) {
+                        return mine + row * (kUnits * 16u) + ((u ^ (kF32 ? row & 7u : (row >> 1) & 3u)) * 16u);
+                    };
+                    if (kRows) {                                       // this thread's 32 results go down a column
+#pragma unroll
+                        for (uint32_t i = 0; i < 32u; i++) {
+                            if (kF32) *reinterpret_cast<uint32_t *>(unit(i, lane / 4u) + (lane % 4u) * 4u) = v[c][i];
+                            else *reinterpret_cast<uint16_t *>(unit(i, lane / 8u) + (lane % 8u) * 2u) = float_to_bf16_bits(__uint_as_float(v[c][i]));
+                        }
+                    } else {
+#pragma unroll
+                        for (uint32_t u = 0; u < kUnits; u++) {
+                            uint4 x;
+                            if (kF32) {
+                                x = make_uint4(v[c][4u * u % 32u], v[c][(4u * u + 1u) % 32u], v[c][(4u * u + 2u) % 32u], v[c][(4u * u + 3u) % 32u]);
+                            } else {
+                                uint32_t word[4];
+#pragma unroll
+                                for (uint32_t j = 0; j < 4u; j++) {
+                                    word[j] = bf16x2(__uint_as_float(v[c][(8u * u + 2u * j) % 32u]), __uint_as_float(v[c][(8u * u + 2u * j + 1u) % 32u]));
+                                }
+                                x = make_uint4(word[0], word[1], word[2], word[3]);
+                            }
+                            *reinterpret_cast<uint4 *>(unit(lane, u)) = x;
+                        }
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (uint32_t i = 0; i < kUnits; i++) {
+                        const uint32_t r = i * (32u / kUnits) + lane / kUnits, u = lane % kUnits, e = u * (kF32 ? 4u : 8u);
+                        const uint4 x = *reinterpret_cast<const uint4 *>(unit(r, u));
+                        uint64_t to;
+                        if (kRows) {
+                            if (column + r >= it.rows || lane0 + e >= lanes) continue;
+                            to = (uint64_t)(it.row + column + r) * row_length + lane0 + e;
+                        } else {
+                            if (lane0 + r >= a.n || it.column0 + column + e >= a.k) continue;
+                            to = ((uint64_t)it.group * a.n + lane0 + r) * row_length + it.column0 + column + e;
+                        }
+                        if (kF32) {
+                            float4 *out = reinterpret_cast<float4 *>((float *)a.out + to);
+                            float4 f = make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w));
+                            if (a.accumulate) {
+                                const float4 o = *out;
+                                f = make_float4(o.x + f.x, o.y + f.y, o.z + f.z, o.w + f.w);
+                            }
+                            *out = f;
+                        } else {
+                            *reinterpret_cast<uint4 *>((uint16_t *)a.out + to) = x;
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+            if (S::kHalves == 1u && !nothing) turn ^= 1u;
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0 && *abort_flag != 0u) atomicExch(&g_grouped_bf16_status, 1u);
+    if (warp == 1u) {
+        tc_fence_after();
+        tmem_dealloc(tmem, S::kTmem);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+// bf16 [z, y, x] with boxes of 64 x box_y, 128-byte swizzle; what lies outside reads as zero.
+bool make_map(CUtensorMap *map, const void *p, uint32_t x, uint64_t y, uint32_t z, uint32_t box_y) {
+    auto fn = tensor_map_encoder();
+    if (!fn) return false;
+    const cuuint64_t dims[3] = {x, y, z};
+    const cuuint64_t strides[2] = {(cuuint64_t)x * 2u, (cuuint64_t)x * y * 2u};
+    const cuuint32_t box[3] = {64u, box_y, 1u}, steps[3] = {1u, 1u, 1u};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, z != 0u ? 3 : 2, const_cast<void *>(p), dims, strides, box, steps,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+constexpr uint64_t plan_bytes(uint32_t tiles) { return sizeof(Plan) + (uint64_t)tiles * sizeof(Tile); }
+// The most row tiles of up to max_n that the groups can have.
+uint32_t most_tiles(uint32_t rows, uint32_t groups, uint32_t max_n) { return rows / max_n + std::min(rows, groups); }
+
+constexpr uint32_t kFewRows = 64;
+using Wide = Shape<2, 256, 3>;
+using Few = Shape<1, kFewRows, 8>;
+
+template <int kForm, bool kF32, typename S>
+bool launch(const Product &p, cudaStream_t stream) {
+    constexpr bool kRows = kForm != kByWeight;
+    auto kernel = grouped_bf16_kernel<kForm, kF32, S>;
+    CUtensorMap ma, mb;
+    if (kForm == kForward) {
+        if (!make_map(&ma, p.b, p.k, p.n, p.groups, 128u) || !make_map(&mb, p.a, p.k, p.rows, 0u, 32u)) return false;
+    } else if (kForm == kByInput) {
+        if (!make_map(&ma, p.b, p.k, p.n, p.groups, 64u) || !make_map(&mb, p.a, p.n, p.rows, 0u, 32u)) return false;
+    } else {
+        if (!make_map(&ma, p.a, p.n, p.rows, 0u, 64u) || !make_map(&mb, p.b, p.k, p.rows, 0u, 64u)) return false;
+    }
+    const uint32_t lanes = kForm == kByInput ? p.k : p.n, tiles = most_tiles(p.rows, p.groups, S::kMaxN);
+    TcArgs a{p.out, p.offsets, (Plan *)p.workspace, (const Tile *)((Plan *)p.workspace + 1), p.rows, p.groups, p.n, p.k,
+             (lanes + 128u * S::kHalves - 1u) / (128u * S::kHalves), (p.k + S::kMaxN - 1u) / S::kMaxN, p.accumulate};
+    const uint64_t items = kRows ? (uint64_t)tiles * a.lane_tiles : (uint64_t)p.groups * a.lane_tiles * a.column_tiles;
+    if (items > 0x7fffffffull || !set_max_dynamic_smem((const void *)kernel, S::kBytes)) return false;
+    const bool planned = kRows ? launch_chained(grouped_plan_kernel, 1, kMaxGroups, 0, stream, a.plan, (Tile *)a.tiles, p.offsets, p.rows, p.groups,
+                                                S::kMaxN, tiles)
+                               : launch_chained(grouped_counter_kernel, 1, 1, 0, stream, a.plan);
+    return planned && launch_chained(kernel, (uint32_t)std::min<uint64_t>(items, sm_count()), kThreads, S::kBytes, stream, ma, mb, a);
+}
+
+template <int kForm, typename S>
+bool launch_typed(const Product &p, cudaStream_t stream) {
+    return p.f32 ? launch<kForm, true, S>(p, stream) : launch<kForm, false, S>(p, stream);
+}
+
+}  // namespace
+
+uint64_t k3::gb::tc_workspace_bytes(uint32_t rows, uint32_t groups) { return plan_bytes(most_tiles(rows, groups, kFewRows)); }
+
+bool k3::gb::product_tc(const Product &p, cudaStream_t stream) {
+    if (p.form == kByWeight) return launch_typed<kByWeight, Wide>(p, stream);
+    const bool few = p.rows <= 24u * std::min(p.rows, p.groups);
+    if (p.form == kForward) return few ? launch_typed<kForward, Few>(p, stream) : launch_typed<kForward, Wide>(p, stream);
+    return few ? launch_typed<kByInput, Few>(p, stream) : launch_typed<kByInput, Wide>(p, stream);
+}
+
+uint32_t k3_grouped_bf16_status() {
+    uint32_t v = 0xffffffffu;
+    if (cudaMemcpyFromSymbol(&v, g_grouped_bf16_status, sizeof(v)) != cudaSuccess) (void)cudaGetLastError();
+    return v;
+}
+
+bool k3_grouped_bf16_status_clear() {
+    const uint32_t zero = 0u;
+    const bool ok = cudaMemcpyToSymbol(g_grouped_bf16_status, &zero, sizeof(zero)) == cudaSuccess;
+    if (!ok) (void)cudaGetLastError();
+    return ok;
+}
