@@ -30,7 +30,7 @@ extern "C" {
  * itself) [rows, hidden] of `type`, weight bf16 [hidden]; y bf16 [rows, hidden]
  * or NULL; codes [rows, hidden rounded up to 16], 16-byte aligned, with scales
  * f32 [rows, ceil(hidden / 128) rounded up to 4], or both NULL; rstd f32 [rows]
- * or NULL.  One of y and codes at least.  hidden <= 65536, epsilon > 0. */
+ * or NULL.  One of y and codes at least.  hidden <= 16384, epsilon > 0. */
 bool k3_moe_norm(void *sum, void *y, void *codes, void *scales, void *rstd, const void *x,
                  const void *residual, const void *weight, uint32_t rows, uint32_t hidden, int type,
                  float epsilon, void *stream);

@@ -68,7 +68,9 @@ __global__ void __launch_bounds__(kThreads) activation_grad_kernel(ActivationGra
         routed = route < a.route_count;
         const float weight = !routed ? 0.0f : a.weights ? a.weights[route] : 1.0f;
         const uint64_t base = row * a.columns;
-        for (uint32_t c = t * 8u; c < a.columns; c += kTeam * 8u) {
+        // a thread's eight columns are neighbours, or (rows that are not whole vectors) kTeam apart
+        constexpr uint32_t kStep = kVector ? 1u : kTeam;
+        for (uint32_t c = kVector ? t * 8u : t; c < a.columns; c += kTeam * 8u) {
             uint32_t g[4] = {}, u[4] = {}, d[4] = {};
             if (kVector) {
                 const uint4 vg = *reinterpret_cast<const uint4 *>(a.gate + base + c), vu = *reinterpret_cast<const uint4 *>(a.up + base + c);
@@ -79,10 +81,11 @@ __global__ void __launch_bounds__(kThreads) activation_grad_kernel(ActivationGra
             } else {
 #pragma unroll
                 for (uint32_t i = 0; i < 8u; i++) {
-                    if (c + i >= a.columns) continue;
-                    g[i / 2u] |= (uint32_t)a.gate[base + c + i] << (16u * (i & 1u));
-                    u[i / 2u] |= (uint32_t)a.up[base + c + i] << (16u * (i & 1u));
-                    d[i / 2u] |= (uint32_t)a.d_out[base + c + i] << (16u * (i & 1u));
+                    if (c + i * kStep >= a.columns) continue;
+                    const uint64_t at = base + c + i * kStep;
+                    g[i / 2u] |= (uint32_t)a.gate[at] << (16u * (i & 1u));
+                    u[i / 2u] |= (uint32_t)a.up[at] << (16u * (i & 1u));
+                    d[i / 2u] |= (uint32_t)a.d_out[at] << (16u * (i & 1u));
                 }
             }
             uint32_t dg[4], du[4], sc[4];
@@ -104,10 +107,11 @@ __global__ void __launch_bounds__(kThreads) activation_grad_kernel(ActivationGra
             } else {
 #pragma unroll
                 for (uint32_t i = 0; i < 8u; i++) {
-                    if (c + i >= a.columns) continue;
-                    a.d_gate[base + c + i] = (uint16_t)(dg[i / 2u] >> (16u * (i & 1u)));
-                    a.d_up[base + c + i] = (uint16_t)(du[i / 2u] >> (16u * (i & 1u)));
-                    if (a.scaled) a.scaled[base + c + i] = (uint16_t)(sc[i / 2u] >> (16u * (i & 1u)));
+                    if (c + i * kStep >= a.columns) continue;
+                    const uint64_t at = base + c + i * kStep;
+                    a.d_gate[at] = (uint16_t)(dg[i / 2u] >> (16u * (i & 1u)));
+                    a.d_up[at] = (uint16_t)(du[i / 2u] >> (16u * (i & 1u)));
+                    if (a.scaled) a.scaled[at] = (uint16_t)(sc[i / 2u] >> (16u * (i & 1u)));
                 }
             }
         }

@@ -135,6 +135,8 @@ uint32_t k3_balance_status();      // 2: a balance or router gradient call saw a
 bool k3_balance_status_clear();
 uint32_t k3_grouped_bf16_status();
 bool k3_grouped_bf16_status_clear();
+uint32_t k3_norm_status();
+bool k3_norm_status_clear();
 uint32_t k3_fp8_wide_status();
 bool k3_fp8_wide_status_clear();
 uint32_t k3_fp8_few_status();

@@ -11,7 +11,7 @@
 // An item is kHalves x 128 lanes by up to kMaxN columns over the whole depth, 64 of it per stage.  One block per SM:
 //   warp 0       loads by TMA
 //   warp 1       MMA issuer, owns the tensor memory: an accumulator of kMaxN columns for each of two halves
-//   warp 2       draws items from a counter and tells the others, one ahead
+//   warp 2       draws items from a counter and tells the others, when the loads of the one before come to an end
 //   warp 3       by weight: clears what a group's last stage holds of the rows behind the group
 //   warps 4-11   results: lane quadrant warp % 4, every second chunk of 32 columns; the accumulator is free again once
 //                it is in registers, before anything is stored
@@ -39,6 +39,7 @@ namespace {
 constexpr uint32_t kThreads = 384, kResultWarps = 8, kDepth = 64;      // depth of a stage: 128 bytes of bf16
 constexpr uint32_t kBox = 64 * kDepth * 2;                             // 8 KB: 64 x 64 elements
 constexpr uint32_t kSlots = 2;                                         // items that are known ahead
+constexpr uint32_t kAhead = 6;                                         // stages before an item's last in which the next is drawn
 constexpr uint32_t kNoItem = 0xffffffffu;
 
 __device__ uint32_t g_grouped_bf16_status = 0;
@@ -120,7 +121,7 @@ __global__ void __launch_bounds__(kMaxGroups) grouped_plan_kernel(Plan *plan, Ti
     uint32_t first = scan - count;
     for (uint32_t w = 0; w < warp; w++) first += sums[w];
     if (count != 0u) {
-        const uint32_t size = ((end - begin + count - 1u) / count + 31u) & ~31u;
+        const uint32_t size = ((end - begin + count - 1u) / count + 15u) & ~15u;
         for (uint32_t i = 0; i < count && first + i < capacity; i++) {
             Tile t{g, begin + i * size, min(size, end - begin - i * size), first, min(count, capacity - first), {}};
             tiles[first + i] = t;
@@ -154,7 +155,8 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     uint64_t *acc_empty = acc_full + 2;                                // [2]
     uint64_t *item_full = acc_empty + 2;                               // [kSlots]
     uint64_t *item_empty = item_full + kSlots;                         // [kSlots]
-    uint64_t *loaded = item_empty + kSlots;                            // [1] a last stage to be cleared is there
+    uint64_t *wanted = item_empty + kSlots;                            // [1] the loads come to an end
+    uint64_t *loaded = wanted + 1;                                     // [1] a last stage to be cleared is there
     uint64_t *cleared = loaded + 1;                                    // [1] and its rows behind the group are zeros
     uint64_t *done = cleared + 1;                                      // [1] every MMA issued has run
     Item *items = reinterpret_cast<Item *>(done + 1);                  // [kSlots]
@@ -178,6 +180,7 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             mbar_init(&item_full[s], 1);
             mbar_init(&item_empty[s], 2u + kResultWarps + (kRows ? 0u : 1u));
         }
+        mbar_init(wanted, 1);
         mbar_init(loaded, 1);
         mbar_init(cleared, 1);
         mbar_init(done, 1);
@@ -227,7 +230,9 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 const uint32_t blocks = (depth_of(it) + kDepth - 1u) / kDepth, halves = halves_of(it), columns = columns_of(it);
                 const uint32_t b_boxes = kRows ? (columns + 31u) / 32u : (columns + 63u) / 64u;
                 const uint32_t bytes = halves * 2u * kBox + b_boxes * (kRows ? kBox / 2u : kBox);
+                if (blocks <= kAhead) mbar_arrive(wanted);
                 for (uint32_t kb = 0; kb < blocks; kb++) {
+                    if (kb + kAhead == blocks - 1u) mbar_arrive(wanted);
                     if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag)) { ok = false; break; }
                     unsigned char *at = base + s * S::kStage, *bt = at + S::kA;
                     const int32_t d = (int32_t)(kb * kDepth), r = (int32_t)it.row;
@@ -271,7 +276,7 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 item_done();
                 const uint32_t depth = depth_of(it), blocks = (depth + kDepth - 1u) / kDepth, halves = halves_of(it);
                 const uint32_t columns = columns_of(it);
-                const uint32_t idesc = idesc_of(kRows ? (columns + 31u) & ~31u : (columns + 15u) & ~15u, kADepth, kBDepth);
+                const uint32_t idesc = idesc_of((columns + 15u) & ~15u, kADepth, kBDepth);
                 for (uint32_t kb = 0; ok && kb < blocks; kb++) {
                     const bool last = kb + 1u == blocks;
                     if (!mbar_wait(&full[s], ph, abort_flag)) { ok = false; break; }
@@ -314,10 +319,10 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             }
         }
     } else if (warp == 2u) {
-        // ---------------------------------------------------------------------- items, one ahead
+        // ------------------------------------------------- items, each shortly before its loads
         if (elect_one()) {
             const uint32_t total = kRows ? a.plan->tiles * a.lane_tiles : a.groups * a.lane_tiles * a.column_tiles;
-            uint32_t w = blockIdx.x;
+            uint32_t w = blockIdx.x, want_phase = 0u;
             for (;;) {
                 Item it{kNoItem, 0u, 0u, 0u, 0u};
                 if (w < total) {
@@ -337,7 +342,8 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 items[slot] = it;
                 mbar_arrive(&item_full[slot]);
                 item_done();
-                if (it.group == kNoItem) break;
+                if (it.group == kNoItem || !mbar_wait(wanted, want_phase, abort_flag)) break;
+                want_phase ^= 1u;
                 w = gridDim.x + atomicAdd(&a.plan->counter, 1u);
             }
         }

@@ -602,7 +602,7 @@ extern "C" uint32_t k3_moe_device_status(void) {
     if (cudaMemcpyFromSymbol(&v, g_tc_status, sizeof(v)) != cudaSuccess) (void)cudaGetLastError();
     return v | k3_decode_mx_status() | k3_decode_status() | k3_decode_shared_status() | k3_grouped_mx_status() |
            k3_grouped_mx4_status() | k3_dispatch_status() | k3_balance_status() | k3_fp8_wide_status() |
-           k3_fp8_few_status() | k3_grouped_bf16_status();
+           k3_fp8_few_status() | k3_grouped_bf16_status() | k3_norm_status();
 }
 
 bool k3_status_words_clear() {
@@ -617,6 +617,7 @@ bool k3_status_words_clear() {
     ok = k3_fp8_wide_status_clear() && ok;
     ok = k3_fp8_few_status_clear() && ok;
     ok = k3_grouped_bf16_status_clear() && ok;
+    ok = k3_norm_status_clear() && ok;
     ok = k3_grouped_mx_status_clear() && ok;
     ok = k3_grouped_mx4_status_clear() && ok;
     return ok;

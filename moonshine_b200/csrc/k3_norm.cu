@@ -8,6 +8,7 @@
 // so the 16 lanes of half a warp hold a block of 128, whose largest magnitude is four shuffles away.
 #include "k3_common.cuh"
 #include "k3_fp8_ptx.cuh"
+#include "k3_grouped.h"
 #include "k3_moe_norm.h"
 
 #include <algorithm>
@@ -17,15 +18,23 @@ using namespace k3::fp8;
 
 namespace {
 
-constexpr uint32_t kMaxHidden = 65536;
+constexpr uint32_t kMaxHidden = 16384;
 
-// Eight neighbouring elements as they lie in memory.
+// Eight elements of a row as they lie in memory.  kVector: neighbours, c .. c + 7, of rows that start on 16 bytes and are
+// whole vectors.  Otherwise c, c + 16, .. c + 112: the half warp still holds a block of 128, and its 16 lanes read
+// neighbours (rows of 3583 f32: the gradient 30.8 us of 1021 rows with eight neighbours per thread, now %%).
+template <bool kVector>
+K3_DEVINL constexpr uint32_t column_of(uint32_t c, uint32_t i) { return kVector ? c + i : c + 16u * i; }
+// the first column of a thread's vector: thread `at` of those that lie along the row
+template <bool kVector>
+K3_DEVINL constexpr uint32_t first_column(uint32_t at) { return kVector ? at * 8u : at / 16u * kBlock + at % 16u; }
+
 template <bool kF32>
 struct Eight {
     static constexpr uint32_t kWords = kF32 ? 8u : 4u;
     uint32_t w[kWords];
 
-    // elements c .. c + 7 of a row, zeros past its end.  kVector: rows start on 16 bytes and are whole vectors.
+    // zeros past the row's end
     template <bool kVector>
     K3_DEVINL void load(const void *row, uint32_t c, uint32_t columns) {
 #pragma unroll
@@ -40,9 +49,9 @@ struct Eight {
         } else {
 #pragma unroll
             for (uint32_t i = 0; i < 8u; i++) {
-                if (c + i >= columns) continue;
-                if (kF32) w[i % kWords] = ((const uint32_t *)row)[c + i];
-                else w[i / 2u] |= (uint32_t)((const uint16_t *)row)[c + i] << (16u * (i & 1u));
+                if (column_of<kVector>(c, i) >= columns) continue;
+                if (kF32) w[i % kWords] = ((const uint32_t *)row)[column_of<kVector>(c, i)];
+                else w[i / 2u] |= (uint32_t)((const uint16_t *)row)[column_of<kVector>(c, i)] << (16u * (i & 1u));
             }
         }
     }
@@ -58,9 +67,9 @@ struct Eight {
         } else {
 #pragma unroll
             for (uint32_t i = 0; i < 8u; i++) {
-                if (c + i >= columns) continue;
-                if (kF32) ((uint32_t *)row)[c + i] = w[i % kWords];
-                else ((uint16_t *)row)[c + i] = (uint16_t)(w[i / 2u] >> (16u * (i & 1u)));
+                if (column_of<kVector>(c, i) >= columns) continue;
+                if (kF32) ((uint32_t *)row)[column_of<kVector>(c, i)] = w[i % kWords];
+                else ((uint16_t *)row)[column_of<kVector>(c, i)] = (uint16_t)(w[i / 2u] >> (16u * (i & 1u)));
             }
         }
     }
@@ -100,6 +109,54 @@ struct NormArgs {
     float epsilon;
 };
 
+// The normalised elements of a thread's vector to y, and to codes with the largest magnitude of the half warp's block.
+// All lanes of a warp call it; `live`: the row exists.
+template <bool kF32, bool kVector>
+K3_DEVINL void put_normed(const NormArgs &a, const Eight<kF32> &s, const Eight<false> &w, float rstd, uint64_t row, uint32_t c, bool live) {
+    const uint32_t hidden = a.hidden, pitch = pitch_of(hidden);
+    float y[8];
+#pragma unroll
+    for (uint32_t i = 0; i < 8u; i++) y[i] = __fmul_rn(__fmul_rn(s.value(i), rstd), w.value(i));
+    if (a.y != nullptr) {
+        Eight<false> out;
+        out.set(y);
+        out.template store<kVector>(a.y + row * hidden, c, live ? hidden : 0u);
+    }
+    if (a.codes == nullptr) return;
+    uint32_t most = 0u;
+#pragma unroll
+    for (uint32_t i = 0; i < 8u; i++) {
+        // zeros past the row's end times a NaN rstd are NaN: they are no part of the block
+        if (column_of<kVector>(c, i) < hidden) most = max(most, __float_as_uint(y[i]) & 0x7fffffffu);
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    const float scale = scale_of(most), inverse = inverse_of(scale), lift = lift_of(scale), by = scale * lift;
+    uint32_t h[4];
+#pragma unroll
+    for (uint32_t i = 0; i < 4u; i++) {
+        h[i] = codes2(divided(y[2u * i] * lift, by, inverse), divided(y[2u * i + 1u] * lift, by, inverse));
+        if (column_of<kVector>(c, 2u * i) >= hidden) h[i] = 0u;      // zeros in the padding
+        else if (column_of<kVector>(c, 2u * i + 1u) >= hidden) h[i] &= 0xffu;
+    }
+    if (!live) return;
+    uint8_t *codes = a.codes + row * pitch;
+    if (kVector) {
+        if (c < pitch) *reinterpret_cast<uint2 *>(codes + c) = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; i++) {
+            if (column_of<kVector>(c, i) < pitch) codes[column_of<kVector>(c, i)] = (uint8_t)(h[i / 2u] >> (8u * (i & 1u)));
+        }
+    }
+    if (c < hidden && (c & 127u) == 0u) a.scales[row * scale_pitch_of(hidden) + c / kBlock] = scale;
+}
+// The scales' row behind its blocks.  t: a thread's place in the row's team.
+K3_DEVINL void put_scale_padding(const NormArgs &a, uint64_t row, uint32_t t) {
+    const uint32_t blocks = blocks_of(a.hidden), pitch = scale_pitch_of(a.hidden);
+    if (a.codes != nullptr && t < pitch - blocks) a.scales[row * pitch + blocks + t] = 0.0f;
+}
+
 // kTeam threads per row, kVectors vectors of 8 columns each.
 template <bool kF32, bool kVector, uint32_t kTeam, uint32_t kVectors>
 __global__ void __launch_bounds__(threads_of(kTeam)) norm_kernel(NormArgs a) {
@@ -111,18 +168,19 @@ __global__ void __launch_bounds__(threads_of(kTeam)) norm_kernel(NormArgs a) {
     const bool live = task < a.rows;                                 // the shuffles want every lane
     const uint64_t row = live ? task : 0u;
     const uint32_t columns = live ? a.hidden : 0u;
+    auto first = [&](uint32_t v) { return first_column<kVector>(v * kTeam + t); };
     const char *x = (const char *)a.x + row * a.hidden * kSize;
     const char *residual = (const char *)a.residual + row * a.hidden * kSize;
     Eight<kF32> s[kVectors], r[kVectors];
     Eight<false> w[kVectors];
 #pragma unroll
-    for (uint32_t v = 0; v < kVectors; v++) s[v].template load<kVector>(x, (v * kTeam + t) * 8u, columns);
+    for (uint32_t v = 0; v < kVectors; v++) s[v].template load<kVector>(x, first(v), columns);
     if (a.residual != nullptr) {
 #pragma unroll
-        for (uint32_t v = 0; v < kVectors; v++) r[v].template load<kVector>(residual, (v * kTeam + t) * 8u, columns);
+        for (uint32_t v = 0; v < kVectors; v++) r[v].template load<kVector>(residual, first(v), columns);
     }
 #pragma unroll
-    for (uint32_t v = 0; v < kVectors; v++) w[v].template load<kVector>(a.weight, (v * kTeam + t) * 8u, columns);
+    for (uint32_t v = 0; v < kVectors; v++) w[v].template load<kVector>(a.weight, first(v), columns);
     if (a.residual != nullptr) {
 #pragma unroll
         for (uint32_t v = 0; v < kVectors; v++) {
@@ -135,7 +193,7 @@ __global__ void __launch_bounds__(threads_of(kTeam)) norm_kernel(NormArgs a) {
     if (a.sum != nullptr) {
         char *sum = (char *)a.sum + row * a.hidden * kSize;
 #pragma unroll
-        for (uint32_t v = 0; v < kVectors; v++) s[v].template store<kVector>(sum, (v * kTeam + t) * 8u, columns);
+        for (uint32_t v = 0; v < kVectors; v++) s[v].template store<kVector>(sum, first(v), columns);
     }
     float squares = 0.0f;
 #pragma unroll
@@ -146,41 +204,9 @@ __global__ void __launch_bounds__(threads_of(kTeam)) norm_kernel(NormArgs a) {
     squares = team_sum<kTeam>(squares, scratch);
     const float rstd = 1.0f / sqrtf(squares / (float)a.hidden + a.epsilon);
     if (live && t == 0u && a.rstd != nullptr) a.rstd[row] = rstd;
-    const uint32_t pitch = pitch_of(a.hidden), blocks = blocks_of(a.hidden), scale_pitch = scale_pitch_of(a.hidden);
 #pragma unroll
-    for (uint32_t v = 0; v < kVectors; v++) {
-        const uint32_t c = (v * kTeam + t) * 8u;
-        float y[8];
-#pragma unroll
-        for (uint32_t i = 0; i < 8u; i++) y[i] = __fmul_rn(__fmul_rn(s[v].value(i), rstd), w[v].value(i));
-        if (a.y != nullptr) {
-            Eight<false> out;
-            out.set(y);
-            out.template store<kVector>(a.y + row * a.hidden, c, columns);
-        }
-        if (a.codes != nullptr) {
-            uint32_t most = 0u;
-#pragma unroll
-            for (uint32_t i = 0; i < 8u; i++) {
-                // zeros past the row's end times an infinite rstd are NaN: they are no part of the block
-                if (c + i < a.hidden) most = max(most, __float_as_uint(y[i]) & 0x7fffffffu);
-            }
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-            const float scale = scale_of(most), inverse = inverse_of(scale), lift = lift_of(scale), by = scale * lift;
-            uint32_t h[4];
-#pragma unroll
-            for (uint32_t i = 0; i < 4u; i++) {
-                h[i] = codes2(divided(y[2u * i] * lift, by, inverse), divided(y[2u * i + 1u] * lift, by, inverse));
-                if (c + 2u * i + 1u >= a.hidden) h[i] = c + 2u * i < a.hidden ? h[i] & 0xffu : 0u;
-            }
-            if (live && c < pitch) {
-                *reinterpret_cast<uint2 *>(a.codes + row * pitch + c) = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
-            }
-            if (live && c < a.hidden && (c & 127u) == 0u) a.scales[row * scale_pitch + c / kBlock] = scale;
-        }
-    }
-    if (live && a.codes != nullptr && t < scale_pitch - blocks) a.scales[row * scale_pitch + blocks + t] = 0.0f;
+    for (uint32_t v = 0; v < kVectors; v++) put_normed<kF32, kVector>(a, s[v], w[v], rstd, row, first(v), live);
+    if (live) put_scale_padding(a, row, t);
     pdl_trigger();
 }
 
@@ -194,6 +220,32 @@ struct NormGradArgs {
     uint32_t rows, hidden;
 };
 
+// A vector's part of the row's sum of w dy s rstd, and of the weight's gradient.
+template <bool kF32>
+K3_DEVINL float add_products(const Eight<false> &dy, const Eight<kF32> &s, const Eight<false> &w, float rstd, float dot, float (&dw)[8]) {
+#pragma unroll
+    for (uint32_t i = 0; i < 8u; i++) {
+        const float g = dy.value(i), h = s.value(i) * rstd;
+        dot = fmaf(g * w.value(i), h, dot);
+        dw[i] = fmaf(g, h, dw[i]);
+    }
+    return dot;
+}
+// A vector of dx; mean: that of w dy s rstd over the row.
+template <bool kF32>
+K3_DEVINL Eight<kF32> input_gradient(const Eight<false> &dy, const Eight<kF32> &s, const Eight<false> &w, const Eight<kF32> &d, bool with_d,
+                                     float rstd, float mean) {
+    float f[8];
+#pragma unroll
+    for (uint32_t i = 0; i < 8u; i++) {
+        f[i] = rstd * fmaf(-(s.value(i) * rstd), mean, dy.value(i) * w.value(i));
+        if (with_d) f[i] += d.value(i);
+    }
+    Eight<kF32> out;
+    out.set(f);
+    return out;
+}
+
 // Rows team, team + teams, ..; the weight's gradient stays in registers over all of them.
 template <bool kF32, bool kVector, uint32_t kTeam, uint32_t kVectors>
 __global__ void __launch_bounds__(threads_of(kTeam)) norm_backward_kernel(NormGradArgs a) {
@@ -202,79 +254,50 @@ __global__ void __launch_bounds__(threads_of(kTeam)) norm_backward_kernel(NormGr
     __shared__ float scratch[2][32];
     extern __shared__ float shared_dw[];                             // [kTeams][hidden], several teams only
     const uint32_t t = threadIdx.x % kTeam, team = threadIdx.x / kTeam;
+    auto first = [&](uint32_t v) { return first_column<kVector>(v * kTeam + t); };
     Eight<false> w[kVectors];
     float dw[kVectors][8];
 #pragma unroll
     for (uint32_t v = 0; v < kVectors; v++) {
-        w[v].template load<kVector>(a.weight, (v * kTeam + t) * 8u, a.hidden);
+        w[v].template load<kVector>(a.weight, first(v), a.hidden);
 #pragma unroll
         for (uint32_t i = 0; i < 8u; i++) dw[v][i] = 0.0f;
     }
     uint32_t turn = 0u;
-    for (uint64_t first = (uint64_t)blockIdx.x * kTeams; first < a.rows; first += (uint64_t)gridDim.x * kTeams, turn ^= 1u) {
-        const bool live = first + team < a.rows;
-        const uint64_t row = live ? first + team : 0u;
+    for (uint64_t at = (uint64_t)blockIdx.x * kTeams; at < a.rows; at += (uint64_t)gridDim.x * kTeams, turn ^= 1u) {
+        const bool live = at + team < a.rows;
+        const uint64_t row = live ? at + team : 0u;
         const uint32_t columns = live ? a.hidden : 0u;
         Eight<false> dy[kVectors];
         Eight<kF32> s[kVectors], d[kVectors];
 #pragma unroll
         for (uint32_t v = 0; v < kVectors; v++) {
-            dy[v].template load<kVector>(a.dy + row * a.hidden, (v * kTeam + t) * 8u, columns);
-            s[v].template load<kVector>((const char *)a.sum + row * a.hidden * kSize, (v * kTeam + t) * 8u, columns);
+            dy[v].template load<kVector>(a.dy + row * a.hidden, first(v), columns);
+            s[v].template load<kVector>((const char *)a.sum + row * a.hidden * kSize, first(v), columns);
+            if (a.d_sum != nullptr) d[v].template load<kVector>((const char *)a.d_sum + row * a.hidden * kSize, first(v), columns);
         }
-        if (a.d_sum != nullptr) {
-#pragma unroll
-            for (uint32_t v = 0; v < kVectors; v++) {
-                d[v].template load<kVector>((const char *)a.d_sum + row * a.hidden * kSize, (v * kTeam + t) * 8u, columns);
-            }
-        }
-        const float rstd = live ? a.rstd[row] : 0.0f;
+        const float rstd = live ? a.rstd[row] : 0.0f;                // with it zeros in the rows that do not exist
         float dot = 0.0f;
 #pragma unroll
-        for (uint32_t v = 0; v < kVectors; v++) {
-#pragma unroll
-            for (uint32_t i = 0; i < 8u; i++) {
-                const float g = dy[v].value(i), h = s[v].value(i) * rstd;
-                dot = fmaf(g * w[v].value(i), h, dot);
-                if (live) dw[v][i] = fmaf(g, h, dw[v][i]);
-            }
-        }
-        dot = team_sum<kTeam>(dot, scratch[turn]) / (float)a.hidden;
+        for (uint32_t v = 0; v < kVectors; v++) dot = add_products<kF32>(dy[v], s[v], w[v], rstd, dot, dw[v]);
+        const float mean = team_sum<kTeam>(dot, scratch[turn]) / (float)a.hidden;
         char *dx = (char *)a.dx + row * a.hidden * kSize;
 #pragma unroll
         for (uint32_t v = 0; v < kVectors; v++) {
-            float f[8];
-#pragma unroll
-            for (uint32_t i = 0; i < 8u; i++) {
-                const float h = s[v].value(i) * rstd;
-                f[i] = rstd * fmaf(-h, dot, dy[v].value(i) * w[v].value(i));
-                if (a.d_sum != nullptr) f[i] += d[v].value(i);
-            }
-            Eight<kF32> out;
-            out.set(f);
-            out.template store<kVector>(dx, (v * kTeam + t) * 8u, columns);
+            input_gradient<kF32>(dy[v], s[v], w[v], d[v], a.d_sum != nullptr, rstd, mean).template store<kVector>(dx, first(v), columns);
         }
     }
     if (a.partial == nullptr) return;
     float *to = a.partial + (uint64_t)blockIdx.x * a.hidden;
-    if (kTeams == 1u) {
 #pragma unroll
-        for (uint32_t v = 0; v < kVectors; v++) {
+    for (uint32_t v = 0; v < kVectors; v++) {
 #pragma unroll
-            for (uint32_t i = 0; i < 8u; i++) {
-                const uint32_t c = (v * kTeam + t) * 8u + i;
-                if (c < a.hidden) to[c] = dw[v][i];
-            }
+        for (uint32_t i = 0; i < 8u; i++) {
+            const uint32_t c = column_of<kVector>(first(v), i);
+            if (c < a.hidden) (kTeams == 1u ? to : shared_dw + team * a.hidden)[c] = dw[v][i];
         }
-    } else {
-#pragma unroll
-        for (uint32_t v = 0; v < kVectors; v++) {
-#pragma unroll
-            for (uint32_t i = 0; i < 8u; i++) {
-                const uint32_t c = (v * kTeam + t) * 8u + i;
-                if (c < a.hidden) shared_dw[team * a.hidden + c] = dw[v][i];
-            }
-        }
+    }
+    if (kTeams > 1u) {
         __syncthreads();
         for (uint32_t c = threadIdx.x; c < a.hidden; c += kThreads) {
             float sum = shared_dw[c];
@@ -306,6 +329,196 @@ __global__ void __launch_bounds__(256) norm_weight_kernel(float *d_weight, const
     }
 }
 
+// ------------------------------------------------------------------------------------- rows through a ring
+// Many rows of more than 1024 columns: one block per SM takes rows block, block + blocks, ..  A seventeenth warp copies
+// whole rows into a ring of stages in shared memory, up to 192 KB ahead, so that memory is never waited for while a row's
+// sum goes around the other sixteen.
+constexpr uint32_t kRingThreads = 512, kRingWarps = kRingThreads / kWarp, kRingBytes = 196608, kMaxStages = 8;
+
+__device__ uint32_t g_norm_status = 0;
+
+K3_DEVINL void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),
+                 "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+
+struct Ring {
+    unsigned char *base;
+    uint64_t *full, *empty;
+    volatile uint32_t *abort_flag;
+    uint32_t stages, stage_bytes;
+
+    K3_DEVINL void init(unsigned char *smem, uint32_t stages_, uint32_t stage_bytes_) {
+        base = smem + 256u;
+        full = reinterpret_cast<uint64_t *>(smem);
+        empty = full + kMaxStages;
+        abort_flag = reinterpret_cast<uint32_t *>(empty + kMaxStages);
+        stages = stages_;
+        stage_bytes = stage_bytes_;
+        if (threadIdx.x == 0u) {
+            *abort_flag = 0u;
+            for (uint32_t s = 0; s < stages; s++) {
+                mbar_init(&full[s], 1);
+                mbar_init(&empty[s], kRingWarps);
+            }
+            fence_barrier_init();
+        }
+        __syncthreads();
+    }
+    // The copying thread: rows first, first + step, ..; each from up to three places, side by side in a stage.
+    K3_DEVINL void fill(uint64_t first, uint64_t step, uint64_t rows, const char *a, uint32_t a_bytes, const char *b, uint32_t b_bytes,
+                        const char *c, uint32_t c_bytes) {
+        uint32_t s = 0u, ph = 0u, issued = 0u;
+        for (uint64_t row = first; row < rows; row += step) {
+            if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag)) break;
+            unsigned char *to = base + s * stage_bytes;
+            mbar_arrive_expect_tx(&full[s], a_bytes + b_bytes + c_bytes);
+            bulk_load(to, a + row * a_bytes, a_bytes, &full[s]);
+            if (b_bytes != 0u) bulk_load(to + a_bytes, b + row * b_bytes, b_bytes, &full[s]);
+            if (c_bytes != 0u) bulk_load(to + a_bytes + b_bytes, c + row * c_bytes, c_bytes, &full[s]);
+            issued++;
+            if (++s == stages) { s = 0u; ph ^= 1u; }
+        }
+        if (*abort_flag != 0u) {                                     // nothing may land in a block that has left
+            for (uint32_t i = issued > stages ? issued - stages : 0u; i < issued; i++) mbar_drain(&full[i % stages], (i / stages) & 1u);
+        }
+    }
+};
+
+// Sum over the sixteen warps; `scratch` alternates between two rows.
+K3_DEVINL float ring_sum(float v, float *scratch) {
+    v = warp_sum(v);
+    if (threadIdx.x % kWarp == 0u) scratch[threadIdx.x / kWarp] = v;
+    asm volatile("bar.sync 1, 512;" ::: "memory");
+    v = scratch[threadIdx.x % kRingWarps];
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+template <bool kF32, uint32_t kVectors>
+__global__ void __launch_bounds__(kRingThreads + kWarp, 1) norm_ring_kernel(NormArgs a, uint32_t stages) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ float scratch[2][kRingWarps];
+    const uint32_t bytes = a.hidden * (kF32 ? 4u : 2u), more = a.residual != nullptr ? bytes : 0u;
+    Ring ring;
+    ring.init(smem, stages, bytes + more);
+    pdl_wait();
+    if (threadIdx.x >= kRingThreads) {
+        if (elect_one()) ring.fill(blockIdx.x, gridDim.x, a.rows, (const char *)a.x, bytes, (const char *)a.residual, more, nullptr, 0u);
+    } else {
+        const uint32_t t = threadIdx.x;
+        auto first = [&](uint32_t v) { return (v * kRingThreads + t) * 8u; };
+        Eight<false> w[kVectors];
+#pragma unroll
+        for (uint32_t v = 0; v < kVectors; v++) w[v].template load<true>(a.weight, first(v), a.hidden);
+        uint32_t st = 0u, ph = 0u, turn = 0u;
+        bool ok = true;
+        for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1u) {
+            ok = ok && mbar_wait(&ring.full[st], ph, ring.abort_flag);   // given up: the sums below still meet
+            const unsigned char *in = ring.base + st * ring.stage_bytes;
+            Eight<kF32> s[kVectors];
+            float squares = 0.0f;
+#pragma unroll
+            for (uint32_t v = 0; v < kVectors; v++) s[v].template load<true>(in, first(v), a.hidden);
+            if (more != 0u) {
+#pragma unroll
+                for (uint32_t v = 0; v < kVectors; v++) {
+                    Eight<kF32> r;
+                    r.template load<true>(in + bytes, first(v), a.hidden);
+                    float f[8];
+#pragma unroll
+                    for (uint32_t i = 0; i < 8u; i++) f[i] = s[v].value(i) + r.value(i);
+                    s[v].set(f);
+                }
+            }
+            __syncwarp();
+            if (t % kWarp == 0u) mbar_arrive(&ring.empty[st]);
+            if (++st == stages) { st = 0u; ph ^= 1u; }
+#pragma unroll
+            for (uint32_t v = 0; v < kVectors; v++) {
+                if (a.sum != nullptr) s[v].template store<true>((char *)a.sum + row * bytes, first(v), a.hidden);
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; i++) squares = fmaf(s[v].value(i), s[v].value(i), squares);
+            }
+            const float rstd = 1.0f / sqrtf(ring_sum(squares, scratch[turn]) / (float)a.hidden + a.epsilon);
+            if (t == 0u && a.rstd != nullptr) a.rstd[row] = rstd;
+#pragma unroll
+            for (uint32_t v = 0; v < kVectors; v++) put_normed<kF32, true>(a, s[v], w[v], rstd, row, first(v), true);
+            put_scale_padding(a, row, t);
+        }
+    }
+    pdl_trigger();
+    __syncthreads();
+    if (threadIdx.x == 0u && *ring.abort_flag != 0u) atomicExch(&g_norm_status, 1u);
+}
+
+template <bool kF32, uint32_t kVectors>
+__global__ void __launch_bounds__(kRingThreads + kWarp, 1) norm_backward_ring_kernel(NormGradArgs a, uint32_t stages) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ float scratch[2][kRingWarps];
+    const uint32_t bytes = a.hidden * (kF32 ? 4u : 2u), more = a.d_sum != nullptr ? bytes : 0u;
+    Ring ring;
+    ring.init(smem, stages, a.hidden * 2u + bytes + more);
+    pdl_wait();
+    if (threadIdx.x >= kRingThreads) {
+        if (elect_one()) {
+            ring.fill(blockIdx.x, gridDim.x, a.rows, (const char *)a.dy, a.hidden * 2u, (const char *)a.sum, bytes, (const char *)a.d_sum, more);
+        }
+    } else {
+        const uint32_t t = threadIdx.x;
+        auto first = [&](uint32_t v) { return (v * kRingThreads + t) * 8u; };
+        Eight<false> w[kVectors];
+        float dw[kVectors][8];
+#pragma unroll
+        for (uint32_t v = 0; v < kVectors; v++) {
+            w[v].template load<true>(a.weight, first(v), a.hidden);
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; i++) dw[v][i] = 0.0f;
+        }
+        uint32_t st = 0u, ph = 0u, turn = 0u;
+        bool ok = true;
+        for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1u) {
+            const float rstd = a.rstd[row];
+            ok = ok && mbar_wait(&ring.full[st], ph, ring.abort_flag);
+            const unsigned char *in = ring.base + st * ring.stage_bytes;
+            Eight<false> dy[kVectors];
+            Eight<kF32> s[kVectors], d[kVectors];
+            float dot = 0.0f;
+#pragma unroll
+            for (uint32_t v = 0; v < kVectors; v++) {
+                dy[v].template load<true>(in, first(v), a.hidden);
+                s[v].template load<true>(in + a.hidden * 2u, first(v), a.hidden);
+                if (more != 0u) d[v].template load<true>(in + a.hidden * 2u + bytes, first(v), a.hidden);
+            }
+            __syncwarp();
+            if (t % kWarp == 0u) mbar_arrive(&ring.empty[st]);
+            if (++st == stages) { st = 0u; ph ^= 1u; }
+#pragma unroll
+            for (uint32_t v = 0; v < kVectors; v++) dot = add_products<kF32>(dy[v], s[v], w[v], rstd, dot, dw[v]);
+            const float mean = ring_sum(dot, scratch[turn]) / (float)a.hidden;
+#pragma unroll
+            for (uint32_t v = 0; v < kVectors; v++) {
+                input_gradient<kF32>(dy[v], s[v], w[v], d[v], more != 0u, rstd, mean)
+                    .template store<true>((char *)a.dx + row * bytes, first(v), a.hidden);
+            }
+        }
+        if (a.partial != nullptr) {
+            float *to = a.partial + (uint64_t)blockIdx.x * a.hidden;
+#pragma unroll
+            for (uint32_t v = 0; v < kVectors; v++) {
+                if (first(v) >= a.hidden) continue;
+                *reinterpret_cast<float4 *>(to + first(v)) = make_float4(dw[v][0], dw[v][1], dw[v][2], dw[v][3]);
+                *reinterpret_cast<float4 *>(to + first(v) + 4u) = make_float4(dw[v][4], dw[v][5], dw[v][6], dw[v][7]);
+            }
+        }
+    }
+    pdl_trigger();
+    __syncthreads();
+    if (threadIdx.x == 0u && *ring.abort_flag != 0u) atomicExch(&g_norm_status, 1u);
+}
+
 // ------------------------------------------------------------------------------------------------ host
 bool aligned(const void *p, uint32_t bytes) { return ((uintptr_t)p & (bytes - 1u)) == 0u; }
 
@@ -320,35 +533,63 @@ bool by_size(uint32_t hidden, F &&launch) {
     if (hidden <= 2048u) return K3_SIZE(256u, 1u);
     if (hidden <= 4096u) return K3_SIZE(256u, 2u);
     if (hidden <= 8192u) return K3_SIZE(256u, 4u);
-    if (hidden <= 16384u) return K3_SIZE(1024u, 2u);
-    if (hidden <= 32768u) return K3_SIZE(1024u, 4u);
-    return K3_SIZE(1024u, 8u);
+    return K3_SIZE(1024u, 2u);
 #undef K3_SIZE
 }
+template <typename F>
+bool by_ring_size(uint32_t hidden, F &&launch) {
+    using std::integral_constant;
+    return hidden <= 4096u ? launch(integral_constant<uint32_t, 1u>{}) : launch(integral_constant<uint32_t, 2u>{});
+}
+uint32_t ring_stages(uint32_t stage_bytes) { return std::min(kRingBytes / stage_bytes, kMaxStages); }
 
-template <bool kF32, bool kVector>
-bool launch_norm(const NormArgs &a, cudaStream_t stream) {
+template <typename K, typename A>
+bool launch_ring(K kernel, const A &a, uint32_t blocks, uint32_t stage_bytes, cudaStream_t stream) {
+    const uint32_t stages = ring_stages(stage_bytes), bytes = 256u + stages * stage_bytes;
+    return set_max_dynamic_smem((const void *)kernel, 256u + kRingBytes) && launch_chained(kernel, blocks, kRingThreads + kWarp, bytes, stream, a, stages);
+}
+
+// The ring pays once every SM has a few rows.
+bool ring_suits(uint32_t rows, uint32_t hidden, bool vector, uint32_t stage_bytes) {
+    return vector && hidden > 1024u && hidden <= 8192u && rows >= 4u * (uint32_t)sm_count() && ring_stages(stage_bytes) >= 2u;
+}
+
+template <bool kF32>
+bool launch_norm(const NormArgs &a, bool vector, cudaStream_t stream) {
+    const uint32_t stage = a.hidden * (kF32 ? 4u : 2u) * (a.residual ? 2u : 1u);
+    if (ring_suits(a.rows, a.hidden, vector, stage)) {
+        return by_ring_size(a.hidden, [&](auto vectors) {
+            return launch_ring(norm_ring_kernel<kF32, decltype(vectors)::value>, a, (uint32_t)sm_count(), stage, stream);
+        });
+    }
     return by_size(a.hidden, [&](auto team, auto vectors) {
         constexpr uint32_t kTeam = decltype(team)::value, kThreads = threads_of(kTeam), kTeams = kThreads / kTeam;
-        return launch_chained(norm_kernel<kF32, kVector, kTeam, decltype(vectors)::value>, (a.rows + kTeams - 1u) / kTeams, kThreads, 0,
-                              stream, a);
+        auto kernel = vector ? norm_kernel<kF32, true, kTeam, decltype(vectors)::value> : norm_kernel<kF32, false, kTeam, decltype(vectors)::value>;
+        return launch_chained(kernel, (a.rows + kTeams - 1u) / kTeams, kThreads, 0, stream, a);
     });
 }
 
-// Blocks of the gradient: two per SM of a B200, so that the partial rows of the weight's gradient do not depend on
-// the device.
-constexpr uint32_t kGradBlocks = 296;
+// Blocks of the gradient, each with a partial row of the weight's: up to two per SM.
 uint32_t grad_blocks(uint32_t rows, uint32_t hidden) {
     const uint32_t teams = hidden <= 1024u ? 8u : 1u;
-    return std::min((rows + teams - 1u) / teams, kGradBlocks);
+    return std::min((rows + teams - 1u) / teams, 2u * (uint32_t)sm_count());
 }
 
-template <bool kF32, bool kVector>
-bool launch_backward(const NormGradArgs &a, cudaStream_t stream) {
+template <bool kF32>
+bool launch_backward(const NormGradArgs &a, bool vector, uint32_t &blocks, cudaStream_t stream) {
+    const uint32_t stage = a.hidden * (2u + (kF32 ? 4u : 2u) * (a.d_sum ? 2u : 1u));
+    blocks = grad_blocks(a.rows, a.hidden);
+    if (ring_suits(a.rows, a.hidden, vector, stage)) {
+        blocks = (uint32_t)sm_count();
+        return by_ring_size(a.hidden, [&](auto vectors) {
+            return launch_ring(norm_backward_ring_kernel<kF32, decltype(vectors)::value>, a, blocks, stage, stream);
+        });
+    }
     return by_size(a.hidden, [&](auto team, auto vectors) {
         constexpr uint32_t kTeam = decltype(team)::value, kThreads = threads_of(kTeam), kTeams = kThreads / kTeam;
-        return launch_chained(norm_backward_kernel<kF32, kVector, kTeam, decltype(vectors)::value>, grad_blocks(a.rows, a.hidden), kThreads,
-                              kTeams > 1u ? kTeams * a.hidden * 4u : 0u, stream, a);
+        auto kernel = vector ? norm_backward_kernel<kF32, true, kTeam, decltype(vectors)::value>
+                             : norm_backward_kernel<kF32, false, kTeam, decltype(vectors)::value>;
+        return launch_chained(kernel, blocks, kThreads, kTeams > 1u ? kTeams * a.hidden * 4u : 0u, stream, a);
     });
 }
 
@@ -372,8 +613,7 @@ extern "C" bool k3_moe_norm(void *sum, void *y, void *codes, void *scales, void 
                      hidden, epsilon};
     const bool vector = hidden % 8u == 0u && aligned(sum, 16u) && aligned(x, 16u) && aligned(residual, 16u) && aligned(weight, 16u) &&
                         aligned(y, 16u);
-    if (f32) return vector ? launch_norm<true, true>(a, (cudaStream_t)stream) : launch_norm<true, false>(a, (cudaStream_t)stream);
-    return vector ? launch_norm<false, true>(a, (cudaStream_t)stream) : launch_norm<false, false>(a, (cudaStream_t)stream);
+    return f32 ? launch_norm<true>(a, vector, (cudaStream_t)stream) : launch_norm<false>(a, vector, (cudaStream_t)stream);
 }
 
 extern "C" size_t k3_moe_norm_workspace_bytes(uint32_t rows, uint32_t hidden) {
@@ -403,9 +643,22 @@ extern "C" bool k3_moe_norm_backward(void *dx, void *d_weight, const void *dy, c
                          (const float *)rstd, rows, hidden};
     const bool vector = hidden % 8u == 0u && aligned(dx, 16u) && aligned(dy, 16u) && aligned(sum, 16u) && aligned(d_sum, 16u) &&
                         aligned(weight, 16u);
-    const bool ok = f32 ? (vector ? launch_backward<true, true>(a, (cudaStream_t)stream) : launch_backward<true, false>(a, (cudaStream_t)stream))
-                        : (vector ? launch_backward<false, true>(a, (cudaStream_t)stream) : launch_backward<false, false>(a, (cudaStream_t)stream));
+    uint32_t blocks = 0u;
+    const bool ok = f32 ? launch_backward<true>(a, vector, blocks, (cudaStream_t)stream) : launch_backward<false>(a, vector, blocks, (cudaStream_t)stream);
     if (!ok || !d_weight) return ok;
     return launch_chained(norm_weight_kernel, (hidden + 31u) / 32u, 256, 0, (cudaStream_t)stream, (float *)d_weight,
-                          (const float *)workspace, grad_blocks(rows, hidden), hidden, accumulate);
+                          (const float *)workspace, blocks, hidden, accumulate);
+}
+
+uint32_t k3_norm_status() {
+    uint32_t v = 0xffffffffu;
+    if (cudaMemcpyFromSymbol(&v, g_norm_status, sizeof(v)) != cudaSuccess) (void)cudaGetLastError();
+    return v;
+}
+
+bool k3_norm_status_clear() {
+    const uint32_t zero = 0u;
+    const bool ok = cudaMemcpyToSymbol(g_norm_status, &zero, sizeof(zero)) == cudaSuccess;
+    if (!ok) (void)cudaGetLastError();
+    return ok;
 }
