@@ -349,7 +349,8 @@ struct Ring {
     volatile uint32_t *abort_flag;
     uint32_t stages, stage_bytes;
 
-    K3_DEVINL void init(unsigned char *smem, uint32_t stages_, uint32_t stage_bytes_) {
+    // readers: warps that take a row out of its stage
+    K3_DEVINL void init(unsigned char *smem, uint32_t stages_, uint32_t stage_bytes_, uint32_t readers) {
         base = smem + 256u;
         full = reinterpret_cast<uint64_t *>(smem);
         empty = full + kMaxStages;
@@ -360,7 +361,7 @@ struct Ring {
             *abort_flag = 0u;
             for (uint32_t s = 0; s < stages; s++) {
                 mbar_init(&full[s], 1);
-                mbar_init(&empty[s], kRingWarps);
+                mbar_init(&empty[s], readers);
             }
             fence_barrier_init();
         }
@@ -386,36 +387,40 @@ struct Ring {
     }
 };
 
-// Sum over the sixteen warps; `scratch` alternates between two rows.
+// Sum over the kTeam threads of a row; `scratch`, a float per warp of the team, alternates between two rows.
+template <uint32_t kTeam>
 K3_DEVINL float ring_sum(float v, float *scratch) {
+    constexpr uint32_t kWarps = kTeam / kWarp;
     v = warp_sum(v);
-    if (threadIdx.x % kWarp == 0u) scratch[threadIdx.x / kWarp] = v;
-    asm volatile("bar.sync 1, 512;" ::: "memory");
-    v = scratch[threadIdx.x % kRingWarps];
+    if (threadIdx.x % kWarp == 0u) scratch[threadIdx.x % kTeam / kWarp] = v;
+    asm volatile("bar.sync %0, %1;" ::"r"(1u + threadIdx.x / kTeam), "n"(kTeam) : "memory");
+    v = scratch[threadIdx.x % kWarps];
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    for (int o = kWarps / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
 
+// Two rows at a time, each by half of the block: one row's sum goes around while the other's results are stored.
 template <bool kF32, uint32_t kVectors>
 __global__ void __launch_bounds__(kRingThreads + kWarp, 1) norm_ring_kernel(NormArgs a, uint32_t stages) {
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ float scratch[2][kRingWarps];
+    constexpr uint32_t kTeam = kRingThreads / 2u;
+    __shared__ float scratch[2][2][kTeam / kWarp];
     const uint32_t bytes = a.hidden * (kF32 ? 4u : 2u), more = a.residual != nullptr ? bytes : 0u;
     Ring ring;
-    ring.init(smem, stages, bytes + more);
+    ring.init(smem, stages, bytes + more, kTeam / kWarp);
     pdl_wait();
     if (threadIdx.x >= kRingThreads) {
         if (elect_one()) ring.fill(blockIdx.x, gridDim.x, a.rows, (const char *)a.x, bytes, (const char *)a.residual, more, nullptr, 0u);
     } else {
-        const uint32_t t = threadIdx.x;
-        auto first = [&](uint32_t v) { return (v * kRingThreads + t) * 8u; };
+        const uint32_t t = threadIdx.x % kTeam, team = threadIdx.x / kTeam;
+        auto first = [&](uint32_t v) { return (v * kTeam + t) * 8u; };
         Eight<false> w[kVectors];
 #pragma unroll
         for (uint32_t v = 0; v < kVectors; v++) w[v].template load<true>(a.weight, first(v), a.hidden);
-        uint32_t st = 0u, ph = 0u, turn = 0u;
+        uint32_t st = team % stages, ph = (team / stages) & 1u, turn = 0u;
         bool ok = true;
-        for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1u) {
+        for (uint64_t row = blockIdx.x + (uint64_t)team * gridDim.x; row < a.rows; row += 2u * (uint64_t)gridDim.x, turn ^= 1u) {
             ok = ok && mbar_wait(&ring.full[st], ph, ring.abort_flag);   // given up: the sums below still meet
             const unsigned char *in = ring.base + st * ring.stage_bytes;
             Eight<kF32> s[kVectors];
@@ -435,14 +440,15 @@ __global__ void __launch_bounds__(kRingThreads + kWarp, 1) norm_ring_kernel(Norm
             }
             __syncwarp();
             if (t % kWarp == 0u) mbar_arrive(&ring.empty[st]);
-            if (++st == stages) { st = 0u; ph ^= 1u; }
+            st += 2u;
+            if (st >= stages) { st -= stages; ph ^= 1u; }
 #pragma unroll
             for (uint32_t v = 0; v < kVectors; v++) {
                 if (a.sum != nullptr) s[v].template store<true>((char *)a.sum + row * bytes, first(v), a.hidden);
 #pragma unroll
                 for (uint32_t i = 0; i < 8u; i++) squares = fmaf(s[v].value(i), s[v].value(i), squares);
             }
-            const float rstd = 1.0f / sqrtf(ring_sum(squares, scratch[turn]) / (float)a.hidden + a.epsilon);
+            const float rstd = 1.0f / sqrtf(ring_sum<kTeam>(squares, scratch[team][turn]) / (float)a.hidden + a.epsilon);
             if (t == 0u && a.rstd != nullptr) a.rstd[row] = rstd;
 #pragma unroll
             for (uint32_t v = 0; v < kVectors; v++) put_normed<kF32, true>(a, s[v], w[v], rstd, row, first(v), true);
@@ -460,7 +466,7 @@ __global__ void __launch_bounds__(kRingThreads + kWarp, 1) norm_backward_ring_ke
     __shared__ float scratch[2][kRingWarps];
     const uint32_t bytes = a.hidden * (kF32 ? 4u : 2u), more = a.d_sum != nullptr ? bytes : 0u;
     Ring ring;
-    ring.init(smem, stages, a.hidden * 2u + bytes + more);
+    ring.init(smem, stages, a.hidden * 2u + bytes + more, kRingWarps);
     pdl_wait();
     if (threadIdx.x >= kRingThreads) {
         if (elect_one()) {
@@ -497,7 +503,7 @@ __global__ void __launch_bounds__(kRingThreads + kWarp, 1) norm_backward_ring_ke
             if (++st == stages) { st = 0u; ph ^= 1u; }
 #pragma unroll
             for (uint32_t v = 0; v < kVectors; v++) dot = add_products<kF32>(dy[v], s[v], w[v], rstd, dot, dw[v]);
-            const float mean = ring_sum(dot, scratch[turn]) / (float)a.hidden;
+            const float mean = ring_sum<kRingThreads>(dot, scratch[turn]) / (float)a.hidden;
 #pragma unroll
             for (uint32_t v = 0; v < kVectors; v++) {
                 input_gradient<kF32>(dy[v], s[v], w[v], d[v], more != 0u, rstd, mean)
@@ -536,6 +542,7 @@ bool by_size(uint32_t hidden, F &&launch) {
     return K3_SIZE(1024u, 2u);
 #undef K3_SIZE
 }
+// Vectors of 8 columns per thread where 512 threads share a row.
 template <typename F>
 bool by_ring_size(uint32_t hidden, F &&launch) {
     using std::integral_constant;
@@ -559,7 +566,7 @@ bool launch_norm(const NormArgs &a, bool vector, cudaStream_t stream) {
     const uint32_t stage = a.hidden * (kF32 ? 4u : 2u) * (a.residual ? 2u : 1u);
     if (ring_suits(a.rows, a.hidden, vector, stage)) {
         return by_ring_size(a.hidden, [&](auto vectors) {
-            return launch_ring(norm_ring_kernel<kF32, decltype(vectors)::value>, a, (uint32_t)sm_count(), stage, stream);
+            return launch_ring(norm_ring_kernel<kF32, 2u * decltype(vectors)::value>, a, (uint32_t)sm_count(), stage, stream);
         });
     }
     return by_size(a.hidden, [&](auto team, auto vectors) {

@@ -117,7 +117,7 @@ class GatedActivation:
         rows, columns = _matrix(gate, "gate")
         _check(up, "up", torch.bfloat16, (rows, columns))
         _placed(("gate", gate), ("up", up))
-        out = gate.new_empty((rows, columns))
+        out = torch.empty_like(gate)
         if rows and columns:
             _done(ops.k3_moe_activation_bf16(out, gate, up, rows * columns, self.activation, self.beta, self.linear_beta),
                   "k3_moe_activation_bf16")
@@ -143,11 +143,13 @@ class GatedActivation:
         if offsets is not None and (offsets.dtype is not torch.int32 or offsets.dim() != 1 or offsets.shape[0] < 2):
             raise ValueError(f"offsets: expected int32 [groups + 1], got {offsets.dtype} {list(offsets.shape)}")
         _placed(("d_out", d_out), ("gate", gate), ("up", up), ("weights", weights), ("routes", routes), ("offsets", offsets))
-        d_gate, d_up, scaled = (d_out.new_empty((rows, columns)) for _ in range(3))
+        d_gate, d_up, scaled = torch.empty_like(d_out), torch.empty_like(d_out), torch.empty_like(d_out)
         count = rows if weights is None else weights.numel()
         # routes that no row has get no gradient
-        make = d_out.new_empty if offsets is None and count == rows and rows and columns else d_out.new_zeros
-        d_weights = make((rows,) if weights is None else weights.shape, dtype=torch.float32)
+        if offsets is None and count == rows and rows and columns:
+            d_weights = d_out.new_empty(rows, dtype=torch.float32) if weights is None else torch.empty_like(weights)
+        else:
+            d_weights = d_out.new_zeros((rows,) if weights is None else weights.shape, dtype=torch.float32)
         if rows and columns:
             _done(ops.k3_moe_activation_backward(d_gate, d_up, scaled, d_weights, d_out, gate, up, weights, routes, offsets,
                                                  0 if offsets is None else offsets.shape[0] - 1, rows, columns, count,
