@@ -12,7 +12,7 @@
 //   warp 0       loads by TMA
 //   warp 1       MMA issuer, owns the tensor memory: an accumulator of kMaxN columns for each of two halves
 //   warp 2       draws items from a counter and tells the others, when the loads of the one before come to an end
-//   warp 3       by weight: clears what a group's last stage holds of the rows behind the group
+//   warp 3       by weight: clears what a group's first stage holds of the rows behind its part of the group
 //   warps 4-11   results: lane quadrant warp % 4, every second chunk of 32 columns; the accumulator is free again once
 //                it is in registers, before anything is stored
 // Items that share a matrix are neighbours in the order, so it is in L2 for all but one of them.  Their results do not
@@ -53,10 +53,12 @@ struct Tile {
     uint32_t group, row, rows, first, count, pad[3];                   // first .. first + count - 1: the group's tiles
 };
 
-template <uint32_t kHalves_, uint32_t kMaxN_, uint32_t kStages_>
+template <uint32_t kCtas_, uint32_t kHalves_, uint32_t kMaxN_, uint32_t kStages_>
 struct Shape {
-    static constexpr uint32_t kHalves = kHalves_, kMaxN = kMaxN_, kStages = kStages_;
-    static constexpr uint32_t kA = kHalves * 2u * kBox, kStage = kA + kMaxN * kDepth * 2u;
+    static constexpr uint32_t kCtas = kCtas_, kHalves = kHalves_, kMaxN = kMaxN_, kStages = kStages_;
+    static constexpr uint32_t kHalf = 128u * kCtas, kLanes = kHalf * kHalves;
+    static constexpr uint32_t kStep = 16u * kCtas;                     // of an MMA's columns
+    static constexpr uint32_t kA = kHalves * 2u * kBox, kStage = kA + kMaxN / kCtas * kDepth * 2u;
     static constexpr uint32_t kStore = kStages * kStage;               // 4 KB per result warp
     static constexpr uint32_t kBars = kStore + kResultWarps * 4096u;
     static constexpr uint32_t kBytes = kBars + 512u + 1024u;           // the last: alignment
@@ -82,8 +84,8 @@ struct Item {
 
 // Instruction descriptor, kind::f16, as make_idesc_bf16, with bits 15 and 16 for operands whose depth is not what lies
 // side by side.
-K3_DEVINL constexpr uint32_t idesc_of(uint32_t n, bool a_by_depth, bool b_by_depth) {
-    return make_idesc_bf16(128u, n) | (a_by_depth ? 1u << 15 : 0u) | (b_by_depth ? 1u << 16 : 0u);
+K3_DEVINL constexpr uint32_t idesc_of(uint32_t m, uint32_t n, bool a_by_depth, bool b_by_depth) {
+    return make_idesc_bf16(m, n) | (a_by_depth ? 1u << 15 : 0u) | (b_by_depth ? 1u << 16 : 0u);
 }
 // Shared-memory descriptor of a tile whose rows are its depth: boxes of 64 elements x 64 rows of 128 bytes with the
 // 128-byte swizzle, 8 KB apart (the leading offset); groups of 8 rows are 1024 bytes apart (the stride offset).
@@ -91,18 +93,115 @@ K3_DEVINL uint64_t make_desc_by_depth(uint32_t smem_addr) {
     return (make_desc_sw128(smem_addr) & ~((uint64_t)0x3fffu << 16)) | ((uint64_t)(kBox >> 4) << 16);
 }
 
-K3_DEVINL void tma_load_3d(void *dst, const void *map, uint64_t *bar, int32_t x, int32_t y, int32_t z) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes "
-        "[%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
-        "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
-        : "memory");
+// ------------------------------------------------------------------- what a pair of blocks adds
+// The place of `p` in the shared memory of block `rank` of the cluster.
+K3_DEVINL uint32_t place_in(const void *p, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+    return r;
+}
+K3_DEVINL void arrive_at(uint32_t bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// The same after which nothing that this thread wrote is read: a release would first wait for its stores to memory.
+K3_DEVINL void arrive_relaxed_at(uint32_t bar) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+K3_DEVINL void store_at(uint32_t to, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(v) : "memory"); }
+// mbar_wait for arrivals from the other block
+K3_DEVINL bool wait_cluster(uint64_t *bar, uint32_t parity, volatile uint32_t *abort_flag) {
+    const unsigned long long t0 = global_timer_ns();
+    for (uint32_t spin = 1;; spin++) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.b32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if ((spin & 63u) == 0u) {
+            if (*abort_flag != 0u) return false;
+            if (global_timer_ns() - t0 > kWaitLimitNs) break;
+        }
+    }
+    *abort_flag = 1u;
+    return false;
+}
+
+// Loads of 2 and 3 dimensions.  kCtas 2: `bar` is the first block's barrier, wherever the copy goes.
+template <uint32_t kCtas>
+K3_DEVINL void load_2d(void *dst, const void *map, uint32_t bar, int32_t x, int32_t y) {
+    if constexpr (kCtas == 2u) {
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
+                smem_u32(dst)),
+            "l"(map), "r"(bar), "r"(x), "r"(y)
+            : "memory");
+    } else {
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+                     "l"(map), "r"(bar), "r"(x), "r"(y)
+                     : "memory");
+    }
+}
+template <uint32_t kCtas>
+K3_DEVINL void load_3d(void *dst, const void *map, uint32_t bar, int32_t x, int32_t y, int32_t z) {
+    if constexpr (kCtas == 2u) {
+        asm volatile(
+            "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+                smem_u32(dst)),
+            "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+            : "memory");
+    } else {
+        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+                         smem_u32(dst)),
+                     "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+                     : "memory");
+    }
+}
+template <uint32_t kCtas>
+K3_DEVINL void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (kCtas == 2u) {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+            : "memory");
+    } else {
+        mma_f16_ss(d, a, b, idesc, accumulate);
+    }
+}
+// `bar`, of both blocks, once every MMA issued so far has run
+template <uint32_t kCtas>
+K3_DEVINL void commit(uint64_t *bar) {
+    if constexpr (kCtas == 2u) {
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+                     "h"((uint16_t)3)
+                     : "memory");
+    } else {
+        mma_commit(bar);
+    }
+}
+template <uint32_t kCtas>
+K3_DEVINL void alloc_tmem(uint32_t *slot, uint32_t columns) {
+    if constexpr (kCtas == 2u) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+        tmem_alloc(slot, columns);
+        tmem_relinquish();
+    }
+}
+template <uint32_t kCtas>
+K3_DEVINL void free_tmem(uint32_t tmem, uint32_t columns) {
+    if constexpr (kCtas == 2u) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
+    else tmem_dealloc(tmem, columns);
 }
 
 // ------------------------------------------------------------------------------------------- the plan
-// One thread per group.  A group's rows in as few tiles of up to max_n as there can be, equally large.
+// One thread per group.  A group's rows in as few tiles of up to max_n as there can be, equally large but for one step.
 __global__ void __launch_bounds__(kMaxGroups) grouped_plan_kernel(Plan *plan, Tile *tiles, const uint32_t *offsets, uint32_t rows,
-                                                                  uint32_t groups, uint32_t max_n, uint32_t capacity) {
+                                                                  uint32_t groups, uint32_t max_n, uint32_t step, uint32_t capacity) {
     pdl_trigger();
     pdl_wait();
     __shared__ uint32_t sums[kMaxGroups / kWarp];
@@ -121,10 +220,11 @@ __global__ void __launch_bounds__(kMaxGroups) grouped_plan_kernel(Plan *plan, Ti
     uint32_t first = scan - count;
     for (uint32_t w = 0; w < warp; w++) first += sums[w];
     if (count != 0u) {
-        const uint32_t size = ((end - begin + count - 1u) / count + 15u) & ~15u;
-        for (uint32_t i = 0; i < count && first + i < capacity; i++) {
-            Tile t{g, begin + i * size, min(size, end - begin - i * size), first, min(count, capacity - first), {}};
-            tiles[first + i] = t;
+        const uint32_t steps = (end - begin + step - 1u) / step, each = steps / count, more = steps - each * count;
+        for (uint32_t i = 0, row = begin; i < count && first + i < capacity; i++) {
+            const uint32_t size = min((each + (i < more ? 1u : 0u)) * step, end - row);
+            tiles[first + i] = Tile{g, row, size, first, min(count, capacity - first), {}};
+            row += size;
         }
     }
     if (g == kMaxGroups - 1u) {
@@ -146,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, TcArgs a) {
     constexpr bool kRows = kForm != kByWeight;                         // the columns are rows of the group
     constexpr bool kADepth = kForm != kForward, kBDepth = kForm == kByWeight;
-    constexpr uint32_t kLanes = 128u * S::kHalves;
+    constexpr uint32_t kCtas = S::kCtas;
     extern __shared__ unsigned char smem_raw[];
     unsigned char *base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint64_t *full = reinterpret_cast<uint64_t *>(base + S::kBars);    // [kStages]
@@ -156,13 +256,14 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     uint64_t *item_full = acc_empty + 2;                               // [kSlots]
     uint64_t *item_empty = item_full + kSlots;                         // [kSlots]
     uint64_t *wanted = item_empty + kSlots;                            // [1] the loads come to an end
-    uint64_t *loaded = wanted + 1;                                     // [1] a last stage to be cleared is there
-    uint64_t *cleared = loaded + 1;                                    // [1] and its rows behind the group are zeros
-    uint64_t *done = cleared + 1;                                      // [1] every MMA issued has run
+    uint64_t *armed = wanted + 1;                                      // [kStages] a stage that has to be cleared is being loaded
+    uint64_t *cleared = armed + S::kStages;                            // [kStages] and its rows behind the group are zeros
+    uint64_t *done = cleared + S::kStages;                                      // [1] every MMA issued has run
     Item *items = reinterpret_cast<Item *>(done + 1);                  // [kSlots]
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(items + kSlots);
     volatile uint32_t *abort_flag = tmem_slot + 1;
     const uint32_t warp = warp_index(), lane = threadIdx.x % kWarp;
+    const uint32_t rank = kCtas == 2u ? cluster_rank() : 0u;           // the first of a pair issues its MMAs and draws its items
     // the extent along the lanes, the depth, and the output's row length
     const uint32_t lanes = kForm == kByInput ? a.k : a.n;
 
@@ -171,49 +272,60 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         for (uint32_t s = 0; s < S::kStages; s++) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
+            mbar_init(&armed[s], 1);
+            mbar_init(&cleared[s], 1);
         }
         for (uint32_t s = 0; s < 2u; s++) {
             mbar_init(&acc_full[s], 1);
-            mbar_init(&acc_empty[s], kResultWarps);
+            mbar_init(&acc_empty[s], kResultWarps * kCtas);
         }
         for (uint32_t s = 0; s < kSlots; s++) {
             mbar_init(&item_full[s], 1);
-            mbar_init(&item_empty[s], 2u + kResultWarps + (kRows ? 0u : 1u));
+            mbar_init(&item_empty[s], 1u + (1u + kResultWarps + (kRows ? 0u : 1u)) * kCtas);
         }
         mbar_init(wanted, 1);
-        mbar_init(loaded, 1);
-        mbar_init(cleared, 1);
         mbar_init(done, 1);
         fence_barrier_init();
         prefetch_tensormap(&map_a);
         prefetch_tensormap(&map_b);
     }
-    if (warp == 1u) {
-        tmem_alloc(tmem_slot, S::kTmem);
-        tmem_relinquish();
-    }
+    if (warp == 1u) alloc_tmem<kCtas>(tmem_slot, S::kTmem);
     tc_fence_before();
     __syncthreads();
+    if (kCtas == 2u) cluster_barrier();                                // the other block's barriers are there
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     pdl_wait();
 
+    // for arrivals that may come from the other block
+    auto wait_at = [&](uint64_t *bar, uint32_t phase) {
+        return kCtas == 2u ? wait_cluster(bar, phase, abort_flag) : mbar_wait(bar, phase, abort_flag);
+    };
     // Items one after the other, as every role reads them.
     uint32_t slot = 0u, slot_phase = 0u;
     auto next_item = [&](Item &it) {
-        if (!mbar_wait(&item_full[slot], slot_phase, abort_flag)) return false;
+        if (!wait_at(&item_full[slot], slot_phase)) return false;
         it = items[slot];
         return it.group != kNoItem;
     };
-    auto item_read = [&]() {                                           // by one thread
-        mbar_arrive(&item_empty[slot]);
+    // an arrival at a barrier of the first block: what this thread read is free
+    auto arrive_first = [&](uint64_t *bar) {
+        if (kCtas == 2u) arrive_relaxed_at(place_in(bar, 0u));
+        else mbar_arrive(bar);
     };
+    auto item_read = [&]() { arrive_first(&item_empty[slot]); };       // by one thread
     auto item_done = [&]() {
         if (++slot == kSlots) { slot = 0u; slot_phase ^= 1u; }
     };
     auto depth_of = [&](const Item &it) { return kForm == kForward ? a.k : kForm == kByInput ? a.n : it.rows; };
-    auto halves_of = [&](const Item &it) { return min(S::kHalves, (lanes - it.lane0 + 127u) / 128u); };
+    // by weight: the rows of the first block, so that those behind it are whole, and what is behind the group's rows is
+    // cleared while the products of the item before still run
+    auto first_rows = [](uint32_t depth) { return (depth - 1u) % kDepth + 1u; };
+    auto halves_of = [&](const Item &it) { return min(S::kHalves, (lanes - it.lane0 + S::kHalf - 1u) / S::kHalf); };
     auto columns_of = [&](const Item &it) { return kRows ? it.rows : min(S::kMaxN, a.k - it.column0); };
+    // of an MMA, and how many of them this block holds
+    auto steps_of = [&](uint32_t columns) { return (columns + S::kStep - 1u) / S::kStep * S::kStep; };
+    auto boxes_of = [&](uint32_t columns) { return (steps_of(columns) / kCtas + (kRows ? 31u : 63u)) / (kRows ? 32u : 64u); };
 
     // an accumulator half in registers is 128 of them: 2 x 128 x 232 + 128 x 40 are the 384 x 168 of the launch
     constexpr bool kShares = S::kMaxN == 256u;
@@ -228,38 +340,40 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 item_read();
                 item_done();
                 const uint32_t blocks = (depth_of(it) + kDepth - 1u) / kDepth, halves = halves_of(it), columns = columns_of(it);
-                const uint32_t b_boxes = kRows ? (columns + 31u) / 32u : (columns + 63u) / 64u;
+                const uint32_t b_boxes = boxes_of(columns), b_first = rank * (steps_of(columns) / kCtas);
                 const uint32_t bytes = halves * 2u * kBox + b_boxes * (kRows ? kBox / 2u : kBox);
-                if (blocks <= kAhead) mbar_arrive(wanted);
+                if (rank == 0u && blocks <= kAhead) mbar_arrive(wanted);
                 for (uint32_t kb = 0; kb < blocks; kb++) {
-                    if (kb + kAhead == blocks - 1u) mbar_arrive(wanted);
+                    if (rank == 0u && kb + kAhead == blocks - 1u) mbar_arrive(wanted);
                     if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag)) { ok = false; break; }
                     unsigned char *at = base + s * S::kStage, *bt = at + S::kA;
-                    const int32_t d = (int32_t)(kb * kDepth), r = (int32_t)it.row;
-                    mbar_arrive_expect_tx(&full[s], bytes);
+                    const int32_t d = (int32_t)(kRows || kb == 0u ? kb * kDepth : first_rows(it.rows) + (kb - 1u) * kDepth), r = (int32_t)it.row;
+                    if (rank == 0u) mbar_arrive_expect_tx(&full[s], bytes * kCtas);
+                    const uint32_t bar = kCtas == 2u ? place_in(&full[s], 0u) : smem_u32(&full[s]);
                     for (uint32_t h = 0; h < halves; h++) {
-                        const int32_t l = (int32_t)(it.lane0 + 128u * h);
+                        const int32_t l = (int32_t)(it.lane0 + S::kHalf * h + 128u * rank);
                         unsigned char *to = at + h * 2u * kBox;
                         if (kForm == kForward) {
-                            tma_load_3d(to, &map_a, &full[s], d, l, (int32_t)it.group);
+                            load_3d<kCtas>(to, &map_a, bar, d, l, (int32_t)it.group);
                         } else if (kForm == kByInput) {
-                            tma_load_3d(to, &map_a, &full[s], l, d, (int32_t)it.group);
-                            tma_load_3d(to + kBox, &map_a, &full[s], l + 64, d, (int32_t)it.group);
+                            load_3d<kCtas>(to, &map_a, bar, l, d, (int32_t)it.group);
+                            load_3d<kCtas>(to + kBox, &map_a, bar, l + 64, d, (int32_t)it.group);
                         } else {
-                            tma_load_2d(to, &map_a, &full[s], l, r + d);
-                            tma_load_2d(to + kBox, &map_a, &full[s], l + 64, r + d);
+                            load_2d<kCtas>(to, &map_a, bar, l, r + d);
+                            load_2d<kCtas>(to + kBox, &map_a, bar, l + 64, r + d);
                         }
                     }
                     for (uint32_t b = 0; b < b_boxes; b++) {
-                        if (kRows) tma_load_2d(bt + b * (kBox / 2u), &map_b, &full[s], d, r + (int32_t)(32u * b));
-                        else tma_load_2d(bt + b * kBox, &map_b, &full[s], (int32_t)(it.column0 + 64u * b), r + d);
+                        if (kRows) load_2d<kCtas>(bt + b * (kBox / 2u), &map_b, bar, d, r + (int32_t)(b_first + 32u * b));
+                        else load_2d<kCtas>(bt + b * kBox, &map_b, bar, (int32_t)(it.column0 + b_first + 64u * b), r + d);
                     }
+                    if (!kRows && kb == 0u && it.rows % 16u != 0u) mbar_arrive(&armed[s]);
                     issued++;
                     if (++s == S::kStages) { s = 0u; ph ^= 1u; }
                 }
             }
             pdl_trigger();                                             // the blocks of the next kernel may take places as these leave
-            if (*abort_flag != 0u) {                                   // nothing may land in a block that has left
+            if (rank == 0u && *abort_flag != 0u) {                     // nothing may land in a block that has left
                 for (uint32_t i = issued > S::kStages ? issued - S::kStages : 0u; i < issued; i++) {
                     mbar_drain(&full[i % S::kStages], (i / S::kStages) & 1u);
                 }
@@ -267,62 +381,76 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         }
     } else if (warp == 1u) {
         // ------------------------------------------------------------------------------- MMA
-        if (elect_one()) {
-            uint32_t s = 0u, ph = 0u, clear_phase = 0u, turn = 0u, acc_phase[2] = {1u, 1u};
+        if (rank == 0u && elect_one()) {
+            uint32_t s = 0u, ph = 0u, clear_phases = 0u, turn = 0u, acc_phase[2] = {1u, 1u};
             bool ok = true;
             Item it;
             while (ok && next_item(it)) {
                 item_read();
                 item_done();
                 const uint32_t depth = depth_of(it), blocks = (depth + kDepth - 1u) / kDepth, halves = halves_of(it);
-                const uint32_t columns = columns_of(it);
-                const uint32_t idesc = idesc_of((columns + 15u) & ~15u, kADepth, kBDepth);
-                for (uint32_t kb = 0; ok && kb < blocks; kb++) {
-                    const bool last = kb + 1u == blocks;
-                    if (!mbar_wait(&full[s], ph, abort_flag)) { ok = false; break; }
-                    // by weight: only the steps of 16 that have rows, the last of them with zeros behind the group
-                    const uint32_t steps = kRows || !last ? 4u : (depth - kb * kDepth + 15u) / 16u;
-                    const bool clear = !kRows && last && depth % 16u != 0u;
-                    if (clear) mbar_arrive(loaded);
-                    const uint32_t at = smem_u32(base + s * S::kStage);
+                const uint32_t idesc = idesc_of(S::kHalf, steps_of(columns_of(it)), kADepth, kBDepth);
+                // by weight: the first block has what does not fill one, in the steps of 16 that it takes
+                const uint32_t first_steps = kRows ? 4u : (first_rows(depth) + 15u) / 16u;
+                auto free = [&](uint32_t acc) {
+                    const bool is = wait_at(&acc_empty[acc], acc_phase[acc]);
+                    acc_phase[acc] ^= 1u;
+                    return is;
+                };
+                // a stage's products for one half of the lanes
+                auto half = [&](uint32_t stage, uint32_t kb, uint32_t h, uint32_t acc) {
+                    const uint32_t at = smem_u32(base + stage * S::kStage), ah = at + h * 2u * kBox, d = tmem + acc * S::kMaxN;
+                    const uint64_t da = kADepth ? make_desc_by_depth(ah) : make_desc_sw128(ah);
                     const uint64_t db = kBDepth ? make_desc_by_depth(at + S::kA) : make_desc_sw128(at + S::kA);
-                    for (uint32_t h = 0; h < halves; h++) {
-                        const uint32_t acc = S::kHalves == 2u ? h : turn;
-                        if (kb == 0u) {
-                            if (!mbar_wait(&acc_empty[acc], acc_phase[acc], abort_flag)) { ok = false; break; }
-                            acc_phase[acc] ^= 1u;
-                        }
-                        if (clear && h == 0u) {
-                            if (!mbar_wait(cleared, clear_phase, abort_flag)) { ok = false; break; }
-                            clear_phase ^= 1u;
-                        }
-                        tc_fence_after();
-                        const uint32_t ah = at + h * 2u * kBox, d = tmem + acc * S::kMaxN;
-                        const uint64_t da = kADepth ? make_desc_by_depth(ah) : make_desc_sw128(ah);
+                    tc_fence_after();
+                    const uint32_t steps = kb == 0u ? first_steps : 4u;
 #pragma unroll
-                        for (uint32_t j = 0; j < 4u; j++) {            // 16 of the depth: 32 bytes on, or 16 rows of 128
-                            if (j < steps) {
-                                mma_f16_ss(d, da + (kADepth ? 128u : 2u) * j, db + (kBDepth ? 128u : 2u) * j, idesc, kb != 0u || j != 0u);
-                            }
-                        }
-                        if (last) mma_commit(&acc_full[acc]);
+                    for (uint32_t j = 0; j < 4u; j++) {                // 16 of the depth: 32 bytes on, or 16 rows of 128
+                        if (j < steps) mma<kCtas>(d, da + (kADepth ? 128u : 2u) * j, db + (kBDepth ? 128u : 2u) * j, idesc, kb != 0u || j != 0u);
                     }
-                    if (!ok) break;
-                    mma_commit(&empty[s]);
+                    if (kb + 1u == blocks) commit<kCtas>(&acc_full[acc]);
+                };
+                uint32_t ahead = 0u;                                   // blocks 1 .. ahead have run for the first half
+                for (uint32_t kb = 0; ok && kb < blocks; kb++) {
+                    const uint32_t acc = S::kHalves == 2u ? 0u : turn;
+                    if (kb == 0u || kb > ahead) {
+                        ok = mbar_wait(&full[s], ph, abort_flag);
+                        if (!kRows && ok && kb == 0u && depth % 16u != 0u) {
+                            ok = mbar_wait(&cleared[s], (clear_phases >> s) & 1u, abort_flag);
+                            clear_phases ^= 1u << s;
+                        }
+                        if (!ok || (kb == 0u && !(ok = free(acc)))) break;
+                        half(s, kb, 0u, acc);
+                    }
+                    if (S::kHalves == 2u && halves == 2u) {
+                        if (kb == 0u) {
+                            // While the second accumulator is read (its results wait for the first's to be stored) the first half
+                            // runs ahead, as far as the ring reaches.
+                            uint32_t s2 = s, ph2 = ph;
+                            while (ok && ahead + 1u < min(S::kStages, blocks) && !mbar_test(&acc_empty[1], acc_phase[1])) {
+                                if (++s2 == S::kStages) { s2 = 0u; ph2 ^= 1u; }
+                                ok = mbar_wait(&full[s2], ph2, abort_flag);
+                                if (ok) half(s2, ++ahead, 0u, 0u);
+                            }
+                            if (!ok || !(ok = free(1u))) break;
+                        }
+                        half(s, kb, 1u, 1u);
+                    }
+                    commit<kCtas>(&empty[s]);
                     if (++s == S::kStages) { s = 0u; ph ^= 1u; }
                 }
                 if (S::kHalves == 1u && blocks != 0u) turn ^= 1u;
             }
             if (*abort_flag != 0u) {
-                mma_commit(done);
+                commit<kCtas>(done);
                 mbar_drain(done, 0u);
             }
         }
     } else if (warp == 2u) {
         // ------------------------------------------------- items, each shortly before its loads
-        if (elect_one()) {
+        if (rank == 0u && elect_one()) {
             const uint32_t total = kRows ? a.plan->tiles * a.lane_tiles : a.groups * a.lane_tiles * a.column_tiles;
-            uint32_t w = blockIdx.x, want_phase = 0u;
+            uint32_t w = blockIdx.x / kCtas, want_phase = 0u;
             for (;;) {
                 Item it{kNoItem, 0u, 0u, 0u, 0u};
                 if (w < total) {
@@ -330,40 +458,51 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                         const Tile of = a.tiles[w / a.lane_tiles];
                         const uint32_t local = w - of.first * a.lane_tiles, t = local % of.count;
                         const Tile tile = t + of.first == w / a.lane_tiles ? of : a.tiles[of.first + t];
-                        it = {tile.group, tile.row, tile.rows, local / of.count * kLanes, 0u};
+                        it = {tile.group, tile.row, tile.rows, local / of.count * S::kLanes, 0u};
                     } else {
                         const uint32_t per = a.lane_tiles * a.column_tiles, g = w / per, at = w - g * per;
                         uint32_t begin, end;
                         group_rows(a.offsets, g, a.rows, begin, end);
-                        it = {g, begin, end - begin, at / a.column_tiles * kLanes, at % a.column_tiles * S::kMaxN};
+                        it = {g, begin, end - begin, at / a.column_tiles * S::kLanes, at % a.column_tiles * S::kMaxN};
                     }
                 }
-                if (!mbar_wait(&item_empty[slot], slot_phase ^ 1u, abort_flag)) break;
+                if (!wait_at(&item_empty[slot], slot_phase ^ 1u)) break;
                 items[slot] = it;
                 mbar_arrive(&item_full[slot]);
+                if (kCtas == 2u) {
+                    const uint32_t to = place_in(&items[slot], 1u);
+                    store_at(to, it.group);
+                    store_at(to + 4u, it.row);
+                    store_at(to + 8u, it.rows);
+                    store_at(to + 12u, it.lane0);
+                    store_at(to + 16u, it.column0);
+                    arrive_at(place_in(&item_full[slot], 1u));
+                }
                 item_done();
                 if (it.group == kNoItem || !mbar_wait(wanted, want_phase, abort_flag)) break;
                 want_phase ^= 1u;
-                w = gridDim.x + atomicAdd(&a.plan->counter, 1u);
+                w = gridDim.x / kCtas + atomicAdd(&a.plan->counter, 1u);
             }
         }
     } else if (warp == 3u) {
         if (!kRows) {
-            // ---------------------------------------------------- rows behind the group in its last stage
-            uint32_t used = 0u, load_phase = 0u;                       // stages so far
+            // --------------------------------------------------- rows behind the group in its first block
+            static_assert(kRows || kCtas == 1u, "a block clears and multiplies its own shared memory");
+            uint32_t used = 0u, phases = 0u;                           // stages so far; of armed[], a bit each
             Item it;
             while (next_item(it)) {
                 __syncwarp();
                 if (lane == 0u) item_read();
                 item_done();
-                const uint32_t blocks = (it.rows + kDepth - 1u) / kDepth;
-                used += blocks;
+                const uint32_t s = used % S::kStages, ph = (used / S::kStages) & 1u;
+                used += (it.rows + kDepth - 1u) / kDepth;
                 if (it.rows % 16u == 0u) continue;
-                if (!mbar_wait(loaded, load_phase, abort_flag)) break;
-                load_phase ^= 1u;
-                unsigned char *at = base + (used - 1u) % S::kStages * S::kStage;
-                const uint32_t a_boxes = halves_of(it) * 2u, boxes = a_boxes + (columns_of(it) + 63u) / 64u;
-                const uint32_t from = it.rows % kDepth, rows = (16u - from % 16u) % 16u;
+                // once the load is under way the stage's barrier is in the phase that this one's parity names
+                if (!mbar_wait(&armed[s], (phases >> s) & 1u, abort_flag) || !mbar_wait(&full[s], ph, abort_flag)) break;
+                phases ^= 1u << s;
+                unsigned char *at = base + s * S::kStage;
+                const uint32_t a_boxes = halves_of(it) * 2u, boxes = a_boxes + boxes_of(columns_of(it));
+                const uint32_t from = it.rows % kDepth, rows = 16u - from % 16u;
                 for (uint32_t e = lane; e < boxes * rows * 8u; e += kWarp) {
                     const uint32_t box = e / (rows * 8u), in = e - box * rows * 8u;
                     unsigned char *to = box < a_boxes ? at + box * kBox : at + S::kA + (box - a_boxes) * kBox;
@@ -371,7 +510,7 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 }
                 fence_proxy_async();
                 __syncwarp();
-                if (lane == 0u) mbar_arrive(cleared);
+                if (lane == 0u) mbar_arrive(&cleared[s]);
             }
         }
     } else {
@@ -406,7 +545,7 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     for (uint32_t c = 0; c < kChunks; c++) k3::fp8::tmem_ld_wait_for(v[c]);
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0u) mbar_arrive(&acc_empty[acc]);
+                    if (lane == 0u) arrive_first(&acc_empty[acc]);
                 } else {
 #pragma unroll
                     for (uint32_t c = 0; c < kChunks; c++) {
@@ -414,7 +553,7 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                         for (uint32_t i = 0; i < 32u; i++) v[c][i] = 0u;
                     }
                 }
-                const uint32_t lane0 = it.lane0 + 128u * h + 32u * q;  // this warp's first lane
+                const uint32_t lane0 = it.lane0 + S::kHalf * h + 128u * rank + 32u * q;      // this warp's first lane
 #pragma unroll
                 for (uint32_t c = 0; c < kChunks; c++) {
                     const uint32_t column = (2u * c + part) * 32u;
@@ -453,7 +592,7 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                         const uint32_t r = i * (32u / kUnits) + lane / kUnits, u = lane % kUnits, e = u * (kF32 ? 4u : 8u);
                         const uint4 x = *reinterpret_cast<const uint4 *>(unit(r, u));
                         uint64_t to;
-                        if (kRows) {
+                        if (kRows) {                                   // a pair's second block may have no lane that exists
                             if (column + r >= it.rows || lane0 + e >= lanes) continue;
                             to = (uint64_t)(it.row + column + r) * row_length + lane0 + e;
                         } else {
@@ -481,10 +620,11 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
 
     tc_fence_before();
     __syncthreads();
+    if (kCtas == 2u) cluster_barrier();                                // nobody leaves while the other may signal here
     if (threadIdx.x == 0 && *abort_flag != 0u) atomicExch(&g_grouped_bf16_status, 1u);
     if (warp == 1u) {
         tc_fence_after();
-        tmem_dealloc(tmem, S::kTmem);
+        free_tmem<kCtas>(tmem, S::kTmem);
     }
 }
 
@@ -506,8 +646,9 @@ constexpr uint64_t plan_bytes(uint32_t tiles) { return sizeof(Plan) + (uint64_t)
 uint32_t most_tiles(uint32_t rows, uint32_t groups, uint32_t max_n) { return rows / max_n + std::min(rows, groups); }
 
 constexpr uint32_t kFewRows = 64;
-using Wide = Shape<2, 256, 3>;
-using Few = Shape<1, kFewRows, 8>;
+using Wide = Shape<2, 2, 256, 4>;
+using WideWeight = Shape<1, 2, 256, 3>;
+using Few = Shape<1, 1, kFewRows, 8>;
 
 template <int kForm, bool kF32, typename S>
 bool launch(const Product &p, cudaStream_t stream) {
@@ -523,13 +664,15 @@ bool launch(const Product &p, cudaStream_t stream) {
     }
     const uint32_t lanes = kForm == kByInput ? p.k : p.n, tiles = most_tiles(p.rows, p.groups, S::kMaxN);
     TcArgs a{p.out, p.offsets, (Plan *)p.workspace, (const Tile *)((Plan *)p.workspace + 1), p.rows, p.groups, p.n, p.k,
-             (lanes + 128u * S::kHalves - 1u) / (128u * S::kHalves), (p.k + S::kMaxN - 1u) / S::kMaxN, p.accumulate};
+             (lanes + S::kLanes - 1u) / S::kLanes, (p.k + S::kMaxN - 1u) / S::kMaxN, p.accumulate};
     const uint64_t items = kRows ? (uint64_t)tiles * a.lane_tiles : (uint64_t)p.groups * a.lane_tiles * a.column_tiles;
     if (items > 0x7fffffffull || !set_max_dynamic_smem((const void *)kernel, S::kBytes)) return false;
     const bool planned = kRows ? launch_chained(grouped_plan_kernel, 1, kMaxGroups, 0, stream, a.plan, (Tile *)a.tiles, p.offsets, p.rows, p.groups,
-                                                S::kMaxN, tiles)
+                                                S::kMaxN, S::kStep, tiles)
                                : launch_chained(grouped_counter_kernel, 1, 1, 0, stream, a.plan);
-    return planned && launch_chained(kernel, (uint32_t)std::min<uint64_t>(items, sm_count()), kThreads, S::kBytes, stream, ma, mb, a);
+    const uint32_t places = (uint32_t)sm_count() / S::kCtas;
+    return planned && launch_chained_cluster(kernel, (uint32_t)std::min<uint64_t>(items, places) * S::kCtas, kThreads, dim3(S::kCtas, 1, 1), S::kBytes,
+                                             stream, ma, mb, a);
 }
 
 template <int kForm, typename S>
@@ -542,7 +685,7 @@ bool launch_typed(const Product &p, cudaStream_t stream) {
 uint64_t k3::gb::tc_workspace_bytes(uint32_t rows, uint32_t groups) { return plan_bytes(most_tiles(rows, groups, kFewRows)); }
 
 bool k3::gb::product_tc(const Product &p, cudaStream_t stream) {
-    if (p.form == kByWeight) return launch_typed<kByWeight, Wide>(p, stream);
+    if (p.form == kByWeight) return launch_typed<kByWeight, WideWeight>(p, stream);
     const bool few = p.rows <= 24u * std::min(p.rows, p.groups);
     if (p.form == kForward) return few ? launch_typed<kForward, Few>(p, stream) : launch_typed<kForward, Wide>(p, stream);
     return few ? launch_typed<kByInput, Few>(p, stream) : launch_typed<kByInput, Wide>(p, stream);
