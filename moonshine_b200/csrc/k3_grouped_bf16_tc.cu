@@ -24,6 +24,7 @@
 #include "k3_grouped_bf16.h"
 
 #include <algorithm>
+#include <cmath>
 
 using namespace k3;
 using namespace k3::tc;
@@ -39,6 +40,7 @@ namespace {
 constexpr uint32_t kThreads = 384, kResultWarps = 8, kDepth = 64;      // depth of a stage: 128 bytes of bf16
 constexpr uint32_t kBox = 64 * kDepth * 2;                             // 8 KB: 64 x 64 elements
 constexpr uint32_t kSlots = 2;                                         // items that are known ahead
+constexpr uint32_t kMaxParts = 8;                                      // of an item's depth: the portable cluster
 constexpr uint32_t kAhead = 6;                                         // stages before an item's last in which the next is drawn
 constexpr uint32_t kNoItem = 0xffffffffu;
 
@@ -53,8 +55,9 @@ struct Tile {
     uint32_t group, row, rows, first, count, pad[3];                   // first .. first + count - 1: the group's tiles
 };
 
-template <uint32_t kCtas_, uint32_t kHalves_, uint32_t kMaxN_, uint32_t kStages_>
+template <uint32_t kCtas_, uint32_t kHalves_, uint32_t kMaxN_, uint32_t kStages_, bool kSplit_ = false>
 struct Shape {
+    static constexpr bool kSplit = kSplit_;
     static constexpr uint32_t kCtas = kCtas_, kHalves = kHalves_, kMaxN = kMaxN_, kStages = kStages_;
     static constexpr uint32_t kHalf = 128u * kCtas, kLanes = kHalf * kHalves;
     static constexpr uint32_t kStep = 16u * kCtas;                     // of an MMA's columns
@@ -63,6 +66,7 @@ struct Shape {
     static constexpr uint32_t kBars = kStore + kResultWarps * 4096u;
     static constexpr uint32_t kBytes = kBars + 512u + 1024u;           // the last: alignment
     static constexpr uint32_t kTmem = 2u * kMaxN;
+    static_assert(!kSplit || (kCtas == 1u && kLanes * kMaxN * 4u <= kResultWarps * 4096u), "a part's sums take the stores' place");
     static_assert(kBytes <= 232448u && kTmem <= 512u && (kTmem & (kTmem - 1u)) == 0u, "");
 };
 
@@ -70,7 +74,7 @@ struct TcArgs {
     void *out;
     const uint32_t *offsets;
     Plan *plan;
-    const Tile *tiles;
+    Tile *tiles;
     uint32_t rows, groups, n, k;
     uint32_t lane_tiles;                                               // items side by side along the lanes
     uint32_t column_tiles;                                             // by weight: and along the columns
@@ -317,6 +321,13 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     auto item_done = [&]() {
         if (++slot == kSlots) { slot = 0u; slot_phase ^= 1u; }
     };
+    // blocks of the depth: all, or the part of a cluster's block
+    const uint32_t split = S::kSplit ? cluster_rank() : 0u, splits = S::kSplit ? cluster_size() : 1u;
+    auto range_of = [&](uint32_t blocks, uint32_t &begin, uint32_t &end) {
+        const uint32_t each = (blocks + splits - 1u) / splits;
+        begin = min(split * each, blocks);
+        end = min(begin + each, blocks);
+    };
     auto depth_of = [&](const Item &it) { return kForm == kForward ? a.k : kForm == kByInput ? a.n : it.rows; };
     // by weight: the rows of the first block, so that those behind it are whole, and what is behind the group's rows is
     // cleared while the products of the item before still run
@@ -339,12 +350,14 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             while (ok && next_item(it)) {
                 item_read();
                 item_done();
-                const uint32_t blocks = (depth_of(it) + kDepth - 1u) / kDepth, halves = halves_of(it), columns = columns_of(it);
+                const uint32_t halves = halves_of(it), columns = columns_of(it);
+                uint32_t begin, end;
+                range_of((depth_of(it) + kDepth - 1u) / kDepth, begin, end);
                 const uint32_t b_boxes = boxes_of(columns), b_first = rank * (steps_of(columns) / kCtas);
                 const uint32_t bytes = halves * 2u * kBox + b_boxes * (kRows ? kBox / 2u : kBox);
-                if (rank == 0u && blocks <= kAhead) mbar_arrive(wanted);
-                for (uint32_t kb = 0; kb < blocks; kb++) {
-                    if (rank == 0u && kb + kAhead == blocks - 1u) mbar_arrive(wanted);
+                if (rank == 0u && end - begin <= kAhead) mbar_arrive(wanted);
+                for (uint32_t kb = begin; kb < end; kb++) {
+                    if (rank == 0u && kb + kAhead == end - 1u) mbar_arrive(wanted);
                     if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag)) { ok = false; break; }
                     unsigned char *at = base + s * S::kStage, *bt = at + S::kA;
                     const int32_t d = (int32_t)(kRows || kb == 0u ? kb * kDepth : first_rows(it.rows) + (kb - 1u) * kDepth), r = (int32_t)it.row;
@@ -388,7 +401,9 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             while (ok && next_item(it)) {
                 item_read();
                 item_done();
-                const uint32_t depth = depth_of(it), blocks = (depth + kDepth - 1u) / kDepth, halves = halves_of(it);
+                const uint32_t depth = depth_of(it), halves = halves_of(it);
+                uint32_t begin, end;
+                range_of((depth + kDepth - 1u) / kDepth, begin, end);
                 const uint32_t idesc = idesc_of(S::kHalf, steps_of(columns_of(it)), kADepth, kBDepth);
                 // by weight: the first block has what does not fill one, in the steps of 16 that it takes
                 const uint32_t first_steps = kRows ? 4u : (first_rows(depth) + 15u) / 16u;
@@ -406,28 +421,28 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     const uint32_t steps = kb == 0u ? first_steps : 4u;
 #pragma unroll
                     for (uint32_t j = 0; j < 4u; j++) {                // 16 of the depth: 32 bytes on, or 16 rows of 128
-                        if (j < steps) mma<kCtas>(d, da + (kADepth ? 128u : 2u) * j, db + (kBDepth ? 128u : 2u) * j, idesc, kb != 0u || j != 0u);
+                        if (j < steps) mma<kCtas>(d, da + (kADepth ? 128u : 2u) * j, db + (kBDepth ? 128u : 2u) * j, idesc, kb != begin || j != 0u);
                     }
-                    if (kb + 1u == blocks) commit<kCtas>(&acc_full[acc]);
+                    if (kb + 1u == end) commit<kCtas>(&acc_full[acc]);
                 };
-                uint32_t ahead = 0u;                                   // blocks 1 .. ahead have run for the first half
-                for (uint32_t kb = 0; ok && kb < blocks; kb++) {
+                uint32_t ahead = begin;                                // blocks up to this one have run for the first half
+                for (uint32_t kb = begin; ok && kb < end; kb++) {
                     const uint32_t acc = S::kHalves == 2u ? 0u : turn;
-                    if (kb == 0u || kb > ahead) {
+                    if (kb == begin || kb > ahead) {
                         ok = mbar_wait(&full[s], ph, abort_flag);
                         if (!kRows && ok && kb == 0u && depth % 16u != 0u) {
                             ok = mbar_wait(&cleared[s], (clear_phases >> s) & 1u, abort_flag);
                             clear_phases ^= 1u << s;
                         }
-                        if (!ok || (kb == 0u && !(ok = free(acc)))) break;
+                        if (!ok || (kb == begin && !(ok = free(acc)))) break;
                         half(s, kb, 0u, acc);
                     }
                     if (S::kHalves == 2u && halves == 2u) {
-                        if (kb == 0u) {
+                        if (kb == begin) {
                             // While the second accumulator is read (its results wait for the first's to be stored) the first half
                             // runs ahead, as far as the ring reaches.
                             uint32_t s2 = s, ph2 = ph;
-                            while (ok && ahead + 1u < min(S::kStages, blocks) && !mbar_test(&acc_empty[1], acc_phase[1])) {
+                            while (ok && ahead + 1u < min(begin + S::kStages, end) && !mbar_test(&acc_empty[1], acc_phase[1])) {
                                 if (++s2 == S::kStages) { s2 = 0u; ph2 ^= 1u; }
                                 ok = mbar_wait(&full[s2], ph2, abort_flag);
                                 if (ok) half(s2, ++ahead, 0u, 0u);
@@ -439,7 +454,7 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     commit<kCtas>(&empty[s]);
                     if (++s == S::kStages) { s = 0u; ph ^= 1u; }
                 }
-                if (S::kHalves == 1u && blocks != 0u) turn ^= 1u;
+                if (S::kHalves == 1u && begin != end) turn ^= 1u;
             }
             if (*abort_flag != 0u) {
                 commit<kCtas>(done);
@@ -450,7 +465,7 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         // ------------------------------------------------- items, each shortly before its loads
         if (rank == 0u && elect_one()) {
             const uint32_t total = kRows ? a.plan->tiles * a.lane_tiles : a.groups * a.lane_tiles * a.column_tiles;
-            uint32_t w = blockIdx.x / kCtas, want_phase = 0u;
+            uint32_t w = blockIdx.x / (S::kSplit ? splits : kCtas), want_phase = 0u;
             for (;;) {
                 Item it{kNoItem, 0u, 0u, 0u, 0u};
                 if (w < total) {
@@ -481,7 +496,7 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 item_done();
                 if (it.group == kNoItem || !mbar_wait(wanted, want_phase, abort_flag)) break;
                 want_phase ^= 1u;
-                w = gridDim.x / kCtas + atomicAdd(&a.plan->counter, 1u);
+                w = S::kSplit ? total : gridDim.x / kCtas + atomicAdd(&a.plan->counter, 1u);
             }
         }
     } else if (warp == 3u) {
@@ -496,7 +511,7 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 item_done();
                 const uint32_t s = used % S::kStages, ph = (used / S::kStages) & 1u;
                 used += (it.rows + kDepth - 1u) / kDepth;
-                if (it.rows % 16u == 0u) continue;
+                if (it.rows % 16u == 0u || split != 0u) continue;      // the first block is the first part's
                 // once the load is under way the stage's barrier is in the phase that this one's parity names
                 if (!mbar_wait(&armed[s], (phases >> s) & 1u, abort_flag) || !mbar_wait(&full[s], ph, abort_flag)) break;
                 phases ^= 1u << s;
@@ -527,8 +542,10 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             if (lane == 0u) item_read();
             item_done();
             const uint32_t halves = halves_of(it), columns = columns_of(it);
-            const bool nothing = depth_of(it) == 0u;                   // by weight: a group without rows
-            if (nothing && a.accumulate) continue;
+            uint32_t begin, end;
+            range_of((depth_of(it) + kDepth - 1u) / kDepth, begin, end);
+            const bool nothing = begin == end;                         // by weight: a group without rows; a part with no blocks
+            if (!S::kSplit && nothing && a.accumulate) continue;
             for (uint32_t h = 0; h < halves; h++) {
                 const uint32_t acc = S::kHalves == 2u ? h : turn;
                 constexpr uint32_t kChunks = S::kMaxN / 64u;           // of 32 columns, for this warp
@@ -552,6 +569,23 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
 #pragma unroll
                         for (uint32_t i = 0; i < 32u; i++) v[c][i] = 0u;
                     }
+                }
+                if (S::kSplit) {
+                    // this part's sums where the others read them: of a row of the group [column][128], by weight [128][columns]
+                    // in units of 16 bytes permuted by the lane
+                    float *sums = reinterpret_cast<float *>(base + S::kStore);
+                    const uint32_t at = 32u * q + lane;
+                    if (kRows) {
+#pragma unroll
+                        for (uint32_t i = 0; i < 32u; i++) sums[(part * 32u + i) * 128u + at] = __uint_as_float(v[0][i]);
+                    } else {
+#pragma unroll
+                        for (uint32_t u = 0; u < 8u; u++) {
+                            reinterpret_cast<uint4 *>(sums)[at * (S::kMaxN / 4u) + ((part * 8u + u) ^ (at & 7u))] =
+                                make_uint4(v[0][4u * u], v[0][4u * u + 1u], v[0][4u * u + 2u], v[0][4u * u + 3u]);
+                        }
+                    }
+                    continue;
                 }
                 // 32 x 32 at a time through shared memory: rows of the output, units of 16 bytes, permuted by the row.  This
                 // thread then stores a unit of every kApart-th row; where that goes is worked out once per half (with the
@@ -617,6 +651,43 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         }
     }
 
+    if (S::kSplit) {
+        // the parts' sums in ascending order of the depth; each block adds its share of the item
+        __syncwarp();
+        cluster_barrier();
+        const Item it = items[0];
+        if (*abort_flag == 0u && it.group != kNoItem) {
+            const uint32_t columns = columns_of(it), units = kRows ? 32u : (columns + 3u) / 4u;
+            const uint32_t all = (kRows ? columns : 128u) * units, share = (all + splits - 1u) / splits, past = min(all, (split + 1u) * share);
+            for (uint32_t e = split * share + threadIdx.x; e < past; e += kThreads) {
+                const uint32_t major = e / units, u = e - major * units;             // of the group [column], by weight [lane]
+                const uint32_t row = kRows ? it.row + major : it.lane0 + major, column = (kRows ? it.lane0 : it.column0) + 4u * u;
+                if (kRows ? column >= lanes : row >= a.n) continue;
+                const float *from = reinterpret_cast<const float *>(base + S::kStore) +
+                                    (kRows ? major * 128u + 4u * u : major * S::kMaxN + 4u * (u ^ (major & 7u)));
+                float4 x[kMaxParts];                                   // all under way before the first is added
+#pragma unroll
+                for (uint32_t r = 0; r < kMaxParts; r++) {
+                    if (r < splits) x[r] = cluster_load4(from, r);
+                }
+                float4 sum = x[0];
+#pragma unroll
+                for (uint32_t r = 1; r < kMaxParts; r++) {
+                    if (r < splits) sum = make_float4(sum.x + x[r].x, sum.y + x[r].y, sum.z + x[r].z, sum.w + x[r].w);
+                }
+                const uint64_t to = ((kRows ? 0u : (uint64_t)it.group * a.n) + row) * (kRows ? lanes : a.k) + column;
+                if (kF32) {
+                    float4 *out = reinterpret_cast<float4 *>((float *)a.out + to);
+                    if (a.accumulate) sum = make_float4(out->x + sum.x, out->y + sum.y, out->z + sum.z, out->w + sum.w);
+                    *out = sum;
+                } else {
+                    *reinterpret_cast<uint2 *>((uint16_t *)a.out + to) = make_uint2(bf16x2(sum.x, sum.y), bf16x2(sum.z, sum.w));
+                }
+            }
+        }
+        __syncwarp();
+        cluster_barrier();                                             // nobody leaves while its sums are read
+    }
     tc_fence_before();
     __syncthreads();
     if (kCtas == 2u) cluster_barrier();                                // nobody leaves while the other may signal here
@@ -642,15 +713,28 @@ bool make_map(CUtensorMap *map, const void *p, uint32_t x, uint64_t y, uint32_t 
 
 constexpr uint64_t plan_bytes(uint32_t tiles) { return sizeof(Plan) + (uint64_t)tiles * sizeof(Tile); }
 // The most row tiles of up to max_n that the groups can have.
-uint32_t most_tiles(uint32_t rows, uint32_t groups, uint32_t max_n) { return rows / max_n + std::min(rows, groups); }
+uint32_t most_tiles(uint32_t rows, uint32_t groups, uint32_t max_n) {
+    return (uint32_t)((rows + (uint64_t)(max_n - 1u) * std::min(rows, groups)) / max_n);
+}
 
 constexpr uint32_t kFewRows = 64;
 using Wide = Shape<2, 2, 256, 4>;
-using WideWeight = Shape<1, 2, 256, 3>;
+using Square = Shape<2, 1, 256, 6>;
+using Middle = Shape<1, 1, 128, 6>;
 using Few = Shape<1, 1, kFewRows, 8>;
+using FewSplit = Shape<1, 1, kFewRows, 8, true>;
+using WideWeight = Shape<1, 2, 256, 3>;
 
+// Items of a call, at most.
+template <int kForm, typename S>
+uint64_t items_of(const Product &p) {
+    const uint64_t lanes = ((kForm == kByInput ? p.k : p.n) + S::kLanes - 1u) / S::kLanes;
+    return lanes * (kForm == kByWeight ? (uint64_t)p.groups * ((p.k + S::kMaxN - 1u) / S::kMaxN) : most_tiles(p.rows, p.groups, S::kMaxN));
+}
+
+// parts: blocks that share an item's depth (S::kSplit)
 template <int kForm, bool kF32, typename S>
-bool launch(const Product &p, cudaStream_t stream) {
+bool launch(const Product &p, uint32_t parts, cudaStream_t stream) {
     constexpr bool kRows = kForm != kByWeight;
     auto kernel = grouped_bf16_kernel<kForm, kF32, S>;
     CUtensorMap ma, mb;
@@ -662,21 +746,92 @@ bool launch(const Product &p, cudaStream_t stream) {
         if (!make_map(&ma, p.a, p.n, p.rows, 0u, 64u) || !make_map(&mb, p.b, p.k, p.rows, 0u, 64u)) return false;
     }
     const uint32_t lanes = kForm == kByInput ? p.k : p.n, tiles = most_tiles(p.rows, p.groups, S::kMaxN);
-    TcArgs a{p.out, p.offsets, (Plan *)p.workspace, (const Tile *)((Plan *)p.workspace + 1), p.rows, p.groups, p.n, p.k,
-             (lanes + S::kLanes - 1u) / S::kLanes, (p.k + S::kMaxN - 1u) / S::kMaxN, p.accumulate};
-    const uint64_t items = kRows ? (uint64_t)tiles * a.lane_tiles : (uint64_t)p.groups * a.lane_tiles * a.column_tiles;
-    if (items > 0x7fffffffull || !set_max_dynamic_smem((const void *)kernel, S::kBytes)) return false;
-    const bool planned = kRows ? launch_chained(grouped_plan_kernel, 1, kMaxGroups, 0, stream, a.plan, (Tile *)a.tiles, p.offsets, p.rows, p.groups,
+    const TcArgs a{p.out, p.offsets, (Plan *)p.workspace, (Tile *)((Plan *)p.workspace + 1), p.rows, p.groups, p.n, p.k,
+                   (lanes + S::kLanes - 1u) / S::kLanes, (p.k + S::kMaxN - 1u) / S::kMaxN, p.accumulate};
+    const uint64_t items = items_of<kForm, S>(p), places = S::kSplit ? items : (uint64_t)sm_count() / S::kCtas;
+    if (items * parts > 0x7fffffffull || !set_max_dynamic_smem((const void *)kernel, S::kBytes)) return false;
+    const uint32_t cluster = S::kSplit ? parts : S::kCtas;
+    const bool planned = kRows ? launch_chained(grouped_plan_kernel, 1, kMaxGroups, 0, stream, a.plan, a.tiles, p.offsets, p.rows, p.groups,
                                                 S::kMaxN, S::kStep, tiles)
-                               : launch_chained(grouped_counter_kernel, 1, 1, 0, stream, a.plan);
-    const uint32_t places = (uint32_t)sm_count() / S::kCtas;
-    return planned && launch_chained_cluster(kernel, (uint32_t)std::min<uint64_t>(items, places) * S::kCtas, kThreads, dim3(S::kCtas, 1, 1), S::kBytes,
-                                             stream, ma, mb, a);
+                               : S::kSplit || launch_chained(grouped_counter_kernel, 1, 1, 0, stream, a.plan);
+    return planned && launch_chained_cluster(kernel, (uint32_t)std::min(items, places) * cluster, kThreads, dim3(cluster, 1, 1), S::kBytes, stream,
+                                             ma, mb, a);
 }
 
 template <int kForm, typename S>
-bool launch_typed(const Product &p, cudaStream_t stream) {
-    return p.f32 ? launch<kForm, true, S>(p, stream) : launch<kForm, false, S>(p, stream);
+bool launch_typed(const Product &p, cudaStream_t stream, uint32_t parts = 1u) {
+    return p.f32 ? launch<kForm, true, S>(p, parts, stream) : launch<kForm, false, S>(p, parts, stream);
+}
+
+// Which shape.  The host knows the rows and groups of a call, not how they are spread, so it takes every group that can
+// have rows to have equally many, and of the shapes the one with the shortest time by what was measured on a B200 (us, and
+// ns per stage of 64 of the depth): `fixed` for a call, `item` for an item's results, and per stage base + column x columns,
+// alone in a single round of items, full where the SMs share memory and power over several.  Over 192 calls of 1 to 64 groups
+// of 1 to 2048 rows at 2048 x 7168, 7168 x 2048, 2048 x 1024 and 512 x 512 the shape that this takes is 0.7 % from the best
+// on average, 26 % at worst; always taking the largest, 66 %.  What each is for:
+//   Few      up to 64 rows per group: bound by the matrices' bytes, 6.4 TB/s at 64 groups of 8 rows of 2048 x 7168 (274 us; Middle 294)
+//   Middle   up to 128, or too few items for larger ones (4 groups of 256 rows: 35 us; Few 53, Square 43)
+//   Square   pairs of blocks with two accumulators (16 groups of 256 rows of 7168 x 2048: 107 us; Wide 115, Middle 134)
+//   Wide     least traffic per product, so least power, which bounds large calls (64 groups of 512 rows 725 us; Square 822)
+struct Cost {
+    double fixed, item, alone, alone_column, full, full_column;
+};
+template <typename S>
+double time_of(const Cost &c, double items, double stages, double columns) {
+    const double rounds = items / ((double)sm_count() / S::kCtas);
+    if (rounds <= 1.0) return c.fixed + c.item + stages * (c.alone + c.alone_column * columns) * 1e-3;
+    return c.fixed + (rounds + 0.4) * (c.item + stages * (c.full + c.full_column * columns) * 1e-3);
+}
+constexpr Cost kFewCost = {4.5, 0.0, 225, 0.1, 240, 0.6}, kMiddleCost = {5, 1, 232, 0.12, 245, 0.5}, kSquareCost = {6, 1.5, 210, 0.5, 165, 1.33},
+               kWideCost = {8, 8, 120, 1.9, 380, 2.06};
+constexpr Cost kFewWeight = {2.8, 1, 190, 0.1, 240, 0.6}, kMiddleWeight = {3, 1.2, 200, 0.4, 245, 0.5}, kWideWeight = {3, 4, 350, 1.2, 400, 1.2};
+
+// Few items: the blocks that share the depth of each, as many as there are SMs for.  The parts' way through the cluster costs
+// about 6.5 us and 0.05 per column; one group of 8 rows of 2048 x 7168 takes 9.6 us in eight parts, 25.9 in one.
+template <int kForm>
+uint32_t parts_of(const Product &p, uint32_t stages, double columns, double shortest) {
+    const uint64_t items = items_of<kForm, FewSplit>(p);
+    if (items * 2u > (uint64_t)sm_count()) return 1u;
+    auto kernel = grouped_bf16_kernel<kForm, true, FewSplit>;
+    if (!set_max_dynamic_smem((const void *)kernel, FewSplit::kBytes)) return 1u;
+    const ActiveClusters active = active_clusters((const void *)kernel, kThreads, FewSplit::kBytes);
+    uint32_t parts = std::max(1u, std::min(kMaxParts, stages));
+    while (parts > 1u && active.of_size[parts] < items) parts--;
+    return 6.5 + 0.05 * columns + 0.23 * ((stages + parts - 1u) / parts) < shortest ? parts : 1u;
+}
+
+template <int kForm>
+bool rows_product(const Product &p, cudaStream_t stream) {
+    const uint32_t groups = std::min(p.rows, p.groups), stages = ((kForm == kForward ? p.k : p.n) + kDepth - 1u) / kDepth;
+    const double rows = (double)p.rows / groups;
+    auto time = [&](auto shape, const Cost &c) {
+        using S = decltype(shape);
+        const double tiles = std::ceil(rows / S::kMaxN), lanes = (double)(((kForm == kByInput ? p.k : p.n) + S::kLanes - 1u) / S::kLanes);
+        return time_of<S>(c, groups * tiles * lanes, stages, rows / tiles);
+    };
+    const double few = time(Few{}, kFewCost), middle = time(Middle{}, kMiddleCost), square = time(Square{}, kSquareCost);
+    const double wide = time(Wide{}, kWideCost), shortest = rows <= kFewRows ? few : std::min({few, middle, square, wide});
+    const uint32_t parts = parts_of<kForm>(p, stages, std::min(rows, (double)kFewRows), shortest);
+    if (parts > 1u) return launch_typed<kForm, FewSplit>(p, stream, parts);
+    if (shortest == few) return launch_typed<kForm, Few>(p, stream);
+    if (shortest == middle) return launch_typed<kForm, Middle>(p, stream);
+    return shortest == square ? launch_typed<kForm, Square>(p, stream) : launch_typed<kForm, Wide>(p, stream);
+}
+
+// By weight the lanes and columns are the matrices', the depth the rows; one block per item, for pairs multiply two operands
+// that lie by their depth 10 % more slowly (4096 rows of 8 groups, without the stores: 669 us, pairs 729).
+bool weight_product(const Product &p, cudaStream_t stream) {
+    const uint32_t stages = std::max(1u, (p.rows / p.groups + kDepth - 1u) / kDepth);
+    auto time = [&](auto shape, const Cost &c) {
+        using S = decltype(shape);
+        return time_of<S>(c, (double)items_of<kByWeight, S>(p), stages, std::min(p.k, S::kMaxN));
+    };
+    const double few = time(Few{}, kFewWeight), middle = time(Middle{}, kMiddleWeight), wide = time(WideWeight{}, kWideWeight);
+    const double shortest = std::min({few, middle, wide});
+    const uint32_t parts = parts_of<kByWeight>(p, stages, std::min(p.k, kFewRows), shortest);
+    if (parts > 1u) return launch_typed<kByWeight, FewSplit>(p, stream, parts);
+    if (shortest == few) return launch_typed<kByWeight, Few>(p, stream);
+    return shortest == middle ? launch_typed<kByWeight, Middle>(p, stream) : launch_typed<kByWeight, WideWeight>(p, stream);
 }
 
 }  // namespace
@@ -684,10 +839,8 @@ bool launch_typed(const Product &p, cudaStream_t stream) {
 uint64_t k3::gb::tc_workspace_bytes(uint32_t rows, uint32_t groups) { return plan_bytes(most_tiles(rows, groups, kFewRows)); }
 
 bool k3::gb::product_tc(const Product &p, cudaStream_t stream) {
-    if (p.form == kByWeight) return launch_typed<kByWeight, WideWeight>(p, stream);
-    const bool few = p.rows <= 24u * std::min(p.rows, p.groups);
-    if (p.form == kForward) return few ? launch_typed<kForward, Few>(p, stream) : launch_typed<kForward, Wide>(p, stream);
-    return few ? launch_typed<kByInput, Few>(p, stream) : launch_typed<kByInput, Wide>(p, stream);
+    if (p.form == kByWeight) return weight_product(p, stream);
+    return p.form == kForward ? rows_product<kForward>(p, stream) : rows_product<kByInput>(p, stream);
 }
 
 uint32_t k3_grouped_bf16_status() {
