@@ -39,7 +39,7 @@ namespace {
 
 constexpr uint32_t kThreads = 384, kResultWarps = 8, kDepth = 64;      // depth of a stage: 128 bytes of bf16
 constexpr uint32_t kBox = 64 * kDepth * 2;                             // 8 KB: 64 x 64 elements
-constexpr uint32_t kSlots = 2;                                         // items that are known ahead
+constexpr uint32_t kSlots = 4;                                         // items that are known ahead
 constexpr uint32_t kMaxParts = 8;                                      // of an item's depth: the portable cluster
 constexpr uint32_t kAhead = 6;                                         // stages before an item's last in which the next is drawn
 constexpr uint32_t kNoItem = 0xffffffffu;
@@ -78,12 +78,14 @@ struct TcArgs {
     uint32_t rows, groups, n, k;
     uint32_t lane_tiles;                                               // items side by side along the lanes
     uint32_t column_tiles;                                             // by weight: and along the columns
+    uint32_t batch;                                                    // items per draw
     int accumulate;
 };
 
 struct Item {
     uint32_t group, row, rows;                                         // by weight: the group's rows, all of them
     uint32_t lane0, column0;                                           // by weight: column0 of k
+    uint32_t draw;                                                     // 1: the last one drawn
 };
 
 // Instruction descriptor, kind::f16, as make_idesc_bf16, with bits 15 and 16 for operands whose depth is not what lies
@@ -355,9 +357,9 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 range_of((depth_of(it) + kDepth - 1u) / kDepth, begin, end);
                 const uint32_t b_boxes = boxes_of(columns), b_first = rank * (steps_of(columns) / kCtas);
                 const uint32_t bytes = halves * 2u * kBox + b_boxes * (kRows ? kBox / 2u : kBox);
-                if (rank == 0u && end - begin <= kAhead) mbar_arrive(wanted);
+                if (rank == 0u && it.draw != 0u && end - begin <= kAhead) mbar_arrive(wanted);
                 for (uint32_t kb = begin; kb < end; kb++) {
-                    if (rank == 0u && kb + kAhead == end - 1u) mbar_arrive(wanted);
+                    if (rank == 0u && it.draw != 0u && kb + kAhead == end - 1u) mbar_arrive(wanted);
                     if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag)) { ok = false; break; }
                     unsigned char *at = base + s * S::kStage, *bt = at + S::kA;
                     const int32_t d = (int32_t)(kRows || kb == 0u ? kb * kDepth : first_rows(it.rows) + (kb - 1u) * kDepth), r = (int32_t)it.row;
@@ -465,20 +467,21 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         // ------------------------------------------------- items, each shortly before its loads
         if (rank == 0u && elect_one()) {
             const uint32_t total = kRows ? a.plan->tiles * a.lane_tiles : a.groups * a.lane_tiles * a.column_tiles;
-            uint32_t w = blockIdx.x / (S::kSplit ? splits : kCtas), want_phase = 0u;
+            uint32_t w = blockIdx.x / (S::kSplit ? splits : kCtas) * a.batch, left = a.batch, want_phase = 0u;
             for (;;) {
-                Item it{kNoItem, 0u, 0u, 0u, 0u};
+                Item it{kNoItem, 0u, 0u, 0u, 0u, 0u};
+                left--;
                 if (w < total) {
                     if (kRows) {
                         const Tile of = a.tiles[w / a.lane_tiles];
                         const uint32_t local = w - of.first * a.lane_tiles, t = local % of.count;
                         const Tile tile = t + of.first == w / a.lane_tiles ? of : a.tiles[of.first + t];
-                        it = {tile.group, tile.row, tile.rows, local / of.count * S::kLanes, 0u};
+                        it = {tile.group, tile.row, tile.rows, local / of.count * S::kLanes, 0u, left == 0u};
                     } else {
                         const uint32_t per = a.lane_tiles * a.column_tiles, g = w / per, at = w - g * per;
                         uint32_t begin, end;
                         group_rows(a.offsets, g, a.rows, begin, end);
-                        it = {g, begin, end - begin, at / a.column_tiles * S::kLanes, at % a.column_tiles * S::kMaxN};
+                        it = {g, begin, end - begin, at / a.column_tiles * S::kLanes, at % a.column_tiles * S::kMaxN, left == 0u};
                     }
                 }
                 if (!wait_at(&item_empty[slot], slot_phase ^ 1u)) break;
@@ -491,12 +494,19 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     store_at(to + 8u, it.rows);
                     store_at(to + 12u, it.lane0);
                     store_at(to + 16u, it.column0);
+                    store_at(to + 20u, it.draw);
                     arrive_at(place_in(&item_full[slot], 1u));
                 }
                 item_done();
-                if (it.group == kNoItem || !mbar_wait(wanted, want_phase, abort_flag)) break;
+                if (it.group == kNoItem) break;
+                if (left != 0u) {
+                    w++;
+                    continue;
+                }
+                if (!mbar_wait(wanted, want_phase, abort_flag)) break;
                 want_phase ^= 1u;
-                w = S::kSplit ? total : gridDim.x / kCtas + atomicAdd(&a.plan->counter, 1u);
+                left = a.batch;
+                w = S::kSplit ? total : gridDim.x / kCtas * a.batch + atomicAdd(&a.plan->counter, a.batch);
             }
         }
     } else if (warp == 3u) {
@@ -732,6 +742,14 @@ uint64_t items_of(const Product &p) {
     return lanes * (kForm == kByWeight ? (uint64_t)p.groups * ((p.k + S::kMaxN - 1u) / S::kMaxN) : most_tiles(p.rows, p.groups, S::kMaxN));
 }
 
+// Items per draw.  A draw takes about 1.3 us from the wish to the item, which items of a few stages do not cover; four at a
+// time where every SM has 16 of them or more.
+template <int kForm, typename S>
+uint32_t batch_of(const Product &p) {
+    const uint32_t depth = kForm == kForward ? p.k : kForm == kByInput ? p.n : p.rows / p.groups;
+    return !S::kSplit && depth <= 4u * kDepth && items_of<kForm, S>(p) >= 16u * (uint64_t)sm_count() / S::kCtas ? 4u : 1u;
+}
+
 // parts: blocks that share an item's depth (S::kSplit)
 template <int kForm, bool kF32, typename S>
 bool launch(const Product &p, uint32_t parts, cudaStream_t stream) {
@@ -747,7 +765,7 @@ bool launch(const Product &p, uint32_t parts, cudaStream_t stream) {
     }
     const uint32_t lanes = kForm == kByInput ? p.k : p.n, tiles = most_tiles(p.rows, p.groups, S::kMaxN);
     const TcArgs a{p.out, p.offsets, (Plan *)p.workspace, (Tile *)((Plan *)p.workspace + 1), p.rows, p.groups, p.n, p.k,
-                   (lanes + S::kLanes - 1u) / S::kLanes, (p.k + S::kMaxN - 1u) / S::kMaxN, p.accumulate};
+                   (lanes + S::kLanes - 1u) / S::kLanes, (p.k + S::kMaxN - 1u) / S::kMaxN, batch_of<kForm, S>(p), p.accumulate};
     const uint64_t items = items_of<kForm, S>(p), places = S::kSplit ? items : (uint64_t)sm_count() / S::kCtas;
     if (items * parts > 0x7fffffffull || !set_max_dynamic_smem((const void *)kernel, S::kBytes)) return false;
     const uint32_t cluster = S::kSplit ? parts : S::kCtas;
