@@ -79,6 +79,7 @@ struct TcArgs {
     uint32_t lane_tiles;                                               // items side by side along the lanes
     uint32_t column_tiles;                                             // by weight: and along the columns
     uint32_t batch;                                                    // items per draw
+    bool single;                                                       // an item per block at most: no plan, nothing is drawn
     int accumulate;
 };
 
@@ -205,7 +206,57 @@ K3_DEVINL void free_tmem(uint32_t tmem, uint32_t columns) {
 }
 
 // ------------------------------------------------------------------------------------------- the plan
-// One thread per group.  A group's rows in as few tiles of up to max_n as there can be, equally large but for one step.
+// Tile i of a group's `count`: as few as there can be of up to max_n rows, equally large but for one step.
+K3_DEVINL Tile tile_of(uint32_t group, uint32_t begin, uint32_t end, uint32_t first, uint32_t count, uint32_t i, uint32_t step) {
+    const uint32_t steps = (end - begin + step - 1u) / step, each = steps / count, more = steps - each * count;
+    const uint32_t row = begin + (each * i + min(i, more)) * step;
+    return Tile{group, row, min((each + (i < more ? 1u : 0u)) * step, end - row), first, count, {}};
+}
+
+// A call with an item for every block at most and up to kSearched groups needs no plan: a warp looks its item up.  The tile
+// that item w of lane_tiles per tile belongs to, its place along the lanes in `lane_tile`; false past the last.
+constexpr uint32_t kSearched = 128;
+K3_DEVINL bool search_tile(const uint32_t *offsets, uint32_t rows, uint32_t groups, uint32_t max_n, uint32_t step, uint32_t w,
+                           uint32_t lane_tiles, Tile &tile, uint32_t &lane_tile) {
+    constexpr uint32_t kEach = kSearched / kWarp;
+    const uint32_t lane = threadIdx.x % kWarp, t = w / lane_tiles;
+    uint32_t begin[kEach], end[kEach], sum = 0u;
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; i++) {
+        const uint32_t g = lane * kEach + i;
+        begin[i] = end[i] = 0u;
+        if (g < groups) group_rows(offsets, g, rows, begin[i], end[i]);
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; i++) sum += (end[i] - begin[i] + max_n - 1u) / max_n;
+    uint32_t scan = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, scan, o);
+        if (lane >= (uint32_t)o) scan += up;
+    }
+    uint32_t first = scan - sum;
+    const uint32_t holder = __ballot_sync(0xffffffffu, t >= first && t < scan);
+    if (holder == 0u) return false;
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; i++) {
+        const uint32_t count = (end[i] - begin[i] + max_n - 1u) / max_n;
+        if (t >= first && t < first + count) {
+            const uint32_t local = w - first * lane_tiles;
+            tile = tile_of(lane * kEach + i, begin[i], end[i], first, count, local % count, step);
+            lane_tile = local / count;
+        }
+        first += count;
+    }
+    const uint32_t from = __ffs(holder) - 1u;
+    tile.group = __shfl_sync(0xffffffffu, tile.group, from);
+    tile.row = __shfl_sync(0xffffffffu, tile.row, from);
+    tile.rows = __shfl_sync(0xffffffffu, tile.rows, from);
+    lane_tile = __shfl_sync(0xffffffffu, lane_tile, from);
+    return true;
+}
+
+// One thread per group.
 __global__ void __launch_bounds__(kMaxGroups) grouped_plan_kernel(Plan *plan, Tile *tiles, const uint32_t *offsets, uint32_t rows,
                                                                   uint32_t groups, uint32_t max_n, uint32_t step, uint32_t capacity) {
     pdl_trigger();
@@ -226,11 +277,11 @@ __global__ void __launch_bounds__(kMaxGroups) grouped_plan_kernel(Plan *plan, Ti
     uint32_t first = scan - count;
     for (uint32_t w = 0; w < warp; w++) first += sums[w];
     if (count != 0u) {
-        const uint32_t steps = (end - begin + step - 1u) / step, each = steps / count, more = steps - each * count;
-        for (uint32_t i = 0, row = begin; i < count && first + i < capacity; i++) {
-            const uint32_t size = min((each + (i < more ? 1u : 0u)) * step, end - row);
-            tiles[first + i] = Tile{g, row, size, first, min(count, capacity - first), {}};
-            row += size;
+        const uint32_t held = min(count, capacity - min(capacity, first));
+        for (uint32_t i = 0; i < held; i++) {
+            Tile t = tile_of(g, begin, end, first, count, i, step);
+            t.count = held;                                            // (fewer only if offsets descend)
+            tiles[first + i] = t;
         }
     }
     if (g == kMaxGroups - 1u) {
@@ -465,40 +516,62 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         }
     } else if (warp == 2u) {
         // ------------------------------------------------- items, each shortly before its loads
-        if (rank == 0u && elect_one()) {
+        auto publish = [&](const Item &it) {                           // by one thread
+            if (!wait_at(&item_empty[slot], slot_phase ^ 1u)) return false;
+            items[slot] = it;
+            mbar_arrive(&item_full[slot]);
+            if (kCtas == 2u) {
+                const uint32_t to = place_in(&items[slot], 1u);
+                store_at(to, it.group);
+                store_at(to + 4u, it.row);
+                store_at(to + 8u, it.rows);
+                store_at(to + 12u, it.lane0);
+                store_at(to + 16u, it.column0);
+                store_at(to + 20u, it.draw);
+                arrive_at(place_in(&item_full[slot], 1u));
+            }
+            item_done();
+            return it.group != kNoItem;
+        };
+        const Item none{kNoItem, 0u, 0u, 0u, 0u, 0u};
+        auto weight_item = [&](uint32_t w) {                           // by weight: matrices side by side, then groups
+            const uint32_t per = a.lane_tiles * a.column_tiles, g = w / per, at = w - g * per;
+            uint32_t begin, end;
+            group_rows(a.offsets, g, a.rows, begin, end);
+            return Item{g, begin, end - begin, at / a.column_tiles * S::kLanes, at % a.column_tiles * S::kMaxN, 0u};
+        };
+        uint32_t w = blockIdx.x / (S::kSplit ? splits : kCtas);
+        if (rank == 0u && a.single) {
+            Item it = none;
+            if (kRows) {
+                Tile tile{};
+                uint32_t lane_tile = 0u;
+                if (search_tile(a.offsets, a.rows, a.groups, S::kMaxN, S::kStep, w, a.lane_tiles, tile, lane_tile)) {
+                    it = Item{tile.group, tile.row, tile.rows, lane_tile * S::kLanes, 0u, 0u};
+                }
+            } else if (w < a.groups * a.lane_tiles * a.column_tiles) {
+                it = weight_item(w);
+            }
+            if (elect_one() && publish(it)) publish(none);
+        } else if (rank == 0u && elect_one()) {
             const uint32_t total = kRows ? a.plan->tiles * a.lane_tiles : a.groups * a.lane_tiles * a.column_tiles;
-            uint32_t w = blockIdx.x / (S::kSplit ? splits : kCtas) * a.batch, left = a.batch, want_phase = 0u;
+            uint32_t left = a.batch, want_phase = 0u;
+            w *= a.batch;
             for (;;) {
-                Item it{kNoItem, 0u, 0u, 0u, 0u, 0u};
+                Item it = none;
                 left--;
                 if (w < total) {
                     if (kRows) {
                         const Tile of = a.tiles[w / a.lane_tiles];
                         const uint32_t local = w - of.first * a.lane_tiles, t = local % of.count;
                         const Tile tile = t + of.first == w / a.lane_tiles ? of : a.tiles[of.first + t];
-                        it = {tile.group, tile.row, tile.rows, local / of.count * S::kLanes, 0u, left == 0u};
+                        it = Item{tile.group, tile.row, tile.rows, local / of.count * S::kLanes, 0u, 0u};
                     } else {
-                        const uint32_t per = a.lane_tiles * a.column_tiles, g = w / per, at = w - g * per;
-                        uint32_t begin, end;
-                        group_rows(a.offsets, g, a.rows, begin, end);
-                        it = {g, begin, end - begin, at / a.column_tiles * S::kLanes, at % a.column_tiles * S::kMaxN, left == 0u};
+                        it = weight_item(w);
                     }
+                    it.draw = left == 0u;
                 }
-                if (!wait_at(&item_empty[slot], slot_phase ^ 1u)) break;
-                items[slot] = it;
-                mbar_arrive(&item_full[slot]);
-                if (kCtas == 2u) {
-                    const uint32_t to = place_in(&items[slot], 1u);
-                    store_at(to, it.group);
-                    store_at(to + 4u, it.row);
-                    store_at(to + 8u, it.rows);
-                    store_at(to + 12u, it.lane0);
-                    store_at(to + 16u, it.column0);
-                    store_at(to + 20u, it.draw);
-                    arrive_at(place_in(&item_full[slot], 1u));
-                }
-                item_done();
-                if (it.group == kNoItem) break;
+                if (!publish(it)) break;
                 if (left != 0u) {
                     w++;
                     continue;
@@ -506,7 +579,7 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 if (!mbar_wait(wanted, want_phase, abort_flag)) break;
                 want_phase ^= 1u;
                 left = a.batch;
-                w = S::kSplit ? total : gridDim.x / kCtas * a.batch + atomicAdd(&a.plan->counter, a.batch);
+                w = gridDim.x / kCtas * a.batch + atomicAdd(&a.plan->counter, a.batch);
             }
         }
     } else if (warp == 3u) {
@@ -764,14 +837,15 @@ bool launch(const Product &p, uint32_t parts, cudaStream_t stream) {
         if (!make_map(&ma, p.a, p.n, p.rows, 0u, 64u) || !make_map(&mb, p.b, p.k, p.rows, 0u, 64u)) return false;
     }
     const uint32_t lanes = kForm == kByInput ? p.k : p.n, tiles = most_tiles(p.rows, p.groups, S::kMaxN);
-    const TcArgs a{p.out, p.offsets, (Plan *)p.workspace, (Tile *)((Plan *)p.workspace + 1), p.rows, p.groups, p.n, p.k,
-                   (lanes + S::kLanes - 1u) / S::kLanes, (p.k + S::kMaxN - 1u) / S::kMaxN, batch_of<kForm, S>(p), p.accumulate};
     const uint64_t items = items_of<kForm, S>(p), places = S::kSplit ? items : (uint64_t)sm_count() / S::kCtas;
-    if (items * parts > 0x7fffffffull || !set_max_dynamic_smem((const void *)kernel, S::kBytes)) return false;
+    const bool single = items <= places && (!kRows || p.groups <= kSearched);
+    const TcArgs a{p.out, p.offsets, (Plan *)p.workspace, (Tile *)((Plan *)p.workspace + 1), p.rows, p.groups, p.n, p.k,
+                   (lanes + S::kLanes - 1u) / S::kLanes, (p.k + S::kMaxN - 1u) / S::kMaxN, batch_of<kForm, S>(p), single, p.accumulate};
+    if (items * parts > 0x7fffffffull || (S::kSplit && !single) || !set_max_dynamic_smem((const void *)kernel, S::kBytes)) return false;
     const uint32_t cluster = S::kSplit ? parts : S::kCtas;
-    const bool planned = kRows ? launch_chained(grouped_plan_kernel, 1, kMaxGroups, 0, stream, a.plan, a.tiles, p.offsets, p.rows, p.groups,
-                                                S::kMaxN, S::kStep, tiles)
-                               : S::kSplit || launch_chained(grouped_counter_kernel, 1, 1, 0, stream, a.plan);
+    const bool planned = single || (kRows ? launch_chained(grouped_plan_kernel, 1, kMaxGroups, 0, stream, a.plan, a.tiles, p.offsets, p.rows,
+                                                           p.groups, S::kMaxN, S::kStep, tiles)
+                                          : launch_chained(grouped_counter_kernel, 1, 1, 0, stream, a.plan));
     return planned && launch_chained_cluster(kernel, (uint32_t)std::min(items, places) * cluster, kThreads, dim3(cluster, 1, 1), S::kBytes, stream,
                                              ma, mb, a);
 }
@@ -809,7 +883,7 @@ constexpr Cost kFewWeight = {2.8, 1, 190, 0.1, 240, 0.6}, kMiddleWeight = {3, 1.
 template <int kForm>
 uint32_t parts_of(const Product &p, uint32_t stages, double columns, double shortest) {
     const uint64_t items = items_of<kForm, FewSplit>(p);
-    if (items * 2u > (uint64_t)sm_count()) return 1u;
+    if (items * 2u > (uint64_t)sm_count() || (kForm != kByWeight && p.groups > kSearched)) return 1u;
     auto kernel = grouped_bf16_kernel<kForm, true, FewSplit>;
     if (!set_max_dynamic_smem((const void *)kernel, FewSplit::kBytes)) return 1u;
     const ActiveClusters active = active_clusters((const void *)kernel, kThreads, FewSplit::kBytes);
