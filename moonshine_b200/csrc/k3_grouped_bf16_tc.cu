@@ -855,12 +855,13 @@ bool launch_typed(const Product &p, cudaStream_t stream, uint32_t parts = 1u) {
     return p.f32 ? launch<kForm, true, S>(p, parts, stream) : launch<kForm, false, S>(p, parts, stream);
 }
 
-// Which shape.  The host knows the rows and groups of a call, not how they are spread, so it takes every group that can
-// have rows to have equally many, and of the shapes the one with the shortest time by what was measured on a B200 (us, and
-// ns per stage of 64 of the depth): `fixed` for a call, `item` for an item's results, and per stage base + column x columns,
-// alone in a single round of items, full where the SMs share memory and power over several.  Over 192 calls of 1 to 64 groups
-// of 1 to 2048 rows at 2048 x 7168, 7168 x 2048, 2048 x 1024 and 512 x 512 the shape that this takes is 0.7 % from the best
-// on average, 26 % at worst; always taking the largest, 66 %.  What each is for:
+// Which shape.  The host knows the rows and groups of a call, not how they are spread: it takes a third of the groups to hold
+// all rows, each equally many, which lies between even loads and loads by Zipf's law, whose rows lie in groups of four times
+// the mean; and of the shapes the one with the shortest time by what was measured on a B200 (us, and ns per stage of 64 of
+// the depth): `fixed` for a call, `item` for an item's results, and per stage base + column x columns, alone in a single round
+// of items, full where the SMs share memory and power over several.  Over 176 calls of 1 to 64 even groups of 1 to 2048 rows
+// at 2048 x 7168, 7168 x 2048, 2048 x 1024 and 512 x 512 the shape that this takes is 2.4 % from the best on average, over
+// eight of 16 to 896 uneven groups 3.2 % (with all groups holding rows 0.8 and 13.6 %).  What each is for:
 //   Few      up to 64 rows per group: bound by the matrices' bytes, 6.4 TB/s at 64 groups of 8 rows of 2048 x 7168 (274 us; Middle 294)
 //   Middle   up to 128, or too few items for larger ones (4 groups of 256 rows: 35 us; Few 53, Square 43)
 //   Square   pairs of blocks with two accumulators (16 groups of 256 rows of 7168 x 2048: 107 us; Wide 115, Middle 134)
@@ -894,8 +895,8 @@ uint32_t parts_of(const Product &p, uint32_t stages, double columns, double shor
 
 template <int kForm>
 bool rows_product(const Product &p, cudaStream_t stream) {
-    const uint32_t groups = std::min(p.rows, p.groups), stages = ((kForm == kForward ? p.k : p.n) + kDepth - 1u) / kDepth;
-    const double rows = (double)p.rows / groups;
+    const uint32_t stages = ((kForm == kForward ? p.k : p.n) + kDepth - 1u) / kDepth;
+    const double rows = std::min(3.0 * p.rows / std::min(p.rows, p.groups), (double)p.rows), groups = p.rows / rows;
     auto time = [&](auto shape, const Cost &c) {
         using S = decltype(shape);
         const double tiles = std::ceil(rows / S::kMaxN), lanes = (double)(((kForm == kByInput ? p.k : p.n) + S::kLanes - 1u) / S::kLanes);
