@@ -12,8 +12,12 @@ on the current CUDA device.
     dx = up.by_input(dy, offsets, dtype=torch.float32)
     dw = grouped.GroupedWeightGradient(experts, n, k).forward(dy, x, offsets)
     d_gate, d_up, scaled, d_weights = grouped.GatedActivation("swiglu").backward(d_out, gate, up, weights, routes)
+
+``RoutedExperts`` is all of it for one layer: dispatch, products, activation and weighted sum, and their gradients.
 """
 from __future__ import annotations
+
+from typing import NamedTuple
 
 import torch
 
@@ -155,3 +159,97 @@ class GatedActivation:
                                                  0 if offsets is None else offsets.shape[0] - 1, rows, columns, count,
                                                  self.activation, self.beta, self.linear_beta), "k3_moe_activation_backward")
         return d_gate, d_up, scaled, d_weights
+
+
+class Routed(NamedTuple):
+    """What a forward pass of ``RoutedExperts`` leaves for the backward pass: the dispatch, and the rows it grouped."""
+    offsets: torch.Tensor                    # int32 [experts + 1]
+    routes: torch.Tensor                     # int32 [rows]: the route token * top_k + rank of a row
+    tokens: torch.Tensor                     # int32 [rows]: its token
+    place: torch.Tensor                      # int32 [tokens * top_k]: the row of a route
+    weights: torch.Tensor
+    x: torch.Tensor                          # bf16 [rows, hidden]
+    gate: torch.Tensor                       # bf16 [rows, expert_hidden]
+    up: torch.Tensor
+
+
+class ExpertGradients(NamedTuple):
+    x: torch.Tensor                          # bf16 [tokens, hidden]
+    weights: torch.Tensor                    # f32 [tokens, top_k], for ``balance.RouterBalance.backward``
+    w1: torch.Tensor                         # f32, as the matrices
+    w3: torch.Tensor
+    w2: torch.Tensor
+
+
+class RoutedExperts:
+    """The routed experts of a layer in bf16: gate ``w1`` and up ``w3`` [experts, expert_hidden, hidden], down ``w2``
+    [experts, hidden, expert_hidden], hidden a multiple of 8.  The products' results are rounded to bf16, as are the rows' gradients; the
+    gradient by x adds those of gate and up in f32 before its rounding.  Neither pass waits for the GPU."""
+
+    def __init__(self, w1: torch.Tensor, w3: torch.Tensor, w2: torch.Tensor, top_k: int, activation: str = "swiglu",
+                 beta: float = 4.0, linear_beta: float = 25.0):
+        self.gate, self.up, self.down = GroupedProduct(w1), GroupedProduct(w3), GroupedProduct(w2)
+        experts, expert_hidden, hidden = w1.shape
+        if w3.shape != w1.shape or w2.shape != (experts, hidden, expert_hidden):
+            raise ValueError(f"w1, w3 and w2: expected {list(w1.shape)} twice and {[experts, hidden, expert_hidden]}, got {list(w3.shape)} and "
+                             f"{list(w2.shape)}")
+        if hidden % 8:
+            raise ValueError(f"w1: expected a multiple of 8 columns, which the weighted sum wants, got {hidden}")
+        if not 0 < top_k <= min(experts, 32):
+            raise ValueError(f"top_k: 1 to {min(experts, 32)}, got {top_k}")
+        self.experts, self.hidden, self.expert_hidden, self.top_k = experts, hidden, expert_hidden, top_k
+        self.activation = GatedActivation(activation, beta, linear_beta)
+        self._by_w1, self._by_w3 = (GroupedWeightGradient(experts, expert_hidden, hidden) for _ in range(2))
+        self._by_w2 = GroupedWeightGradient(experts, hidden, expert_hidden)
+        self._workspace = _Workspace(lambda tokens: ops.k3_moe_dispatch_workspace_bytes(tokens, top_k, experts))
+
+    def _gather(self, x, tokens):
+        rows = x.new_empty((tokens.shape[0], self.hidden))
+        _done(ops.k3_rocm_gather_rows_bf16(rows, x, tokens, tokens.shape[0], self.hidden), "k3_rocm_gather_rows_bf16")
+        return rows
+
+    def _combine(self, rows, place, weights):
+        out = rows.new_empty((weights.shape[0], self.hidden))
+        _done(ops.k3_moe_combine(out, rows, place, weights, None, weights.shape[0], self.top_k, self.hidden), "k3_moe_combine")
+        return out
+
+    def forward(self, x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor) -> tuple[torch.Tensor, Routed]:
+        """x bf16 [tokens, hidden], ids int32 (each below the experts) and weights f32 [tokens, top_k], as ``k3_moe_route``
+        writes them -> bf16 [tokens, hidden], and what ``backward`` reads."""
+        tokens, _ = _matrix(x, "x", self.hidden)
+        _check(ids, "ids", torch.int32, (tokens, self.top_k))
+        _check(weights, "weights", torch.float32, (tokens, self.top_k))
+        _placed(("x", x), ("ids", ids), ("weights", weights), tables=self.gate._device)
+        rows = tokens * self.top_k
+        # zeros: what a dispatch leaves out (an id that is no expert's) stays an index inside
+        offsets, routes, of_row, place = (ids.new_zeros(n) for n in (self.experts + 1, rows, rows, rows))
+        if tokens == 0:
+            nothing = x.new_empty((0, self.expert_hidden))
+            return x.new_empty((0, self.hidden)), Routed(offsets, routes, of_row, place, weights, x, nothing, nothing)
+        ws = self._workspace.of(tokens, x.device)
+        _done(ops.k3_moe_dispatch_build(offsets, routes, of_row, place, ids, tokens, self.top_k, self.experts, ws, self._workspace.bytes),
+              "k3_moe_dispatch_build")
+        x_rows = self._gather(x, of_row)
+        gate, up = self.gate.forward(x_rows, offsets), self.up.forward(x_rows, offsets)
+        out = self._combine(self.down.forward(self.activation.forward(gate, up), offsets), place, weights)
+        return out, Routed(offsets, routes, of_row, place, weights, x_rows, gate, up)
+
+    def backward(self, d_out: torch.Tensor, saved: Routed) -> ExpertGradients:
+        """d_out bf16 [tokens, hidden] and what ``forward`` left -> the gradients by x, the routing weights and the matrices."""
+        tokens, _ = _matrix(d_out, "d_out", self.hidden)
+        if saved.weights.shape[0] != tokens:
+            raise ValueError(f"d_out: expected {saved.weights.shape[0]} tokens, got {tokens}")
+        _placed(("d_out", d_out), tables=self.gate._device)
+        offsets = saved.offsets
+        if tokens == 0:
+            d_gate = d_up = scaled = saved.gate
+            dx, d_rows, d_weights = d_out, d_out, torch.empty_like(saved.weights)
+        else:
+            d_rows = self._gather(d_out, saved.tokens)
+            d_gate, d_up, scaled, d_weights = self.activation.backward(self.down.by_input(d_rows, offsets), saved.gate, saved.up,
+                                                                       saved.weights, saved.routes, offsets)
+            by_rows = self.gate.by_input(d_gate, offsets, dtype=torch.float32)
+            self.up.by_input(d_up, offsets, into=by_rows)
+            dx = self._combine(by_rows.to(torch.bfloat16), saved.place, torch.ones_like(saved.weights))
+        return ExpertGradients(dx, d_weights, self._by_w1.forward(d_gate, saved.x, offsets), self._by_w3.forward(d_up, saved.x, offsets),
+                               self._by_w2.forward(d_rows, scaled, offsets))
