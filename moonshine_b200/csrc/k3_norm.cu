@@ -220,26 +220,32 @@ struct NormGradArgs {
     uint32_t rows, hidden;
 };
 
-// A vector's part of the row's sum of w dy s rstd, and of the weight's gradient.
+// Two neighbouring elements as f32.
 template <bool kF32>
-K3_DEVINL float add_products(const Eight<false> &dy, const Eight<kF32> &s, const Eight<false> &w, float rstd, float dot, float (&dw)[8]) {
+K3_DEVINL uint64_t pair_of(const Eight<kF32> &e, uint32_t i) { return pack2(e.value(2u * i), e.value(2u * i + 1u)); }
+
+// A vector's part of the row's sum of w dy s rstd, and of the weight's gradient, two elements at a time.
+template <bool kF32>
+K3_DEVINL uint64_t add_products(const Eight<false> &dy, const Eight<kF32> &s, const Eight<false> &w, uint64_t rstd, uint64_t dot, uint64_t (&dw)[4]) {
 #pragma unroll
-    for (uint32_t i = 0; i < 8u; i++) {
-        const float g = dy.value(i), h = s.value(i) * rstd;
-        dot = fmaf(g * w.value(i), h, dot);
-        dw[i] = fmaf(g, h, dw[i]);
+    for (uint32_t i = 0; i < 4u; i++) {
+        const uint64_t g = pair_of(dy, i), h = mul2(pair_of(s, i), rstd);
+        dot = fma2(mul2(g, pair_of(w, i)), h, dot);
+        dw[i] = fma2(g, h, dw[i]);
     }
     return dot;
 }
-// A vector of dx; mean: that of w dy s rstd over the row.
+// A vector of dx; minus_mean: the negative of the mean of w dy s rstd over the row.
 template <bool kF32>
 K3_DEVINL Eight<kF32> input_gradient(const Eight<false> &dy, const Eight<kF32> &s, const Eight<false> &w, const Eight<kF32> &d, bool with_d,
-                                     float rstd, float mean) {
+                                     uint64_t rstd, uint64_t minus_mean) {
     float f[8];
 #pragma unroll
-    for (uint32_t i = 0; i < 8u; i++) {
-        f[i] = rstd * fmaf(-(s.value(i) * rstd), mean, dy.value(i) * w.value(i));
-        if (with_d) f[i] += d.value(i);
+    for (uint32_t i = 0; i < 4u; i++) {
+        const uint64_t x = fma2(mul2(pair_of(s, i), rstd), minus_mean, mul2(pair_of(dy, i), pair_of(w, i)));
+        const uint64_t r = with_d ? fma2(x, rstd, pair_of(d, i)) : mul2(x, rstd);
+        f[2u * i] = lo2(r);
+        f[2u * i + 1u] = hi2(r);
     }
     Eight<kF32> out;
     out.set(f);
@@ -256,12 +262,12 @@ __global__ void __launch_bounds__(threads_of(kTeam)) norm_backward_kernel(NormGr
     const uint32_t t = threadIdx.x % kTeam, team = threadIdx.x / kTeam;
     auto first = [&](uint32_t v) { return first_column<kVector>(v * kTeam + t); };
     Eight<false> w[kVectors];
-    float dw[kVectors][8];
+    uint64_t dw[kVectors][4];
 #pragma unroll
     for (uint32_t v = 0; v < kVectors; v++) {
         w[v].template load<kVector>(a.weight, first(v), a.hidden);
 #pragma unroll
-        for (uint32_t i = 0; i < 8u; i++) dw[v][i] = 0.0f;
+        for (uint32_t i = 0; i < 4u; i++) dw[v][i] = 0ull;
     }
     uint32_t turn = 0u;
     for (uint64_t at = (uint64_t)blockIdx.x * kTeams; at < a.rows; at += (uint64_t)gridDim.x * kTeams, turn ^= 1u) {
@@ -277,14 +283,14 @@ __global__ void __launch_bounds__(threads_of(kTeam)) norm_backward_kernel(NormGr
             if (a.d_sum != nullptr) d[v].template load<kVector>((const char *)a.d_sum + row * a.hidden * kSize, first(v), columns);
         }
         const float rstd = live ? a.rstd[row] : 0.0f;                // with it zeros in the rows that do not exist
-        float dot = 0.0f;
+        uint64_t dots = 0ull;
 #pragma unroll
-        for (uint32_t v = 0; v < kVectors; v++) dot = add_products<kF32>(dy[v], s[v], w[v], rstd, dot, dw[v]);
-        const float mean = team_sum<kTeam>(dot, scratch[turn]) / (float)a.hidden;
+        for (uint32_t v = 0; v < kVectors; v++) dots = add_products<kF32>(dy[v], s[v], w[v], both2(rstd), dots, dw[v]);
+        const float mean = team_sum<kTeam>(lo2(dots) + hi2(dots), scratch[turn]) / (float)a.hidden;
         char *dx = (char *)a.dx + row * a.hidden * kSize;
 #pragma unroll
         for (uint32_t v = 0; v < kVectors; v++) {
-            input_gradient<kF32>(dy[v], s[v], w[v], d[v], a.d_sum != nullptr, rstd, mean).template store<kVector>(dx, first(v), columns);
+            input_gradient<kF32>(dy[v], s[v], w[v], d[v], a.d_sum != nullptr, both2(rstd), both2(-mean)).template store<kVector>(dx, first(v), columns);
         }
     }
     if (a.partial == nullptr) return;
@@ -294,7 +300,7 @@ __global__ void __launch_bounds__(threads_of(kTeam)) norm_backward_kernel(NormGr
 #pragma unroll
         for (uint32_t i = 0; i < 8u; i++) {
             const uint32_t c = column_of<kVector>(first(v), i);
-            if (c < a.hidden) (kTeams == 1u ? to : shared_dw + team * a.hidden)[c] = dw[v][i];
+            if (c < a.hidden) (kTeams == 1u ? to : shared_dw + team * a.hidden)[c] = i & 1u ? hi2(dw[v][i / 2u]) : lo2(dw[v][i / 2u]);
         }
     }
     if (kTeams > 1u) {
@@ -330,10 +336,12 @@ __global__ void __launch_bounds__(256) norm_weight_kernel(float *d_weight, const
 }
 
 // ------------------------------------------------------------------------------------- rows through a ring
-// Many rows of more than 1024 columns: one block per SM takes rows block, block + blocks, ..  A seventeenth warp copies
-// whole rows into a ring of stages in shared memory, up to 192 KB ahead, so that memory is never waited for while a row's
-// sum goes around the other sixteen.
-constexpr uint32_t kRingThreads = 512, kRingWarps = kRingThreads / kWarp, kRingBytes = 196608, kMaxStages = 8;
+// Many rows of more than 1024 columns: one block per SM, in one or two teams that take a row each in turn, from a ring of
+// stages in shared memory with whole rows, up to 192 KB per block, so that memory is never waited for while a row's sum goes
+// around the team.  Forward a seventeenth warp fills the ring and a stage is free once its row is in registers.  Backward,
+// where that warp would leave 96 registers per thread instead of 128, a thread of the team fills it when the sum is there.
+// (Forward that way 8192 x 7168 takes 101 us, with the warp 92; backward 91 and 96, in f32 4096 x 7168 76 and 90.)
+constexpr uint32_t kRingThreads = 512, kRingBytes = 196608, kRingHidden = 8192, kMaxStages = 8;
 
 __device__ uint32_t g_norm_status = 0;
 
@@ -343,46 +351,82 @@ K3_DEVINL void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *b
                  : "memory");
 }
 
+// Up to three arrays' rows, side by side in a stage.
+struct RowSources {
+    const char *at[3];
+    uint32_t bytes[3];
+};
+
+// A ring of stages; its k-th row is first + k step.
 struct Ring {
+    // a stage and the parity of its use
+    struct Turn {
+        uint32_t s, ph;
+        K3_DEVINL void advance(uint32_t by, uint32_t stages) {
+            s += by;
+            if (s >= stages) { s -= stages; ph ^= 1u; }
+        }
+    };
     unsigned char *base;
     uint64_t *full, *empty;
     volatile uint32_t *abort_flag;
     uint32_t stages, stage_bytes;
+    Turn next;                               // of the thread that loads
+    uint64_t first, step, next_row, rows;
 
-    // readers: warps that take a row out of its stage
-    K3_DEVINL void init(unsigned char *smem, uint32_t stages_, uint32_t stage_bytes_, uint32_t readers) {
-        base = smem + 256u;
-        full = reinterpret_cast<uint64_t *>(smem);
-        empty = full + kMaxStages;
-        abort_flag = reinterpret_cast<uint32_t *>(empty + kMaxStages);
+    // Ring `at` of `rings` in the block; readers: warps that take a row out of its stage, 0 where a barrier of theirs says
+    // that they have.  All threads of the block.
+    K3_DEVINL void init(unsigned char *smem, uint32_t stages_, uint32_t stage_bytes_, uint32_t at, uint32_t rings, uint32_t readers,
+                        uint64_t rows_) {
         stages = stages_;
         stage_bytes = stage_bytes_;
+        full = reinterpret_cast<uint64_t *>(smem) + at * stages;
+        empty = full + kMaxStages;
+        abort_flag = reinterpret_cast<uint32_t *>(smem + 16u * kMaxStages);
+        base = smem + 256u + at * stages * stage_bytes;
+        next = {0u, 0u};
+        first = next_row = blockIdx.x + (uint64_t)at * gridDim.x;
+        step = (uint64_t)rings * gridDim.x;
+        rows = rows_;
         if (threadIdx.x == 0u) {
             *abort_flag = 0u;
-            for (uint32_t s = 0; s < stages; s++) {
+            for (uint32_t s = 0; s < stages * rings; s++) {
                 mbar_init(&full[s], 1);
-                mbar_init(&empty[s], readers);
+                if (readers != 0u) mbar_init(&empty[s], readers);
             }
             fence_barrier_init();
         }
         __syncthreads();
     }
-    // The copying thread: rows first, first + step, ..; each from up to three places, side by side in a stage.
-    K3_DEVINL void fill(uint64_t first, uint64_t step, uint64_t rows, const char *a, uint32_t a_bytes, const char *b, uint32_t b_bytes,
-                        const char *c, uint32_t c_bytes) {
-        uint32_t s = 0u, ph = 0u, issued = 0u;
-        for (uint64_t row = first; row < rows; row += step) {
-            if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag)) break;
-            unsigned char *to = base + s * stage_bytes;
-            mbar_arrive_expect_tx(&full[s], a_bytes + b_bytes + c_bytes);
-            bulk_load(to, a + row * a_bytes, a_bytes, &full[s]);
-            if (b_bytes != 0u) bulk_load(to + a_bytes, b + row * b_bytes, b_bytes, &full[s]);
-            if (c_bytes != 0u) bulk_load(to + a_bytes + b_bytes, c + row * c_bytes, c_bytes, &full[s]);
-            issued++;
-            if (++s == stages) { s = 0u; ph ^= 1u; }
+    // one thread: the next row into its stage, which is free; false if there is none
+    K3_DEVINL bool load_next(const RowSources &from) {
+        if (next_row >= rows || *abort_flag != 0u) return false;
+        unsigned char *to = base + next.s * stage_bytes;
+        mbar_arrive_expect_tx(&full[next.s], stage_bytes);
+#pragma unroll
+        for (uint32_t i = 0; i < 3u; i++) {
+            if (from.bytes[i] == 0u) continue;
+            bulk_load(to, from.at[i] + next_row * from.bytes[i], from.bytes[i], &full[next.s]);
+            to += from.bytes[i];
         }
-        if (*abort_flag != 0u) {                                     // nothing may land in a block that has left
-            for (uint32_t i = issued > stages ? issued - stages : 0u; i < issued; i++) mbar_drain(&full[i % stages], (i / stages) & 1u);
+        next.advance(1u, stages);
+        next_row += step;
+        return true;
+    }
+    // one thread: all rows, as stages become free
+    K3_DEVINL void fill(const RowSources &from) {
+        while (mbar_wait(&empty[next.s], next.ph ^ 1u, abort_flag) && load_next(from)) {}
+    }
+    // a row is in its stage; false: given up
+    K3_DEVINL bool wait(const Turn &t) { return mbar_wait(&full[t.s], t.ph, abort_flag); }
+    K3_DEVINL const unsigned char *place(const Turn &t) const { return base + t.s * stage_bytes; }
+    K3_DEVINL void release(const Turn &t) { mbar_arrive(&empty[t.s]); }              // one thread of each reader
+    // the thread that loads, at its end: nothing may land in a block that has left.  The last use of each stage.
+    K3_DEVINL void drain() {
+        if (*abort_flag == 0u) return;
+        for (uint32_t s = 0; s < stages; s++) {
+            const uint32_t last = s < next.s ? next.ph : next.ph ^ 1u;
+            if (s < next.s || next_row >= first + stages * step) mbar_drain(&full[s], last);
         }
     }
 };
@@ -400,29 +444,34 @@ K3_DEVINL float ring_sum(float v, float *scratch) {
     return v;
 }
 
-// Two rows at a time, each by half of the block: one row's sum goes around while the other's results are stored.
+// One ring, whose rows the two halves of the block take in turn.
 template <bool kF32, uint32_t kVectors>
 __global__ void __launch_bounds__(kRingThreads + kWarp, 1) norm_ring_kernel(NormArgs a, uint32_t stages) {
     extern __shared__ __align__(128) unsigned char smem[];
-    constexpr uint32_t kTeam = kRingThreads / 2u;
-    __shared__ float scratch[2][2][kTeam / kWarp];
+    constexpr uint32_t kTeams = 2u, kTeam = kRingThreads / kTeams;
+    __shared__ float scratch[kTeams][2][kTeam / kWarp];
     const uint32_t bytes = a.hidden * (kF32 ? 4u : 2u), more = a.residual != nullptr ? bytes : 0u;
     Ring ring;
-    ring.init(smem, stages, bytes + more, kTeam / kWarp);
+    ring.init(smem, stages, bytes + more, 0u, 1u, kTeam / kWarp, a.rows);
     pdl_wait();
     if (threadIdx.x >= kRingThreads) {
-        if (elect_one()) ring.fill(blockIdx.x, gridDim.x, a.rows, (const char *)a.x, bytes, (const char *)a.residual, more, nullptr, 0u);
+        if (elect_one()) {
+            ring.fill({{(const char *)a.x, (const char *)a.residual, nullptr}, {bytes, more, 0u}});
+            ring.drain();
+        }
     } else {
         const uint32_t t = threadIdx.x % kTeam, team = threadIdx.x / kTeam;
         auto first = [&](uint32_t v) { return (v * kTeam + t) * 8u; };
         Eight<false> w[kVectors];
 #pragma unroll
         for (uint32_t v = 0; v < kVectors; v++) w[v].template load<true>(a.weight, first(v), a.hidden);
-        uint32_t st = team % stages, ph = (team / stages) & 1u, turn = 0u;
         bool ok = true;
-        for (uint64_t row = blockIdx.x + (uint64_t)team * gridDim.x; row < a.rows; row += 2u * (uint64_t)gridDim.x, turn ^= 1u) {
-            ok = ok && mbar_wait(&ring.full[st], ph, ring.abort_flag);   // given up: the sums below still meet
-            const unsigned char *in = ring.base + st * ring.stage_bytes;
+        uint32_t turn = 0u;
+        Ring::Turn at{0u, 0u};
+        at.advance(team, stages);
+        for (uint64_t row = ring.first + team * ring.step; row < a.rows; row += kTeams * ring.step, turn ^= 1u) {
+            ok = ok && ring.wait(at);                                // given up: the sums below still meet
+            const unsigned char *in = ring.place(at);
             Eight<kF32> s[kVectors];
             float squares = 0.0f;
 #pragma unroll
@@ -439,9 +488,8 @@ __global__ void __launch_bounds__(kRingThreads + kWarp, 1) norm_ring_kernel(Norm
                 }
             }
             __syncwarp();
-            if (t % kWarp == 0u) mbar_arrive(&ring.empty[st]);
-            st += 2u;
-            if (st >= stages) { st -= stages; ph ^= 1u; }
+            if (t % kWarp == 0u) ring.release(at);
+            at.advance(kTeams, stages);
 #pragma unroll
             for (uint32_t v = 0; v < kVectors; v++) {
                 if (a.sum != nullptr) s[v].template store<true>((char *)a.sum + row * bytes, first(v), a.hidden);
@@ -460,66 +508,69 @@ __global__ void __launch_bounds__(kRingThreads + kWarp, 1) norm_ring_kernel(Norm
     if (threadIdx.x == 0u && *ring.abort_flag != 0u) atomicExch(&g_norm_status, 1u);
 }
 
-template <bool kF32, uint32_t kVectors>
-__global__ void __launch_bounds__(kRingThreads + kWarp, 1) norm_backward_ring_kernel(NormGradArgs a, uint32_t stages) {
+// A ring for each team.
+template <bool kF32, uint32_t kVectors, uint32_t kTeam>
+__global__ void __launch_bounds__(kRingThreads, 1) norm_backward_ring_kernel(NormGradArgs a, uint32_t stages) {
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ float scratch[2][kRingWarps];
+    constexpr uint32_t kTeams = kRingThreads / kTeam;
+    __shared__ float scratch[kTeams][2][kTeam / kWarp];
+    const uint32_t t = threadIdx.x % kTeam, team = threadIdx.x / kTeam;
     const uint32_t bytes = a.hidden * (kF32 ? 4u : 2u), more = a.d_sum != nullptr ? bytes : 0u;
+    const RowSources from = {{(const char *)a.dy, (const char *)a.sum, (const char *)a.d_sum}, {a.hidden * 2u, bytes, more}};
     Ring ring;
-    ring.init(smem, stages, a.hidden * 2u + bytes + more, kRingWarps);
+    ring.init(smem, stages, a.hidden * 2u + bytes + more, team, kTeams, 0u, a.rows);
     pdl_wait();
-    if (threadIdx.x >= kRingThreads) {
-        if (elect_one()) {
-            ring.fill(blockIdx.x, gridDim.x, a.rows, (const char *)a.dy, a.hidden * 2u, (const char *)a.sum, bytes, (const char *)a.d_sum, more);
-        }
-    } else {
-        const uint32_t t = threadIdx.x;
-        auto first = [&](uint32_t v) { return (v * kRingThreads + t) * 8u; };
-        Eight<false> w[kVectors];
-        float dw[kVectors][8];
+    if (t == 0u) {
+        for (uint32_t i = 0; i < stages; i++) ring.load_next(from);
+    }
+    auto first = [&](uint32_t v) { return (v * kTeam + t) * 8u; };
+    Eight<false> w[kVectors];
+    uint64_t dw[kVectors][4];
+#pragma unroll
+    for (uint32_t v = 0; v < kVectors; v++) {
+        w[v].template load<true>(a.weight, first(v), a.hidden);
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; i++) dw[v][i] = 0ull;
+    }
+    bool ok = true;
+    uint32_t turn = 0u;
+    Ring::Turn at{0u, 0u};
+    float next_rstd = ring.first < a.rows ? a.rstd[ring.first] : 0.0f;               // on its way while the row before is worked on
+    for (uint64_t row = ring.first; row < a.rows; row += ring.step, turn ^= 1u) {
+        const float rstd = next_rstd;
+        if (row + ring.step < a.rows) next_rstd = a.rstd[row + ring.step];
+        ok = ok && ring.wait(at);
+        const unsigned char *in = ring.place(at);
+        at.advance(1u, stages);
+        Eight<false> dy[kVectors];
+        Eight<kF32> s[kVectors], d[kVectors];
+        uint64_t dots = 0ull;
 #pragma unroll
         for (uint32_t v = 0; v < kVectors; v++) {
-            w[v].template load<true>(a.weight, first(v), a.hidden);
-#pragma unroll
-            for (uint32_t i = 0; i < 8u; i++) dw[v][i] = 0.0f;
+            dy[v].template load<true>(in, first(v), a.hidden);
+            s[v].template load<true>(in + a.hidden * 2u, first(v), a.hidden);
+            if (more != 0u) d[v].template load<true>(in + a.hidden * 2u + bytes, first(v), a.hidden);
         }
-        uint32_t st = 0u, ph = 0u, turn = 0u;
-        bool ok = true;
-        for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1u) {
-            const float rstd = a.rstd[row];
-            ok = ok && mbar_wait(&ring.full[st], ph, ring.abort_flag);
-            const unsigned char *in = ring.base + st * ring.stage_bytes;
-            Eight<false> dy[kVectors];
-            Eight<kF32> s[kVectors], d[kVectors];
-            float dot = 0.0f;
 #pragma unroll
-            for (uint32_t v = 0; v < kVectors; v++) {
-                dy[v].template load<true>(in, first(v), a.hidden);
-                s[v].template load<true>(in + a.hidden * 2u, first(v), a.hidden);
-                if (more != 0u) d[v].template load<true>(in + a.hidden * 2u + bytes, first(v), a.hidden);
-            }
-            __syncwarp();
-            if (t % kWarp == 0u) mbar_arrive(&ring.empty[st]);
-            if (++st == stages) { st = 0u; ph ^= 1u; }
+        for (uint32_t v = 0; v < kVectors; v++) dots = add_products<kF32>(dy[v], s[v], w[v], both2(rstd), dots, dw[v]);
+        const float mean = ring_sum<kTeam>(lo2(dots) + hi2(dots), scratch[team][turn]) / (float)a.hidden;
+        if (t == 0u) ring.load_next(from);
 #pragma unroll
-            for (uint32_t v = 0; v < kVectors; v++) dot = add_products<kF32>(dy[v], s[v], w[v], rstd, dot, dw[v]);
-            const float mean = ring_sum<kRingThreads>(dot, scratch[turn]) / (float)a.hidden;
-#pragma unroll
-            for (uint32_t v = 0; v < kVectors; v++) {
-                input_gradient<kF32>(dy[v], s[v], w[v], d[v], more != 0u, rstd, mean)
-                    .template store<true>((char *)a.dx + row * bytes, first(v), a.hidden);
-            }
-        }
-        if (a.partial != nullptr) {
-            float *to = a.partial + (uint64_t)blockIdx.x * a.hidden;
-#pragma unroll
-            for (uint32_t v = 0; v < kVectors; v++) {
-                if (first(v) >= a.hidden) continue;
-                *reinterpret_cast<float4 *>(to + first(v)) = make_float4(dw[v][0], dw[v][1], dw[v][2], dw[v][3]);
-                *reinterpret_cast<float4 *>(to + first(v) + 4u) = make_float4(dw[v][4], dw[v][5], dw[v][6], dw[v][7]);
-            }
+        for (uint32_t v = 0; v < kVectors; v++) {
+            input_gradient<kF32>(dy[v], s[v], w[v], d[v], more != 0u, both2(rstd), both2(-mean))
+                .template store<true>((char *)a.dx + row * bytes, first(v), a.hidden);
         }
     }
+    if (a.partial != nullptr) {
+        float *to = a.partial + ((uint64_t)blockIdx.x * kTeams + team) * a.hidden;
+#pragma unroll
+        for (uint32_t v = 0; v < kVectors; v++) {
+            if (first(v) >= a.hidden) continue;
+            *reinterpret_cast<ulonglong2 *>(to + first(v)) = make_ulonglong2(dw[v][0], dw[v][1]);
+            *reinterpret_cast<ulonglong2 *>(to + first(v) + 4u) = make_ulonglong2(dw[v][2], dw[v][3]);
+        }
+    }
+    if (t == 0u) ring.drain();
     pdl_trigger();
     __syncthreads();
     if (threadIdx.x == 0u && *ring.abort_flag != 0u) atomicExch(&g_norm_status, 1u);
@@ -548,17 +599,17 @@ bool by_ring_size(uint32_t hidden, F &&launch) {
     using std::integral_constant;
     return hidden <= 4096u ? launch(integral_constant<uint32_t, 1u>{}) : launch(integral_constant<uint32_t, 2u>{});
 }
-uint32_t ring_stages(uint32_t stage_bytes) { return std::min(kRingBytes / stage_bytes, kMaxStages); }
+uint32_t ring_stages(uint32_t stage_bytes, uint32_t rings) { return std::min(kRingBytes / stage_bytes, kMaxStages) / rings; }
 
 template <typename K, typename A>
-bool launch_ring(K kernel, const A &a, uint32_t blocks, uint32_t stage_bytes, cudaStream_t stream) {
-    const uint32_t stages = ring_stages(stage_bytes), bytes = 256u + stages * stage_bytes;
-    return set_max_dynamic_smem((const void *)kernel, 256u + kRingBytes) && launch_chained(kernel, blocks, kRingThreads + kWarp, bytes, stream, a, stages);
+bool launch_ring(K kernel, const A &a, uint32_t threads, uint32_t stage_bytes, uint32_t rings, cudaStream_t stream) {
+    const uint32_t stages = ring_stages(stage_bytes, rings), bytes = 256u + rings * stages * stage_bytes;
+    return set_max_dynamic_smem((const void *)kernel, 256u + kRingBytes) && launch_chained(kernel, (uint32_t)sm_count(), threads, bytes, stream, a, stages);
 }
 
 // The ring pays once every SM has a few rows.
 bool ring_suits(uint32_t rows, uint32_t hidden, bool vector, uint32_t stage_bytes) {
-    return vector && hidden > 1024u && hidden <= 8192u && rows >= 4u * (uint32_t)sm_count() && ring_stages(stage_bytes) >= 2u;
+    return vector && hidden > 1024u && hidden <= kRingHidden && rows >= 4u * (uint32_t)sm_count() && ring_stages(stage_bytes, 1u) >= 2u;
 }
 
 template <bool kF32>
@@ -566,7 +617,7 @@ bool launch_norm(const NormArgs &a, bool vector, cudaStream_t stream) {
     const uint32_t stage = a.hidden * (kF32 ? 4u : 2u) * (a.residual ? 2u : 1u);
     if (ring_suits(a.rows, a.hidden, vector, stage)) {
         return by_ring_size(a.hidden, [&](auto vectors) {
-            return launch_ring(norm_ring_kernel<kF32, 2u * decltype(vectors)::value>, a, (uint32_t)sm_count(), stage, stream);
+            return launch_ring(norm_ring_kernel<kF32, 2u * decltype(vectors)::value>, a, kRingThreads + kWarp, stage, 1u, stream);
         });
     }
     return by_size(a.hidden, [&](auto team, auto vectors) {
@@ -587,9 +638,14 @@ bool launch_backward(const NormGradArgs &a, bool vector, uint32_t &blocks, cudaS
     const uint32_t stage = a.hidden * (2u + (kF32 ? 4u : 2u) * (a.d_sum ? 2u : 1u));
     blocks = grad_blocks(a.rows, a.hidden);
     if (ring_suits(a.rows, a.hidden, vector, stage)) {
-        blocks = (uint32_t)sm_count();
+        // two rows at a time up to 4096 columns of bf16; more, and f32, have no registers for it (8192 x 7168 133 us, one 91)
+        const bool two = !kF32 && a.hidden <= 4096u;
+        blocks = (two ? 2u : 1u) * (uint32_t)sm_count();
+        if constexpr (!kF32) {
+            if (two) return launch_ring(norm_backward_ring_kernel<kF32, 2u, kRingThreads / 2u>, a, kRingThreads, stage, 2u, stream);
+        }
         return by_ring_size(a.hidden, [&](auto vectors) {
-            return launch_ring(norm_backward_ring_kernel<kF32, decltype(vectors)::value>, a, blocks, stage, stream);
+            return launch_ring(norm_backward_ring_kernel<kF32, decltype(vectors)::value, kRingThreads>, a, kRingThreads, stage, 1u, stream);
         });
     }
     return by_size(a.hidden, [&](auto team, auto vectors) {
