@@ -109,47 +109,98 @@ struct NormArgs {
     float epsilon;
 };
 
-// The normalised elements of a thread's vector to y, and to codes with the largest magnitude of the half warp's block.
-// All lanes of a warp call it; `live`: the row exists.
-template <bool kF32, bool kVector>
-K3_DEVINL void put_normed(const NormArgs &a, const Eight<kF32> &s, const Eight<false> &w, float rstd, uint64_t row, uint32_t c, bool live) {
+// Two neighbouring elements as f32.
+template <bool kF32>
+K3_DEVINL uint64_t pair_of(const Eight<kF32> &e, uint32_t i) { return pack2(e.value(2u * i), e.value(2u * i + 1u)); }
+
+constexpr uint32_t kSigns = 0x80008000u;                             // of two bf16
+K3_DEVINL void negate(Eight<false> &w) {
+#pragma unroll
+    for (uint32_t i = 0; i < 4u; i++) w.w[i] ^= kSigns;
+}
+// the largest of a and the magnitudes of b and c; NaN if one of them is
+K3_DEVINL float largest_of(float a, float b, float c) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// The normalised elements of a thread's vectors to y, and to codes with the largest magnitude of the half warp's block.
+// All lanes of a warp call it; `live`: the row exists.  minus_w: the weight's negatives, for the quotients want -y.  The
+// vectors go side by side through every step: one after the other, each with its shuffles and its reciprocal, 8192 x 7168
+// took 94 to 102 us.
+template <bool kF32, bool kVector, uint32_t kVectors, typename First>
+K3_DEVINL void put_normed(const NormArgs &a, const Eight<kF32> (&s)[kVectors], const Eight<false> (&minus_w)[kVectors], float rstd, uint64_t row,
+                          First first, bool live) {
     const uint32_t hidden = a.hidden, pitch = pitch_of(hidden);
-    float y[8];
+    const uint64_t rstd2 = both2(rstd);
+    uint64_t y[kVectors][4];                                         // negative
+    uint32_t most[kVectors];
 #pragma unroll
-    for (uint32_t i = 0; i < 8u; i++) y[i] = __fmul_rn(__fmul_rn(s.value(i), rstd), w.value(i));
+    for (uint32_t v = 0; v < kVectors; v++) {
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; i++) y[v][i] = mul2(mul2(pair_of(s[v], i), rstd2), pair_of(minus_w[v], i));
+    }
     if (a.y != nullptr) {
-        Eight<false> out;
-        out.set(y);
-        out.template store<kVector>(a.y + row * hidden, c, live ? hidden : 0u);
-    }
-    if (a.codes == nullptr) return;
-    uint32_t most = 0u;
 #pragma unroll
-    for (uint32_t i = 0; i < 8u; i++) {
-        // zeros past the row's end times a NaN rstd are NaN: they are no part of the block
-        if (column_of<kVector>(c, i) < hidden) most = max(most, __float_as_uint(y[i]) & 0x7fffffffu);
-    }
+        for (uint32_t v = 0; v < kVectors; v++) {
+            Eight<false> out;
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-    const float scale = scale_of(most), inverse = inverse_of(scale), lift = lift_of(scale), by = scale * lift;
-    uint32_t h[4];
-#pragma unroll
-    for (uint32_t i = 0; i < 4u; i++) {
-        h[i] = codes2(divided(y[2u * i] * lift, by, inverse), divided(y[2u * i + 1u] * lift, by, inverse));
-        if (column_of<kVector>(c, 2u * i) >= hidden) h[i] = 0u;      // zeros in the padding
-        else if (column_of<kVector>(c, 2u * i + 1u) >= hidden) h[i] &= 0xffu;
-    }
-    if (!live) return;
-    uint8_t *codes = a.codes + row * pitch;
-    if (kVector) {
-        if (c < pitch) *reinterpret_cast<uint2 *>(codes + c) = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
-    } else {
-#pragma unroll
-        for (uint32_t i = 0; i < 8u; i++) {
-            if (column_of<kVector>(c, i) < pitch) codes[column_of<kVector>(c, i)] = (uint8_t)(h[i / 2u] >> (8u * (i & 1u)));
+            for (uint32_t i = 0; i < 4u; i++) out.w[i] = bf16x2(lo2(y[v][i]), hi2(y[v][i])) ^ kSigns;
+            out.template store<kVector>(a.y + row * hidden, first(v), live ? hidden : 0u);
         }
     }
-    if (c < hidden && (c & 127u) == 0u) a.scales[row * scale_pitch_of(hidden) + c / kBlock] = scale;
+    if (a.codes == nullptr) return;
+#pragma unroll
+    for (uint32_t v = 0; v < kVectors; v++) {
+        const uint32_t c = first(v);
+        float largest = 0.0f;
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; i++) {
+            if (!kVector) {                                          // past the row's end: no part of the block, whatever rstd is
+                y[v][i] = pack2(column_of<kVector>(c, 2u * i) < hidden ? lo2(y[v][i]) : 0.0f,
+                                column_of<kVector>(c, 2u * i + 1u) < hidden ? hi2(y[v][i]) : 0.0f);
+            }
+            largest = largest_of(largest, lo2(y[v][i]), hi2(y[v][i]));
+        }
+        most[v] = kVector && c >= hidden ? 0u : __float_as_uint(largest);
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+#pragma unroll
+        for (uint32_t v = 0; v < kVectors; v++) most[v] = max(most[v], __shfl_xor_sync(0xffffffffu, most[v], o));
+    }
+    uint2 codes[kVectors];
+#pragma unroll
+    for (uint32_t v = 0; v < kVectors; v++) {
+        const float scale = scale_of(most[v]), lift = lift_of(scale);
+        const uint64_t by = both2(scale * lift), inverse = both2(-inverse_of(scale)), lift2 = both2(lift);
+        uint32_t h[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; i++) {
+            const uint64_t q = divided2(mul2(y[v][i], lift2), by, inverse);
+            h[i] = codes2(lo2(q), hi2(q));
+        }
+        codes[v] = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+        if (kVector && first(v) >= hidden) codes[v] = make_uint2(0u, 0u);            // zeros in the padding: the quotient is one of 0, or NaN
+        most[v] = __float_as_uint(scale);
+    }
+    if (!live) return;
+#pragma unroll
+    for (uint32_t v = 0; v < kVectors; v++) {
+        const uint32_t c = first(v);
+        uint8_t *to = a.codes + row * pitch;
+        if (kVector) {
+            if (c < pitch) *reinterpret_cast<uint2 *>(to + c) = codes[v];
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; i++) {
+                const uint32_t at = column_of<kVector>(c, i);
+                if (at < pitch) to[at] = at < hidden ? (uint8_t)((i < 4u ? codes[v].x : codes[v].y) >> (8u * (i & 3u))) : 0u;
+            }
+        }
+        if (c < hidden && (c & 127u) == 0u) a.scales[row * scale_pitch_of(hidden) + c / kBlock] = __uint_as_float(most[v]);
+    }
 }
 // The scales' row behind its blocks.  t: a thread's place in the row's team.
 K3_DEVINL void put_scale_padding(const NormArgs &a, uint64_t row, uint32_t t) {
@@ -205,7 +256,8 @@ __global__ void __launch_bounds__(threads_of(kTeam)) norm_kernel(NormArgs a) {
     const float rstd = 1.0f / sqrtf(squares / (float)a.hidden + a.epsilon);
     if (live && t == 0u && a.rstd != nullptr) a.rstd[row] = rstd;
 #pragma unroll
-    for (uint32_t v = 0; v < kVectors; v++) put_normed<kF32, kVector>(a, s[v], w[v], rstd, row, first(v), live);
+    for (uint32_t v = 0; v < kVectors; v++) negate(w[v]);
+    put_normed<kF32, kVector>(a, s, w, rstd, row, first, live);
     if (live) put_scale_padding(a, row, t);
     pdl_trigger();
 }
@@ -219,10 +271,6 @@ struct NormGradArgs {
     const float *rstd;
     uint32_t rows, hidden;
 };
-
-// Two neighbouring elements as f32.
-template <bool kF32>
-K3_DEVINL uint64_t pair_of(const Eight<kF32> &e, uint32_t i) { return pack2(e.value(2u * i), e.value(2u * i + 1u)); }
 
 // A vector's part of the row's sum of w dy s rstd, and of the weight's gradient, two elements at a time.
 template <bool kF32>
@@ -444,16 +492,29 @@ K3_DEVINL float ring_sum(float v, float *scratch) {
     return v;
 }
 
-// One ring, whose rows the two halves of the block take in turn.
-template <bool kF32, uint32_t kVectors>
+// One ring, whose rows the block's teams take in turn: a row's way (its sum, largest magnitudes, scales) takes longer than its
+// instructions, so several are under way.  Teams of 128 threads in bf16, of 256 in f32, which holds twice the words.
+// The stages are a multiple of the teams, so that a stage's rows are all of one team: it has taken out a stage's row before it
+// waits for the next one there, and a wait by parity never meets a phase that another team's row has yet to end.
+template <bool kF32, uint32_t kVectors, uint32_t kTeams>
 __global__ void __launch_bounds__(kRingThreads + kWarp, 1) norm_ring_kernel(NormArgs a, uint32_t stages) {
     extern __shared__ __align__(128) unsigned char smem[];
-    constexpr uint32_t kTeams = 2u, kTeam = kRingThreads / kTeams;
+    constexpr uint32_t kTeam = kRingThreads / kTeams;
+    constexpr uint32_t kTogether = kVectors < 4u ? kVectors : 4u;    // vectors side by side in put_normed
     __shared__ float scratch[kTeams][2][kTeam / kWarp];
     const uint32_t bytes = a.hidden * (kF32 ? 4u : 2u), more = a.residual != nullptr ? bytes : 0u;
     Ring ring;
     ring.init(smem, stages, bytes + more, 0u, 1u, kTeam / kWarp, a.rows);
     pdl_wait();
+    // the weight lies behind the ring: in registers it would be one in six of them
+    unsigned char *weight = ring.base + stages * ring.stage_bytes;
+    for (uint32_t c = threadIdx.x * 8u; c < a.hidden; c += blockDim.x * 8u) {
+        Eight<false> w;
+        w.template load<true>(a.weight, c, a.hidden);
+        negate(w);
+        w.template store<true>(weight, c, a.hidden);
+    }
+    __syncthreads();
     if (threadIdx.x >= kRingThreads) {
         if (elect_one()) {
             ring.fill({{(const char *)a.x, (const char *)a.residual, nullptr}, {bytes, more, 0u}});
@@ -462,13 +523,9 @@ __global__ void __launch_bounds__(kRingThreads + kWarp, 1) norm_ring_kernel(Norm
     } else {
         const uint32_t t = threadIdx.x % kTeam, team = threadIdx.x / kTeam;
         auto first = [&](uint32_t v) { return (v * kTeam + t) * 8u; };
-        Eight<false> w[kVectors];
-#pragma unroll
-        for (uint32_t v = 0; v < kVectors; v++) w[v].template load<true>(a.weight, first(v), a.hidden);
         bool ok = true;
         uint32_t turn = 0u;
-        Ring::Turn at{0u, 0u};
-        at.advance(team, stages);
+        Ring::Turn at{team, 0u};
         for (uint64_t row = ring.first + team * ring.step; row < a.rows; row += kTeams * ring.step, turn ^= 1u) {
             ok = ok && ring.wait(at);                                // given up: the sums below still meet
             const unsigned char *in = ring.place(at);
@@ -499,7 +556,16 @@ __global__ void __launch_bounds__(kRingThreads + kWarp, 1) norm_ring_kernel(Norm
             const float rstd = 1.0f / sqrtf(ring_sum<kTeam>(squares, scratch[team][turn]) / (float)a.hidden + a.epsilon);
             if (t == 0u && a.rstd != nullptr) a.rstd[row] = rstd;
 #pragma unroll
-            for (uint32_t v = 0; v < kVectors; v++) put_normed<kF32, true>(a, s[v], w[v], rstd, row, first(v), true);
+            for (uint32_t v = 0; v < kVectors; v += kTogether) {
+                Eight<kF32> some[kTogether];
+                Eight<false> w[kTogether];
+#pragma unroll
+                for (uint32_t i = 0; i < kTogether; i++) {
+                    some[i] = s[v + i];
+                    w[i].template load<true>(weight, first(v + i), a.hidden);
+                }
+                put_normed<kF32, true>(a, some, w, rstd, row, [&](uint32_t i) { return first(v + i); }, true);
+            }
             put_scale_padding(a, row, t);
         }
     }
@@ -599,25 +665,29 @@ bool by_ring_size(uint32_t hidden, F &&launch) {
     using std::integral_constant;
     return hidden <= 4096u ? launch(integral_constant<uint32_t, 1u>{}) : launch(integral_constant<uint32_t, 2u>{});
 }
-uint32_t ring_stages(uint32_t stage_bytes, uint32_t rings) { return std::min(kRingBytes / stage_bytes, kMaxStages) / rings; }
+// Stages for each of `teams`.
+uint32_t team_stages(uint32_t stage_bytes, uint32_t teams) { return std::min(kRingBytes / stage_bytes, kMaxStages) / teams; }
 
 template <typename K, typename A>
-bool launch_ring(K kernel, const A &a, uint32_t threads, uint32_t stage_bytes, uint32_t rings, cudaStream_t stream) {
-    const uint32_t stages = ring_stages(stage_bytes, rings), bytes = 256u + rings * stages * stage_bytes;
-    return set_max_dynamic_smem((const void *)kernel, 256u + kRingBytes) && launch_chained(kernel, (uint32_t)sm_count(), threads, bytes, stream, a, stages);
+bool launch_ring(K kernel, const A &a, uint32_t threads, uint32_t stage_bytes, uint32_t rings, uint32_t stages, cudaStream_t stream) {
+    const uint32_t bytes = 256u + rings * stages * stage_bytes + a.hidden * 2u;
+    return set_max_dynamic_smem((const void *)kernel, 256u + kRingBytes + kRingHidden * 2u) &&
+           launch_chained(kernel, (uint32_t)sm_count(), threads, bytes, stream, a, stages);
 }
 
 // The ring pays once every SM has a few rows.
-bool ring_suits(uint32_t rows, uint32_t hidden, bool vector, uint32_t stage_bytes) {
-    return vector && hidden > 1024u && hidden <= kRingHidden && rows >= 4u * (uint32_t)sm_count() && ring_stages(stage_bytes, 1u) >= 2u;
+bool ring_suits(uint32_t rows, uint32_t hidden, bool vector) {
+    return vector && hidden > 1024u && hidden <= kRingHidden && rows >= 4u * (uint32_t)sm_count();
 }
 
 template <bool kF32>
 bool launch_norm(const NormArgs &a, bool vector, cudaStream_t stream) {
     const uint32_t stage = a.hidden * (kF32 ? 4u : 2u) * (a.residual ? 2u : 1u);
-    if (ring_suits(a.rows, a.hidden, vector, stage)) {
+    constexpr uint32_t kTeams = kF32 ? 2u : 4u;
+    const uint32_t stages = team_stages(stage, kTeams) * kTeams;
+    if (ring_suits(a.rows, a.hidden, vector) && stages != 0u) {
         return by_ring_size(a.hidden, [&](auto vectors) {
-            return launch_ring(norm_ring_kernel<kF32, 2u * decltype(vectors)::value>, a, kRingThreads + kWarp, stage, 1u, stream);
+            return launch_ring(norm_ring_kernel<kF32, decltype(vectors)::value * kTeams, kTeams>, a, kRingThreads + kWarp, stage, 1u, stages, stream);
         });
     }
     return by_size(a.hidden, [&](auto team, auto vectors) {
@@ -637,15 +707,17 @@ template <bool kF32>
 bool launch_backward(const NormGradArgs &a, bool vector, uint32_t &blocks, cudaStream_t stream) {
     const uint32_t stage = a.hidden * (2u + (kF32 ? 4u : 2u) * (a.d_sum ? 2u : 1u));
     blocks = grad_blocks(a.rows, a.hidden);
-    if (ring_suits(a.rows, a.hidden, vector, stage)) {
-        // two rows at a time up to 4096 columns of bf16; more, and f32, have no registers for it (8192 x 7168 133 us, one 91)
-        const bool two = !kF32 && a.hidden <= 4096u;
-        blocks = (two ? 2u : 1u) * (uint32_t)sm_count();
+    // two rows at a time up to 4096 columns of bf16; more, and f32, have no registers for it (8192 x 7168 133 us, one 91)
+    const uint32_t teams = !kF32 && a.hidden <= 4096u ? 2u : 1u, stages = team_stages(stage, teams);
+    if (ring_suits(a.rows, a.hidden, vector) && stages >= 2u) {
+        blocks = teams * (uint32_t)sm_count();
         if constexpr (!kF32) {
-            if (two) return launch_ring(norm_backward_ring_kernel<kF32, 2u, kRingThreads / 2u>, a, kRingThreads, stage, 2u, stream);
+            if (teams == 2u) {
+                return launch_ring(norm_backward_ring_kernel<kF32, 2u, kRingThreads / 2u>, a, kRingThreads, stage, 2u, stages, stream);
+            }
         }
         return by_ring_size(a.hidden, [&](auto vectors) {
-            return launch_ring(norm_backward_ring_kernel<kF32, decltype(vectors)::value, kRingThreads>, a, kRingThreads, stage, 1u, stream);
+            return launch_ring(norm_backward_ring_kernel<kF32, decltype(vectors)::value, kRingThreads>, a, kRingThreads, stage, 1u, stages, stream);
         });
     }
     return by_size(a.hidden, [&](auto team, auto vectors) {

@@ -60,7 +60,7 @@ class GroupedProduct:
         to, add = _output(x, (rows, columns), dtype, out, into)
         _placed((name, x), ("offsets", offsets), ("out", out), ("into", into), tables=self._device)
         if to is None:
-            to = x.new_empty((rows, columns), dtype=dtype)
+            to = torch.empty(rows, columns, dtype=dtype, device=x.device)
         if rows:
             ws = self._workspace.of(rows, x.device)
             _done(getattr(ops, call)(to, x, self.w, offsets, rows, self.groups, self.n, self.k, _OUT[to.dtype], add, ws,
@@ -101,7 +101,7 @@ class GroupedWeightGradient:
                 return dy.new_zeros(shape, dtype=dtype)
             return to if add else to.zero_()
         if to is None:
-            to = dy.new_empty(shape, dtype=dtype)
+            to = torch.empty(*shape, dtype=dtype, device=dy.device)
         ws = self._workspace.of(rows, dy.device)
         _done(ops.k3_moe_grouped_by_weight(to, dy, x, offsets, rows, self.groups, self.n, self.k, _OUT[to.dtype], add, ws,
                                            self._workspace.bytes), "k3_moe_grouped_by_weight")

@@ -45,11 +45,14 @@ class RmsNorm:
         if not (y or codes):
             raise ValueError("y and codes: one of them at least")
         _placed(("x", x), ("residual", residual), tables=self._device)
-        total = x if residual is None else torch.empty_like(x)       # a third less of the host's time than new_empty
-        out = x.new_empty((rows, hidden), dtype=torch.bfloat16) if y else None
-        q = x.new_empty((rows, pitch(hidden)), dtype=torch.float8_e4m3fn) if codes else None
-        scales = x.new_empty((rows, scale_pitch(hidden)), dtype=torch.float32) if codes else None
-        rstd = x.new_empty(rows, dtype=torch.float32)
+        # sizes one by one and empty_like: 1.3 to 1.5 us of the host's time each, new_empty of a tuple 1.9
+        total = x if residual is None else torch.empty_like(x)
+        out = torch.empty_like(x, dtype=torch.bfloat16) if y else None
+        q = scales = None
+        if codes:
+            q = torch.empty(rows, pitch(hidden), dtype=torch.float8_e4m3fn, device=x.device)
+            scales = torch.empty(rows, scale_pitch(hidden), dtype=torch.float32, device=x.device)
+        rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
         if rows:
             _done(ops.k3_moe_norm(None if residual is None else total, out, q, scales, rstd, x, residual, self.weight, rows, hidden,
                                   _TYPES[x.dtype], self.epsilon), "k3_moe_norm")
