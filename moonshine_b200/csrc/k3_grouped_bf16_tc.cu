@@ -671,8 +671,9 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     continue;
                 }
                 // 32 x 32 at a time through shared memory: rows of the output, units of 16 bytes, permuted by the row.  This
-                // thread then stores a unit of every kApart-th row; where that goes is worked out once per half (with the
-                // products in every store the weight's gradient of 32 groups of 16 rows of 2048 x 7168 took 288 us, now %%).
+                // thread then stores a unit of every kApart-th row; where that goes is worked out once per half (results of
+                // 32 groups of 16 rows by 2048 x 7168, without the stores themselves: 150 us, with the products for the address in
+                // every store 280; with them 287, the rate of the memory).
                 constexpr uint32_t kUnits = kF32 ? 8u : 4u, kApart = 32u / kUnits, kSize = kF32 ? 4u : 2u;
                 auto unit = [&](uint32_t row, uint32_t u) {
                     return mine + row * (kUnits * 16u) + ((u ^ (kF32 ? row & 7u : (row >> 1) & 3u)) * 16u);

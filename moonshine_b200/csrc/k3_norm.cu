@@ -22,7 +22,7 @@ constexpr uint32_t kMaxHidden = 16384;
 
 // Eight elements of a row as they lie in memory.  kVector: neighbours, c .. c + 7, of rows that start on 16 bytes and are
 // whole vectors.  Otherwise c, c + 16, .. c + 112: the half warp still holds a block of 128, and its 16 lanes read
-// neighbours (rows of 3583 f32: the gradient 30.8 us of 1021 rows with eight neighbours per thread, now %%).
+// neighbours (rows of 3583 f32: the gradient of 1021 rows 20.7 us, 30.8 with eight neighbours per thread).
 template <bool kVector>
 K3_DEVINL constexpr uint32_t column_of(uint32_t c, uint32_t i) { return kVector ? c + i : c + 16u * i; }
 // the first column of a thread's vector: thread `at` of those that lie along the row
@@ -126,9 +126,9 @@ K3_DEVINL float largest_of(float a, float b, float c) {
 }
 
 // The normalised elements of a thread's vectors to y, and to codes with the largest magnitude of the half warp's block.
-// All lanes of a warp call it; `live`: the row exists.  minus_w: the weight's negatives, for the quotients want -y.  The
-// vectors go side by side through every step: one after the other, each with its shuffles and its reciprocal, 8192 x 7168
-// took 94 to 102 us.
+// All lanes of a warp call it; `live`: the row exists.  minus_w: the weight's negatives, for the quotients want -y.  Two
+// elements at a time and the vectors side by side through every step, 8192 x 7168 to codes alone takes 58 us; element by
+// element, and one vector after the other with its shuffles and its reciprocal, it took 78.
 template <bool kF32, bool kVector, uint32_t kVectors, typename First>
 K3_DEVINL void put_normed(const NormArgs &a, const Eight<kF32> (&s)[kVectors], const Eight<false> (&minus_w)[kVectors], float rstd, uint64_t row,
                           First first, bool live) {
@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(256) norm_weight_kernel(float *d_weight, const
 // stages in shared memory with whole rows, up to 192 KB per block, so that memory is never waited for while a row's sum goes
 // around the team.  Forward a seventeenth warp fills the ring and a stage is free once its row is in registers.  Backward,
 // where that warp would leave 96 registers per thread instead of 128, a thread of the team fills it when the sum is there.
-// (Forward that way 8192 x 7168 takes 101 us, with the warp 92; backward 91 and 96, in f32 4096 x 7168 76 and 90.)
+// (Forward that way 8192 x 7168 took 101 us, with the warp 92; backward 91 and 96, in f32 4096 x 7168 76 and 90.)
 constexpr uint32_t kRingThreads = 512, kRingBytes = 196608, kRingHidden = 8192, kMaxStages = 8;
 
 __device__ uint32_t g_norm_status = 0;
@@ -500,7 +500,7 @@ template <bool kF32, uint32_t kVectors, uint32_t kTeams>
 __global__ void __launch_bounds__(kRingThreads + kWarp, 1) norm_ring_kernel(NormArgs a, uint32_t stages) {
     extern __shared__ __align__(128) unsigned char smem[];
     constexpr uint32_t kTeam = kRingThreads / kTeams;
-    constexpr uint32_t kTogether = kVectors < 4u ? kVectors : 4u;    // vectors side by side in put_normed
+    constexpr uint32_t kTogether = kVectors < 2u ? kVectors : 2u;    // vectors side by side in put_normed: with four 12 bytes spill
     __shared__ float scratch[kTeams][2][kTeam / kWarp];
     const uint32_t bytes = a.hidden * (kF32 ? 4u : 2u), more = a.residual != nullptr ? bytes : 0u;
     Ring ring;
