@@ -14,9 +14,13 @@
  * hold (NaN, say) enters nothing.  An offset past `rows` counts as `rows`, one
  * below its predecessor ends an empty group; nothing outside is read or written.
  *
- * Sums are f32 (tensor cores), rounded once to the output's type.  Their order
- * depends on the sizes of the call and the size of the row's group, not on which
- * SM takes what: the same call gives the same bits.  What is not finite in a row
+ * Sums are f32, rounded once to the output's type.  The tensor cores cut an
+ * addition of 16 products off instead of rounding it; f32 outputs lie about 1e-6
+ * of their norm from the exact ones whatever the depth (by weight 4e-6 for a
+ * group of 4096 rows where the average is below 1088), bf16 outputs within their
+ * rounding.
+ * The order of the sums depends on the sizes of the call and the size of the
+ * row's group, not on which SM takes what: the same call gives the same bits.  What is not finite in a row
  * or a matrix makes the results that it enters not finite, and no others.
  *
  * Any n and k are taken.  Matrices whose rows are whole units of 16 bytes (n and

@@ -108,6 +108,29 @@ def test_larger(form, n, k, rows, groups):
         check(run(form, x, dy, w, on_device(offsets), dtype=dtype), value, size, depth_of(form, n, k, offsets), dtype)
 
 
+@pytest.mark.parametrize("form", ["forward", "by_input"])
+@pytest.mark.parametrize("rows", [8, 300, 2500])
+@pytest.mark.parametrize("depth", [1024, 1025 * 8, 7168])
+def test_deep_sums_in_f32(form, rows, depth):
+    """An accumulator takes 64 additions of 16 products, each cut off by 2^-23 of the sum at most, then segments are added
+    with rounding (at most 9 here): 64 x 2^-23 and 9 x 2^-24 of what has been summed, which is below the result's norm."""
+    wide = 520
+    x, dy, w = inputs(rows + depth, rows, 1, *((wide, depth) if form == "forward" else (depth, wide)))
+    value, _ = reference(form, x, dy, w, [0, rows])
+    got = run(form, x, dy, w, on_device([0, rows]), dtype=F32)
+    assert float((got.double() - value).norm() / value.norm()) <= 64 * 2.0 ** -23 + 9 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("n,k,groups,rows", [(520, 264, 1, 3001), (2048, 1032, 6, 9011), (72, 40, 4, 30000)])
+def test_deep_gradients_in_f32(n, k, groups, rows):
+    """The same of the weight's gradient, whose depth is a group's rows (here equally many)."""
+    x, dy, w = inputs(rows, rows, groups, n, k)
+    offsets = [rows * i // groups for i in range(groups + 1)]
+    value, _ = reference("by_weight", x, dy, w, offsets)
+    got = run("by_weight", x, dy, w, on_device(offsets), dtype=F32)
+    assert float((got.double() - value).norm() / value.norm()) <= 64 * 2.0 ** -23 + 31 * 2.0 ** -24
+
+
 @pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("groups", [1, 1000, 1024])
 def test_numbers_of_groups(form, groups):
