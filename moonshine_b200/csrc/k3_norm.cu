@@ -493,7 +493,7 @@ K3_DEVINL float ring_sum(float v, float *scratch) {
 }
 
 // One ring, whose rows the block's teams take in turn: a row's way (its sum, largest magnitudes, scales) takes longer than its
-// instructions, so several are under way.  Teams of 128 threads in bf16, of 256 in f32, which holds twice the words.
+// instructions, so several are under way.  Teams of 128 threads or, in f32, which holds twice the words, 256.
 // The stages are a multiple of the teams, so that a stage's rows are all of one team: it has taken out a stage's row before it
 // waits for the next one there, and a wait by parity never meets a phase that another team's row has yet to end.
 template <bool kF32, uint32_t kVectors, uint32_t kTeams>
@@ -683,12 +683,22 @@ bool ring_suits(uint32_t rows, uint32_t hidden, bool vector) {
 template <bool kF32>
 bool launch_norm(const NormArgs &a, bool vector, cudaStream_t stream) {
     const uint32_t stage = a.hidden * (kF32 ? 4u : 2u) * (a.residual ? 2u : 1u);
-    constexpr uint32_t kTeams = kF32 ? 2u : 4u;
-    const uint32_t stages = team_stages(stage, kTeams) * kTeams;
-    if (ring_suits(a.rows, a.hidden, vector) && stages != 0u) {
+    // With the sum, bf16 rows and codes written the memory serves all better with no more than 64 KB of reads under way per SM
+    // (8192 x 7168 92 us, with 115 KB 98 to 100); with fewer of them four teams and 115 KB are better (without the sum 61 us,
+    // the other way 70; without the bf16 rows 77, the other way 80).
+    const bool all = a.sum != nullptr && a.y != nullptr && a.codes != nullptr;
+    auto ring = [&](auto teams) {
+        constexpr uint32_t kTeams = decltype(teams)::value;
+        const uint32_t held = team_stages(stage, kTeams), stages = (all ? std::min(held, std::max(1u, 65536u / stage / kTeams)) : held) * kTeams;
         return by_ring_size(a.hidden, [&](auto vectors) {
             return launch_ring(norm_ring_kernel<kF32, decltype(vectors)::value * kTeams, kTeams>, a, kRingThreads + kWarp, stage, 1u, stages, stream);
         });
+    };
+    if (ring_suits(a.rows, a.hidden, vector) && team_stages(stage, 2u) != 0u) {
+        if constexpr (!kF32) {
+            if (!all) return ring(std::integral_constant<uint32_t, 4u>{});
+        }
+        return ring(std::integral_constant<uint32_t, 2u>{});
     }
     return by_size(a.hidden, [&](auto team, auto vectors) {
         constexpr uint32_t kTeam = decltype(team)::value, kThreads = threads_of(kTeam), kTeams = kThreads / kTeam;
