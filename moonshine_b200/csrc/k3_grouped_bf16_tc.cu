@@ -4,19 +4,31 @@
 //   forward    A = w_g   [n, k], m a feature of the output, c a row of the group, r < k
 //   by input   A = w_g^T [k, n], m a feature of the input,  c a row of the group, r < n
 //   by weight  A = dy^T  [n, rows], B = x^T [k, rows],      r a row of the group
-// A group's rows are the N extent of the first two, which takes any multiple of 16: a group of 130 rows costs a tile
-// of 160, where rows as lanes would cost 256.  What lies in memory with its depth in neighbouring rows (w by input,
-// both operands by weight) goes to shared memory as it is and is read "MN-major".
+// A group's rows are the N extent of the first two, which takes any multiple of 16 (pairs of blocks: 32): a group of 130
+// rows costs a tile of 144, where rows as lanes would cost 256.  What lies in memory with its depth in neighbouring rows
+// (w by input, both operands by weight) goes to shared memory as it is and is read "MN-major".
 //
 // An item is kHalves x 128 lanes by up to kMaxN columns over the whole depth, 64 of it per stage.  One block per SM:
 //   warp 0       loads by TMA
-//   warp 1       MMA issuer, owns the tensor memory: an accumulator of kMaxN columns for each of two halves
+//   warp 1       MMA issuer, owns the tensor memory: two accumulators of kMaxN columns, for the item's two halves or, where
+//                it has one, for two items in turn
 //   warp 2       draws items from a counter and tells the others, when the loads of the one before come to an end
 //   warp 3       by weight: clears what a group's first stage holds of the rows behind its part of the group
 //   warps 4-11   results: lane quadrant warp % 4, every second chunk of 32 columns; the accumulator is free again once
 //                it is in registers, before anything is stored
 // Items that share a matrix are neighbours in the order, so it is in L2 for all but one of them.  Their results do not
 // depend on who draws what.
+//
+// kCtas 2: a pair of blocks (cta_group::2) shares an item of twice the lanes.  Each loads its lanes and half of the columns,
+// which both tensor cores read, so the columns come from L2 once for two SMs; the first block draws, waits and issues.
+// Arrivals across the pair carry no release where nothing written is handed over: a release waits for the warp's stores, and
+// the weight's gradient of 32 groups of 128 rows took 409 us with it and 318 without.
+// kSplit: a cluster of up to eight blocks shares an item's depth and adds its sums through distributed shared memory.
+//
+// What bounds it.  Large calls: power.  64 groups of 512 rows, 2048 x 7168, 20 in a row: 670 to 710 us = 1360 to 1440 TFLOP/s;
+// for seconds 776 us = 1240 at 990 W and 1170 MHz, where the tensor pipes are busy 0.87 of the time (the library's plain
+// product of 32768 rows: 1323 TFLOP/s at 988 W, 1282 MHz, 0.85; it reads 0.5 GB where 64 matrices are 2.3).  Few rows per
+// group: the matrices' bytes, 6.2 to 6.9 TB/s.
 //
 // Every wait is bounded; on give-up the block raises the status word, waits for its copies and frees its tensor memory.
 #include "k3_fp8_ptx.cuh"

@@ -5,7 +5,9 @@
 //
 // Bound by memory: a row is read once, kept in registers over the row's sum, and written once.  A row belongs to a
 // warp (up to 1024 columns) or to a block of 256 or 1024 threads; a thread holds vectors of 8 neighbouring columns,
-// so the 16 lanes of half a warp hold a block of 128, whose largest magnitude is four shuffles away.
+// so the 16 lanes of half a warp hold a block of 128, whose largest magnitude is four shuffles away.  Many rows go through a
+// ring in shared memory (below).  8192 x 7168 bf16: forward with sum, bf16 rows and codes 92 us, 5.7 TB/s; backward with the
+// weight's gradient 82 us, 5.7 TB/s.
 #include "k3_common.cuh"
 #include "k3_fp8_ptx.cuh"
 #include "k3_grouped.h"
@@ -384,11 +386,11 @@ __global__ void __launch_bounds__(256) norm_weight_kernel(float *d_weight, const
 }
 
 // ------------------------------------------------------------------------------------- rows through a ring
-// Many rows of more than 1024 columns: one block per SM, in one or two teams that take a row each in turn, from a ring of
-// stages in shared memory with whole rows, up to 192 KB per block, so that memory is never waited for while a row's sum goes
-// around the team.  Forward a seventeenth warp fills the ring and a stage is free once its row is in registers.  Backward,
-// where that warp would leave 96 registers per thread instead of 128, a thread of the team fills it when the sum is there.
-// (Forward that way 8192 x 7168 took 101 us, with the warp 92; backward 91 and 96, in f32 4096 x 7168 76 and 90.)
+// The gradient of many rows of more than 1024 columns: one block per SM, in one or two teams that take a row each in turn, so
+// that the weight's gradient stays in registers, from a ring of stages in shared memory with whole rows, up to 192 KB per
+// block, so that memory is never waited for while a row's sum goes around the team.  A thread of the team fills the ring: a
+// stage is free once its row's sum is there.  (A seventeenth warp for that would leave 96 registers per thread instead of 128:
+// 8192 x 7168 96 us; without a ring 136.)  Forward nothing stays from row to row, and a block per row needs no ring.
 constexpr uint32_t kRingThreads = 512, kRingBytes = 196608, kRingHidden = 8192, kMaxStages = 8;
 
 __device__ uint32_t g_norm_status = 0;
@@ -416,21 +418,18 @@ struct Ring {
         }
     };
     unsigned char *base;
-    uint64_t *full, *empty;
+    uint64_t *full;
     volatile uint32_t *abort_flag;
     uint32_t stages, stage_bytes;
     Turn next;                               // of the thread that loads
     uint64_t first, step, next_row, rows;
 
-    // Ring `at` of `rings` in the block; readers: warps that take a row out of its stage, 0 where a barrier of theirs says
-    // that they have.  All threads of the block.
-    K3_DEVINL void init(unsigned char *smem, uint32_t stages_, uint32_t stage_bytes_, uint32_t at, uint32_t rings, uint32_t readers,
-                        uint64_t rows_) {
+    // ring `at` of `rings` in the block; all threads of the block
+    K3_DEVINL void init(unsigned char *smem, uint32_t stages_, uint32_t stage_bytes_, uint32_t at, uint32_t rings, uint64_t rows_) {
         stages = stages_;
         stage_bytes = stage_bytes_;
         full = reinterpret_cast<uint64_t *>(smem) + at * stages;
-        empty = full + kMaxStages;
-        abort_flag = reinterpret_cast<uint32_t *>(smem + 16u * kMaxStages);
+        abort_flag = reinterpret_cast<uint32_t *>(smem + 8u * kMaxStages);
         base = smem + 256u + at * stages * stage_bytes;
         next = {0u, 0u};
         first = next_row = blockIdx.x + (uint64_t)at * gridDim.x;
@@ -438,17 +437,14 @@ struct Ring {
         rows = rows_;
         if (threadIdx.x == 0u) {
             *abort_flag = 0u;
-            for (uint32_t s = 0; s < stages * rings; s++) {
-                mbar_init(&full[s], 1);
-                if (readers != 0u) mbar_init(&empty[s], readers);
-            }
+            for (uint32_t s = 0; s < stages * rings; s++) mbar_init(&full[s], 1);
             fence_barrier_init();
         }
         __syncthreads();
     }
-    // one thread: the next row into its stage, which is free; false if there is none
-    K3_DEVINL bool load_next(const RowSources &from) {
-        if (next_row >= rows || *abort_flag != 0u) return false;
+    // one thread: the next row, if there is one, into its stage, which is free
+    K3_DEVINL void load_next(const RowSources &from) {
+        if (next_row >= rows || *abort_flag != 0u) return;
         unsigned char *to = base + next.s * stage_bytes;
         mbar_arrive_expect_tx(&full[next.s], stage_bytes);
 #pragma unroll
@@ -459,16 +455,10 @@ struct Ring {
         }
         next.advance(1u, stages);
         next_row += step;
-        return true;
-    }
-    // one thread: all rows, as stages become free
-    K3_DEVINL void fill(const RowSources &from) {
-        while (mbar_wait(&empty[next.s], next.ph ^ 1u, abort_flag) && load_next(from)) {}
     }
     // a row is in its stage; false: given up
     K3_DEVINL bool wait(const Turn &t) { return mbar_wait(&full[t.s], t.ph, abort_flag); }
     K3_DEVINL const unsigned char *place(const Turn &t) const { return base + t.s * stage_bytes; }
-    K3_DEVINL void release(const Turn &t) { mbar_arrive(&empty[t.s]); }              // one thread of each reader
     // the thread that loads, at its end: nothing may land in a block that has left.  The last use of each stage.
     K3_DEVINL void drain() {
         if (*abort_flag == 0u) return;
@@ -492,89 +482,8 @@ K3_DEVINL float ring_sum(float v, float *scratch) {
     return v;
 }
 
-// One ring, whose rows the block's teams take in turn: a row's way (its sum, largest magnitudes, scales) takes longer than its
-// instructions, so several are under way.  Teams of 128 threads or, in f32, which holds twice the words, 256.
-// The stages are a multiple of the teams, so that a stage's rows are all of one team: it has taken out a stage's row before it
-// waits for the next one there, and a wait by parity never meets a phase that another team's row has yet to end.
-template <bool kF32, uint32_t kVectors, uint32_t kTeams>
-__global__ void __launch_bounds__(kRingThreads + kWarp, 1) norm_ring_kernel(NormArgs a, uint32_t stages) {
-    extern __shared__ __align__(128) unsigned char smem[];
-    constexpr uint32_t kTeam = kRingThreads / kTeams;
-    constexpr uint32_t kTogether = kVectors < 2u ? kVectors : 2u;    // vectors side by side in put_normed: with four 12 bytes spill
-    __shared__ float scratch[kTeams][2][kTeam / kWarp];
-    const uint32_t bytes = a.hidden * (kF32 ? 4u : 2u), more = a.residual != nullptr ? bytes : 0u;
-    Ring ring;
-    ring.init(smem, stages, bytes + more, 0u, 1u, kTeam / kWarp, a.rows);
-    pdl_wait();
-    // the weight lies behind the ring: in registers it would be one in six of them
-    unsigned char *weight = ring.base + stages * ring.stage_bytes;
-    for (uint32_t c = threadIdx.x * 8u; c < a.hidden; c += blockDim.x * 8u) {
-        Eight<false> w;
-        w.template load<true>(a.weight, c, a.hidden);
-        negate(w);
-        w.template store<true>(weight, c, a.hidden);
-    }
-    __syncthreads();
-    if (threadIdx.x >= kRingThreads) {
-        if (elect_one()) {
-            ring.fill({{(const char *)a.x, (const char *)a.residual, nullptr}, {bytes, more, 0u}});
-            ring.drain();
-        }
-    } else {
-        const uint32_t t = threadIdx.x % kTeam, team = threadIdx.x / kTeam;
-        auto first = [&](uint32_t v) { return (v * kTeam + t) * 8u; };
-        bool ok = true;
-        uint32_t turn = 0u;
-        Ring::Turn at{team, 0u};
-        for (uint64_t row = ring.first + team * ring.step; row < a.rows; row += kTeams * ring.step, turn ^= 1u) {
-            ok = ok && ring.wait(at);                                // given up: the sums below still meet
-            const unsigned char *in = ring.place(at);
-            Eight<kF32> s[kVectors];
-            float squares = 0.0f;
-#pragma unroll
-            for (uint32_t v = 0; v < kVectors; v++) s[v].template load<true>(in, first(v), a.hidden);
-            if (more != 0u) {
-#pragma unroll
-                for (uint32_t v = 0; v < kVectors; v++) {
-                    Eight<kF32> r;
-                    r.template load<true>(in + bytes, first(v), a.hidden);
-                    float f[8];
-#pragma unroll
-                    for (uint32_t i = 0; i < 8u; i++) f[i] = s[v].value(i) + r.value(i);
-                    s[v].set(f);
-                }
-            }
-            __syncwarp();
-            if (t % kWarp == 0u) ring.release(at);
-            at.advance(kTeams, stages);
-#pragma unroll
-            for (uint32_t v = 0; v < kVectors; v++) {
-                if (a.sum != nullptr) s[v].template store<true>((char *)a.sum + row * bytes, first(v), a.hidden);
-#pragma unroll
-                for (uint32_t i = 0; i < 8u; i++) squares = fmaf(s[v].value(i), s[v].value(i), squares);
-            }
-            const float rstd = 1.0f / sqrtf(ring_sum<kTeam>(squares, scratch[team][turn]) / (float)a.hidden + a.epsilon);
-            if (t == 0u && a.rstd != nullptr) a.rstd[row] = rstd;
-#pragma unroll
-            for (uint32_t v = 0; v < kVectors; v += kTogether) {
-                Eight<kF32> some[kTogether];
-                Eight<false> w[kTogether];
-#pragma unroll
-                for (uint32_t i = 0; i < kTogether; i++) {
-                    some[i] = s[v + i];
-                    w[i].template load<true>(weight, first(v + i), a.hidden);
-                }
-                put_normed<kF32, true>(a, some, w, rstd, row, [&](uint32_t i) { return first(v + i); }, true);
-            }
-            put_scale_padding(a, row, t);
-        }
-    }
-    pdl_trigger();
-    __syncthreads();
-    if (threadIdx.x == 0u && *ring.abort_flag != 0u) atomicExch(&g_norm_status, 1u);
-}
-
-// A ring for each team.
+// A ring for each team: a stage's rows are all of one team, which has taken out a stage's row before it waits for the next
+// one there, so that a wait by parity never meets a phase that another team's row has yet to end.
 template <bool kF32, uint32_t kVectors, uint32_t kTeam>
 __global__ void __launch_bounds__(kRingThreads, 1) norm_backward_ring_kernel(NormGradArgs a, uint32_t stages) {
     extern __shared__ __align__(128) unsigned char smem[];
@@ -584,7 +493,7 @@ __global__ void __launch_bounds__(kRingThreads, 1) norm_backward_ring_kernel(Nor
     const uint32_t bytes = a.hidden * (kF32 ? 4u : 2u), more = a.d_sum != nullptr ? bytes : 0u;
     const RowSources from = {{(const char *)a.dy, (const char *)a.sum, (const char *)a.d_sum}, {a.hidden * 2u, bytes, more}};
     Ring ring;
-    ring.init(smem, stages, a.hidden * 2u + bytes + more, team, kTeams, 0u, a.rows);
+    ring.init(smem, stages, a.hidden * 2u + bytes + more, team, kTeams, a.rows);
     pdl_wait();
     if (t == 0u) {
         for (uint32_t i = 0; i < stages; i++) ring.load_next(from);
@@ -669,37 +578,20 @@ bool by_ring_size(uint32_t hidden, F &&launch) {
 uint32_t team_stages(uint32_t stage_bytes, uint32_t teams) { return std::min(kRingBytes / stage_bytes, kMaxStages) / teams; }
 
 template <typename K, typename A>
-bool launch_ring(K kernel, const A &a, uint32_t threads, uint32_t stage_bytes, uint32_t rings, uint32_t stages, cudaStream_t stream) {
-    const uint32_t bytes = 256u + rings * stages * stage_bytes + a.hidden * 2u;
-    return set_max_dynamic_smem((const void *)kernel, 256u + kRingBytes + kRingHidden * 2u) &&
-           launch_chained(kernel, (uint32_t)sm_count(), threads, bytes, stream, a, stages);
+bool launch_ring(K kernel, const A &a, uint32_t stage_bytes, uint32_t rings, uint32_t stages, cudaStream_t stream) {
+    const uint32_t bytes = 256u + rings * stages * stage_bytes;
+    return set_max_dynamic_smem((const void *)kernel, 256u + kRingBytes) &&
+           launch_chained(kernel, (uint32_t)sm_count(), kRingThreads, bytes, stream, a, stages);
 }
 
-// The ring pays once every SM has a few rows.
+// The ring pays once every SM has two rows (us, with / without: 300 x 7168 16 / 22, 300 x 4096 14 / 16, 300 x 2048 12 / 12,
+// 148 x 4096 14 / 12).
 bool ring_suits(uint32_t rows, uint32_t hidden, bool vector) {
-    return vector && hidden > 1024u && hidden <= kRingHidden && rows >= 4u * (uint32_t)sm_count();
+    return vector && hidden > 1024u && hidden <= kRingHidden && rows >= 2u * (uint32_t)sm_count();
 }
 
 template <bool kF32>
 bool launch_norm(const NormArgs &a, bool vector, cudaStream_t stream) {
-    const uint32_t stage = a.hidden * (kF32 ? 4u : 2u) * (a.residual ? 2u : 1u);
-    // With the sum, bf16 rows and codes written the memory serves all better with no more than 64 KB of reads under way per SM
-    // (8192 x 7168 92 us, with 115 KB 98 to 100); with fewer of them four teams and 115 KB are better (without the sum 61 us,
-    // the other way 70; without the bf16 rows 77, the other way 80).
-    const bool all = a.sum != nullptr && a.y != nullptr && a.codes != nullptr;
-    auto ring = [&](auto teams) {
-        constexpr uint32_t kTeams = decltype(teams)::value;
-        const uint32_t held = team_stages(stage, kTeams), stages = (all ? std::min(held, std::max(1u, 65536u / stage / kTeams)) : held) * kTeams;
-        return by_ring_size(a.hidden, [&](auto vectors) {
-            return launch_ring(norm_ring_kernel<kF32, decltype(vectors)::value * kTeams, kTeams>, a, kRingThreads + kWarp, stage, 1u, stages, stream);
-        });
-    };
-    if (ring_suits(a.rows, a.hidden, vector) && team_stages(stage, 2u) != 0u) {
-        if constexpr (!kF32) {
-            if (!all) return ring(std::integral_constant<uint32_t, 4u>{});
-        }
-        return ring(std::integral_constant<uint32_t, 2u>{});
-    }
     return by_size(a.hidden, [&](auto team, auto vectors) {
         constexpr uint32_t kTeam = decltype(team)::value, kThreads = threads_of(kTeam), kTeams = kThreads / kTeam;
         auto kernel = vector ? norm_kernel<kF32, true, kTeam, decltype(vectors)::value> : norm_kernel<kF32, false, kTeam, decltype(vectors)::value>;
@@ -723,11 +615,11 @@ bool launch_backward(const NormGradArgs &a, bool vector, uint32_t &blocks, cudaS
         blocks = teams * (uint32_t)sm_count();
         if constexpr (!kF32) {
             if (teams == 2u) {
-                return launch_ring(norm_backward_ring_kernel<kF32, 2u, kRingThreads / 2u>, a, kRingThreads, stage, 2u, stages, stream);
+                return launch_ring(norm_backward_ring_kernel<kF32, 2u, kRingThreads / 2u>, a, stage, 2u, stages, stream);
             }
         }
         return by_ring_size(a.hidden, [&](auto vectors) {
-            return launch_ring(norm_backward_ring_kernel<kF32, decltype(vectors)::value, kRingThreads>, a, kRingThreads, stage, 1u, stages, stream);
+            return launch_ring(norm_backward_ring_kernel<kF32, decltype(vectors)::value, kRingThreads>, a, stage, 1u, stages, stream);
         });
     }
     return by_size(a.hidden, [&](auto team, auto vectors) {
