@@ -9,7 +9,7 @@
 //
 // Bound by memory: 12 bytes per element, each read or written once.  A row belongs to a warp, or, where there are
 // fewer rows than warps to fill the SMs, to a block; its sum for the routing weight is taken in a fixed order.  32768 x 2048:
-// 127 us, 6.3 TB/s.
+// SwiGLU 127 us, 6.3 TB/s, SiTU 156 us, with three exponentials and three reciprocals per element.
 #include "k3_common.cuh"
 #include "k3_fp8_ptx.cuh"
 #include "k3_moe_ops.h"
@@ -31,35 +31,45 @@ struct ActivationGradArgs {
     float beta, by_beta, linear_beta, by_linear_beta;
 };
 
+// Of the activation itself, for two elements.
 struct Derived {
-    float d_gate, d_up, act;                     // of the activation itself
+    uint64_t d_gate, d_up, act;
 };
 
-// tanh x and 1 / cosh^2 x of one exponential and one reciprocal (with two of each the exponential unit bound SiTU, 32768 x
-// 2048 at 215 us).  tanh: its Taylor series up to x^11 below 0.4, where the next term is 6e-8 of the value.
+K3_DEVINL uint64_t pair_of(uint32_t v) { return pack2(bf16_lo(v), bf16_hi(v)); }
+K3_DEVINL uint32_t bf16_of(uint64_t v) { return bf16x2(lo2(v), hi2(v)); }
+// exp(-by x)
+K3_DEVINL float exp_of(float by, float x) { return exp2_fast(-by * kLog2E * x); }
+K3_DEVINL uint64_t reciprocal2(uint64_t d) { return pack2(reciprocal_fast(lo2(d)), reciprocal_fast(hi2(d))); }
+
+// tanh x = (1 - e) / (1 + e) and 1 / (4 cosh^2 x), e = exp(-2 |x|).  Below 0.1, where 1 - e would lose the value's bits,
+// tanh x = x - x^3 / 3 + 2 x^5 / 15, whose next term is 6e-8 of the value.
 struct Bounded {
-    float tanh, slope;
+    uint64_t tanh, slope;
 };
-K3_DEVINL Bounded bounded(float x) {
-    const float e = __expf(-2.0f * fabsf(x)), r = __fdividef(1.0f, 1.0f + e), y = x * x;
-    float p = fmaf(y, -1382.0f / 155925.0f, 62.0f / 2835.0f);
-    p = fmaf(y, p, -17.0f / 315.0f);
-    p = fmaf(y, p, 2.0f / 15.0f);
-    p = fmaf(y, p, -1.0f / 3.0f);
-    return {fabsf(x) < 0.4f ? fmaf(x * y, p, x) : copysignf((1.0f - e) * r, x), 4.0f * e * r * r};
+K3_DEVINL float tanh_of(float x, float near, float far) { return fabsf(x) < 0.1f ? near : copysignf(far, x); }
+K3_DEVINL Bounded bounded(uint64_t x) {
+    const uint64_t one = both2(1.0f), y = mul2(x, x);
+    const uint64_t e = pack2(exp_of(2.0f, fabsf(lo2(x))), exp_of(2.0f, fabsf(hi2(x))));
+    const uint64_t r = reciprocal2(add2(e, one)), far = mul2(fma2(e, both2(-1.0f), one), r);
+    const uint64_t near = fma2(mul2(x, y), fma2(y, both2(2.0f / 15.0f), both2(-1.0f / 3.0f)), x);
+    return {pack2(tanh_of(lo2(x), lo2(near), lo2(far)), tanh_of(hi2(x), hi2(near), hi2(far))), mul2(mul2(e, r), r)};
 }
 
+// Two elements at a time: element by element the arithmetic bounds SiTU (32768 x 2048, one array for all inputs: 180 us, 149 in
+// pairs, 98 SwiGLU, which the memory bounds).
 template <bool kSitu>
-K3_DEVINL Derived derive(const ActivationGradArgs &a, float g, float u) {
-    const float e = __expf(-fabsf(g)), r = __fdividef(1.0f, 1.0f + e);
-    const float sig = g >= 0.0f ? r : e * r, rest = g >= 0.0f ? e * r : r;
+K3_DEVINL Derived derive(const ActivationGradArgs &a, uint64_t g, uint64_t u) {
+    // s = 1 / (1 + e), 1 - s = e / (1 + e).  From 88 on both s and s g are 0, and e stays finite.
+    const uint64_t e = pack2(exp_of(1.0f, fmaxf(lo2(g), -88.0f)), exp_of(1.0f, fmaxf(hi2(g), -88.0f)));
+    const uint64_t sig = reciprocal2(add2(e, both2(1.0f))), rest = mul2(e, sig);
     if (!kSitu) {
-        const float left = g * sig;
-        return {fmaf(left, rest, sig) * u, left, left * u};
+        const uint64_t left = mul2(g, sig);
+        return {mul2(fma2(left, rest, sig), u), left, mul2(left, u)};
     }
-    const Bounded x = bounded(g * a.by_beta), y = bounded(u * a.by_linear_beta);
-    const float left = a.beta * x.tanh * sig, right = a.linear_beta * y.tanh;
-    return {fmaf(x.slope, sig, left * rest) * right, left * y.slope, left * right};
+    const Bounded x = bounded(mul2(g, both2(a.by_beta))), y = bounded(mul2(u, both2(a.by_linear_beta)));
+    const uint64_t left = mul2(mul2(x.tanh, both2(a.beta)), sig), right = mul2(y.tanh, both2(a.linear_beta)), four = both2(4.0f);
+    return {mul2(fma2(mul2(x.slope, four), sig, mul2(left, rest)), right), mul2(left, mul2(y.slope, four)), mul2(left, right)};
 }
 
 template <bool kSitu, bool kVector, uint32_t kTeam>
@@ -69,14 +79,14 @@ __global__ void __launch_bounds__(kThreads) activation_grad_kernel(ActivationGra
     const uint32_t t = threadIdx.x % kTeam;
     const uint64_t row = (uint64_t)blockIdx.x * (kThreads / kTeam) + threadIdx.x / kTeam;
     const bool live = row < a.rows && (a.offsets == nullptr || (row >= a.offsets[0] && row < a.offsets[a.groups]));
-    float sum = 0.0f;
+    uint64_t sums = 0ull;
     uint32_t route = 0u;
     bool routed = false;
     if (live) {
         route = a.routes ? a.routes[row] : (uint32_t)row;
         routed = route < a.route_count;
         const float weight = !routed ? 0.0f : a.weights ? a.weights[route] : 1.0f;
-        const uint64_t base = row * a.columns;
+        const uint64_t base = row * a.columns, weight2 = both2(weight);
         // a thread's eight columns are neighbours, or (rows that are not whole vectors) kTeam apart
         constexpr uint32_t kStep = kVector ? 1u : kTeam;
         for (uint32_t c = kVector ? t * 8u : t; c < a.columns; c += kTeam * 8u) {
@@ -100,14 +110,12 @@ __global__ void __launch_bounds__(kThreads) activation_grad_kernel(ActivationGra
             uint32_t dg[4], du[4], sc[4];
 #pragma unroll
             for (uint32_t i = 0; i < 4u; i++) {
-                const Derived lo = derive<kSitu>(a, bf16_lo(g[i]), bf16_lo(u[i])), hi = derive<kSitu>(a, bf16_hi(g[i]), bf16_hi(u[i]));
-                const float d0 = bf16_lo(d[i]), d1 = bf16_hi(d[i]);
-                sum = fmaf(d0, lo.act, sum);                          // + 0 past the row's end
-                sum = fmaf(d1, hi.act, sum);
-                const float w0 = weight * d0, w1 = weight * d1;
-                dg[i] = bf16x2(w0 * lo.d_gate, w1 * hi.d_gate);
-                du[i] = bf16x2(w0 * lo.d_up, w1 * hi.d_up);
-                sc[i] = bf16x2(weight * lo.act, weight * hi.act);
+                const Derived f = derive<kSitu>(a, pair_of(g[i]), pair_of(u[i]));
+                const uint64_t out = pair_of(d[i]), weighted = mul2(out, weight2);
+                sums = fma2(out, f.act, sums);                          // + 0 past the row's end
+                dg[i] = bf16_of(mul2(weighted, f.d_gate));
+                du[i] = bf16_of(mul2(weighted, f.d_up));
+                sc[i] = bf16_of(mul2(weight2, f.act));
             }
             if (kVector) {
                 *reinterpret_cast<uint4 *>(a.d_gate + base + c) = make_uint4(dg[0], dg[1], dg[2], dg[3]);
@@ -126,7 +134,7 @@ __global__ void __launch_bounds__(kThreads) activation_grad_kernel(ActivationGra
         }
     }
     if (a.d_weights == nullptr) return;
-    sum = warp_sum(sum);
+    float sum = warp_sum(lo2(sums) + hi2(sums));
     if (kTeam != kWarp) {
         if (threadIdx.x % kWarp == 0u) scratch[threadIdx.x / kWarp] = sum;
         __syncthreads();

@@ -5,9 +5,9 @@
 //
 // Bound by memory: a row is read once, kept in registers over the row's sum, and written once.  A row belongs to a
 // warp (up to 1024 columns) or to a block of 256 or 1024 threads; a thread holds vectors of 8 neighbouring columns,
-// so the 16 lanes of half a warp hold a block of 128, whose largest magnitude is four shuffles away.  Many rows go through a
-// ring in shared memory (below).  8192 x 7168 bf16: forward with sum, bf16 rows and codes 92 us, 5.7 TB/s; backward with the
-// weight's gradient 82 us, 5.7 TB/s.
+// so the 16 lanes of half a warp hold a block of 128, whose largest magnitude is four shuffles away.  The gradient of
+// many rows goes through a ring in shared memory (below).  8192 x 7168 bf16: forward with sum, bf16 rows and codes 86 us,
+// 6.1 TB/s; backward with the weight's gradient 82 us, 5.7 TB/s.
 #include "k3_common.cuh"
 #include "k3_fp8_ptx.cuh"
 #include "k3_grouped.h"
@@ -129,7 +129,7 @@ K3_DEVINL float largest_of(float a, float b, float c) {
 
 // The normalised elements of a thread's vectors to y, and to codes with the largest magnitude of the half warp's block.
 // All lanes of a warp call it; `live`: the row exists.  minus_w: the weight's negatives, for the quotients want -y.  Two
-// elements at a time and the vectors side by side through every step, 8192 x 7168 to codes alone takes 58 us; element by
+// elements at a time and the vectors side by side through every step, 8192 x 7168 to codes alone takes 59 us; element by
 // element, and one vector after the other with its shuffles and its reciprocal, it took 78.
 template <bool kF32, bool kVector, uint32_t kVectors, typename First>
 K3_DEVINL void put_normed(const NormArgs &a, const Eight<kF32> (&s)[kVectors], const Eight<false> (&minus_w)[kVectors], float rstd, uint64_t row,
