@@ -32,5 +32,8 @@ bool product_any(const Product &p, cudaStream_t stream);
 // n and k multiples of 8, all pointers but the offsets on 16 bytes
 bool product_tc(const Product &p, cudaStream_t stream);
 uint64_t tc_workspace_bytes(uint32_t rows, uint32_t groups);
+// by weight, as product_tc, for the groups of up to kOuterRows rows
+constexpr uint32_t kOuterRows = 16;
+bool product_outer(const Product &p, cudaStream_t stream);
 
 }  // namespace k3::gb

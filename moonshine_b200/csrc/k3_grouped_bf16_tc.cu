@@ -13,6 +13,7 @@
 //   warp 1       MMA issuer, owns the tensor memory: two accumulators of kMaxN columns, for the item's two halves or, where
 //                it has one, for two items in turn
 //   warp 2       draws items from a counter and tells the others, when the loads of the one before come to an end
+//                by weight beside another kernel for small groups (least): every gridDim-th item, where its group is not small
 //   warp 3       by weight: clears what a group's first stage holds of the rows behind its part of the group
 //   warps 4-11   results: lane quadrant warp % 4, every second chunk of 32 columns; the accumulator is free again once
 //                it is in registers, before anything is stored
@@ -92,6 +93,7 @@ struct TcArgs {
     uint32_t column_tiles;                                             // by weight: and along the columns
     uint32_t batch;                                                    // items per draw
     bool single;                                                       // an item per block at most: no plan, nothing is drawn
+    uint32_t least;                                                    // by weight: groups of fewer rows are left out
     int accumulate;
 };
 
@@ -558,7 +560,23 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             return Item{g, begin, end - begin, at / a.column_tiles * S::kLanes, at % a.column_tiles * S::kMaxN, 0u};
         };
         uint32_t w = blockIdx.x / (S::kSplit ? splits : kCtas);
-        if (rank == 0u && a.single) {
+        if (!kRows && a.least != 0u) {
+            // the items of the groups that are this kernel's, 32 looked at together, every gridDim-th the block's
+            const uint32_t total = a.groups * a.lane_tiles * a.column_tiles, step = gridDim.x;
+            bool more = true;
+            for (uint64_t first = blockIdx.x; more && first < total; first += (uint64_t)kWarp * step) {
+                const uint64_t at = first + (uint64_t)lane * step;
+                const Item it = at < total ? weight_item((uint32_t)at) : none;
+                for (uint32_t mask = __ballot_sync(0xffffffffu, at < total && it.rows >= a.least); more && mask != 0u; mask &= mask - 1u) {
+                    const uint32_t from = __ffs(mask) - 1u;
+                    const Item next{__shfl_sync(0xffffffffu, it.group, from), __shfl_sync(0xffffffffu, it.row, from), __shfl_sync(0xffffffffu, it.rows, from),
+                                    __shfl_sync(0xffffffffu, it.lane0, from), __shfl_sync(0xffffffffu, it.column0, from), 0u};
+                    if (lane == 0u) more = publish(next);
+                    more = __shfl_sync(0xffffffffu, more, 0);
+                }
+            }
+            if (lane == 0u && more) publish(none);
+        } else if (rank == 0u && a.single) {
             Item it = none;
             if (kRows) {
                 Tile tile{};
@@ -860,9 +878,9 @@ uint32_t batch_of(const Product &p) {
     return !S::kSplit && depth <= 4u * kDepth && items_of<kForm, S>(p) >= 16u * (uint64_t)sm_count() / S::kCtas ? 4u : 1u;
 }
 
-// parts: blocks that share an item's depth (S::kSplit)
+// parts: blocks that share an item's depth (S::kSplit); least: as TcArgs
 template <int kForm, bool kF32, typename S>
-bool launch(const Product &p, uint32_t parts, cudaStream_t stream) {
+bool launch(const Product &p, uint32_t parts, uint32_t least, cudaStream_t stream) {
     constexpr bool kRows = kForm != kByWeight;
     auto kernel = grouped_bf16_kernel<kForm, kF32, S>;
     CUtensorMap ma, mb;
@@ -877,10 +895,10 @@ bool launch(const Product &p, uint32_t parts, cudaStream_t stream) {
     const uint64_t items = items_of<kForm, S>(p), places = S::kSplit ? items : (uint64_t)sm_count() / S::kCtas;
     const bool single = items <= places && (!kRows || p.groups <= kSearched);
     const TcArgs a{p.out, p.offsets, (Plan *)p.workspace, (Tile *)((Plan *)p.workspace + 1), p.rows, p.groups, p.n, p.k,
-                   (lanes + S::kLanes - 1u) / S::kLanes, (p.k + S::kMaxN - 1u) / S::kMaxN, batch_of<kForm, S>(p), single, p.accumulate};
+                   (lanes + S::kLanes - 1u) / S::kLanes, (p.k + S::kMaxN - 1u) / S::kMaxN, batch_of<kForm, S>(p), single, least, p.accumulate};
     if (items * parts > 0x7fffffffull || (S::kSplit && !single) || !set_max_dynamic_smem((const void *)kernel, S::kBytes)) return false;
     const uint32_t cluster = S::kSplit ? parts : S::kCtas;
-    const bool planned = single || (kRows ? launch_chained(grouped_plan_kernel, 1, kMaxGroups, 0, stream, a.plan, a.tiles, p.offsets, p.rows,
+    const bool planned = single || least != 0u || (kRows ? launch_chained(grouped_plan_kernel, 1, kMaxGroups, 0, stream, a.plan, a.tiles, p.offsets, p.rows,
                                                            p.groups, S::kMaxN, S::kStep, tiles)
                                           : launch_chained(grouped_counter_kernel, 1, 1, 0, stream, a.plan));
     return planned && launch_chained_cluster(kernel, (uint32_t)std::min(items, places) * cluster, kThreads, dim3(cluster, 1, 1), S::kBytes, stream,
@@ -888,8 +906,8 @@ bool launch(const Product &p, uint32_t parts, cudaStream_t stream) {
 }
 
 template <int kForm, typename S>
-bool launch_typed(const Product &p, cudaStream_t stream, uint32_t parts = 1u) {
-    return p.f32 ? launch<kForm, true, S>(p, parts, stream) : launch<kForm, false, S>(p, parts, stream);
+bool launch_typed(const Product &p, cudaStream_t stream, uint32_t parts = 1u, uint32_t least = 0u) {
+    return p.f32 ? launch<kForm, true, S>(p, parts, least, stream) : launch<kForm, false, S>(p, parts, least, stream);
 }
 
 // Which shape.  The host knows the rows and groups of a call, not how they are spread: it takes a third of the groups to hold
@@ -952,6 +970,7 @@ bool rows_product(const Product &p, cudaStream_t stream) {
 // By weight the lanes and columns are the matrices', the depth the rows; one block per item, for pairs multiply two operands
 // that lie by their depth 10 % more slowly (4096 rows of 8 groups, without the stores: 669 us, pairs 729).
 bool weight_product(const Product &p, cudaStream_t stream) {
+    if (p.rows <= kOuterRows) return product_outer(p, stream);
     const uint32_t stages = std::max(1u, (p.rows / p.groups + kDepth - 1u) / kDepth);
     auto time = [&](auto shape, const Cost &c) {
         using S = decltype(shape);
@@ -961,12 +980,20 @@ bool weight_product(const Product &p, cudaStream_t stream) {
     const double shortest = std::min({few, middle, wide});
     const uint32_t parts = parts_of<kByWeight>(p, stages, std::min(p.k, kFewRows), shortest);
     if (parts > 1u) return launch_typed<kByWeight, FewSplit>(p, stream, parts);
-    if (shortest == few) return launch_typed<kByWeight, Few>(p, stream);
-    if (shortest == middle) return launch_typed<kByWeight, Middle>(p, stream);
+    // Few rows per group: those of up to 16 rows go to the other kernel, whose time is its stores, and what this one then takes to
+    // look the groups over.  bf16 and f32, us, here alone / both: 896 groups of 3 rows, 264 x 520 143 / 68 and 156 / 96, by
+    // Zipf's law 119 / 74 and 139 / 104; 32 groups of 8, 2048 x 7168 197 / 168 and 317 / 287, of 12 195 / 180 and 320 / 295, of 16 195 /
+    // 195 and 320 / 313; 128 groups of 3, 512 x 1024 39 / 35 and 53 / 55, so f32 stays here.
+    const double bytes = (double)p.groups * p.n * p.k * (p.f32 ? 4.0 : 2.0), stores = 3.0 + bytes / 6.1e6, both = 10.0 + bytes / 6.9e6;
+    const bool outer = p.rows <= 12u * (uint64_t)p.groups && both < std::max(shortest, stores);
+    if (outer && !product_outer(p, stream)) return false;
+    const uint32_t least = outer ? kOuterRows + 1u : 0u;
+    if (shortest == few) return launch_typed<kByWeight, Few>(p, stream, 1u, least);
+    if (shortest == middle) return launch_typed<kByWeight, Middle>(p, stream, 1u, least);
     // f32 and groups of more than 1024 rows: with segments (8 groups of 4096 rows 770 us instead of 695, and 1e-6 of the
     // gradient's norm from 64 bits instead of 4e-6)
-    if (p.f32 && p.rows / p.groups > 17u * kDepth) return launch<kByWeight, true, DeepWeight>(p, 1u, stream);
-    return launch_typed<kByWeight, WideWeight>(p, stream);
+    if (p.f32 && p.rows / p.groups > 17u * kDepth) return launch<kByWeight, true, DeepWeight>(p, 1u, 0u, stream);
+    return launch_typed<kByWeight, WideWeight>(p, stream, 1u, least);
 }
 
 }  // namespace

@@ -299,3 +299,78 @@ def test_rows_that_do_not_start_on_16_bytes():
         check(run(form, odd(x), odd(dy), odd(w), dev, dtype=F32), value, size, depth_of(form, n, k, offsets), F32)
         out = torch.zeros(value.numel() + 1, dtype=BF16, device="cuda")[1:].view(value.shape)
         check(run(form, x, dy, w, dev, out=out), value, size, depth_of(form, n, k, offsets), BF16)
+
+
+def spread(groups, sizes, front=0):
+    """Offsets of groups whose sizes go through `sizes` in turn, rows of no group in front."""
+    cuts = [front]
+    for g in range(groups):
+        cuts.append(cuts[-1] + sizes[g % len(sizes)])
+    return cuts
+
+
+# few rows per group on average: groups on both sides of 16 rows, which different kernels take, side by side
+MIXED = [[1], [3, 0, 16, 0, 1], [15, 17, 0, 0, 2], [0] * 40 + [130, 16, 0, 1, 33], [0] * 895 + [1200], [16, 0, 0]]
+
+
+@pytest.mark.parametrize("n,k", [(264, 136), (40, 520), (1032, 64), (72, 264)])
+@pytest.mark.parametrize("case", range(len(MIXED)))
+def test_gradients_of_small_groups_beside_large_ones(n, k, case):
+    offsets = spread(896, MIXED[case], front=3)
+    rows = offsets[-1] + 5
+    x, dy, w = inputs(case, rows, 896, n, k)
+    x[:3], x[-5:], dy[:3], dy[-5:] = float("nan"), float("nan"), float("inf"), float("nan")
+    value, size = reference("by_weight", x, dy, w, offsets)
+    depth = depth_of("by_weight", n, k, offsets)
+    for dtype in (BF16, F32):
+        check(run("by_weight", x, dy, w, on_device(offsets), dtype=dtype), value, size, depth, dtype)
+    into = torch.randn(value.shape, generator=torch.Generator(device="cuda").manual_seed(case), device="cuda")
+    before = into.clone()
+    run("by_weight", x, dy, w, on_device(offsets), into=into)
+    check(into, value + before.double(), size + before.double().abs(), depth + 1, F32)
+    empty = [g for g in range(896) if offsets[g] == offsets[g + 1]]
+    assert torch.equal(into[empty], before[empty])
+
+
+@pytest.mark.parametrize("rows", [1, 7, 16, 60])
+@pytest.mark.parametrize("n,k", [(2120, 2056), (72, 15368)])
+def test_gradients_of_a_few_rows_of_large_matrices(rows, n, k):
+    groups = 12
+    offsets = spread(groups, [rows // groups])[:-1] + [rows]
+    x, dy, w = inputs(rows, rows, groups, n, k)
+    value, size = reference("by_weight", x, dy, w, offsets)
+    for dtype in (BF16, F32):
+        check(run("by_weight", x, dy, w, on_device(offsets), dtype=dtype), value, size, depth_of("by_weight", n, k, offsets), dtype)
+
+
+def test_a_row_that_is_not_finite_among_small_groups():
+    offsets = spread(896, [2, 16, 17, 1, 0])
+    x, dy, w = inputs(16, offsets[-1], 896, 264, 136)
+    bad = [5, 6, 7, 401, 895]
+    for g in bad:
+        if offsets[g] < offsets[g + 1]:
+            x[offsets[g]], dy[offsets[g + 1] - 1] = float("nan"), float("inf")
+    value, size = reference("by_weight", x, dy, w, offsets)
+    got = run("by_weight", x, dy, w, on_device(offsets), dtype=F32)
+    keep = [g for g in range(896) if g not in bad]
+    check(got[keep], value[keep], size[keep], 17, F32)
+    assert not any(bool(torch.isfinite(got[g]).all()) for g in bad if offsets[g] < offsets[g + 1])
+
+
+def test_captured_with_groups_that_become_large():
+    groups, n, k, rows = 896, 264, 136, 4000
+    x, dy, w = inputs(17, rows, groups, n, k)
+    all_offsets = [spread(groups, s) for s in ([4], [0, 0, 0, 16], [17, 0, 0, 0, 0], [0] * 895 + [4000], [0])]
+    dev = on_device(all_offsets[0])
+    gradient = grouped.GroupedWeightGradient(groups, n, k)
+    gradient.forward(dy, x, dev)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = gradient.forward(dy, x, dev)
+    for offsets in all_offsets:
+        dev.copy_(on_device(offsets))
+        graph.replay()
+        value, size = reference("by_weight", x, dy, w, offsets)
+        check(out, value, size, depth_of("by_weight", n, k, offsets), F32)
+    assert ops.k3_moe_device_status() == 0
