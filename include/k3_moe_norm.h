@@ -11,6 +11,8 @@
  * y is f32 until it is stored: bf16 rows are y rounded once, codes are those of
  * y itself with a scale per row and 128 columns (format "rows" of
  * k3_moe_fp8.h).  A block of 128 that is not finite gets the scale NaN.
+ * Sums are f32; their order depends on hidden and, where it is no multiple of 8,
+ * on the row's place modulo 8: the same call gives the same bits.
  */
 #ifndef K3_MOE_NORM_H
 #define K3_MOE_NORM_H

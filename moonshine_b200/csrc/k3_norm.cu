@@ -23,7 +23,7 @@ namespace {
 constexpr uint32_t kMaxHidden = 16384;
 
 // Eight elements of a row as they lie in memory.  kVector: neighbours, c .. c + 7, of rows that start on 16 bytes and are
-// whole vectors.  Otherwise c, c + 16, .. c + 112: the half warp still holds a block of 128, and its 16 lanes read
+// whole vectors.  Otherwise (matrices that start elsewhere) c, c + 16, .. c + 112: the half warp still holds a block of 128, and its 16 lanes read
 // neighbours (rows of 3583 f32: the gradient of 1021 rows 20.7 us, 30.8 with eight neighbours per thread).
 template <bool kVector>
 K3_DEVINL constexpr uint32_t column_of(uint32_t c, uint32_t i) { return kVector ? c + i : c + 16u * i; }
@@ -74,6 +74,58 @@ struct Eight {
                 else ((uint16_t *)row)[column_of<kVector>(c, i)] = (uint16_t)(w[i / 2u] >> (16u * (i & 1u)));
             }
         }
+    }
+    // Of a matrix of `total` elements on 16 bytes those from `at` on, a multiple of 8, of which the first is in column c of the row
+    // (below 0: in the row in front).  In two steps, so that no branch stands between the loads of several: the matrix's last
+    // elements and zeros for those of other rows come second.
+    K3_DEVINL void fetch(const void *matrix, uint64_t at, uint64_t total, int32_t c, int32_t columns) {
+        load<true>((const char *)matrix + at * (kF32 ? 4u : 2u), 0u, c > -8 && c < columns && at + 8u <= total ? 8u : 0u);
+    }
+    K3_DEVINL void finish(const void *matrix, uint64_t at, uint64_t total, int32_t c, int32_t columns) {
+        if (c <= -8 || c >= columns || (c >= 0 && c + 8 <= columns)) return;
+        if (at + 8u > total) {
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; i++) {
+                if (at + i >= total) continue;
+                if (kF32) w[i % kWords] = ((const uint32_t *)matrix)[at + i];
+                else w[i / 2u] |= (uint32_t)((const uint16_t *)matrix)[at + i] << (16u * (i & 1u));
+            }
+        }
+#pragma unroll
+        for (int32_t i = 0; i < 8; i++) {
+            if (c + i >= 0 && c + i < columns) continue;
+            if (kF32) w[i % kWords] = 0u;
+            else w[i / 2] &= i & 1 ? 0xffffu : 0xffff0000u;
+        }
+    }
+    K3_DEVINL void store_flat(void *matrix, uint64_t at, int32_t c, int32_t columns) const {
+        if (c >= 0 && c + 8 <= columns) {
+            store<true>((char *)matrix + at * (kF32 ? 4u : 2u), 0u, 8u);
+            return;
+        }
+#pragma unroll
+        for (int32_t i = 0; i < 8; i++) {
+            if (c + i < 0 || c + i >= columns) continue;
+            if (kF32) ((uint32_t *)matrix)[at + i] = w[i % kWords];
+            else ((uint16_t *)matrix)[at + i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+        }
+    }
+    // elements by .. by + 7 of two neighbours, by < 8
+    K3_DEVINL void between(const Eight &first, const Eight &second, uint32_t by) {
+        uint32_t v[2u * kWords];
+#pragma unroll
+        for (uint32_t i = 0; i < kWords; i++) {
+            v[i] = first.w[i];
+            v[kWords + i] = second.w[i];
+        }
+#pragma unroll
+        for (uint32_t bit = 4u; bit > (kF32 ? 0u : 1u); bit /= 2u) {
+            const uint32_t words = kF32 ? bit : bit / 2u;
+#pragma unroll
+            for (uint32_t i = 0; i + words < 2u * kWords; i++) v[i] = by & bit ? v[i + words] : v[i];
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kWords; i++) w[i] = kF32 || (by & 1u) == 0u ? v[i] : __byte_perm(v[i], v[i + 1u], 0x5432);
     }
     K3_DEVINL float value(uint32_t i) const {
         if (kF32) return __uint_as_float(w[i % kWords]);
@@ -128,10 +180,11 @@ K3_DEVINL float largest_of(float a, float b, float c) {
 }
 
 // The normalised elements of a thread's vectors to y, and to codes with the largest magnitude of the half warp's block.
-// All lanes of a warp call it; `live`: the row exists.  minus_w: the weight's negatives, for the quotients want -y.  Two
+// All lanes of a warp call it; `live`: the row exists; kPartial: a vector may
+// lie across the row's end, and y is not asked for.  minus_w: the weight's negatives, for the quotients want -y.  Two
 // elements at a time and the vectors side by side through every step, 8192 x 7168 to codes alone takes 59 us; element by
 // element, and one vector after the other with its shuffles and its reciprocal, it took 78.
-template <bool kF32, bool kVector, uint32_t kVectors, typename First>
+template <bool kF32, bool kVector, bool kPartial = false, uint32_t kVectors, typename First>
 K3_DEVINL void put_normed(const NormArgs &a, const Eight<kF32> (&s)[kVectors], const Eight<false> (&minus_w)[kVectors], float rstd, uint64_t row,
                           First first, bool live) {
     const uint32_t hidden = a.hidden, pitch = pitch_of(hidden);
@@ -143,7 +196,7 @@ K3_DEVINL void put_normed(const NormArgs &a, const Eight<kF32> (&s)[kVectors], c
 #pragma unroll
         for (uint32_t i = 0; i < 4u; i++) y[v][i] = mul2(mul2(pair_of(s[v], i), rstd2), pair_of(minus_w[v], i));
     }
-    if (a.y != nullptr) {
+    if (!kPartial && a.y != nullptr) {
 #pragma unroll
         for (uint32_t v = 0; v < kVectors; v++) {
             Eight<false> out;
@@ -159,7 +212,7 @@ K3_DEVINL void put_normed(const NormArgs &a, const Eight<kF32> (&s)[kVectors], c
         float largest = 0.0f;
 #pragma unroll
         for (uint32_t i = 0; i < 4u; i++) {
-            if (!kVector) {                                          // past the row's end: no part of the block, whatever rstd is
+            if (!kVector || kPartial) {                              // past the row's end: no part of the block, whatever rstd is
                 y[v][i] = pack2(column_of<kVector>(c, 2u * i) < hidden ? lo2(y[v][i]) : 0.0f,
                                 column_of<kVector>(c, 2u * i + 1u) < hidden ? hi2(y[v][i]) : 0.0f);
             }
@@ -185,6 +238,10 @@ K3_DEVINL void put_normed(const NormArgs &a, const Eight<kF32> (&s)[kVectors], c
         }
         codes[v] = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
         if (kVector && first(v) >= hidden) codes[v] = make_uint2(0u, 0u);            // zeros in the padding: the quotient is one of 0, or NaN
+        if (kPartial && first(v) < hidden && hidden - first(v) < 8u) {
+            const uint64_t mask = (1ull << (8u * (hidden - first(v)))) - 1u;
+            codes[v] = make_uint2(codes[v].x & (uint32_t)mask, codes[v].y & (uint32_t)(mask >> 32));
+        }
         most[v] = __float_as_uint(scale);
     }
     if (!live) return;
@@ -261,6 +318,110 @@ __global__ void __launch_bounds__(threads_of(kTeam)) norm_kernel(NormArgs a) {
     for (uint32_t v = 0; v < kVectors; v++) negate(w[v]);
     put_normed<kF32, kVector>(a, s, w, rstd, row, first, live);
     if (live) put_scale_padding(a, row, t);
+    pdl_trigger();
+}
+
+// Rows whose length is no multiple of 8 start anywhere in a vector.  A thread's vectors are then those of the matrix as a whole, and
+// hold the row from column -o on, o the row's place modulo 8: the loads and stores of all rows are whole but at a row's ends (4096 x 7001
+// bf16 forward with both outputs 80 us, element by element 113; backward 94 and 217; 2048 x 3583 f32 33 and 33, 37 and 41).  The weight's vectors lie across these, as do codes and their blocks, for which
+// the row goes through shared memory.
+K3_DEVINL Eight<false> weight_from(const uint16_t *weight, int32_t c, uint32_t o, uint32_t hidden) {
+    const int32_t at = o != 0u ? c + (int32_t)o - 8 : c;
+    Eight<false> first, second;
+    first.fetch(weight, (uint64_t)(int64_t)at, hidden, at, (int32_t)hidden);
+    second.fetch(weight, (uint64_t)(at + 8), hidden, at + 8, (int32_t)hidden);
+    first.finish(weight, (uint64_t)(int64_t)at, hidden, at, (int32_t)hidden);
+    second.finish(weight, (uint64_t)(at + 8), hidden, at + 8, (int32_t)hidden);
+    first.between(first, second, (8u - o) & 7u);
+    return first;
+}
+constexpr uint32_t flat_units(uint32_t hidden) { return (hidden + 7u) / 8u + 1u; }
+
+template <bool kF32, uint32_t kTeam, uint32_t kVectors>
+__global__ void __launch_bounds__(threads_of(kTeam), kTeam == 256u && kVectors == 4u && !kF32 ? 4 : 0) norm_flat_kernel(NormArgs a) {
+    pdl_wait();
+    __shared__ float scratch[32];
+    extern __shared__ __align__(16) unsigned char row_smem[];             // codes only: [kTeams][flat_units] vectors
+    constexpr uint32_t kTeams = threads_of(kTeam) / kTeam, kUnit = kF32 ? 32u : 16u;
+    const uint32_t t = threadIdx.x % kTeam, units = flat_units(a.hidden);
+    const uint64_t task = (uint64_t)blockIdx.x * kTeams + threadIdx.x / kTeam, total = (uint64_t)a.rows * a.hidden;
+    const bool live = task < a.rows;
+    const uint64_t row = live ? task : 0u, from = row * a.hidden / 8u * 8u;
+    const uint32_t o = (uint32_t)(row * a.hidden - from);
+    const int32_t columns = live ? (int32_t)a.hidden : -8;
+    auto unit = [&](uint32_t v) { return v * kTeam + t; };
+    auto column = [&](uint32_t v) { return (int32_t)(unit(v) * 8u) - (int32_t)o; };
+    Eight<kF32> s[kVectors], r[kVectors];
+#pragma unroll
+    for (uint32_t v = 0; v < kVectors; v++) s[v].fetch(a.x, from + unit(v) * 8u, total, column(v), columns);
+    if (a.residual != nullptr) {
+#pragma unroll
+        for (uint32_t v = 0; v < kVectors; v++) r[v].fetch(a.residual, from + unit(v) * 8u, total, column(v), columns);
+    }
+#pragma unroll
+    for (uint32_t v = 0; v < kVectors; v++) s[v].finish(a.x, from + unit(v) * 8u, total, column(v), columns);
+    if (a.residual != nullptr) {
+#pragma unroll
+        for (uint32_t v = 0; v < kVectors; v++) {
+            r[v].finish(a.residual, from + unit(v) * 8u, total, column(v), columns);
+            float f[8];
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; i++) f[i] = s[v].value(i) + r[v].value(i);
+            s[v].set(f);
+        }
+    }
+    if (a.sum != nullptr) {
+#pragma unroll
+        for (uint32_t v = 0; v < kVectors; v++) s[v].store_flat(a.sum, from + unit(v) * 8u, column(v), columns);
+    }
+    float squares = 0.0f;
+#pragma unroll
+    for (uint32_t v = 0; v < kVectors; v++) {
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; i++) squares = fmaf(s[v].value(i), s[v].value(i), squares);
+    }
+    unsigned char *mine = row_smem + threadIdx.x / kTeam * units * kUnit;
+    if (a.codes != nullptr) {
+#pragma unroll
+        for (uint32_t v = 0; v < kVectors; v++) s[v].template store<true>(mine, unit(v) * 8u, units * 8u);
+    }
+    squares = team_sum<kTeam>(squares, scratch);                     // the row is in shared memory behind it
+    const float rstd = 1.0f / sqrtf(squares / (float)a.hidden + a.epsilon);
+    if (live && t == 0u && a.rstd != nullptr) a.rstd[row] = rstd;
+    if (a.y != nullptr) {
+        const uint64_t rstd2 = both2(rstd);
+#pragma unroll
+        for (uint32_t v = 0; v < kVectors; v++) {
+            const Eight<false> w = weight_from(a.weight, column(v), o, a.hidden);
+            Eight<false> out;
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; i++) {
+                const uint64_t y = mul2(mul2(pair_of(s[v], i), rstd2), pair_of(w, i));
+                out.w[i] = bf16x2(lo2(y), hi2(y));
+            }
+            out.store_flat(a.y, from + unit(v) * 8u, column(v), columns);
+        }
+    }
+    if (a.codes != nullptr) {
+        if (kTeam == kWarp) __syncwarp();
+        Eight<false> w[kVectors];
+#pragma unroll
+        for (uint32_t v = 0; v < kVectors; v++) {
+            Eight<kF32> first, second;
+            const uint32_t c = unit(v) * 8u;
+            first.template load<true>(mine, c, units * 8u);
+            second.template load<true>(mine, c + 8u, units * 8u);
+            s[v].between(first, second, o);
+            w[v].fetch(a.weight, c, a.hidden, (int32_t)c, (int32_t)a.hidden);
+        }
+#pragma unroll
+        for (uint32_t v = 0; v < kVectors; v++) {
+            w[v].finish(a.weight, unit(v) * 8u, a.hidden, (int32_t)(unit(v) * 8u), (int32_t)a.hidden);
+            negate(w[v]);
+        }
+        put_normed<kF32, true, true>(a, s, w, rstd, row, [&](uint32_t v) { return unit(v) * 8u; }, live);
+        if (live) put_scale_padding(a, row, t);
+    }
     pdl_trigger();
 }
 
@@ -360,6 +521,76 @@ __global__ void __launch_bounds__(threads_of(kTeam)) norm_backward_kernel(NormGr
             for (uint32_t i = 1; i < kTeams; i++) sum += shared_dw[i * a.hidden + c];
             to[c] = sum;
         }
+    }
+}
+
+// norm_backward_kernel by the matrix's vectors.  Rows that a team takes are a multiple of 8 apart, so their places modulo 8 are
+// the same, and the columns of its weight gradient too.
+template <bool kF32, uint32_t kTeam, uint32_t kVectors>
+__global__ void __launch_bounds__(threads_of(kTeam)) norm_backward_flat_kernel(NormGradArgs a) {
+    pdl_wait();
+    constexpr uint32_t kThreads = threads_of(kTeam), kTeams = kThreads / kTeam;
+    __shared__ float scratch[2][32];
+    extern __shared__ float shared_dw[];                             // [kTeams][hidden]
+    const uint32_t t = threadIdx.x % kTeam, team = threadIdx.x / kTeam;
+    const uint64_t total = (uint64_t)a.rows * a.hidden;
+    const uint32_t o = (uint32_t)(((uint64_t)blockIdx.x * kTeams + team) * a.hidden % 8u);
+    auto column = [&](uint32_t v) { return (int32_t)((v * kTeam + t) * 8u) - (int32_t)o; };
+    Eight<false> w[kVectors];
+    uint64_t dw[kVectors][4];
+#pragma unroll
+    for (uint32_t v = 0; v < kVectors; v++) {
+        w[v] = weight_from(a.weight, column(v), o, a.hidden);
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; i++) dw[v][i] = 0ull;
+    }
+    uint32_t turn = 0u;
+    for (uint64_t at = (uint64_t)blockIdx.x * kTeams; at < a.rows; at += (uint64_t)gridDim.x * kTeams, turn ^= 1u) {
+        const bool live = at + team < a.rows;
+        const uint64_t from = live ? (at + team) * a.hidden - o : 0u;
+        const int32_t columns = live ? (int32_t)a.hidden : -8;
+        Eight<false> dy[kVectors];
+        Eight<kF32> s[kVectors], d[kVectors];
+#pragma unroll
+        for (uint32_t v = 0; v < kVectors; v++) {
+            const uint64_t f = from + (v * kTeam + t) * 8u;
+            dy[v].fetch(a.dy, f, total, column(v), columns);
+            s[v].fetch(a.sum, f, total, column(v), columns);
+            if (a.d_sum != nullptr) d[v].fetch(a.d_sum, f, total, column(v), columns);
+        }
+#pragma unroll
+        for (uint32_t v = 0; v < kVectors; v++) {
+            const uint64_t f = from + (v * kTeam + t) * 8u;
+            dy[v].finish(a.dy, f, total, column(v), columns);
+            s[v].finish(a.sum, f, total, column(v), columns);
+            if (a.d_sum != nullptr) d[v].finish(a.d_sum, f, total, column(v), columns);
+        }
+        const float rstd = live ? a.rstd[at + team] : 0.0f;
+        uint64_t dots = 0ull;
+#pragma unroll
+        for (uint32_t v = 0; v < kVectors; v++) dots = add_products<kF32>(dy[v], s[v], w[v], both2(rstd), dots, dw[v]);
+        const float mean = team_sum<kTeam>(lo2(dots) + hi2(dots), scratch[turn]) / (float)a.hidden;
+#pragma unroll
+        for (uint32_t v = 0; v < kVectors; v++) {
+            input_gradient<kF32>(dy[v], s[v], w[v], d[v], a.d_sum != nullptr, both2(rstd), both2(-mean))
+                .store_flat(a.dx, from + (v * kTeam + t) * 8u, column(v), columns);
+        }
+    }
+    if (a.partial == nullptr) return;
+#pragma unroll
+    for (uint32_t v = 0; v < kVectors; v++) {
+#pragma unroll
+        for (int32_t i = 0; i < 8; i++) {
+            const int32_t c = column(v) + i;
+            if (c >= 0 && c < (int32_t)a.hidden) shared_dw[team * a.hidden + c] = i & 1 ? hi2(dw[v][i / 2]) : lo2(dw[v][i / 2]);
+        }
+    }
+    __syncthreads();
+    float *to = a.partial + (uint64_t)blockIdx.x * a.hidden;
+    for (uint32_t c = threadIdx.x; c < a.hidden; c += kThreads) {
+        float sum = shared_dw[c];
+        for (uint32_t i = 1; i < kTeams; i++) sum += shared_dw[i * a.hidden + c];
+        to[c] = sum;
     }
 }
 
@@ -590,8 +821,21 @@ bool ring_suits(uint32_t rows, uint32_t hidden, bool vector) {
     return vector && hidden > 1024u && hidden <= kRingHidden && rows >= 2u * (uint32_t)sm_count();
 }
 
+// Rows by the matrix's vectors: no whole vectors, and places for one more.
+bool flat_suits(uint32_t hidden) { return hidden % 8u != 0u && hidden + 7u <= kMaxHidden; }
+
 template <bool kF32>
-bool launch_norm(const NormArgs &a, bool vector, cudaStream_t stream) {
+bool launch_norm(const NormArgs &a, bool on_16, cudaStream_t stream) {
+    const bool vector = on_16 && a.hidden % 8u == 0u;
+    if (on_16 && flat_suits(a.hidden)) {
+        return by_size(a.hidden + 7u, [&](auto team, auto vectors) {
+            constexpr uint32_t kTeam = decltype(team)::value, kThreads = threads_of(kTeam), kTeams = kThreads / kTeam;
+            auto kernel = norm_flat_kernel<kF32, kTeam, decltype(vectors)::value>;
+            const uint32_t bytes = a.codes != nullptr ? kTeams * flat_units(a.hidden) * (kF32 ? 32u : 16u) : 0u;
+            return set_max_dynamic_smem((const void *)kernel, kTeams * flat_units(kTeams > 1u ? 1024u : kMaxHidden) * 32u) &&
+                   launch_chained(kernel, (a.rows + kTeams - 1u) / kTeams, kThreads, bytes, stream, a);
+        });
+    }
     return by_size(a.hidden, [&](auto team, auto vectors) {
         constexpr uint32_t kTeam = decltype(team)::value, kThreads = threads_of(kTeam), kTeams = kThreads / kTeam;
         auto kernel = vector ? norm_kernel<kF32, true, kTeam, decltype(vectors)::value> : norm_kernel<kF32, false, kTeam, decltype(vectors)::value>;
@@ -600,13 +844,19 @@ bool launch_norm(const NormArgs &a, bool vector, cudaStream_t stream) {
 }
 
 // Blocks of the gradient, each with a partial row of the weight's: up to two per SM.
-uint32_t grad_blocks(uint32_t rows, uint32_t hidden) {
-    const uint32_t teams = hidden <= 1024u ? 8u : 1u;
+uint32_t most_grad_blocks(uint32_t rows, uint32_t hidden) {
+    const uint32_t teams = (hidden % 8u != 0u ? hidden + 7u : hidden) <= 1024u ? 8u : 1u;
     return std::min((rows + teams - 1u) / teams, 2u * (uint32_t)sm_count());
+}
+// A multiple of 8 where a block takes several rows.
+uint32_t grad_blocks(uint32_t rows, uint32_t hidden) {
+    const uint32_t most = most_grad_blocks(rows, hidden);
+    return most == 2u * (uint32_t)sm_count() ? most / 8u * 8u : most;
 }
 
 template <bool kF32>
-bool launch_backward(const NormGradArgs &a, bool vector, uint32_t &blocks, cudaStream_t stream) {
+bool launch_backward(const NormGradArgs &a, bool on_16, uint32_t &blocks, cudaStream_t stream) {
+    const bool vector = on_16 && a.hidden % 8u == 0u;
     const uint32_t stage = a.hidden * (2u + (kF32 ? 4u : 2u) * (a.d_sum ? 2u : 1u));
     blocks = grad_blocks(a.rows, a.hidden);
     // two rows at a time up to 4096 columns of bf16; more, and f32, have no registers for it (8192 x 7168 133 us, one 91)
@@ -620,6 +870,14 @@ bool launch_backward(const NormGradArgs &a, bool vector, uint32_t &blocks, cudaS
         }
         return by_ring_size(a.hidden, [&](auto vectors) {
             return launch_ring(norm_backward_ring_kernel<kF32, decltype(vectors)::value, kRingThreads>, a, stage, 1u, stages, stream);
+        });
+    }
+    if (on_16 && flat_suits(a.hidden)) {
+        return by_size(a.hidden + 7u, [&](auto team, auto vectors) {
+            constexpr uint32_t kTeam = decltype(team)::value, kThreads = threads_of(kTeam), kTeams = kThreads / kTeam;
+            auto kernel = norm_backward_flat_kernel<kF32, kTeam, decltype(vectors)::value>;
+            return set_max_dynamic_smem((const void *)kernel, kTeams * (kTeams > 1u ? 1024u : kMaxHidden) * 4u) &&
+                   launch_chained(kernel, blocks, kThreads, kTeams * a.hidden * 4u, stream, a);
         });
     }
     return by_size(a.hidden, [&](auto team, auto vectors) {
@@ -648,14 +906,13 @@ extern "C" bool k3_moe_norm(void *sum, void *y, void *codes, void *scales, void 
     }
     const NormArgs a{sum, (uint16_t *)y, (uint8_t *)codes, (float *)scales, (float *)rstd, x, residual, (const uint16_t *)weight, rows,
                      hidden, epsilon};
-    const bool vector = hidden % 8u == 0u && aligned(sum, 16u) && aligned(x, 16u) && aligned(residual, 16u) && aligned(weight, 16u) &&
-                        aligned(y, 16u);
-    return f32 ? launch_norm<true>(a, vector, (cudaStream_t)stream) : launch_norm<false>(a, vector, (cudaStream_t)stream);
+    const bool on_16 = aligned(sum, 16u) && aligned(x, 16u) && aligned(residual, 16u) && aligned(weight, 16u) && aligned(y, 16u);
+    return f32 ? launch_norm<true>(a, on_16, (cudaStream_t)stream) : launch_norm<false>(a, on_16, (cudaStream_t)stream);
 }
 
 extern "C" size_t k3_moe_norm_workspace_bytes(uint32_t rows, uint32_t hidden) {
     if (rows == 0u || !sizes_ok(rows, hidden, K3_MOE_NORM_F32)) return 0;
-    return ((size_t)grad_blocks(rows, hidden) * hidden * 4u + 15u) / 16u * 16u;
+    return ((size_t)most_grad_blocks(rows, hidden) * hidden * 4u + 15u) / 16u * 16u;
 }
 
 extern "C" bool k3_moe_norm_backward(void *dx, void *d_weight, const void *dy, const void *sum, const void *rstd, const void *d_sum,
@@ -678,10 +935,9 @@ extern "C" bool k3_moe_norm_backward(void *dx, void *d_weight, const void *dy, c
     if (d_weight && (!workspace || !aligned(workspace, 16u) || workspace_bytes < k3_moe_norm_workspace_bytes(rows, hidden))) return false;
     const NormGradArgs a{dx, d_weight ? (float *)workspace : nullptr, (const uint16_t *)dy, (const uint16_t *)weight, sum, d_sum,
                          (const float *)rstd, rows, hidden};
-    const bool vector = hidden % 8u == 0u && aligned(dx, 16u) && aligned(dy, 16u) && aligned(sum, 16u) && aligned(d_sum, 16u) &&
-                        aligned(weight, 16u);
+    const bool on_16 = aligned(dx, 16u) && aligned(dy, 16u) && aligned(sum, 16u) && aligned(d_sum, 16u) && aligned(weight, 16u);
     uint32_t blocks = 0u;
-    const bool ok = f32 ? launch_backward<true>(a, vector, blocks, (cudaStream_t)stream) : launch_backward<false>(a, vector, blocks, (cudaStream_t)stream);
+    const bool ok = f32 ? launch_backward<true>(a, on_16, blocks, (cudaStream_t)stream) : launch_backward<false>(a, on_16, blocks, (cudaStream_t)stream);
     if (!ok || !d_weight) return ok;
     return launch_chained(norm_weight_kernel, (hidden + 31u) / 32u, 256, 0, (cudaStream_t)stream, (float *)d_weight,
                           (const float *)workspace, blocks, hidden, accumulate);

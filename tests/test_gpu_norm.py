@@ -222,3 +222,68 @@ def test_into_the_linear_layer():
     with pytest.raises(ValueError, match="codes: expected"):
         linear.forward_codes(r.codes[:, :-16], r.scales)
     assert linear.forward_codes(r.codes[:0], r.scales[:0]).shape == (0, wide)
+
+
+# no multiple of 8: a row starts anywhere in a vector; around the changes of kernel, whose places are for 7 elements more
+ODD = [2, 3, 5, 12, 100, 249, 250, 505, 506, 777, 1017, 1018, 1020, 1023, 2041, 2042, 4089, 4090, 5003, 8185, 8186, 16377, 16378, 16383]
+
+
+@pytest.mark.parametrize("hidden", ODD)
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows", [2, 37, 301, 1301])
+def test_lengths_that_are_no_whole_vectors(hidden, dtype, rows):
+    x, residual, dy, d_sum, weight = inputs(hidden + rows, rows, hidden, dtype)
+    call = norm.RmsNorm(weight, EPSILON)
+    for y, codes in ((True, False), (False, True), (True, True)):
+        r = call.forward(x, residual, y=y, codes=codes)
+        check_forward(r, x, residual, weight)
+    want, size, want_w, size_w = gradient(dy, r.sum, r.rstd, d_sum, weight)
+    dx, d_weight = call.backward(dy, r.sum, r.rstd, d_sum)
+    check(dx, want, HALF[dtype] * want.abs() + 2 * SUM * size)
+    check(d_weight, want_w, (rows + 4) * 2.0 ** -24 * size_w)
+    assert ops.k3_moe_device_status() == 0
+
+
+@pytest.mark.parametrize("hidden", [24, 777, 1024, 3583, 9000])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows", [3, 700])
+def test_rows_that_do_not_start_on_16_bytes(hidden, dtype, rows):
+    """Each tensor one element behind such a place; what is in front and behind stays."""
+    odd = lambda t: torch.cat([t.new_full((1,), 7.0), t.reshape(-1), t.new_full((1,), 7.0)])[1:-1].view(t.shape)  # noqa: E731
+    plain = inputs(hidden - rows, rows, hidden, dtype)
+    x, residual, dy, d_sum, weight = map(odd, plain)
+    call = norm.RmsNorm(weight, EPSILON)
+    r = call.forward(x, residual, codes=True)
+    check_forward(r, x, residual, weight)
+    want, size, want_w, size_w = gradient(dy, r.sum, r.rstd, d_sum, weight)
+    dx, d_weight = call.backward(dy, r.sum, r.rstd, d_sum)
+    check(dx, want, HALF[dtype] * want.abs() + 2 * SUM * size)
+    check(d_weight, want_w, (rows + 4) * 2.0 ** -24 * size_w)
+    guard = torch.full((rows * hidden + 2,), 5.0, dtype=dtype, device="cuda")
+    y = torch.full((rows * hidden + 2,), 5.0, dtype=BF16, device="cuda")
+    kind = ops.NORM_F32 if dtype is F32 else ops.NORM_BF16
+    rstd = torch.empty(rows, device="cuda")
+    assert ops.k3_moe_norm(guard[1:], y[1:], None, None, rstd, x, residual, weight, rows, hidden, kind, EPSILON)
+    assert torch.equal(guard[1:-1].view(rows, hidden), r.sum)
+    assert all(float(t[i]) == 5.0 for t in (guard, y) for i in (0, -1))
+
+
+@pytest.mark.parametrize("hidden", [3, 250, 777, 2042, 5003])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_nothing_behind_the_last_row_is_written_or_read(hidden, dtype):
+    """Outputs and inputs as the first part of larger tensors, whose rest is NaN and stays."""
+    rows = 13
+    longer = lambda t: torch.cat([t.reshape(-1), t.new_full((40,), float("nan"))])  # noqa: E731
+    plain = inputs(hidden, rows, hidden, dtype)
+    x, residual, dy, d_sum, weight = map(longer, plain)
+    kind = ops.NORM_F32 if dtype is F32 else ops.NORM_BF16
+    want = norm.RmsNorm(plain[4], EPSILON).forward(plain[0], plain[1])
+    out, y, rstd = longer(torch.empty_like(plain[0])), longer(torch.empty_like(plain[2])), torch.empty(rows, device="cuda")
+    n = rows * hidden
+    assert ops.k3_moe_norm(out, y, None, None, rstd, x, residual, weight, rows, hidden, kind, EPSILON)
+    assert torch.equal(out[:n].view(rows, hidden), want.sum) and torch.equal(y[:n].view(rows, hidden), want.y) and torch.equal(rstd, want.rstd)
+    dx, _ = norm.RmsNorm(plain[4], EPSILON).backward(plain[2], want.sum, want.rstd, plain[3])
+    s, grad = longer(want.sum), longer(torch.empty_like(plain[0]))
+    assert ops.k3_moe_norm_backward(grad, None, dy, s, rstd, d_sum, weight, rows, hidden, kind, 0, None, 0)
+    assert torch.equal(grad[:n].view(rows, hidden), dx)
+    assert all(bool(torch.isnan(t[n:]).all()) for t in (out, y, grad))
