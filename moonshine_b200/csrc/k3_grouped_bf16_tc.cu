@@ -13,7 +13,7 @@
 //   warp 1       MMA issuer, owns the tensor memory: two accumulators of kMaxN columns, for the item's two halves or, where
 //                it has one, for two items in turn
 //   warp 2       draws items from a counter and tells the others, when the loads of the one before come to an end
-//                by weight beside another kernel for small groups (least): every gridDim-th item, where its group is not small
+//                by weight beside a kernel that takes the small groups: every gridDim-th item, where its group is another
 //   warp 3       by weight: clears what a group's first stage holds of the rows behind its part of the group
 //   warps 4-11   results: lane quadrant warp % 4, every second chunk of 32 columns; the accumulator is free again once
 //                it is in registers, before anything is stored
@@ -93,7 +93,7 @@ struct TcArgs {
     uint32_t column_tiles;                                             // by weight: and along the columns
     uint32_t batch;                                                    // items per draw
     bool single;                                                       // an item per block at most: no plan, nothing is drawn
-    uint32_t least;                                                    // by weight: groups of fewer rows are left out
+    uint32_t least, most;                                              // by weight: groups of fewer and of more rows are left out
     int accumulate;
 };
 
@@ -319,9 +319,10 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     constexpr bool kADepth = kForm != kForward, kBDepth = kForm == kByWeight;
     constexpr uint32_t kCtas = S::kCtas;
     // The tensor cores cut the sums off instead of rounding them, 2^-24 or so of the sum per 16 of the depth, always towards
-    // zero: 8e-6 of the result's norm at a depth of 7168.  For f32 results an accumulator therefore takes up to 16 blocks, a
-    // segment, and the warps behind it add the segments, rounded.  (Not with two halves, whose sums no registers would hold.)
-    constexpr uint32_t kSegment = kF32 && S::kHalves == 1u ? 16u : 0xffffffffu;
+    // zero: 8e-6 of the result's norm at a depth of 7168.  For f32 results an accumulator therefore takes up to 8 blocks, a
+    // segment, and the warps behind it add the segments, rounded: 6e-7 at any depth (16 blocks 1.1e-6, 4 3e-7).  64 groups of 512
+    // rows, 2048 x 7168, by input: 16 blocks 725 us, 8 733, 4 758.  (Not with two halves, whose sums no registers would hold.)
+    constexpr uint32_t kSegment = kF32 && S::kHalves == 1u ? 8u : 0xffffffffu;
     extern __shared__ unsigned char smem_raw[];
     unsigned char *base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint64_t *full = reinterpret_cast<uint64_t *>(base + S::kBars);    // [kStages]
@@ -567,7 +568,7 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             for (uint64_t first = blockIdx.x; more && first < total; first += (uint64_t)kWarp * step) {
                 const uint64_t at = first + (uint64_t)lane * step;
                 const Item it = at < total ? weight_item((uint32_t)at) : none;
-                for (uint32_t mask = __ballot_sync(0xffffffffu, at < total && it.rows >= a.least); more && mask != 0u; mask &= mask - 1u) {
+                for (uint32_t mask = __ballot_sync(0xffffffffu, at < total && it.rows >= a.least && it.rows <= a.most); more && mask != 0u; mask &= mask - 1u) {
                     const uint32_t from = __ffs(mask) - 1u;
                     const Item next{__shfl_sync(0xffffffffu, it.group, from), __shfl_sync(0xffffffffu, it.row, from), __shfl_sync(0xffffffffu, it.rows, from),
                                     __shfl_sync(0xffffffffu, it.lane0, from), __shfl_sync(0xffffffffu, it.column0, from), 0u};
@@ -586,6 +587,7 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 }
             } else if (w < a.groups * a.lane_tiles * a.column_tiles) {
                 it = weight_item(w);
+                if (it.rows > a.most) it = none;
             }
             if (elect_one() && publish(it)) publish(none);
         } else if (rank == 0u && elect_one()) {
@@ -594,6 +596,7 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             w *= a.batch;
             for (;;) {
                 Item it = none;
+                bool skip = false;
                 left--;
                 if (w < total) {
                     if (kRows) {
@@ -603,16 +606,19 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                         it = Item{tile.group, tile.row, tile.rows, local / of.count * S::kLanes, 0u, 0u};
                     } else {
                         it = weight_item(w);
+                        skip = it.rows > a.most;
                     }
                     it.draw = left == 0u;
                 }
-                if (!publish(it)) break;
+                if (!skip && !publish(it)) break;
                 if (left != 0u) {
                     w++;
                     continue;
                 }
-                if (!mbar_wait(wanted, want_phase, abort_flag)) break;
-                want_phase ^= 1u;
+                if (!skip) {                                           // no item asks for the next draw where the last was left out
+                    if (!mbar_wait(wanted, want_phase, abort_flag)) break;
+                    want_phase ^= 1u;
+                }
                 left = a.batch;
                 w = gridDim.x / kCtas * a.batch + atomicAdd(&a.plan->counter, a.batch);
             }
@@ -878,9 +884,10 @@ uint32_t batch_of(const Product &p) {
     return !S::kSplit && depth <= 4u * kDepth && items_of<kForm, S>(p) >= 16u * (uint64_t)sm_count() / S::kCtas ? 4u : 1u;
 }
 
-// parts: blocks that share an item's depth (S::kSplit); least: as TcArgs
+// parts: blocks that share an item's depth (S::kSplit); least, most: as TcArgs
+constexpr uint32_t kAll = 0xffffffffu;
 template <int kForm, bool kF32, typename S>
-bool launch(const Product &p, uint32_t parts, uint32_t least, cudaStream_t stream) {
+bool launch(const Product &p, cudaStream_t stream, uint32_t parts = 1u, uint32_t least = 0u, uint32_t most = kAll) {
     constexpr bool kRows = kForm != kByWeight;
     auto kernel = grouped_bf16_kernel<kForm, kF32, S>;
     CUtensorMap ma, mb;
@@ -895,7 +902,7 @@ bool launch(const Product &p, uint32_t parts, uint32_t least, cudaStream_t strea
     const uint64_t items = items_of<kForm, S>(p), places = S::kSplit ? items : (uint64_t)sm_count() / S::kCtas;
     const bool single = items <= places && (!kRows || p.groups <= kSearched);
     const TcArgs a{p.out, p.offsets, (Plan *)p.workspace, (Tile *)((Plan *)p.workspace + 1), p.rows, p.groups, p.n, p.k,
-                   (lanes + S::kLanes - 1u) / S::kLanes, (p.k + S::kMaxN - 1u) / S::kMaxN, batch_of<kForm, S>(p), single, least, p.accumulate};
+                   (lanes + S::kLanes - 1u) / S::kLanes, (p.k + S::kMaxN - 1u) / S::kMaxN, batch_of<kForm, S>(p), single, least, most, p.accumulate};
     if (items * parts > 0x7fffffffull || (S::kSplit && !single) || !set_max_dynamic_smem((const void *)kernel, S::kBytes)) return false;
     const uint32_t cluster = S::kSplit ? parts : S::kCtas;
     const bool planned = single || least != 0u || (kRows ? launch_chained(grouped_plan_kernel, 1, kMaxGroups, 0, stream, a.plan, a.tiles, p.offsets, p.rows,
@@ -907,7 +914,7 @@ bool launch(const Product &p, uint32_t parts, uint32_t least, cudaStream_t strea
 
 template <int kForm, typename S>
 bool launch_typed(const Product &p, cudaStream_t stream, uint32_t parts = 1u, uint32_t least = 0u) {
-    return p.f32 ? launch<kForm, true, S>(p, parts, least, stream) : launch<kForm, false, S>(p, parts, least, stream);
+    return p.f32 ? launch<kForm, true, S>(p, stream, parts, least) : launch<kForm, false, S>(p, stream, parts, least);
 }
 
 // Which shape.  The host knows the rows and groups of a call, not how they are spread: it takes a third of the groups to hold
@@ -958,7 +965,7 @@ bool rows_product(const Product &p, cudaStream_t stream) {
         return time_of<S>(c, groups * tiles * lanes, stages, rows / tiles);
     };
     const double few = time(Few{}, kFewCost), middle = time(Middle{}, kMiddleCost), square = time(Square{}, kSquareCost);
-    const bool deep = p.f32 && stages > 16u;                          // Wide has no segments
+    const bool deep = p.f32 && stages > 8u;                           // Wide has no segments
     const double wide = deep ? INFINITY : time(Wide{}, kWideCost), shortest = rows <= kFewRows ? few : std::min({few, middle, square, wide});
     const uint32_t parts = parts_of<kForm>(p, stages, std::min(rows, (double)kFewRows), shortest);
     if (parts > 1u) return launch_typed<kForm, FewSplit>(p, stream, parts);
@@ -990,10 +997,13 @@ bool weight_product(const Product &p, cudaStream_t stream) {
     const uint32_t least = outer ? kOuterRows + 1u : 0u;
     if (shortest == few) return launch_typed<kByWeight, Few>(p, stream, 1u, least);
     if (shortest == middle) return launch_typed<kByWeight, Middle>(p, stream, 1u, least);
-    // f32 and groups of more than 1024 rows: with segments (8 groups of 4096 rows 770 us instead of 695, and 1e-6 of the
-    // gradient's norm from 64 bits instead of 4e-6)
-    if (p.f32 && p.rows / p.groups > 17u * kDepth) return launch<kByWeight, true, DeepWeight>(p, 1u, 0u, stream);
-    return launch_typed<kByWeight, WideWeight>(p, stream, 1u, least);
+    if (!p.f32) return launch<kByWeight, false, WideWeight>(p, stream, 1u, least);
+    // f32: without segments up to 17 blocks, 1e-6 of the gradient's norm from 64 bits at the most; deeper groups with them, 5e-7
+    // (a group of 4096 rows 4e-6 without).  32 groups of 1024 rows 838 us, with segments 913; 32 of 256 417 and 391.
+    constexpr uint32_t kDeep = 17u * kDepth;
+    if (p.rows / p.groups > kDeep) return launch<kByWeight, true, DeepWeight>(p, stream, 1u, least);
+    return launch<kByWeight, true, WideWeight>(p, stream, 1u, least, kDeep) &&
+           (p.rows <= kDeep || launch<kByWeight, true, DeepWeight>(p, stream, 1u, kDeep + 1u));
 }
 
 }  // namespace

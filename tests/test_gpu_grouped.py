@@ -374,3 +374,25 @@ def test_captured_with_groups_that_become_large():
         value, size = reference("by_weight", x, dy, w, offsets)
         check(out, value, size, depth_of("by_weight", n, k, offsets), F32)
     assert ops.k3_moe_device_status() == 0
+
+
+@pytest.mark.parametrize("n,k", [(520, 264), (2048, 1032), (264, 520), (384, 2048)])
+@pytest.mark.parametrize("sizes", [[3000, 40, 0, 20], [17, 1088, 1089, 1100, 5, 2500], [0, 0, 0, 0, 0, 0, 5000, 1]])
+def test_deep_groups_among_others_in_f32(n, k, sizes):
+    """An accumulator takes up to 68 additions of 16 products, each cut off by 2^-23 of the sum at most; segments are added
+    with rounding, at most 10 here."""
+    offsets = spread(len(sizes) * 5, sizes)
+    rows = offsets[-1]
+    x, dy, w = inputs(n + sizes[0], rows, len(offsets) - 1, n, k)
+    value, _ = reference("by_weight", x, dy, w, offsets)
+    into = torch.ones(value.shape, device="cuda")
+    got = run("by_weight", x, dy, w, on_device(offsets), dtype=F32)
+    run("by_weight", x, dy, w, on_device(offsets), into=into)
+    for g, (a, b) in enumerate(zip(offsets, offsets[1:])):
+        if a == b:
+            assert not got[g].any() and bool((into[g] == 1).all())
+            continue
+        norm = value[g].norm()
+        assert float((got[g].double() - value[g]).norm() / norm) <= 68 * 2.0 ** -23 + 10 * 2.0 ** -24
+        assert float((into[g].double() - 1 - value[g]).norm()) <= (69 * 2.0 ** -23 + 10 * 2.0 ** -24) * float((value[g].abs() + 1).norm())
+    assert ops.k3_moe_device_status() == 0
