@@ -118,6 +118,14 @@ __global__ void __launch_bounds__(kThreads) grouped_outer_kernel(OuterArgs a) {
     uint32_t row, end;
     group_rows(a.offsets, group, a.rows, row, end);
     if (end - row > kOuterRows || (row == end && a.accumulate)) return;
+    if (row == end) {
+        // zeros: the matrix from end to end, a part per warp (896 groups of 264 x 520, 75 of them with rows: 47 us, by tiles 63)
+        const uint64_t units = (uint64_t)a.n * a.k / (kF32 ? 4u : 8u), part = (units + tasks - 1u) / tasks;
+        uint4 *to = reinterpret_cast<uint4 *>(a.out) + group * units;
+        const uint64_t past = min(units, (at + 1u) * part);
+        for (uint64_t i = at * part + lane; i < past; i += kWarp) to[i] = make_uint4(0u, 0u, 0u, 0u);
+        return;
+    }
     const uint32_t k0 = at % a.tiles_k * kTileK;
     uint32_t m0 = at / a.tiles_k * a.each * kTileN;
     const uint32_t m_end = min(m0 + a.each * kTileN, a.n);
