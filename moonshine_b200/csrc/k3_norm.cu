@@ -322,9 +322,9 @@ __global__ void __launch_bounds__(threads_of(kTeam)) norm_kernel(NormArgs a) {
 }
 
 // Rows whose length is no multiple of 8 start anywhere in a vector.  A thread's vectors are then those of the matrix as a whole, and
-// hold the row from column -o on, o the row's place modulo 8: the loads and stores of all rows are whole but at a row's ends (4096 x 7001
-// bf16 forward with both outputs 80 us, element by element 113; backward 94 and 217; 2048 x 3583 f32 33 and 33, 37 and 41).  The weight's vectors lie across these, as do codes and their blocks, for which
-// the row goes through shared memory.
+// hold the row from column -o on, o the row's place modulo 8: loads and stores are whole but at a row's ends.  The weight's
+// vectors lie across these, as do codes and their blocks, for which the row goes through shared memory.  4096 x 7001 bf16: forward
+// with both outputs 80 us, element by element 113; backward 94 and 217; 2048 x 3583 f32: 33 and 33, 37 and 41.
 K3_DEVINL Eight<false> weight_from(const uint16_t *weight, int32_t c, uint32_t o, uint32_t hidden) {
     const int32_t at = o != 0u ? c + (int32_t)o - 8 : c;
     Eight<false> first, second;
