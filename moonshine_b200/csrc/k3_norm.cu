@@ -815,10 +815,10 @@ bool launch_ring(K kernel, const A &a, uint32_t stage_bytes, uint32_t rings, uin
            launch_chained(kernel, (uint32_t)sm_count(), kRingThreads, bytes, stream, a, stages);
 }
 
-// The ring pays once every SM has two rows (us, with / without: 300 x 7168 16 / 22, 300 x 4096 14 / 16, 300 x 2048 12 / 12,
-// 148 x 4096 14 / 12).
+// The ring pays once every SM has a row (us, with / without: 148 x 7168 14 / 16, 250 x 7168 16 / 20, 290 x 7168 16 / 22, 250 x 4104
+// 14 / 16, f32 250 x 2048 14 / 14).
 bool ring_suits(uint32_t rows, uint32_t hidden, bool vector) {
-    return vector && hidden > 1024u && hidden <= kRingHidden && rows >= 2u * (uint32_t)sm_count();
+    return vector && hidden > 1024u && hidden <= kRingHidden && rows >= (uint32_t)sm_count();
 }
 
 // Rows by the matrix's vectors: no whole vectors, and places for one more.
@@ -859,8 +859,8 @@ bool launch_backward(const NormGradArgs &a, bool on_16, uint32_t &blocks, cudaSt
     const bool vector = on_16 && a.hidden % 8u == 0u;
     const uint32_t stage = a.hidden * (2u + (kF32 ? 4u : 2u) * (a.d_sum ? 2u : 1u));
     blocks = grad_blocks(a.rows, a.hidden);
-    // two rows at a time up to 4096 columns of bf16; more, and f32, have no registers for it (8192 x 7168 133 us, one 91)
-    const uint32_t teams = !kF32 && a.hidden <= 4096u ? 2u : 1u, stages = team_stages(stage, teams);
+    // two rows at a time up to 4096 columns of bf16 where there are as many; more, and f32, have no registers for it (8192 x 7168 133 us, one 91)
+    const uint32_t teams = !kF32 && a.hidden <= 4096u && a.rows >= 2u * (uint32_t)sm_count() ? 2u : 1u, stages = team_stages(stage, teams);
     if (ring_suits(a.rows, a.hidden, vector) && stages >= 2u) {
         blocks = teams * (uint32_t)sm_count();
         if constexpr (!kF32) {

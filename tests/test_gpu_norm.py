@@ -287,3 +287,19 @@ def test_nothing_behind_the_last_row_is_written_or_read(hidden, dtype):
     assert ops.k3_moe_norm_backward(grad, None, dy, s, rstd, d_sum, weight, rows, hidden, kind, 0, None, 0)
     assert torch.equal(grad[:n].view(rows, hidden), dx)
     assert all(bool(torch.isnan(t[n:]).all()) for t in (out, y, grad))
+
+
+@pytest.mark.parametrize("hidden", [1032, 2048, 4096, 4104, 8192])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_about_a_row_or_two_per_sm(hidden, dtype):
+    """Where the gradient changes from blocks of a row to rows through a ring, and from one row at a time to two."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    for rows in (sms - 1, sms, sms + 1, 2 * sms - 1, 2 * sms, 2 * sms + 1, 3 * sms):
+        s, _, dy, d_sum, weight = inputs(hidden + rows, rows, hidden, dtype)
+        rstd = torch.rsqrt(s.double().square().mean(1) + EPSILON).float()
+        for extra in (None, d_sum):
+            want, size, want_w, size_w = gradient(dy, s, rstd, extra, weight)
+            dx, d_weight = norm.RmsNorm(weight, EPSILON).backward(dy, s, rstd, extra)
+            check(dx, want, HALF[dtype] * want.abs() + 2 * SUM * size)
+            check(d_weight, want_w, (rows + 4) * 2.0 ** -24 * size_w)
+    assert ops.k3_moe_device_status() == 0
