@@ -131,10 +131,11 @@ class GatedActivation:
                  routes: torch.Tensor | None = None, offsets: torch.Tensor | None = None):
         """d_out, gate, up bf16 [rows, columns] -> d_gate, d_up, scaled (bf16) and d_weights.
 
-        Row r belongs to route ``routes[r]`` (int32 [rows], each route once; None: route r), whose routing weight is
+        Row r belongs to route ``routes[r]`` (int32 [rows], no route twice; None: route r), whose routing weight is
         that element of ``weights`` (f32, [tokens, top_k] say; None: 1 for each row).  ``d_out`` is the gradient that the
         down matrix sends back for the unweighted row; ``scaled``, weight times activation, is what that matrix's own
-        gradient reads.  d_weights f32 has the shape of ``weights``, [rows] without them.  With ``offsets`` rows outside of
+        gradient reads.  d_weights f32 has the shape of ``weights``, [rows] without them, and is 0
+        for a route without a row; a row whose route is past the weights has weight 0.  With ``offsets`` rows outside of
         the groups are left out."""
         rows, columns = _matrix(d_out, "d_out")
         _check(gate, "gate", torch.bfloat16, (rows, columns))
@@ -149,8 +150,8 @@ class GatedActivation:
         _placed(("d_out", d_out), ("gate", gate), ("up", up), ("weights", weights), ("routes", routes), ("offsets", offsets))
         d_gate, d_up, scaled = torch.empty_like(d_out), torch.empty_like(d_out), torch.empty_like(d_out)
         count = rows if weights is None else weights.numel()
-        # routes that no row has get no gradient
-        if offsets is None and count == rows and rows and columns:
+        # zeros for routes that no row has, which only a table of routes can leave out
+        if routes is None and offsets is None and rows and columns:
             d_weights = d_out.new_empty(rows, dtype=torch.float32) if weights is None else torch.empty_like(weights)
         else:
             d_weights = d_out.new_zeros((rows,) if weights is None else weights.shape, dtype=torch.float32)
