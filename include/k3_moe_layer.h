@@ -193,7 +193,8 @@ bool k3_moe_shared_expert_ws(const k3_moe_layer_desc *desc, void *out, void *act
 
 /* Combine: out[t] = bf16( bf16(sum_r weights[t,r] * rows[index[t*top_k+r]])
  * + shared[t] ), r ascending; index == NULL means the identity; shared ==
- * NULL skips the add (k3_engine_prefill.inc:1575-1580, 1598-1603). */
+ * NULL skips the add (k3_engine_prefill.inc:1575-1580, 1598-1603).  An index of
+ * UINT32_MAX is a route without a row: it adds nothing, whatever its weight. */
 bool k3_moe_combine(void *out, const void *rows, const void *index,
                     const void *weights, const void *shared, uint32_t tokens,
                     uint32_t top_k, uint32_t hidden, void *stream);

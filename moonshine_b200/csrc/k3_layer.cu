@@ -95,7 +95,10 @@ grouped_rows_kernel(uint16_t *__restrict__ out, const uint16_t *__restrict__ in,
 }
 
 // out[t] = bf16( bf16( bf16(sum_r w[t,r] * rows[idx[t,r]]) + shared[t] ) + residual[t] )
-// (shared and residual optional)
+// (shared and residual optional).  A route whose index is kNoRow has no row: it adds nothing, whatever its weight.  The
+// others are listed without it, so that the rows' loads stay without a condition (8192 tokens x 16 of 7168: 309 us, 308 for
+// rows that are all there; with a condition at each load 333).
+constexpr uint32_t kNoRow = 0xffffffffu;
 __global__ void __launch_bounds__(256)
 combine_kernel(uint16_t *__restrict__ out, const uint16_t *rows,
                const uint32_t *index, const float *weights,
@@ -103,20 +106,32 @@ combine_kernel(uint16_t *__restrict__ out, const uint16_t *rows,
                uint32_t tokens, uint32_t top_k, uint32_t hidden) {
     pdl_wait();
     __shared__ float w_s[32];
-    __shared__ uint32_t idx_s[32];
+    __shared__ uint32_t idx_s[32], present_s;
     for (uint32_t token = blockIdx.x; token < tokens; token += gridDim.x) {
         __syncthreads();
-        if (threadIdx.x < top_k) {
+        if (threadIdx.x < kWarp) {
             const uint32_t route = token * top_k + threadIdx.x;
-            w_s[threadIdx.x] = weights[route];
-            idx_s[threadIdx.x] = index ? index[route] : route;
+            uint32_t at = kNoRow;
+            float w = 0.0f;
+            if (threadIdx.x < top_k) {
+                w = weights[route];
+                at = index ? index[route] : route;
+            }
+            const uint32_t present = __ballot_sync(0xffffffffu, at != kNoRow);
+            if (at != kNoRow) {
+                const uint32_t place = __popc(present & ((1u << threadIdx.x) - 1u));
+                w_s[place] = w;
+                idx_s[place] = at;
+            }
+            if (threadIdx.x == 0u) present_s = __popc(present);
         }
         __syncthreads();
+        const uint32_t present = present_s;
         for (uint32_t c = blockIdx.y * blockDim.x + threadIdx.x; c < hidden / 8u;
              c += gridDim.y * blockDim.x) {
             float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-            for (uint32_t r = 0; r < top_k; r++) {
+            for (uint32_t r = 0; r < present; r++) {
                 const uint4 q = reinterpret_cast<const uint4 *>(rows + (uint64_t)idx_s[r] * hidden)[c];
                 const float w = w_s[r];
                 acc[0] = fmaf(w, bf16_lo(q.x), acc[0]);

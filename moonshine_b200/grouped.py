@@ -167,7 +167,7 @@ class Routed(NamedTuple):
     offsets: torch.Tensor                    # int32 [experts + 1]
     routes: torch.Tensor                     # int32 [rows]: the route token * top_k + rank of a row
     tokens: torch.Tensor                     # int32 [rows]: its token
-    place: torch.Tensor                      # int32 [tokens * top_k]: the row of a route
+    place: torch.Tensor                      # int32 [tokens * top_k]: the row of a route, -1 where it has none
     weights: torch.Tensor
     x: torch.Tensor                          # bf16 [rows, hidden]
     gate: torch.Tensor                       # bf16 [rows, expert_hidden]
@@ -215,15 +215,17 @@ class RoutedExperts:
         return out
 
     def forward(self, x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor) -> tuple[torch.Tensor, Routed]:
-        """x bf16 [tokens, hidden], ids int32 (each below the experts) and weights f32 [tokens, top_k], as ``k3_moe_route``
-        writes them -> bf16 [tokens, hidden], and what ``backward`` reads."""
+        """x bf16 [tokens, hidden], ids int32 and weights f32 [tokens, top_k], as ``k3_moe_route`` writes them -> bf16
+        [tokens, hidden], and what ``backward`` reads.  An id that is no expert's adds nothing and has no gradients; it
+        raises bit 1 of ``k3_moe_device_status``."""
         tokens, _ = _matrix(x, "x", self.hidden)
         _check(ids, "ids", torch.int32, (tokens, self.top_k))
         _check(weights, "weights", torch.float32, (tokens, self.top_k))
         _placed(("x", x), ("ids", ids), ("weights", weights), tables=self.gate._device)
         rows = tokens * self.top_k
-        # zeros: what a dispatch leaves out (an id that is no expert's) stays an index inside
-        offsets, routes, of_row, place = (ids.new_zeros(n) for n in (self.experts + 1, rows, rows, rows))
+        # what a dispatch leaves out (an id that is no expert's): zeros stay an index inside, a place of -1 adds nothing
+        offsets, routes, of_row = (ids.new_zeros(n) for n in (self.experts + 1, rows, rows))
+        place = ids.new_full((rows,), -1)
         if tokens == 0:
             nothing = x.new_empty((0, self.expert_hidden))
             return x.new_empty((0, self.hidden)), Routed(offsets, routes, of_row, place, weights, x, nothing, nothing)
