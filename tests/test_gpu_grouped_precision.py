@@ -5,7 +5,10 @@ cuts off half a unit on average, at most 2^-24 of the sum so far, always towards
 sqrt(i / 32) of the segment's, so a segment loses at most 32 x 2/3 x 2^-24 of itself.  Without segments the same count gives 2.5e-6
 at a depth of 2048 and 9e-6 at 7168.
 
-Segments are added with rounding, 2^-23 / sqrt(12) of the sum so far each: sqrt(segments / 2) x 2^-23 / sqrt(12)."""
+FMA pipes: each of a segment's 512 additions is rounded, 2^-23 / sqrt(12) of the sum so far at most; independent errors make that
+sqrt(512 / 2) of it.  One sum over the whole depth would lose sqrt(depth / 2).
+
+Segments are added with rounding in both: sqrt(segments / 2) x 2^-23 / sqrt(12)."""
 import math
 
 import pytest
@@ -24,6 +27,10 @@ ROUNDED = 2.0 ** -23 / math.sqrt(12)
 
 def tensor_core_bound(depth):
     return 32 * 2 / 3 * 2.0 ** -24 + math.sqrt(math.ceil(depth / 512) / 2) * ROUNDED
+
+
+def fma_bound(depth):
+    return (math.sqrt(512 / 2) + math.sqrt(math.ceil(depth / 512) / 2)) * ROUNDED
 
 
 def normal(seed, *shape):
@@ -55,6 +62,12 @@ def test_tensor_cores_by_rows(form, rows, wide, depth):
     assert by_rows(form, rows, wide, depth) <= tensor_core_bound(depth)
 
 
+@pytest.mark.parametrize("form", ["forward", "by_input"])
+@pytest.mark.parametrize("depth", [2049, 7169, 16387])
+def test_fma_pipes_by_rows(form, depth):
+    assert by_rows(form, 40, 130, depth) <= fma_bound(depth)
+
+
 def by_weight(n, k, sizes):
     offsets = [0]
     for size in sizes:
@@ -73,3 +86,10 @@ def test_tensor_cores_by_weight(n, k, sizes):
     for size, error in zip(sizes, by_weight(n, k, sizes)):
         if size:
             assert error <= tensor_core_bound(size), (size, error)
+
+
+def test_fma_pipes_by_weight():
+    sizes = [2049, 17, 0, 32770, 7168]
+    for size, error in zip(sizes, by_weight(130, 65, sizes)):
+        if size:
+            assert error <= fma_bound(size), (size, error)
