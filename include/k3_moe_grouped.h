@@ -16,9 +16,8 @@
  *
  * Sums are f32, rounded once to the output's type.  The tensor cores cut an
  * addition of 16 products off instead of rounding it; f32 outputs of theirs lie
- * about 6e-7 of their norm from the exact ones whatever the depth (by weight up to
- * 1e-6 for groups of up to 1088 rows), of the FMA pipes about 2e-7.  A bf16 output
- * is the rounding of a sum that lies up to 1.2e-9 of the norm off per step of the
+ * about 6e-7 of their norm from the exact ones whatever the depth, those of the
+ * FMA pipes about 2e-7.  A bf16 output is the rounding of a sum that lies up to 1.2e-9 of the norm off per step of the
  * depth (8e-6 at 7168), so one in some hundreds is the neighbour of the nearest.
  * The order of the sums depends on the sizes of the call and the size of the
  * row's group, not on which SM takes what: the same call gives the same bits.  What is not finite in a row

@@ -93,7 +93,7 @@ struct TcArgs {
     uint32_t column_tiles;                                             // by weight: and along the columns
     uint32_t batch;                                                    // items per draw
     bool single;                                                       // an item per block at most: no plan, nothing is drawn
-    uint32_t least, most;                                              // by weight: groups of fewer and of more rows are left out
+    uint32_t least;                                                    // by weight: groups of fewer rows are left out
     int accumulate;
 };
 
@@ -568,7 +568,7 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             for (uint64_t first = blockIdx.x; more && first < total; first += (uint64_t)kWarp * step) {
                 const uint64_t at = first + (uint64_t)lane * step;
                 const Item it = at < total ? weight_item((uint32_t)at) : none;
-                for (uint32_t mask = __ballot_sync(0xffffffffu, at < total && it.rows >= a.least && it.rows <= a.most); more && mask != 0u; mask &= mask - 1u) {
+                for (uint32_t mask = __ballot_sync(0xffffffffu, at < total && it.rows >= a.least); more && mask != 0u; mask &= mask - 1u) {
                     const uint32_t from = __ffs(mask) - 1u;
                     const Item next{__shfl_sync(0xffffffffu, it.group, from), __shfl_sync(0xffffffffu, it.row, from), __shfl_sync(0xffffffffu, it.rows, from),
                                     __shfl_sync(0xffffffffu, it.lane0, from), __shfl_sync(0xffffffffu, it.column0, from), 0u};
@@ -587,7 +587,6 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 }
             } else if (w < a.groups * a.lane_tiles * a.column_tiles) {
                 it = weight_item(w);
-                if (it.rows > a.most) it = none;
             }
             if (elect_one() && publish(it)) publish(none);
         } else if (rank == 0u && elect_one()) {
@@ -596,7 +595,6 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             w *= a.batch;
             for (;;) {
                 Item it = none;
-                bool skip = false;
                 left--;
                 if (w < total) {
                     if (kRows) {
@@ -606,19 +604,16 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                         it = Item{tile.group, tile.row, tile.rows, local / of.count * S::kLanes, 0u, 0u};
                     } else {
                         it = weight_item(w);
-                        skip = it.rows > a.most;
                     }
                     it.draw = left == 0u;
                 }
-                if (!skip && !publish(it)) break;
+                if (!publish(it)) break;
                 if (left != 0u) {
                     w++;
                     continue;
                 }
-                if (!skip) {                                           // no item asks for the next draw where the last was left out
-                    if (!mbar_wait(wanted, want_phase, abort_flag)) break;
-                    want_phase ^= 1u;
-                }
+                if (!mbar_wait(wanted, want_phase, abort_flag)) break;
+                want_phase ^= 1u;
                 left = a.batch;
                 w = gridDim.x / kCtas * a.batch + atomicAdd(&a.plan->counter, a.batch);
             }
@@ -884,10 +879,9 @@ uint32_t batch_of(const Product &p) {
     return !S::kSplit && depth <= 4u * kDepth && items_of<kForm, S>(p) >= 16u * (uint64_t)sm_count() / S::kCtas ? 4u : 1u;
 }
 
-// parts: blocks that share an item's depth (S::kSplit); least, most: as TcArgs
-constexpr uint32_t kAll = 0xffffffffu;
+// parts: blocks that share an item's depth (S::kSplit); least: as TcArgs
 template <int kForm, bool kF32, typename S>
-bool launch(const Product &p, cudaStream_t stream, uint32_t parts = 1u, uint32_t least = 0u, uint32_t most = kAll) {
+bool launch(const Product &p, cudaStream_t stream, uint32_t parts = 1u, uint32_t least = 0u) {
     constexpr bool kRows = kForm != kByWeight;
     auto kernel = grouped_bf16_kernel<kForm, kF32, S>;
     CUtensorMap ma, mb;
@@ -902,7 +896,7 @@ bool launch(const Product &p, cudaStream_t stream, uint32_t parts = 1u, uint32_t
     const uint64_t items = items_of<kForm, S>(p), places = S::kSplit ? items : (uint64_t)sm_count() / S::kCtas;
     const bool single = items <= places && (!kRows || p.groups <= kSearched);
     const TcArgs a{p.out, p.offsets, (Plan *)p.workspace, (Tile *)((Plan *)p.workspace + 1), p.rows, p.groups, p.n, p.k,
-                   (lanes + S::kLanes - 1u) / S::kLanes, (p.k + S::kMaxN - 1u) / S::kMaxN, batch_of<kForm, S>(p), single, least, most, p.accumulate};
+                   (lanes + S::kLanes - 1u) / S::kLanes, (p.k + S::kMaxN - 1u) / S::kMaxN, batch_of<kForm, S>(p), single, least, p.accumulate};
     if (items * parts > 0x7fffffffull || (S::kSplit && !single) || !set_max_dynamic_smem((const void *)kernel, S::kBytes)) return false;
     const uint32_t cluster = S::kSplit ? parts : S::kCtas;
     const bool planned = single || least != 0u || (kRows ? launch_chained(grouped_plan_kernel, 1, kMaxGroups, 0, stream, a.plan, a.tiles, p.offsets, p.rows,
@@ -998,12 +992,12 @@ bool weight_product(const Product &p, cudaStream_t stream) {
     if (shortest == few) return launch_typed<kByWeight, Few>(p, stream, 1u, least);
     if (shortest == middle) return launch_typed<kByWeight, Middle>(p, stream, 1u, least);
     if (!p.f32) return launch<kByWeight, false, WideWeight>(p, stream, 1u, least);
-    // f32: without segments up to 17 blocks, 1e-6 of the gradient's norm from 64 bits at the most; deeper groups with them, 5e-7
-    // (a group of 4096 rows 4e-6 without).  32 groups of 1024 rows 838 us, with segments 913; 32 of 256 417 and 391.
-    constexpr uint32_t kDeep = 17u * kDepth;
-    if (p.rows / p.groups > kDeep) return launch<kByWeight, true, DeepWeight>(p, stream, 1u, least);
-    return launch<kByWeight, true, WideWeight>(p, stream, 1u, least, kDeep) &&
-           (p.rows <= kDeep || launch<kByWeight, true, DeepWeight>(p, stream, 1u, kDeep + 1u));
+    // f32 in segments, so items of one half, whatever the group's size: 4.7e-7 of the gradient's norm from 64 bits where two halves
+    // without segments are 2.3e-7 at 256 rows, 1.0e-6 at 1024 and 4.4e-6 at 4096.  Longest where all groups hold some 1000 rows: 32 of
+    // 1024 rows, 2048 x 7168, 980 us, 898 without segments; 32 of 512 607 and 580, of 256 421 and 424, of 2000 1660 either way; 32 of
+    // 512 rows by Zipf's law, 512 x 1024, 38 us, 57 with larger groups in a launch of their own (20 calls in a row).  The shape is
+    // the one that the times of two halves give, on average 2 % from the best of the three over 193 calls.
+    return launch<kByWeight, true, DeepWeight>(p, stream, 1u, least);
 }
 
 }  // namespace

@@ -39,7 +39,7 @@ def normal(seed, *shape):
 
 
 def on_device(offsets):
-    return torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    return torch.tensor(list(offsets), dtype=torch.int32, device="cuda")
 
 
 def off(got, want):
@@ -86,6 +86,20 @@ def test_tensor_cores_by_weight(n, k, sizes):
     for size, error in zip(sizes, by_weight(n, k, sizes)):
         if size:
             assert error <= tensor_core_bound(size), (size, error)
+
+
+@pytest.mark.parametrize("groups,n,k", [(32, 2048, 1032), (40, 520, 2056), (300, 264, 520)])
+@pytest.mark.parametrize("segments", [2, 3])
+def test_every_512_rows_of_a_group_are_summed_by_themselves(groups, n, k, segments):
+    """So a group's gradient is the f32 sum of those of its parts of 512 rows, to the last bit, whatever the group's size."""
+    rows = groups * segments * 512
+    dy, x = normal(n, rows, n), normal(k, rows, k)
+    whole, parts = (grouped.GroupedWeightGradient(g, n, k).forward(dy, x, on_device(range(0, rows + 1, rows // g)))
+                    for g in (groups, groups * segments))
+    want = parts[::segments].clone()
+    for i in range(1, segments):
+        want += parts[i::segments]
+    assert torch.equal(whole, want)
 
 
 def test_fma_pipes_by_weight():
