@@ -22,8 +22,10 @@
 //
 // kCtas 2: a pair of blocks (cta_group::2) shares an item of twice the lanes.  Each loads its lanes and half of the columns,
 // which both tensor cores read, so the columns come from L2 once for two SMs; the first block draws, waits and issues.
-// Arrivals across the pair carry no release where nothing written is handed over: a release waits for the warp's stores, and
-// the weight's gradient of 32 groups of 128 rows took 409 us with it and 318 without.
+// A release across the pair waits for the stores of the warp that does it (the weight's gradient of 32 groups of 128 rows, in pairs,
+// took 409 us so and 318 without), so warps that store do none.  That the second block's have read an item they tell its warp 2,
+// which has no stores and hands it on.  That they have read an accumulator needs no release: what follows it are tcgen05
+// operations alone, ordered by tcgen05.wait::ld and the tcgen05 fences on both sides of the arrival.
 // kSplit: a cluster of up to eight blocks shares an item's depth and adds its sums through distributed shared memory.
 //
 // What bounds it.  Large calls: power.  64 groups of 512 rows, 2048 x 7168, 20 in a row: 670 to 710 us = 1360 to 1440 TFLOP/s;
@@ -79,6 +81,8 @@ struct Shape {
     static constexpr uint32_t kBars = kStore + kResultWarps * 4096u;
     static constexpr uint32_t kBytes = kBars + 512u + 1024u;           // the last: alignment
     static constexpr uint32_t kTmem = 2u * kMaxN;
+    // barriers, items, and two words
+    static_assert((4u * kStages + 4u + 3u * kSlots + 2u) * 8u + kSlots * 24u + 8u <= 512u, "");
     static_assert(!kSplit || (kCtas == 1u && kLanes * kMaxN * 4u <= kResultWarps * 4096u), "a part's sums take the stores' place");
     static_assert(kBytes <= 232448u && kTmem <= 512u && (kTmem & (kTmem - 1u)) == 0u, "");
 };
@@ -102,6 +106,7 @@ struct Item {
     uint32_t lane0, column0;                                           // by weight: column0 of k
     uint32_t draw;                                                     // 1: the last one drawn
 };
+static_assert(sizeof(Item) == 24u, "what Shape leaves room for");
 
 // Instruction descriptor, kind::f16, as make_idesc_bf16, with bits 15 and 16 for operands whose depth is not what lies
 // side by side.
@@ -122,7 +127,8 @@ K3_DEVINL uint32_t place_in(const void *p, uint32_t rank) {
     return r;
 }
 K3_DEVINL void arrive_at(uint32_t bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
-// The same after which nothing that this thread wrote is read: a release would first wait for its stores to memory.
+// The same between tcgen05.fence::before_thread_sync here and ::after_thread_sync there, which order tcgen05 operations; nothing
+// else is ordered by it.
 K3_DEVINL void arrive_relaxed_at(uint32_t bar) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -334,8 +340,9 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     uint64_t *wanted = item_empty + kSlots;                            // [1] the loads come to an end
     uint64_t *armed = wanted + 1;                                      // [kStages] a stage that has to be cleared is being loaded
     uint64_t *cleared = armed + S::kStages;                            // [kStages] and its rows behind the group are zeros
-    uint64_t *done = cleared + S::kStages;                                      // [1] every MMA issued has run
-    Item *items = reinterpret_cast<Item *>(done + 1);                  // [kSlots]
+    uint64_t *done = cleared + S::kStages;                             // [1] every MMA issued has run
+    uint64_t *item_read_here = done + 1;                               // [kSlots] the second block of a pair: its warps have read it
+    Item *items = reinterpret_cast<Item *>(item_read_here + kSlots);   // [kSlots]
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(items + kSlots);
     volatile uint32_t *abort_flag = tmem_slot + 1;
     const uint32_t warp = warp_index(), lane = threadIdx.x % kWarp;
@@ -357,7 +364,9 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         }
         for (uint32_t s = 0; s < kSlots; s++) {
             mbar_init(&item_full[s], 1);
-            mbar_init(&item_empty[s], 1u + (1u + kResultWarps + (kRows ? 0u : 1u)) * kCtas);
+            // the MMAs', the loads', the results' and the clearing warp; of a second block the one that hands on
+            mbar_init(&item_empty[s], 2u + kResultWarps + (kRows ? 0u : 1u) + (kCtas - 1u));
+            mbar_init(&item_read_here[s], 1u + kResultWarps);
         }
         mbar_init(wanted, 1);
         mbar_init(done, 1);
@@ -384,12 +393,13 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         it = items[slot];
         return it.group != kNoItem;
     };
-    // an arrival at a barrier of the first block: what this thread read is free
-    auto arrive_first = [&](uint64_t *bar) {
-        if (kCtas == 2u) arrive_relaxed_at(place_in(bar, 0u));
-        else mbar_arrive(bar);
+    // by one thread of a warp that has read an accumulator
+    auto accumulator_read = [&](uint32_t acc) {
+        if (kCtas == 2u) arrive_relaxed_at(place_in(&acc_empty[acc], 0u));
+        else mbar_arrive(&acc_empty[acc]);
     };
-    auto item_read = [&]() { arrive_first(&item_empty[slot]); };       // by one thread
+    // by one thread of a warp that has read the item
+    auto item_read = [&]() { mbar_arrive(rank == 0u ? &item_empty[slot] : &item_read_here[slot]); };
     auto item_done = [&]() {
         if (++slot == kSlots) { slot = 0u; slot_phase ^= 1u; }
     };
@@ -561,7 +571,15 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             return Item{g, begin, end - begin, at / a.column_tiles * S::kLanes, at % a.column_tiles * S::kMaxN, 0u};
         };
         uint32_t w = blockIdx.x / (S::kSplit ? splits : kCtas);
-        if (!kRows && a.least != 0u) {
+        if (kCtas == 2u && rank == 1u) {
+            if (elect_one()) {                                         // the block's warps have read an item: on to the first block
+                Item it;
+                while (next_item(it) && mbar_wait(&item_read_here[slot], slot_phase, abort_flag)) {
+                    arrive_at(place_in(&item_empty[slot], 0u));
+                    item_done();
+                }
+            }
+        } else if (!kRows && a.least != 0u) {
             // the items of the groups that are this kernel's, 32 looked at together, every gridDim-th the block's
             const uint32_t total = a.groups * a.lane_tiles * a.column_tiles, step = gridDim.x;
             bool more = true;
@@ -681,7 +699,7 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     for (uint32_t c = 0; c < kChunks; c++) k3::fp8::tmem_ld_wait_for(v[c]);
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0u) arrive_first(&acc_empty[acc]);
+                    if (lane == 0u) accumulator_read(acc);
                     for (uint32_t kb = begin; end - kb > kSegment; kb += kSegment) {           // the item's other segments
                         turn ^= 1u;
                         if (!mbar_wait(&acc_full[turn], acc_phase[turn], abort_flag)) { ok = false; break; }
@@ -697,7 +715,7 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                         }
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0u) arrive_first(&acc_empty[turn]);
+                        if (lane == 0u) accumulator_read(turn);
                     }
                     if (!ok) break;
                 } else {
