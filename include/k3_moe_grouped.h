@@ -13,15 +13,19 @@
  * offsets[groups] on belong to no group: they are not written, and what they
  * hold (NaN, say) enters nothing.  An offset past `rows` counts as `rows`, one
  * below its predecessor ends an empty group; nothing outside is read or written.
+ * (Where offsets descend, groups may overlap: a row of several has the result of
+ * any of them, and rows may be left as they are.)
  *
  * Sums are f32, rounded once to the output's type.  The tensor cores cut an
  * addition of 16 products off instead of rounding it; f32 outputs of theirs lie
- * about 6e-7 of their norm from the exact ones whatever the depth, those of the
- * FMA pipes about 2e-7.  A bf16 output is the rounding of a sum that lies up to 1.2e-9 of the norm off per step of the
- * depth (8e-6 at 7168), so one in some hundreds is the neighbour of the nearest.
+ * about 5e-7 of their norm from the exact ones whatever the depth, those of the
+ * FMA pipes about 2e-7.  A bf16 output is the rounding of a sum that lies up to
+ * 1.2e-9 of the norm off per step of the depth (8e-6 at 7168), so one in some
+ * hundreds is the neighbour of the nearest.
  * The order of the sums depends on the sizes of the call and the size of the
- * row's group, not on which SM takes what: the same call gives the same bits.  What is not finite in a row
- * or a matrix makes the results that it enters not finite, and no others.
+ * row's group, not on which SM takes what: the same call gives the same bits.
+ * What is not finite in a row or a matrix makes the results that it enters not
+ * finite, and no others.
  *
  * Any n and k are taken.  Matrices whose rows are whole units of 16 bytes (n and
  * k multiples of 8, 16-byte aligned pointers) run on the tensor cores, others on
