@@ -31,10 +31,12 @@ struct AnyArgs {
 // The group that row tile `tile` of all groups' tiles belongs to and its first row; false past the last tile.
 // All threads of the block call it.
 K3_DEVINL bool find_tile(const AnyArgs &a, uint32_t tile, uint32_t &group, uint32_t &row, uint32_t &end) {
-    __shared__ uint32_t sums[kThreads / kWarp], found[3];
+    __shared__ uint64_t sums[kThreads / kWarp];                    // 64 bits: overlapping groups can have more than 2^32 tiles
+    __shared__ uint32_t found[3];
     constexpr uint32_t kEach = kMaxGroups / kThreads;
     const uint32_t warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
-    uint32_t tiles[kEach], mine = 0u;
+    uint32_t tiles[kEach];
+    uint64_t mine = 0u;
 #pragma unroll
     for (uint32_t i = 0; i < kEach; i++) {
         const uint32_t g = threadIdx.x * kEach + i;
@@ -43,16 +45,16 @@ K3_DEVINL bool find_tile(const AnyArgs &a, uint32_t tile, uint32_t &group, uint3
         tiles[i] = (past - begin + kTile - 1u) / kTile;
         mine += tiles[i];
     }
-    uint32_t scan = mine;
+    uint64_t scan = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t up = __shfl_up_sync(0xffffffffu, scan, o);
+        const uint64_t up = __shfl_up_sync(0xffffffffu, scan, o);
         if (lane >= (uint32_t)o) scan += up;
     }
     if (lane == 31u) sums[warp] = scan;
     if (threadIdx.x == 0u) found[0] = 0xffffffffu;
     __syncthreads();
-    uint32_t first = scan - mine;
+    uint64_t first = scan - mine;
     for (uint32_t w = 0; w < warp; w++) first += sums[w];
 #pragma unroll
     for (uint32_t i = 0; i < kEach; i++) {
@@ -60,7 +62,7 @@ K3_DEVINL bool find_tile(const AnyArgs &a, uint32_t tile, uint32_t &group, uint3
             uint32_t begin, past;
             group_rows(a.offsets, threadIdx.x * kEach + i, a.rows, begin, past);
             found[0] = threadIdx.x * kEach + i;
-            found[1] = begin + (tile - first) * kTile;
+            found[1] = begin + (tile - (uint32_t)first) * kTile;
             found[2] = past;
         }
         first += tiles[i];

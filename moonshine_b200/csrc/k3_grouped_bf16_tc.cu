@@ -276,37 +276,38 @@ K3_DEVINL bool search_tile(const uint32_t *offsets, uint32_t rows, uint32_t grou
     return true;
 }
 
-// One thread per group.
+// One thread per group.  Tiles are counted in 64 bits: overlapping groups, where offsets descend, can have more than 2^32, and a
+// place that wrapped would be another group's.
 __global__ void __launch_bounds__(kMaxGroups) grouped_plan_kernel(Plan *plan, Tile *tiles, const uint32_t *offsets, uint32_t rows,
                                                                   uint32_t groups, uint32_t max_n, uint32_t step, uint32_t capacity) {
     pdl_trigger();
     pdl_wait();
-    __shared__ uint32_t sums[kMaxGroups / kWarp];
+    __shared__ uint64_t sums[kMaxGroups / kWarp];
     const uint32_t g = threadIdx.x, lane = g % kWarp, warp = g / kWarp;
     uint32_t begin = 0u, end = 0u;
     if (g < groups) group_rows(offsets, g, rows, begin, end);
     const uint32_t count = (end - begin + max_n - 1u) / max_n;
-    uint32_t scan = count;
+    uint64_t scan = count;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t up = __shfl_up_sync(0xffffffffu, scan, o);
+        const uint64_t up = __shfl_up_sync(0xffffffffu, scan, o);
         if (lane >= (uint32_t)o) scan += up;
     }
     if (lane == 31u) sums[warp] = scan;
     __syncthreads();
-    uint32_t first = scan - count;
+    uint64_t first = scan - count;
     for (uint32_t w = 0; w < warp; w++) first += sums[w];
     if (count != 0u) {
-        const uint32_t held = min(count, capacity - min(capacity, first));
+        const uint32_t held = first < capacity ? min(count, capacity - (uint32_t)first) : 0u;
         for (uint32_t i = 0; i < held; i++) {
-            Tile t = tile_of(g, begin, end, first, count, i, step);
+            Tile t = tile_of(g, begin, end, (uint32_t)first, count, i, step);
             t.count = held;                                            // (fewer only if offsets descend)
             tiles[first + i] = t;
         }
     }
     if (g == kMaxGroups - 1u) {
         plan->counter = 0u;
-        plan->tiles = min(first + count, capacity);
+        plan->tiles = (uint32_t)min(first + count, (uint64_t)capacity);
     }
 }
 

@@ -110,3 +110,28 @@ def test_by_weight(n, k, kind, groups, rows):
         torch.cuda.synchronize()
         assert guards_stand(buffer) and ops.k3_moe_device_status() == 0
         assert torch.equal(out, want.to(dtype))
+
+
+@pytest.mark.parametrize("n,k", [(8, 8), (7, 7)])
+def test_more_than_2_to_32_tiles(n, k):
+    """512 groups of about 2^29 rows each, which overlap: their tiles' places pass 32 bits."""
+    rows = (1 << 29) + (1 << 20)
+    r = random.Random(n)
+    offsets = [r.randrange(1000) if g % 2 == 0 else rows - r.randrange(1000) for g in range(1025)]
+    a, matrix = integers(3, 1 << 20, k).repeat(rows >> 20, 1), integers(4, n, k)
+    buffer, out = guarded((rows, n), BF16)
+    grouped.GroupedProduct(matrix.expand(1024, n, k).contiguous()).forward(a, torch.tensor(offsets, dtype=torch.int32, device="cuda"), out=out)
+    torch.cuda.synchronize()
+    assert guards_stand(buffer) and ops.k3_moe_device_status() == 0
+    want = (a[:1 << 20].float() @ matrix.float().t()).to(BF16)
+    for i in range(rows >> 20):
+        part = out[i << 20:(i + 1) << 20]
+        inside = torch.ones(1 << 20, dtype=torch.bool, device="cuda")
+        if i == 0:
+            inside[:offsets[0]] = False                                     # the first group's rows have room for all of their tiles
+        if i == (rows >> 20) - 1:
+            inside[(1 << 20) - (rows - offsets[1]):] = False
+        assert torch.equal(part[inside], want[inside])
+        assert bool(((part == want) | (part == 7.5)).all())
+    del a, out, buffer
+    torch.cuda.empty_cache()
