@@ -10,7 +10,10 @@
  *   y    = s rstd weight
  * y is f32 until it is stored: bf16 rows are y rounded once, codes are those of
  * y itself with a scale per row and 128 columns (format "rows" of
- * k3_moe_fp8.h).  A block of 128 that is not finite gets the scale NaN.
+ * k3_moe_fp8.h).  Of bf16 x they are the exact ones: the rounding of 448 s weight /
+ * max |s weight| of the block, ties to even.  A block of 128 that is not finite
+ * gets the scale NaN.  Where the sum of a row's squares passes f32's range, from
+ * |s| of about 1e17 on, rstd is 0.
  * Sums are f32; their order depends on hidden and, where it is no multiple of 8,
  * on the row's place modulo 8: the same call gives the same bits.
  */

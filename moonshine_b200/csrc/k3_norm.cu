@@ -184,28 +184,41 @@ K3_DEVINL float largest_of(float a, float b, float c) {
 // lie across the row's end, and y is not asked for.  minus_w: the weight's negatives, for the quotients want -y.  Two
 // elements at a time and the vectors side by side through every step, 8192 x 7168 to codes alone takes 59 us; element by
 // element, and one vector after the other with its shuffles and its reciprocal, it took 78.
+//
+// Codes of bf16 rows: with rstd = f m, f a power of two, and p = s f w, y is p m, the scale max |p| m / 448 and y / scale therefore
+// 448 p / max |p|.  p and 448 p are exact and the quotient is rounded once, so that those in the middle between two codes, one in
+// some thousands, go to the even one; by way of y the last bit of rstd decided (8192 x 7168 with both outputs 83 us, now 84).
+// Of f32 rows p is y.
 template <bool kF32, bool kVector, bool kPartial = false, uint32_t kVectors, typename First>
 K3_DEVINL void put_normed(const NormArgs &a, const Eight<kF32> (&s)[kVectors], const Eight<false> (&minus_w)[kVectors], float rstd, uint64_t row,
                           First first, bool live) {
     const uint32_t hidden = a.hidden, pitch = pitch_of(hidden);
-    const uint64_t rstd2 = both2(rstd);
-    uint64_t y[kVectors][4];                                         // negative
-    uint32_t most[kVectors];
+    uint64_t p[kVectors][4];                                         // negative
+    auto scale_rows = [&](float by) {
 #pragma unroll
-    for (uint32_t v = 0; v < kVectors; v++) {
+        for (uint32_t v = 0; v < kVectors; v++) {
 #pragma unroll
-        for (uint32_t i = 0; i < 4u; i++) y[v][i] = mul2(mul2(pair_of(s[v], i), rstd2), pair_of(minus_w[v], i));
-    }
+            for (uint32_t i = 0; i < 4u; i++) p[v][i] = mul2(mul2(pair_of(s[v], i), both2(by)), pair_of(minus_w[v], i));
+        }
+    };
+    if (kF32) scale_rows(rstd);
     if (!kPartial && a.y != nullptr) {
+        const uint64_t rstd2 = both2(rstd);
 #pragma unroll
         for (uint32_t v = 0; v < kVectors; v++) {
             Eight<false> out;
 #pragma unroll
-            for (uint32_t i = 0; i < 4u; i++) out.w[i] = bf16x2(lo2(y[v][i]), hi2(y[v][i])) ^ kSigns;
+            for (uint32_t i = 0; i < 4u; i++) {
+                const uint64_t y = kF32 ? p[v][i] : mul2(mul2(pair_of(s[v], i), rstd2), pair_of(minus_w[v], i));
+                out.w[i] = bf16x2(lo2(y), hi2(y)) ^ kSigns;
+            }
             out.template store<kVector>(a.y + row * hidden, first(v), live ? hidden : 0u);
         }
     }
     if (a.codes == nullptr) return;
+    const float m = kF32 ? 1.0f : __uint_as_float((__float_as_uint(rstd) & 0x7fffffu) | 0x3f800000u);
+    if (!kF32) scale_rows(__uint_as_float(__float_as_uint(rstd) & 0x7f800000u));
+    uint32_t most[kVectors];
 #pragma unroll
     for (uint32_t v = 0; v < kVectors; v++) {
         const uint32_t c = first(v);
@@ -213,10 +226,10 @@ K3_DEVINL void put_normed(const NormArgs &a, const Eight<kF32> (&s)[kVectors], c
 #pragma unroll
         for (uint32_t i = 0; i < 4u; i++) {
             if (!kVector || kPartial) {                              // past the row's end: no part of the block, whatever rstd is
-                y[v][i] = pack2(column_of<kVector>(c, 2u * i) < hidden ? lo2(y[v][i]) : 0.0f,
-                                column_of<kVector>(c, 2u * i + 1u) < hidden ? hi2(y[v][i]) : 0.0f);
+                p[v][i] = pack2(column_of<kVector>(c, 2u * i) < hidden ? lo2(p[v][i]) : 0.0f,
+                                column_of<kVector>(c, 2u * i + 1u) < hidden ? hi2(p[v][i]) : 0.0f);
             }
-            largest = largest_of(largest, lo2(y[v][i]), hi2(y[v][i]));
+            largest = largest_of(largest, lo2(p[v][i]), hi2(p[v][i]));
         }
         most[v] = kVector && c >= hidden ? 0u : __float_as_uint(largest);
     }
@@ -228,12 +241,15 @@ K3_DEVINL void put_normed(const NormArgs &a, const Eight<kF32> (&s)[kVectors], c
     uint2 codes[kVectors];
 #pragma unroll
     for (uint32_t v = 0; v < kVectors; v++) {
-        const float scale = scale_of(most[v]), lift = lift_of(scale);
-        const uint64_t by = both2(scale * lift), inverse = both2(-inverse_of(scale)), lift2 = both2(lift);
+        const float largest = __uint_as_float(most[v]), scale = scale_of(__float_as_uint(largest * m));
+        // (the smallest scale: as if `largest` were what it is for; the lift keeps remainders normal and 448 p finite)
+        const float divisor = kF32 ? scale : scale == 0x1p-126f ? 448.0f * 0x1p-126f * reciprocal_fast(m) : largest;
+        const float lift = !kF32 && divisor > 0x1p100f ? 0x1p-64f : lift_of(divisor);
+        const uint64_t by = both2(divisor * lift), inverse = both2(-inverse_of(divisor * lift)), factor = both2(kF32 ? lift : 448.0f * lift);
         uint32_t h[4];
 #pragma unroll
         for (uint32_t i = 0; i < 4u; i++) {
-            const uint64_t q = divided2(mul2(y[v][i], lift2), by, inverse);
+            const uint64_t q = divided2(mul2(p[v][i], factor), by, inverse);
             h[i] = codes2(lo2(q), hi2(q));
         }
         codes[v] = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
