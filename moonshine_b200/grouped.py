@@ -150,11 +150,12 @@ class GatedActivation:
         _placed(("d_out", d_out), ("gate", gate), ("up", up), ("weights", weights), ("routes", routes), ("offsets", offsets))
         d_gate, d_up, scaled = torch.empty_like(d_out), torch.empty_like(d_out), torch.empty_like(d_out)
         count = rows if weights is None else weights.numel()
-        # zeros for routes that no row has, which only a table of routes can leave out
-        if routes is None and offsets is None and rows and columns:
-            d_weights = d_out.new_empty(rows, dtype=torch.float32) if weights is None else torch.empty_like(weights)
+        # zeros for routes that no row has, which only a table of routes can leave out (4 us of the host's time)
+        whole = routes is None and offsets is None and rows and columns
+        if weights is None:
+            d_weights = (torch.empty if whole else torch.zeros)(rows, dtype=torch.float32, device=d_out.device)
         else:
-            d_weights = d_out.new_zeros((rows,) if weights is None else weights.shape, dtype=torch.float32)
+            d_weights = torch.empty_like(weights) if whole else torch.zeros_like(weights)
         if rows and columns:
             _done(ops.k3_moe_activation_backward(d_gate, d_up, scaled, d_weights, d_out, gate, up, weights, routes, offsets,
                                                  0 if offsets is None else offsets.shape[0] - 1, rows, columns, count,
