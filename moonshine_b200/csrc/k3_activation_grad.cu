@@ -9,7 +9,8 @@
 //
 // Bound by memory: 12 bytes per element, each read or written once.  A row belongs to a warp, or, where there are
 // fewer rows than warps to fill the SMs, to a block; its sum for the routing weight is taken in a fixed order.  32768 x 2048:
-// SwiGLU 127 to 129 us, 6.3 TB/s, SiTU 135, with three exponentials and three reciprocals per element.
+// SwiGLU 127 to 129 us, 6.3 TB/s, SiTU 135, with three exponentials and three reciprocals per element.  SiTU with a block per row
+// spills 44 bytes of registers under the bound of five blocks per SM.
 #include "k3_common.cuh"
 #include "k3_fp8_ptx.cuh"
 #include "k3_moe_ops.h"

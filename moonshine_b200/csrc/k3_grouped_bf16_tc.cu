@@ -28,10 +28,11 @@
 // operations alone, ordered by tcgen05.wait::ld and the tcgen05 fences on both sides of the arrival.
 // kSplit: a cluster of up to eight blocks shares an item's depth and adds its sums through distributed shared memory.
 //
-// What bounds it.  Large calls: power.  64 groups of 512 rows, 2048 x 7168, 20 in a row: 670 to 710 us = 1360 to 1440 TFLOP/s;
-// for seconds 776 us = 1240 at 990 W and 1170 MHz, where the tensor pipes are busy 0.87 of the time (the library's plain
-// product of 32768 rows: 1323 TFLOP/s at 988 W, 1282 MHz, 0.85; it reads 0.5 GB where 64 matrices are 2.3).  Few rows per
-// group: the matrices' bytes, 6.2 to 6.9 TB/s.
+// What bounds it.  Large calls: power, and what the last of a group's column tiles leaves empty.  64 groups of 512 rows, 2048 x
+// 7168, bf16 forward, 20 in a row after a pause: 676 to 712 us on two B200s = 1350 to 1420 TFLOP/s; for four seconds 854 us = 1130 at
+// 989 W and 1065 MHz (the library's plain product of 32768 rows: 1350 TFLOP/s at 993 W and 1312 MHz; it reads 0.5 GB where 64
+// matrices are 2.3).  64 groups of 520 rows, which take a third tile, 814 us, of 560 818, of 640 921.  Few rows per group: the
+// matrices' bytes, 6.2 to 6.9 TB/s.
 //
 // Every wait is bounded; on give-up the block raises the status word, waits for its copies and frees its tensor memory.
 #include "k3_fp8_ptx.cuh"
@@ -327,8 +328,9 @@ grouped_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     constexpr uint32_t kCtas = S::kCtas;
     // The tensor cores cut the sums off instead of rounding them, 2^-24 or so of the sum per 16 of the depth, always towards
     // zero: 8e-6 of the result's norm at a depth of 7168.  For f32 results an accumulator therefore takes up to 8 blocks, a
-    // segment, and the warps behind it add the segments, rounded: 6e-7 at any depth (16 blocks 1.1e-6, 4 3e-7).  64 groups of 512
-    // rows, 2048 x 7168, by input: 16 blocks 725 us, 8 733, 4 758.  (Not with two halves, whose sums no registers would hold.)
+    // segment, and the warps behind it add the segments, rounded: 4.8e-7 at any depth (16 blocks 1.0e-6, 4 2.5e-7).  64 groups of 512
+    // rows, 2048 x 7168, in pairs of blocks with one half (Square), 20 in a row: forward 767 us (16 blocks 762, 4 781, without segments
+    // 750), by input 821 (818, 857, 810).  Two halves, whose sums no registers would hold, have none; Wide takes 731 us forward.
     constexpr uint32_t kSegment = kF32 && S::kHalves == 1u ? 8u : 0xffffffffu;
     extern __shared__ unsigned char smem_raw[];
     unsigned char *base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -940,7 +942,8 @@ bool launch_typed(const Product &p, cudaStream_t stream, uint32_t parts = 1u, ui
 //   Few      up to 64 rows per group: bound by the matrices' bytes, 6.4 TB/s at 64 groups of 8 rows of 2048 x 7168 (274 us; Middle 294)
 //   Middle   up to 128, or too few items for larger ones (4 groups of 256 rows: 35 us; Few 53, Square 43)
 //   Square   pairs of blocks with two accumulators (16 groups of 256 rows of 7168 x 2048: 107 us; Wide 115, Middle 134)
-//   Wide     least traffic per product, so least power, which bounds large calls (64 groups of 512 rows 725 us; Square 822)
+//   Wide     least traffic per product, so least power, which bounds large calls (64 groups of 512 rows of 2048 x 7168, forward, bf16,
+//            712 us 20 in a row and 848 for 0.8 s; Square 735 and 876)
 struct Cost {
     double fixed, item, alone, alone_column, full, full_column;
 };

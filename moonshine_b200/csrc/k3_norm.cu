@@ -6,8 +6,9 @@
 // Bound by memory: a row is read once, kept in registers over the row's sum, and written once.  A row belongs to a
 // warp (up to 1024 columns) or to a block of 256 or 1024 threads; a thread holds vectors of 8 neighbouring columns,
 // so the 16 lanes of half a warp hold a block of 128, whose largest magnitude is four shuffles away.  The gradient of
-// many rows goes through a ring in shared memory (below).  8192 x 7168 bf16: forward with sum, bf16 rows and codes 86 us,
-// 6.1 TB/s; backward with the weight's gradient 82 us, 5.7 TB/s.
+// many rows goes through a ring in shared memory (below).  8192 x 7168 bf16: forward with sum, bf16 rows and codes 84 us 20 times
+// over the same arrays, 90 over others, 6.3 and 5.9 TB/s; backward with the weight's gradient 79 us, 5.9 TB/s.  The gradient of more than
+// 8192 columns, 1024 threads to a row, spills 132 to 272 bytes of registers.
 #include "k3_common.cuh"
 #include "k3_fp8_ptx.cuh"
 #include "k3_grouped.h"
@@ -339,8 +340,9 @@ __global__ void __launch_bounds__(threads_of(kTeam)) norm_kernel(NormArgs a) {
 
 // Rows whose length is no multiple of 8 start anywhere in a vector.  A thread's vectors are then those of the matrix as a whole, and
 // hold the row from column -o on, o the row's place modulo 8: loads and stores are whole but at a row's ends.  The weight's
-// vectors lie across these, as do codes and their blocks, for which the row goes through shared memory.  4096 x 7001 bf16: forward
-// with both outputs 80 us, element by element 113; backward 94 and 217; 2048 x 3583 f32: 33 and 33, 37 and 41.
+// vectors lie across these, as do codes and their blocks, for which the row goes through shared memory.  20 times over the same arrays:
+// 4096 x 7001 bf16 forward with both outputs 76 us, element by element 108, of 7008 columns 44; backward 85, 209 and 43; f32 forward 107,
+// 103 and 68, backward 102, 144 and 66; 2048 x 3583 f32 forward 26, 25 and 17, backward 25, 29 and 24.
 K3_DEVINL Eight<false> weight_from(const uint16_t *weight, int32_t c, uint32_t o, uint32_t hidden) {
     const int32_t at = o != 0u ? c + (int32_t)o - 8 : c;
     Eight<false> first, second;
