@@ -18,7 +18,7 @@ def layer(seed, experts, expert_hidden, hidden):
     return normal(experts, expert_hidden, hidden), normal(experts, expert_hidden, hidden), normal(experts, hidden, expert_hidden)
 
 
-@pytest.mark.parametrize("tokens", [1, 5, 200])
+@pytest.mark.parametrize("tokens", [1, 5, 200, 3000])
 def test_an_id_that_is_no_experts_adds_nothing(tokens):
     """Against the same call with an expert in its place whose matrices are zeros: the same bits, and the status word says so."""
     experts, top_k, hidden = 6, 3, 40
